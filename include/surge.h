@@ -322,6 +322,95 @@ sg_err sg_gpu_run_delta_chunk(sg_gpu *g, void *S, void *qkv, void *out, void *ga
 sg_err sg_gpu_run_rmsnorm_gated_chunk(sg_gpu *g, void *y, void *z, void *out, void *w,
                                       const uint32_t params[8]);
 
+/* ---------------------------------------------------------------------
+ * Additions with no reference counterpart: an 8-bit K/V cache with the
+ * attention that reads it, rotary positions with several axes, and the choice
+ * of a token from processed logits. Manner as above: synchronous on the
+ * library's stream (work that another stream has queued on a wrapped device
+ * buffer must have finished), one caller per sg_gpu at a time, f32 unless
+ * stated, buffers 4-byte aligned (codes 16-byte), shapes and sizes checked on
+ * the host before any launch. They run on the handle's device whichever is
+ * current, and leave the current one as it was. Positions are counted in 32
+ * bits, bytes in 64.
+ *
+ * The 8-bit cache. Two buffers hold K and V of one layer:
+ *   codes  int8 [tile][n_kv][2][16 hd], a tile being 16 positions; half 0 the
+ *          keys, position r of the tile and dim d at
+ *          [d / 64][d / 16 % 4][r][d % 16], half 1 the values, at
+ *          [d / 64][r / 4][d % 16][d / 16 % 4][r % 4]: the orders in which the
+ *          matrix instructions take them;
+ *   scales f32 [position / block][n_kv][2] (K, V), block = 16, 32, 64 or 128
+ *          positions. x = code * scale, |code| <= 127.
+ * sg_kv8_code_bytes / sg_kv8_scale_bytes: what `cap` positions need (0 for a
+ * shape that is not supported). hd = 64, 128 or 256. A larger cache has the
+ * same layout from its start, so the buffers may hold more than a call uses.
+ *
+ * sg_gpu_run_kv8_store: rows [base, base + n) from k and v (row stride p[5]
+ *   floats, 0 = n_kv hd; [n_kv][hd] in a row). Per block, head and half the
+ *   scale is s = max|x| / 127 (an f32 division) and a code is x / s rounded to
+ *   the nearest integer, ties to even. In a block that goes on (base inside
+ *   it) s is not below the scale it has, and if s grows the codes of its rows
+ *   before base are rounded again to the nearest of code * s_old / s; a block
+ *   that starts at base or after it is new, whatever its scale held. A value
+ *   that f16 cannot hold (|x| >= 65520, NaN) makes the block's scale NaN, and
+ *   whatever reads the block NaN, until the block is stored from its start.
+ *   Storing at base drops the rows from base on: codes of rows >= base + n
+ *   stay as they were and mean nothing. The result for a block depends on how
+ *   its rows came in, one by one or together, by at most the roundings above.
+ *   p: [0]=n_kv [1]=hd [2]=block [3]=base [4]=n [5]=row stride.
+ * sg_gpu_run_kv8_load: rows [base, base + n) as values, code * scale, to k and
+ *   v (row stride p[5], 0 = n_kv hd; with a stride the rows of k and v may
+ *   interleave in one allocation). Same p.
+ * sg_gpu_run_attn_decode_kv8: as sg_gpu_run_attn_decode_f16, over the cache.
+ *   q [n_heads][q_stride], out [n_heads][hd]; seq 0 gives zeros. n_heads a
+ *   multiple of n_kv, at most 16 times it.
+ *   p: [0]=n_heads [1]=n_kv [2]=hd [3]=seq [4]=q_stride [5]=scale bits [6]=block.
+ * sg_gpu_run_attn_prefill_kv8: as sg_gpu_run_attn_prefill: q [n][n_heads]
+ *   [q_stride], out [n][n_heads][hd]; token t sees positions 0 .. base + t of
+ *   a cache that holds base + n.
+ *   p: [0]=n_heads [1]=n_kv [2]=hd [3]=base [4]=n [5]=q_stride [6]=scale bits
+ *   [7]=block.
+ * Both keep q.k exact up to q's rounding to 24 bits of its head's largest
+ * element and sum in f32; reruns give the same bits. */
+uint64_t sg_kv8_code_bytes(uint32_t n_kv, uint32_t hd, uint64_t cap);
+uint64_t sg_kv8_scale_bytes(uint32_t n_kv, uint32_t block, uint64_t cap);
+sg_err sg_gpu_run_kv8_store(sg_gpu *g, void *k, void *v, void *codes, void *scales, const uint32_t params[8]);
+sg_err sg_gpu_run_kv8_load(sg_gpu *g, void *codes, void *scales, void *k, void *v, const uint32_t params[8]);
+sg_err sg_gpu_run_attn_decode_kv8(sg_gpu *g, void *q, void *codes, void *scales, void *out, const uint32_t params[8]);
+sg_err sg_gpu_run_attn_prefill_kv8(sg_gpu *g, void *q, void *codes, void *scales, void *out, const uint32_t params[8]);
+
+/* Rotary positions with three axes (time, height, width; text has the three
+ * alike): x, out [n][heads] slices at row stride p[7] (0 = heads * stride) and
+ * head stride p[3] (0 = head_dim); pos int32 [3][n]. Pair i of the half-split
+ * rotation turns by pos[axis(i)] * theta^(-2 i / rope_dim), the angle and its
+ * sine and cosine in double, then rounded to f32. p[5] = s0 | s1 << 8 |
+ * s2 << 16 | order << 24, s0 + s1 + s2 = rope_dim / 2 pairs per axis. order 0:
+ * axis 0's pairs, then axis 1's, then axis 2's. order 1, interleaved: axis 1
+ * has the pairs i % 3 == 1 below 3 s1, axis 2 those of i % 3 == 2 below 3 s2,
+ * axis 0 the others. Dims from rope_dim on are copied; gaps between slices are
+ * not written. out may be x (the same address) but not overlap it otherwise.
+ * p: [0]=head_dim (<= 256) [1]=rope_dim [2]=heads [3]=stride [4]=n [5]=sections
+ * [6]=theta bits [7]=row stride. */
+sg_err sg_gpu_run_rope_axes(sg_gpu *g, void *x, void *pos, void *out, const uint32_t params[8]);
+
+/* Token counts: counts u32 [rows][vocab] += the occurrences in ids int32
+ * [rows][n] (ids outside [0, vocab) are skipped, so -1 pads a ragged row);
+ * cleared first when p[3] is 1. p: [0]=n (may be 0) [1]=vocab [2]=rows [3]=clear. */
+sg_err sg_gpu_run_token_counts(sg_gpu *g, void *ids, void *counts, const uint32_t params[8]);
+
+/* Logits under penalties, a bias and a mask, and the token they choose. Per
+ * row and id, in f32 and this order: where counts[row][id] = c > 0, x > 0 ? x /
+ * repetition : x * repetition, then - c * frequency - presence; + bias[id]; -inf
+ * where bit id % 32 of mask[row][id / 32] is 0. counts u32 [rows][vocab], bias
+ * f32 [vocab] and mask u32 [rows][ceil(vocab / 32)] may each be NULL. out
+ * [rows][vocab] may be logits. token u32 [rows]: the lowest id of the largest
+ * value that is above -inf, 0xFFFFFFFF if there is none (nothing allowed);
+ * NaN is never chosen. repetition > 0 and finite (1 = none), frequency and
+ * presence finite (0 = none).
+ * p: [0]=vocab [1]=rows [2]=repetition bits [3]=frequency bits [4]=presence bits. */
+sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void *mask, void *out, void *token,
+                         const uint32_t params[8]);
+
 /* Decode (surge.h:1260-1274). */
 sg_err sg_gpu_load_model(sg_gpu *g, const sg_model *m);
 sg_err sg_gpu_state_new(sg_gpu *g, const sg_model *m, uint32_t max_ctx);

@@ -114,6 +114,15 @@ _SIGS = {
     "sg_gpu_run_gdn_step": (SgErr, [C.c_void_p] * 5 + [C.POINTER(C.c_uint32)]),
     "sg_gpu_run_gdn_chunk": (SgErr, [C.c_void_p] * 5 + [C.POINTER(C.c_uint32)]),
     "sg_gpu_run_attn_chunk": (SgErr, [C.c_void_p] * 5 + [C.POINTER(C.c_uint32)]),
+    "sg_kv8_code_bytes": (C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint64]),
+    "sg_kv8_scale_bytes": (C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint64]),
+    "sg_gpu_run_kv8_store": (SgErr, [C.c_void_p] * 5 + [C.POINTER(C.c_uint32)]),
+    "sg_gpu_run_kv8_load": (SgErr, [C.c_void_p] * 5 + [C.POINTER(C.c_uint32)]),
+    "sg_gpu_run_attn_decode_kv8": (SgErr, [C.c_void_p] * 5 + [C.POINTER(C.c_uint32)]),
+    "sg_gpu_run_attn_prefill_kv8": (SgErr, [C.c_void_p] * 5 + [C.POINTER(C.c_uint32)]),
+    "sg_gpu_run_rope_axes": (SgErr, [C.c_void_p] * 4 + [C.POINTER(C.c_uint32)]),
+    "sg_gpu_run_token_counts": (SgErr, [C.c_void_p] * 3 + [C.POINTER(C.c_uint32)]),
+    "sg_gpu_run_logits": (SgErr, [C.c_void_p] * 7 + [C.POINTER(C.c_uint32)]),
     "sg_gpu_splitk_online_dispatches": (C.c_uint64, [C.c_void_p]),
     "sg_gpu_splitk_online_selected": (C.c_bool, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32,
                                                  C.c_uint32]),
@@ -304,6 +313,33 @@ class Gpu:
     def attn_chunk(self, inp, w, kv, out, p):
         check(lib().sg_gpu_run_attn_chunk(self.handle, inp.handle, w.handle, kv.handle, out.handle,
                                            params(p)))
+
+    def kv8_store(self, k, v, codes, scales, p):
+        check(lib().sg_gpu_run_kv8_store(self.handle, k.handle, v.handle, codes.handle, scales.handle, params(p)))
+
+    def kv8_load(self, codes, scales, k, v, p):
+        check(lib().sg_gpu_run_kv8_load(self.handle, codes.handle, scales.handle, k.handle, v.handle, params(p)))
+
+    def attn_decode_kv8(self, q, codes, scales, out, p):
+        check(lib().sg_gpu_run_attn_decode_kv8(self.handle, q.handle, codes.handle, scales.handle, out.handle,
+                                               params(p)))
+
+    def attn_prefill_kv8(self, q, codes, scales, out, p):
+        check(lib().sg_gpu_run_attn_prefill_kv8(self.handle, q.handle, codes.handle, scales.handle, out.handle,
+                                                params(p)))
+
+    def rope_axes(self, x, pos, out, p):
+        check(lib().sg_gpu_run_rope_axes(self.handle, x.handle, pos.handle, out.handle, params(p)))
+
+    def token_counts(self, ids, counts, p):
+        """ids may be None when p[0] is 0."""
+        check(lib().sg_gpu_run_token_counts(self.handle, ids.handle if ids is not None else None, counts.handle,
+                                            params(p)))
+
+    def logits(self, logits, counts, bias, mask, out, token, p):
+        """counts, bias and mask may be None."""
+        h = [b.handle if b is not None else None for b in (logits, counts, bias, mask, out, token)]
+        check(lib().sg_gpu_run_logits(self.handle, *h, params(p)))
 
     def dispatch_counts(self):
         """(per_head, gqa, online) partial dispatches encoded since sg_gpu_state_new."""

@@ -873,6 +873,221 @@ sg_err sg_gpu_run_gdn_chunk(sg_gpu *g, void *in, void *w, void *state, void *out
 }
 
 /* ---------------------------------------------------------------------
+ * The 8-bit K/V cache, rotary positions with axes, logits (surge.h). No
+ * reference counterpart. These run on the handle's device whichever is
+ * current; the current one is put back.
+ * --------------------------------------------------------------------- */
+
+static sg_err on_device(const sg_gpu *g, int *was) {
+    HIPCHK(hipGetDevice(was), "hipGetDevice");
+    if (*was != g->dev) HIPCHK(hipSetDevice(g->dev), "hipSetDevice");
+    return SG_OK;
+}
+static sg_err back_to(const sg_gpu *g, int was, sg_err e) {
+    if (was != g->dev && hipSetDevice(was) != hipSuccess && !sg_failed(e)) return (sg_err){"gpu: hipSetDevice failed"};
+    return e;
+}
+static bool aligned(const void *buf, uintptr_t to) { return !((uintptr_t)((const gbuf *)buf)->dev & (to - 1)); }
+
+uint64_t sg_kv8_code_bytes(uint32_t n_kv, uint32_t hd, uint64_t cap) {
+    if (!sgk_kv8_shape_ok(n_kv, hd, 16) || cap > UINT32_MAX) return 0;
+    return (cap + SGK_KV8_TILE - 1) / SGK_KV8_TILE * n_kv * (2ull * SGK_KV8_TILE * hd);
+}
+uint64_t sg_kv8_scale_bytes(uint32_t n_kv, uint32_t block, uint64_t cap) {
+    if (!sgk_kv8_shape_ok(n_kv, 64, block) || cap > UINT32_MAX) return 0;
+    return (cap + block - 1) / block * n_kv * 8;
+}
+
+/* The shape, and the two buffers for `cap` positions (counted in 64 bits, so
+ * that base + n is checked before it could wrap). */
+static sg_err kv8_check(const char *who, void *codes, void *scales, uint32_t n_kv, uint32_t hd, uint32_t block, uint64_t cap) {
+    if (!sgk_kv8_shape_ok(n_kv, hd, block) || n_kv > 65535)
+        return errf("gpu: %s: n_kv in [1, 65535], head_dim 64, 128 or 256, block 16, 32, 64 or 128", who);
+    if (cap > UINT32_MAX - 128u) return errf("gpu: %s: %llu positions", who, (unsigned long long)cap);
+    sg_err e;
+    if (sg_failed(e = need(codes, sg_kv8_code_bytes(n_kv, hd, cap), "codes")) ||
+        sg_failed(e = need(scales, sg_kv8_scale_bytes(n_kv, block, cap), "scales"))) return e;
+    if (!aligned(codes, 16) || !aligned(scales, 4)) return errf("gpu: %s: codes must be 16-byte, scales 4-byte aligned", who);
+    return SG_OK;
+}
+
+/* Rows [n][n_kv hd] at a stride in k and v, and the cache, for store and load. */
+static sg_err kv8_rows_check(const char *who, void *k, void *v, void *codes, void *scales, const uint32_t p[8], uint64_t *stride) {
+    const uint32_t nkv = p[0], hd = p[1], n = p[4];
+    sg_err e = kv8_check(who, codes, scales, nkv, hd, p[2], (uint64_t)p[3] + n);
+    if (sg_failed(e)) return e;
+    if (!n || n > 1u << 27) return errf("gpu: %s: n must be in [1, 2^27]", who);
+    const uint64_t w = (uint64_t)nkv * hd;
+    *stride = p[5] ? p[5] : w;
+    if (*stride < w) return errf("gpu: %s: row stride below n_kv * head_dim", who);
+    const uint64_t bytes = ((n - 1) * *stride + w) * 4;
+    if (sg_failed(e = need(k, bytes, "k")) || sg_failed(e = need(v, bytes, "v"))) return e;
+    if (!aligned(k, 4) || !aligned(v, 4)) return errf("gpu: %s: k and v must be 4-byte aligned", who);
+    if (overlap(codes, scales) || overlap(codes, k) || overlap(codes, v) || overlap(scales, k) || overlap(scales, v))
+        return errf("gpu: %s: the cache must not overlap the rows", who);
+    return SG_OK;
+}
+
+sg_err sg_gpu_run_kv8_store(sg_gpu *g, void *k, void *v, void *codes, void *scales, const uint32_t p[8]) {
+    if (!g || !k || !v || !codes || !scales || !p) return (sg_err){"gpu: kv8_store got a NULL argument"};
+    uint64_t stride;
+    sg_err e = kv8_rows_check("kv8_store", k, v, codes, scales, p, &stride);
+    if (sg_failed(e)) return e;
+    int was;
+    if (sg_failed(e = on_device(g, &was))) return e;
+    void *ins[4] = {k, v, codes, scales};
+    if (!sg_failed(e = push(ins, 4)))
+        e = finish(g, sgk_kv8_store(DEV(k), DEV(v), stride, DEV(codes), DEV(scales), p[0], p[1], p[2], p[3], p[4], g->stream),
+                   ins + 2, 2);
+    return back_to(g, was, e);
+}
+
+sg_err sg_gpu_run_kv8_load(sg_gpu *g, void *codes, void *scales, void *k, void *v, const uint32_t p[8]) {
+    if (!g || !k || !v || !codes || !scales || !p) return (sg_err){"gpu: kv8_load got a NULL argument"};
+    uint64_t stride;
+    sg_err e = kv8_rows_check("kv8_load", k, v, codes, scales, p, &stride);
+    if (sg_failed(e)) return e;
+    /* k and v in one allocation: their rows may interleave, not collide */
+    const char *ka = DEV(k), *va = DEV(v);
+    const uint64_t w = (uint64_t)p[0] * p[1] * 4, sb = stride * 4, span = (uint64_t)(p[4] - 1) * sb + w;
+    const uint64_t off = ka < va ? (uint64_t)(va - ka) : (uint64_t)(ka - va);
+    if (off < span && (off % sb < w || off % sb > sb - w)) return (sg_err){"gpu: kv8_load: rows of k and v overlap"};
+    int was;
+    if (sg_failed(e = on_device(g, &was))) return e;
+    void *bufs[4] = {codes, scales, k, v};
+    if (!sg_failed(e = push(bufs, 4)))
+        e = finish(g, sgk_kv8_load(DEV(codes), DEV(scales), DEV(k), DEV(v), stride, p[0], p[1], p[2], p[3], p[4], g->stream),
+                   bufs + 2, 2);
+    return back_to(g, was, e);
+}
+
+static sg_err attn_kv8_oneshot(sg_gpu *g, const char *who, void *q, void *codes, void *scales, void *out, uint32_t nh,
+                               uint32_t nkv, uint32_t hd, uint32_t base, uint32_t n, uint32_t qs, uint32_t scale, uint32_t block) {
+    if (!g || !q || !codes || !scales || !out) return errf("gpu: %s got a NULL argument", who);
+    sg_err e = kv8_check(who, codes, scales, nkv, hd, block, (uint64_t)base + n);
+    if (sg_failed(e)) return e;
+    if (!nh || nh % nkv || nh / nkv > SGK_KV8_MAX_GROUP)
+        return errf("gpu: %s: n_heads must be a multiple of n_kv_heads, at most %u times it", who, SGK_KV8_MAX_GROUP);
+    if (qs < hd) return errf("gpu: %s: q_stride < head_dim", who);
+    const uint64_t rows = (uint64_t)(n ? n : 1) * nh;
+    if (sg_failed(e = need(q, ((rows - 1) * qs + hd) * 4, "q")) || sg_failed(e = need(out, rows * hd * 4, "out"))) return e;
+    if (!aligned(q, 4) || !aligned(out, 4)) return errf("gpu: %s: q and out must be 4-byte aligned", who);
+    if (overlap(out, q) || overlap(out, codes) || overlap(out, scales)) return errf("gpu: %s: out overlaps an input", who);
+    int was;
+    if (sg_failed(e = on_device(g, &was))) return e;
+    void *ins[3] = {q, codes, scales}, *outs[1] = {out};
+    if (!sg_failed(e = push(ins, 3))) {
+        if (!n) {                       /* no key at all: zeros */
+            e = finish(g, sgk_fill_f32(DEV(out), 0.0f, rows * hd, g->stream), outs, 1);
+        } else {
+            const sgk_kv8_attn a = {DEV(q), DEV(codes), DEV(scales), DEV(out), nh, nkv, hd, block, qs, base, n,
+                                    (uint64_t)nh * qs, fbits(scale)};
+            e = finish(g, sgk_kv8_attention(&a, g->stream), outs, 1);
+        }
+    }
+    return back_to(g, was, e);
+}
+
+sg_err sg_gpu_run_attn_decode_kv8(sg_gpu *g, void *q, void *codes, void *scales, void *out, const uint32_t p[8]) {
+    if (!p) return (sg_err){"gpu: attn_decode_kv8 got a NULL argument"};
+    const uint32_t seq = p[3];
+    return attn_kv8_oneshot(g, "attn_decode_kv8", q, codes, scales, out, p[0], p[1], p[2], seq ? seq - 1 : 0, seq ? 1 : 0, p[4],
+                            p[5], p[6]);
+}
+
+sg_err sg_gpu_run_attn_prefill_kv8(sg_gpu *g, void *q, void *codes, void *scales, void *out, const uint32_t p[8]) {
+    if (!p) return (sg_err){"gpu: attn_prefill_kv8 got a NULL argument"};
+    if (!p[4]) return (sg_err){"gpu: attn_prefill_kv8: n is zero"};
+    return attn_kv8_oneshot(g, "attn_prefill_kv8", q, codes, scales, out, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
+}
+
+static void rope_inv_freq(double inv[SGK_ROPE_HALF], uint32_t rd, float theta);
+
+sg_err sg_gpu_run_rope_axes(sg_gpu *g, void *x, void *pos, void *out, const uint32_t p[8]) {
+    if (!g || !x || !pos || !out || !p) return (sg_err){"gpu: rope_axes got a NULL argument"};
+    const uint32_t hd = p[0], rd = p[1], nh = p[2], hs = p[3] ? p[3] : hd, n = p[4], half = rd / 2;
+    const uint32_t sec[3] = {p[5] & 255, p[5] >> 8 & 255, p[5] >> 16 & 255}, order = p[5] >> 24;
+    const float theta = fbits(p[6]);
+    if (!hd || hd > 256 || rd < 2 || rd > hd || rd % 2 || !nh || nh > 65535 || hs < hd || !n)
+        return (sg_err){"gpu: rope_axes: bad shape"};
+    const uint64_t w = (uint64_t)(nh - 1) * hs + hd, row = p[7] ? p[7] : (uint64_t)nh * hs;
+    if (row < w) return (sg_err){"gpu: rope_axes: row stride below the heads' width"};
+    if (!(theta > 0.0f) || isinf(theta)) return (sg_err){"gpu: rope_axes: theta must be positive and finite"};
+    if (order > 1 || sec[0] + sec[1] + sec[2] != half) return (sg_err){"gpu: rope_axes: sections must add up to rope_dim / 2, order 0 or 1"};
+    if (order && ((sec[1] && 3 * sec[1] - 2 >= half) || (sec[2] && 3 * sec[2] - 1 >= half)))
+        return (sg_err){"gpu: rope_axes: sections do not fit the interleaved order"};
+    uint8_t axis[SGK_ROPE_HALF];
+    for (uint32_t i = 0; i < half; i++) {
+        const uint32_t m = i % 3;
+        axis[i] = (uint8_t)(order ? (m && i < 3 * sec[m] ? m : 0) : i < sec[0] ? 0 : i < sec[0] + sec[1] ? 1 : 2);
+    }
+    sg_err e;
+    const uint64_t bytes = ((n - 1) * row + w) * 4;
+    if (sg_failed(e = need(x, bytes, "x")) || sg_failed(e = need(out, bytes, "out")) || sg_failed(e = need(pos, 12ull * n, "pos"))) return e;
+    if (!aligned(x, 4) || !aligned(out, 4) || !aligned(pos, 4)) return (sg_err){"gpu: rope_axes: buffers must be 4-byte aligned"};
+    if (overlap(out, pos) || (overlap(out, x) && DEV(out) != DEV(x))) return (sg_err){"gpu: rope_axes: out overlaps an input"};
+    double inv[SGK_ROPE_HALF];
+    rope_inv_freq(inv, rd, theta);
+    int was;
+    if (sg_failed(e = on_device(g, &was))) return e;
+    void *ins[3] = {x, pos, out}, *outs[1] = {out};     /* out too: its gaps stay as they are */
+    if (!sg_failed(e = push(ins, out == x ? 2 : 3))) {
+        const sgk_rope_axes_args a = {DEV(x), DEV(pos), DEV(out), row, hd, rd, nh, hs, n};
+        e = finish(g, sgk_rope_axes(&a, inv, axis, g->stream), outs, 1);
+    }
+    return back_to(g, was, e);
+}
+
+sg_err sg_gpu_run_token_counts(sg_gpu *g, void *ids, void *counts, const uint32_t p[8]) {
+    if (!g || !counts || !p || (p[0] && !ids)) return (sg_err){"gpu: token_counts got a NULL argument"};
+    const uint32_t n = p[0], vocab = p[1], rows = p[2];
+    if (!vocab || vocab > INT32_MAX || !rows || rows > 65535 || p[3] > 1)
+        return (sg_err){"gpu: token_counts: bad shape (vocab in [1, 2^31), rows in [1, 65535], clear 0 or 1)"};
+    sg_err e;
+    if ((n && sg_failed(e = need(ids, (uint64_t)n * rows * 4, "ids"))) ||
+        sg_failed(e = need(counts, (uint64_t)vocab * rows * 4, "counts"))) return e;
+    if (!aligned(counts, 4) || (n && !aligned(ids, 4))) return (sg_err){"gpu: token_counts: buffers must be 4-byte aligned"};
+    if (n && overlap(ids, counts)) return (sg_err){"gpu: token_counts: buffers must not overlap"};
+    int was;
+    if (sg_failed(e = on_device(g, &was))) return e;
+    void *bufs[2] = {counts, n ? ids : NULL};
+    if (!sg_failed(e = push(bufs, 2)))
+        e = finish(g, sgk_token_counts(n ? DEV(ids) : NULL, DEV(counts), n, vocab, rows, p[3] != 0, g->stream), bufs, 1);
+    return back_to(g, was, e);
+}
+
+sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void *mask, void *out, void *token,
+                         const uint32_t p[8]) {
+    if (!g || !logits || !out || !token || !p) return (sg_err){"gpu: logits got a NULL argument"};
+    const uint32_t vocab = p[0], rows = p[1];
+    const float rep = fbits(p[2]), freq = fbits(p[3]), pres = fbits(p[4]);
+    if (!vocab || vocab > INT32_MAX || !rows || rows > 65535)
+        return (sg_err){"gpu: logits: bad shape (vocab in [1, 2^31), rows in [1, 65535])"};
+    if (!(rep > 0.0f) || isinf(rep) || !isfinite(freq) || !isfinite(pres))
+        return (sg_err){"gpu: logits: repetition must be positive and finite, frequency and presence finite"};
+    const uint64_t lb = (uint64_t)vocab * rows * 4;
+    sg_err e;
+    if (sg_failed(e = need(logits, lb, "logits")) || sg_failed(e = need(out, lb, "out")) ||
+        sg_failed(e = need(token, (uint64_t)rows * 4, "token")) || (counts && sg_failed(e = need(counts, lb, "counts"))) ||
+        (bias && sg_failed(e = need(bias, (uint64_t)vocab * 4, "bias"))) ||
+        (mask && sg_failed(e = need(mask, (uint64_t)(vocab + 31) / 32 * rows * 4, "mask")))) return e;
+    void *bufs[6] = {logits, counts, bias, mask, out, token}, *outs[2] = {out, token};
+    for (int i = 0; i < 6; i++) {
+        if (bufs[i] && !aligned(bufs[i], 4)) return (sg_err){"gpu: logits: buffers must be 4-byte aligned"};
+        if ((i < 5 && overlap(token, bufs[i])) || (i < 4 && overlap(out, bufs[i]) && !(i == 0 && DEV(out) == DEV(logits))))
+            return (sg_err){"gpu: logits: an output overlaps another buffer"};
+    }
+    int was;
+    if (sg_failed(e = on_device(g, &was))) return e;
+    void *part;
+    if (!sg_failed(e = scratch(g, sgk_logits_part_bytes(rows), &part)) && !sg_failed(e = push(bufs, 4))) {
+        const sgk_logits_args a = {DEV(logits), DEV(counts), DEV(bias), DEV(mask), DEV(out), DEV(token), vocab, rows, rep, freq, pres};
+        e = finish(g, sgk_logits(&a, part, g->stream), outs, 2);
+    }
+    return back_to(g, was, e);
+}
+
+/* ---------------------------------------------------------------------
  * prefill per-op hooks (surge.h:787-800, 1133-1142): the chunk kernels the
  * prefill path runs, one synchronous call each, with the reference's
  * argument layouts and params.

@@ -371,6 +371,59 @@ uint32_t sgk_device_cus(void);
 hipError_t sgk_read(const void *p, uint64_t bytes, float *out, uint32_t blocks, hipStream_t s);
 hipError_t sgk_empty(hipStream_t s);
 
+/* The 8-bit K/V cache (kv8.hip): codes int8 [tile of 16][n_kv][2][16 hd] in the
+ * matrix instructions' orders, scales f32 [position / block][n_kv][2]; see
+ * surge.h for the layout and the quantiser. */
+#define SGK_KV8_TILE 16u
+SGK_HD static inline int sgk_kv8_shape_ok(uint32_t n_kv, uint32_t hd, uint32_t block) {
+    return n_kv && (hd == 64 || hd == 128 || hd == 256) && (block == 16 || block == 32 || block == 64 || block == 128);
+}
+hipError_t sgk_kv8_store(const float *k, const float *v, uint64_t stride, int8_t *codes, float *scales, uint32_t n_kv,
+                         uint32_t hd, uint32_t block, uint32_t base, uint32_t n, hipStream_t s);
+hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, float *k, float *v, uint64_t stride, uint32_t n_kv,
+                        uint32_t hd, uint32_t block, uint32_t base, uint32_t n, hipStream_t s);
+/* Causal attention of ntok tokens at positions base .. base+ntok-1 over the
+ * cache; token z's head h at q + z*q_tok + h*q_stride, out [ntok][n_heads][hd]. */
+typedef struct {
+    const float *q;
+    const int8_t *codes;
+    const float *scales;
+    float *out;
+    uint32_t n_heads, n_kv, hd, block, q_stride, base, ntok;
+    uint64_t q_tok;
+    float scale;
+} sgk_kv8_attn;
+#define SGK_KV8_MAX_GROUP 16u       /* query heads per kv head */
+hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, hipStream_t s);
+
+/* Rotary positions with three axes (token.hip). inv and axis: rope_dim/2
+ * inverse frequencies and axes (host memory, read before return). */
+typedef struct {
+    const float *x;
+    const int32_t *pos;         /* [3][n] */
+    float *out;
+    uint64_t row;               /* floats between tokens */
+    uint32_t head_dim, rope_dim, heads, stride, n;
+} sgk_rope_axes_args;
+hipError_t sgk_rope_axes(const sgk_rope_axes_args *a, const double *inv, const uint8_t *axis, hipStream_t s);
+
+/* counts[row][id] += occurrences; cleared first with clear != 0. */
+hipError_t sgk_token_counts(const int32_t *ids, uint32_t *counts, uint32_t n, uint32_t vocab, uint32_t rows, int clear,
+                            hipStream_t s);
+typedef struct {
+    const float *x;
+    const uint32_t *counts;     /* or NULL */
+    const float *bias;          /* or NULL */
+    const uint32_t *mask;       /* or NULL */
+    float *out;
+    uint32_t *token;
+    uint32_t vocab, rows;
+    float rep, freq, pres;
+} sgk_logits_args;
+/* part: scratch of sgk_logits_part_bytes(rows). */
+uint64_t sgk_logits_part_bytes(uint32_t rows);
+hipError_t sgk_logits(const sgk_logits_args *a, void *part, hipStream_t s);
+
 /* The device-resident workspace of the no-allocation entry points: a
  * file-scope device array of SGK_SCRATCH_BYTES in kernels.hip. Call
  * sgk_scratch_init(dev) once per device with that device current; then
