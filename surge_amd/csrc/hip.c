@@ -982,7 +982,9 @@ static sg_err attn_kv8_oneshot(sg_gpu *g, const char *who, void *q, void *codes,
         } else {
             const sgk_kv8_attn a = {DEV(q), DEV(codes), DEV(scales), DEV(out), nh, nkv, hd, block, qs, base, n,
                                     (uint64_t)nh * qs, fbits(scale)};
-            e = finish(g, sgk_kv8_attention(&a, g->stream), outs, 1);
+            const uint64_t bytes = sgk_kv8_attn_scratch(&a);
+            void *t = NULL;
+            if (!bytes || !sg_failed(e = scratch(g, bytes, &t))) e = finish(g, sgk_kv8_attention(&a, t, g->stream), outs, 1);
         }
     }
     return back_to(g, was, e);

@@ -394,7 +394,9 @@ typedef struct {
     float scale;
 } sgk_kv8_attn;
 #define SGK_KV8_MAX_GROUP 16u       /* query heads per kv head */
-hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, hipStream_t s);
+/* scratch: sgk_kv8_attn_scratch(a) bytes, 16-byte aligned (NULL if that is 0). */
+uint64_t sgk_kv8_attn_scratch(const sgk_kv8_attn *a);
+hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hipStream_t s);
 
 /* Rotary positions with three axes (token.hip). inv and axis: rope_dim/2
  * inverse frequencies and axes (host memory, read before return). */

@@ -248,9 +248,298 @@ __global__ void __launch_bounds__(TPB) k_kv8_attn(sgk_kv8_attn a) {
     if (t < hd) a.out[((size_t)z * a.n_heads + h) * hd + t] = o / l;
 }
 
-extern "C" hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, hipStream_t s) {
+// ---------------------------------------------------------------------------
+// Attention of few rows (tokens x the query heads of one kv head, at most 16),
+// split over the keys: decode, and chunks of a few tokens. Every wave streams
+// its own steps of 32 keys straight from the cache into operands:
+//  - q in fixed point against its row's largest element, 24 bits as three int8
+//    digits (q = sq (65536 d2 + 256 d1 + d0)): the score product is three
+//    v_mfma_i32_16x16x64_i8 on the key codes as they lie, its sums exact, and
+//    the keys are never converted;
+//  - S^T = K Q^T leaves lane (li, lg) row li's scores of keys 4 lg .. 4 lg + 3
+//    of both tiles, the order of the value records' dwords, so V^T P^T runs on
+//    v_mfma_f32_16x16x32_f16 with the codes as f16 (exact) and p in two halves;
+//  - the values' scale goes into p: w = p s_V. The running maximum is taken
+//    over score + log2 s_V, so that w <= 2^12 whatever the scales are, while
+//    the sum of p, at most 2^92 a key (log2 s_V >= -80), stays in f32's range.
+//    2^12 keeps w's lower half above f16's subnormals down to 2^-26 of the
+//    largest.
+// No barrier or LDS in the key loop; the waves' maxima, sums and outputs join
+// at the end. Bound by the cache's bytes.
+// ---------------------------------------------------------------------------
+struct kv8_part { float *m, *s, *acc; };    // [token][head][split] maxima and sums, [..][hd] outputs; NULL: one split
+
+#define KV8_P2 12.0f
+
+// 16 f32 of a row as the three digits' operand bytes
+__device__ __forceinline__ void q_digits(const float (&x)[16], float inv, v4i &d0, v4i &d1, v4i &d2) {
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        uint32_t b0 = 0, b1 = 0, b2 = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int q = (int)rintf(x[4 * w + e] * inv);
+            const int l0 = (int8_t)q, r1 = (q - l0) >> 8, l1 = (int8_t)r1, l2 = (r1 - l1) >> 8;
+            b0 |= (uint32_t)(l0 & 0xFF) << (8 * e);
+            b1 |= (uint32_t)(l1 & 0xFF) << (8 * e);
+            b2 |= (uint32_t)(l2 & 0xFF) << (8 * e);
+        }
+        d0[w] = (int)b0; d1[w] = (int)b1; d2[w] = (int)b2;
+    }
+}
+// A row's q (spread over the four lanes of its column) as digits; returns the
+// factor of the integer scores, sq * mul, NaN if an element is not finite.
+template <int NC>
+__device__ __forceinline__ float q_row(const float *q, bool on, bool al, uint32_t lg, float mul, v4i (&d)[3][NC]) {
+    float x[NC][16];
+    uint32_t mx = 0;
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+            if (on) v = ld4(q + 64 * c + 16 * lg + 4 * w, al);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[c][4 * w + e] = v[e];
+                mx = max(mx, __float_as_uint(v[e]) & 0x7FFFFFFFu);
+            }
+        }
+    mx = max(mx, swap16(mx));
+    mx = max(mx, swap32(mx));
+    const bool bad = mx >= 0x7F800000u;
+    float am = bad ? 0.0f : __uint_as_float(mx);
+    const float up = am < 0x1p-60f ? 0x1p64f : 1.0f;    // a row near the end of the range, times 2^64
+    am *= up;
+    const float inv = am > 0.0f ? 8323072.0f / am : 0.0f;       // 127 * 65536
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[c][e] = bad ? 0.0f : x[c][e] * up;
+        q_digits(x[c], inv, d[0][c], d[1][c], d[2][c]);
+    }
+    return bad ? NAN : am / 8323072.0f * mul / up;
+}
+// the score sums of the three digits as one float (a2 * 256 + a1 < 2^31)
+__device__ __forceinline__ float q_join(int a0, int a1, int a2) {
+    return fmaf((float)(a2 * 256 + a1), 256.0f, (float)a0);
+}
+// eight codes (two dwords) as f16: the byte + 128 under 1024's exponent, less 1152
+__device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
+    const f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+    const uint32_t ua = a ^ 0x80808080u, ub = b ^ 0x80808080u;
+    f16x8 r;
+    auto put = [&](int at, uint32_t u, uint32_t sel) {
+        const f16x2 v = __builtin_bit_cast(f16x2, (uint32_t)__builtin_amdgcn_perm(0x64646464u, u, sel)) - off;
+        r[at] = v[0];
+        r[at + 1] = v[1];
+    };
+    put(0, ua, 0x04010400u);
+    put(2, ua, 0x04030402u);
+    put(4, ub, 0x04010400u);
+    put(6, ub, 0x04030402u);
+    return r;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part part, int al) {
+    constexpr int NC = HD / 64, NT = HD / 16, OLD = HD + 4;
+    __shared__ float wm[4][16], wl[4][16];
+    __shared__ __align__(16) float ob[2][16 * OLD];
+    const uint32_t t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const uint32_t hk = blockIdx.y, sp = blockIdx.x, S = gridDim.x, G = a.n_heads / a.n_kv, R = a.ntok * G;
+    const uint32_t ntile = (uint32_t)(((uint64_t)a.base + a.ntok + KV8_T - 1) / KV8_T), nstep = (ntile + 1) / 2;
+    const uint32_t s0 = (uint32_t)((uint64_t)sp * nstep / S), s1 = (uint32_t)((uint64_t)(sp + 1) * nstep / S);
+    const uint32_t bsh = __builtin_ctz(a.block / KV8_T);
+    const uint32_t tok = li < R ? li / G : 0, rpos = a.base + tok;
+    const int8_t *codes = a.codes + (size_t)hk * (2 * KV8_T * HD) + lane * 16;
+    const size_t rec = (size_t)a.n_kv * (2 * KV8_T * HD);
+    const float *scales = a.scales + 2 * hk;
+    const size_t srec = 2 * (size_t)a.n_kv;
+
+    v4u kr[2][NC], vr[2][NC];
+    float ks[2], vs[2], nks[2], nvs[2];
+    auto tile_of = [&](uint32_t step, int u) { return min(2 * step + u, ntile - 1); };
+    auto load_k = [&](uint32_t step) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const v4u *p = (const v4u *)(codes + tile_of(step, u) * rec);
+#pragma unroll
+            for (int c = 0; c < NC; c++) kr[u][c] = __builtin_nontemporal_load(p + c * 64);
+        }
+    };
+    auto load_v = [&](uint32_t step) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const v4u *p = (const v4u *)(codes + tile_of(step, u) * rec + KV8_T * HD);
+#pragma unroll
+            for (int c = 0; c < NC; c++) vr[u][c] = __builtin_nontemporal_load(p + c * 64);
+        }
+    };
+    auto load_s = [&](uint32_t step) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const float *p = scales + (size_t)(tile_of(step, u) >> bsh) * srec;
+            nks[u] = p[0];
+            nvs[u] = p[1];
+        }
+    };
+    uint32_t step = s0 + wave;
+    if (step < s1) {
+        load_s(step);
+        load_k(step);
+        load_v(step);
+    }
+    v4i qd[3][NC];
+    const float qf = q_row<NC>(a.q + tok * a.q_tok + (size_t)(hk * G + li % G) * a.q_stride, li < R, al, lg,
+                               a.scale * 1.44269504088896340736f, qd);
+    f32x4 o[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) o[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float mrun = -INFINITY, lsum = 0.0f;
+    for (; step < s1; step += 4) {
+        float sc[2][4], tm = -INFINITY;
+        const bool whole = step * 32 + 31 <= a.base;            // every row sees every key
+#pragma unroll
+        for (int u = 0; u < 2; u++) { ks[u] = nks[u]; vs[u] = nvs[u]; }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            v4i s[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int d = 0; d < 3; d++)
+                    s[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, kr[u][c]), qd[d][c], s[d], 0, 0, 0);
+            const float f = qf * ks[u], lv = __builtin_amdgcn_logf(fmaxf(vs[u], 0x1p-80f));
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                sc[u][e] = q_join(s[0][e], s[1][e], s[2][e]) * f;
+                if (whole || step * 32 + u * 16 + 4 * lg + e <= rpos) tm = fmaxf(tm, sc[u][e] + lv);
+            }
+        }
+        const bool more = step + 4 < s1;
+        if (more) { load_s(step + 4); load_k(step + 4); }
+        tm = fmaxf(tm, swap16f(tm));
+        tm = fmaxf(tm, swap32f(tm));
+        const float mnew = fmaxf(mrun, tm), m0 = mnew - KV8_P2;
+        const float al2 = mrun == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrun - mnew);
+        mrun = mnew;
+        lsum *= al2;
+        f16x8 ph, pl;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const bool on = whole || step * 32 + u * 16 + 4 * lg + e <= rpos;
+                const float p = on ? __builtin_amdgcn_exp2f(sc[u][e] - m0) : 0.0f;
+                lsum += p;
+                const float w = on ? p * vs[u] : 0.0f;
+                const _Float16 h = (_Float16)w;
+                ph[4 * u + e] = h;
+                pl[4 * u + e] = (_Float16)(w - (float)h);
+            }
+        if (__builtin_amdgcn_ballot_w64(al2 != 1.0f)) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) o[n] *= al2;
+        }
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const f16x8 v = codes_f16(vr[0][c][j], vr[1][c][j]);
+                o[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[4 * c + j], 0, 0, 0);
+                o[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[4 * c + j], 0, 0, 0);
+            }
+        if (more) load_v(step + 4);
+    }
+    // join the four waves: maxima and sums first, then outputs 2 + 0, 3 + 1, both
+    lsum += swap16f(lsum);
+    lsum += swap32f(lsum);
+    if (lg == 0) { wm[wave][li] = mrun; wl[wave][li] = lsum; }
+    __syncthreads();
+    const float M = fmaxf(fmaxf(wm[0][li], wm[1][li]), fmaxf(wm[2][li], wm[3][li]));
+    const float f = mrun == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrun - M);
+#pragma unroll
+    for (int n = 0; n < NT; n++) o[n] *= f;
+    float *mine = &ob[wave & 1][li * OLD + 4 * lg];
+    if (wave >= 2) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) *(f32x4 *)(mine + 16 * n) = o[n];
+    }
+    __syncthreads();
+    if (wave < 2) {
+#pragma unroll
+        for (int n = 0; n < NT; n++) *(f32x4 *)(mine + 16 * n) += o[n];
+    }
+    __syncthreads();
+    for (uint32_t i = t; i < R * (HD / 4); i += TPB) {
+        const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
+        const f32x4 v = *(const f32x4 *)&ob[0][r * OLD + d] + *(const f32x4 *)&ob[1][r * OLD + d];
+        const float m = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+            l += wl[w][r] * (wm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wm[w][r] - m));
+        const size_t row = (size_t)(r / G) * a.n_heads + hk * G + r % G;
+        if (S == 1) {
+            st4(a.out + row * HD + d, v / l, !((uintptr_t)a.out & 15));
+        } else {
+            *(f32x4 *)(part.acc + (row * S + sp) * HD + d) = v;
+            // base e for the combine; a sum that is NaN has to reach it whatever the maximum
+            if (d == 0) { part.m[row * S + sp] = l != l ? 0.0f : m * 0.69314718055994530942f; part.s[row * S + sp] = l; }
+        }
+    }
+}
+
+// How a call runs. Few rows: the key-split form, in as many splits as give
+// every wave a step, up to two workgroups per CU (what is resident).
+struct kv8_plan { bool wave; uint32_t splits; };
+static kv8_plan kv8_plan_of(const sgk_kv8_attn *a) {
+    kv8_plan p = {(uint64_t)a->ntok * (a->n_heads / a->n_kv) <= 16, 1};
+    const uint64_t steps = ((uint64_t)a->base + a->ntok + 31) / 32;
+    if (p.wave) {
+        uint64_t most = 2ull * sgk_device_cus() / a->n_kv, want = (steps + 3) / 4;
+        if (most > 1024) most = 1024;
+        if (most < 1) most = 1;
+        p.splits = (uint32_t)(want < most ? want : most);
+    }
+    return p;
+}
+
+extern "C" uint64_t sgk_kv8_attn_scratch(const sgk_kv8_attn *a) {
+    const kv8_plan p = kv8_plan_of(a);
+    return p.splits > 1 ? (uint64_t)a->ntok * a->n_heads * p.splits * (a->hd + 2) * 4 : 0;
+}
+
+extern "C" hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hipStream_t s) {
     if (!a->ntok || !a->n_heads) return hipSuccess;
-    if (!sgk_kv8_shape_ok(a->n_kv, a->hd, a->block) || ((uintptr_t)a->codes & 15)) return hipErrorInvalidValue;
+    if (!sgk_kv8_shape_ok(a->n_kv, a->hd, a->block) || ((uintptr_t)a->codes & 15) || a->n_heads % a->n_kv ||
+        a->n_heads / a->n_kv > SGK_KV8_MAX_GROUP) return hipErrorInvalidValue;
+    const kv8_plan p = kv8_plan_of(a);
+    if (p.splits > 1 && !scratch) return hipErrorInvalidValue;
+    const int al = !((uintptr_t)a->q & 15) && a->q_stride % 4 == 0 && a->q_tok % 4 == 0;
+    const uint64_t rows = (uint64_t)a->ntok * a->n_heads * p.splits;
+    kv8_part part = {};
+    if (p.splits > 1) {                 // outputs first, as they are stored 16 bytes at a time
+        part.acc = (float *)scratch;
+        part.m = part.acc + rows * a->hd;
+        part.s = part.m + rows;
+    }
+    if (p.wave) {
+        const dim3 grid(p.splits, a->n_kv);
+        switch (a->hd) {
+        case 64: hipLaunchKernelGGL(k_kv8_wave<64>, grid, dim3(TPB), 0, s, *a, part, al); break;
+        case 128: hipLaunchKernelGGL(k_kv8_wave<128>, grid, dim3(TPB), 0, s, *a, part, al); break;
+        default: hipLaunchKernelGGL(k_kv8_wave<256>, grid, dim3(TPB), 0, s, *a, part, al); break;
+        }
+        if (p.splits == 1) return hipGetLastError();
+        sgk_attn c = {};
+        c.m = part.m; c.s = part.s; c.acc = part.acc; c.out = a->out; c.n_heads = a->n_heads; c.n_kv = a->n_kv; c.hd = a->hd;
+        c.out_tok = a->n_heads * a->hd; c.n_splits = p.splits; c.max_splits = p.splits; c.ntok = a->ntok;
+        const hipError_t e = hipGetLastError();
+        return e == hipSuccess ? sgk_attn_combine(&c, s) : e;
+    }
     for (uint32_t z = 0; z < a->ntok; z += 32768) {
         sgk_kv8_attn b = *a;
         b.q += z * a->q_tok; b.out += (size_t)z * a->n_heads * a->hd; b.base += z;
