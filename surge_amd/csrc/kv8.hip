@@ -204,51 +204,6 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
 }
 
 // ---------------------------------------------------------------------------
-// Attention, one workgroup per (token, query head): per tile of 16 positions
-// thread (chunk c, position r) sums hd/16 products, 16 chunks per position are
-// added through LDS, then thread d accumulates dim d. The running maximum and
-// sum are kept per thread, the same in all of them.
-// ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(TPB) k_kv8_attn(sgk_kv8_attn a) {
-    __shared__ float qs[256];
-    __shared__ float ds[16][KV8_T + 1];
-    const uint32_t t = threadIdx.x, h = blockIdx.x, z = blockIdx.y, hd = a.hd, hk = h / (a.n_heads / a.n_kv);
-    const uint32_t last = a.base + z;
-    const float *q = a.q + z * a.q_tok + (size_t)h * a.q_stride;
-    if (t < hd) qs[t] = q[t];
-    __syncthreads();
-    const uint32_t c = t / 16, r = t % 16, cw = hd / 16;
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (uint32_t tile = 0; tile <= last / KV8_T; tile++) {
-        const float *sc = a.scales + ((size_t)(tile * KV8_T / a.block) * a.n_kv + hk) * 2;
-        const int8_t *rec = a.codes + rec_at(tile, a.n_kv, hk, hd);
-        float dot = 0.0f;
-        for (uint32_t e = 0; e < cw; e++) dot = fmaf(qs[c * cw + e], (float)rec[key_at(r, c * cw + e)], dot);
-        ds[c][r] = dot;
-        __syncthreads();
-        float sv[KV8_T], tm = -INFINITY;
-        for (uint32_t j = 0; j < KV8_T; j++) {
-            float x = 0.0f;
-            for (uint32_t i = 0; i < 16; i++) x += ds[i][j];
-            sv[j] = tile * KV8_T + j <= last ? x * sc[0] * a.scale : -INFINITY;
-            tm = fmaxf(tm, sv[j]);
-        }
-        const float mn = fmaxf(m, tm), al = m == -INFINITY ? 0.0f : expf(m - mn);
-        m = mn;
-        l *= al;
-        o *= al;
-        for (uint32_t j = 0; j < KV8_T; j++) {
-            if (tile * KV8_T + j > last) break;
-            const float p = expf(sv[j] - m);
-            l += p;
-            if (t < hd) o = fmaf(p, (float)rec[KV8_T * hd + val_at(j, t)] * sc[1], o);
-        }
-        __syncthreads();
-    }
-    if (t < hd) a.out[((size_t)z * a.n_heads + h) * hd + t] = o / l;
-}
-
-// ---------------------------------------------------------------------------
 // Attention of few rows (tokens x the query heads of one kv head, at most 16),
 // split over the keys: decode, and chunks of a few tokens. Every wave streams
 // its own steps of 32 keys straight from the cache into operands:
@@ -492,18 +447,222 @@ __global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part pa
     }
 }
 
-// How a call runs. Few rows: the key-split form, in as many splits as give
-// every wave a step, up to two workgroups per CU (what is resident).
-struct kv8_plan { bool wave; uint32_t splits; };
-static kv8_plan kv8_plan_of(const sgk_kv8_attn *a) {
-    kv8_plan p = {(uint64_t)a->ntok * (a->n_heads / a->n_kv) <= 16, 1};
-    const uint64_t steps = ((uint64_t)a->base + a->ntok + 31) / 32;
-    if (p.wave) {
-        uint64_t most = 2ull * sgk_device_cus() / a->n_kv, want = (steps + 3) / 4;
-        if (most > 1024) most = 1024;
-        if (most < 1) most = 1;
-        p.splits = (uint32_t)(want < most ? want : most);
+// ---------------------------------------------------------------------------
+// Attention of many rows: a workgroup takes NW x CT x 16 consecutive rows
+// (token-major, the query heads of one kv head inside a token, so any group
+// size fills them) and walks its keys in tiles of 64, staged once in LDS for
+// all of them: the key codes as they lie (1 KB per operand fragment, 16 bytes
+// a lane, no bank conflict), the value codes turned into f16 on the way. The
+// arithmetic is the wave form's; a wave holds CT column tiles of 16 rows.
+// Both tiles are double-buffered: the next tile's loads are requested right
+// after a barrier, stored behind the current tile's products, one barrier per
+// tile. Grid: (row block, kv head, key split), the longest rows first.
+// ---------------------------------------------------------------------------
+template <int HD, int NW, int CT>
+__global__ void __launch_bounds__(NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_part part, int al) {
+    constexpr int NC = HD / 64, NT = HD / 16, NTH = NW * 64, ROWS = NW * CT * 16;
+    constexpr int KCH = 4 * NC * 64, VUN = 2 * NC * 64;     // 16-byte chunks of keys, units (two chunks) of values
+    constexpr int KPT = (KCH + NTH - 1) / NTH, VPT = (VUN + NTH - 1) / NTH;
+    __shared__ v4u kb[2][KCH];
+    __shared__ v4u vb[2][2 * NT * 64];
+    const uint32_t t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const uint32_t hk = blockIdx.y, sp = blockIdx.z, S = gridDim.z, G = a.n_heads / a.n_kv;
+    const uint64_t R = (uint64_t)a.ntok * G, r0 = (uint64_t)(gridDim.x - 1 - blockIdx.x) * ROWS;
+    const uint32_t lastk = a.base + (uint32_t)(min(r0 + ROWS, R) - 1) / G;      // the block's last visible key
+    const uint32_t nrec = lastk / KV8_T + 1, nt = lastk / 64 + 1;
+    const uint32_t k0 = (uint32_t)((uint64_t)sp * nt / S), k1 = (uint32_t)((uint64_t)(sp + 1) * nt / S);
+    const uint32_t bsh = __builtin_ctz(a.block / KV8_T);
+    const size_t rec = (size_t)a.n_kv * (2 * KV8_T * HD);
+    const int8_t *codes = a.codes + (size_t)hk * (2 * KV8_T * HD);
+    const float *scales = a.scales + 2 * hk;
+    const size_t srec = 2 * (size_t)a.n_kv;
+
+    v4u kr[KPT], vr[VPT][2];
+    auto load = [&](uint32_t kt) {
+#pragma unroll
+        for (int x = 0; x < KPT; x++) {
+            const uint32_t i = t + x * NTH;
+            if (KCH % NTH == 0 || i < KCH)
+                kr[x] = *(const v4u *)(codes + min(4 * kt + i / (NC * 64), nrec - 1) * rec + i % (NC * 64) * 16);
+        }
+#pragma unroll
+        for (int x = 0; x < VPT; x++) {
+            const uint32_t i = t + x * NTH;
+            if (VUN % NTH == 0 || i < VUN)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    vr[x][h] = *(const v4u *)(codes + min(4 * kt + i / (NC * 64) * 2 + h, nrec - 1) * rec + KV8_T * HD +
+                                              i % (NC * 64) * 16);
+        }
+    };
+    auto stage = [&](int b) {
+#pragma unroll
+        for (int x = 0; x < KPT; x++) {
+            const uint32_t i = t + x * NTH;
+            if (KCH % NTH == 0 || i < KCH) kb[b][i] = kr[x];
+        }
+#pragma unroll
+        for (int x = 0; x < VPT; x++) {
+            const uint32_t i = t + x * NTH;
+            if (VUN % NTH == 0 || i < VUN)
+#pragma unroll
+                for (int j = 0; j < 4; j++)         // fragment (pair, dim tile 4 c + j)
+                    vb[b][(i / 64 * 4 + j) * 64 + i % 64] = __builtin_bit_cast(v4u, codes_f16(vr[x][0][j], vr[x][1][j]));
+        }
+    };
+
+    if (k0 < k1) load(k0);
+    v4i qd[CT][3][NC];
+    float qf[CT], mrun[CT], lsum[CT];
+    uint32_t rpos[CT];
+    f32x4 o[CT][NT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        const uint64_t r = r0 + (wave * CT + ct) * 16 + li;
+        const uint32_t tok = r < R ? (uint32_t)(r / G) : 0, g = r < R ? (uint32_t)(r % G) : 0;
+        rpos[ct] = a.base + tok;
+        qf[ct] = q_row<NC>(a.q + tok * a.q_tok + (size_t)(hk * G + g) * a.q_stride, r < R, al, lg,
+                           a.scale * 1.44269504088896340736f, qd[ct]);
+        mrun[ct] = -INFINITY;
+        lsum[ct] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NT; n++) o[ct][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
+    // the wave's first and last visible keys: no mask up to the one, no work past the other
+    const uint64_t rw = r0 + wave * CT * 16;
+    const bool on = rw < R;
+    const uint32_t wfirst = on ? a.base + (uint32_t)(rw / G) : 0, wlast = on ? a.base + (uint32_t)((min(rw + CT * 16, R) - 1) / G) : 0;
+    if (k0 < k1) stage(0);
+    __syncthreads();
+    for (uint32_t kt = k0; kt < k1; kt++) {
+        const int b = (kt - k0) & 1;
+        const bool more = kt + 1 < k1;
+        if (more) load(kt + 1);
+        if (on && kt * 64 <= wlast) {
+            const bool whole = kt * 64 + 63 <= wfirst;
+            float ks[4], vs[4], sc[CT][4][4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const float *p = scales + (size_t)(min(4 * kt + u, nrec - 1) >> bsh) * srec;
+                ks[u] = p[0];
+                vs[u] = p[1];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                v4i s[CT][3];
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                    for (int d = 0; d < 3; d++) s[ct][d] = (v4i){0, 0, 0, 0};
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    const v4i kf = __builtin_bit_cast(v4i, kb[b][(u * NC + c) * 64 + lane]);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                        for (int d = 0; d < 3; d++)
+                            s[ct][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qd[ct][d][c], s[ct][d], 0, 0, 0);
+                }
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[ct][u][e] = q_join(s[ct][0][e], s[ct][1][e], s[ct][2][e]) * (qf[ct] * ks[u]);
+            }
+            f16x8 ph[CT][2], pl[CT][2];
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                float tm = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const float lv = __builtin_amdgcn_logf(fmaxf(vs[u], 0x1p-80f));
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (whole || kt * 64 + u * 16 + 4 * lg + e <= rpos[ct]) tm = fmaxf(tm, sc[ct][u][e] + lv);
+                }
+                tm = fmaxf(tm, swap16f(tm));
+                tm = fmaxf(tm, swap32f(tm));
+                const float mnew = fmaxf(mrun[ct], tm), m0 = mnew - KV8_P2;
+                const float al2 = mrun[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrun[ct] - mnew);
+                mrun[ct] = mnew;
+                lsum[ct] *= al2;
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const bool vis = whole || kt * 64 + u * 16 + 4 * lg + e <= rpos[ct];
+                        const float p = vis ? __builtin_amdgcn_exp2f(sc[ct][u][e] - m0) : 0.0f;
+                        lsum[ct] += p;
+                        const float w = vis ? p * vs[u] : 0.0f;
+                        const _Float16 h = (_Float16)w;
+                        ph[ct][u >> 1][4 * (u & 1) + e] = h;
+                        pl[ct][u >> 1][4 * (u & 1) + e] = (_Float16)(w - (float)h);
+                    }
+                if (__builtin_amdgcn_ballot_w64(al2 != 1.0f)) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++) o[ct][n] *= al2;
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < 2; m++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const f16x8 vf = __builtin_bit_cast(f16x8, vb[b][(m * NT + n) * 64 + lane]);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++) {
+                        o[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[ct][m], o[ct][n], 0, 0, 0);
+                        o[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[ct][m], o[ct][n], 0, 0, 0);
+                    }
+                }
+        }
+        if (more) stage(b ^ 1);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+        lsum[ct] += swap16f(lsum[ct]);
+        lsum[ct] += swap32f(lsum[ct]);
+        const uint64_t r = r0 + (wave * CT + ct) * 16 + li;
+        if (r >= R) continue;
+        const float l = lsum[ct];
+        const size_t row = (size_t)(r / G) * a.n_heads + hk * G + (uint32_t)(r % G);
+        if (S == 1) {
+            const bool oal = !((uintptr_t)a.out & 15);
+#pragma unroll
+            for (int n = 0; n < NT; n++) st4(a.out + row * HD + 16 * n + 4 * lg, o[ct][n] / l, oal);
+        } else {
+            float *acc = part.acc + (row * S + sp) * HD + 4 * lg;
+#pragma unroll
+            for (int n = 0; n < NT; n++) *(f32x4 *)(acc + 16 * n) = o[ct][n];
+            if (lg == 0) { part.m[row * S + sp] = l != l ? 0.0f : mrun[ct] * 0.69314718055994530942f; part.s[row * S + sp] = l; }
+        }
+    }
+}
+
+// How a call runs. Few rows: the key-split form, in as many splits as give
+// every wave a step, up to two workgroups per CU (what is resident). More:
+// row blocks, their keys split until the chip is full.
+#ifndef KV8_NW
+#define KV8_NW 8
+#define KV8_CT 1
+#endif
+#define KV8_ROWS (KV8_NW * KV8_CT * 16u)
+struct kv8_plan { bool wave; uint32_t splits, blocks; };
+static kv8_plan kv8_plan_of(const sgk_kv8_attn *a) {
+    const uint64_t rows = (uint64_t)a->ntok * (a->n_heads / a->n_kv);
+    kv8_plan p = {rows <= 16, 1, (uint32_t)((rows + KV8_ROWS - 1) / KV8_ROWS)};
+    const uint64_t keys = (uint64_t)a->base + a->ntok, cus = sgk_device_cus();
+    uint64_t most, want;
+    if (p.wave) {
+        most = 2 * cus / a->n_kv;
+        want = (keys + 127) / 128;
+    } else {
+        most = (cus + (uint64_t)p.blocks * a->n_kv - 1) / ((uint64_t)p.blocks * a->n_kv);
+        want = (keys + 127) / 128;
+    }
+    if (most > 1024) most = 1024;
+    if (most < 1) most = 1;
+    p.splits = (uint32_t)(want < most ? want : most);
     return p;
 }
 
@@ -526,25 +685,22 @@ extern "C" hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hi
         part.m = part.acc + rows * a->hd;
         part.s = part.m + rows;
     }
-    if (p.wave) {
-        const dim3 grid(p.splits, a->n_kv);
-        switch (a->hd) {
-        case 64: hipLaunchKernelGGL(k_kv8_wave<64>, grid, dim3(TPB), 0, s, *a, part, al); break;
-        case 128: hipLaunchKernelGGL(k_kv8_wave<128>, grid, dim3(TPB), 0, s, *a, part, al); break;
-        default: hipLaunchKernelGGL(k_kv8_wave<256>, grid, dim3(TPB), 0, s, *a, part, al); break;
-        }
-        if (p.splits == 1) return hipGetLastError();
-        sgk_attn c = {};
-        c.m = part.m; c.s = part.s; c.acc = part.acc; c.out = a->out; c.n_heads = a->n_heads; c.n_kv = a->n_kv; c.hd = a->hd;
-        c.out_tok = a->n_heads * a->hd; c.n_splits = p.splits; c.max_splits = p.splits; c.ntok = a->ntok;
-        const hipError_t e = hipGetLastError();
-        return e == hipSuccess ? sgk_attn_combine(&c, s) : e;
+#define KC(H)                                                                                                                 \
+    do {                                                                                                                      \
+        if (p.wave) hipLaunchKernelGGL(k_kv8_wave<H>, dim3(p.splits, a->n_kv), dim3(TPB), 0, s, *a, part, al);                \
+        else hipLaunchKernelGGL((k_kv8_tile<H, KV8_NW, KV8_CT>), dim3(p.blocks, a->n_kv, p.splits), dim3(KV8_NW * 64), 0, s,  \
+                                *a, part, al);                                                                                \
+    } while (0)
+    switch (a->hd) {
+    case 64: KC(64); break;
+    case 128: KC(128); break;
+    default: KC(256); break;
     }
-    for (uint32_t z = 0; z < a->ntok; z += 32768) {
-        sgk_kv8_attn b = *a;
-        b.q += z * a->q_tok; b.out += (size_t)z * a->n_heads * a->hd; b.base += z;
-        b.ntok = a->ntok - z < 32768 ? a->ntok - z : 32768;
-        hipLaunchKernelGGL(k_kv8_attn, dim3(a->n_heads, b.ntok), dim3(TPB), 0, s, b);
-    }
-    return hipGetLastError();
+#undef KC
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.splits == 1) return e;
+    sgk_attn c = {};
+    c.m = part.m; c.s = part.s; c.acc = part.acc; c.out = a->out; c.n_heads = a->n_heads; c.n_kv = a->n_kv; c.hd = a->hd;
+    c.out_tok = a->n_heads * a->hd; c.n_splits = p.splits; c.max_splits = p.splits; c.ntok = a->ntok;
+    return sgk_attn_combine(&c, s);
 }
