@@ -347,8 +347,8 @@ sg_err sg_gpu_run_rmsnorm_gated_chunk(sg_gpu *g, void *y, void *z, void *out, vo
  *
  * sg_gpu_run_kv8_store: rows [base, base + n) from k and v (row stride p[5]
  *   floats, 0 = n_kv hd; [n_kv][hd] in a row). Per block, head and half the
- *   scale is s = max|x| / 127 (an f32 division) and a code is x / s rounded to
- *   the nearest integer, ties to even. In a block that goes on (base inside
+ *   scale is s = max|x| * (1/127), an f32 product with the f32 nearest to 1/127,
+ *   and a code is x / s rounded to the nearest integer, ties to even. In a block that goes on (base inside
  *   it) s is not below the scale it has, and if s grows the codes of its rows
  *   before base are rounded again to the nearest of code * s_old / s; a block
  *   that starts at base or after it is new, whatever its scale held. A value

@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(TPB) k_kv8_store(kv8_store_args a, int al) {
     mx = max(max(red[0], red[1]), max(red[2], red[3]));
     // 65520 and above round to infinity in f16; NaN's bits are above those
     const bool poison = mx >= 0x477FF000u || was != was;
-    float s = fmaxf(__uint_as_float(poison ? 0 : mx) / 127.0f, poison ? 0.0f : was);
+    float s = fmaxf(__uint_as_float(poison ? 0 : mx) * (1.0f / 127.0f), poison ? 0.0f : was);
     const bool grew = kept && s > was && !poison;
     if (t == 0) *sp = poison ? NAN : s;
     // a scale near the end of the range: x / s is the same for both times 2^64

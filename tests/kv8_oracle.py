@@ -59,7 +59,7 @@ class Cache:
                         self.scales[b, h, half] = np.nan
                         new = np.zeros(rows.shape, np.int64)
                     else:
-                        s = max(np.float32(np.float64(mx) / 127), was)
+                        s = max(np.float32(mx) * (np.float32(1) / np.float32(127)), was)
                         self.scales[b, h, half] = s
                         new = nearest(rows, s)
                         if kept and s > was:
