@@ -1082,7 +1082,7 @@ sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void
     int was;
     if (sg_failed(e = on_device(g, &was))) return e;
     void *part;
-    if (!sg_failed(e = scratch(g, sgk_logits_part_bytes(rows), &part)) && !sg_failed(e = push(bufs, 4))) {
+    if (!sg_failed(e = scratch(g, sgk_logits_part_bytes(vocab, rows), &part)) && !sg_failed(e = push(bufs, 4))) {
         const sgk_logits_args a = {DEV(logits), DEV(counts), DEV(bias), DEV(mask), DEV(out), DEV(token), vocab, rows, rep, freq, pres};
         e = finish(g, sgk_logits(&a, part, g->stream), outs, 2);
     }

@@ -422,8 +422,8 @@ typedef struct {
     uint32_t vocab, rows;
     float rep, freq, pres;
 } sgk_logits_args;
-/* part: scratch of sgk_logits_part_bytes(rows). */
-uint64_t sgk_logits_part_bytes(uint32_t rows);
+/* part: scratch of sgk_logits_part_bytes(vocab, rows). */
+uint64_t sgk_logits_part_bytes(uint32_t vocab, uint32_t rows);
 hipError_t sgk_logits(const sgk_logits_args *a, void *part, hipStream_t s);
 
 /* The device-resident workspace of the no-allocation entry points: a

@@ -6,100 +6,197 @@
 #include "kernels.h"
 
 // ---------------------------------------------------------------------------
-// Rotary positions with three axes. A workgroup takes RA_TOK tokens: first
-// their cos and sin per pair, one thread each (the angle and its functions in
-// double: a far position times a frequency loses the angle in 32 bits), then
-// every head's slice, four dims and their four partners per thread (or the
-// dims behind rope_dim, copied). Each element is read and written by one
-// thread, both halves of a pair by the same one, so out may be x.
+// Rotary positions with three axes. A workgroup takes a token and some of its
+// heads: cos and sin of the token's pairs once, one thread each (the angle and
+// its functions in double: a far position times a frequency loses the angle in
+// 32 bits), then a slice (token, head) per 2^wl lanes. The first slice's loads
+// go out before the angles, whose chain is as long as a trip to memory.
+// Bound by memory for many tokens, by that chain for one.
 // ---------------------------------------------------------------------------
-#define RA_TOK 4u
 struct rope_tab { double inv[SGK_ROPE_HALF]; uint8_t axis[SGK_ROPE_HALF]; };
 
-// one slice unit: V dims at d and, below rope_dim, their partners at d + half
-template <int V>
-__device__ __forceinline__ void rope_unit(const float *x, float *o, uint32_t d, uint32_t half, uint32_t rope_dim, bool copy,
-                                          const float *cs) {
-    if (d < half) {
-        float a[V], b[V];
-#pragma unroll
-        for (int e = 0; e < V; e++) { a[e] = x[d + e]; b[e] = x[d + half + e]; }
-#pragma unroll
-        for (int e = 0; e < V; e++) {
-            const float c = cs[d + e], s = cs[half + d + e];
-            o[d + e] = a[e] * c - b[e] * s;
-            o[d + half + e] = b[e] * c + a[e] * s;
+__device__ __forceinline__ void rope_angles(const sgk_rope_axes_args &a, const rope_tab &tab, uint64_t z, float *cs) {
+    const uint32_t half = a.rope_dim / 2, t = threadIdx.x;
+    __syncthreads();
+    if (t < half) {
+        double s, c;
+        sincos((double)a.pos[(uint64_t)tab.axis[t] * a.n + z] * tab.inv[t], &s, &c);
+        cs[t] = (float)c;
+        cs[half + t] = (float)s;
+    }
+    __syncthreads();
+}
+
+// Four dims per lane, the whole slice in one 16-byte load and store of a lane
+// group, the partners' dims in a second load (from cache). A group reads all of
+// a slice before it writes, so out may be x. hper: heads per workgroup.
+__global__ void __launch_bounds__(TPB) k_rope_axes4(sgk_rope_axes_args a, rope_tab tab, uint32_t hper, uint32_t wl) {
+    __shared__ __align__(16) float cs[2 * SGK_ROPE_HALF];
+    const uint32_t half = a.rope_dim / 2, t = threadIdx.x, d = (t & ((1u << wl) - 1)) * 4, hstep = TPB >> wl;
+    const uint32_t h0 = blockIdx.y * hper, h1 = min(h0 + hper, a.heads);
+    const bool on = d < a.head_dim, first = d < half, turn = d < a.rope_dim;
+    const uint32_t w = first ? d : d - half;
+    for (uint64_t z = blockIdx.x; z < a.n; z += gridDim.x) {
+        uint32_t h = h0 + (t >> wl);
+        f32x4 v, o;
+        uint64_t at;
+        auto fetch = [&]() {
+            at = z * a.row + (uint64_t)h * a.stride + d;
+            if (h < h1 && on) {
+                v = *(const f32x4 *)(a.x + at);
+                if (turn) o = *(const f32x4 *)(first ? a.x + at + half : a.x + at - half);
+            }
+        };
+        fetch();
+        rope_angles(a, tab, z, cs);
+        f32x4 c, s;
+        if (turn) {
+            c = *(const f32x4 *)&cs[w];
+            s = *(const f32x4 *)&cs[half + w];
+            if (first) s = -s;
         }
-    } else if (copy) {
-        const uint32_t t = d - half + rope_dim;     // units past the pairs: the dims behind rope_dim
-#pragma unroll
-        for (int e = 0; e < V; e++) o[t + e] = x[t + e];
+        while (h < h1) {
+            if (on) *(f32x4 *)(a.out + at) = turn ? v * c + o * s : v;
+            h += hstep;
+            fetch();
+        }
     }
 }
 
-template <int V>
-__global__ void __launch_bounds__(TPB) k_rope_axes(sgk_rope_axes_args a, rope_tab tab) {
-    __shared__ float cs[RA_TOK][2 * SGK_ROPE_HALF];
-    const uint32_t half = a.rope_dim / 2, t = threadIdx.x;
-    // a slice's units: half / V of pairs, then (head_dim - rope_dim) / V copies
-    const uint32_t upr = (a.head_dim - half) / V;
-    const bool copy = a.x != a.out;
-    for (uint64_t z0 = (uint64_t)blockIdx.x * RA_TOK; z0 < a.n; z0 += (uint64_t)gridDim.x * RA_TOK) {
-        const uint32_t nt = min((uint64_t)RA_TOK, a.n - z0);
-        __syncthreads();
-        for (uint32_t i = t; i < nt * half; i += TPB) {
-            const uint32_t z = i / half, f = i % half;
-            double s, c;
-            sincos((double)a.pos[(uint64_t)tab.axis[f] * a.n + z0 + z] * tab.inv[f], &s, &c);
-            cs[z][f] = (float)c;
-            cs[z][half + f] = (float)s;
-        }
-        __syncthreads();
-        const uint32_t per = a.heads * upr;
-        for (uint32_t i = t; i < nt * per; i += TPB) {
-            const uint32_t z = i / per, h = (i % per) / upr, u = i % upr;
-            const uint64_t at = (z0 + z) * a.row + (uint64_t)h * a.stride;
-            rope_unit<V>(a.x + at, a.out + at, u * V, half, a.rope_dim, copy, cs[z]);
-        }
+// Any size and alignment: a lane takes a pair, or a dim behind rope_dim.
+__global__ void __launch_bounds__(TPB) k_rope_axes1(sgk_rope_axes_args a, rope_tab tab, uint32_t hper, uint32_t wl) {
+    __shared__ float cs[2 * SGK_ROPE_HALF];
+    const uint32_t half = a.rope_dim / 2, t = threadIdx.x, units = a.head_dim - half;
+    const uint32_t h0 = blockIdx.y * hper, h1 = min(h0 + hper, a.heads);
+    for (uint64_t z = blockIdx.x; z < a.n; z += gridDim.x) {
+        rope_angles(a, tab, z, cs);
+        for (uint32_t h = h0 + (t >> wl); h < h1; h += TPB >> wl)
+            for (uint32_t u = t & ((1u << wl) - 1); u < units; u += 1u << wl) {
+                const uint64_t at = z * a.row + (uint64_t)h * a.stride + u;
+                if (u < half) {
+                    const float lo = a.x[at], hi = a.x[at + half], c = cs[u], s = cs[half + u];
+                    a.out[at] = lo * c - hi * s;
+                    a.out[at + half] = hi * c + lo * s;
+                } else {
+                    a.out[at + half] = a.x[at + half];
+                }
+            }
     }
 }
 
 extern "C" hipError_t sgk_rope_axes(const sgk_rope_axes_args *a, const double *inv, const uint8_t *axis, hipStream_t s) {
     const uint32_t half = a->rope_dim / 2;
     if (!a->n || !a->heads) return hipSuccess;
-    if (!half || half > SGK_ROPE_HALF || a->rope_dim > a->head_dim) return hipErrorInvalidValue;
+    if (!half || half > SGK_ROPE_HALF || a->rope_dim > a->head_dim || a->head_dim > 256) return hipErrorInvalidValue;
     rope_tab tab = {};
     for (uint32_t i = 0; i < half; i++) { tab.inv[i] = inv[i]; tab.axis[i] = axis[i]; }
-    const uint64_t blocks = ((uint64_t)a->n + RA_TOK - 1) / RA_TOK;
-    const uint32_t grid = (uint32_t)(blocks < 65536 ? blocks : 65536);
-    hipLaunchKernelGGL(k_rope_axes<1>, dim3(grid), dim3(TPB), 0, s, *a, tab);
+    const bool v4 = !(((uintptr_t)a->x | (uintptr_t)a->out) & 15) && a->row % 4 == 0 && a->stride % 4 == 0 && half % 4 == 0 &&
+                    a->head_dim % 4 == 0;
+    const uint32_t units = v4 ? a->head_dim / 4 : a->head_dim - half;
+    uint32_t wl = 0;
+    while (wl < 6 && (1u << wl) < units) wl++;
+    // few tokens: their heads spread until every CU has a workgroup, a slice to a lane group
+    const uint32_t per = TPB >> wl, want = (uint32_t)(((uint64_t)sgk_device_cus() + a->n - 1) / a->n);
+    const uint32_t hs = min(want, (a->heads + per - 1) / per), hper = (a->heads + hs - 1) / hs;
+    const dim3 grid(min(a->n, 1u << 20), (a->heads + hper - 1) / hper);
+    if (v4) hipLaunchKernelGGL(k_rope_axes4, grid, dim3(TPB), 0, s, *a, tab, hper, wl);
+    else hipLaunchKernelGGL(k_rope_axes1, grid, dim3(TPB), 0, s, *a, tab, hper, wl);
     return hipGetLastError();
 }
 
 // ---------------------------------------------------------------------------
-// Token counts: integer atomics, so the order of equal ids does not matter.
+// Token counts. Text repeats itself: added one by one, the commonest id's
+// additions to one address wait for each other across the chip (about 30 ns
+// each; 16 rows of 32000 ids with a fifth of them alike took 182 us). So a
+// workgroup first counts TC_IDS ids in a table in LDS, open addressing, then
+// adds each distinct id once. Integer additions: their order does not matter.
 // ---------------------------------------------------------------------------
+#define TC_IDS 2048u
+#define TC_SLOTS 4096u      // twice the ids, so a free slot is always found
+#define TC_FREE 0xFFFFFFFFu
 __global__ void __launch_bounds__(TPB) k_zero_u32(uint32_t *p, uint64_t n) {
     for (uint64_t i = (uint64_t)blockIdx.x * TPB + threadIdx.x; i < n; i += (uint64_t)gridDim.x * TPB) p[i] = 0;
 }
 __global__ void __launch_bounds__(TPB) k_token_counts(const int32_t *ids, uint32_t *counts, uint32_t n, uint32_t vocab,
                                                       uint32_t rows) {
+    __shared__ uint32_t key[TC_SLOTS], num[TC_SLOTS];
+    const uint32_t t = threadIdx.x;
     for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y)
-        for (uint64_t i = (uint64_t)blockIdx.x * TPB + threadIdx.x; i < n; i += (uint64_t)gridDim.x * TPB) {
-            const uint32_t id = (uint32_t)ids[(uint64_t)r * n + i];
-            if (id < vocab) atomicAdd(counts + (uint64_t)r * vocab + id, 1u);
+        for (uint64_t i0 = (uint64_t)blockIdx.x * TC_IDS; i0 < n; i0 += (uint64_t)gridDim.x * TC_IDS) {
+            const uint32_t m = (uint32_t)min((uint64_t)TC_IDS, n - i0);
+            uint32_t id[TC_IDS / TPB];
+#pragma unroll
+            for (uint32_t x = 0; x < TC_IDS / TPB; x++) {
+                const uint32_t i = t + x * TPB;
+                id[x] = i < m ? (uint32_t)ids[(uint64_t)r * n + i0 + i] : TC_FREE;
+            }
+            for (uint32_t i = t; i < TC_SLOTS; i += TPB) { key[i] = TC_FREE; num[i] = 0; }
+            __syncthreads();
+#pragma unroll
+            for (uint32_t x = 0; x < TC_IDS / TPB; x++) {
+                if (id[x] >= vocab) continue;
+                for (uint32_t s = id[x] * 2654435761u >> 20;; s = (s + 1) & (TC_SLOTS - 1)) {
+                    const uint32_t was = atomicCAS(&key[s], TC_FREE, id[x]);
+                    if (was != TC_FREE && was != id[x]) continue;
+                    atomicAdd(&num[s], 1u);
+                    break;
+                }
+            }
+            __syncthreads();
+            for (uint32_t i = t; i < TC_SLOTS; i += TPB)
+                if (key[i] != TC_FREE) atomicAdd(counts + (uint64_t)r * vocab + key[i], num[i]);
+            __syncthreads();
         }
+}
+
+// Counts from nothing: a workgroup owns TR_IDS ids of a row, reads the row's
+// whole history and counts its own in LDS, so there is nothing to clear first
+// and no addition to memory.
+#define TR_IDS 8192u
+// A row's history up to which this form runs (whole call, 151936 ids, Zipf's
+// law with exponent 1.2 / one id only): 900 ids of 1 row 15.3 / 15.1 us, the
+// table form 18.5 / 18.6; 32000 of 1 row 22.9 / 41.5, table 22.2 / 20.5; 32000
+// of 16 rows 24.7 / 49.1, table 30.0 / 21.5. Past it the longest part's walk
+// over the history decides, and the table form spreads that.
+#define TR_MOST 32768u
+__global__ void __launch_bounds__(TPB) k_token_recount(const int32_t *ids, uint32_t *counts, uint32_t n, uint32_t vocab, uint32_t rows) {
+    __shared__ uint32_t num[TR_IDS];
+    const uint32_t t = threadIdx.x, v0 = blockIdx.x * TR_IDS, nv = min(TR_IDS, vocab - v0);
+    for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
+        for (uint32_t i = t; i < nv; i += TPB) num[i] = 0;
+        __syncthreads();
+        const int32_t *row = ids + (uint64_t)r * n;
+        constexpr uint32_t U = 8;
+        for (uint32_t i0 = 0; i0 < n; i0 += U * TPB) {
+            uint32_t id[U];
+#pragma unroll
+            for (uint32_t x = 0; x < U; x++) {
+                const uint32_t i = i0 + x * TPB + t;
+                id[x] = i < n ? (uint32_t)row[i] : 0xFFFFFFFFu;
+            }
+#pragma unroll
+            for (uint32_t x = 0; x < U; x++)
+                if (id[x] - v0 < nv) atomicAdd(&num[id[x] - v0], 1u);
+        }
+        __syncthreads();
+        for (uint32_t i = t; i < nv; i += TPB) counts[(uint64_t)r * vocab + v0 + i] = num[i];
+        __syncthreads();
+    }
 }
 
 extern "C" hipError_t sgk_token_counts(const int32_t *ids, uint32_t *counts, uint32_t n, uint32_t vocab, uint32_t rows,
                                        int clear, hipStream_t s) {
     if (!vocab || !rows) return hipSuccess;
+    if (clear && n && n <= TR_MOST) {
+        hipLaunchKernelGGL(k_token_recount, dim3((vocab + TR_IDS - 1) / TR_IDS, rows), dim3(TPB), 0, s, ids, counts, n, vocab, rows);
+        return hipGetLastError();
+    }
     if (clear) {
         const uint64_t b = ((uint64_t)rows * vocab + TPB - 1) / TPB;
         hipLaunchKernelGGL(k_zero_u32, dim3((uint32_t)(b < 2048 ? b : 2048)), dim3(TPB), 0, s, counts, (uint64_t)rows * vocab);
     }
     if (n) {
-        const uint64_t b = ((uint64_t)n + TPB - 1) / TPB;
+        const uint64_t b = ((uint64_t)n + TC_IDS - 1) / TC_IDS;
         hipLaunchKernelGGL(k_token_counts, dim3((uint32_t)(b < 1024 ? b : 1024), rows < 65535 ? rows : 65535), dim3(TPB), 0, s,
                            ids, counts, n, vocab, rows);
     }
@@ -111,23 +208,28 @@ extern "C" hipError_t sgk_token_counts(const int32_t *ids, uint32_t *counts, uin
 // best (value, id); a second launch folds the parts. The best is the largest
 // value, ties to the lowest id, so no order of the folds changes it. NaN is
 // never better, and -inf neither: a row with nothing allowed has no token.
+// A thread takes four neighbouring ids a step, 16 bytes of each input where
+// addresses allow. Bound by memory for many rows, by the launches for one.
 // ---------------------------------------------------------------------------
-#define LG_PARTS 64u
+#define LG_PARTS 256u       // parts of all rows together that fill the chip; a row has at least one
 struct lg_best { float v; uint32_t i; };
 #define LG_NONE 0xFFFFFFFFu
 
 __device__ __forceinline__ void lg_better(lg_best &b, float v, uint32_t i) {
     if (v > b.v || (v == b.v && i < b.i && b.i != LG_NONE)) { b.v = v; b.i = i; }
 }
-__device__ __forceinline__ lg_best lg_fold(lg_best b, lg_best *red) {
-    const uint32_t t = threadIdx.x;
-    red[t] = b;
+// the best of the workgroup, in thread 0
+__device__ __forceinline__ lg_best lg_fold(lg_best b) {
+    __shared__ lg_best red[TPB / 64];
+#define LG_STEP(F) lg_better(b, __uint_as_float(F(__float_as_uint(b.v))), F(b.i))
+    // a partner's NONE is never better: its value is -inf
+    LG_STEP(dppu<0xB1>); LG_STEP(dppu<0x4E>); LG_STEP(dppu<0x141>); LG_STEP(dppu<0x128>); LG_STEP(swap16); LG_STEP(swap32);
+#undef LG_STEP
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = b;
     __syncthreads();
-    for (uint32_t o = TPB / 2; o; o >>= 1) {
-        if (t < o) { lg_best x = red[t]; lg_better(x, red[t + o].v, red[t + o].i); red[t] = x; }
-        __syncthreads();
-    }
-    return red[0];
+#pragma unroll
+    for (int w = 0; w < TPB / 64; w++) lg_better(b, red[w].v, red[w].i);
+    return b;
 }
 __device__ __forceinline__ float lg_value(const sgk_logits_args &a, float x, uint32_t c, float bias, bool ok) {
     if (c) {
@@ -137,33 +239,69 @@ __device__ __forceinline__ float lg_value(const sgk_logits_args &a, float x, uin
     return ok ? x + bias : -INFINITY;
 }
 
+template <bool V4>
 __global__ void __launch_bounds__(TPB) k_logits(sgk_logits_args a, lg_best *part) {
-    __shared__ lg_best red[TPB];
-    const uint64_t r = blockIdx.y, row = r * a.vocab, words = (a.vocab + 31) / 32;
+    const uint64_t r = blockIdx.y, row = r * a.vocab;
+    const uint32_t words = (a.vocab + 31) / 32, quads = (a.vocab + 3) / 4;
     lg_best b = {-INFINITY, LG_NONE};
-    for (uint64_t i = (uint64_t)blockIdx.x * TPB + threadIdx.x; i < a.vocab; i += (uint64_t)gridDim.x * TPB) {
-        const uint32_t c = a.counts ? a.counts[row + i] : 0;
-        const bool ok = !a.mask || (a.mask[r * words + i / 32] >> (i % 32) & 1);
-        const float x = lg_value(a, a.x[row + i], c, a.bias ? a.bias[i] : 0.0f, ok);
-        a.out[row + i] = x;
-        lg_better(b, x, (uint32_t)i);
+    for (uint32_t q = blockIdx.x * TPB + threadIdx.x; q < quads; q += gridDim.x * TPB) {
+        const uint32_t i = 4 * q, n = V4 ? 4 : min(4u, a.vocab - i);
+        float x[4] = {0, 0, 0, 0}, bias[4] = {0, 0, 0, 0};
+        uint32_t c[4] = {0, 0, 0, 0};
+        const uint32_t bits = a.mask ? a.mask[r * words + i / 32] >> (i % 32) : 0xF;   // four ids share a word
+        if (V4) {
+            const f32x4 v = *(const f32x4 *)(a.x + row + i);
+            const v4u cv = a.counts ? *(const v4u *)(a.counts + row + i) : (v4u){0, 0, 0, 0};
+            const f32x4 bv = a.bias ? *(const f32x4 *)(a.bias + i) : (f32x4){0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; e++) { x[e] = v[e]; c[e] = cv[e]; bias[e] = bv[e]; }
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                if (e >= n) break;
+                x[e] = a.x[row + i + e];
+                if (a.counts) c[e] = a.counts[row + i + e];
+                if (a.bias) bias[e] = a.bias[i + e];
+            }
+        }
+        f32x4 o;
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) {
+            o[e] = lg_value(a, x[e], c[e], bias[e], bits >> e & 1);
+            if (e < n) lg_better(b, o[e], i + e);
+        }
+        if (V4) *(f32x4 *)(a.out + row + i) = o;
+        else
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++)
+                if (e < n) a.out[row + i + e] = o[e];
     }
-    b = lg_fold(b, red);
-    if (threadIdx.x == 0) part[r * gridDim.x + blockIdx.x] = b;
+    b = lg_fold(b);
+    if (threadIdx.x == 0) {
+        if (gridDim.x == 1) a.token[r] = b.i;
+        else part[r * gridDim.x + blockIdx.x] = b;
+    }
 }
 __global__ void __launch_bounds__(TPB) k_logits_token(const lg_best *part, uint32_t parts, uint32_t *token) {
-    __shared__ lg_best red[TPB];
     lg_best b = {-INFINITY, LG_NONE};
     if (threadIdx.x < parts) b = part[(uint64_t)blockIdx.x * parts + threadIdx.x];
-    b = lg_fold(b, red);
+    b = lg_fold(b);
     if (threadIdx.x == 0) token[blockIdx.x] = b.i;
 }
 
-extern "C" uint64_t sgk_logits_part_bytes(uint32_t rows) { return (uint64_t)rows * LG_PARTS * sizeof(lg_best); }
+// parts of a row: one per 4 TPB ids, until the rows together fill the chip a few times
+static uint32_t lg_parts(uint32_t vocab, uint32_t rows) {
+    const uint32_t need = (uint32_t)(((uint64_t)vocab + 4 * TPB - 1) / (4 * TPB)), most = max(1u, 4 * LG_PARTS / rows);
+    return min(min(need, most), (uint32_t)TPB);
+}
+extern "C" uint64_t sgk_logits_part_bytes(uint32_t vocab, uint32_t rows) { return (uint64_t)rows * lg_parts(vocab, rows) * sizeof(lg_best); }
 extern "C" hipError_t sgk_logits(const sgk_logits_args *a, void *part, hipStream_t s) {
     if (!a->vocab || !a->rows) return hipSuccess;
-    const uint32_t need = (uint32_t)(((uint64_t)a->vocab + TPB - 1) / TPB), parts = need < LG_PARTS ? need : LG_PARTS;
-    hipLaunchKernelGGL(k_logits, dim3(parts, a->rows), dim3(TPB), 0, s, *a, (lg_best *)part);
-    hipLaunchKernelGGL(k_logits_token, dim3(a->rows), dim3(TPB), 0, s, (const lg_best *)part, parts, a->token);
+    const uint32_t parts = lg_parts(a->vocab, a->rows);
+    const bool v4 = !(((uintptr_t)a->x | (uintptr_t)a->out | (uintptr_t)a->counts | (uintptr_t)a->bias) & 15) && a->vocab % 4 == 0;
+    const dim3 grid(parts, a->rows);
+    if (v4) hipLaunchKernelGGL(k_logits<true>, grid, dim3(TPB), 0, s, *a, (lg_best *)part);
+    else hipLaunchKernelGGL(k_logits<false>, grid, dim3(TPB), 0, s, *a, (lg_best *)part);
+    if (parts > 1) hipLaunchKernelGGL(k_logits_token, dim3(a->rows), dim3(TPB), 0, s, (const lg_best *)part, parts, a->token);
     return hipGetLastError();
 }
