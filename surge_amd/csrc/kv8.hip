@@ -296,6 +296,57 @@ __device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
     return r;
 }
 
+// One tile group's scores (UN tiles of 16 keys) to weights, online: updates the
+// running maximum and sum of the row, gives the weights' f16 halves in operand
+// order and what the output so far is to be multiplied by. MASK: key 16 u +
+// 4 lg + e is visible up to rel (keys before the group's first make it
+// negative); without it all are.
+template <int UN, bool MASK>
+__device__ __forceinline__ float softmax_step(float (&sc)[UN][4], const float (&vs)[UN], int rel, float &mrun, float &lsum,
+                                              f16x8 (&ph)[UN / 2], f16x8 (&pl)[UN / 2]) {
+    const int lg4 = (threadIdx.x & 63) >> 4 << 2;
+    float tm = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < UN; u++) {
+        if (MASK) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (16 * u + lg4 + e > rel) sc[u][e] = -INFINITY;
+        }
+        const float m4 = fmaxf(fmaxf(sc[u][0], sc[u][1]), fmaxf(sc[u][2], sc[u][3]));
+        tm = fmaxf(tm, m4 + __builtin_amdgcn_logf(fmaxf(vs[u], 0x1p-80f)));
+    }
+    tm = fmaxf(tm, swap16f(tm));
+    tm = fmaxf(tm, swap32f(tm));
+    const float mnew = fmaxf(mrun, tm), m0 = mnew - KV8_P2;
+    const float al = mrun == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrun - mnew);
+    mrun = mnew;
+    float l = lsum * al;
+#pragma unroll
+    for (int u = 0; u < UN; u++) {
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            // masked keys apart: a row with no key yet has m0 = -inf, and a block's scale may be NaN
+            const bool vis = !MASK || 16 * u + lg4 + e <= rel;
+            const float p = vis ? __builtin_amdgcn_exp2f(sc[u][e] - m0) : 0.0f;
+            l += p;
+            w[e] = vis ? p * vs[u] : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+            const f16x2 h = __builtin_convertvector((f32x2){w[e], w[e + 1]}, f16x2);
+            const int at = 4 * (u & 1) + e;
+            ph[u / 2][at] = h[0];
+            ph[u / 2][at + 1] = h[1];
+            pl[u / 2][at] = (_Float16)fmaf((float)h[0], -1.0f, w[e]);
+            pl[u / 2][at + 1] = (_Float16)fmaf((float)h[1], -1.0f, w[e + 1]);
+        }
+    }
+    lsum = l;
+    return al;
+}
+
 template <int HD>
 __global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part part, int al) {
     constexpr int NC = HD / 64, NT = HD / 16, OLD = HD + 4;
@@ -354,8 +405,7 @@ __global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part pa
     for (int n = 0; n < NT; n++) o[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     float mrun = -INFINITY, lsum = 0.0f;
     for (; step < s1; step += 4) {
-        float sc[2][4], tm = -INFINITY;
-        const bool whole = step * 32 + 31 <= a.base;            // every row sees every key
+        float sc[2][4];
 #pragma unroll
         for (int u = 0; u < 2; u++) { ks[u] = nks[u]; vs[u] = nvs[u]; }
 #pragma unroll
@@ -366,34 +416,16 @@ __global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part pa
 #pragma unroll
                 for (int d = 0; d < 3; d++)
                     s[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, kr[u][c]), qd[d][c], s[d], 0, 0, 0);
-            const float f = qf * ks[u], lv = __builtin_amdgcn_logf(fmaxf(vs[u], 0x1p-80f));
+            const float f = qf * ks[u];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                sc[u][e] = q_join(s[0][e], s[1][e], s[2][e]) * f;
-                if (whole || step * 32 + u * 16 + 4 * lg + e <= rpos) tm = fmaxf(tm, sc[u][e] + lv);
-            }
+            for (int e = 0; e < 4; e++) sc[u][e] = q_join(s[0][e], s[1][e], s[2][e]) * f;
         }
         const bool more = step + 4 < s1;
         if (more) { load_s(step + 4); load_k(step + 4); }
-        tm = fmaxf(tm, swap16f(tm));
-        tm = fmaxf(tm, swap32f(tm));
-        const float mnew = fmaxf(mrun, tm), m0 = mnew - KV8_P2;
-        const float al2 = mrun == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrun - mnew);
-        mrun = mnew;
-        lsum *= al2;
-        f16x8 ph, pl;
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const bool on = whole || step * 32 + u * 16 + 4 * lg + e <= rpos;
-                const float p = on ? __builtin_amdgcn_exp2f(sc[u][e] - m0) : 0.0f;
-                lsum += p;
-                const float w = on ? p * vs[u] : 0.0f;
-                const _Float16 h = (_Float16)w;
-                ph[4 * u + e] = h;
-                pl[4 * u + e] = (_Float16)(w - (float)h);
-            }
+        f16x8 ph[1], pl[1];
+        const float al2 = step * 32 + 31 <= a.base      // every row sees every key
+                              ? softmax_step<2, false>(sc, vs, 0, mrun, lsum, ph, pl)
+                              : softmax_step<2, true>(sc, vs, (int)(rpos - step * 32), mrun, lsum, ph, pl);
         if (__builtin_amdgcn_ballot_w64(al2 != 1.0f)) {
 #pragma unroll
             for (int n = 0; n < NT; n++) o[n] *= al2;
@@ -403,8 +435,8 @@ __global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part pa
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const f16x8 v = codes_f16(vr[0][c][j], vr[1][c][j]);
-                o[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, o[4 * c + j], 0, 0, 0);
-                o[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, o[4 * c + j], 0, 0, 0);
+                o[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[0], o[4 * c + j], 0, 0, 0);
+                o[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[0], o[4 * c + j], 0, 0, 0);
             }
         if (more) load_v(step + 4);
     }
@@ -572,32 +604,8 @@ __global__ void __launch_bounds__(NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_part p
             f16x8 ph[CT][2], pl[CT][2];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
-                float tm = -INFINITY;
-#pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    const float lv = __builtin_amdgcn_logf(fmaxf(vs[u], 0x1p-80f));
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (whole || kt * 64 + u * 16 + 4 * lg + e <= rpos[ct]) tm = fmaxf(tm, sc[ct][u][e] + lv);
-                }
-                tm = fmaxf(tm, swap16f(tm));
-                tm = fmaxf(tm, swap32f(tm));
-                const float mnew = fmaxf(mrun[ct], tm), m0 = mnew - KV8_P2;
-                const float al2 = mrun[ct] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrun[ct] - mnew);
-                mrun[ct] = mnew;
-                lsum[ct] *= al2;
-#pragma unroll
-                for (int u = 0; u < 4; u++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const bool vis = whole || kt * 64 + u * 16 + 4 * lg + e <= rpos[ct];
-                        const float p = vis ? __builtin_amdgcn_exp2f(sc[ct][u][e] - m0) : 0.0f;
-                        lsum[ct] += p;
-                        const float w = vis ? p * vs[u] : 0.0f;
-                        const _Float16 h = (_Float16)w;
-                        ph[ct][u >> 1][4 * (u & 1) + e] = h;
-                        pl[ct][u >> 1][4 * (u & 1) + e] = (_Float16)(w - (float)h);
-                    }
+                const float al2 = whole ? softmax_step<4, false>(sc[ct], vs, 0, mrun[ct], lsum[ct], ph[ct], pl[ct])
+                                        : softmax_step<4, true>(sc[ct], vs, (int)(rpos[ct] - kt * 64), mrun[ct], lsum[ct], ph[ct], pl[ct]);
                 if (__builtin_amdgcn_ballot_w64(al2 != 1.0f)) {
 #pragma unroll
                     for (int n = 0; n < NT; n++) o[ct][n] *= al2;
@@ -640,29 +648,37 @@ __global__ void __launch_bounds__(NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_part p
 }
 
 // How a call runs. Few rows: the key-split form, in as many splits as give
-// every wave a step, up to two workgroups per CU (what is resident). More:
-// row blocks, their keys split until the chip is full.
-#ifndef KV8_NW
+// every wave a step, up to two workgroups per CU (what is resident). More: row
+// blocks, one workgroup per CU at a time, their keys split where that shortens
+// the launch: rounds x (a part's tiles + KV8_TAIL for its start and end) tiles
+// of KV8_TILE_US, against the partials' way to memory and back.
 #define KV8_NW 8
 #define KV8_CT 1
-#endif
 #define KV8_ROWS (KV8_NW * KV8_CT * 16u)
+#define KV8_TILE_US 2.5         /* at head_dim 256 */
+#define KV8_TAIL 3.0
+#define KV8_PART_BYTES (256ull << 20)
 struct kv8_plan { bool wave; uint32_t splits, blocks; };
 static kv8_plan kv8_plan_of(const sgk_kv8_attn *a) {
-    const uint64_t rows = (uint64_t)a->ntok * (a->n_heads / a->n_kv);
+    const uint64_t G = a->n_heads / a->n_kv, rows = a->ntok * G, keys = (uint64_t)a->base + a->ntok, cus = sgk_device_cus();
     kv8_plan p = {rows <= 16, 1, (uint32_t)((rows + KV8_ROWS - 1) / KV8_ROWS)};
-    const uint64_t keys = (uint64_t)a->base + a->ntok, cus = sgk_device_cus();
-    uint64_t most, want;
     if (p.wave) {
-        most = 2 * cus / a->n_kv;
-        want = (keys + 127) / 128;
-    } else {
-        most = (cus + (uint64_t)p.blocks * a->n_kv - 1) / ((uint64_t)p.blocks * a->n_kv);
-        want = (keys + 127) / 128;
+        uint64_t most = 2 * cus / a->n_kv, want = (keys + 127) / 128;
+        if (most > 1024) most = 1024;
+        if (most < 1) most = 1;
+        p.splits = (uint32_t)(want < most ? want : most);
+        return p;
     }
+    const uint64_t wgs = (uint64_t)p.blocks * a->n_kv, tiles = (keys + 63) / 64, prow = (uint64_t)a->ntok * a->n_heads * a->hd * 4;
+    uint64_t most = wgs < cus ? 2 * cus / wgs : 8;
     if (most > 1024) most = 1024;
-    if (most < 1) most = 1;
-    p.splits = (uint32_t)(want < most ? want : most);
+    if (most > tiles) most = tiles;
+    double best = 0.0;
+    for (uint64_t S = 1; S <= most && (S == 1 || S * prow <= KV8_PART_BYTES); S++) {
+        const double rounds = (double)((wgs * S + cus - 1) / cus), part = (double)((tiles + S - 1) / S) + KV8_TAIL;
+        const double cost = rounds * part * KV8_TILE_US * a->hd / 256 + (S > 1 ? 5.0 + (double)(2 * S * prow) / 4.0e6 : 0.0);
+        if (S == 1 || cost < best) { best = cost; p.splits = (uint32_t)S; }
+    }
     return p;
 }
 
