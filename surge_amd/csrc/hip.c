@@ -969,6 +969,7 @@ static sg_err attn_kv8_oneshot(sg_gpu *g, const char *who, void *q, void *codes,
     if (!nh || nh % nkv || nh / nkv > SGK_KV8_MAX_GROUP)
         return errf("gpu: %s: n_heads must be a multiple of n_kv_heads, at most %u times it", who, SGK_KV8_MAX_GROUP);
     if (qs < hd) return errf("gpu: %s: q_stride < head_dim", who);
+    if ((uint64_t)n * (nh / nkv) > 1u << 30) return errf("gpu: %s: more than 2^30 query rows per kv head", who);
     const uint64_t rows = (uint64_t)(n ? n : 1) * nh;
     if (sg_failed(e = need(q, ((rows - 1) * qs + hd) * 4, "q")) || sg_failed(e = need(out, rows * hd * 4, "out"))) return e;
     if (!aligned(q, 4) || !aligned(out, 4)) return errf("gpu: %s: q and out must be 4-byte aligned", who);

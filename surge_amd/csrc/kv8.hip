@@ -204,8 +204,9 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
 }
 
 // ---------------------------------------------------------------------------
-// Attention of few rows (tokens x the query heads of one kv head, at most 16),
-// split over the keys: decode, and chunks of a few tokens. Every wave streams
+// Attention of few rows: decode, and small chunks. A workgroup takes 16 rows
+// (token-major, the query heads of one kv head inside a token) and a part of
+// the keys. Every wave streams
 // its own steps of 32 keys straight from the cache into operands:
 //  - q in fixed point against its row's largest element, 24 bits as three int8
 //    digits (q = sq (65536 d2 + 256 d1 + d0)): the score product is three
@@ -226,24 +227,24 @@ struct kv8_part { float *m, *s, *acc; };    // [token][head][split] maxima and s
 
 #define KV8_P2 12.0f
 
-// 16 f32 of a row as the three digits' operand bytes
+// 16 f32 of a row as the three digits' operand bytes: with 0x808080 added, the
+// bytes of round(x inv) are its balanced digits plus 128, carries and all.
 __device__ __forceinline__ void q_digits(const float (&x)[16], float inv, v4i &d0, v4i &d1, v4i &d2) {
 #pragma unroll
     for (int w = 0; w < 4; w++) {
-        uint32_t b0 = 0, b1 = 0, b2 = 0;
+        uint32_t t[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int q = (int)rintf(x[4 * w + e] * inv);
-            const int l0 = (int8_t)q, r1 = (q - l0) >> 8, l1 = (int8_t)r1, l2 = (r1 - l1) >> 8;
-            b0 |= (uint32_t)(l0 & 0xFF) << (8 * e);
-            b1 |= (uint32_t)(l1 & 0xFF) << (8 * e);
-            b2 |= (uint32_t)(l2 & 0xFF) << (8 * e);
-        }
-        d0[w] = (int)b0; d1[w] = (int)b1; d2[w] = (int)b2;
+        for (int e = 0; e < 4; e++) t[e] = (uint32_t)((int)rintf(x[4 * w + e] * inv) + 0x808080);
+        // bytes 0 and 1 of two elements, then byte 2; perm picks 0-3 from its second argument, 4-7 from its first
+        const uint32_t a = __builtin_amdgcn_perm(t[1], t[0], 0x05010400u), b = __builtin_amdgcn_perm(t[3], t[2], 0x05010400u);
+        const uint32_t c = __builtin_amdgcn_perm(t[1], t[0], 0x0C0C0602u), d = __builtin_amdgcn_perm(t[3], t[2], 0x0C0C0602u);
+        d0[w] = (int)(__builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u);
+        d1[w] = (int)(__builtin_amdgcn_perm(b, a, 0x07060302u) ^ 0x80808080u);
+        d2[w] = (int)(__builtin_amdgcn_perm(d, c, 0x05040100u) ^ 0x80808080u);
     }
 }
 // A row's q (spread over the four lanes of its column) as digits; returns the
-// factor of the integer scores, sq * mul, NaN if an element is not finite.
+// factor of the integer scores, sq * |mul|, NaN if an element is not finite.
 template <int NC>
 __device__ __forceinline__ float q_row(const float *q, bool on, bool al, uint32_t lg, float mul, v4i (&d)[3][NC]) {
     float x[NC][16];
@@ -266,14 +267,14 @@ __device__ __forceinline__ float q_row(const float *q, bool on, bool al, uint32_
     float am = bad ? 0.0f : __uint_as_float(mx);
     const float up = am < 0x1p-60f ? 0x1p64f : 1.0f;    // a row near the end of the range, times 2^64
     am *= up;
-    const float inv = am > 0.0f ? 8323072.0f / am : 0.0f;       // 127 * 65536
+    const float inv = am > 0.0f ? copysignf(8323072.0f / am, mul) : 0.0f;       // 127 * 65536; a negative scale turns q
 #pragma unroll
     for (int c = 0; c < NC; c++) {
 #pragma unroll
         for (int e = 0; e < 16; e++) x[c][e] = bad ? 0.0f : x[c][e] * up;
         q_digits(x[c], inv, d[0][c], d[1][c], d[2][c]);
     }
-    return bad ? NAN : am / 8323072.0f * mul / up;
+    return bad ? NAN : am / 8323072.0f * fabsf(mul) / up;
 }
 // the score sums of the three digits as one float (a2 * 256 + a1 < 2^31)
 __device__ __forceinline__ float q_join(int a0, int a1, int a2) {
@@ -296,25 +297,49 @@ __device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
     return r;
 }
 
-// One tile group's scores (UN tiles of 16 keys) to weights, online: updates the
-// running maximum and sum of the row, gives the weights' f16 halves in operand
-// order and what the output so far is to be multiplied by. MASK: key 16 u +
-// 4 lg + e is visible up to rel (keys before the group's first make it
-// negative); without it all are.
-template <int UN, bool MASK>
-__device__ __forceinline__ float softmax_step(float (&sc)[UN][4], const float (&vs)[UN], int rel, float &mrun, float &lsum,
-                                              f16x8 (&ph)[UN / 2], f16x8 (&pl)[UN / 2]) {
+// Whether a group's least scales (the same in every lane) are those of the
+// usual case; NaN is not, where the minimum shows it.
+__device__ __forceinline__ bool scales_usual(float ks, float vs) {
+    return __builtin_amdgcn_readfirstlane(ks >= 0.0f && vs >= 0x1p-80f);
+}
+
+// w[0], w[1] as f16 and what is left of them, packed
+__device__ __forceinline__ void split2(float w0, float w1, f16x2 &hi, f16x2 &lo) {
+    hi = __builtin_convertvector((f32x2){w0, w1}, f16x2);
+    uint32_t l;
+    asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(l) : "v"(hi), "v"(w0));
+    asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(l) : "v"(hi), "v"(w1));
+    lo = __builtin_bit_cast(f16x2, l);
+}
+
+// One group of UN tiles' scores to weights, online: updates the row's running
+// maximum and sum, gives the weights' f16 halves in operand order and what the
+// output so far is to be multiplied by. x: the integer scores; f: what they are
+// to be multiplied by (scale, q's unit, the keys' scale); vs: the values'
+// scales; both per tile. Key 16 u + 4 lg + e is visible up to rel.
+// The usual group has all its keys visible, f >= 0 and vs >= 2^-80: then the
+// weight is one fma and one exp2, w = 2^(x f + log2 vs - m0), and the sum of p
+// is the sum of w / vs (an error of log2 vs is in both, and drops out). GEN
+// takes any: masked keys apart (a row with no key yet has m0 = -inf), a scale
+// of zero or NaN.
+template <int UN, bool GEN>
+__device__ __forceinline__ float softmax_step(float (&x)[UN][4], const float (&f)[UN], const float (&vs)[UN], int rel, float &mrun,
+                                              float &lsum, f16x8 (&ph)[UN / 2], f16x8 (&pl)[UN / 2]) {
     const int lg4 = (threadIdx.x & 63) >> 4 << 2;
-    float tm = -INFINITY;
+    float tm = -INFINITY, lv[UN];
 #pragma unroll
     for (int u = 0; u < UN; u++) {
-        if (MASK) {
+        if (GEN) {
+            lv[u] = __builtin_amdgcn_logf(fmaxf(fabsf(vs[u]), 0x1p-80f));
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (16 * u + lg4 + e > rel) sc[u][e] = -INFINITY;
+            for (int e = 0; e < 4; e++) {
+                x[u][e] = 16 * u + lg4 + e <= rel ? x[u][e] * f[u] : -INFINITY;
+                tm = fmaxf(tm, x[u][e] + lv[u]);
+            }
+        } else {
+            lv[u] = __builtin_amdgcn_logf(vs[u]);
+            tm = fmaxf(tm, fmaf(fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])), f[u], lv[u]));
         }
-        const float m4 = fmaxf(fmaxf(sc[u][0], sc[u][1]), fmaxf(sc[u][2], sc[u][3]));
-        tm = fmaxf(tm, m4 + __builtin_amdgcn_logf(fmaxf(vs[u], 0x1p-80f)));
     }
     tm = fmaxf(tm, swap16f(tm));
     tm = fmaxf(tm, swap32f(tm));
@@ -325,22 +350,29 @@ __device__ __forceinline__ float softmax_step(float (&sc)[UN][4], const float (&
 #pragma unroll
     for (int u = 0; u < UN; u++) {
         float w[4];
+        if (GEN) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            // masked keys apart: a row with no key yet has m0 = -inf, and a block's scale may be NaN
-            const bool vis = !MASK || 16 * u + lg4 + e <= rel;
-            const float p = vis ? __builtin_amdgcn_exp2f(sc[u][e] - m0) : 0.0f;
-            l += p;
-            w[e] = vis ? p * vs[u] : 0.0f;
+            for (int e = 0; e < 4; e++) {
+                const bool vis = 16 * u + lg4 + e <= rel;
+                const float p = vis ? __builtin_amdgcn_exp2f(x[u][e] - m0) : 0.0f;
+                l += p;
+                w[e] = vis ? p * vs[u] : 0.0f;
+            }
+        } else {
+            const float c = lv[u] - m0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_exp2f(fmaf(x[u][e], f[u], c));
+            l = fmaf((w[0] + w[1]) + (w[2] + w[3]), __builtin_amdgcn_rcpf(vs[u]), l);
         }
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
-            const f16x2 h = __builtin_convertvector((f32x2){w[e], w[e + 1]}, f16x2);
+            f16x2 hi, lo;
+            split2(w[e], w[e + 1], hi, lo);
             const int at = 4 * (u & 1) + e;
-            ph[u / 2][at] = h[0];
-            ph[u / 2][at + 1] = h[1];
-            pl[u / 2][at] = (_Float16)fmaf((float)h[0], -1.0f, w[e]);
-            pl[u / 2][at + 1] = (_Float16)fmaf((float)h[1], -1.0f, w[e + 1]);
+            ph[u / 2][at] = hi[0];
+            ph[u / 2][at + 1] = hi[1];
+            pl[u / 2][at] = lo[0];
+            pl[u / 2][at + 1] = lo[1];
         }
     }
     lsum = l;
@@ -354,11 +386,12 @@ __global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part pa
     __shared__ __align__(16) float ob[2][16 * OLD];
     const uint32_t t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const uint32_t hk = blockIdx.y, sp = blockIdx.x, S = gridDim.x, G = a.n_heads / a.n_kv, R = a.ntok * G;
-    const uint32_t ntile = (uint32_t)(((uint64_t)a.base + a.ntok + KV8_T - 1) / KV8_T), nstep = (ntile + 1) / 2;
+    const uint32_t hk = blockIdx.y, sp = blockIdx.x, S = gridDim.x, G = a.n_heads / a.n_kv;
+    const uint32_t r0 = blockIdx.z * 16, R = min(a.ntok * G - r0, 16u), first = a.base + r0 / G;    // first: visible to all rows
+    const uint32_t ntile = (a.base + (r0 + R - 1) / G) / KV8_T + 1, nstep = (ntile + 1) / 2;
     const uint32_t s0 = (uint32_t)((uint64_t)sp * nstep / S), s1 = (uint32_t)((uint64_t)(sp + 1) * nstep / S);
     const uint32_t bsh = __builtin_ctz(a.block / KV8_T);
-    const uint32_t tok = li < R ? li / G : 0, rpos = a.base + tok;
+    const uint32_t tok = (r0 + min(li, R - 1)) / G, head = hk * G + (r0 + min(li, R - 1)) % G, rpos = a.base + tok;
     const int8_t *codes = a.codes + (size_t)hk * (2 * KV8_T * HD) + lane * 16;
     const size_t rec = (size_t)a.n_kv * (2 * KV8_T * HD);
     const float *scales = a.scales + 2 * hk;
@@ -398,8 +431,7 @@ __global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part pa
         load_v(step);
     }
     v4i qd[3][NC];
-    const float qf = q_row<NC>(a.q + tok * a.q_tok + (size_t)(hk * G + li % G) * a.q_stride, li < R, al, lg,
-                               a.scale * 1.44269504088896340736f, qd);
+    const float qf = q_row<NC>(a.q + tok * a.q_tok + (size_t)head * a.q_stride, li < R, al, lg, a.scale * 1.44269504088896340736f, qd);
     f32x4 o[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) o[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -416,16 +448,16 @@ __global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part pa
 #pragma unroll
                 for (int d = 0; d < 3; d++)
                     s[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, kr[u][c]), qd[d][c], s[d], 0, 0, 0);
-            const float f = qf * ks[u];
 #pragma unroll
-            for (int e = 0; e < 4; e++) sc[u][e] = q_join(s[0][e], s[1][e], s[2][e]) * f;
+            for (int e = 0; e < 4; e++) sc[u][e] = q_join(s[0][e], s[1][e], s[2][e]);
         }
         const bool more = step + 4 < s1;
         if (more) { load_s(step + 4); load_k(step + 4); }
         f16x8 ph[1], pl[1];
-        const float al2 = step * 32 + 31 <= a.base      // every row sees every key
-                              ? softmax_step<2, false>(sc, vs, 0, mrun, lsum, ph, pl)
-                              : softmax_step<2, true>(sc, vs, (int)(rpos - step * 32), mrun, lsum, ph, pl);
+        const float f[2] = {qf * ks[0], qf * ks[1]};
+        const bool usual = step * 32 + 31 <= first && scales_usual(fminf(ks[0], ks[1]), fminf(vs[0], vs[1]));
+        const float al2 = usual ? softmax_step<2, false>(sc, f, vs, 0, mrun, lsum, ph, pl)
+                                : softmax_step<2, true>(sc, f, vs, (int)(rpos - step * 32), mrun, lsum, ph, pl);
         if (__builtin_amdgcn_ballot_w64(al2 != 1.0f)) {
 #pragma unroll
             for (int n = 0; n < NT; n++) o[n] *= al2;
@@ -468,7 +500,7 @@ __global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part pa
 #pragma unroll
         for (int w = 0; w < 4; w++)
             l += wl[w][r] * (wm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wm[w][r] - m));
-        const size_t row = (size_t)(r / G) * a.n_heads + hk * G + r % G;
+        const size_t row = (size_t)((r0 + r) / G) * a.n_heads + hk * G + (r0 + r) % G;
         if (S == 1) {
             st4(a.out + row * HD + d, v / l, !((uintptr_t)a.out & 15));
         } else {
@@ -480,197 +512,279 @@ __global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part pa
 }
 
 // ---------------------------------------------------------------------------
-// Attention of many rows: a workgroup takes NW x CT x 16 consecutive rows
+// Attention of many rows: a workgroup takes 128 consecutive rows, 16 to a wave
 // (token-major, the query heads of one kv head inside a token, so any group
-// size fills them) and walks its keys in tiles of 64, staged once in LDS for
+// size fills them), and walks its keys in tiles of 64, staged once in LDS for
 // all of them: the key codes as they lie (1 KB per operand fragment, 16 bytes
 // a lane, no bank conflict), the value codes turned into f16 on the way. The
-// arithmetic is the wave form's; a wave holds CT column tiles of 16 rows.
-// Both tiles are double-buffered: the next tile's loads are requested right
-// after a barrier, stored behind the current tile's products, one barrier per
-// tile. Grid: (row block, kv head, key split), the longest rows first.
+// arithmetic is the wave form's.
+// A tile's work is matrix products (112 instructions of 16 cycles at head_dim
+// 256) and softmax (340 vector instructions of 4 cycles and more). Waves that
+// run it in step leave the matrix units idle through the softmax: 46% busy.
+// So a wave alternates steps of products (the last tile's P V, this one's
+// K Q^T) and steps of softmax, and the two waves of a SIMD (w and w + 4) are
+// one step apart, a barrier after every step: one is in its products while the
+// other is in its softmax. Both tiles are double-buffered; a wave requests its
+// part of the next tile in a products step and stores it behind the softmax.
+// Grid: (row block, kv head, key split), the longest rows first.
 // ---------------------------------------------------------------------------
-template <int HD, int NW, int CT>
-__global__ void __launch_bounds__(NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_part part, int al) {
-    constexpr int NC = HD / 64, NT = HD / 16, NTH = NW * 64, ROWS = NW * CT * 16;
+#define KV8_NW 8
+#define KV8_ROWS (KV8_NW * 16u)
+
+// LDS done, then the barrier; loads from memory stay in flight
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int HD>
+__global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_part part, int al) {
+    constexpr int NC = HD / 64, NT = HD / 16, NTH = KV8_NW * 64;
     constexpr int KCH = 4 * NC * 64, VUN = 2 * NC * 64;     // 16-byte chunks of keys, units (two chunks) of values
     constexpr int KPT = (KCH + NTH - 1) / NTH, VPT = (VUN + NTH - 1) / NTH;
     __shared__ v4u kb[2][KCH];
     __shared__ v4u vb[2][2 * NT * 64];
+    __shared__ __align__(16) float sb[4][8];    // the tiles' scales (4 of keys, 4 of values): read up to two steps after the codes
     const uint32_t t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int grp = wave >> 2;
     const uint32_t hk = blockIdx.y, sp = blockIdx.z, S = gridDim.z, G = a.n_heads / a.n_kv;
-    const uint64_t R = (uint64_t)a.ntok * G, r0 = (uint64_t)(gridDim.x - 1 - blockIdx.x) * ROWS;
-    const uint32_t lastk = a.base + (uint32_t)(min(r0 + ROWS, R) - 1) / G;      // the block's last visible key
+    const uint64_t R = (uint64_t)a.ntok * G, r0 = (uint64_t)(gridDim.x - 1 - blockIdx.x) * KV8_ROWS;
+    const uint32_t lastk = a.base + (uint32_t)((min(r0 + KV8_ROWS, R) - 1) / G);      // the block's last visible key
     const uint32_t nrec = lastk / KV8_T + 1, nt = lastk / 64 + 1;
-    const uint32_t k0 = (uint32_t)((uint64_t)sp * nt / S), k1 = (uint32_t)((uint64_t)(sp + 1) * nt / S);
+    const uint32_t k0 = (uint32_t)((uint64_t)sp * nt / S), n = (uint32_t)((uint64_t)(sp + 1) * nt / S) - k0;    // tiles k0 .. k0 + n - 1
     const uint32_t bsh = __builtin_ctz(a.block / KV8_T);
     const size_t rec = (size_t)a.n_kv * (2 * KV8_T * HD);
     const int8_t *codes = a.codes + (size_t)hk * (2 * KV8_T * HD);
     const float *scales = a.scales + 2 * hk;
     const size_t srec = 2 * (size_t)a.n_kv;
 
+    // This thread's chunks of tile i (counted from k0): a uniform address and an
+    // offset of its own, except in the tile that the cache's end cuts.
     v4u kr[KPT], vr[VPT][2];
-    auto load = [&](uint32_t kt) {
+    float sr = 0.0f;
+    const uint32_t rec32 = (uint32_t)rec;       // a record row is at most 2^29 bytes
+    auto load = [&](uint32_t i, bool k, bool v) {
+        const uint32_t r4 = 4 * (k0 + i), last = nrec - 1 - r4;     // records from the tile's first that exist
+        const int8_t *p = codes + (size_t)r4 * rec;
+        const bool whole = last >= 3;
+        if (k) {
 #pragma unroll
-        for (int x = 0; x < KPT; x++) {
-            const uint32_t i = t + x * NTH;
-            if (KCH % NTH == 0 || i < KCH)
-                kr[x] = *(const v4u *)(codes + min(4 * kt + i / (NC * 64), nrec - 1) * rec + i % (NC * 64) * 16);
+            for (int x = 0; x < KPT; x++) {
+                const uint32_t c = t + x * NTH, u = c / (NC * 64), w = c % (NC * 64) * 16;
+                if (KCH % NTH == 0 || c < KCH) kr[x] = *(const v4u *)(p + ((whole ? u : min(u, last)) * rec32 + w));
+            }
         }
+        if (v) {
 #pragma unroll
-        for (int x = 0; x < VPT; x++) {
-            const uint32_t i = t + x * NTH;
-            if (VUN % NTH == 0 || i < VUN)
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-                    vr[x][h] = *(const v4u *)(codes + min(4 * kt + i / (NC * 64) * 2 + h, nrec - 1) * rec + KV8_T * HD +
-                                              i % (NC * 64) * 16);
+            for (int x = 0; x < VPT; x++) {
+                const uint32_t c = t + x * NTH, u = c / (NC * 64) * 2, w = c % (NC * 64) * 16 + KV8_T * HD;
+                if (VUN % NTH == 0 || c < VUN) {
+                    vr[x][0] = *(const v4u *)(p + ((whole ? u : min(u, last)) * rec32 + w));
+                    vr[x][1] = *(const v4u *)(p + ((whole ? u + 1 : min(u + 1, last)) * rec32 + w));
+                }
+            }
         }
     };
-    auto stage = [&](int b) {
+    auto load_s = [&](uint32_t i) {     // the first eight threads: a scale each
+        if (t < 8) sr = scales[(size_t)(min(4 * (k0 + i) + t % 4, nrec - 1) >> bsh) * srec + t / 4];
+    };
+    auto stage_k = [&](uint32_t i) {
 #pragma unroll
         for (int x = 0; x < KPT; x++) {
-            const uint32_t i = t + x * NTH;
-            if (KCH % NTH == 0 || i < KCH) kb[b][i] = kr[x];
+            const uint32_t c = t + x * NTH;
+            if (KCH % NTH == 0 || c < KCH) kb[i & 1][c] = kr[x];
         }
+        if (t < 8) sb[i & 3][t] = sr;
+    };
+    auto stage_v = [&](uint32_t i) {
 #pragma unroll
         for (int x = 0; x < VPT; x++) {
-            const uint32_t i = t + x * NTH;
-            if (VUN % NTH == 0 || i < VUN)
+            const uint32_t c = t + x * NTH;
+            if (VUN % NTH == 0 || c < VUN)
 #pragma unroll
-                for (int j = 0; j < 4; j++)         // fragment (pair, dim tile 4 c + j)
-                    vb[b][(i / 64 * 4 + j) * 64 + i % 64] = __builtin_bit_cast(v4u, codes_f16(vr[x][0][j], vr[x][1][j]));
+                for (int j = 0; j < 4; j++)         // fragment (pair of tiles, dims 16 (4 c + j) ..)
+                    vb[i & 1][(c / 64 * 4 + j) * 64 + c % 64] = __builtin_bit_cast(v4u, codes_f16(vr[x][0][j], vr[x][1][j]));
         }
     };
 
-    if (k0 < k1) load(k0);
-    v4i qd[CT][3][NC];
-    float qf[CT], mrun[CT], lsum[CT];
-    uint32_t rpos[CT];
-    f32x4 o[CT][NT];
+    if (n) { load(0, true, false); load_s(0); }
+    const uint64_t r = r0 + wave * 16 + li, rw = r0 + wave * 16;
+    const uint32_t tok = r < R ? (uint32_t)r / G : 0, head = hk * G + (r < R ? (uint32_t)r % G : 0), rpos = a.base + tok;
+    v4i qd[3][NC];
+    const float qf = q_row<NC>(a.q + tok * a.q_tok + (size_t)head * a.q_stride, r < R, al, lg, a.scale * 1.44269504088896340736f, qd);
+    float mrun = -INFINITY, lsum = 0.0f, resc = 1.0f;
+    f32x4 o[NT];
 #pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-        const uint64_t r = r0 + (wave * CT + ct) * 16 + li;
-        const uint32_t tok = r < R ? (uint32_t)(r / G) : 0, g = r < R ? (uint32_t)(r % G) : 0;
-        rpos[ct] = a.base + tok;
-        qf[ct] = q_row<NC>(a.q + tok * a.q_tok + (size_t)(hk * G + g) * a.q_stride, r < R, al, lg,
-                           a.scale * 1.44269504088896340736f, qd[ct]);
-        mrun[ct] = -INFINITY;
-        lsum[ct] = 0.0f;
-#pragma unroll
-        for (int n = 0; n < NT; n++) o[ct][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
+    for (int d = 0; d < NT; d++) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     // the wave's first and last visible keys: no mask up to the one, no work past the other
-    const uint64_t rw = r0 + wave * CT * 16;
-    const bool on = rw < R;
-    const uint32_t wfirst = on ? a.base + (uint32_t)(rw / G) : 0, wlast = on ? a.base + (uint32_t)((min(rw + CT * 16, R) - 1) / G) : 0;
-    if (k0 < k1) stage(0);
-    __syncthreads();
-    for (uint32_t kt = k0; kt < k1; kt++) {
-        const int b = (kt - k0) & 1;
-        const bool more = kt + 1 < k1;
-        if (more) load(kt + 1);
-        if (on && kt * 64 <= wlast) {
-            const bool whole = kt * 64 + 63 <= wfirst;
-            float ks[4], vs[4], sc[CT][4][4];
+    const uint32_t wfirst = a.base + (uint32_t)rw / G;
+    const uint32_t wtiles = rw < R ? (a.base + (uint32_t)(min(rw + 16, R) - 1) / G) / 64 + 1 : 0;
+    const uint32_t ntw = wtiles > k0 ? min(wtiles - k0, n) : 0;
+    float sc[4][4];
+    f16x8 ph[2], pl[2];
+    // Step of products, tile i: P V of tile i - 1, K Q^T of tile i. The other
+    // wave of the SIMD is in its softmax, so the wave has to cover the LDS reads
+    // itself: fragments go through a ring of eight, each requested seven ahead
+    // (14 products, 224 cycles), and the two halves of a P V pair are two
+    // products apart. At the ends it multiplies zeros (no tile -1: its weights
+    // and values are) or what nobody reads (no tile n).
+    auto products = [&](uint32_t i) {
+        constexpr int NV = 2 * NT, NK = 4 * NC, RING = 8;
+        const v4u *vt = vb[(i + 1) & 1] + lane, *kt = kb[i & 1] + lane;
+        v4u fr[RING];
+        auto fetch = [&](int k) {
+            if (k < NV + NK) fr[k % RING] = k < NV ? vt[k * 64] : kt[(k - NV) * 64];
+        };
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const float *p = scales + (size_t)(min(4 * kt + u, nrec - 1) >> bsh) * srec;
-                ks[u] = p[0];
-                vs[u] = p[1];
-            }
+        for (int k = 0; k < RING - 1; k++) fetch(k);
+        if (__builtin_amdgcn_ballot_w64(resc != 1.0f)) {
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                v4i s[CT][3];
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                    for (int d = 0; d < 3; d++) s[ct][d] = (v4i){0, 0, 0, 0};
-#pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    const v4i kf = __builtin_bit_cast(v4i, kb[b][(u * NC + c) * 64 + lane]);
-#pragma unroll
-                    for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                        for (int d = 0; d < 3; d++)
-                            s[ct][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kf, qd[ct][d][c], s[ct][d], 0, 0, 0);
-                }
-#pragma unroll
-                for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) sc[ct][u][e] = q_join(s[ct][0][e], s[ct][1][e], s[ct][2][e]) * (qf[ct] * ks[u]);
-            }
-            f16x8 ph[CT][2], pl[CT][2];
-#pragma unroll
-            for (int ct = 0; ct < CT; ct++) {
-                const float al2 = whole ? softmax_step<4, false>(sc[ct], vs, 0, mrun[ct], lsum[ct], ph[ct], pl[ct])
-                                        : softmax_step<4, true>(sc[ct], vs, (int)(rpos[ct] - kt * 64), mrun[ct], lsum[ct], ph[ct], pl[ct]);
-                if (__builtin_amdgcn_ballot_w64(al2 != 1.0f)) {
-#pragma unroll
-                    for (int n = 0; n < NT; n++) o[ct][n] *= al2;
-                }
-            }
-#pragma unroll
-            for (int m = 0; m < 2; m++)
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const f16x8 vf = __builtin_bit_cast(f16x8, vb[b][(m * NT + n) * 64 + lane]);
-#pragma unroll
-                    for (int ct = 0; ct < CT; ct++) {
-                        o[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[ct][m], o[ct][n], 0, 0, 0);
-                        o[ct][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[ct][m], o[ct][n], 0, 0, 0);
-                    }
-                }
+            for (int d = 0; d < NT; d++) o[d] *= resc;
         }
-        if (more) stage(b ^ 1);
-        __syncthreads();
+#pragma unroll
+        for (int k = 0; k <= NV; k++) {
+            if (k) o[(k - 1) % NT] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, fr[(k - 1) % RING]), pl[(k - 1) / NT],
+                                                                            o[(k - 1) % NT], 0, 0, 0);
+            if (k < NV) o[k % NT] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, fr[k % RING]), ph[k / NT], o[k % NT], 0, 0, 0);
+            if (k < NV) fetch(k + RING - 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        v4i s[3];
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            const int u = k / NC, c = k % NC;
+            if (c == 0) s[0] = s[1] = s[2] = (v4i){0, 0, 0, 0};
+#pragma unroll
+            for (int d = 0; d < 3; d++)
+                s[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, fr[(NV + k) % RING]), qd[d][c], s[d], 0, 0, 0);
+            fetch(NV + k + RING - 1);
+            if (c == NC - 1) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) sc[u][e] = q_join(s[0][e], s[1][e], s[2][e]);
+            }
+        }
+    };
+    auto weights = [&](uint32_t i) {
+        const f32x4 k4 = *(const f32x4 *)&sb[i & 3][0], v4 = *(const f32x4 *)&sb[i & 3][4];
+        const float vs[4] = {v4[0], v4[1], v4[2], v4[3]}, f[4] = {qf * k4[0], qf * k4[1], qf * k4[2], qf * k4[3]};
+        const uint32_t key = (k0 + i) * 64;
+        const bool usual = key + 63 <= wfirst && scales_usual(fminf(fminf(k4[0], k4[1]), fminf(k4[2], k4[3])),
+                                                              fminf(fminf(v4[0], v4[1]), fminf(v4[2], v4[3])));
+        resc = usual ? softmax_step<4, false>(sc, f, vs, 0, mrun, lsum, ph, pl)
+                     : softmax_step<4, true>(sc, f, vs, (int)(rpos - key), mrun, lsum, ph, pl);
+    };
+
+    ph[0] = ph[1] = pl[0] = pl[1] = (f16x8){};
+#pragma unroll
+    for (int x = 0; x < 2 * NT * 64; x += NTH)
+        if (2 * NT * 64 % NTH == 0 || t + x < 2 * NT * 64) vb[1][t + x] = (v4u){0, 0, 0, 0};
+    if (n) {
+        stage_k(0);
+        load(1, n > 1, false);
+        if (n > 1) load_s(1);
+        load(0, false, true);
     }
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-        lsum[ct] += swap16f(lsum[ct]);
-        lsum[ct] += swap32f(lsum[ct]);
-        const uint64_t r = r0 + (wave * CT + ct) * 16 + li;
-        if (r >= R) continue;
-        const float l = lsum[ct];
-        const size_t row = (size_t)(r / G) * a.n_heads + hk * G + (uint32_t)(r % G);
-        if (S == 1) {
-            const bool oal = !((uintptr_t)a.out & 15);
-#pragma unroll
-            for (int n = 0; n < NT; n++) st4(a.out + row * HD + 16 * n + 4 * lg, o[ct][n] / l, oal);
+    lds_barrier();
+    // Period i (two steps, one barrier): group 0 does the products of tile i and
+    // the softmax of i, group 1 the softmax of i - 1 and the products of i. Read
+    // are the keys of tile i and the values of i - 1; written, in a wave's
+    // softmax step, the keys of i + 1 and the values of i, requested a period ago.
+    for (uint32_t h = 0; n && h < 2 * n + 2; h++) {
+        const int x = (int)h - grp, i = x >> 1;
+        if (!(x & 1)) {
+            if (ntw) products(i);
         } else {
-            float *acc = part.acc + (row * S + sp) * HD + 4 * lg;
-#pragma unroll
-            for (int n = 0; n < NT; n++) *(f32x4 *)(acc + 16 * n) = o[ct][n];
-            if (lg == 0) { part.m[row * S + sp] = l != l ? 0.0f : mrun[ct] * 0.69314718055994530942f; part.s[row * S + sp] = l; }
+            const uint32_t next = h >> 1;
+            if (next + 1 < n) stage_k(next + 1);
+            if (next < n) stage_v(next);
+            load(next + 2, next + 2 < n, false);
+            if (next + 2 < n) load_s(next + 2);
+            load(next + 1, false, next + 1 < n);
+            if (i >= 0 && (uint32_t)i < ntw) {
+                weights(i);
+            } else {
+                ph[0] = ph[1] = pl[0] = pl[1] = (f16x8){};
+                resc = 1.0f;
+            }
         }
+        if (h & 1) lds_barrier();
+    }
+    lsum += swap16f(lsum);
+    lsum += swap32f(lsum);
+    if (r >= R) return;
+    const float l = lsum;
+    const size_t row = (size_t)tok * a.n_heads + head;
+    if (S == 1) {
+        const bool oal = !((uintptr_t)a.out & 15);
+#pragma unroll
+        for (int d = 0; d < NT; d++) st4(a.out + row * HD + 16 * d + 4 * lg, o[d] / l, oal);
+    } else {
+        float *acc = part.acc + (row * S + sp) * HD + 4 * lg;
+#pragma unroll
+        for (int d = 0; d < NT; d++) *(f32x4 *)(acc + 16 * d) = o[d];
+        if (lg == 0) { part.m[row * S + sp] = l != l ? 0.0f : mrun * 0.69314718055994530942f; part.s[row * S + sp] = l; }
     }
 }
 
-// How a call runs. Few rows: the key-split form, in as many splits as give
-// every wave a step, up to two workgroups per CU (what is resident). More: row
-// blocks, one workgroup per CU at a time, their keys split where that shortens
-// the launch: rounds x (a part's tiles + KV8_TAIL for its start and end) tiles
-// of KV8_TILE_US, against the partials' way to memory and back.
-#define KV8_NW 8
-#define KV8_CT 1
-#define KV8_ROWS (KV8_NW * KV8_CT * 16u)
+// Join of few splits of many rows: four dims of a row per lane, all splits'
+// loads in flight, nothing shared between lanes. (k_attn_combine, a workgroup
+// per row, joins many splits of few rows.) A row's first maximum is the
+// smallest that any split may have, so a split without a visible key has
+// weight zero; NaN sums reach the output.
+#define KV8_JOIN 8u
+template <int HD>
+__global__ void __launch_bounds__(TPB) k_kv8_join(kv8_part p, float *out, uint64_t rows, uint32_t S, int al) {
+    constexpr uint32_t L = HD / 4;
+    const uint64_t row = (uint64_t)blockIdx.x * (TPB / L) + threadIdx.x / L;
+    const uint32_t d = threadIdx.x % L * 4;
+    if (row >= rows) return;
+    f32x4 acc[KV8_JOIN];
+    float m[KV8_JOIN], l[KV8_JOIN], M = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (uint32_t k = 0; k < KV8_JOIN; k++) {
+        const bool on = k < S;
+        m[k] = on ? p.m[row * S + k] : -INFINITY;
+        l[k] = on ? p.s[row * S + k] : 0.0f;
+        acc[k] = on ? *(const f32x4 *)(p.acc + (row * S + k) * HD + d) : (f32x4){0.f, 0.f, 0.f, 0.f};
+        M = fmaxf(M, m[k]);
+    }
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (uint32_t k = 0; k < KV8_JOIN; k++) {
+        const float w = m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[k] - M) * 1.44269504088896340736f);
+        sum = fmaf(l[k], w, sum);
+        o += acc[k] * w;
+    }
+    st4(out + row * HD + d, o / sum, al);
+}
+
+// How a call runs. The wave form: small calls, in as many key splits as give
+// every wave a step, up to two workgroups per CU (what is resident). Else row
+// blocks in tiles, one workgroup per CU at a time, their keys split where that
+// shortens the launch: rounds x (a part's tiles + KV8_TAIL for its start and
+// end) tiles of KV8_TILE_US, against the partials' way to memory and back.
+// KV8_SMALL, in waves' steps of 32 keys x head_dim, is where the two meet
+// (whole call, us, wave / tile): 24 heads of 256 on 4, 8040 keys, 240 rows
+// (3.9M) 48.9 / 50.4, 462 rows (7.5M) 67.7 / 61.2, 1300 keys, 1800 rows (4.7M)
+// 47.9 / 65.5; 32 of 128 on 8, 8020 keys, 80 rows (1.3M) 32.2 / 36.0, 8077 keys,
+// 308 rows (5.2M) 58.1 / 55.0; 12 of 64, 32077 keys, 77 rows (3.9M) 59.5 / 60.5.
+#define KV8_SMALL (1ull << 22)
 #define KV8_TILE_US 2.5         /* at head_dim 256 */
 #define KV8_TAIL 3.0
 #define KV8_PART_BYTES (256ull << 20)
 struct kv8_plan { bool wave; uint32_t splits, blocks; };
 static kv8_plan kv8_plan_of(const sgk_kv8_attn *a) {
     const uint64_t G = a->n_heads / a->n_kv, rows = a->ntok * G, keys = (uint64_t)a->base + a->ntok, cus = sgk_device_cus();
-    kv8_plan p = {rows <= 16, 1, (uint32_t)((rows + KV8_ROWS - 1) / KV8_ROWS)};
+    const bool wave = rows <= 16 || (rows + 15) / 16 * a->n_kv * ((keys + 31) / 32) * a->hd <= KV8_SMALL;
+    const uint64_t per = wave ? 16 : KV8_ROWS, wgs = (rows + per - 1) / per * a->n_kv;
+    kv8_plan p = {wave, 1, (uint32_t)((rows + per - 1) / per)};
     if (p.wave) {
-        uint64_t most = 2 * cus / a->n_kv, want = (keys + 127) / 128;
+        uint64_t most = 2 * cus / wgs, want = (keys + 127) / 128;
         if (most > 1024) most = 1024;
         if (most < 1) most = 1;
         p.splits = (uint32_t)(want < most ? want : most);
         return p;
     }
-    const uint64_t wgs = (uint64_t)p.blocks * a->n_kv, tiles = (keys + 63) / 64, prow = (uint64_t)a->ntok * a->n_heads * a->hd * 4;
-    uint64_t most = wgs < cus ? 2 * cus / wgs : 8;
+    const uint64_t tiles = (keys + 63) / 64, prow = (uint64_t)a->ntok * a->n_heads * a->hd * 4;
+    uint64_t most = wgs < cus ? 2 * cus / wgs : KV8_JOIN;
     if (most > 1024) most = 1024;
     if (most > tiles) most = tiles;
     double best = 0.0;
@@ -703,9 +817,8 @@ extern "C" hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hi
     }
 #define KC(H)                                                                                                                 \
     do {                                                                                                                      \
-        if (p.wave) hipLaunchKernelGGL(k_kv8_wave<H>, dim3(p.splits, a->n_kv), dim3(TPB), 0, s, *a, part, al);                \
-        else hipLaunchKernelGGL((k_kv8_tile<H, KV8_NW, KV8_CT>), dim3(p.blocks, a->n_kv, p.splits), dim3(KV8_NW * 64), 0, s,  \
-                                *a, part, al);                                                                                \
+        if (p.wave) hipLaunchKernelGGL(k_kv8_wave<H>, dim3(p.splits, a->n_kv, p.blocks), dim3(TPB), 0, s, *a, part, al);      \
+        else hipLaunchKernelGGL(k_kv8_tile<H>, dim3(p.blocks, a->n_kv, p.splits), dim3(KV8_NW * 64), 0, s, *a, part, al);     \
     } while (0)
     switch (a->hd) {
     case 64: KC(64); break;
@@ -713,8 +826,19 @@ extern "C" hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hi
     default: KC(256); break;
     }
 #undef KC
-    const hipError_t e = hipGetLastError();
+    hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
+    if (p.splits <= KV8_JOIN) {
+        const uint64_t n = (uint64_t)a->ntok * a->n_heads, per = TPB / (a->hd / 4);
+        const dim3 grid((uint32_t)((n + per - 1) / per));
+        const int oal = !((uintptr_t)a->out & 15);
+        switch (a->hd) {
+        case 64: hipLaunchKernelGGL(k_kv8_join<64>, grid, dim3(TPB), 0, s, part, a->out, n, p.splits, oal); break;
+        case 128: hipLaunchKernelGGL(k_kv8_join<128>, grid, dim3(TPB), 0, s, part, a->out, n, p.splits, oal); break;
+        default: hipLaunchKernelGGL(k_kv8_join<256>, grid, dim3(TPB), 0, s, part, a->out, n, p.splits, oal); break;
+        }
+        return hipGetLastError();
+    }
     sgk_attn c = {};
     c.m = part.m; c.s = part.s; c.acc = part.acc; c.out = a->out; c.n_heads = a->n_heads; c.n_kv = a->n_kv; c.hd = a->hd;
     c.out_tok = a->n_heads * a->hd; c.n_splits = p.splits; c.max_splits = p.splits; c.ntok = a->ntok;

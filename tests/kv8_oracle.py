@@ -100,7 +100,7 @@ def attention(q, cache, base, scale):
                 s = kk @ qq * scale
                 p = np.exp(s - s.max())
                 out[t, h] = p @ vv / p.sum()
-                ds = scale * 2 * u * np.abs(qq).max() * np.abs(kk).sum(1).max() + 16 * u * np.abs(s).max()
+                ds = abs(scale) * 2 * u * np.abs(qq).max() * np.abs(kk).sum(1).max() + 16 * u * np.abs(s).max()
                 bound[t, h] = (2 * (ds + 6 * u) + (m / 16 + 64) * u) * np.abs(vv).max()
     return out, bound
 

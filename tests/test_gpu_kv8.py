@@ -351,3 +351,55 @@ def test_cache_past_32_bits(gpu):
             assert (np.abs(out.array[h] - want) <= bound).all()
     codes.free()
     scales.free()
+
+
+# ---------------------------------------------------------------- sizes past the small-call form
+
+@pytest.mark.parametrize("nh,nkv,hd,block,base,n", [
+    (24, 4, 256, 64, 3001, 203), (32, 8, 128, 16, 3000, 301), (12, 12, 64, 32, 8000, 401), (16, 1, 256, 128, 0, 800),
+    (6, 2, 256, 64, 20000, 121), (10, 2, 128, 32, 15, 1500)])
+def test_prefill_tiles(gpu, nh, nkv, hd, block, base, n):
+    rng = np.random.default_rng(n)
+    c = filled(rng, nkv, hd, block, base + n)
+    q = rng.standard_normal((n, nh, hd)).astype(np.float32)
+    want, bound = K.attention(q, c, base, 1 / math.sqrt(hd))
+    got = attend(gpu, c, q, base, 1 / math.sqrt(hd))
+    close(got, want, bound)
+    assert np.array_equal(got, attend(gpu, c, q, base, 1 / math.sqrt(hd)))
+
+
+def test_prefill_tiles_scales_and_nan(gpu):
+    """The tile form on scales far apart, blocks of zeros, a poisoned block that only the last tokens see, and
+    rows of q that are not finite, zero, or near the ends of the range."""
+    rng = np.random.default_rng(21)
+    seq, n, nh, hd = 6000, 128, 16, 256
+    c = filled(rng, 1, hd, 16, seq)
+    nb = -(-seq // 16)
+    c.scales[:nb, :, 1] = 2.0 ** rng.integers(-40, 9, (nb, 1))
+    c.scales[3, :, 1], c.scales[5] = 0, 0
+    c.codes[3, :, 1], c.codes[5] = 0, 0
+    c.scales[7, :, 0] *= 30
+    c.scales[-(-seq // 16) - 4] = np.nan                        # positions 5936 .. 5951
+    q = (rng.standard_normal((n, nh, hd)) * np.exp(rng.standard_normal((n, nh, 1)) * 2)).astype(np.float32)
+    q[3, 2, 9], q[4, 5, 200], q[5, 1] = np.nan, -np.inf, 0
+    q[6, 0] *= 1e-30
+    q[7, 0] *= 1e-42
+    got = attend(gpu, c, q, seq - n, 1 / 16)
+    sees = seq - n + np.arange(n) >= 5936
+    assert np.isnan(got[sees]).all() and sees.any() and not sees.all()
+    bad = ~np.isfinite(q).all(axis=2)
+    assert np.isnan(got[bad]).all()
+    c.scales[-(-seq // 16) - 4] = 0.01
+    want, bound = K.attention(np.where(np.isfinite(q), q, 0), c, seq - n, 1 / 16)
+    ok = ~bad & ~sees[:, None]
+    close(got[ok], want[ok], bound[ok])
+
+
+@pytest.mark.parametrize("n,seq", [(1, 500), (30, 500), (128, 6000)])
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+def test_scale_of_either_sign(gpu, n, seq, scale):
+    rng = np.random.default_rng(n)
+    c = filled(rng, 1, 256, 32, seq)
+    q = rng.standard_normal((n, 16, 256)).astype(np.float32)
+    want, bound = K.attention(q, c, seq - n, float(np.float32(scale)))
+    close(attend(gpu, c, q, seq - n, scale), want, bound)
