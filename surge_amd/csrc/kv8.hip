@@ -27,10 +27,11 @@ __device__ __forceinline__ uint32_t val_at(uint32_t r, uint32_t d) {
 
 // ---------------------------------------------------------------------------
 // Store. One workgroup per (block, kv head, half) holds the block's new rows
-// in registers: one read for the maximum and the codes. A unit is 16 elements,
-// a row's 16 dims for keys (one 16-byte code store) or 4 positions x 4 dims for
-// values (four dwords, transposed in registers); U units per thread.
-// Rows before base keep their codes unless the scale grows.
+// in registers: one read for the maximum and the codes. Keys go four dims of a
+// row at a time, a wave taking 8 rows x 32 dims (whole lines of the rows, 128
+// bytes of codes at a time); values 4 positions x 4 dims, transposed in
+// registers into a dword per dim. 4 U fours per thread. Rows before base keep
+// their codes unless the scale grows.
 // ---------------------------------------------------------------------------
 struct kv8_store_args {
     const float *x[2];
@@ -40,104 +41,145 @@ struct kv8_store_args {
     uint32_t n_kv, hd, block, base, n;
 };
 
-// x / s to the nearest integer, ties to even, decided exactly: q = rint(x * (1/s))
-// is within one of it, and the remainder x - q s is exact in one fma.
-__device__ __forceinline__ int quant(float x, float s, float inv) {
-    float q = rintf(x * inv);
-    const float r = fmaf(-q, s, x), a = 2.0f * fabsf(r);
-    if (a > s || (a == s && ((int)q & 1))) q += copysignf(1.0f, r);
-    return (int)fminf(fmaxf(q, -127.0f), 127.0f);
-}
-__device__ __forceinline__ int8_t requant(int8_t c, double was, double s) {
-    return (int8_t)rint((double)c * was / s);
+// Where four of a wave's keys lie: chunk c is 8 rows x 32 dims.
+__device__ __forceinline__ void key_four(uint32_t c, uint32_t hd, uint32_t &r, uint32_t &d) {
+    const uint32_t lane = threadIdx.x & 63;
+    r = c / (hd / 32) * 8 + lane / 8;
+    d = c % (hd / 32) * 32 + lane % 8 * 4;
 }
 
-template <int U>
-__global__ void __launch_bounds__(TPB) k_kv8_store(kv8_store_args a, int al) {
-    __shared__ uint32_t red[4];
-    const uint32_t t = threadIdx.x, h = blockIdx.y, half = blockIdx.z, hd = a.hd;
-    const uint32_t blk = a.base / a.block + blockIdx.x, p0 = blk * a.block;
+// Four x / s to the nearest integers, ties to even, as bytes. q = rint(x * (1/s))
+// can be wrong only where x / s is within 2^-16 of a tie; there the remainder
+// x - q s, exact in one fma, decides. Clamped for a scale near the end of the
+// range, whose rounding may leave |x / s| above 127.
+__device__ __forceinline__ uint32_t quant4(f32x4 x, float s, float inv) {
+    float q[4];
+    bool close = false;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float t = x[e] * inv;
+        q[e] = rintf(t);
+        close |= !(fabsf(t - q[e]) < 0.4999f);
+    }
+    if (close) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float r = fmaf(-q[e], s, x[e]), a = 2.0f * fabsf(r);
+            if (a > s || (a == s && ((int)q[e] & 1))) q[e] += copysignf(1.0f, r);
+            q[e] = fminf(fmaxf(q[e], -127.0f), 127.0f);
+        }
+    }
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) w |= (uint32_t)((int)q[e] & 0xFF) << (8 * e);
+    return w;
+}
+__device__ __forceinline__ uint32_t requant4(uint32_t c, double was, double s) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) w |= (uint32_t)((int)rint((double)(int8_t)(c >> (8 * e)) * was / s) & 0xFF) << (8 * e);
+    return w;
+}
+// bytes of a where the mask's bytes are set, else of b
+__device__ __forceinline__ uint32_t pick_bytes(uint32_t mask, uint32_t a, uint32_t b) { return (a & mask) | (b & ~mask); }
+
+// Workgroups in the order of the rows in memory: a block's heads and halves side by side.
+// NTH threads, 4 U fours each: a large block takes more threads, not more
+// registers (8190 rows of 4 heads of 256 in blocks of 64: 25 us with 4 units in
+// each of 256 threads, 140 registers).
+template <int U, int NTH>
+__global__ void __launch_bounds__(NTH, 4) k_kv8_store(kv8_store_args a, uint32_t first, int al) {
+    __shared__ uint32_t red[NTH / 64];
+    const uint32_t id = first + blockIdx.x, t = threadIdx.x, half = id & 1, h = id / 2 % a.n_kv, hd = a.hd;
+    const uint32_t blk = a.base / a.block + id / 2 / a.n_kv, p0 = blk * a.block;
     const uint32_t lo = max(p0, a.base), hi = (uint32_t)min((uint64_t)p0 + a.block, (uint64_t)a.base + a.n);
     const uint32_t kept = lo - p0, rows = hi - p0;      // rows kept .. rows-1 of the block are new
-    const uint32_t units = a.block * hd / 16, d4 = hd / 4, d16 = hd / 16;
+    const uint32_t fours = a.block * hd / 4, d4 = hd / 4;
     const float *x = a.x[half] + (size_t)(lo - a.base) * a.stride + (size_t)h * hd;
     float *sp = a.scales + ((size_t)blk * a.n_kv + h) * 2 + half;
     const float was = kept ? *sp : 0.0f;
-    f32x4 v[U][4];
-    uint32_t mx = 0;
+    int8_t *codes = a.codes + (size_t)half * KV8_T * hd;
+    f32x4 v[4 * U];
+    uint32_t old[U][4], mx = 0;
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        const uint32_t i = t + u * TPB;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const uint32_t r = half ? i / d4 * 4 + j : i / d16, d = half ? i % d4 * 4 : i % d16 * 16 + 4 * j;
-            v[u][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-            if (i < units && r >= kept && r < rows) v[u][j] = ld4(x + (size_t)(r - kept) * a.stride + d, al);
-#pragma unroll
-            for (int e = 0; e < 4; e++) mx = max(mx, __float_as_uint(v[u][j][e]) & 0x7FFFFFFFu);
-        }
+    for (int i = 0; i < 4 * U; i++) {
+        uint32_t r, d;
+        const bool in = half ? (t + i / 4 * NTH) * 4 < fours : (t + i * NTH) < fours;
+        if (half) { r = (t + i / 4 * NTH) / d4 * 4 + i % 4; d = (t + i / 4 * NTH) % d4 * 4; }
+        else key_four((t >> 6) + i * (NTH / 64), hd, r, d);
+        v[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        if (in && r >= kept && r < rows) v[i] = ld4(x + (size_t)(r - kept) * a.stride + d, al);
     }
+    // the dwords of values that hold rows which are not new, asked for early
+    auto load_old = [&](int u, uint32_t r, uint32_t d) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (r < rows && (r < kept || r + 4 > rows))
+                old[u][e] = *(const uint32_t *)(codes + rec_at((p0 + r) / KV8_T, a.n_kv, h, hd) + val_at(r % KV8_T, d + e));
+    };
+    if (half && (kept || rows < a.block)) {
+#pragma unroll
+        for (int u = 0; u < U; u++) load_old(u, (t + u * NTH) / d4 * 4, (t + u * NTH) % d4 * 4);
+    }
+#pragma unroll
+    for (int i = 0; i < 4 * U; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) mx = max(mx, __float_as_uint(v[i][e]) & 0x7FFFFFFFu);
     mx = wave_umax(mx);
     if ((t & 63) == 0) red[t >> 6] = mx;
     __syncthreads();
-    mx = max(max(red[0], red[1]), max(red[2], red[3]));
+#pragma unroll
+    for (int w = 0; w < NTH / 64; w++) mx = max(mx, red[w]);
     // 65520 and above round to infinity in f16; NaN's bits are above those
     const bool poison = mx >= 0x477FF000u || was != was;
-    float s = fmaxf(__uint_as_float(poison ? 0 : mx) * (1.0f / 127.0f), poison ? 0.0f : was);
+    const float s = fmaxf(__uint_as_float(poison ? 0 : mx) * (1.0f / 127.0f), poison ? 0.0f : was);
     const bool grew = kept && s > was && !poison;
     if (t == 0) *sp = poison ? NAN : s;
     // a scale near the end of the range: x / s is the same for both times 2^64
     const float up = s < 0x1p-60f ? 0x1p64f : 1.0f, sq = s * up, inv = s > 0.0f ? 1.0f / sq : 0.0f;
     const bool zero = poison || s == 0.0f;
 #pragma unroll
+    for (int i = 0; i < 4 * U; i++) v[i] = zero ? (f32x4){0.f, 0.f, 0.f, 0.f} : v[i] * up;
+    const float sz = zero ? 1.0f : sq;
+    if (!half) {
+#pragma unroll
+        for (int i = 0; i < 4 * U; i++) {
+            uint32_t r, d;
+            key_four((t >> 6) + i * (NTH / 64), hd, r, d);
+            if (t + i * NTH >= fours || r >= rows || (r < kept && !grew)) continue;
+            uint32_t *p = (uint32_t *)(codes + rec_at((p0 + r) / KV8_T, a.n_kv, h, hd) + key_at(r % KV8_T, d));
+            *p = r < kept ? requant4(*p, was, s) : quant4(v[i], sz, inv);
+        }
+        return;
+    }
+#pragma unroll
     for (int u = 0; u < U; u++) {
-        const uint32_t i = t + u * TPB;
-        if (i >= units) continue;
+        const uint32_t r = (t + u * NTH) / d4 * 4, d = (t + u * NTH) % d4 * 4;
+        if ((t + u * NTH) * 4 >= fours || r >= rows || (r + 4 <= kept && !grew)) continue;
         uint32_t w[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            uint32_t c = 0;
+        for (int j = 0; j < 4; j++) w[j] = quant4(v[4 * u + j], sz, inv);
+        // rows to dims: a 4 x 4 transpose of bytes
+        const uint32_t a01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), a23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+        const uint32_t b01 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u), b23 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+        uint32_t c[4] = {__builtin_amdgcn_perm(a23, a01, 0x05040100u), __builtin_amdgcn_perm(a23, a01, 0x07060302u),
+                         __builtin_amdgcn_perm(b23, b01, 0x05040100u), __builtin_amdgcn_perm(b23, b01, 0x07060302u)};
+        if (r < kept || r + 4 > rows) {     // some of the four rows are not new
+            uint32_t isnew = 0, iskept = 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++) c |= (uint32_t)(zero ? 0 : quant(v[u][j][e] * up, sq, inv) & 0xFF) << (8 * e);
-            w[j] = c;
-        }
-        if (!half) {
-            const uint32_t r = i / d16, d = i % d16 * 16;
-            if (r >= rows || (r < kept && !grew)) continue;
-            int8_t *p = a.codes + rec_at((p0 + r) / KV8_T, a.n_kv, h, hd) + key_at(r % KV8_T, d);
-            if (r < kept) {
-                v4u old = *(const v4u *)p;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    uint32_t c = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) c |= (uint32_t)(requant((int8_t)(old[j] >> (8 * e)), was, s) & 0xFF) << (8 * e);
-                    w[j] = c;
-                }
+            for (uint32_t j = 0; j < 4; j++) {
+                if (r + j >= kept && r + j < rows) isnew |= 0xFFu << (8 * j);
+                if (r + j < kept) iskept |= 0xFFu << (8 * j);
             }
-            *(v4u *)p = (v4u){w[0], w[1], w[2], w[3]};
-        } else {
-            const uint32_t r = i / d4 * 4, d = i % d4 * 4;
-            if (r >= rows || (r + 4 <= kept && !grew)) continue;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                uint32_t *p = (uint32_t *)(a.codes + a.hd * KV8_T + rec_at((p0 + r) / KV8_T, a.n_kv, h, hd) + val_at(r % KV8_T, d + e));
-                uint32_t c = 0;
-#pragma unroll
-                for (int j = 0; j < 4; j++) c |= (w[j] >> (8 * e) & 0xFF) << (8 * j);
-                if (r < kept || r + 4 > rows) {     // some of the four rows are not new
-                    const uint32_t old = *p;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if (r + j >= kept && r + j < rows) continue;
-                        const int8_t o = (int8_t)(old >> (8 * j));
-                        const uint32_t b = (uint32_t)(uint8_t)(r + j < kept && grew ? requant(o, was, s) : o);
-                        c = (c & ~(0xFFu << (8 * j))) | b << (8 * j);
-                    }
-                }
-                *p = c;
+                const uint32_t o = old[u][e], k = grew && iskept ? pick_bytes(iskept, requant4(o, was, s), o) : o;
+                c[e] = pick_bytes(isnew, c[e], k);
             }
         }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            *(uint32_t *)(codes + rec_at((p0 + r) / KV8_T, a.n_kv, h, hd) + val_at(r % KV8_T, d + e)) = c[e];
     }
 }
 
@@ -147,49 +189,61 @@ extern "C" hipError_t sgk_kv8_store(const float *k, const float *v, uint64_t str
     if (!sgk_kv8_shape_ok(n_kv, hd, block) || ((uintptr_t)codes & 15)) return hipErrorInvalidValue;
     kv8_store_args a = {{k, v}, codes, scales, stride, n_kv, hd, block, base, n};
     const int al = !((uintptr_t)k & 15) && !((uintptr_t)v & 15) && stride % 4 == 0;
-    const uint32_t blocks = (uint32_t)(((uint64_t)base + n + block - 1) / block) - base / block;
-    const dim3 grid(blocks, n_kv, 2);
+    const uint64_t wgs = (((uint64_t)base + n + block - 1) / block - base / block) * n_kv * 2;
+    if (wgs > UINT32_MAX) return hipErrorInvalidValue;
     const uint32_t units = block * hd / 16;
-#define SC(U) hipLaunchKernelGGL(k_kv8_store<U>, grid, dim3(TPB), 0, s, a, al)
-    if (units <= TPB) SC(1);
-    else if (units <= 2 * TPB) SC(2);
-    else if (units <= 4 * TPB) SC(4);
-    else SC(8);
+    for (uint64_t first = 0; first < wgs; first += 1u << 21) {      // a launch has fewer than 2^32 threads
+        const dim3 grid((uint32_t)(wgs - first < 1u << 21 ? wgs - first : 1u << 21));
+#define SC(U, N) hipLaunchKernelGGL((k_kv8_store<U, N>), grid, dim3(N), 0, s, a, (uint32_t)first, al)
+        if (units <= 256) SC(1, 256);
+        else if (units <= 512) SC(2, 256);
+        else if (units <= 1024) SC(2, 512);
+        else SC(2, 1024);
 #undef SC
+    }
     return hipGetLastError();
 }
 
 // ---------------------------------------------------------------------------
-// Load: a workgroup per (tile, kv head, half), a thread per unit as above.
+// Load: hd threads per (tile, kv head, half), whole waves; fours as above.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(TPB) k_kv8_load(const int8_t *codes, const float *scales, float *k, float *v,
                                                   uint64_t stride, uint32_t n_kv, uint32_t hd, uint32_t block,
-                                                  uint32_t base, uint32_t n, int al) {
-    const uint32_t tile = base / KV8_T + blockIdx.x, h = blockIdx.y, half = blockIdx.z, i = threadIdx.x;
-    if (i >= hd) return;                                // 16 hd / 16 units
+                                                  uint32_t base, uint32_t n, uint32_t first, uint32_t halves, int al) {
+    const uint32_t hs = __builtin_ctz(hd), id = first + (blockIdx.x * TPB + threadIdx.x >> hs);
+    if (id >= halves) return;
+    const uint32_t i = threadIdx.x & (hd - 1), half = id & 1, rec = id / 2;
+    const uint32_t tile = base / KV8_T + rec / n_kv, h = rec % n_kv;
     const float s = scales[((size_t)(tile * KV8_T / block) * n_kv + h) * 2 + half];
-    const int8_t *rec = codes + rec_at(tile, n_kv, h, hd) + (size_t)half * KV8_T * hd;
-    const uint64_t p0 = (uint64_t)tile * KV8_T;
-    uint32_t w[4];
+    const int8_t *c = codes + rec_at(tile, n_kv, h, hd) + (size_t)half * KV8_T * hd;
+    float *out = (half ? v : k) + (size_t)h * hd;
+    const uint64_t p0 = (uint64_t)tile * KV8_T, end = (uint64_t)base + n;
+    uint32_t w[4], r[4], d[4];
     if (!half) {
-        const uint32_t r = i % 16, d = i / 16 * 16;
-        const v4u q = *(const v4u *)(rec + key_at(r, d));
-        if (p0 + r < base || p0 + r >= (uint64_t)base + n) return;
-        float *o = k + (size_t)(p0 + r - base) * stride + (size_t)h * hd + d;
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            st4(o + 4 * j, (f32x4){(int8_t)q[j] * s, (int8_t)(q[j] >> 8) * s, (int8_t)(q[j] >> 16) * s, (int8_t)(q[j] >> 24) * s}, al);
-    } else {
-        const uint32_t r = i / (hd / 4) * 4, d = i % (hd / 4) * 4;
-#pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = *(const uint32_t *)(rec + val_at(r, d + e));
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            if (p0 + r + j < base || p0 + r + j >= (uint64_t)base + n) continue;
-            st4(v + (size_t)(p0 + r + j - base) * stride + (size_t)h * hd + d,
-                (f32x4){(int8_t)(w[0] >> (8 * j)) * s, (int8_t)(w[1] >> (8 * j)) * s, (int8_t)(w[2] >> (8 * j)) * s,
-                        (int8_t)(w[3] >> (8 * j)) * s}, al);
+            key_four((i >> 6) + j * (hd / 64), hd, r[j], d[j]);
+            w[j] = *(const uint32_t *)(c + key_at(r[j], d[j]));
         }
+    } else {
+        const uint32_t r0 = i / (hd / 4) * 4, d0 = i % (hd / 4) * 4;
+        uint32_t b[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) b[e] = *(const uint32_t *)(c + val_at(r0, d0 + e));
+        const uint32_t a01 = __builtin_amdgcn_perm(b[1], b[0], 0x05010400u), a23 = __builtin_amdgcn_perm(b[3], b[2], 0x05010400u);
+        const uint32_t b01 = __builtin_amdgcn_perm(b[1], b[0], 0x07030602u), b23 = __builtin_amdgcn_perm(b[3], b[2], 0x07030602u);
+        w[0] = __builtin_amdgcn_perm(a23, a01, 0x05040100u);
+        w[1] = __builtin_amdgcn_perm(a23, a01, 0x07060302u);
+        w[2] = __builtin_amdgcn_perm(b23, b01, 0x05040100u);
+        w[3] = __builtin_amdgcn_perm(b23, b01, 0x07060302u);
+#pragma unroll
+        for (int j = 0; j < 4; j++) { r[j] = r0 + j; d[j] = d0; }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if (p0 + r[j] < base || p0 + r[j] >= end) continue;
+        st4(out + (size_t)(p0 + r[j] - base) * stride + d[j],
+            (f32x4){(int8_t)w[j] * s, (int8_t)(w[j] >> 8) * s, (int8_t)(w[j] >> 16) * s, (int8_t)(w[j] >> 24) * s}, al);
     }
 }
 
@@ -199,7 +253,14 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
     if (!sgk_kv8_shape_ok(n_kv, hd, block) || ((uintptr_t)codes & 15)) return hipErrorInvalidValue;
     const int al = !((uintptr_t)k & 15) && !((uintptr_t)v & 15) && stride % 4 == 0;
     const uint32_t tiles = (uint32_t)(((uint64_t)base + n + KV8_T - 1) / KV8_T) - base / KV8_T;
-    hipLaunchKernelGGL(k_kv8_load, dim3(tiles, n_kv, 2), dim3(TPB), 0, s, codes, scales, k, v, stride, n_kv, hd, block, base, n, al);
+    const uint64_t halves = (uint64_t)tiles * n_kv * 2;
+    const uint32_t most = 1u << 20;         // of a launch: fewer than 2^32 threads
+    if (halves > UINT32_MAX - most) return hipErrorInvalidValue;
+    for (uint64_t first = 0; first < halves; first += most) {
+        const uint64_t m = halves - first < most ? halves - first : most;
+        hipLaunchKernelGGL(k_kv8_load, dim3((uint32_t)((m * hd + TPB - 1) / TPB)), dim3(TPB), 0, s, codes, scales, k, v, stride, n_kv, hd,
+                           block, base, n, (uint32_t)first, (uint32_t)(first + m), al);
+    }
     return hipGetLastError();
 }
 
