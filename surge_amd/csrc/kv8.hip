@@ -210,7 +210,7 @@ extern "C" hipError_t sgk_kv8_store(const float *k, const float *v, uint64_t str
 __global__ void __launch_bounds__(TPB) k_kv8_load(const int8_t *codes, const float *scales, float *k, float *v,
                                                   uint64_t stride, uint32_t n_kv, uint32_t hd, uint32_t block,
                                                   uint32_t base, uint32_t n, uint32_t first, uint32_t halves, int al) {
-    const uint32_t hs = __builtin_ctz(hd), id = first + (blockIdx.x * TPB + threadIdx.x >> hs);
+    const uint32_t hs = __builtin_ctz(hd), id = first + ((blockIdx.x * TPB + threadIdx.x) >> hs);
     if (id >= halves) return;
     const uint32_t i = threadIdx.x & (hd - 1), half = id & 1, rec = id / 2;
     const uint32_t tile = base / KV8_T + rec / n_kv, h = rec % n_kv;
@@ -304,12 +304,10 @@ __device__ __forceinline__ void q_digits(const float (&x)[16], float inv, v4i &d
         d2[w] = (int)(__builtin_amdgcn_perm(d, c, 0x05040100u) ^ 0x80808080u);
     }
 }
-// A row's q (spread over the four lanes of its column) as digits; returns the
-// factor of the integer scores, sq * |mul|, NaN if an element is not finite.
+// A row's q, spread over the four lanes of its column. Asked for before the
+// first keys and values, which would otherwise have to arrive first.
 template <int NC>
-__device__ __forceinline__ float q_row(const float *q, bool on, bool al, uint32_t lg, float mul, v4i (&d)[3][NC]) {
-    float x[NC][16];
-    uint32_t mx = 0;
+__device__ __forceinline__ void q_load(const float *q, bool on, bool al, uint32_t lg, float (&x)[NC][16]) {
 #pragma unroll
     for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -317,11 +315,18 @@ __device__ __forceinline__ float q_row(const float *q, bool on, bool al, uint32_
             f32x4 v = {0.f, 0.f, 0.f, 0.f};
             if (on) v = ld4(q + 64 * c + 16 * lg + 4 * w, al);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                x[c][4 * w + e] = v[e];
-                mx = max(mx, __float_as_uint(v[e]) & 0x7FFFFFFFu);
-            }
+            for (int e = 0; e < 4; e++) x[c][4 * w + e] = v[e];
         }
+}
+// It as digits; returns the factor of the integer scores, sq * |mul|, NaN if an
+// element is not finite.
+template <int NC>
+__device__ __forceinline__ float q_row(float (&x)[NC][16], float mul, v4i (&d)[3][NC]) {
+    uint32_t mx = 0;
+#pragma unroll
+    for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) mx = max(mx, __float_as_uint(x[c][e]) & 0x7FFFFFFFu);
     mx = max(mx, swap16(mx));
     mx = max(mx, swap32(mx));
     const bool bad = mx >= 0x7F800000u;
@@ -440,11 +445,11 @@ __device__ __forceinline__ float softmax_step(float (&x)[UN][4], const float (&f
     return al;
 }
 
-template <int HD>
-__global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part part, int al) {
+template <int HD, int NW>
+__global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part part, int al) {
     constexpr int NC = HD / 64, NT = HD / 16, OLD = HD + 4;
-    __shared__ float wm[4][16], wl[4][16];
-    __shared__ __align__(16) float ob[2][16 * OLD];
+    __shared__ float wm[NW][16], wl[NW][16];
+    __shared__ __align__(16) float ob[NW][16 * OLD];
     const uint32_t t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const uint32_t hk = blockIdx.y, sp = blockIdx.x, S = gridDim.x, G = a.n_heads / a.n_kv;
@@ -486,18 +491,21 @@ __global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part pa
         }
     };
     uint32_t step = s0 + wave;
-    if (step < s1) {
+    const bool any = step < s1;
+    float xq[NC][16];
+    q_load<NC>(a.q + tok * a.q_tok + (size_t)head * a.q_stride, li < R && any, al, lg, xq);
+    if (any) {
         load_s(step);
         load_k(step);
         load_v(step);
     }
     v4i qd[3][NC];
-    const float qf = q_row<NC>(a.q + tok * a.q_tok + (size_t)head * a.q_stride, li < R, al, lg, a.scale * 1.44269504088896340736f, qd);
+    const float qf = q_row<NC>(xq, a.scale * 1.44269504088896340736f, qd);
     f32x4 o[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) o[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     float mrun = -INFINITY, lsum = 0.0f;
-    for (; step < s1; step += 4) {
+    for (; step < s1; step += NW) {
         float sc[2][4];
 #pragma unroll
         for (int u = 0; u < 2; u++) { ks[u] = nks[u]; vs[u] = nvs[u]; }
@@ -512,8 +520,8 @@ __global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part pa
 #pragma unroll
             for (int e = 0; e < 4; e++) sc[u][e] = q_join(s[0][e], s[1][e], s[2][e]);
         }
-        const bool more = step + 4 < s1;
-        if (more) { load_s(step + 4); load_k(step + 4); }
+        const bool more = step + NW < s1;
+        if (more) { load_s(step + NW); load_k(step + NW); }
         f16x8 ph[1], pl[1];
         const float f[2] = {qf * ks[0], qf * ks[1]};
         const bool usual = step * 32 + 31 <= first && scales_usual(fminf(ks[0], ks[1]), fminf(vs[0], vs[1]));
@@ -531,36 +539,29 @@ __global__ void __launch_bounds__(TPB, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part pa
                 o[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[0], o[4 * c + j], 0, 0, 0);
                 o[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[0], o[4 * c + j], 0, 0, 0);
             }
-        if (more) load_v(step + 4);
+        if (more) load_v(step + NW);
     }
-    // join the four waves: maxima and sums first, then outputs 2 + 0, 3 + 1, both
+    // join the waves that had a step: each leaves its maximum, sum and output, one barrier
+    const uint32_t waves = min(s1 - s0, (uint32_t)NW);
     lsum += swap16f(lsum);
     lsum += swap32f(lsum);
-    if (lg == 0) { wm[wave][li] = mrun; wl[wave][li] = lsum; }
-    __syncthreads();
-    const float M = fmaxf(fmaxf(wm[0][li], wm[1][li]), fmaxf(wm[2][li], wm[3][li]));
-    const float f = mrun == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrun - M);
+    if (any && li < R) {
+        if (lg == 0) { wm[wave][li] = mrun; wl[wave][li] = lsum; }
+        float *dst = &ob[wave][li * OLD + 4 * lg];
 #pragma unroll
-    for (int n = 0; n < NT; n++) o[n] *= f;
-    float *mine = &ob[wave & 1][li * OLD + 4 * lg];
-    if (wave >= 2) {
-#pragma unroll
-        for (int n = 0; n < NT; n++) *(f32x4 *)(mine + 16 * n) = o[n];
+        for (int n = 0; n < NT; n++) *(f32x4 *)(dst + 16 * n) = o[n];
     }
     __syncthreads();
-    if (wave < 2) {
-#pragma unroll
-        for (int n = 0; n < NT; n++) *(f32x4 *)(mine + 16 * n) += o[n];
-    }
-    __syncthreads();
-    for (uint32_t i = t; i < R * (HD / 4); i += TPB) {
+    for (uint32_t i = t; i < R * (HD / 4); i += NW * 64) {
         const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
-        const f32x4 v = *(const f32x4 *)&ob[0][r * OLD + d] + *(const f32x4 *)&ob[1][r * OLD + d];
-        const float m = fmaxf(fmaxf(wm[0][r], wm[1][r]), fmaxf(wm[2][r], wm[3][r]));
-        float l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < 4; w++)
-            l += wl[w][r] * (wm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wm[w][r] - m));
+        float m = -INFINITY, l = 0.0f;
+        for (uint32_t w = 0; w < waves; w++) m = fmaxf(m, wm[w][r]);
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t w = 0; w < waves; w++) {
+            const float f = wm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wm[w][r] - m);
+            l = fmaf(wl[w][r], f, l);
+            v += *(const f32x4 *)&ob[w][r * OLD + d] * f;
+        }
         const size_t row = (size_t)((r0 + r) / G) * a.n_heads + hk * G + (r0 + r) % G;
         if (S == 1) {
             st4(a.out + row * HD + d, v / l, !((uintptr_t)a.out & 15));
@@ -666,11 +667,13 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
         }
     };
 
-    if (n) { load(0, true, false); load_s(0); }
     const uint64_t r = r0 + wave * 16 + li, rw = r0 + wave * 16;
     const uint32_t tok = r < R ? (uint32_t)r / G : 0, head = hk * G + (r < R ? (uint32_t)r % G : 0), rpos = a.base + tok;
+    float xq[NC][16];
+    q_load<NC>(a.q + tok * a.q_tok + (size_t)head * a.q_stride, r < R, al, lg, xq);
+    if (n) { load(0, true, false); load_s(0); }
     v4i qd[3][NC];
-    const float qf = q_row<NC>(a.q + tok * a.q_tok + (size_t)head * a.q_stride, r < R, al, lg, a.scale * 1.44269504088896340736f, qd);
+    const float qf = q_row<NC>(xq, a.scale * 1.44269504088896340736f, qd);
     float mrun = -INFINITY, lsum = 0.0f, resc = 1.0f;
     f32x4 o[NT];
 #pragma unroll
@@ -817,8 +820,14 @@ __global__ void __launch_bounds__(TPB) k_kv8_join(kv8_part p, float *out, uint64
     st4(out + row * HD + d, o / sum, al);
 }
 
-// How a call runs. The wave form: small calls, in as many key splits as give
-// every wave a step, up to two workgroups per CU (what is resident). Else row
+// How a call runs. The wave form, small calls: workgroups of eight waves, one a
+// CU (two at head_dim 64), where their waves get more than a step of 32 keys
+// each and there are not more workgroups than that without a split; else of
+// four, a step to each wave (whole call, us, eight / four waves:
+// 24 heads of 256 on 4, 32771 keys 31.4 / 33.5, 700 keys 24.3 / 22.7; 32 of 128
+// on 8, 262000 keys 98.6 / 105, 5000 keys 22.6 / 22.2), and one workgroup alone
+// up to KV8_ONE steps a wave, where a second launch to join costs more (300
+// keys, one / split: head_dim 256 21.5 / 21.7, 64 18.0 / 18.8). Else row
 // blocks in tiles, one workgroup per CU at a time, their keys split where that
 // shortens the launch: rounds x (a part's tiles + KV8_TAIL for its start and
 // end) tiles of KV8_TILE_US, against the partials' way to memory and back.
@@ -828,19 +837,23 @@ __global__ void __launch_bounds__(TPB) k_kv8_join(kv8_part p, float *out, uint64
 // 47.9 / 65.5; 32 of 128 on 8, 8020 keys, 80 rows (1.3M) 32.2 / 36.0, 8077 keys,
 // 308 rows (5.2M) 58.1 / 55.0; 12 of 64, 32077 keys, 77 rows (3.9M) 59.5 / 60.5.
 #define KV8_SMALL (1ull << 22)
+#define KV8_ONE 3
 #define KV8_TILE_US 2.5         /* at head_dim 256 */
 #define KV8_TAIL 3.0
 #define KV8_PART_BYTES (256ull << 20)
-struct kv8_plan { bool wave; uint32_t splits, blocks; };
+struct kv8_plan { uint32_t waves, splits, blocks; };     // waves: of a workgroup of the wave form, 0 for tiles
 static kv8_plan kv8_plan_of(const sgk_kv8_attn *a) {
     const uint64_t G = a->n_heads / a->n_kv, rows = a->ntok * G, keys = (uint64_t)a->base + a->ntok, cus = sgk_device_cus();
     const bool wave = rows <= 16 || (rows + 15) / 16 * a->n_kv * ((keys + 31) / 32) * a->hd <= KV8_SMALL;
     const uint64_t per = wave ? 16 : KV8_ROWS, wgs = (rows + per - 1) / per * a->n_kv;
-    kv8_plan p = {wave, 1, (uint32_t)((rows + per - 1) / per)};
-    if (p.wave) {
-        uint64_t most = 2 * cus / wgs, want = (keys + 127) / 128;
-        if (most > 1024) most = 1024;
+    kv8_plan p = {wave ? 4u : 0u, 1, (uint32_t)((rows + per - 1) / per)};
+    if (wave) {
+        const uint64_t steps = (keys + 31) / 32;
+        uint64_t most = (a->hd == 64 ? 2 : 1) * cus / wgs;
+        if (most > 512) most = 512;
+        if (most && steps > 8 * most) { p.waves = 8; p.splits = (uint32_t)most; return p; }
         if (most < 1) most = 1;
+        const uint64_t want = steps <= KV8_ONE * 4 ? 1 : (steps + 3) / 4;
         p.splits = (uint32_t)(want < most ? want : most);
         return p;
     }
@@ -876,9 +889,11 @@ extern "C" hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hi
         part.m = part.acc + rows * a->hd;
         part.s = part.m + rows;
     }
+    const dim3 wgrid(p.splits, a->n_kv, p.blocks);
 #define KC(H)                                                                                                                 \
     do {                                                                                                                      \
-        if (p.wave) hipLaunchKernelGGL(k_kv8_wave<H>, dim3(p.splits, a->n_kv, p.blocks), dim3(TPB), 0, s, *a, part, al);      \
+        if (p.waves == 8) hipLaunchKernelGGL((k_kv8_wave<H, 8>), wgrid, dim3(512), 0, s, *a, part, al);                        \
+        else if (p.waves) hipLaunchKernelGGL((k_kv8_wave<H, 4>), wgrid, dim3(256), 0, s, *a, part, al);                       \
         else hipLaunchKernelGGL(k_kv8_tile<H>, dim3(p.blocks, a->n_kv, p.splits), dim3(KV8_NW * 64), 0, s, *a, part, al);     \
     } while (0)
     switch (a->hd) {

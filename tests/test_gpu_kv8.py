@@ -207,6 +207,20 @@ def test_decode_long(gpu, nh, nkv, hd, seq, block):
     assert np.array_equal(got, attend(gpu, c, q, seq - 1, 1 / math.sqrt(hd), "decode"))
 
 
+@pytest.mark.parametrize("nh,nkv,hd,block,base,n", [
+    (24, 4, 256, 64, 17003, 1), (32, 8, 128, 16, 9003, 1), (12, 12, 64, 32, 11999, 1), (24, 4, 256, 32, 11990, 5),
+    (16, 8, 128, 128, 9000, 9), (64, 64, 64, 64, 2100, 3)])
+def test_few_rows_deep(gpu, nh, nkv, hd, block, base, n):
+    """Workgroups of eight waves, whose waves take several steps each."""
+    rng = np.random.default_rng(base)
+    c = filled(rng, nkv, hd, block, base + n)
+    q = rng.standard_normal((n, nh, hd)).astype(np.float32)
+    want, bound = K.attention(q, c, base, 1 / math.sqrt(hd))
+    got = attend(gpu, c, q, base, 1 / math.sqrt(hd), "decode" if n == 1 else "prefill")
+    close(got, want, bound)
+    assert np.array_equal(got, attend(gpu, c, q, base, 1 / math.sqrt(hd), "decode" if n == 1 else "prefill"))
+
+
 @pytest.mark.parametrize("nh,nkv,hd,block", [(8, 2, 256, 32), (6, 1, 64, 16), (16, 1, 128, 64), (4, 4, 128, 128), (10, 2, 64, 32)])
 @pytest.mark.parametrize("base,n", [(0, 1), (0, 2), (0, 17), (3, 5), (31, 33), (64, 64), (100, 77), (257, 130), (1000, 3)])
 def test_prefill(gpu, nh, nkv, hd, block, base, n):
