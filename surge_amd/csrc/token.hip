@@ -149,46 +149,54 @@ __global__ void __launch_bounds__(TPB) k_token_counts(const int32_t *ids, uint32
         }
 }
 
-// Counts from nothing: a workgroup owns TR_IDS ids of a row, reads the row's
-// whole history and counts its own in LDS, so there is nothing to clear first
-// and no addition to memory.
+// Up to TR_MOST ids a row: a workgroup owns TR_IDS ids of the vocabulary, reads
+// the row's whole history and counts its own in LDS, alike neighbours of a
+// thread at once, so nothing is cleared first and no two additions meet in
+// memory. Whole call, us, 151936 ids, Zipf's law with exponent 1.2 / one id
+// only, against the table form: 900 ids of 1 row 14.1 / 14.0, 18.5 / 18.6;
+// 32000 of 1 row 18.5 / 17.1, 22.2 / 20.5; 131072 of 16 rows 44 / 32, 104 / 33;
+// 262144 of 1 row 55 / 50, 56 / 22. Past TR_MOST the walk over the history
+// decides, and the table form spreads that.
 #define TR_IDS 8192u
-// A row's history up to which this form runs (whole call, 151936 ids, Zipf's
-// law with exponent 1.2 / one id only): 900 ids of 1 row 15.3 / 15.1 us, the
-// table form 18.5 / 18.6; 32000 of 1 row 22.9 / 41.5, table 22.2 / 20.5; 32000
-// of 16 rows 24.7 / 49.1, table 30.0 / 21.5. Past it the longest part's walk
-// over the history decides, and the table form spreads that.
-#define TR_MOST 32768u
-__global__ void __launch_bounds__(TPB) k_token_recount(const int32_t *ids, uint32_t *counts, uint32_t n, uint32_t vocab, uint32_t rows) {
+#define TR_THREADS 1024
+#define TR_U 8u
+#define TR_MOST 131072u
+__global__ void __launch_bounds__(TR_THREADS) k_token_recount(const int32_t *ids, uint32_t *counts, uint32_t n, uint32_t vocab, int clear) {
     __shared__ uint32_t num[TR_IDS];
     const uint32_t t = threadIdx.x, v0 = blockIdx.x * TR_IDS, nv = min(TR_IDS, vocab - v0);
-    for (uint32_t r = blockIdx.y; r < rows; r += gridDim.y) {
-        for (uint32_t i = t; i < nv; i += TPB) num[i] = 0;
-        __syncthreads();
-        const int32_t *row = ids + (uint64_t)r * n;
-        constexpr uint32_t U = 8;
-        for (uint32_t i0 = 0; i0 < n; i0 += U * TPB) {
-            uint32_t id[U];
+    const uint32_t r = blockIdx.y;
+    for (uint32_t i = t; i < nv; i += TR_THREADS) num[i] = 0;
+    __syncthreads();
+    const int32_t *row = ids + (uint64_t)r * n;
+    constexpr uint32_t U = TR_U;
+    for (uint32_t i0 = 0; i0 < n; i0 += U * TR_THREADS) {
+        uint32_t id[U];
 #pragma unroll
-            for (uint32_t x = 0; x < U; x++) {
-                const uint32_t i = i0 + x * TPB + t;
-                id[x] = i < n ? (uint32_t)row[i] : 0xFFFFFFFFu;
-            }
-#pragma unroll
-            for (uint32_t x = 0; x < U; x++)
-                if (id[x] - v0 < nv) atomicAdd(&num[id[x] - v0], 1u);
+        for (uint32_t x = 0; x < U; x++) {
+            const uint32_t i = i0 + x * TR_THREADS + t;
+            id[x] = i < n ? (uint32_t)row[i] : 0xFFFFFFFFu;
         }
-        __syncthreads();
-        for (uint32_t i = t; i < nv; i += TPB) counts[(uint64_t)r * vocab + v0 + i] = num[i];
-        __syncthreads();
+        uint32_t c = 1;         // of id[x] so far: alike neighbours are added once
+#pragma unroll
+        for (uint32_t x = 0; x < U; x++) {
+            if (x + 1 < U && id[x] == id[x + 1]) { c++; continue; }
+            if (id[x] - v0 < nv) atomicAdd(&num[id[x] - v0], c);
+            c = 1;
+        }
+    }
+    __syncthreads();
+    uint32_t *out = counts + (uint64_t)r * vocab + v0;
+    for (uint32_t i = t; i < nv; i += TR_THREADS) {
+        if (clear) out[i] = num[i];
+        else if (num[i]) out[i] += num[i];
     }
 }
 
 extern "C" hipError_t sgk_token_counts(const int32_t *ids, uint32_t *counts, uint32_t n, uint32_t vocab, uint32_t rows,
                                        int clear, hipStream_t s) {
     if (!vocab || !rows) return hipSuccess;
-    if (clear && n && n <= TR_MOST) {
-        hipLaunchKernelGGL(k_token_recount, dim3((vocab + TR_IDS - 1) / TR_IDS, rows), dim3(TPB), 0, s, ids, counts, n, vocab, rows);
+    if (n && n <= TR_MOST) {
+        hipLaunchKernelGGL(k_token_recount, dim3((vocab + TR_IDS - 1) / TR_IDS, rows), dim3(TR_THREADS), 0, s, ids, counts, n, vocab, clear);
         return hipGetLastError();
     }
     if (clear) {
@@ -211,7 +219,7 @@ extern "C" hipError_t sgk_token_counts(const int32_t *ids, uint32_t *counts, uin
 // A thread takes four neighbouring ids a step, 16 bytes of each input where
 // addresses allow. Bound by memory for many rows, by the launches for one.
 // ---------------------------------------------------------------------------
-#define LG_PARTS 256u       // parts of all rows together that fill the chip; a row has at least one
+#define LG_WGS 3072u         // workgroups of all rows together, at most; a row has at least one
 struct lg_best { float v; uint32_t i; };
 #define LG_NONE 0xFFFFFFFFu
 
@@ -291,7 +299,7 @@ __global__ void __launch_bounds__(TPB) k_logits_token(const lg_best *part, uint3
 
 // parts of a row: one per 4 TPB ids, until the rows together fill the chip a few times
 static uint32_t lg_parts(uint32_t vocab, uint32_t rows) {
-    const uint32_t need = (uint32_t)(((uint64_t)vocab + 4 * TPB - 1) / (4 * TPB)), most = max(1u, 4 * LG_PARTS / rows);
+    const uint32_t need = (uint32_t)(((uint64_t)vocab + 4 * TPB - 1) / (4 * TPB)), most = max(1u, LG_WGS / rows);
     return min(min(need, most), (uint32_t)TPB);
 }
 extern "C" uint64_t sgk_logits_part_bytes(uint32_t vocab, uint32_t rows) { return (uint64_t)rows * lg_parts(vocab, rows) * sizeof(lg_best); }
