@@ -53,15 +53,14 @@ __device__ __forceinline__ void key_four(uint32_t c, uint32_t hd, uint32_t &r, u
 // x - q s, exact in one fma, decides. Clamped for a scale near the end of the
 // range, whose rounding may leave |x / s| above 127.
 __device__ __forceinline__ uint32_t quant4(f32x4 x, float s, float inv) {
-    float q[4];
-    bool close = false;
+    float q[4], far = 0.0f;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         const float t = x[e] * inv;
         q[e] = rintf(t);
-        close |= !(fabsf(t - q[e]) < 0.4999f);
+        far = fmaxf(far, fabsf(t - q[e]));
     }
-    if (close) {
+    if (!(far < 0.4999f)) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const float r = fmaf(-q[e], s, x[e]), a = 2.0f * fabsf(r);
@@ -69,10 +68,9 @@ __device__ __forceinline__ uint32_t quant4(f32x4 x, float s, float inv) {
             q[e] = fminf(fmaxf(q[e], -127.0f), 127.0f);
         }
     }
-    uint32_t w = 0;
-#pragma unroll
-    for (int e = 0; e < 4; e++) w |= (uint32_t)((int)q[e] & 0xFF) << (8 * e);
-    return w;
+    const uint32_t lo = __builtin_amdgcn_perm((uint32_t)(int)q[1], (uint32_t)(int)q[0], 0x0C0C0400u);
+    const uint32_t hi = __builtin_amdgcn_perm((uint32_t)(int)q[3], (uint32_t)(int)q[2], 0x0C0C0400u);
+    return lo | hi << 16;
 }
 __device__ __forceinline__ uint32_t requant4(uint32_t c, double was, double s) {
     uint32_t w = 0;
@@ -138,9 +136,11 @@ __global__ void __launch_bounds__(NTH, 4) k_kv8_store(kv8_store_args a, uint32_t
     // a scale near the end of the range: x / s is the same for both times 2^64
     const float up = s < 0x1p-60f ? 0x1p64f : 1.0f, sq = s * up, inv = s > 0.0f ? 1.0f / sq : 0.0f;
     const bool zero = poison || s == 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4 * U; i++) v[i] = zero ? (f32x4){0.f, 0.f, 0.f, 0.f} : v[i] * up;
     const float sz = zero ? 1.0f : sq;
+    if (zero || up != 1.0f) {
+#pragma unroll
+        for (int i = 0; i < 4 * U; i++) v[i] = zero ? (f32x4){0.f, 0.f, 0.f, 0.f} : v[i] * up;
+    }
     if (!half) {
 #pragma unroll
         for (int i = 0; i < 4 * U; i++) {
