@@ -134,6 +134,8 @@ struct sg_gpu {
     int attn_arm;
     uint64_t n_per_head, n_gqa, n_online;
 
+    hipEvent_t done;        /* of the last kernel of a call that waits for that kernel (finish_done) */
+
     /* one-shot scratch */
     void *tmp;
     uint64_t tmp_bytes;
@@ -217,6 +219,11 @@ sg_err sg_gpu_init(sg_gpu **out) {
         free(g);
         return (sg_err){"gpu: hipStreamCreate failed"};
     }
+    if (hipEventCreateWithFlags(&g->done, hipEventDisableTiming) != hipSuccess) {
+        hipStreamDestroy(g->stream);
+        free(g);
+        return (sg_err){"gpu: hipEventCreate failed"};
+    }
     const char *ev = getenv("SURGE_HIP_GRAPH");
     g->use_graph = !(ev && strcmp(ev, "0") == 0);
     g->attn_splitk = g->attn_gqa = true;       /* the defaults until a state reads the environment */
@@ -237,6 +244,7 @@ void sg_gpu_free(sg_gpu *g) {
     model_free(g);
     while (g->n_allocs) dfree(g, g->allocs[g->n_allocs - 1].p);
     free(g->allocs);
+    hipEventDestroy(g->done);
     hipStreamDestroy(g->stream);
     free(g);
 }
@@ -883,6 +891,21 @@ static sg_err on_device(const sg_gpu *g, int *was) {
     if (*was != g->dev) HIPCHK(hipSetDevice(g->dev), "hipSetDevice");
     return SG_OK;
 }
+/* finish() for calls whose launcher took g->done: waits for the last kernel
+ * itself, not for a packet behind it. */
+static sg_err finish_done(sg_gpu *g, hipError_t launch, void *const *outs, int n) {
+    if (launch != hipSuccess) {
+        hipStreamSynchronize(g->stream);        /* what was launched before the failure */
+        return errf("gpu: kernel launch failed: %s", hipGetErrorString(launch));
+    }
+    HIPCHK(hipEventSynchronize(g->done), "kernel execution");
+    for (int i = 0; i < n; i++) {
+        if (!outs[i]) continue;
+        sg_err e = sg_gpu_buf_download(outs[i]);
+        if (sg_failed(e)) return e;
+    }
+    return SG_OK;
+}
 static sg_err back_to(const sg_gpu *g, int was, sg_err e) {
     if (was != g->dev && hipSetDevice(was) != hipSuccess && !sg_failed(e)) return (sg_err){"gpu: hipSetDevice failed"};
     return e;
@@ -937,8 +960,8 @@ sg_err sg_gpu_run_kv8_store(sg_gpu *g, void *k, void *v, void *codes, void *scal
     if (sg_failed(e = on_device(g, &was))) return e;
     void *ins[4] = {k, v, codes, scales};
     if (!sg_failed(e = push(ins, 4)))
-        e = finish(g, sgk_kv8_store(DEV(k), DEV(v), stride, DEV(codes), DEV(scales), p[0], p[1], p[2], p[3], p[4], g->stream),
-                   ins + 2, 2);
+        e = finish_done(g, sgk_kv8_store(DEV(k), DEV(v), stride, DEV(codes), DEV(scales), p[0], p[1], p[2], p[3], p[4], g->stream, g->done),
+                        ins + 2, 2);
     return back_to(g, was, e);
 }
 
@@ -956,8 +979,8 @@ sg_err sg_gpu_run_kv8_load(sg_gpu *g, void *codes, void *scales, void *k, void *
     if (sg_failed(e = on_device(g, &was))) return e;
     void *bufs[4] = {codes, scales, k, v};
     if (!sg_failed(e = push(bufs, 4)))
-        e = finish(g, sgk_kv8_load(DEV(codes), DEV(scales), DEV(k), DEV(v), stride, p[0], p[1], p[2], p[3], p[4], g->stream),
-                   bufs + 2, 2);
+        e = finish_done(g, sgk_kv8_load(DEV(codes), DEV(scales), DEV(k), DEV(v), stride, p[0], p[1], p[2], p[3], p[4], g->stream, g->done),
+                        bufs + 2, 2);
     return back_to(g, was, e);
 }
 
@@ -985,7 +1008,7 @@ static sg_err attn_kv8_oneshot(sg_gpu *g, const char *who, void *q, void *codes,
                                     (uint64_t)nh * qs, fbits(scale)};
             const uint64_t bytes = sgk_kv8_attn_scratch(&a);
             void *t = NULL;
-            if (!bytes || !sg_failed(e = scratch(g, bytes, &t))) e = finish(g, sgk_kv8_attention(&a, t, g->stream), outs, 1);
+            if (!bytes || !sg_failed(e = scratch(g, bytes, &t))) e = finish_done(g, sgk_kv8_attention(&a, t, g->stream, g->done), outs, 1);
         }
     }
     return back_to(g, was, e);
@@ -1036,7 +1059,7 @@ sg_err sg_gpu_run_rope_axes(sg_gpu *g, void *x, void *pos, void *out, const uint
     void *ins[3] = {x, pos, out}, *outs[1] = {out};     /* out too: its gaps stay as they are */
     if (!sg_failed(e = push(ins, out == x ? 2 : 3))) {
         const sgk_rope_axes_args a = {DEV(x), DEV(pos), DEV(out), row, hd, rd, nh, hs, n};
-        e = finish(g, sgk_rope_axes(&a, inv, axis, g->stream), outs, 1);
+        e = finish_done(g, sgk_rope_axes(&a, inv, axis, g->stream, g->done), outs, 1);
     }
     return back_to(g, was, e);
 }
@@ -1055,7 +1078,7 @@ sg_err sg_gpu_run_token_counts(sg_gpu *g, void *ids, void *counts, const uint32_
     if (sg_failed(e = on_device(g, &was))) return e;
     void *bufs[2] = {counts, n ? ids : NULL};
     if (!sg_failed(e = push(bufs, 2)))
-        e = finish(g, sgk_token_counts(n ? DEV(ids) : NULL, DEV(counts), n, vocab, rows, p[3] != 0, g->stream), bufs, 1);
+        e = !n && !p[3] ? SG_OK : finish_done(g, sgk_token_counts(n ? DEV(ids) : NULL, DEV(counts), n, vocab, rows, p[3] != 0, g->stream, g->done), bufs, 1);
     return back_to(g, was, e);
 }
 
@@ -1085,7 +1108,7 @@ sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void
     void *part;
     if (!sg_failed(e = scratch(g, sgk_logits_part_bytes(vocab, rows), &part)) && !sg_failed(e = push(bufs, 4))) {
         const sgk_logits_args a = {DEV(logits), DEV(counts), DEV(bias), DEV(mask), DEV(out), DEV(token), vocab, rows, rep, freq, pres};
-        e = finish(g, sgk_logits(&a, part, g->stream), outs, 2);
+        e = finish_done(g, sgk_logits(&a, part, g->stream, g->done), outs, 2);
     }
     return back_to(g, was, e);
 }

@@ -371,7 +371,9 @@ uint32_t sgk_device_cus(void);
 hipError_t sgk_read(const void *p, uint64_t bytes, float *out, uint32_t blocks, hipStream_t s);
 hipError_t sgk_empty(hipStream_t s);
 
-/* The 8-bit K/V cache (kv8.hip): codes int8 [tile of 16][n_kv][2][16 hd] in the
+/* Below, `done` (or NULL) becomes the event of the last kernel's completion.
+ *
+ * The 8-bit K/V cache (kv8.hip): codes int8 [tile of 16][n_kv][2][16 hd] in the
  * matrix instructions' orders, scales f32 [position / block][n_kv][2]; see
  * surge.h for the layout and the quantiser. */
 #define SGK_KV8_TILE 16u
@@ -379,9 +381,9 @@ SGK_HD static inline int sgk_kv8_shape_ok(uint32_t n_kv, uint32_t hd, uint32_t b
     return n_kv && (hd == 64 || hd == 128 || hd == 256) && (block == 16 || block == 32 || block == 64 || block == 128);
 }
 hipError_t sgk_kv8_store(const float *k, const float *v, uint64_t stride, int8_t *codes, float *scales, uint32_t n_kv,
-                         uint32_t hd, uint32_t block, uint32_t base, uint32_t n, hipStream_t s);
+                         uint32_t hd, uint32_t block, uint32_t base, uint32_t n, hipStream_t s, hipEvent_t done);
 hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, float *k, float *v, uint64_t stride, uint32_t n_kv,
-                        uint32_t hd, uint32_t block, uint32_t base, uint32_t n, hipStream_t s);
+                        uint32_t hd, uint32_t block, uint32_t base, uint32_t n, hipStream_t s, hipEvent_t done);
 /* Causal attention of ntok tokens at positions base .. base+ntok-1 over the
  * cache; token z's head h at q + z*q_tok + h*q_stride, out [ntok][n_heads][hd]. */
 typedef struct {
@@ -396,7 +398,7 @@ typedef struct {
 #define SGK_KV8_MAX_GROUP 16u       /* query heads per kv head */
 /* scratch: sgk_kv8_attn_scratch(a) bytes, 16-byte aligned (NULL if that is 0). */
 uint64_t sgk_kv8_attn_scratch(const sgk_kv8_attn *a);
-hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hipStream_t s);
+hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hipStream_t s, hipEvent_t done);
 
 /* Rotary positions with three axes (token.hip). inv and axis: rope_dim/2
  * inverse frequencies and axes (host memory, read before return). */
@@ -407,11 +409,12 @@ typedef struct {
     uint64_t row;               /* floats between tokens */
     uint32_t head_dim, rope_dim, heads, stride, n;
 } sgk_rope_axes_args;
-hipError_t sgk_rope_axes(const sgk_rope_axes_args *a, const double *inv, const uint8_t *axis, hipStream_t s);
+hipError_t sgk_rope_axes(const sgk_rope_axes_args *a, const double *inv, const uint8_t *axis, hipStream_t s, hipEvent_t done);
 
-/* counts[row][id] += occurrences; cleared first with clear != 0. */
+/* counts[row][id] += occurrences; cleared first with clear != 0 (n == 0 without
+ * it is refused). */
 hipError_t sgk_token_counts(const int32_t *ids, uint32_t *counts, uint32_t n, uint32_t vocab, uint32_t rows, int clear,
-                            hipStream_t s);
+                            hipStream_t s, hipEvent_t done);
 typedef struct {
     const float *x;
     const uint32_t *counts;     /* or NULL */
@@ -424,7 +427,7 @@ typedef struct {
 } sgk_logits_args;
 /* part: scratch of sgk_logits_part_bytes(vocab, rows). */
 uint64_t sgk_logits_part_bytes(uint32_t vocab, uint32_t rows);
-hipError_t sgk_logits(const sgk_logits_args *a, void *part, hipStream_t s);
+hipError_t sgk_logits(const sgk_logits_args *a, void *part, hipStream_t s, hipEvent_t done);
 
 /* The device-resident workspace of the no-allocation entry points: a
  * file-scope device array of SGK_SCRATCH_BYTES in kernels.hip. Call

@@ -184,7 +184,8 @@ __global__ void __launch_bounds__(NTH, 4) k_kv8_store(kv8_store_args a, uint32_t
 }
 
 extern "C" hipError_t sgk_kv8_store(const float *k, const float *v, uint64_t stride, int8_t *codes, float *scales,
-                                    uint32_t n_kv, uint32_t hd, uint32_t block, uint32_t base, uint32_t n, hipStream_t s) {
+                                    uint32_t n_kv, uint32_t hd, uint32_t block, uint32_t base, uint32_t n, hipStream_t s,
+                                    hipEvent_t done) {
     if (!n) return hipSuccess;
     if (!sgk_kv8_shape_ok(n_kv, hd, block) || ((uintptr_t)codes & 15)) return hipErrorInvalidValue;
     kv8_store_args a = {{k, v}, codes, scales, stride, n_kv, hd, block, base, n};
@@ -194,7 +195,8 @@ extern "C" hipError_t sgk_kv8_store(const float *k, const float *v, uint64_t str
     const uint32_t units = block * hd / 16;
     for (uint64_t first = 0; first < wgs; first += 1u << 21) {      // a launch has fewer than 2^32 threads
         const dim3 grid((uint32_t)(wgs - first < 1u << 21 ? wgs - first : 1u << 21));
-#define SC(U, N) hipLaunchKernelGGL((k_kv8_store<U, N>), grid, dim3(N), 0, s, a, (uint32_t)first, al)
+        const hipEvent_t ev = first + (1u << 21) < wgs ? NULL : done;
+#define SC(U, N) launch(k_kv8_store<U, N>, grid, N, s, ev, a, (uint32_t)first, al)
         if (units <= 256) SC(1, 256);
         else if (units <= 512) SC(2, 256);
         else if (units <= 1024) SC(2, 512);
@@ -248,7 +250,8 @@ __global__ void __launch_bounds__(TPB) k_kv8_load(const int8_t *codes, const flo
 }
 
 extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, float *k, float *v, uint64_t stride,
-                                   uint32_t n_kv, uint32_t hd, uint32_t block, uint32_t base, uint32_t n, hipStream_t s) {
+                                   uint32_t n_kv, uint32_t hd, uint32_t block, uint32_t base, uint32_t n, hipStream_t s,
+                                   hipEvent_t done) {
     if (!n) return hipSuccess;
     if (!sgk_kv8_shape_ok(n_kv, hd, block) || ((uintptr_t)codes & 15)) return hipErrorInvalidValue;
     const int al = !((uintptr_t)k & 15) && !((uintptr_t)v & 15) && stride % 4 == 0;
@@ -258,8 +261,8 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
     if (halves > UINT32_MAX - most) return hipErrorInvalidValue;
     for (uint64_t first = 0; first < halves; first += most) {
         const uint64_t m = halves - first < most ? halves - first : most;
-        hipLaunchKernelGGL(k_kv8_load, dim3((uint32_t)((m * hd + TPB - 1) / TPB)), dim3(TPB), 0, s, codes, scales, k, v, stride, n_kv, hd,
-                           block, base, n, (uint32_t)first, (uint32_t)(first + m), al);
+        launch(k_kv8_load, dim3((uint32_t)((m * hd + TPB - 1) / TPB)), TPB, s, first + most < halves ? NULL : done, codes, scales, k, v,
+               stride, n_kv, hd, block, base, n, (uint32_t)first, (uint32_t)(first + m), al);
     }
     return hipGetLastError();
 }
@@ -567,8 +570,8 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
             st4(a.out + row * HD + d, v / l, !((uintptr_t)a.out & 15));
         } else {
             *(f32x4 *)(part.acc + (row * S + sp) * HD + d) = v;
-            // base e for the combine; a sum that is NaN has to reach it whatever the maximum
-            if (d == 0) { part.m[row * S + sp] = l != l ? 0.0f : m * 0.69314718055994530942f; part.s[row * S + sp] = l; }
+            // a sum that is NaN has to reach the join whatever the maximum
+            if (d == 0) { part.m[row * S + sp] = l != l ? 0.0f : m; part.s[row * S + sp] = l; }
         }
     }
 }
@@ -784,15 +787,14 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
         float *acc = part.acc + (row * S + sp) * HD + 4 * lg;
 #pragma unroll
         for (int d = 0; d < NT; d++) *(f32x4 *)(acc + 16 * d) = o[d];
-        if (lg == 0) { part.m[row * S + sp] = l != l ? 0.0f : mrun * 0.69314718055994530942f; part.s[row * S + sp] = l; }
+        if (lg == 0) { part.m[row * S + sp] = l != l ? 0.0f : mrun; part.s[row * S + sp] = l; }
     }
 }
 
 // Join of few splits of many rows: four dims of a row per lane, all splits'
-// loads in flight, nothing shared between lanes. (k_attn_combine, a workgroup
-// per row, joins many splits of few rows.) A row's first maximum is the
-// smallest that any split may have, so a split without a visible key has
-// weight zero; NaN sums reach the output.
+// loads in flight, nothing shared between lanes. A row's first split sees a
+// key, so the largest maximum is a number and a split without a key weighs
+// nothing; NaN sums reach the output.
 #define KV8_JOIN 8u
 template <int HD>
 __global__ void __launch_bounds__(TPB) k_kv8_join(kv8_part p, float *out, uint64_t rows, uint32_t S, int al) {
@@ -813,11 +815,61 @@ __global__ void __launch_bounds__(TPB) k_kv8_join(kv8_part p, float *out, uint64
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (uint32_t k = 0; k < KV8_JOIN; k++) {
-        const float w = m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[k] - M) * 1.44269504088896340736f);
+        const float w = m[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[k] - M);
         sum = fmaf(l[k], w, sum);
         o += acc[k] * w;
     }
     st4(out + row * HD + d, o / sum, al);
+}
+
+// Join of many splits of few rows: a workgroup per row and 64 dims, 16 lanes of
+// four dims for every 16th split; the first four splits of a lane are asked
+// for before the weights.
+#define KV8_COMB 512u
+__global__ void __launch_bounds__(TPB) k_kv8_comb(kv8_part p, float *out, uint32_t hd, uint32_t S, int al) {
+    __shared__ float wt[KV8_COMB], red[4], sum[4];
+    __shared__ f32x4 pt[16][16];
+    const uint32_t t = threadIdx.x, lane = t & 15, g = t >> 4, d = blockIdx.y * 64 + lane * 4;
+    const size_t row = blockIdx.x, at = row * S;
+    const f32x4 *acc = (const f32x4 *)(p.acc + at * hd + d);
+    const uint32_t step = hd / 4;
+    f32x4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) v[u] = g + 16 * u < S ? acc[(size_t)(g + 16 * u) * step] : (f32x4){0.f, 0.f, 0.f, 0.f};
+    float m[KV8_COMB / TPB], l[KV8_COMB / TPB], M = -INFINITY;
+#pragma unroll
+    for (uint32_t x = 0; x < KV8_COMB / TPB; x++) {
+        const uint32_t k = t + x * TPB;
+        m[x] = k < S ? p.m[at + k] : -INFINITY;
+        l[x] = k < S ? p.s[at + k] : 0.0f;
+        M = fmaxf(M, m[x]);
+    }
+    M = wave_fmax(M);
+    if ((t & 63) == 0) red[t >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float L = 0.0f;
+#pragma unroll
+    for (uint32_t x = 0; x < KV8_COMB / TPB; x++) {
+        const float w = m[x] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[x] - M);
+        if (t + x * TPB < S) wt[t + x * TPB] = w;
+        L = fmaf(l[x], w, L);
+    }
+    L = wave_fsum(L);
+    if ((t & 63) == 0) sum[t >> 6] = L;
+    __syncthreads();
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+        if (g + 16 * u < S) o += v[u] * wt[g + 16 * u];
+    for (uint32_t k = g + 64; k < S; k += 16) o += acc[(size_t)k * step] * wt[k];
+    pt[g][lane] = o;
+    __syncthreads();
+    if (t >= 16) return;
+    o = pt[0][t];
+#pragma unroll
+    for (int x = 1; x < 16; x++) o += pt[x][t];
+    st4(out + row * hd + d, o / ((sum[0] + sum[1]) + (sum[2] + sum[3])), al);
 }
 
 // How a call runs. The wave form, small calls: workgroups of eight waves, one a
@@ -850,7 +902,7 @@ static kv8_plan kv8_plan_of(const sgk_kv8_attn *a) {
     if (wave) {
         const uint64_t steps = (keys + 31) / 32;
         uint64_t most = (a->hd == 64 ? 2 : 1) * cus / wgs;
-        if (most > 512) most = 512;
+        if (most > KV8_COMB) most = KV8_COMB;
         if (most && steps > 8 * most) { p.waves = 8; p.splits = (uint32_t)most; return p; }
         if (most < 1) most = 1;
         const uint64_t want = steps <= KV8_ONE * 4 ? 1 : (steps + 3) / 4;
@@ -859,7 +911,7 @@ static kv8_plan kv8_plan_of(const sgk_kv8_attn *a) {
     }
     const uint64_t tiles = (keys + 63) / 64, prow = (uint64_t)a->ntok * a->n_heads * a->hd * 4;
     uint64_t most = wgs < cus ? 2 * cus / wgs : KV8_JOIN;
-    if (most > 1024) most = 1024;
+    if (most > KV8_COMB) most = KV8_COMB;
     if (most > tiles) most = tiles;
     double best = 0.0;
     for (uint64_t S = 1; S <= most && (S == 1 || S * prow <= KV8_PART_BYTES); S++) {
@@ -875,7 +927,7 @@ extern "C" uint64_t sgk_kv8_attn_scratch(const sgk_kv8_attn *a) {
     return p.splits > 1 ? (uint64_t)a->ntok * a->n_heads * p.splits * (a->hd + 2) * 4 : 0;
 }
 
-extern "C" hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hipStream_t s) {
+extern "C" hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hipStream_t s, hipEvent_t done) {
     if (!a->ntok || !a->n_heads) return hipSuccess;
     if (!sgk_kv8_shape_ok(a->n_kv, a->hd, a->block) || ((uintptr_t)a->codes & 15) || a->n_heads % a->n_kv ||
         a->n_heads / a->n_kv > SGK_KV8_MAX_GROUP) return hipErrorInvalidValue;
@@ -890,11 +942,12 @@ extern "C" hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hi
         part.s = part.m + rows;
     }
     const dim3 wgrid(p.splits, a->n_kv, p.blocks);
-#define KC(H)                                                                                                                 \
-    do {                                                                                                                      \
-        if (p.waves == 8) hipLaunchKernelGGL((k_kv8_wave<H, 8>), wgrid, dim3(512), 0, s, *a, part, al);                        \
-        else if (p.waves) hipLaunchKernelGGL((k_kv8_wave<H, 4>), wgrid, dim3(256), 0, s, *a, part, al);                       \
-        else hipLaunchKernelGGL(k_kv8_tile<H>, dim3(p.blocks, a->n_kv, p.splits), dim3(KV8_NW * 64), 0, s, *a, part, al);     \
+    const hipEvent_t ev = p.splits > 1 ? NULL : done;
+#define KC(H)                                                                                                     \
+    do {                                                                                                          \
+        if (p.waves == 8) launch(k_kv8_wave<H, 8>, wgrid, 512, s, ev, *a, part, al);                              \
+        else if (p.waves) launch(k_kv8_wave<H, 4>, wgrid, 256, s, ev, *a, part, al);                              \
+        else launch(k_kv8_tile<H>, dim3(p.blocks, a->n_kv, p.splits), KV8_NW * 64, s, ev, *a, part, al);          \
     } while (0)
     switch (a->hd) {
     case 64: KC(64); break;
@@ -902,21 +955,19 @@ extern "C" hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hi
     default: KC(256); break;
     }
 #undef KC
-    hipError_t e = hipGetLastError();
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    if (p.splits <= KV8_JOIN) {
-        const uint64_t n = (uint64_t)a->ntok * a->n_heads, per = TPB / (a->hd / 4);
-        const dim3 grid((uint32_t)((n + per - 1) / per));
-        const int oal = !((uintptr_t)a->out & 15);
-        switch (a->hd) {
-        case 64: hipLaunchKernelGGL(k_kv8_join<64>, grid, dim3(TPB), 0, s, part, a->out, n, p.splits, oal); break;
-        case 128: hipLaunchKernelGGL(k_kv8_join<128>, grid, dim3(TPB), 0, s, part, a->out, n, p.splits, oal); break;
-        default: hipLaunchKernelGGL(k_kv8_join<256>, grid, dim3(TPB), 0, s, part, a->out, n, p.splits, oal); break;
-        }
+    const uint64_t n = (uint64_t)a->ntok * a->n_heads, per = TPB / (a->hd / 4);
+    const int oal = !((uintptr_t)a->out & 15);
+    if (p.splits > KV8_JOIN) {
+        launch(k_kv8_comb, dim3((uint32_t)n, a->hd / 64), TPB, s, done, part, a->out, a->hd, p.splits, oal);
         return hipGetLastError();
     }
-    sgk_attn c = {};
-    c.m = part.m; c.s = part.s; c.acc = part.acc; c.out = a->out; c.n_heads = a->n_heads; c.n_kv = a->n_kv; c.hd = a->hd;
-    c.out_tok = a->n_heads * a->hd; c.n_splits = p.splits; c.max_splits = p.splits; c.ntok = a->ntok;
-    return sgk_attn_combine(&c, s);
+    const dim3 grid((uint32_t)((n + per - 1) / per));
+    switch (a->hd) {
+    case 64: launch(k_kv8_join<64>, grid, TPB, s, done, part, a->out, n, p.splits, oal); break;
+    case 128: launch(k_kv8_join<128>, grid, TPB, s, done, part, a->out, n, p.splits, oal); break;
+    default: launch(k_kv8_join<256>, grid, TPB, s, done, part, a->out, n, p.splits, oal); break;
+    }
+    return hipGetLastError();
 }

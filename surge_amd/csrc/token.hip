@@ -84,7 +84,8 @@ __global__ void __launch_bounds__(TPB) k_rope_axes1(sgk_rope_axes_args a, rope_t
     }
 }
 
-extern "C" hipError_t sgk_rope_axes(const sgk_rope_axes_args *a, const double *inv, const uint8_t *axis, hipStream_t s) {
+extern "C" hipError_t sgk_rope_axes(const sgk_rope_axes_args *a, const double *inv, const uint8_t *axis, hipStream_t s,
+                                    hipEvent_t done) {
     const uint32_t half = a->rope_dim / 2;
     if (!a->n || !a->heads) return hipSuccess;
     if (!half || half > SGK_ROPE_HALF || a->rope_dim > a->head_dim || a->head_dim > 256) return hipErrorInvalidValue;
@@ -99,8 +100,8 @@ extern "C" hipError_t sgk_rope_axes(const sgk_rope_axes_args *a, const double *i
     const uint32_t per = TPB >> wl, want = (uint32_t)(((uint64_t)sgk_device_cus() + a->n - 1) / a->n);
     const uint32_t hs = min(want, (a->heads + per - 1) / per), hper = (a->heads + hs - 1) / hs;
     const dim3 grid(min(a->n, 1u << 20), (a->heads + hper - 1) / hper);
-    if (v4) hipLaunchKernelGGL(k_rope_axes4, grid, dim3(TPB), 0, s, *a, tab, hper, wl);
-    else hipLaunchKernelGGL(k_rope_axes1, grid, dim3(TPB), 0, s, *a, tab, hper, wl);
+    if (v4) launch(k_rope_axes4, grid, TPB, s, done, *a, tab, hper, wl);
+    else launch(k_rope_axes1, grid, TPB, s, done, *a, tab, hper, wl);
     return hipGetLastError();
 }
 
@@ -193,20 +194,19 @@ __global__ void __launch_bounds__(TR_THREADS) k_token_recount(const int32_t *ids
 }
 
 extern "C" hipError_t sgk_token_counts(const int32_t *ids, uint32_t *counts, uint32_t n, uint32_t vocab, uint32_t rows,
-                                       int clear, hipStream_t s) {
-    if (!vocab || !rows) return hipSuccess;
+                                       int clear, hipStream_t s, hipEvent_t done) {
+    if (!vocab || !rows || (!n && !clear)) return hipErrorInvalidValue;     // nothing to launch, nothing to wait for
     if (n && n <= TR_MOST) {
-        hipLaunchKernelGGL(k_token_recount, dim3((vocab + TR_IDS - 1) / TR_IDS, rows), dim3(TR_THREADS), 0, s, ids, counts, n, vocab, clear);
+        launch(k_token_recount, dim3((vocab + TR_IDS - 1) / TR_IDS, rows), TR_THREADS, s, done, ids, counts, n, vocab, clear);
         return hipGetLastError();
     }
     if (clear) {
         const uint64_t b = ((uint64_t)rows * vocab + TPB - 1) / TPB;
-        hipLaunchKernelGGL(k_zero_u32, dim3((uint32_t)(b < 2048 ? b : 2048)), dim3(TPB), 0, s, counts, (uint64_t)rows * vocab);
+        launch(k_zero_u32, dim3((uint32_t)(b < 2048 ? b : 2048)), TPB, s, n ? NULL : done, counts, (uint64_t)rows * vocab);
     }
     if (n) {
         const uint64_t b = ((uint64_t)n + TC_IDS - 1) / TC_IDS;
-        hipLaunchKernelGGL(k_token_counts, dim3((uint32_t)(b < 1024 ? b : 1024), rows < 65535 ? rows : 65535), dim3(TPB), 0, s,
-                           ids, counts, n, vocab, rows);
+        launch(k_token_counts, dim3((uint32_t)(b < 1024 ? b : 1024), rows), TPB, s, done, ids, counts, n, vocab, rows);
     }
     return hipGetLastError();
 }
@@ -303,13 +303,14 @@ static uint32_t lg_parts(uint32_t vocab, uint32_t rows) {
     return min(min(need, most), (uint32_t)TPB);
 }
 extern "C" uint64_t sgk_logits_part_bytes(uint32_t vocab, uint32_t rows) { return (uint64_t)rows * lg_parts(vocab, rows) * sizeof(lg_best); }
-extern "C" hipError_t sgk_logits(const sgk_logits_args *a, void *part, hipStream_t s) {
+extern "C" hipError_t sgk_logits(const sgk_logits_args *a, void *part, hipStream_t s, hipEvent_t done) {
     if (!a->vocab || !a->rows) return hipSuccess;
     const uint32_t parts = lg_parts(a->vocab, a->rows);
     const bool v4 = !(((uintptr_t)a->x | (uintptr_t)a->out | (uintptr_t)a->counts | (uintptr_t)a->bias) & 15) && a->vocab % 4 == 0;
     const dim3 grid(parts, a->rows);
-    if (v4) hipLaunchKernelGGL(k_logits<true>, grid, dim3(TPB), 0, s, *a, (lg_best *)part);
-    else hipLaunchKernelGGL(k_logits<false>, grid, dim3(TPB), 0, s, *a, (lg_best *)part);
-    if (parts > 1) hipLaunchKernelGGL(k_logits_token, dim3(a->rows), dim3(TPB), 0, s, (const lg_best *)part, parts, a->token);
+    const hipEvent_t ev = parts > 1 ? NULL : done;
+    if (v4) launch(k_logits<true>, grid, TPB, s, ev, *a, (lg_best *)part);
+    else launch(k_logits<false>, grid, TPB, s, ev, *a, (lg_best *)part);
+    if (parts > 1) launch(k_logits_token, dim3(a->rows), TPB, s, done, (const lg_best *)part, parts, a->token);
     return hipGetLastError();
 }
