@@ -50,8 +50,7 @@ __device__ __forceinline__ void key_four(uint32_t c, uint32_t hd, uint32_t &r, u
 
 // Four x / s to the nearest integers, ties to even, as bytes. q = rint(x * (1/s))
 // can be wrong only where x / s is within 2^-16 of a tie; there the remainder
-// x - q s, exact in one fma, decides. Clamped for a scale near the end of the
-// range, whose rounding may leave |x / s| above 127.
+// x - q s, exact in one fma, decides.
 __device__ __forceinline__ uint32_t quant4(f32x4 x, float s, float inv) {
     float q[4], far = 0.0f;
 #pragma unroll
@@ -65,7 +64,6 @@ __device__ __forceinline__ uint32_t quant4(f32x4 x, float s, float inv) {
         for (int e = 0; e < 4; e++) {
             const float r = fmaf(-q[e], s, x[e]), a = 2.0f * fabsf(r);
             if (a > s || (a == s && ((int)q[e] & 1))) q[e] += copysignf(1.0f, r);
-            q[e] = fminf(fmaxf(q[e], -127.0f), 127.0f);
         }
     }
     const uint32_t lo = __builtin_amdgcn_perm((uint32_t)(int)q[1], (uint32_t)(int)q[0], 0x0C0C0400u);
@@ -138,8 +136,11 @@ __global__ void __launch_bounds__(NTH, 4) k_kv8_store(kv8_store_args a, uint32_t
     const bool zero = poison || s == 0.0f;
     const float sz = zero ? 1.0f : sq;
     if (zero || up != 1.0f) {
+        const float top = zero ? 0.0f : 127.0f * sz;    // there the scale's own rounding may leave |x / s| above 127
 #pragma unroll
-        for (int i = 0; i < 4 * U; i++) v[i] = zero ? (f32x4){0.f, 0.f, 0.f, 0.f} : v[i] * up;
+        for (int i = 0; i < 4 * U; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[i][e] = __builtin_amdgcn_fmed3f(v[i][e] * up, -top, top);
     }
     if (!half) {
 #pragma unroll
@@ -270,8 +271,8 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
 // ---------------------------------------------------------------------------
 // Attention of few rows: decode, and small chunks. A workgroup takes 16 rows
 // (token-major, the query heads of one kv head inside a token) and a part of
-// the keys. Every wave streams
-// its own steps of 32 keys straight from the cache into operands:
+// the keys. Every wave streams its own steps of 32 keys straight from the
+// cache into operands:
 //  - q in fixed point against its row's largest element, 24 bits as three int8
 //    digits (q = sq (65536 d2 + 256 d1 + d0)): the score product is three
 //    v_mfma_i32_16x16x64_i8 on the key codes as they lie, its sums exact, and
@@ -385,16 +386,17 @@ __device__ __forceinline__ void split2(float w0, float w1, f16x2 &hi, f16x2 &lo)
 // maximum and sum, gives the weights' f16 halves in operand order and what the
 // output so far is to be multiplied by. x: the integer scores; f: what they are
 // to be multiplied by (scale, q's unit, the keys' scale); vs: the values'
-// scales; both per tile. Key 16 u + 4 lg + e is visible up to rel.
+// scales; both per tile. Key `key` + 16 u + 4 lg + e is visible up to pos (groups
+// are aligned, so that the sum stays in 32 bits at the last position, too).
 // The usual group has all its keys visible, f >= 0 and vs >= 2^-80: then the
 // weight is one fma and one exp2, w = 2^(x f + log2 vs - m0), and the sum of p
 // is the sum of w / vs (an error of log2 vs is in both, and drops out). GEN
 // takes any: masked keys apart (a row with no key yet has m0 = -inf), a scale
 // of zero or NaN.
 template <int UN, bool GEN>
-__device__ __forceinline__ float softmax_step(float (&x)[UN][4], const float (&f)[UN], const float (&vs)[UN], int rel, float &mrun,
-                                              float &lsum, f16x8 (&ph)[UN / 2], f16x8 (&pl)[UN / 2]) {
-    const int lg4 = (threadIdx.x & 63) >> 4 << 2;
+__device__ __forceinline__ float softmax_step(float (&x)[UN][4], const float (&f)[UN], const float (&vs)[UN], uint32_t key, uint32_t pos,
+                                              float &mrun, float &lsum, f16x8 (&ph)[UN / 2], f16x8 (&pl)[UN / 2]) {
+    const uint32_t k0 = key + ((threadIdx.x & 63) >> 4 << 2);
     float tm = -INFINITY, lv[UN];
 #pragma unroll
     for (int u = 0; u < UN; u++) {
@@ -402,7 +404,7 @@ __device__ __forceinline__ float softmax_step(float (&x)[UN][4], const float (&f
             lv[u] = __builtin_amdgcn_logf(fmaxf(fabsf(vs[u]), 0x1p-80f));
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                x[u][e] = 16 * u + lg4 + e <= rel ? x[u][e] * f[u] : -INFINITY;
+                x[u][e] = k0 + 16 * u + e <= pos ? x[u][e] * f[u] : -INFINITY;
                 tm = fmaxf(tm, x[u][e] + lv[u]);
             }
         } else {
@@ -422,7 +424,7 @@ __device__ __forceinline__ float softmax_step(float (&x)[UN][4], const float (&f
         if (GEN) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const bool vis = 16 * u + lg4 + e <= rel;
+                const bool vis = k0 + 16 * u + e <= pos;
                 const float p = vis ? __builtin_amdgcn_exp2f(x[u][e] - m0) : 0.0f;
                 l += p;
                 w[e] = vis ? p * vs[u] : 0.0f;
@@ -528,8 +530,8 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
         f16x8 ph[1], pl[1];
         const float f[2] = {qf * ks[0], qf * ks[1]};
         const bool usual = step * 32 + 31 <= first && scales_usual(fminf(ks[0], ks[1]), fminf(vs[0], vs[1]));
-        const float al2 = usual ? softmax_step<2, false>(sc, f, vs, 0, mrun, lsum, ph, pl)
-                                : softmax_step<2, true>(sc, f, vs, (int)(rpos - step * 32), mrun, lsum, ph, pl);
+        const float al2 = usual ? softmax_step<2, false>(sc, f, vs, 0, 0, mrun, lsum, ph, pl)
+                                : softmax_step<2, true>(sc, f, vs, step * 32, rpos, mrun, lsum, ph, pl);
         if (__builtin_amdgcn_ballot_w64(al2 != 1.0f)) {
 #pragma unroll
             for (int n = 0; n < NT; n++) o[n] *= al2;
@@ -588,9 +590,9 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
 // run it in step leave the matrix units idle through the softmax: 46% busy.
 // So a wave alternates steps of products (the last tile's P V, this one's
 // K Q^T) and steps of softmax, and the two waves of a SIMD (w and w + 4) are
-// one step apart, a barrier after every step: one is in its products while the
-// other is in its softmax. Both tiles are double-buffered; a wave requests its
-// part of the next tile in a products step and stores it behind the softmax.
+// one step apart, a barrier after every two steps: one is in its products while
+// the other is in its softmax. Both tiles are double-buffered; a wave stores its
+// part of the next one and requests that of the one after before its softmax.
 // Grid: (row block, kv head, key split), the longest rows first.
 // ---------------------------------------------------------------------------
 #define KV8_NW 8
@@ -735,8 +737,8 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
         const uint32_t key = (k0 + i) * 64;
         const bool usual = key + 63 <= wfirst && scales_usual(fminf(fminf(k4[0], k4[1]), fminf(k4[2], k4[3])),
                                                               fminf(fminf(v4[0], v4[1]), fminf(v4[2], v4[3])));
-        resc = usual ? softmax_step<4, false>(sc, f, vs, 0, mrun, lsum, ph, pl)
-                     : softmax_step<4, true>(sc, f, vs, (int)(rpos - key), mrun, lsum, ph, pl);
+        resc = usual ? softmax_step<4, false>(sc, f, vs, 0, 0, mrun, lsum, ph, pl)
+                     : softmax_step<4, true>(sc, f, vs, key, rpos, mrun, lsum, ph, pl);
     };
 
     ph[0] = ph[1] = pl[0] = pl[1] = (f16x8){};
@@ -792,9 +794,9 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
 }
 
 // Join of few splits of many rows: four dims of a row per lane, all splits'
-// loads in flight, nothing shared between lanes. A row's first split sees a
-// key, so the largest maximum is a number and a split without a key weighs
-// nothing; NaN sums reach the output.
+// loads in flight, nothing shared between lanes. Every row sees key 0, so the
+// largest maximum is a number, and a split without a key weighs nothing; NaN
+// sums reach the output.
 #define KV8_JOIN 8u
 template <int HD>
 __global__ void __launch_bounds__(TPB) k_kv8_join(kv8_part p, float *out, uint64_t rows, uint32_t S, int al) {

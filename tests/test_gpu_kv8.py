@@ -105,8 +105,14 @@ def test_store_one_by_one(gpu):
 def test_store_special_values(gpu):
     """Ties at half steps, zeros, values near f32's smallest and f16's largest; a value f16 cannot
     hold poisons its block and head only, until the block is stored from its start."""
-    c, d = K.Cache(2, 64, 16, 96), K.Cache(2, 64, 16, 96)
-    x = np.zeros((96, 2, 64), np.float32)
+    c, d = K.Cache(2, 64, 16, 160), K.Cache(2, 64, 16, 160)
+    x = np.zeros((160, 2, 64), np.float32)
+    tiny = np.float32(1.4e-45)                              # 2^-149
+    x[96:112, 0] = (np.arange(64) * 3) * tiny               # 189 steps: a scale of one step, values of 190 of it
+    x[96:112, 1] = -(np.arange(64) + 2) * 2 * tiny
+    x[112:128, 0] = np.arange(64) * np.float32(1e-41)
+    x[112:128, 1] = np.random.default_rng(4).standard_normal((16, 64)) * 1e-37
+    x[128:144] = np.random.default_rng(5).standard_normal((16, 2, 64)) * 1e-20
     x[0:16, :, 0] = 127.0                                   # a scale of one
     x[0:16, :, 1:32] = np.arange(31) + 0.5                  # ties
     x[0:16, :, 32:] = np.nextafter(np.arange(32, dtype=np.float32) + 0.5, np.float32(0))
