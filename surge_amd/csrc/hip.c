@@ -913,11 +913,11 @@ static sg_err back_to(const sg_gpu *g, int was, sg_err e) {
 static bool aligned(const void *buf, uintptr_t to) { return !((uintptr_t)((const gbuf *)buf)->dev & (to - 1)); }
 
 uint64_t sg_kv8_code_bytes(uint32_t n_kv, uint32_t hd, uint64_t cap) {
-    if (!sgk_kv8_shape_ok(n_kv, hd, 16) || cap > UINT32_MAX) return 0;
+    if (!sgk_kv8_shape_ok(n_kv, hd, 16) || n_kv > 65535 || cap > UINT32_MAX) return 0;
     return (cap + SGK_KV8_TILE - 1) / SGK_KV8_TILE * n_kv * (2ull * SGK_KV8_TILE * hd);
 }
 uint64_t sg_kv8_scale_bytes(uint32_t n_kv, uint32_t block, uint64_t cap) {
-    if (!sgk_kv8_shape_ok(n_kv, 64, block) || cap > UINT32_MAX) return 0;
+    if (!sgk_kv8_shape_ok(n_kv, 64, block) || n_kv > 65535 || cap > UINT32_MAX) return 0;
     return (cap + block - 1) / block * n_kv * 8;
 }
 
@@ -994,6 +994,7 @@ static sg_err attn_kv8_oneshot(sg_gpu *g, const char *who, void *q, void *codes,
     if (qs < hd) return errf("gpu: %s: q_stride < head_dim", who);
     if ((uint64_t)n * (nh / nkv) > 1u << 30) return errf("gpu: %s: more than 2^30 query rows per kv head", who);
     const uint64_t rows = (uint64_t)(n ? n : 1) * nh;
+    if (rows > (1ull << 60) / qs) return errf("gpu: %s: q_stride %u is too large", who, qs);     /* the sizes below stay in 64 bits */
     if (sg_failed(e = need(q, ((rows - 1) * qs + hd) * 4, "q")) || sg_failed(e = need(out, rows * hd * 4, "out"))) return e;
     if (!aligned(q, 4) || !aligned(out, 4)) return errf("gpu: %s: q and out must be 4-byte aligned", who);
     if (overlap(out, q) || overlap(out, codes) || overlap(out, scales)) return errf("gpu: %s: out overlaps an input", who);
@@ -1038,6 +1039,7 @@ sg_err sg_gpu_run_rope_axes(sg_gpu *g, void *x, void *pos, void *out, const uint
         return (sg_err){"gpu: rope_axes: bad shape"};
     const uint64_t w = (uint64_t)(nh - 1) * hs + hd, row = p[7] ? p[7] : (uint64_t)nh * hs;
     if (row < w) return (sg_err){"gpu: rope_axes: row stride below the heads' width"};
+    if (row > (1ull << 60) / n) return (sg_err){"gpu: rope_axes: strides are too large"};       /* the sizes below stay in 64 bits */
     if (!(theta > 0.0f) || isinf(theta)) return (sg_err){"gpu: rope_axes: theta must be positive and finite"};
     if (order > 1 || sec[0] + sec[1] + sec[2] != half) return (sg_err){"gpu: rope_axes: sections must add up to rope_dim / 2, order 0 or 1"};
     if (order && ((sec[1] && 3 * sec[1] - 2 >= half) || (sec[2] && 3 * sec[2] - 1 >= half)))

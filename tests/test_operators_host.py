@@ -140,6 +140,18 @@ def test_rope_axes_refuses(change, match):
     refused("sg_gpu_run_rope_axes", (far(10 * 128 * 4), far(10 * 12), far(10 * 128 * 4)), p, match)
 
 
+def test_sizes_that_wrap_64_bits_are_refused():
+    """Strides whose product with the row count passes 2^64 must not come out small."""
+    big = 0xFFFFFFFF
+    refused("sg_gpu_run_rope_axes", (far(1 << 20), far(1 << 40), far(1 << 20)),
+            [64, 32, 65535, big - 3, big, 6 | 5 << 8 | 5 << 16, F(1e7), 0], "too large")
+    refused("sg_gpu_run_attn_prefill_kv8", (far(1 << 20), far(1 << 62), far(1 << 62), far(1 << 20)),
+            [65535 * 16, 65535, 64, 0, 1 << 26, big, F(0.1), 128], "too large")
+    refused("sg_gpu_run_attn_prefill_kv8", (far(1 << 20), far(1 << 62), far(1 << 62), far(1 << 20)),
+            [16, 1, 64, 0, (1 << 26) + 1, 64, F(0.1), 128], "2\\^30")
+    assert S.lib().sg_kv8_code_bytes(65536, 256, 1 << 31) == 0 and S.lib().sg_kv8_scale_bytes(1 << 20, 16, 1 << 31) == 0
+
+
 def test_rope_axes_refuses_overlap():
     p = [64, 32, 2, 0, 10, 6 | 5 << 8 | 5 << 16, F(1e7), 0]
     n = 10 * 128 * 4
