@@ -342,17 +342,19 @@ sg_err sg_gpu_run_rmsnorm_gated_chunk(sg_gpu *g, void *y, void *z, void *out, vo
  *   scales f32 [position / block][n_kv][2] (K, V), block = 16, 32, 64 or 128
  *          positions. x = code * scale, |code| <= 127.
  * sg_kv8_code_bytes / sg_kv8_scale_bytes: what `cap` positions need (0 for a
- * shape that is not supported). hd = 64, 128 or 256. A larger cache has the
- * same layout from its start, so the buffers may hold more than a call uses.
+ * shape that is not supported). hd = 64, 128 or 256, n_kv <= 65535, positions
+ * below 2^32 - 128. A larger cache has the same layout from its start, so the
+ * buffers may hold more than a call uses.
  *
  * sg_gpu_run_kv8_store: rows [base, base + n) from k and v (row stride p[5]
- *   floats, 0 = n_kv hd; [n_kv][hd] in a row). Per block, head and half the
- *   scale is s = max|x| * (1/127), an f32 product with the f32 nearest to 1/127,
- *   and a code is x / s rounded to the nearest integer, ties to even. In a block that goes on (base inside
- *   it) s is not below the scale it has, and if s grows the codes of its rows
- *   before base are rounded again to the nearest of code * s_old / s; a block
- *   that starts at base or after it is new, whatever its scale held. A value
- *   that f16 cannot hold (|x| >= 65520, NaN) makes the block's scale NaN, and
+ *   floats, 0 = n_kv hd; [n_kv][hd] in a row), n in [1, 2^27]. Per block, head
+ *   and half the scale is s = max|x| * (1/127), an f32 product with the f32
+ *   nearest to 1/127, and a code is x / s rounded to the nearest integer, ties
+ *   to even, at most 127 either way. In a block that goes on (base inside it) s
+ *   is not below the scale it has, and if s grows the codes of its rows before
+ *   base are rounded again to the nearest of code * s_old / s; a block that
+ *   starts at base or after it is new, whatever its scale held. A value that
+ *   f16 cannot hold (|x| >= 65520, NaN) makes the block's scale NaN, and
  *   whatever reads the block NaN, until the block is stored from its start.
  *   Storing at base drops the rows from base on: codes of rows >= base + n
  *   stay as they were and mean nothing. The result for a block depends on how
@@ -367,7 +369,7 @@ sg_err sg_gpu_run_rmsnorm_gated_chunk(sg_gpu *g, void *y, void *z, void *out, vo
  *   p: [0]=n_heads [1]=n_kv [2]=hd [3]=seq [4]=q_stride [5]=scale bits [6]=block.
  * sg_gpu_run_attn_prefill_kv8: as sg_gpu_run_attn_prefill: q [n][n_heads]
  *   [q_stride], out [n][n_heads][hd]; token t sees positions 0 .. base + t of
- *   a cache that holds base + n.
+ *   a cache that holds base + n; n * n_heads / n_kv <= 2^30.
  *   p: [0]=n_heads [1]=n_kv [2]=hd [3]=base [4]=n [5]=q_stride [6]=scale bits
  *   [7]=block.
  * Both keep q.k exact up to q's rounding to 24 bits of its head's largest
@@ -389,13 +391,14 @@ sg_err sg_gpu_run_attn_prefill_kv8(sg_gpu *g, void *q, void *codes, void *scales
  * has the pairs i % 3 == 1 below 3 s1, axis 2 those of i % 3 == 2 below 3 s2,
  * axis 0 the others. Dims from rope_dim on are copied; gaps between slices are
  * not written. out may be x (the same address) but not overlap it otherwise.
- * p: [0]=head_dim (<= 256) [1]=rope_dim [2]=heads [3]=stride [4]=n [5]=sections
+ * p: [0]=head_dim (<= 256) [1]=rope_dim [2]=heads (<= 65535) [3]=stride [4]=n [5]=sections
  * [6]=theta bits [7]=row stride. */
 sg_err sg_gpu_run_rope_axes(sg_gpu *g, void *x, void *pos, void *out, const uint32_t params[8]);
 
 /* Token counts: counts u32 [rows][vocab] += the occurrences in ids int32
  * [rows][n] (ids outside [0, vocab) are skipped, so -1 pads a ragged row);
- * cleared first when p[3] is 1. p: [0]=n (may be 0) [1]=vocab [2]=rows [3]=clear. */
+ * cleared first when p[3] is 1. vocab < 2^31, rows <= 65535.
+ * p: [0]=n (may be 0) [1]=vocab [2]=rows [3]=clear. */
 sg_err sg_gpu_run_token_counts(sg_gpu *g, void *ids, void *counts, const uint32_t params[8]);
 
 /* Logits under penalties, a bias and a mask, and the token they choose. Per
@@ -406,7 +409,7 @@ sg_err sg_gpu_run_token_counts(sg_gpu *g, void *ids, void *counts, const uint32_
  * [rows][vocab] may be logits. token u32 [rows]: the lowest id of the largest
  * value that is above -inf, 0xFFFFFFFF if there is none (nothing allowed);
  * NaN is never chosen. repetition > 0 and finite (1 = none), frequency and
- * presence finite (0 = none).
+ * presence finite (0 = none). vocab < 2^31, rows <= 65535.
  * p: [0]=vocab [1]=rows [2]=repetition bits [3]=frequency bits [4]=presence bits. */
 sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void *mask, void *out, void *token,
                          const uint32_t params[8]);

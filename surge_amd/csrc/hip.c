@@ -910,6 +910,9 @@ static sg_err back_to(const sg_gpu *g, int was, sg_err e) {
     if (was != g->dev && hipSetDevice(was) != hipSuccess && !sg_failed(e)) return (sg_err){"gpu: hipSetDevice failed"};
     return e;
 }
+/* An output of which a call writes the first `bytes`: what lies behind is sent
+ * first, so that the download leaves it as it was. */
+static sg_err push_out(void *buf, uint64_t bytes) { return ((const gbuf *)buf)->nbytes > bytes ? sg_gpu_buf_upload(buf) : SG_OK; }
 static bool aligned(const void *buf, uintptr_t to) { return !((uintptr_t)((const gbuf *)buf)->dev & (to - 1)); }
 
 uint64_t sg_kv8_code_bytes(uint32_t n_kv, uint32_t hd, uint64_t cap) {
@@ -1001,7 +1004,7 @@ static sg_err attn_kv8_oneshot(sg_gpu *g, const char *who, void *q, void *codes,
     int was;
     if (sg_failed(e = on_device(g, &was))) return e;
     void *ins[3] = {q, codes, scales}, *outs[1] = {out};
-    if (!sg_failed(e = push(ins, 3))) {
+    if (!sg_failed(e = push(ins, 3)) && !sg_failed(e = push_out(out, rows * hd * 4))) {
         if (!n) {                       /* no key at all: zeros */
             e = finish(g, sgk_fill_f32(DEV(out), 0.0f, rows * hd, g->stream), outs, 1);
         } else {
@@ -1108,7 +1111,8 @@ sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void
     int was;
     if (sg_failed(e = on_device(g, &was))) return e;
     void *part;
-    if (!sg_failed(e = scratch(g, sgk_logits_part_bytes(vocab, rows), &part)) && !sg_failed(e = push(bufs, 4))) {
+    if (!sg_failed(e = scratch(g, sgk_logits_part_bytes(vocab, rows), &part)) && !sg_failed(e = push(bufs, 4)) &&
+        !sg_failed(e = push_out(token, (uint64_t)rows * 4)) && (out == logits || !sg_failed(e = push_out(out, lb)))) {
         const sgk_logits_args a = {DEV(logits), DEV(counts), DEV(bias), DEV(mask), DEV(out), DEV(token), vocab, rows, rep, freq, pres};
         e = finish_done(g, sgk_logits(&a, part, g->stream, g->done), outs, 2);
     }

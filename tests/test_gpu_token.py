@@ -189,6 +189,33 @@ def test_logits_ties_infinities_and_nothing_allowed(gpu):
     assert tok.tolist() == [700, none, none, 17, 9, 0, none, 2222]
 
 
+@pytest.mark.parametrize("n", [0, 1, 3])
+def test_what_lies_behind_an_output_stays(gpu, n):
+    """Buffers larger than a call writes keep their ends, in the host's mirror too."""
+    rng = np.random.default_rng(n)
+    c = K.Cache(2, 64, 16, 64, rng)
+    c.scales[...] = 0.01
+    q = rng.standard_normal((max(n, 1), 4, 64)).astype(np.float32)
+    with Bufs(gpu) as buf:
+        out = buf(np.full((5, 4, 64), 7.0, np.float32))
+        if n < 2:
+            gpu.attn_decode_kv8(buf(q), buf(c.codes), buf(c.scales), out, [4, 2, 64, n * 40, 64, F(0.125), 16])
+        else:
+            gpu.attn_prefill_kv8(buf(q), buf(c.codes), buf(c.scales), out, [4, 2, 64, 40, n, 64, F(0.125), 16])
+        assert (out.array[max(n, 1):] == 7.0).all() and (out.array[:max(n, 1)] != 7.0).all()
+        x = rng.standard_normal((max(n, 1), 40)).astype(np.float32)
+        o, token = buf(np.full((4, 40), 7.0, np.float32)), buf(np.full(6, 77, np.uint32))
+        gpu.logits(buf(x), None, None, None, o, token, [40, max(n, 1), F(1.0), 0, 0, 0, 0, 0])
+        assert (o.array[max(n, 1):] == 7.0).all() and np.array_equal(o.array[:max(n, 1)], x)
+        assert (token.array[max(n, 1):] == 77).all() and np.array_equal(token.array[:max(n, 1)], x.argmax(1))
+        k, v = (buf(np.full((4, 2, 64), 7.0, np.float32)) for _ in range(2))
+        gpu.kv8_load(buf(c.codes), buf(c.scales), k, v, [2, 64, 16, 3, max(n, 1), 0, 0, 0])
+        assert (k.array[max(n, 1):] == 7.0).all() and (v.array[max(n, 1):] == 7.0).all()
+        counts = buf(np.full((4, 40), 3, np.uint32))
+        gpu.token_counts(buf(np.zeros((max(n, 1), 5), np.int32)), counts, [5, 40, max(n, 1), 1])
+        assert (counts.array[max(n, 1):] == 3).all() and (counts.array[:max(n, 1), 0] == 5).all() and not counts.array[:max(n, 1), 1:].any()
+
+
 def test_logits_plain_is_the_argmax(gpu):
     rng = np.random.default_rng(9)
     x = rng.standard_normal((1, 151936)).astype(np.float32)
