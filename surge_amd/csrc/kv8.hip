@@ -874,24 +874,27 @@ __global__ void __launch_bounds__(TPB) k_kv8_comb(kv8_part p, float *out, uint32
     st4(out + row * hd + d, o / ((sum[0] + sum[1]) + (sum[2] + sum[3])), al);
 }
 
-// How a call runs. The wave form, small calls: workgroups of eight waves, one a
-// CU (two at head_dim 64), where their waves get more than a step of 32 keys
-// each and there are not more workgroups than that without a split; else of
-// four, a step to each wave (whole call, us, eight / four waves:
-// 24 heads of 256 on 4, 32771 keys 31.4 / 33.5, 700 keys 24.3 / 22.7; 32 of 128
-// on 8, 262000 keys 98.6 / 105, 5000 keys 22.6 / 22.2), and one workgroup alone
-// up to KV8_ONE steps a wave, where a second launch to join costs more (300
-// keys, one / split: head_dim 256 21.5 / 21.7, 64 18.0 / 18.8). Else row
-// blocks in tiles, one workgroup per CU at a time, their keys split where that
-// shortens the launch: rounds x (a part's tiles + KV8_TAIL for its start and
-// end) tiles of KV8_TILE_US, against the partials' way to memory and back.
-// KV8_SMALL, in waves' steps of 32 keys x head_dim, is where the two meet
-// (whole call, us, wave / tile): 24 heads of 256 on 4, 8040 keys, 240 rows
-// (3.9M) 48.9 / 50.4, 462 rows (7.5M) 67.7 / 61.2, 1300 keys, 1800 rows (4.7M)
-// 47.9 / 65.5; 32 of 128 on 8, 8020 keys, 80 rows (1.3M) 32.2 / 36.0, 8077 keys,
-// 308 rows (5.2M) 58.1 / 55.0; 12 of 64, 32077 keys, 77 rows (3.9M) 59.5 / 60.5.
+// How a call runs. The wave form, small calls (whole calls below in us):
+//  - workgroups of eight waves, one a CU (two at head_dim 64), where their waves
+//    get more than a step of 32 keys each and there are not more workgroups than
+//    that without a split (eight / four waves: 24 heads of 256 on 4, 32771 keys
+//    29.5 / 31.2; 32 of 128 on 8, 262000 keys 97.1 / 103.4, 5000 keys 20.8 both);
+//  - one of eight waves alone up to KV8_ONE steps, as a second launch to join
+//    costs more than a wave's second step (one / splits of four waves: 384 keys,
+//    24 of 256 on 4 20.2 / 21.2, 32 of 128 on 8 16.7 / 19.1, 12 of 64 15.6 / 17.2;
+//    512 keys 22.0 / 21.4, 17.9 / 19.0, 16.3 / 17.1; 768 keys 24.3 / 21.8, 19.4 /
+//    19.0, 17.3 / 17.2);
+//  - else workgroups of four waves, a step to each wave.
+// Else row blocks in tiles, one workgroup per CU at a time, their keys split
+// where that shortens the launch: rounds x (a part's tiles + KV8_TAIL for its
+// start and end) tiles of KV8_TILE_US, against the partials' way to memory and
+// back. KV8_SMALL, in waves' steps of 32 keys x head_dim, is where the two meet
+// (wave / tile): 24 heads of 256 on 4, 8040 keys, 240 rows (3.9M) 45.5 / 51.2,
+// 8077 keys, 462 rows (7.5M) 62.7 / 62.9, 1300 keys, 1800 rows (4.7M) 44.2 /
+// 55.0; 32 of 128 on 8, 8020 keys, 80 rows (1.3M) 28.3 / 34.6, 8077 keys, 308
+// rows (5.2M) 60.9 / 53.7; 12 of 64, 32077 keys, 77 rows (3.9M) 50.6 / 58.9.
 #define KV8_SMALL (1ull << 22)
-#define KV8_ONE 3
+#define KV8_ONE 16
 #define KV8_TILE_US 2.5         /* at head_dim 256 */
 #define KV8_TAIL 3.0
 #define KV8_PART_BYTES (256ull << 20)
@@ -905,10 +908,13 @@ static kv8_plan kv8_plan_of(const sgk_kv8_attn *a) {
         const uint64_t steps = (keys + 31) / 32;
         uint64_t most = (a->hd == 64 ? 2 : 1) * cus / wgs;
         if (most > KV8_COMB) most = KV8_COMB;
-        if (most && steps > 8 * most) { p.waves = 8; p.splits = (uint32_t)most; return p; }
-        if (most < 1) most = 1;
-        const uint64_t want = steps <= KV8_ONE * 4 ? 1 : (steps + 3) / 4;
-        p.splits = (uint32_t)(want < most ? want : most);
+        const bool one = steps > 4 && steps <= KV8_ONE;
+        if (most && (one || steps > 8 * most)) {
+            p.waves = 8;
+            p.splits = one ? 1 : (uint32_t)most;
+        } else if (most > 1) {
+            p.splits = (uint32_t)((steps + 3) / 4 < most ? (steps + 3) / 4 : most);
+        }
         return p;
     }
     const uint64_t tiles = (keys + 63) / 64, prow = (uint64_t)a->ntok * a->n_heads * a->hd * 4;

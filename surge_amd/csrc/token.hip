@@ -153,11 +153,11 @@ __global__ void __launch_bounds__(TPB) k_token_counts(const int32_t *ids, uint32
 // Up to TR_MOST ids a row: a workgroup owns TR_IDS ids of the vocabulary, reads
 // the row's whole history and counts its own in LDS, alike neighbours of a
 // thread at once, so nothing is cleared first and no two additions meet in
-// memory. Whole call, us, 151936 ids, Zipf's law with exponent 1.2 / one id
-// only, against the table form: 900 ids of 1 row 14.1 / 14.0, 18.5 / 18.6;
-// 32000 of 1 row 18.5 / 17.1, 22.2 / 20.5; 131072 of 16 rows 44 / 32, 104 / 33;
-// 262144 of 1 row 55 / 50, 56 / 22. Past TR_MOST the walk over the history
-// decides, and the table form spreads that.
+// memory. Whole call, us, 151936 ids, cleared, this form / the table form, for
+// Zipf's law with exponent 1.2 and for one id only: 900 ids of 1 row 11.4 / 16.4,
+// 12.0 / 17.2; 32000 of 1 row 15.8 / 21.3, 14.8 / 21.1; 131072 of 16 rows 42 /
+// 103, 30 / 33; 262144 of 1 row 53 / 55, 48 / 21. Past TR_MOST the walk over the
+// history decides, and the table form spreads that.
 #define TR_IDS 8192u
 #define TR_THREADS 1024
 #define TR_U 8u
