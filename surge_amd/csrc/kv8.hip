@@ -382,40 +382,60 @@ __device__ __forceinline__ void split2(float w0, float w1, f16x2 &hi, f16x2 &lo)
     lo = __builtin_bit_cast(f16x2, l);
 }
 
+// The largest of two or three; unlike fmaxf's code, operands are taken as they
+// are (no signalling NaN reaches here), one instruction each.
+__device__ __forceinline__ float max2(float a, float b) {
+    float r;
+    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+// Over the wave's four rows of lanes: a swap leaves both partners' values in
+// every lane.
+__device__ __forceinline__ float rows_max(float m, float v) {
+    const uint32_t a = __float_as_uint(v);
+    const auto p = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    const uint32_t b = __float_as_uint(max2(__uint_as_float(p[0]), __uint_as_float(p[1])));
+    const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return max3(m, __uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+
 // One group of UN tiles' scores to weights, online: updates the row's running
 // maximum and sum, gives the weights' f16 halves in operand order and what the
 // output so far is to be multiplied by. x: the integer scores; f: what they are
-// to be multiplied by (scale, q's unit, the keys' scale); vs: the values'
-// scales; both per tile. Key `key` + 16 u + 4 lg + e is visible up to pos (groups
-// are aligned, so that the sum stays in 32 bits at the last position, too).
-// The usual group has all its keys visible, f >= 0 and vs >= 2^-80: then the
-// weight is one fma and one exp2, w = 2^(x f + log2 vs - m0), and the sum of p
-// is the sum of w / vs (an error of log2 vs is in both, and drops out). GEN
-// takes any: masked keys apart (a row with no key yet has m0 = -inf), a scale
-// of zero or NaN.
+// to be multiplied by (scale, q's unit, the keys' scale), per tile. Key `key` +
+// 16 u + 4 lg + e is visible up to pos (groups are aligned, so that the sum
+// stays in 32 bits at the last position, too).
+// The usual group has all its keys visible, f >= 0 and the values' scales vs >=
+// 2^-80: then the weight is one fma and one exp2, w = 2^(x f + lv - m0), and the
+// sum of p is the sum of w rv, with v = lv = log2 vs and rv = 1 / vs (an error
+// of lv is in both, and drops out). GEN takes any, v = vs: masked keys apart (a
+// row with no key yet has m0 = -inf), a scale of zero or NaN.
 template <int UN, bool GEN>
-__device__ __forceinline__ float softmax_step(float (&x)[UN][4], const float (&f)[UN], const float (&vs)[UN], uint32_t key, uint32_t pos,
-                                              float &mrun, float &lsum, f16x8 (&ph)[UN / 2], f16x8 (&pl)[UN / 2]) {
+__device__ __forceinline__ float softmax_step(const float (&x)[UN][4], const float (&f)[UN], const float (&v)[UN], const float (&rv)[UN],
+                                              uint32_t key, uint32_t pos, float &mrun, float &lsum, f16x8 (&ph)[UN / 2],
+                                              f16x8 (&pl)[UN / 2]) {
     const uint32_t k0 = key + ((threadIdx.x & 63) >> 4 << 2);
-    float tm = -INFINITY, lv[UN];
+    float tm = -INFINITY;
 #pragma unroll
     for (int u = 0; u < UN; u++) {
         if (GEN) {
-            lv[u] = __builtin_amdgcn_logf(fmaxf(fabsf(vs[u]), 0x1p-80f));
+            const float lv = __builtin_amdgcn_logf(fmaxf(fabsf(v[u]), 0x1p-80f));
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                x[u][e] = k0 + 16 * u + e <= pos ? x[u][e] * f[u] : -INFINITY;
-                tm = fmaxf(tm, x[u][e] + lv[u]);
+                tm = fmaxf(tm, k0 + 16 * u + e <= pos ? fmaf(x[u][e], f[u], lv) : -INFINITY);
             }
         } else {
-            lv[u] = __builtin_amdgcn_logf(vs[u]);
-            tm = fmaxf(tm, fmaf(fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])), f[u], lv[u]));
+            const float t = fmaf(max2(max3(x[u][0], x[u][1], x[u][2]), x[u][3]), f[u], v[u]);
+            tm = u ? max2(tm, t) : t;
         }
     }
-    tm = fmaxf(tm, swap16f(tm));
-    tm = fmaxf(tm, swap32f(tm));
-    const float mnew = fmaxf(mrun, tm), m0 = mnew - KV8_P2;
-    const float al = mrun == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrun - mnew);
+    const float mnew = rows_max(mrun, tm), m0 = mnew - KV8_P2;
+    const float al = GEN && mrun == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrun - mnew);
     mrun = mnew;
     float l = lsum * al;
 #pragma unroll
@@ -425,15 +445,15 @@ __device__ __forceinline__ float softmax_step(float (&x)[UN][4], const float (&f
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const bool vis = k0 + 16 * u + e <= pos;
-                const float p = vis ? __builtin_amdgcn_exp2f(x[u][e] - m0) : 0.0f;
+                const float p = vis ? __builtin_amdgcn_exp2f(fmaf(x[u][e], f[u], -m0)) : 0.0f;
                 l += p;
-                w[e] = vis ? p * vs[u] : 0.0f;
+                w[e] = vis ? p * v[u] : 0.0f;
             }
         } else {
-            const float c = lv[u] - m0;
+            const float c = v[u] - m0;
 #pragma unroll
             for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_exp2f(fmaf(x[u][e], f[u], c));
-            l = fmaf((w[0] + w[1]) + (w[2] + w[3]), __builtin_amdgcn_rcpf(vs[u]), l);
+            l = fmaf((w[0] + w[1]) + (w[2] + w[3]), rv[u], l);
         }
 #pragma unroll
         for (int e = 0; e < 4; e += 2) {
@@ -530,8 +550,10 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
         f16x8 ph[1], pl[1];
         const float f[2] = {qf * ks[0], qf * ks[1]};
         const bool usual = step * 32 + 31 <= first && scales_usual(fminf(ks[0], ks[1]), fminf(vs[0], vs[1]));
-        const float al2 = usual ? softmax_step<2, false>(sc, f, vs, 0, 0, mrun, lsum, ph, pl)
-                                : softmax_step<2, true>(sc, f, vs, step * 32, rpos, mrun, lsum, ph, pl);
+        const float lv[2] = {__builtin_amdgcn_logf(vs[0]), __builtin_amdgcn_logf(vs[1])};
+        const float rv[2] = {__builtin_amdgcn_rcpf(vs[0]), __builtin_amdgcn_rcpf(vs[1])};
+        const float al2 = usual ? softmax_step<2, false>(sc, f, lv, rv, 0, 0, mrun, lsum, ph, pl)
+                                : softmax_step<2, true>(sc, f, vs, rv, step * 32, rpos, mrun, lsum, ph, pl);
         if (__builtin_amdgcn_ballot_w64(al2 != 1.0f)) {
 #pragma unroll
             for (int n = 0; n < NT; n++) o[n] *= al2;
@@ -608,10 +630,8 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
     constexpr int KPT = (KCH + NTH - 1) / NTH, VPT = (VUN + NTH - 1) / NTH;
     __shared__ v4u kb[2][KCH];
     __shared__ v4u vb[2][2 * NT * 64];
-    __shared__ __align__(16) float sb[4][8];    // the tiles' scales (4 of keys, 4 of values): read up to two steps after the codes
     const uint32_t t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int grp = wave >> 2;
     const uint32_t hk = blockIdx.y, sp = blockIdx.z, S = gridDim.z, G = a.n_heads / a.n_kv;
     const uint64_t R = (uint64_t)a.ntok * G, r0 = (uint64_t)(gridDim.x - 1 - blockIdx.x) * KV8_ROWS;
     const uint32_t lastk = a.base + (uint32_t)((min(r0 + KV8_ROWS, R) - 1) / G);      // the block's last visible key
@@ -623,49 +643,85 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
     const float *scales = a.scales + 2 * hk;
     const size_t srec = 2 * (size_t)a.n_kv;
 
-    // This thread's chunks of tile i (counted from k0): a uniform address and an
-    // offset of its own, except in the tile that the cache's end cuts.
+    // This thread's chunks of a tile (counted from k0): a uniform address and an
+    // offset of its own, computed again only in the tile that the cache's end
+    // cuts. Every thread loads (chunks past the tile's are its first again),
+    // so that no wait for one load has to cover the next.
     v4u kr[KPT], vr[VPT][2];
-    float sr = 0.0f;
     const uint32_t rec32 = (uint32_t)rec;       // a record row is at most 2^29 bytes
-    auto load = [&](uint32_t i, bool k, bool v) {
+    uint32_t koff[KPT], voff[VPT];
+    auto k_at = [&](uint32_t t, int x, uint32_t last) {
+        const uint32_t c = (t + x * NTH) % KCH;
+        return min(c / (NC * 64), last) * rec32 + c % (NC * 64) * 16;
+    };
+    auto v_at = [&](uint32_t t, int x, int j, uint32_t last) {
+        const uint32_t c = (t + x * NTH) % VUN;
+        return min(c / (NC * 64) * 2 + j, last) * rec32 + c % (NC * 64) * 16 + KV8_T * HD;
+    };
+#pragma unroll
+    for (int x = 0; x < KPT; x++) koff[x] = k_at(t, x, 3);
+#pragma unroll
+    for (int x = 0; x < VPT; x++) voff[x] = v_at(t, x, 0, 3);
+    auto load_k = [&](uint32_t i) {
         const uint32_t r4 = 4 * (k0 + i), last = nrec - 1 - r4;     // records from the tile's first that exist
         const int8_t *p = codes + (size_t)r4 * rec;
-        const bool whole = last >= 3;
-        if (k) {
+        uint32_t at[KPT];
 #pragma unroll
-            for (int x = 0; x < KPT; x++) {
-                const uint32_t c = t + x * NTH, u = c / (NC * 64), w = c % (NC * 64) * 16;
-                if (KCH % NTH == 0 || c < KCH) kr[x] = *(const v4u *)(p + ((whole ? u : min(u, last)) * rec32 + w));
-            }
-        }
-        if (v) {
+        for (int x = 0; x < KPT; x++) at[x] = koff[x];
+        if (last < 3) {
+            uint32_t tc = t;
+            asm volatile("" : "+v"(tc));            // here and now, not in registers through the loop
 #pragma unroll
-            for (int x = 0; x < VPT; x++) {
-                const uint32_t c = t + x * NTH, u = c / (NC * 64) * 2, w = c % (NC * 64) * 16 + KV8_T * HD;
-                if (VUN % NTH == 0 || c < VUN) {
-                    vr[x][0] = *(const v4u *)(p + ((whole ? u : min(u, last)) * rec32 + w));
-                    vr[x][1] = *(const v4u *)(p + ((whole ? u + 1 : min(u + 1, last)) * rec32 + w));
-                }
-            }
+            for (int x = 0; x < KPT; x++) at[x] = k_at(tc, x, last);
         }
+#pragma unroll
+        for (int x = 0; x < KPT; x++) kr[x] = *(const v4u *)(p + at[x]);
     };
-    auto load_s = [&](uint32_t i) {     // the first eight threads: a scale each
-        if (t < 8) sr = scales[(size_t)(min(4 * (k0 + i) + t % 4, nrec - 1) >> bsh) * srec + t / 4];
+    auto load_v = [&](uint32_t i) {
+        const uint32_t r4 = 4 * (k0 + i), last = nrec - 1 - r4;
+        const int8_t *p = codes + (size_t)r4 * rec;
+        uint32_t at[VPT][2];
+#pragma unroll
+        for (int x = 0; x < VPT; x++) { at[x][0] = voff[x]; at[x][1] = voff[x] + rec32; }
+        if (last < 3) {
+            uint32_t tc = t;
+            asm volatile("" : "+v"(tc));
+#pragma unroll
+            for (int x = 0; x < VPT; x++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) at[x][j] = v_at(tc, x, j, last);
+        }
+#pragma unroll
+        for (int x = 0; x < VPT; x++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) vr[x][j] = *(const v4u *)(p + at[x][j]);
+    };
+    // A tile's scales, one to a lane: lane j holds record j % 4's of its keys (j
+    // / 4 % 2 == 0) or values. 4 T >> bsh plus j >> bsh is (4 T + j) >> bsh.
+    const uint32_t soff = ((lane & 3) >> bsh) * (uint32_t)srec + (lane >> 2 & 1);
+    float sn;
+    auto load_s = [&](uint32_t i) {
+        const uint32_t r4 = 4 * (k0 + i), last = nrec - 1 - r4;
+        uint32_t at = soff;
+        if (last < 3) {
+            uint32_t lc = lane;
+            asm volatile("" : "+v"(lc));
+            at = (min(lc & 3, last) >> bsh) * (uint32_t)srec + (lc >> 2 & 1);
+        }
+        sn = (scales + (size_t)(r4 >> bsh) * srec)[at];
     };
     auto stage_k = [&](uint32_t i) {
 #pragma unroll
         for (int x = 0; x < KPT; x++) {
             const uint32_t c = t + x * NTH;
-            if (KCH % NTH == 0 || c < KCH) kb[i & 1][c] = kr[x];
+            if (KCH % NTH == 0 || wave * 64 + x * NTH < KCH) kb[i & 1][c] = kr[x];
         }
-        if (t < 8) sb[i & 3][t] = sr;
     };
     auto stage_v = [&](uint32_t i) {
 #pragma unroll
         for (int x = 0; x < VPT; x++) {
             const uint32_t c = t + x * NTH;
-            if (VUN % NTH == 0 || c < VUN)
+            if (VUN % NTH == 0 || wave * 64 + x * NTH < VUN)
 #pragma unroll
                 for (int j = 0; j < 4; j++)         // fragment (pair of tiles, dims 16 (4 c + j) ..)
                     vb[i & 1][(c / 64 * 4 + j) * 64 + c % 64] = __builtin_bit_cast(v4u, codes_f16(vr[x][0][j], vr[x][1][j]));
@@ -676,7 +732,7 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
     const uint32_t tok = r < R ? (uint32_t)r / G : 0, head = hk * G + (r < R ? (uint32_t)r % G : 0), rpos = a.base + tok;
     float xq[NC][16];
     q_load<NC>(a.q + tok * a.q_tok + (size_t)head * a.q_stride, r < R, al, lg, xq);
-    if (n) { load(0, true, false); load_s(0); }
+    if (n) load_k(0);
     v4i qd[3][NC];
     const float qf = q_row<NC>(xq, a.scale * 1.44269504088896340736f, qd);
     float mrun = -INFINITY, lsum = 0.0f, resc = 1.0f;
@@ -731,14 +787,20 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
             }
         }
     };
-    auto weights = [&](uint32_t i) {
-        const f32x4 k4 = *(const f32x4 *)&sb[i & 3][0], v4 = *(const f32x4 *)&sb[i & 3][4];
-        const float vs[4] = {v4[0], v4[1], v4[2], v4[3]}, f[4] = {qf * k4[0], qf * k4[1], qf * k4[2], qf * k4[3]};
+    auto weights = [&](uint32_t i, float sv) {
+        auto from = [](float v, int j) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), j)); };
         const uint32_t key = (k0 + i) * 64;
-        const bool usual = key + 63 <= wfirst && scales_usual(fminf(fminf(k4[0], k4[1]), fminf(k4[2], k4[3])),
-                                                              fminf(fminf(v4[0], v4[1]), fminf(v4[2], v4[3])));
-        resc = usual ? softmax_step<4, false>(sc, f, vs, 0, 0, mrun, lsum, ph, pl)
-                     : softmax_step<4, true>(sc, f, vs, key, rpos, mrun, lsum, ph, pl);
+        const float f[4] = {qf * from(sv, 0), qf * from(sv, 1), qf * from(sv, 2), qf * from(sv, 3)};
+        const float lg2 = __builtin_amdgcn_logf(sv), rc = __builtin_amdgcn_rcpf(sv);
+        const float rv[4] = {from(rc, 4), from(rc, 5), from(rc, 6), from(rc, 7)};
+        const float least = lane & 4 ? 0x1p-80f : 0.0f;
+        if (key + 63 <= wfirst && !__builtin_amdgcn_ballot_w64(!(sv >= least))) {
+            const float lv[4] = {from(lg2, 4), from(lg2, 5), from(lg2, 6), from(lg2, 7)};
+            resc = softmax_step<4, false>(sc, f, lv, rv, 0, 0, mrun, lsum, ph, pl);
+        } else {
+            const float vs[4] = {from(sv, 4), from(sv, 5), from(sv, 6), from(sv, 7)};
+            resc = softmax_step<4, true>(sc, f, vs, rv, key, rpos, mrun, lsum, ph, pl);
+        }
     };
 
     ph[0] = ph[1] = pl[0] = pl[1] = (f16x8){};
@@ -747,34 +809,44 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
         if (2 * NT * 64 % NTH == 0 || t + x < 2 * NT * 64) vb[1][t + x] = (v4u){0, 0, 0, 0};
     if (n) {
         stage_k(0);
-        load(1, n > 1, false);
-        if (n > 1) load_s(1);
-        load(0, false, true);
+        load_k(min(1u, n - 1));
+        load_v(0);
+        load_s(0);
     }
     lds_barrier();
     // Period i (two steps, one barrier): group 0 does the products of tile i and
     // the softmax of i, group 1 the softmax of i - 1 and the products of i. Read
     // are the keys of tile i and the values of i - 1; written, in a wave's
     // softmax step, the keys of i + 1 and the values of i, requested a period ago.
-    for (uint32_t h = 0; n && h < 2 * n + 2; h++) {
-        const int x = (int)h - grp, i = x >> 1;
-        if (!(x & 1)) {
-            if (ntw) products(i);
+    // Past the last tile it stages that one again, where nobody reads it.
+    // A loop for each group: with the two orders in one the compiler keeps the
+    // state of both at the branch, 60 moves a step and a wait for the loads.
+    auto soften = [&](uint32_t next, int i) {
+        stage_k(next + 1);
+        stage_v(next);
+        const float sv = sn;
+        load_k(min(next + 2, n - 1));
+        load_v(min(next + 1, n - 1));
+        load_s(min((uint32_t)(i + 1), n - 1));
+        if (i >= 0 && (uint32_t)i < ntw) {
+            weights(i, sv);
         } else {
-            const uint32_t next = h >> 1;
-            if (next + 1 < n) stage_k(next + 1);
-            if (next < n) stage_v(next);
-            load(next + 2, next + 2 < n, false);
-            if (next + 2 < n) load_s(next + 2);
-            load(next + 1, false, next + 1 < n);
-            if (i >= 0 && (uint32_t)i < ntw) {
-                weights(i);
-            } else {
-                ph[0] = ph[1] = pl[0] = pl[1] = (f16x8){};
-                resc = 1.0f;
-            }
+            ph[0] = ph[1] = pl[0] = pl[1] = (f16x8){};
+            resc = 1.0f;
         }
-        if (h & 1) lds_barrier();
+    };
+    if (n && wave < KV8_NW / 2) {
+        for (uint32_t i = 0; i <= n; i++) {
+            products(i);
+            soften(i, (int)i);
+            lds_barrier();
+        }
+    } else if (n) {
+        for (uint32_t i = 0; i <= n; i++) {
+            soften(i, (int)i - 1);
+            products(i);
+            lds_barrier();
+        }
     }
     lsum += swap16f(lsum);
     lsum += swap32f(lsum);
