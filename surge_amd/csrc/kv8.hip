@@ -530,7 +530,9 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
 #pragma unroll
     for (int n = 0; n < NT; n++) o[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     float mrun = -INFINITY, lsum = 0.0f;
-    for (; step < s1; step += NW) {
+    // The last step stands apart: with its missing loads in the loop, waiting for
+    // a step's keys is waiting for its values as well.
+    auto work = [&](bool more) {
         float sc[2][4];
 #pragma unroll
         for (int u = 0; u < 2; u++) { ks[u] = nks[u]; vs[u] = nvs[u]; }
@@ -545,7 +547,6 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
 #pragma unroll
             for (int e = 0; e < 4; e++) sc[u][e] = q_join(s[0][e], s[1][e], s[2][e]);
         }
-        const bool more = step + NW < s1;
         if (more) { load_s(step + NW); load_k(step + NW); }
         f16x8 ph[1], pl[1];
         const float f[2] = {qf * ks[0], qf * ks[1]};
@@ -567,7 +568,9 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
                 o[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[0], o[4 * c + j], 0, 0, 0);
             }
         if (more) load_v(step + NW);
-    }
+    };
+    for (; step + NW < s1; step += NW) work(true);
+    if (any) work(false);
     // join the waves that had a step: each leaves its maximum, sum and output, one barrier
     const uint32_t waves = min(s1 - s0, (uint32_t)NW);
     lsum += swap16f(lsum);
@@ -747,12 +750,12 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
     f16x8 ph[2], pl[2];
     // Step of products, tile i: P V of tile i - 1, K Q^T of tile i. The other
     // wave of the SIMD is in its softmax, so the wave has to cover the LDS reads
-    // itself: fragments go through a ring of eight, each requested seven ahead
-    // (14 products, 224 cycles), and the two halves of a P V pair are two
+    // itself: fragments go through a ring of five, each requested four ahead (8
+    // products, 128 cycles), and the two halves of a P V pair are two
     // products apart. At the ends it multiplies zeros (no tile -1: its weights
     // and values are) or what nobody reads (no tile n).
     auto products = [&](uint32_t i) {
-        constexpr int NV = 2 * NT, NK = 4 * NC, RING = 8;
+        constexpr int NV = 2 * NT, NK = 4 * NC, RING = 5;
         const v4u *vt = vb[(i + 1) & 1] + lane, *kt = kb[i & 1] + lane;
         v4u fr[RING];
         auto fetch = [&](int k) {
@@ -787,18 +790,18 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
             }
         }
     };
-    auto weights = [&](uint32_t i, float sv) {
+    auto weights = [&](uint32_t i) {
         auto from = [](float v, int j) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), j)); };
         const uint32_t key = (k0 + i) * 64;
-        const float f[4] = {qf * from(sv, 0), qf * from(sv, 1), qf * from(sv, 2), qf * from(sv, 3)};
-        const float lg2 = __builtin_amdgcn_logf(sv), rc = __builtin_amdgcn_rcpf(sv);
+        const float f[4] = {qf * from(sn, 0), qf * from(sn, 1), qf * from(sn, 2), qf * from(sn, 3)};
+        const float lg2 = __builtin_amdgcn_logf(sn), rc = __builtin_amdgcn_rcpf(sn);
         const float rv[4] = {from(rc, 4), from(rc, 5), from(rc, 6), from(rc, 7)};
         const float least = lane & 4 ? 0x1p-80f : 0.0f;
-        if (key + 63 <= wfirst && !__builtin_amdgcn_ballot_w64(!(sv >= least))) {
+        if (key + 63 <= wfirst && !__builtin_amdgcn_ballot_w64(!(sn >= least))) {
             const float lv[4] = {from(lg2, 4), from(lg2, 5), from(lg2, 6), from(lg2, 7)};
             resc = softmax_step<4, false>(sc, f, lv, rv, 0, 0, mrun, lsum, ph, pl);
         } else {
-            const float vs[4] = {from(sv, 4), from(sv, 5), from(sv, 6), from(sv, 7)};
+            const float vs[4] = {from(sn, 4), from(sn, 5), from(sn, 6), from(sn, 7)};
             resc = softmax_step<4, true>(sc, f, vs, rv, key, rpos, mrun, lsum, ph, pl);
         }
     };
@@ -824,16 +827,15 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
     auto soften = [&](uint32_t next, int i) {
         stage_k(next + 1);
         stage_v(next);
-        const float sv = sn;
         load_k(min(next + 2, n - 1));
         load_v(min(next + 1, n - 1));
-        load_s(min((uint32_t)(i + 1), n - 1));
         if (i >= 0 && (uint32_t)i < ntw) {
-            weights(i, sv);
+            weights(i);
         } else {
             ph[0] = ph[1] = pl[0] = pl[1] = (f16x8){};
             resc = 1.0f;
         }
+        load_s(min((uint32_t)(i + 1), n - 1));
     };
     if (n && wave < KV8_NW / 2) {
         for (uint32_t i = 0; i <= n; i++) {
