@@ -31,7 +31,9 @@ __device__ __forceinline__ uint32_t val_at(uint32_t r, uint32_t d) {
 // row at a time, a wave taking 8 rows x 32 dims (whole lines of the rows, 128
 // bytes of codes at a time); values 4 positions x 4 dims, transposed in
 // registers into a dword per dim. 4 U fours per thread. Rows before base keep
-// their codes unless the scale grows.
+// their codes unless the scale grows. Bound by memory: 8190 rows of 4 x 256 (84
+// MB) 25.6 us in a trace with fresh inputs, 19 with the rows in the last cache;
+// a copy of as many bytes takes 17-18. One row 4.6: load, maximum, codes in turn.
 // ---------------------------------------------------------------------------
 struct kv8_store_args {
     const float *x[2];
@@ -208,7 +210,8 @@ extern "C" hipError_t sgk_kv8_store(const float *k, const float *v, uint64_t str
 }
 
 // ---------------------------------------------------------------------------
-// Load: hd threads per (tile, kv head, half), whole waves; fours as above.
+// Load: hd threads per (tile, kv head, half), whole waves; fours as above. Bound
+// by memory: the 84 MB above 15.1 us, 5.6 TB/s; one block 3.0.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(TPB) k_kv8_load(const int8_t *codes, const float *scales, float *k, float *v,
                                                   uint64_t stride, uint32_t n_kv, uint32_t hd, uint32_t block,
@@ -286,7 +289,9 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
 //    2^12 keeps w's lower half above f16's subnormals down to 2^-26 of the
 //    largest.
 // No barrier or LDS in the key loop; the waves' maxima, sums and outputs join
-// at the end. Bound by the cache's bytes.
+// at the end. Bound by the cache's bytes: 262000 keys of 4 x 256 (537 MB) 86 us,
+// 6.2 TB/s, where a plain read reaches 6.6; 32771 of 8 x 128 (67 MB) 15.3, with
+// the waves' start and end in it; 700 of 2 x 256 7.2, one step's chain.
 // ---------------------------------------------------------------------------
 struct kv8_part { float *m, *s, *acc; };    // [token][head][split] maxima and sums, [..][hd] outputs; NULL: one split
 
@@ -610,14 +615,20 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
 // all of them: the key codes as they lie (1 KB per operand fragment, 16 bytes
 // a lane, no bank conflict), the value codes turned into f16 on the way. The
 // arithmetic is the wave form's.
-// A tile's work is matrix products (112 instructions of 16 cycles at head_dim
-// 256) and softmax (340 vector instructions of 4 cycles and more). Waves that
-// run it in step leave the matrix units idle through the softmax: 46% busy.
-// So a wave alternates steps of products (the last tile's P V, this one's
-// K Q^T) and steps of softmax, and the two waves of a SIMD (w and w + 4) are
-// one step apart, a barrier after every two steps: one is in its products while
-// the other is in its softmax. Both tiles are double-buffered; a wave stores its
-// part of the next one and requests that of the one after before its softmax.
+// A tile's work for a wave is 112 matrix products of 16 cycles (head_dim 256)
+// and about 230 vector instructions. Waves that run both in step leave the
+// matrix unit idle through the softmax: 46% busy. So the two waves of a SIMD (w
+// and w + 4) alternate: one is in its products (the last tile's P V, this one's
+// K Q^T) while the other is in its softmax, with a barrier a tile. Beside a
+// wave that keeps the matrix unit busy another issues two vector instructions
+// per product (measured), so 224 products and 460 of those take at least 4100
+// cycles; a tile takes 4800, of which 3584 are the products'.
+// Both tiles are double-buffered; a wave stores its part of the next one and
+// requests that of the one after before its softmax.
+// 24 heads of 256 on 4, 2048 rows at 14336: 1050-1100 us, 720 TFLOP/s of the
+// formula's, and as the matrix unit counts them (weights in two halves, three
+// digits at twice the rate) 1270, where a plain f16 product of 16384^3 reaches
+// 1346: the clock falls to 1.7 GHz under either.
 // Grid: (row block, kv head, key split), the longest rows first.
 // ---------------------------------------------------------------------------
 #define KV8_NW 8
@@ -868,7 +879,8 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
 }
 
 // Join of few splits of many rows: four dims of a row per lane, all splits'
-// loads in flight, nothing shared between lanes. Every row sees key 0, so the
+// loads in flight, nothing shared between lanes (49152 rows of 256, two splits,
+// 151 MB: 23 us). Every row sees key 0, so the
 // largest maximum is a number, and a split without a key weighs nothing; NaN
 // sums reach the output.
 #define KV8_JOIN 8u
@@ -900,7 +912,7 @@ __global__ void __launch_bounds__(TPB) k_kv8_join(kv8_part p, float *out, uint64
 
 // Join of many splits of few rows: a workgroup per row and 64 dims, 16 lanes of
 // four dims for every 16th split; the first four splits of a lane are asked
-// for before the weights.
+// for before the weights. Bound by that chain: 24 rows of 256, 64 splits 4.1 us.
 #define KV8_COMB 512u
 __global__ void __launch_bounds__(TPB) k_kv8_comb(kv8_part p, float *out, uint32_t hd, uint32_t S, int al) {
     __shared__ float wt[KV8_COMB], red[4], sum[4];
@@ -963,11 +975,12 @@ __global__ void __launch_bounds__(TPB) k_kv8_comb(kv8_part p, float *out, uint32
 // where that shortens the launch: rounds x (a part's tiles + KV8_TAIL for its
 // start and end) tiles of KV8_TILE_US, against the partials' way to memory and
 // back. KV8_SMALL, in waves' steps of 32 keys x head_dim, is where the two meet
-// (wave / tile): 24 heads of 256 on 4, 8040 keys, 240 rows (3.9M) 45.5 / 51.2,
-// 8077 keys, 462 rows (7.5M) 62.7 / 62.9, 1300 keys, 1800 rows (4.7M) 44.2 /
-// 55.0; 32 of 128 on 8, 8020 keys, 80 rows (1.3M) 28.3 / 34.6, 8077 keys, 308
-// rows (5.2M) 60.9 / 53.7; 12 of 64, 32077 keys, 77 rows (3.9M) 50.6 / 58.9.
-#define KV8_SMALL (1ull << 22)
+// (wave / tile): 24 heads of 256 on 4, 8040 keys, 240 rows (3.9M) 42.9 / 48.5,
+// 1300 keys, 1800 rows (4.7M) 42.0 / 51.4, 8077 keys, 462 rows (7.5M) 58.3 /
+// 58.6, 32020 keys, 120 rows (8.2M) 58.7 / 56.4; 32 of 128 on 8, 8040 keys, 160
+// rows (2.6M) 32.8 / 40.5, 32020 keys, 80 rows (5.1M) 47.2 / 50.8, 8077 keys, 308
+// rows (5.2M) 52.2 / 49.5; 12 of 64, 32077 keys, 77 rows (3.9M) 46.4 / 55.6.
+#define KV8_SMALL (5ull << 20)
 #define KV8_ONE 16
 #define KV8_TILE_US 2.5         /* at head_dim 256 */
 #define KV8_TAIL 3.0

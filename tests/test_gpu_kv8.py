@@ -377,7 +377,8 @@ def test_cache_past_32_bits(gpu):
 
 @pytest.mark.parametrize("nh,nkv,hd,block,base,n", [
     (24, 4, 256, 64, 3001, 203), (32, 8, 128, 16, 3000, 301), (12, 12, 64, 32, 8000, 401), (16, 1, 256, 128, 0, 800),
-    (6, 2, 256, 64, 20000, 121), (10, 2, 128, 32, 15, 1500)])
+    (6, 2, 256, 64, 20000, 121), (10, 2, 128, 32, 15, 1500), (16, 1, 256, 128, 0, 1000), (8, 4, 64, 16, 6000, 1003),
+    (5, 1, 64, 64, 30000, 310)])
 def test_prefill_tiles(gpu, nh, nkv, hd, block, base, n):
     rng = np.random.default_rng(n)
     c = filled(rng, nkv, hd, block, base + n)
