@@ -327,6 +327,7 @@ __device__ __forceinline__ void q_load(const float *q, bool on, bool al, uint32_
             for (int e = 0; e < 4; e++) x[c][4 * w + e] = v[e];
         }
 }
+#define KV8_QMAX (127.0f * 65536.0f)        // the row's largest element in units of its digits
 // It as digits; returns the factor of the integer scores, sq * |mul|, NaN if an
 // element is not finite.
 template <int NC>
@@ -342,14 +343,14 @@ __device__ __forceinline__ float q_row(float (&x)[NC][16], float mul, v4i (&d)[3
     float am = bad ? 0.0f : __uint_as_float(mx);
     const float up = am < 0x1p-60f ? 0x1p64f : 1.0f;    // a row near the end of the range, times 2^64
     am *= up;
-    const float inv = am > 0.0f ? copysignf(8323072.0f / am, mul) : 0.0f;       // 127 * 65536; a negative scale turns q
+    const float inv = am > 0.0f ? copysignf(KV8_QMAX / am, mul) : 0.0f;       // a negative scale turns q
 #pragma unroll
     for (int c = 0; c < NC; c++) {
 #pragma unroll
         for (int e = 0; e < 16; e++) x[c][e] = bad ? 0.0f : x[c][e] * up;
         q_digits(x[c], inv, d[0][c], d[1][c], d[2][c]);
     }
-    return bad ? NAN : am / 8323072.0f * fabsf(mul) / up;
+    return bad ? NAN : am / KV8_QMAX * fabsf(mul) / up;
 }
 // the score sums of the three digits as one float (a2 * 256 + a1 < 2^31)
 __device__ __forceinline__ float q_join(int a0, int a1, int a2) {
@@ -616,12 +617,12 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
 // a lane, no bank conflict), the value codes turned into f16 on the way. The
 // arithmetic is the wave form's.
 // A tile's work for a wave is 112 matrix products of 16 cycles (head_dim 256)
-// and about 230 vector instructions. Waves that run both in step leave the
+// and about 265 vector instructions. Waves that run both in step leave the
 // matrix unit idle through the softmax: 46% busy. So the two waves of a SIMD (w
 // and w + 4) alternate: one is in its products (the last tile's P V, this one's
 // K Q^T) while the other is in its softmax, with a barrier a tile. Beside a
 // wave that keeps the matrix unit busy another issues two vector instructions
-// per product (measured), so 224 products and 460 of those take at least 4100
+// per product (measured), so 224 products and 530 of those take at least 4200
 // cycles; a tile takes 4800, of which 3584 are the products'.
 // Both tiles are double-buffered; a wave stores its part of the next one and
 // requests that of the one after before its softmax.

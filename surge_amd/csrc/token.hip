@@ -221,7 +221,7 @@ extern "C" hipError_t sgk_token_counts(const int32_t *ids, uint32_t *counts, uin
 // addresses allow. Bound by the latency of its two launches: 151936 ids, 1 row
 // 4.2 + 2.6 us; 16 rows (29 MB) 9.4 + 2.5-4.
 // ---------------------------------------------------------------------------
-#define LG_WGS 3072u         // workgroups of all rows together, at most; a row has at least one
+#define LG_WGS 3200u         // workgroups of all rows together, at most; a row has at least one
 struct lg_best { float v; uint32_t i; };
 #define LG_NONE 0xFFFFFFFFu
 
