@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from typing import Optional, Sequence
 
 import numpy as np
@@ -222,11 +223,15 @@ def check(err: SgErr) -> None:
         raise SurgeError(err.msg.decode())
 
 
+_Params = C.c_uint32 * 8
+_pack_params = struct.Struct("8I").pack
+
+
 def params(vals: Sequence[int]) -> C.Array:
-    p = (C.c_uint32 * 8)()
-    for i, v in enumerate(vals):
-        p[i] = int(v) & 0xFFFFFFFF
-    return p
+    try:                            # 0.4 us; an element at a time 1.0
+        return _Params.from_buffer_copy(_pack_params(*vals, *(0,) * (8 - len(vals))))
+    except (struct.error, TypeError):
+        return _Params(*(int(v) & 0xFFFFFFFF for v in vals))
 
 
 def fbits(x: float) -> int:
