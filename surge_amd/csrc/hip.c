@@ -1031,8 +1031,6 @@ sg_err sg_gpu_run_attn_prefill_kv8(sg_gpu *g, void *q, void *codes, void *scales
     return attn_kv8_oneshot(g, "attn_prefill_kv8", q, codes, scales, out, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
 }
 
-static void rope_inv_freq(double inv[SGK_ROPE_HALF], uint32_t rd, float theta);
-
 sg_err sg_gpu_run_rope_axes(sg_gpu *g, void *x, void *pos, void *out, const uint32_t p[8]) {
     if (!g || !x || !pos || !out || !p) return (sg_err){"gpu: rope_axes got a NULL argument"};
     const uint32_t hd = p[0], rd = p[1], nh = p[2], hs = p[3] ? p[3] : hd, n = p[4], half = rd / 2;
@@ -1047,24 +1045,18 @@ sg_err sg_gpu_run_rope_axes(sg_gpu *g, void *x, void *pos, void *out, const uint
     if (order > 1 || sec[0] + sec[1] + sec[2] != half) return (sg_err){"gpu: rope_axes: sections must add up to rope_dim / 2, order 0 or 1"};
     if (order && ((sec[1] && 3 * sec[1] - 2 >= half) || (sec[2] && 3 * sec[2] - 1 >= half)))
         return (sg_err){"gpu: rope_axes: sections do not fit the interleaved order"};
-    uint8_t axis[SGK_ROPE_HALF];
-    for (uint32_t i = 0; i < half; i++) {
-        const uint32_t m = i % 3;
-        axis[i] = (uint8_t)(order ? (m && i < 3 * sec[m] ? m : 0) : i < sec[0] ? 0 : i < sec[0] + sec[1] ? 1 : 2);
-    }
     sg_err e;
     const uint64_t bytes = ((n - 1) * row + w) * 4;
     if (sg_failed(e = need(x, bytes, "x")) || sg_failed(e = need(out, bytes, "out")) || sg_failed(e = need(pos, 12ull * n, "pos"))) return e;
     if (!aligned(x, 4) || !aligned(out, 4) || !aligned(pos, 4)) return (sg_err){"gpu: rope_axes: buffers must be 4-byte aligned"};
     if (overlap(out, pos) || (overlap(out, x) && DEV(out) != DEV(x))) return (sg_err){"gpu: rope_axes: out overlaps an input"};
-    double inv[SGK_ROPE_HALF];
-    rope_inv_freq(inv, rd, theta);
     int was;
     if (sg_failed(e = on_device(g, &was))) return e;
     void *ins[3] = {x, pos, out}, *outs[1] = {out};     /* out too: its gaps stay as they are */
     if (!sg_failed(e = push(ins, out == x ? 2 : 3))) {
-        const sgk_rope_axes_args a = {DEV(x), DEV(pos), DEV(out), row, hd, rd, nh, hs, n};
-        e = finish_done(g, sgk_rope_axes(&a, inv, axis, g->stream, g->done), outs, 1);
+        const sgk_rope_axes_args a = {DEV(x), DEV(pos), DEV(out), row, -2.0 * log2((double)theta) / rd, hd, rd, nh, hs, n,
+                                      {sec[0], sec[1], sec[2]}, order};
+        e = finish_done(g, sgk_rope_axes(&a, g->stream, g->done), outs, 1);
     }
     return back_to(g, was, e);
 }

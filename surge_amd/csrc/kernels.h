@@ -400,16 +400,17 @@ typedef struct {
 uint64_t sgk_kv8_attn_scratch(const sgk_kv8_attn *a);
 hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hipStream_t s, hipEvent_t done);
 
-/* Rotary positions with three axes (token.hip). inv and axis: rope_dim/2
- * inverse frequencies and axes (host memory, read before return). */
+/* Rotary positions with three axes (token.hip): pair i turns by pos[axis(i)] *
+ * 2^(i step), axis(i) from the sections and the order as in surge.h. */
 typedef struct {
     const float *x;
     const int32_t *pos;         /* [3][n] */
     float *out;
     uint64_t row;               /* floats between tokens */
-    uint32_t head_dim, rope_dim, heads, stride, n;
+    double step;                /* -2 log2(theta) / rope_dim */
+    uint32_t head_dim, rope_dim, heads, stride, n, sections[3], order;
 } sgk_rope_axes_args;
-hipError_t sgk_rope_axes(const sgk_rope_axes_args *a, const double *inv, const uint8_t *axis, hipStream_t s, hipEvent_t done);
+hipError_t sgk_rope_axes(const sgk_rope_axes_args *a, hipStream_t s, hipEvent_t done);
 
 /* counts[row][id] += occurrences; cleared first with clear != 0 (n == 0 without
  * it is refused). */
