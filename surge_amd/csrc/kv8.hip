@@ -293,7 +293,24 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
 // 6.2 TB/s, where a plain read reaches 6.6; 32771 of 8 x 128 (67 MB) 15.3, with
 // the waves' start and end in it; 700 of 2 x 256 7.2, one step's chain.
 // ---------------------------------------------------------------------------
-struct kv8_part { float *m, *s, *acc; };    // [token][head][split] maxima and sums, [..][hd] outputs; NULL: one split
+// What a launch is divided by, with floor(2^32 / d) + 1 (2^32 / d where that is
+// whole): the compiler's division of any two numbers is some 25 dependent
+// instructions, and a wave has several before its first load.
+struct kv8_div { uint32_t d, inv; };
+struct kv8_part {
+    float *m, *s, *acc;         // [token][head][split] maxima and sums, [..][hd] outputs; NULL: one split
+    kv8_div group, splits;      // query heads of a kv head
+};
+__device__ __forceinline__ uint32_t div_by(uint32_t n, kv8_div v) {     // n < 2^31
+    const uint32_t q = v.d == 1 ? n : __umulhi(n, v.inv);
+    return q - (q * v.d > n);
+}
+// Part sp of n units: the first n % splits parts have one more.
+__device__ __forceinline__ void part_of(uint32_t n, uint32_t sp, kv8_div splits, uint32_t &first, uint32_t &end) {
+    const uint32_t q = div_by(n, splits), more = n - q * splits.d;
+    first = sp * q + min(sp, more);
+    end = first + q + (sp < more);
+}
 
 #define KV8_P2 12.0f
 
@@ -483,12 +500,13 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
     __shared__ __align__(16) float ob[NW][16 * OLD];
     const uint32_t t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const uint32_t hk = blockIdx.y, sp = blockIdx.x, S = gridDim.x, G = a.n_heads / a.n_kv;
-    const uint32_t r0 = blockIdx.z * 16, R = min(a.ntok * G - r0, 16u), first = a.base + r0 / G;    // first: visible to all rows
-    const uint32_t ntile = (a.base + (r0 + R - 1) / G) / KV8_T + 1, nstep = (ntile + 1) / 2;
-    const uint32_t s0 = (uint32_t)((uint64_t)sp * nstep / S), s1 = (uint32_t)((uint64_t)(sp + 1) * nstep / S);
+    const uint32_t hk = blockIdx.y, sp = blockIdx.x, S = part.splits.d, G = part.group.d;
+    const uint32_t r0 = blockIdx.z * 16, R = min(a.ntok * G - r0, 16u), first = a.base + div_by(r0, part.group);    // first: visible to all rows
+    const uint32_t ntile = (a.base + div_by(r0 + R - 1, part.group)) / KV8_T + 1, nstep = (ntile + 1) / 2;
+    uint32_t s0, s1;
+    part_of(nstep, sp, part.splits, s0, s1);
     const uint32_t bsh = __builtin_ctz(a.block / KV8_T);
-    const uint32_t tok = (r0 + min(li, R - 1)) / G, head = hk * G + (r0 + min(li, R - 1)) % G, rpos = a.base + tok;
+    const uint32_t row_of = r0 + min(li, R - 1), tok = div_by(row_of, part.group), head = hk * G + row_of - tok * G, rpos = a.base + tok;
     const int8_t *codes = a.codes + (size_t)hk * (2 * KV8_T * HD) + lane * 16;
     const size_t rec = (size_t)a.n_kv * (2 * KV8_T * HD);
     const float *scales = a.scales + 2 * hk;
@@ -577,11 +595,11 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
     };
     for (; step + NW < s1; step += NW) work(true);
     if (any) work(false);
-    // join the waves that had a step: each leaves its maximum, sum and output, one barrier
-    const uint32_t waves = min(s1 - s0, (uint32_t)NW);
+    // join the waves: each leaves its maximum, sum and output (-inf and zeros
+    // without a step), one barrier. All of a row's are asked for at once.
     lsum += swap16f(lsum);
     lsum += swap32f(lsum);
-    if (any && li < R) {
+    if (li < R) {
         if (lg == 0) { wm[wave][li] = mrun; wl[wave][li] = lsum; }
         float *dst = &ob[wave][li * OLD + 4 * lg];
 #pragma unroll
@@ -590,15 +608,20 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
     __syncthreads();
     for (uint32_t i = t; i < R * (HD / 4); i += NW * 64) {
         const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
-        float m = -INFINITY, l = 0.0f;
-        for (uint32_t w = 0; w < waves; w++) m = fmaxf(m, wm[w][r]);
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        for (uint32_t w = 0; w < waves; w++) {
-            const float f = wm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wm[w][r] - m);
+        float wmx[NW], m = -INFINITY, l = 0.0f;
+        f32x4 ov[NW], v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; w++) { wmx[w] = wm[w][r]; ov[w] = *(const f32x4 *)&ob[w][r * OLD + d]; }
+#pragma unroll
+        for (int w = 0; w < NW; w++) m = fmaxf(m, wmx[w]);
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float f = wmx[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wmx[w] - m);
             l = fmaf(wl[w][r], f, l);
-            v += *(const f32x4 *)&ob[w][r * OLD + d] * f;
+            v += ov[w] * f;
         }
-        const size_t row = (size_t)((r0 + r) / G) * a.n_heads + hk * G + (r0 + r) % G;
+        const uint32_t z = div_by(r0 + r, part.group);
+        const size_t row = (size_t)z * a.n_heads + hk * G + (r0 + r - z * G);
         if (S == 1) {
             st4(a.out + row * HD + d, v / l, !((uintptr_t)a.out & 15));
         } else {
@@ -647,11 +670,13 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
     __shared__ v4u vb[2][2 * NT * 64];
     const uint32_t t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const uint32_t hk = blockIdx.y, sp = blockIdx.z, S = gridDim.z, G = a.n_heads / a.n_kv;
+    const uint32_t hk = blockIdx.y, sp = blockIdx.z, S = part.splits.d, G = part.group.d;
     const uint64_t R = (uint64_t)a.ntok * G, r0 = (uint64_t)(gridDim.x - 1 - blockIdx.x) * KV8_ROWS;
-    const uint32_t lastk = a.base + (uint32_t)((min(r0 + KV8_ROWS, R) - 1) / G);      // the block's last visible key
+    const uint32_t lastk = a.base + div_by((uint32_t)(min(r0 + KV8_ROWS, R) - 1), part.group);      // the block's last visible key
     const uint32_t nrec = lastk / KV8_T + 1, nt = lastk / 64 + 1;
-    const uint32_t k0 = (uint32_t)((uint64_t)sp * nt / S), n = (uint32_t)((uint64_t)(sp + 1) * nt / S) - k0;    // tiles k0 .. k0 + n - 1
+    uint32_t k0, k1;
+    part_of(nt, sp, part.splits, k0, k1);
+    const uint32_t n = k1 - k0;             // tiles k0 .. k0 + n - 1
     const uint32_t bsh = __builtin_ctz(a.block / KV8_T);
     const size_t rec = (size_t)a.n_kv * (2 * KV8_T * HD);
     const int8_t *codes = a.codes + (size_t)hk * (2 * KV8_T * HD);
@@ -744,7 +769,7 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
     };
 
     const uint64_t r = r0 + wave * 16 + li, rw = r0 + wave * 16;
-    const uint32_t tok = r < R ? (uint32_t)r / G : 0, head = hk * G + (r < R ? (uint32_t)r % G : 0), rpos = a.base + tok;
+    const uint32_t tok = r < R ? div_by((uint32_t)r, part.group) : 0, head = hk * G + (r < R ? (uint32_t)r - tok * G : 0), rpos = a.base + tok;
     float xq[NC][16];
     q_load<NC>(a.q + tok * a.q_tok + (size_t)head * a.q_stride, r < R, al, lg, xq);
     if (n) load_k(0);
@@ -755,8 +780,8 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
 #pragma unroll
     for (int d = 0; d < NT; d++) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
     // the wave's first and last visible keys: no mask up to the one, no work past the other
-    const uint32_t wfirst = a.base + (uint32_t)rw / G;
-    const uint32_t wtiles = rw < R ? (a.base + (uint32_t)(min(rw + 16, R) - 1) / G) / 64 + 1 : 0;
+    const uint32_t wfirst = a.base + div_by((uint32_t)rw, part.group);
+    const uint32_t wtiles = rw < R ? (a.base + div_by((uint32_t)(min(rw + 16, R) - 1), part.group)) / 64 + 1 : 0;
     const uint32_t ntw = wtiles > k0 ? min(wtiles - k0, n) : 0;
     float sc[4][4];
     f16x8 ph[2], pl[2];
@@ -1023,6 +1048,8 @@ extern "C" uint64_t sgk_kv8_attn_scratch(const sgk_kv8_attn *a) {
     return p.splits > 1 ? (uint64_t)a->ntok * a->n_heads * p.splits * (a->hd + 2) * 4 : 0;
 }
 
+static kv8_div kv8_div_of(uint32_t d) { return (kv8_div){d, d > 1 ? UINT32_MAX / d + 1 : 0}; }
+
 extern "C" hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hipStream_t s, hipEvent_t done) {
     if (!a->ntok || !a->n_heads) return hipSuccess;
     if (!sgk_kv8_shape_ok(a->n_kv, a->hd, a->block) || ((uintptr_t)a->codes & 15) || a->n_heads % a->n_kv ||
@@ -1032,6 +1059,8 @@ extern "C" hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hi
     const int al = !((uintptr_t)a->q & 15) && a->q_stride % 4 == 0 && a->q_tok % 4 == 0;
     const uint64_t rows = (uint64_t)a->ntok * a->n_heads * p.splits;
     kv8_part part = {};
+    part.group = kv8_div_of(a->n_heads / a->n_kv);
+    part.splits = kv8_div_of(p.splits);
     if (p.splits > 1) {                 // outputs first, as they are stored 16 bytes at a time
         part.acc = (float *)scratch;
         part.m = part.acc + rows * a->hd;
