@@ -321,7 +321,7 @@ __device__ __forceinline__ void q_digits(const float (&x)[16], float inv, v4i &d
     for (int w = 0; w < 4; w++) {
         uint32_t t[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) t[e] = (uint32_t)((int)rintf(x[4 * w + e] * inv) + 0x808080);
+        for (int e = 0; e < 4; e++) t[e] = (uint32_t)rintf(fmaf(x[4 * w + e], inv, 8421504.0f));    // 0x808080
         // bytes 0 and 1 of two elements, then byte 2; perm picks 0-3 from its second argument, 4-7 from its first
         const uint32_t a = __builtin_amdgcn_perm(t[1], t[0], 0x05010400u), b = __builtin_amdgcn_perm(t[3], t[2], 0x05010400u);
         const uint32_t c = __builtin_amdgcn_perm(t[1], t[0], 0x0C0C0602u), d = __builtin_amdgcn_perm(t[3], t[2], 0x0C0C0602u);
@@ -330,43 +330,64 @@ __device__ __forceinline__ void q_digits(const float (&x)[16], float inv, v4i &d
         d2[w] = (int)(__builtin_amdgcn_perm(d, c, 0x05040100u) ^ 0x80808080u);
     }
 }
+// The largest magnitude of three, NaN if one is.
+__device__ __forceinline__ float amax3(float a, float b, float c) {
+    float r;
+    asm("v_maximum3_f32 %0, |%1|, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
 // A row's q, spread over the four lanes of its column. Asked for before the
 // first keys and values, which would otherwise have to arrive first.
 template <int NC>
-__device__ __forceinline__ void q_load(const float *q, bool on, bool al, uint32_t lg, float (&x)[NC][16]) {
+__device__ __forceinline__ void q_load(const float *q, bool al, uint32_t lg, float (&x)[NC][16]) {
+    q += 16 * lg;
+    if (al) {
 #pragma unroll
-    for (int c = 0; c < NC; c++)
+        for (int c = 0; c < NC; c++)
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            f32x4 v = {0.f, 0.f, 0.f, 0.f};
-            if (on) v = ld4(q + 64 * c + 16 * lg + 4 * w, al);
+            for (int w = 0; w < 4; w++) {
+                const f32x4 v = *(const f32x4 *)(q + 64 * c + 4 * w);
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[c][4 * w + e] = v[e];
-        }
+                for (int e = 0; e < 4; e++) x[c][4 * w + e] = v[e];
+            }
+    } else {
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[c][e] = q[64 * c + e];
+    }
 }
-#define KV8_QMAX (127.0f * 65536.0f)        // the row's largest element in units of its digits
 // It as digits; returns the factor of the integer scores, sq * |mul|, NaN if an
 // element is not finite.
+#define KV8_QMAX (127.0f * 65536.0f)        // the row's largest element in units of its digits
 template <int NC>
 __device__ __forceinline__ float q_row(float (&x)[NC][16], float mul, v4i (&d)[3][NC]) {
-    uint32_t mx = 0;
-#pragma unroll
-    for (int c = 0; c < NC; c++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) mx = max(mx, __float_as_uint(x[c][e]) & 0x7FFFFFFFu);
-    mx = max(mx, swap16(mx));
-    mx = max(mx, swap32(mx));
-    const bool bad = mx >= 0x7F800000u;
-    float am = bad ? 0.0f : __uint_as_float(mx);
-    const float up = am < 0x1p-60f ? 0x1p64f : 1.0f;    // a row near the end of the range, times 2^64
-    am *= up;
-    const float inv = am > 0.0f ? copysignf(KV8_QMAX / am, mul) : 0.0f;       // a negative scale turns q
+    float mx[NC];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
+        mx[c] = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 16; e++) x[c][e] = bad ? 0.0f : x[c][e] * up;
-        q_digits(x[c], inv, d[0][c], d[1][c], d[2][c]);
+        for (int e = 0; e < 16; e += 2) mx[c] = amax3(x[c][e], x[c][e + 1], mx[c]);
     }
+    float am = mx[0];
+#pragma unroll
+    for (int c = 1; c < NC; c++) am = amax3(am, mx[c], 0.0f);
+    am = amax3(am, swap16f(am), 0.0f);
+    am = amax3(am, swap32f(am), 0.0f);
+    const bool bad = !(am < INFINITY);
+    if (bad) am = 0.0f;
+    float up = 1.0f;
+    if (__builtin_amdgcn_ballot_w64(am < 0x1p-60f)) {   // a row near the end of the range, times 2^64
+        up = am < 0x1p-60f ? 0x1p64f : 1.0f;
+        am *= up;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[c][e] *= up;
+    }
+    const float inv = am > 0.0f ? copysignf(KV8_QMAX / am, mul) : 0.0f;       // a negative scale turns q
+#pragma unroll
+    for (int c = 0; c < NC; c++) q_digits(x[c], inv, d[0][c], d[1][c], d[2][c]);
     return bad ? NAN : am / KV8_QMAX * fabsf(mul) / up;
 }
 // the score sums of the three digits as one float (a2 * 256 + a1 < 2^31)
@@ -541,15 +562,18 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
     };
     uint32_t step = s0 + wave;
     const bool any = step < s1;
-    float xq[NC][16];
-    q_load<NC>(a.q + tok * a.q_tok + (size_t)head * a.q_stride, li < R && any, al, lg, xq);
+    v4i qd[3][NC];
+    float qf = 0.0f;
     if (any) {
+        float xq[NC][16];
+        q_load<NC>(a.q + tok * a.q_tok + (size_t)head * a.q_stride, al, lg, xq);
         load_s(step);
         load_k(step);
+        __builtin_amdgcn_sched_barrier(0);      // all keys, then the values: in the loop's order, whose waits count them
         load_v(step);
+        __builtin_amdgcn_sched_barrier(0);
+        qf = q_row<NC>(xq, a.scale * 1.44269504088896340736f, qd);
     }
-    v4i qd[3][NC];
-    const float qf = q_row<NC>(xq, a.scale * 1.44269504088896340736f, qd);
     f32x4 o[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) o[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -579,7 +603,7 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
         const float rv[2] = {__builtin_amdgcn_rcpf(vs[0]), __builtin_amdgcn_rcpf(vs[1])};
         const float al2 = usual ? softmax_step<2, false>(sc, f, lv, rv, 0, 0, mrun, lsum, ph, pl)
                                 : softmax_step<2, true>(sc, f, vs, rv, step * 32, rpos, mrun, lsum, ph, pl);
-        if (__builtin_amdgcn_ballot_w64(al2 != 1.0f)) {
+        if (step != s0 + wave && __builtin_amdgcn_ballot_w64(al2 != 1.0f)) {       // the first step has nothing to rescale
 #pragma unroll
             for (int n = 0; n < NT; n++) o[n] *= al2;
         }
@@ -771,7 +795,7 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
     const uint64_t r = r0 + wave * 16 + li, rw = r0 + wave * 16;
     const uint32_t tok = r < R ? div_by((uint32_t)r, part.group) : 0, head = hk * G + (r < R ? (uint32_t)r - tok * G : 0), rpos = a.base + tok;
     float xq[NC][16];
-    q_load<NC>(a.q + tok * a.q_tok + (size_t)head * a.q_stride, r < R, al, lg, xq);
+    q_load<NC>(a.q + tok * a.q_tok + (size_t)head * a.q_stride, al, lg, xq);
     if (n) load_k(0);
     v4i qd[3][NC];
     const float qf = q_row<NC>(xq, a.scale * 1.44269504088896340736f, qd);
