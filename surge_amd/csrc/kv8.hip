@@ -25,6 +25,16 @@ __device__ __forceinline__ uint32_t val_at(uint32_t r, uint32_t d) {
     return (d / 64) * 1024 + (r / 4) * 256 + (d % 16) * 16 + (d / 16 % 4) * 4 + r % 4;
 }
 
+// What a launch is divided by, with floor(2^32 / d) + 1 (2^32 / d where that is
+// whole): the compiler's division of any two numbers is some 25 dependent
+// instructions, and a wave has several before its first load.
+struct kv8_div { uint32_t d, inv; };
+__device__ __forceinline__ uint32_t div_by(uint32_t n, kv8_div v) {     // n < 2^31
+    const uint32_t q = v.d == 1 ? n : __umulhi(n, v.inv);
+    return q - (q * v.d > n);
+}
+static kv8_div kv8_div_of(uint32_t d) { return (kv8_div){d, d > 1 ? UINT32_MAX / d + 1 : 0}; }
+
 // ---------------------------------------------------------------------------
 // Store. One workgroup per (block, kv head, half) holds the block's new rows
 // in registers: one read for the maximum and the codes. Keys go four dims of a
@@ -40,14 +50,15 @@ struct kv8_store_args {
     int8_t *codes;
     float *scales;
     uint64_t stride;
-    uint32_t n_kv, hd, block, base, n;
+    uint32_t n_kv, hd, block, base, n, hs, bs;      // hs, bs: log2 of hd and block
+    kv8_div kv;
 };
 
 // Where four of a wave's keys lie: chunk c is 8 rows x 32 dims.
-__device__ __forceinline__ void key_four(uint32_t c, uint32_t hd, uint32_t &r, uint32_t &d) {
+__device__ __forceinline__ void key_four(uint32_t c, uint32_t hs, uint32_t &r, uint32_t &d) {
     const uint32_t lane = threadIdx.x & 63;
-    r = c / (hd / 32) * 8 + lane / 8;
-    d = c % (hd / 32) * 32 + lane % 8 * 4;
+    r = (c >> (hs - 5)) * 8 + lane / 8;
+    d = (c & ((1u << (hs - 5)) - 1)) * 32 + lane % 8 * 4;
 }
 
 // Four x / s to the nearest integers, ties to even, as bytes. q = rint(x * (1/s))
@@ -88,11 +99,11 @@ __device__ __forceinline__ uint32_t pick_bytes(uint32_t mask, uint32_t a, uint32
 template <int U, int NTH>
 __global__ void __launch_bounds__(NTH, 4) k_kv8_store(kv8_store_args a, uint32_t first, int al) {
     __shared__ uint32_t red[NTH / 64];
-    const uint32_t id = first + blockIdx.x, t = threadIdx.x, half = id & 1, h = id / 2 % a.n_kv, hd = a.hd;
-    const uint32_t blk = a.base / a.block + id / 2 / a.n_kv, p0 = blk * a.block;
+    const uint32_t id = first + blockIdx.x, t = threadIdx.x, half = id & 1, hd = a.hd, unit = div_by(id / 2, a.kv), h = id / 2 - unit * a.n_kv;
+    const uint32_t blk = (a.base >> a.bs) + unit, p0 = blk << a.bs;
     const uint32_t lo = max(p0, a.base), hi = (uint32_t)min((uint64_t)p0 + a.block, (uint64_t)a.base + a.n);
     const uint32_t kept = lo - p0, rows = hi - p0;      // rows kept .. rows-1 of the block are new
-    const uint32_t fours = a.block * hd / 4, d4 = hd / 4;
+    const uint32_t fours = hd << a.bs >> 2, ds = a.hs - 2, dm = hd / 4 - 1;
     const float *x = a.x[half] + (size_t)(lo - a.base) * a.stride + (size_t)h * hd;
     float *sp = a.scales + ((size_t)blk * a.n_kv + h) * 2 + half;
     const float was = kept ? *sp : 0.0f;
@@ -103,8 +114,8 @@ __global__ void __launch_bounds__(NTH, 4) k_kv8_store(kv8_store_args a, uint32_t
     for (int i = 0; i < 4 * U; i++) {
         uint32_t r, d;
         const bool in = half ? (t + i / 4 * NTH) * 4 < fours : (t + i * NTH) < fours;
-        if (half) { r = (t + i / 4 * NTH) / d4 * 4 + i % 4; d = (t + i / 4 * NTH) % d4 * 4; }
-        else key_four((t >> 6) + i * (NTH / 64), hd, r, d);
+        if (half) { r = ((t + i / 4 * NTH) >> ds) * 4 + i % 4; d = ((t + i / 4 * NTH) & dm) * 4; }
+        else key_four((t >> 6) + i * (NTH / 64), a.hs, r, d);
         v[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
         if (in && r >= kept && r < rows) v[i] = ld4(x + (size_t)(r - kept) * a.stride + d, al);
     }
@@ -117,7 +128,7 @@ __global__ void __launch_bounds__(NTH, 4) k_kv8_store(kv8_store_args a, uint32_t
     };
     if (half && (kept || rows < a.block)) {
 #pragma unroll
-        for (int u = 0; u < U; u++) load_old(u, (t + u * NTH) / d4 * 4, (t + u * NTH) % d4 * 4);
+        for (int u = 0; u < U; u++) load_old(u, ((t + u * NTH) >> ds) * 4, ((t + u * NTH) & dm) * 4);
     }
 #pragma unroll
     for (int i = 0; i < 4 * U; i++)
@@ -148,7 +159,7 @@ __global__ void __launch_bounds__(NTH, 4) k_kv8_store(kv8_store_args a, uint32_t
 #pragma unroll
         for (int i = 0; i < 4 * U; i++) {
             uint32_t r, d;
-            key_four((t >> 6) + i * (NTH / 64), hd, r, d);
+            key_four((t >> 6) + i * (NTH / 64), a.hs, r, d);
             if (t + i * NTH >= fours || r >= rows || (r < kept && !grew)) continue;
             uint32_t *p = (uint32_t *)(codes + rec_at((p0 + r) / KV8_T, a.n_kv, h, hd) + key_at(r % KV8_T, d));
             *p = r < kept ? requant4(*p, was, s) : quant4(v[i], sz, inv);
@@ -157,7 +168,7 @@ __global__ void __launch_bounds__(NTH, 4) k_kv8_store(kv8_store_args a, uint32_t
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        const uint32_t r = (t + u * NTH) / d4 * 4, d = (t + u * NTH) % d4 * 4;
+        const uint32_t r = ((t + u * NTH) >> ds) * 4, d = ((t + u * NTH) & dm) * 4;
         if ((t + u * NTH) * 4 >= fours || r >= rows || (r + 4 <= kept && !grew)) continue;
         uint32_t w[4];
 #pragma unroll
@@ -191,7 +202,7 @@ extern "C" hipError_t sgk_kv8_store(const float *k, const float *v, uint64_t str
                                     hipEvent_t done) {
     if (!n) return hipSuccess;
     if (!sgk_kv8_shape_ok(n_kv, hd, block) || ((uintptr_t)codes & 15)) return hipErrorInvalidValue;
-    kv8_store_args a = {{k, v}, codes, scales, stride, n_kv, hd, block, base, n};
+    kv8_store_args a = {{k, v}, codes, scales, stride, n_kv, hd, block, base, n, (uint32_t)__builtin_ctz(hd), (uint32_t)__builtin_ctz(block), kv8_div_of(n_kv)};
     const int al = !((uintptr_t)k & 15) && !((uintptr_t)v & 15) && stride % 4 == 0;
     const uint64_t wgs = (((uint64_t)base + n + block - 1) / block - base / block) * n_kv * 2;
     if (wgs > UINT32_MAX) return hipErrorInvalidValue;
@@ -214,13 +225,13 @@ extern "C" hipError_t sgk_kv8_store(const float *k, const float *v, uint64_t str
 // by memory: the 84 MB above 15.1 us, 5.6 TB/s; one block 3.0.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(TPB) k_kv8_load(const int8_t *codes, const float *scales, float *k, float *v,
-                                                  uint64_t stride, uint32_t n_kv, uint32_t hd, uint32_t block,
+                                                  uint64_t stride, kv8_div kv, uint32_t hd, uint32_t block,
                                                   uint32_t base, uint32_t n, uint32_t first, uint32_t halves, int al) {
     const uint32_t hs = __builtin_ctz(hd), id = first + ((blockIdx.x * TPB + threadIdx.x) >> hs);
     if (id >= halves) return;
     const uint32_t i = threadIdx.x & (hd - 1), half = id & 1, rec = id / 2;
-    const uint32_t tile = base / KV8_T + rec / n_kv, h = rec % n_kv;
-    const float s = scales[((size_t)(tile * KV8_T / block) * n_kv + h) * 2 + half];
+    const uint32_t n_kv = kv.d, unit = div_by(rec, kv), tile = base / KV8_T + unit, h = rec - unit * n_kv;
+    const float s = scales[((size_t)(tile >> __builtin_ctz(block / KV8_T)) * n_kv + h) * 2 + half];
     const int8_t *c = codes + rec_at(tile, n_kv, h, hd) + (size_t)half * KV8_T * hd;
     float *out = (half ? v : k) + (size_t)h * hd;
     const uint64_t p0 = (uint64_t)tile * KV8_T, end = (uint64_t)base + n;
@@ -228,11 +239,11 @@ __global__ void __launch_bounds__(TPB) k_kv8_load(const int8_t *codes, const flo
     if (!half) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            key_four((i >> 6) + j * (hd / 64), hd, r[j], d[j]);
+            key_four((i >> 6) + j * (hd / 64), hs, r[j], d[j]);
             w[j] = *(const uint32_t *)(c + key_at(r[j], d[j]));
         }
     } else {
-        const uint32_t r0 = i / (hd / 4) * 4, d0 = i % (hd / 4) * 4;
+        const uint32_t r0 = (i >> (hs - 2)) * 4, d0 = (i & (hd / 4 - 1)) * 4;
         uint32_t b[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) b[e] = *(const uint32_t *)(c + val_at(r0, d0 + e));
@@ -266,7 +277,7 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
     for (uint64_t first = 0; first < halves; first += most) {
         const uint64_t m = halves - first < most ? halves - first : most;
         launch(k_kv8_load, dim3((uint32_t)((m * hd + TPB - 1) / TPB)), TPB, s, first + most < halves ? NULL : done, codes, scales, k, v,
-               stride, n_kv, hd, block, base, n, (uint32_t)first, (uint32_t)(first + m), al);
+               stride, kv8_div_of(n_kv), hd, block, base, n, (uint32_t)first, (uint32_t)(first + m), al);
     }
     return hipGetLastError();
 }
@@ -293,18 +304,10 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
 // 6.2 TB/s, where a plain read reaches 6.6; 32771 of 8 x 128 (67 MB) 15.3, with
 // the waves' start and end in it; 700 of 2 x 256 7.2, one step's chain.
 // ---------------------------------------------------------------------------
-// What a launch is divided by, with floor(2^32 / d) + 1 (2^32 / d where that is
-// whole): the compiler's division of any two numbers is some 25 dependent
-// instructions, and a wave has several before its first load.
-struct kv8_div { uint32_t d, inv; };
 struct kv8_part {
     float *m, *s, *acc;         // [token][head][split] maxima and sums, [..][hd] outputs; NULL: one split
     kv8_div group, splits;      // query heads of a kv head
 };
-__device__ __forceinline__ uint32_t div_by(uint32_t n, kv8_div v) {     // n < 2^31
-    const uint32_t q = v.d == 1 ? n : __umulhi(n, v.inv);
-    return q - (q * v.d > n);
-}
 // Part sp of n units: the first n % splits parts have one more.
 __device__ __forceinline__ void part_of(uint32_t n, uint32_t sp, kv8_div splits, uint32_t &first, uint32_t &end) {
     const uint32_t q = div_by(n, splits), more = n - q * splits.d;
@@ -1071,8 +1074,6 @@ extern "C" uint64_t sgk_kv8_attn_scratch(const sgk_kv8_attn *a) {
     const kv8_plan p = kv8_plan_of(a);
     return p.splits > 1 ? (uint64_t)a->ntok * a->n_heads * p.splits * (a->hd + 2) * 4 : 0;
 }
-
-static kv8_div kv8_div_of(uint32_t d) { return (kv8_div){d, d > 1 ? UINT32_MAX / d + 1 : 0}; }
 
 extern "C" hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hipStream_t s, hipEvent_t done) {
     if (!a->ntok || !a->n_heads) return hipSuccess;
