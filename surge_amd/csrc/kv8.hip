@@ -95,9 +95,10 @@ __device__ __forceinline__ uint32_t pick_bytes(uint32_t mask, uint32_t a, uint32
 // Workgroups in the order of the rows in memory: a block's heads and halves side by side.
 // NTH threads, 4 U fours each: a large block takes more threads, not more
 // registers (8190 rows of 4 heads of 256 in blocks of 64: 25 us with 4 units in
-// each of 256 threads, 140 registers).
+// each of 256 threads, 140 registers). With one unit six waves fit a SIMD (8 x
+// 128, blocks of 16 27.9 -> 26.4 us a call); with two they would spill.
 template <int U, int NTH>
-__global__ void __launch_bounds__(NTH, 4) k_kv8_store(kv8_store_args a, uint32_t first, int al) {
+__global__ void __launch_bounds__(NTH, U == 1 ? 6 : 4) k_kv8_store(kv8_store_args a, uint32_t first, int al) {
     __shared__ uint32_t red[NTH / 64];
     const uint32_t id = first + blockIdx.x, t = threadIdx.x, half = id & 1, hd = a.hd, unit = div_by(id / 2, a.kv), h = id / 2 - unit * a.n_kv;
     const uint32_t blk = (a.base >> a.bs) + unit, p0 = blk << a.bs;
