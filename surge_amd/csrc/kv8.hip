@@ -294,9 +294,7 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
 //    the keys are never converted;
 //  - S^T = K Q^T leaves lane (li, lg) row li's scores of keys 4 lg .. 4 lg + 3
 //    of both tiles, the order of the value records' dwords, so V^T P^T runs on
-//    v_mfma_f32_16x16x32_f16 with p in two halves and the codes as f16 (exact):
-//    (code + 128) 2^-24, a third fewer instructions than code itself; one more
-//    product with 128 2^-24 in every place sums what is to be taken off;
+//    v_mfma_f32_16x16x32_f16 with the codes as f16 (exact) and p in two halves;
 //  - the values' scale goes into p: w = p s_V. The running maximum is taken
 //    over score + log2 s_V, so that w <= 2^12 whatever the scales are, while
 //    the sum of p, at most 2^92 a key (log2 s_V >= -80), stays in f32's range.
@@ -417,15 +415,6 @@ __device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
     return r;
 }
 
-// the same without the difference: (code + 128) 2^-24, f16's subnormals, which
-// the matrix instruction takes as they are
-__device__ __forceinline__ f16x8 codes_sub(uint32_t a, uint32_t b) {
-    const uint32_t ua = a ^ 0x80808080u, ub = b ^ 0x80808080u;
-    const v4u r = {__builtin_amdgcn_perm(0, ua, 0x0C010C00u), __builtin_amdgcn_perm(0, ua, 0x0C030C02u),
-                   __builtin_amdgcn_perm(0, ub, 0x0C010C00u), __builtin_amdgcn_perm(0, ub, 0x0C030C02u)};
-    return __builtin_bit_cast(f16x8, r);
-}
-
 // Whether a group's least scales (the same in every lane) are those of the
 // usual case; NaN is not, where the minimum shows it.
 __device__ __forceinline__ bool scales_usual(float ks, float vs) {
@@ -532,7 +521,7 @@ __device__ __forceinline__ float softmax_step(const float (&x)[UN][4], const flo
 template <int HD, int NW>
 __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_part part, int al) {
     constexpr int NC = HD / 64, NT = HD / 16, OLD = HD + 4;
-    __shared__ float wm[NW][16], wl[NW][16], wb[NW][16];
+    __shared__ float wm[NW][16], wl[NW][16];
     __shared__ __align__(16) float ob[NW][16 * OLD];
     const uint32_t t = threadIdx.x, lane = t & 63, li = lane & 15, lg = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -592,8 +581,6 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
     f32x4 o[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) o[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    f32x4 ob128 = {0.f, 0.f, 0.f, 0.f};        // of codes that are all 0: the same in its four places
-    const v4u c128 = {0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u};
     float mrun = -INFINITY, lsum = 0.0f;
     // The last step stands apart: with its missing loads in the loop, waiting for
     // a step's keys is waiting for its values as well.
@@ -623,15 +610,12 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
         if (step != s0 + wave && __builtin_amdgcn_ballot_w64(al2 != 1.0f)) {       // the first step has nothing to rescale
 #pragma unroll
             for (int n = 0; n < NT; n++) o[n] *= al2;
-            ob128 *= al2;
         }
-        ob128 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, c128), ph[0], ob128, 0, 0, 0);
-        ob128 = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, c128), pl[0], ob128, 0, 0, 0);
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const f16x8 v = codes_sub(vr[0][c][j], vr[1][c][j]);
+                const f16x8 v = codes_f16(vr[0][c][j], vr[1][c][j]);
                 o[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[0], o[4 * c + j], 0, 0, 0);
                 o[4 * c + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[0], o[4 * c + j], 0, 0, 0);
             }
@@ -644,7 +628,7 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
     lsum += swap16f(lsum);
     lsum += swap32f(lsum);
     if (li < R) {
-        if (lg == 0) { wm[wave][li] = mrun; wl[wave][li] = lsum; wb[wave][li] = ob128[0]; }
+        if (lg == 0) { wm[wave][li] = mrun; wl[wave][li] = lsum; }
         float *dst = &ob[wave][li * OLD + 4 * lg];
 #pragma unroll
         for (int n = 0; n < NT; n++) *(f32x4 *)(dst + 16 * n) = o[n];
@@ -652,7 +636,7 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
     __syncthreads();
     for (uint32_t i = t; i < R * (HD / 4); i += NW * 64) {
         const uint32_t r = i / (HD / 4), d = i % (HD / 4) * 4;
-        float wmx[NW], m = -INFINITY, l = 0.0f, b128 = 0.0f;
+        float wmx[NW], m = -INFINITY, l = 0.0f;
         f32x4 ov[NW], v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int w = 0; w < NW; w++) { wmx[w] = wm[w][r]; ov[w] = *(const f32x4 *)&ob[w][r * OLD + d]; }
@@ -662,10 +646,8 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
         for (int w = 0; w < NW; w++) {
             const float f = wmx[w] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(wmx[w] - m);
             l = fmaf(wl[w][r], f, l);
-            b128 = fmaf(wb[w][r], f, b128);
             v += ov[w] * f;
         }
-        v = (v - b128) * 0x1p24f;
         const uint32_t z = div_by(r0 + r, part.group);
         const size_t row = (size_t)z * a.n_heads + hk * G + (r0 + r - z * G);
         if (S == 1) {
