@@ -424,3 +424,24 @@ def test_scale_of_either_sign(gpu, n, seq, scale):
     q = rng.standard_normal((n, 16, 256)).astype(np.float32)
     want, bound = K.attention(q, c, seq - n, float(np.float32(scale)))
     close(attend(gpu, c, q, seq - n, scale), want, bound)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,seq,n", [(24, 4, 256, 20011, 1), (8, 2, 128, 9001, 3), (12, 12, 64, 20011, 1), (8, 1, 256, 20001, 128)])
+def test_values_that_cancel(gpu, nh, nkv, hd, seq, n):
+    """Nearly flat weights over values without a mean: an output is the small remainder of a long sum, and has to
+    be right by its own size. The weights' errors e (twice a score's, which the oracle's bound gives, and 10 u for exp
+    and p s_V in two halves) and the additions' (m / 16 of them, each u of a partial sum that is no larger than the
+    remainder) are independent of the values, so they add as squares: e + u sqrt(m / 16), doubled."""
+    rng = np.random.default_rng(seq + n)
+    c = filled(rng, nkv, hd, 64, seq)
+    q = (rng.standard_normal((n, nh, hd)) * 0.01).astype(np.float32)
+    scale = 1 / math.sqrt(hd)
+    want, _ = K.attention(q, c, seq - n, scale)
+    got = attend(gpu, c, q, seq - n, scale, "decode" if n == 1 else "prefill").astype(np.float64)
+    u = 2.0 ** -24
+    k = c.values(0, seq)
+    most = max(np.abs(k[:, h] @ q[:, g].astype(np.float64).T).max() for g in range(nh) for h in [g * nkv // nh]) * scale
+    ds = scale * 2 * u * np.abs(q).max() * np.abs(k).sum(2).max() + 16 * u * most
+    tol = 2 * (2 * ds + 10 * u + u * math.sqrt(seq / 16))
+    err = np.linalg.norm(got - want, axis=2) / np.linalg.norm(want, axis=2)
+    assert (err <= tol).all(), f"worst error {err.max():.3g}, tolerance {tol:.3g}"
