@@ -1015,27 +1015,28 @@ __global__ void __launch_bounds__(TPB) k_kv8_comb(kv8_part p, float *out, uint32
 }
 
 // How a call runs. The wave form, small calls (whole calls below in us):
-//  - workgroups of eight waves, one a CU (two at head_dim 64), where their waves
-//    get more than a step of 32 keys each and there are not more workgroups than
-//    that without a split (eight / four waves: 24 heads of 256 on 4, 32771 keys
-//    29.5 / 31.2; 32 of 128 on 8, 262000 keys 97.1 / 103.4, 5000 keys 20.8 both);
-//  - one of eight waves alone up to KV8_ONE steps, as a second launch to join
-//    costs more than a wave's second step (one / splits of four waves: 384 keys,
-//    24 of 256 on 4 20.2 / 21.2, 32 of 128 on 8 16.7 / 19.1, 12 of 64 15.6 / 17.2;
-//    512 keys 22.0 / 21.4, 17.9 / 19.0, 16.3 / 17.1; 768 keys 24.3 / 21.8, 19.4 /
-//    19.0, 17.3 / 17.2);
-//  - else workgroups of four waves, a step to each wave.
+//  - one workgroup of eight waves for 5 to 24 steps of 32 keys (20 at head_dim
+//    256), as a second launch to join costs more than a wave's second and third
+//    step (one / splits of four waves: 384 keys, 24 heads of 256 on 4 17.2 / 19.1,
+//    32 of 128 on 8 14.9 / 17.0, 12 of 64 13.6 / 15.4; 640 keys 19.2 / 19.3, 15.9 /
+//    17.0, 14.6 / 15.6; 768 keys 20.8 / 19.3, 16.7 / 17.1, 15.0 / 15.8);
+//  - else parts of the keys, one workgroup a CU (two at head_dim 64) of four
+//    waves, which spend less on their start and join (four / eight: 24 of 256 on
+//    4, 32771 keys 27.4 / 27.8, 5 tokens at 40000 34.6 / 36.3; 32 of 128 on 8, 32771
+//    keys 25.3 / 26.0; two workgroups a CU of four 30.3, 45.2, 28.3);
+//  - of eight below head_dim 256 where a CU has more than 64 steps, which its
+//    vector units and not the cache's bytes bound then (32 of 128 on 8, 40 tokens
+//    at 8000 33.3 / 31.4, 20 at 32000 49.0 / 44.3, 262000 keys 96.0 / 95.3).
 // Else row blocks in tiles, one workgroup per CU at a time, their keys split
 // where that shortens the launch: rounds x (a part's tiles + KV8_TAIL for its
 // start and end) tiles of KV8_TILE_US, against the partials' way to memory and
 // back. KV8_SMALL, in waves' steps of 32 keys x head_dim, is where the two meet
-// (wave / tile): 24 heads of 256 on 4, 8040 keys, 240 rows (3.9M) 42.9 / 48.5,
-// 1300 keys, 1800 rows (4.7M) 42.0 / 51.4, 8077 keys, 462 rows (7.5M) 58.3 /
-// 58.6, 32020 keys, 120 rows (8.2M) 58.7 / 56.4; 32 of 128 on 8, 8040 keys, 160
-// rows (2.6M) 32.8 / 40.5, 32020 keys, 80 rows (5.1M) 47.2 / 50.8, 8077 keys, 308
-// rows (5.2M) 52.2 / 49.5; 12 of 64, 32077 keys, 77 rows (3.9M) 46.4 / 55.6.
+// (wave / tile): 24 heads of 256 on 4, 8040 keys, 240 rows (3.9M) 39.4 / 45.2,
+// 1300 keys, 1800 rows (4.7M) 38.1 / 48.2, 8077 keys, 462 rows (7.5M) 53.8 /
+// 55.2, 32020 keys, 120 rows (8.2M) 55.7 / 54.0; 32 of 128 on 8, 8040 keys, 160
+// rows (2.6M) 30.9 / 38.6, 32020 keys, 80 rows (5.1M) 43.7 / 49.6, 8077 keys, 308
+// rows (5.2M) 50.5 / 48.2; 12 of 64, 32077 keys, 77 rows (3.9M) 43.3 / 54.4.
 #define KV8_SMALL (5ull << 20)
-#define KV8_ONE 16
 #define KV8_TILE_US 2.5         /* at head_dim 256 */
 #define KV8_TAIL 3.0
 #define KV8_PART_BYTES (256ull << 20)
@@ -1049,8 +1050,8 @@ static kv8_plan kv8_plan_of(const sgk_kv8_attn *a) {
         const uint64_t steps = (keys + 31) / 32;
         uint64_t most = (a->hd == 64 ? 2 : 1) * cus / wgs;
         if (most > KV8_COMB) most = KV8_COMB;
-        const bool one = steps > 4 && steps <= KV8_ONE;
-        if (most && (one || steps > 8 * most)) {
+        const bool one = steps > 4 && steps <= (a->hd == 256 ? 20 : 24);
+        if (most && (one || (a->hd < 256 && wgs * steps > 64 * cus))) {
             p.waves = 8;
             p.splits = one ? 1 : (uint32_t)most;
         } else if (most > 1) {
