@@ -42,8 +42,8 @@ static kv8_div kv8_div_of(uint32_t d) { return (kv8_div){d, d > 1 ? UINT32_MAX /
 // bytes of codes at a time); values 4 positions x 4 dims, transposed in
 // registers into a dword per dim. 4 U fours per thread. Rows before base keep
 // their codes unless the scale grows. Bound by memory: 8190 rows of 4 x 256 (84
-// MB) 25.6 us in a trace with fresh inputs, 19 with the rows in the last cache;
-// a copy of as many bytes takes 17-18. One row 4.6: load, maximum, codes in turn.
+// MB) 24.5 us in a trace with fresh inputs, 18 with the rows in the last cache;
+// a copy of as many bytes takes 17-18. One row 4.2: load, maximum, codes in turn.
 // ---------------------------------------------------------------------------
 struct kv8_store_args {
     const float *x[2];
@@ -301,9 +301,10 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
 //    2^12 keeps w's lower half above f16's subnormals down to 2^-26 of the
 //    largest.
 // No barrier or LDS in the key loop; the waves' maxima, sums and outputs join
-// at the end. Bound by the cache's bytes: 262000 keys of 4 x 256 (537 MB) 86 us,
-// 6.2 TB/s, where a plain read reaches 6.6; 32771 of 8 x 128 (67 MB) 15.3, with
-// the waves' start and end in it; 700 of 2 x 256 7.2, one step's chain.
+// at the end. Bound by the cache's bytes: 262000 keys of 4 x 256 (537 MB) 85 us,
+// 6.3 TB/s, where a plain read reaches 6.6; 32771 of 8 x 128 (67 MB) 14.0, with
+// the waves' start and end in it; 700 of 2 x 256 5.9, one step's chain: 2 us to
+// the loads' arrival, then 0.4 in the softmax, 0.7 in either product, 0.9 to join.
 // ---------------------------------------------------------------------------
 struct kv8_part {
     float *m, *s, *acc;         // [token][head][split] maxima and sums, [..][hd] outputs; NULL: one split
@@ -677,10 +678,10 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
 // cycles; a tile takes 4800, of which 3584 are the products'.
 // Both tiles are double-buffered; a wave stores its part of the next one and
 // requests that of the one after before its softmax.
-// 24 heads of 256 on 4, 2048 rows at 14336: 1050-1100 us, 720 TFLOP/s of the
+// 24 heads of 256 on 4, 2048 tokens at 14336: 1010-1060 us, 750 TFLOP/s of the
 // formula's, and as the matrix unit counts them (weights in two halves, three
-// digits at twice the rate) 1270, where a plain f16 product of 16384^3 reaches
-// 1346: the clock falls to 1.7 GHz under either.
+// digits at twice the rate) 1310, where a plain f16 product of 16384^3 reaches
+// 1346: the clock falls to 1.7 GHz under the load.
 // Grid: (row block, kv head, key split), the longest rows first.
 // ---------------------------------------------------------------------------
 #define KV8_NW 8

@@ -12,7 +12,7 @@
 // 32 bits), then a slice (token, head) per 2^wl lanes. The first slice's loads
 // go out before the angles, whose chain is as long as a trip to memory.
 // Bound by memory for many tokens (4093 x 24 heads of 256, 201 MB: 43 us, a copy
-// of them 39), by that chain for one (3.3 us).
+// of them 39), by that chain for one (3.0 us).
 // ---------------------------------------------------------------------------
 // The frequencies are exp2 of a product here (0.35 us less for one token than a
 // table among the arguments, which lie in the host's memory).
@@ -150,21 +150,24 @@ __global__ void __launch_bounds__(TPB) k_token_counts(const int32_t *ids, uint32
         }
 }
 
-// Up to TR_MOST ids a row: a workgroup owns TR_IDS ids of the vocabulary, reads
-// the row's whole history and counts its own in LDS, alike neighbours of a
-// thread at once, so nothing is cleared first and no two additions meet in
-// memory. Whole call, us, 151936 ids, cleared, this form / the table form, for
-// Zipf's law with exponent 1.2 and for one id only: 900 ids of 1 row 11.4 / 16.4,
-// 12.0 / 17.2; 32000 of 1 row 15.8 / 21.3, 14.8 / 21.1; 131072 of 16 rows 42 /
-// 103, 30 / 33; 262144 of 1 row 53 / 55, 48 / 21. Past TR_MOST the walk over the
-// history decides, and the table form spreads that.
+// Up to TR_MOST ids a row: a workgroup owns TR_IDS ids of the vocabulary (TR_FEW
+// where those still find a CU each: 900 ids of 1 row 10.8 us a call against 11.3,
+// of 16 rows 15.2 against 13.0), reads the row's whole history and counts its own
+// in LDS, alike neighbours of a thread at once, so nothing is cleared first and no
+// two additions meet in memory. Whole call, us, 151936 ids, cleared, this form /
+// the table form, for Zipf's law with exponent 1.2 and for one id only: 900 ids of
+// 1 row 10.9 / 16.6, 11.3 / 16.7; 32000 of 1 row 15.6 / 21.2, 14.1 / 20.8; 131072 of
+// 16 rows 41 / 103, 29 / 33; 262144 of 1 row 52 / 54, 47 / 21. Past TR_MOST the walk
+// over the history decides, and the table form spreads that.
 #define TR_IDS 8192u
+#define TR_FEW 2048u
 #define TR_THREADS 1024
 #define TR_U 8u
 #define TR_MOST 131072u
-__global__ void __launch_bounds__(TR_THREADS) k_token_recount(const int32_t *ids, uint32_t *counts, uint32_t n, uint32_t vocab, int clear) {
+__global__ void __launch_bounds__(TR_THREADS) k_token_recount(const int32_t *ids, uint32_t *counts, uint32_t n, uint32_t vocab, uint32_t range,
+                                                              int clear) {
     __shared__ uint32_t num[TR_IDS];
-    const uint32_t t = threadIdx.x, v0 = blockIdx.x * TR_IDS, nv = min(TR_IDS, vocab - v0);
+    const uint32_t t = threadIdx.x, v0 = blockIdx.x * range, nv = min(range, vocab - v0);
     const uint32_t r = blockIdx.y;
     for (uint32_t i = t; i < nv; i += TR_THREADS) num[i] = 0;
     __syncthreads();
@@ -197,7 +200,8 @@ extern "C" hipError_t sgk_token_counts(const int32_t *ids, uint32_t *counts, uin
                                        int clear, hipStream_t s, hipEvent_t done) {
     if (!vocab || !rows || (!n && !clear)) return hipErrorInvalidValue;     // nothing to launch, nothing to wait for
     if (n && n <= TR_MOST) {
-        launch(k_token_recount, dim3((vocab + TR_IDS - 1) / TR_IDS, rows), TR_THREADS, s, done, ids, counts, n, vocab, clear);
+        const uint32_t few = (vocab + TR_FEW - 1) / TR_FEW, range = (uint64_t)few * rows <= sgk_device_cus() ? TR_FEW : TR_IDS;
+        launch(k_token_recount, dim3((vocab + range - 1) / range, rows), TR_THREADS, s, done, ids, counts, n, vocab, range, clear);
         return hipGetLastError();
     }
     if (clear) {
