@@ -227,6 +227,18 @@ def test_few_rows_deep(gpu, nh, nkv, hd, block, base, n):
     assert np.array_equal(got, attend(gpu, c, q, base, 1 / math.sqrt(hd), "decode" if n == 1 else "prefill"))
 
 
+@pytest.mark.parametrize("nh,nkv,hd,block,base,n", [(32, 8, 128, 64, 8000, 40), (12, 12, 64, 32, 12001, 60), (16, 16, 128, 16, 33003, 1)])
+def test_few_rows_much_work(gpu, nh, nkv, hd, block, base, n):
+    """More than 64 steps of 32 keys to a CU: eight waves a workgroup, several steps each, parts joined."""
+    rng = np.random.default_rng(base)
+    c = filled(rng, nkv, hd, block, base + n)
+    q = rng.standard_normal((n, nh, hd)).astype(np.float32)
+    want, bound = K.attention(q, c, base, 1 / math.sqrt(hd))
+    got = attend(gpu, c, q, base, 1 / math.sqrt(hd))
+    close(got, want, bound)
+    assert np.array_equal(got, attend(gpu, c, q, base, 1 / math.sqrt(hd)))
+
+
 @pytest.mark.parametrize("nh,nkv,hd,block", [(8, 2, 256, 32), (6, 1, 64, 16), (16, 1, 128, 64), (4, 4, 128, 128), (10, 2, 64, 32)])
 @pytest.mark.parametrize("base,n", [(0, 1), (0, 2), (0, 17), (3, 5), (31, 33), (64, 64), (100, 77), (257, 130), (1000, 3)])
 def test_prefill(gpu, nh, nkv, hd, block, base, n):
@@ -328,6 +340,32 @@ def test_two_handles_in_turn(gpu):
             a, b = (attend(g, c, q, seq - 1, 0.09, "decode") for g in (gpu, other))
             close(a, want, bound)
             assert np.array_equal(a, b)
+
+
+def test_two_handles_at_once(gpu):
+    """Two sg_gpu, a thread each, calls of several kinds side by side: every result is the one of the call alone."""
+    import threading
+    rng = np.random.default_rng(88)
+    work = []
+    for seq in (700, 5000, 33, 9000):
+        c = filled(rng, 2, 128, 32, seq)
+        q = rng.standard_normal((1, 8, 128)).astype(np.float32)
+        work.append((c, q, seq, attend(gpu, c, q, seq - 1, 0.09, "decode")))
+    wrong = []
+
+    def run(g, order):
+        for k in range(12):
+            c, q, seq, want = work[order[k % 4]]
+            if not np.array_equal(attend(g, c, q, seq - 1, 0.09, "decode"), want):
+                wrong.append(seq)
+
+    with S.Gpu() as other:
+        threads = [threading.Thread(target=run, args=a) for a in ((gpu, (0, 1, 2, 3)), (other, (3, 2, 1, 0)))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    assert not wrong
 
 
 def test_cache_past_32_bits(gpu):
