@@ -15,7 +15,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import struct
-from typing import Optional, Sequence
+from typing import Iterable, Optional, Sequence
 
 import numpy as np
 
@@ -227,7 +227,8 @@ _Params = C.c_uint32 * 8
 _pack_params = struct.Struct("8I").pack
 
 
-def params(vals: Sequence[int]) -> C.Array:
+def params(vals: Iterable[int]) -> C.Array:
+    vals = tuple(vals)              # an iterator has no second pass
     try:                            # 0.4 us; an element at a time 1.0
         return _Params.from_buffer_copy(_pack_params(*vals, *(0,) * (8 - len(vals))))
     except (struct.error, TypeError):

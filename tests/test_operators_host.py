@@ -218,3 +218,19 @@ def test_oracle_store_rows_one_by_one_or_together():
         assert np.array_equal(a.scales, b.scales)
         assert (np.abs(a.values(half, 40) - x[half]) <= 0.5001 * step).all()
         assert (np.abs(b.values(half, 40) - x[half]) <= 0.5001 * step * 8).all()
+
+
+@pytest.mark.parametrize("make", [list, tuple, iter, lambda v: (x for x in v), lambda v: map(int, v), lambda v: dict.fromkeys(v).keys(),
+                                  lambda v: np.array(v, np.int64)])
+def test_params_takes_what_can_be_iterated(make):
+    """Whatever holds the values, and values that are not unsigned 32-bit integers: low 32 bits of each, zeros behind."""
+    assert list(S.params(make([1, 2, 3]))) == [1, 2, 3, 0, 0, 0, 0, 0]
+    assert list(S.params(make([5, -1, 1 << 33 | 7]))) == [5, 0xFFFFFFFF, 7, 0, 0, 0, 0, 0]
+    assert list(S.params(make([]))) == [0] * 8
+    assert list(S.params(make(range(8)))) == list(range(8))
+    with pytest.raises(IndexError):
+        S.params(make(range(9)))
+
+
+def test_params_of_floats():
+    assert list(S.params(x for x in (1.0, np.float32(2.5), np.int32(-2)))) == [1, 2, 0xFFFFFFFE, 0, 0, 0, 0, 0]
