@@ -390,7 +390,9 @@ sg_err sg_gpu_run_attn_prefill_kv8(sg_gpu *g, void *q, void *codes, void *scales
  * axis 0's pairs, then axis 1's, then axis 2's. order 1, interleaved: axis 1
  * has the pairs i % 3 == 1 below 3 s1, axis 2 those of i % 3 == 2 below 3 s2,
  * axis 0 the others. Dims from rope_dim on are copied; gaps between slices are
- * not written. out may be x (the same address) but not overlap it otherwise.
+ * not written. out may be x (the same address) but not overlap it otherwise;
+ * where that is two handles of one memory, x's data count before the call, and
+ * both mirrors hold the result after it.
  * p: [0]=head_dim (<= 256) [1]=rope_dim [2]=heads (<= 65535) [3]=stride [4]=n [5]=sections
  * [6]=theta bits [7]=row stride. */
 sg_err sg_gpu_run_rope_axes(sg_gpu *g, void *x, void *pos, void *out, const uint32_t params[8]);
@@ -406,7 +408,7 @@ sg_err sg_gpu_run_token_counts(sg_gpu *g, void *ids, void *counts, const uint32_
  * repetition : x * repetition, then - c * frequency - presence; + bias[id]; -inf
  * where bit id % 32 of mask[row][id / 32] is 0. counts u32 [rows][vocab], bias
  * f32 [vocab] and mask u32 [rows][ceil(vocab / 32)] may each be NULL. out
- * [rows][vocab] may be logits. token u32 [rows]: the lowest id of the largest
+ * [rows][vocab] may be logits (as with the rotary axes' x and out). token u32 [rows]: the lowest id of the largest
  * value that is above -inf, 0xFFFFFFFF if there is none (nothing allowed);
  * NaN is never chosen. repetition > 0 and finite (1 = none), frequency and
  * presence finite (0 = none). vocab < 2^31, rows <= 65535.

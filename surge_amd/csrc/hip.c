@@ -912,7 +912,18 @@ static sg_err back_to(const sg_gpu *g, int was, sg_err e) {
 }
 /* An output of which a call writes the first `bytes`: what lies behind is sent
  * first, so that the download leaves it as it was. */
-static sg_err push_out(void *buf, uint64_t bytes) { return ((const gbuf *)buf)->nbytes > bytes ? sg_gpu_buf_upload(buf) : SG_OK; }
+static sg_err push_out(void *buf, uint64_t bytes) {
+    const gbuf *b = buf;
+    if (b->kind == BUF_ALLOC && b->nbytes > bytes)
+        HIPCHK(hipMemcpy((char *)b->dev + bytes, (const char *)b->host + bytes, b->nbytes - bytes, hipMemcpyHostToDevice), "upload");
+    return SG_OK;
+}
+/* In place through another handle of the same memory (one of the two a
+ * sg_gpu_wrap_device of the other's): the input is what counts before the call,
+ * so the output's mirror is sent only where the input ends, and the input's
+ * mirror has to follow afterwards. The input's handle then, else NULL. */
+static void *alias_of(const void *out, void *in) { return out != in && DEV(out) == DEV(in) ? in : NULL; }
+static uint64_t size_of(const void *buf) { return ((const gbuf *)buf)->nbytes; }
 static bool aligned(const void *buf, uintptr_t to) { return !((uintptr_t)((const gbuf *)buf)->dev & (to - 1)); }
 
 uint64_t sg_kv8_code_bytes(uint32_t n_kv, uint32_t hd, uint64_t cap) {
@@ -1052,11 +1063,11 @@ sg_err sg_gpu_run_rope_axes(sg_gpu *g, void *x, void *pos, void *out, const uint
     if (overlap(out, pos) || (overlap(out, x) && DEV(out) != DEV(x))) return (sg_err){"gpu: rope_axes: out overlaps an input"};
     int was;
     if (sg_failed(e = on_device(g, &was))) return e;
-    void *ins[3] = {x, pos, out}, *outs[1] = {out};     /* out too: its gaps stay as they are */
-    if (!sg_failed(e = push(ins, out == x ? 2 : 3))) {
+    void *ins[3] = {x, pos, out}, *outs[2] = {out, alias_of(out, x)};       /* out too: its gaps stay as they are */
+    if (!sg_failed(e = push(ins, DEV(out) == DEV(x) ? 2 : 3)) && (!outs[1] || !sg_failed(e = push_out(out, size_of(x))))) {
         const sgk_rope_axes_args a = {DEV(x), DEV(pos), DEV(out), row, -2.0 * log2((double)theta) / rd, hd, rd, nh, hs, n,
                                       {sec[0], sec[1], sec[2]}, order};
-        e = finish_done(g, sgk_rope_axes(&a, g->stream, g->done), outs, 1);
+        e = finish_done(g, sgk_rope_axes(&a, g->stream, g->done), outs, 2);
     }
     return back_to(g, was, e);
 }
@@ -1094,7 +1105,7 @@ sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void
         sg_failed(e = need(token, (uint64_t)rows * 4, "token")) || (counts && sg_failed(e = need(counts, lb, "counts"))) ||
         (bias && sg_failed(e = need(bias, (uint64_t)vocab * 4, "bias"))) ||
         (mask && sg_failed(e = need(mask, (uint64_t)(vocab + 31) / 32 * rows * 4, "mask")))) return e;
-    void *bufs[6] = {logits, counts, bias, mask, out, token}, *outs[2] = {out, token};
+    void *bufs[6] = {logits, counts, bias, mask, out, token}, *outs[3] = {out, token, alias_of(out, logits)};
     for (int i = 0; i < 6; i++) {
         if (bufs[i] && !aligned(bufs[i], 4)) return (sg_err){"gpu: logits: buffers must be 4-byte aligned"};
         if ((i < 5 && overlap(token, bufs[i])) || (i < 4 && overlap(out, bufs[i]) && !(i == 0 && DEV(out) == DEV(logits))))
@@ -1104,9 +1115,9 @@ sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void
     if (sg_failed(e = on_device(g, &was))) return e;
     void *part;
     if (!sg_failed(e = scratch(g, sgk_logits_part_bytes(vocab, rows), &part)) && !sg_failed(e = push(bufs, 4)) &&
-        !sg_failed(e = push_out(token, (uint64_t)rows * 4)) && (out == logits || !sg_failed(e = push_out(out, lb)))) {
+        !sg_failed(e = push_out(token, (uint64_t)rows * 4)) && (out == logits || !sg_failed(e = push_out(out, outs[2] ? size_of(logits) : lb)))) {
         const sgk_logits_args a = {DEV(logits), DEV(counts), DEV(bias), DEV(mask), DEV(out), DEV(token), vocab, rows, rep, freq, pres};
-        e = finish_done(g, sgk_logits(&a, part, g->stream, g->done), outs, 2);
+        e = finish_done(g, sgk_logits(&a, part, g->stream, g->done), outs, 3);
     }
     return back_to(g, was, e);
 }
