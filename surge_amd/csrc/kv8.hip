@@ -295,11 +295,14 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
 //  - S^T = K Q^T leaves lane (li, lg) row li's scores of keys 4 lg .. 4 lg + 3
 //    of both tiles, the order of the value records' dwords, so V^T P^T runs on
 //    v_mfma_f32_16x16x32_f16 with the codes as f16 (exact) and p in two halves;
-//  - the values' scale goes into p: w = p s_V. The running maximum is taken
-//    over score + log2 s_V, so that w <= 2^12 whatever the scales are, while
-//    the sum of p, at most 2^92 a key (log2 s_V >= -80), stays in f32's range.
-//    2^12 keeps w's lower half above f16's subnormals down to 2^-26 of the
-//    largest.
+//  - the values' scale s_V = g 2^e goes into the weights: w = 2^(score + e - m)
+//    g 2^13 with a running maximum m of score + e, kept as an integer. So w <
+//    2^13 whatever the scales are, while the sum of the softmax's own weights, w
+//    / s_V, at most 2^92 a key (e >= -79), stays in f32's range. e - m and the
+//    rescaling by 2^(m - m') are exact, and no rounding is common to a block's
+//    keys; those of the exponents, half a step of score + e - m each, are small
+//    where a weight is large. 2^13 keeps w's lower half above f16's subnormals
+//    down to 2^-25 of the largest.
 // No barrier or LDS in the key loop; the waves' maxima, sums and outputs join
 // at the end. Bound by the cache's bytes: 262000 keys of 4 x 256 (537 MB) 85 us,
 // 6.3 TB/s, where a plain read reaches 6.6; 32771 of 8 x 128 (67 MB) 14.0, with
@@ -317,7 +320,15 @@ __device__ __forceinline__ void part_of(uint32_t n, uint32_t sp, kv8_div splits,
     end = first + q + (sp < more);
 }
 
-#define KV8_P2 12.0f
+#define KV8_P2 13
+// A block's scale of values as its keys' weights take it.
+struct v_scale { float e, g, rs; };         // exponent, 2^KV8_P2 mantissa, 2^KV8_P2 / 2^e
+__device__ __forceinline__ v_scale v_scale_of(float s) {
+    float a;
+    asm("v_max_f32 %0, |%1|, %2" : "=v"(a) : "v"(s), "s"(0x1p-80f));          // zero as if tiny
+    const int e = __builtin_amdgcn_frexp_expf(a);
+    return (v_scale){(float)e, __builtin_amdgcn_ldexpf(s, KV8_P2 - e), __builtin_amdgcn_ldexpf(1.0f, KV8_P2 - e)};     // NaN stays in g
+}
 
 // 16 f32 of a row as the three digits' operand bytes: with 0x808080 added, the
 // bytes of round(x inv) are its balanced digits plus 128, carries and all.
@@ -395,10 +406,17 @@ __device__ __forceinline__ float q_row(float (&x)[NC][16], float mul, v4i (&d)[3
     for (int c = 0; c < NC; c++) q_digits(x[c], inv, d[0][c], d[1][c], d[2][c]);
     return bad ? NAN : am / KV8_QMAX * fabsf(mul) / up;
 }
-// the score sums of the three digits as one float (a2 * 256 + a1 < 2^31)
-__device__ __forceinline__ float q_join(int a0, int a1, int a2) {
-    return fmaf((float)(a2 * 256 + a1), 256.0f, (float)a0);
+// The score sums of the three digits as one float. The lowest's starts at the bits
+// of 1.5 2^23, so that it comes out as a float, that much larger (it is
+// below 2^22, 128 x 127 x 256); the highest's starts at that much less, in its
+// units: a conversion a score less (a2 * 256 + a1 < 2^31).
+struct q_start { v4i lo, hi; };
+__device__ __forceinline__ q_start q_starts() {
+    q_start s = {{0x4B400000, 0x4B400000, 0x4B400000, 0x4B400000}, {-192, -192, -192, -192}};
+    asm volatile("" : "+v"(s.lo), "+v"(s.hi));      // in registers, not made again for every sum
+    return s;
 }
+__device__ __forceinline__ float q_join(int a0, int a1, int a2) { return fmaf((float)(a2 * 256 + a1), 256.0f, __int_as_float(a0)); }
 // eight codes (two dwords) as f16: the byte + 128 under 1024's exponent, less 1152
 __device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
     const f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
@@ -416,19 +434,49 @@ __device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
     return r;
 }
 
-// Whether a group's least scales (the same in every lane) are those of the
-// usual case; NaN is not, where the minimum shows it.
-__device__ __forceinline__ bool scales_usual(float ks, float vs) {
-    return __builtin_amdgcn_readfirstlane(ks >= 0.0f && vs >= 0x1p-80f);
+// Whether a record's scales, by their bits, are those of the usual case: keys'
+// zero or positive, values' at least 2^-80, both finite; and the values' of that
+// case, in scalar registers.
+__device__ __forceinline__ bool scales_usual(uint32_t ks, uint32_t vs) {
+    return ks <= 0x7F7FFFFFu && vs - 0x17800000u <= 0x7F7FFFFFu - 0x17800000u;
+}
+__device__ __forceinline__ v_scale v_scale_usual(uint32_t s) {
+    const uint32_t e = s >> 23;
+    return (v_scale){(float)((int)e - 126), __uint_as_float((s & 0x7FFFFFu) | (126u + KV8_P2) << 23), __uint_as_float((253u + KV8_P2 - e) << 23)};
 }
 
-// w[0], w[1] as f16 and what is left of them, packed
-__device__ __forceinline__ void split2(float w0, float w1, f16x2 &hi, f16x2 &lo) {
-    hi = __builtin_convertvector((f32x2){w0, w1}, f16x2);
-    uint32_t l;
-    asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(l) : "v"(hi), "v"(w0));
-    asm("v_fma_mixhi_f16 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(l) : "v"(hi), "v"(w1));
-    lo = __builtin_bit_cast(f16x2, l);
+// p g as f16 and what is left of it, four of a row: elements at .. at + 3 of the
+// operands. The first half is the product of p's and g's (the mixed fma that
+// would round p g itself takes twice a conversion's or a packed product's
+// cycles), the second what p g exceeds it by, to 2^-22 of p g. UNI: g is the same
+// in every lane, in a scalar register. The compiler does not see the block's
+// instructions: a half is written another instruction after its neighbour, and p,
+// whose exp the next instruction could not take, has been read by then.
+template <bool UNI>
+__device__ __forceinline__ void split4(const float (&p)[4], float g, f16x8 &hi, f16x8 &lo, int at) {
+    const f16x2 gg = __builtin_convertvector((f32x2){g, g}, f16x2);
+    f16x2 h[2];
+    uint32_t l[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) h[i] = __builtin_convertvector((f32x2){p[2 * i], p[2 * i + 1]}, f16x2) * gg;
+#define REST(G)                                                                                                                      \
+    asm("v_fma_mixlo_f16 %0, %2, %6, -%7 op_sel_hi:[0,0,1]\n\t"                                                                      \
+        "v_fma_mixlo_f16 %1, %4, %6, -%8 op_sel_hi:[0,0,1]\n\t"                                                                      \
+        "v_fma_mixhi_f16 %0, %3, %6, -%7 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"                                                       \
+        "v_fma_mixhi_f16 %1, %5, %6, -%8 op_sel:[0,0,1] op_sel_hi:[0,0,1]"                                                           \
+        : "=&v"(l[0]), "=&v"(l[1])                                                                                                   \
+        : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), G(g), "v"(h[0]), "v"(h[1]))
+    if (UNI) REST("s");
+    else REST("v");
+#undef REST
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const f16x2 b = __builtin_bit_cast(f16x2, l[i]);
+        hi[at + 2 * i] = h[i][0];
+        hi[at + 2 * i + 1] = h[i][1];
+        lo[at + 2 * i] = b[0];
+        lo[at + 2 * i + 1] = b[1];
+    }
 }
 
 // The largest of two or three; unlike fmaxf's code, operands are taken as they
@@ -456,64 +504,42 @@ __device__ __forceinline__ float rows_max(float m, float v) {
 // One group of UN tiles' scores to weights, online: updates the row's running
 // maximum and sum, gives the weights' f16 halves in operand order and what the
 // output so far is to be multiplied by. x: the integer scores; f: what they are
-// to be multiplied by (scale, q's unit, the keys' scale), per tile. Key `key` +
-// 16 u + 4 lg + e is visible up to pos (groups are aligned, so that the sum
-// stays in 32 bits at the last position, too).
-// The usual group has all its keys visible, f >= 0 and the values' scales vs >=
-// 2^-80: then the weight is one fma and one exp2, w = 2^(x f + lv - m0), and the
-// sum of p is the sum of w rv, with v = lv = log2 vs and rv = 1 / vs (an error
-// of lv is in both, and drops out). GEN takes any, v = vs: masked keys apart (a
-// row with no key yet has m0 = -inf), a scale of zero or NaN.
+// to be multiplied by (scale, q's unit, the keys' scale), v: the values' scale,
+// per tile. Key `key` + 16 u + 4 lg + e is visible up to pos (groups are aligned,
+// so that the sum stays in 32 bits at the last position, too).
+// The usual group has all its keys visible, f >= 0 and the values' scales at
+// least 2^-80. GEN takes any: masked keys apart (a row with no key yet has the
+// maximum -inf), whose block's scale, NaN perhaps, is not theirs to see.
 template <int UN, bool GEN>
-__device__ __forceinline__ float softmax_step(const float (&x)[UN][4], const float (&f)[UN], const float (&v)[UN], const float (&rv)[UN],
-                                              uint32_t key, uint32_t pos, float &mrun, float &lsum, f16x8 (&ph)[UN / 2],
-                                              f16x8 (&pl)[UN / 2]) {
+__device__ __forceinline__ float softmax_step(const float (&x)[UN][4], const float (&f)[UN], const v_scale (&v)[UN], uint32_t key, uint32_t pos,
+                                              float &mrun, float &lsum, f16x8 (&ph)[UN / 2], f16x8 (&pl)[UN / 2]) {
     const uint32_t k0 = key + ((threadIdx.x & 63) >> 4 << 2);
     float tm = -INFINITY;
 #pragma unroll
     for (int u = 0; u < UN; u++) {
         if (GEN) {
-            const float lv = __builtin_amdgcn_logf(fmaxf(fabsf(v[u]), 0x1p-80f));
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                tm = fmaxf(tm, k0 + 16 * u + e <= pos ? fmaf(x[u][e], f[u], lv) : -INFINITY);
-            }
+            for (int e = 0; e < 4; e++) tm = fmaxf(tm, k0 + 16 * u + e <= pos ? fmaf(x[u][e], f[u], v[u].e) : -INFINITY);
         } else {
-            const float t = fmaf(max2(max3(x[u][0], x[u][1], x[u][2]), x[u][3]), f[u], v[u]);
+            const float t = fmaf(max2(max3(x[u][0], x[u][1], x[u][2]), x[u][3]), f[u], v[u].e);
             tm = u ? max2(tm, t) : t;
         }
     }
-    const float mnew = rows_max(mrun, tm), m0 = mnew - KV8_P2;
+    const float mnew = ceilf(rows_max(mrun, tm));
     const float al = GEN && mrun == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrun - mnew);
     mrun = mnew;
     float l = lsum * al;
 #pragma unroll
     for (int u = 0; u < UN; u++) {
-        float w[4];
-        if (GEN) {
+        const float c = v[u].e - mnew, g = GEN && k0 + 16 * u > pos ? 0.0f : v[u].g;
+        float p[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const bool vis = k0 + 16 * u + e <= pos;
-                const float p = vis ? __builtin_amdgcn_exp2f(fmaf(x[u][e], f[u], -m0)) : 0.0f;
-                l += p;
-                w[e] = vis ? p * v[u] : 0.0f;
-            }
-        } else {
-            const float c = v[u] - m0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_exp2f(fmaf(x[u][e], f[u], c));
-            l = fmaf((w[0] + w[1]) + (w[2] + w[3]), rv[u], l);
+        for (int e = 0; e < 4; e++) {
+            p[e] = __builtin_amdgcn_exp2f(fmaf(x[u][e], f[u], c));
+            if (GEN && k0 + 16 * u + e > pos) p[e] = 0.0f;
         }
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-            f16x2 hi, lo;
-            split2(w[e], w[e + 1], hi, lo);
-            const int at = 4 * (u & 1) + e;
-            ph[u / 2][at] = hi[0];
-            ph[u / 2][at + 1] = hi[1];
-            pl[u / 2][at] = lo[0];
-            pl[u / 2][at + 1] = lo[1];
-        }
+        l = fmaf((p[0] + p[1]) + (p[2] + p[3]), v[u].rs, l);
+        split4<!GEN>(p, g, ph[u / 2], pl[u / 2], 4 * (u & 1));
     }
     lsum = l;
     return al;
@@ -567,6 +593,7 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
     };
     uint32_t step = s0 + wave;
     const bool any = step < s1;
+    const q_start start = q_starts();
     v4i qd[3][NC];
     float qf = 0.0f;
     if (any) {
@@ -591,7 +618,7 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
         for (int u = 0; u < 2; u++) { ks[u] = nks[u]; vs[u] = nvs[u]; }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            v4i s[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+            v4i s[3] = {start.lo, {0, 0, 0, 0}, start.hi};
 #pragma unroll
             for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -602,12 +629,21 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
         }
         if (more) { load_s(step + NW); load_k(step + NW); }
         f16x8 ph[1], pl[1];
-        const float f[2] = {qf * ks[0], qf * ks[1]};
-        const bool usual = step * 32 + 31 <= first && scales_usual(fminf(ks[0], ks[1]), fminf(vs[0], vs[1]));
-        const float lv[2] = {__builtin_amdgcn_logf(vs[0]), __builtin_amdgcn_logf(vs[1])};
-        const float rv[2] = {__builtin_amdgcn_rcpf(vs[0]), __builtin_amdgcn_rcpf(vs[1])};
-        const float al2 = usual ? softmax_step<2, false>(sc, f, lv, rv, 0, 0, mrun, lsum, ph, pl)
-                                : softmax_step<2, true>(sc, f, vs, rv, step * 32, rpos, mrun, lsum, ph, pl);
+        uint32_t kb[2], vb[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            kb[u] = __builtin_amdgcn_readfirstlane(__float_as_uint(ks[u]));
+            vb[u] = __builtin_amdgcn_readfirstlane(__float_as_uint(vs[u]));
+        }
+        const float f[2] = {qf * __uint_as_float(kb[0]), qf * __uint_as_float(kb[1])};
+        float al2;
+        if (step * 32 + 31 <= first && scales_usual(kb[0], vb[0]) && scales_usual(kb[1], vb[1])) {
+            const v_scale v[2] = {v_scale_usual(vb[0]), v_scale_usual(vb[1])};
+            al2 = softmax_step<2, false>(sc, f, v, 0, 0, mrun, lsum, ph, pl);
+        } else {
+            const v_scale v[2] = {v_scale_of(vs[0]), v_scale_of(vs[1])};
+            al2 = softmax_step<2, true>(sc, f, v, step * 32, rpos, mrun, lsum, ph, pl);
+        }
         if (step != s0 + wave && __builtin_amdgcn_ballot_w64(al2 != 1.0f)) {       // the first step has nothing to rescale
 #pragma unroll
             for (int n = 0; n < NT; n++) o[n] *= al2;
@@ -690,8 +726,10 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
 // LDS done, then the barrier; loads from memory stay in flight
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// head_dim 64 stays within the 128 registers that let a second workgroup in (12 of
+// 64, 4096 tokens at 8192: 356 us, with one 439).
 template <int HD>
-__global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_part part, int al) {
+__global__ void __launch_bounds__(KV8_NW * 64, HD == 64 ? 4 : 2) k_kv8_tile(sgk_kv8_attn a, kv8_part part, int al) {
     constexpr int NC = HD / 64, NT = HD / 16, NTH = KV8_NW * 64;
     constexpr int KCH = 4 * NC * 64, VUN = 2 * NC * 64;     // 16-byte chunks of keys, units (two chunks) of values
     constexpr int KPT = (KCH + NTH - 1) / NTH, VPT = (VUN + NTH - 1) / NTH;
@@ -804,6 +842,7 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
     if (n) load_k(0);
     v4i qd[3][NC];
     const float qf = q_row<NC>(xq, a.scale * 1.44269504088896340736f, qd);
+    const q_start start = q_starts();
     float mrun = -INFINITY, lsum = 0.0f, resc = 1.0f;
     f32x4 o[NT];
 #pragma unroll
@@ -845,7 +884,7 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
 #pragma unroll
         for (int k = 0; k < NK; k++) {
             const int u = k / NC, c = k % NC;
-            if (c == 0) s[0] = s[1] = s[2] = (v4i){0, 0, 0, 0};
+            if (c == 0) { s[0] = start.lo; s[1] = (v4i){0, 0, 0, 0}; s[2] = start.hi; }
 #pragma unroll
             for (int d = 0; d < 3; d++)
                 s[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, fr[(NV + k) % RING]), qd[d][c], s[d], 0, 0, 0);
@@ -860,16 +899,14 @@ __global__ void __launch_bounds__(KV8_NW * 64) k_kv8_tile(sgk_kv8_attn a, kv8_pa
         auto from = [](float v, int j) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), j)); };
         const uint32_t key = (k0 + i) * 64;
         const float f[4] = {qf * from(sn, 0), qf * from(sn, 1), qf * from(sn, 2), qf * from(sn, 3)};
-        const float lg2 = __builtin_amdgcn_logf(sn), rc = __builtin_amdgcn_rcpf(sn);
-        const float rv[4] = {from(rc, 4), from(rc, 5), from(rc, 6), from(rc, 7)};
+        const v_scale s = v_scale_of(sn);
+        const v_scale v[4] = {{from(s.e, 4), from(s.g, 4), from(s.rs, 4)}, {from(s.e, 5), from(s.g, 5), from(s.rs, 5)},
+                              {from(s.e, 6), from(s.g, 6), from(s.rs, 6)}, {from(s.e, 7), from(s.g, 7), from(s.rs, 7)}};
         const float least = lane & 4 ? 0x1p-80f : 0.0f;
-        if (key + 63 <= wfirst && !__builtin_amdgcn_ballot_w64(!(sn >= least))) {
-            const float lv[4] = {from(lg2, 4), from(lg2, 5), from(lg2, 6), from(lg2, 7)};
-            resc = softmax_step<4, false>(sc, f, lv, rv, 0, 0, mrun, lsum, ph, pl);
-        } else {
-            const float vs[4] = {from(sn, 4), from(sn, 5), from(sn, 6), from(sn, 7)};
-            resc = softmax_step<4, true>(sc, f, vs, rv, key, rpos, mrun, lsum, ph, pl);
-        }
+        if (key + 63 <= wfirst && !__builtin_amdgcn_ballot_w64(!(sn >= least)))
+            resc = softmax_step<4, false>(sc, f, v, 0, 0, mrun, lsum, ph, pl);
+        else
+            resc = softmax_step<4, true>(sc, f, v, key, rpos, mrun, lsum, ph, pl);
     };
 
     ph[0] = ph[1] = pl[0] = pl[1] = (f16x8){};

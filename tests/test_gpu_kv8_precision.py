@@ -1,0 +1,60 @@
+"""What the attention over the 8-bit cache loses, by each output's own size: blocks
+of values whose scales are far apart, against the same in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+
+import kv8_oracle as K
+from test_gpu_kv8 import attend
+
+pytestmark = pytest.mark.gpu
+
+
+def plain(q, c, base, scale):
+    """K.attention's outputs, all rows of a head at once, and the rms error of a score: q's elements to a unit of
+    max|q| / (127 2^16), so off by that over sqrt(12) each, and two roundings of its own size (its integers joined,
+    its factor), at most u and so u / sqrt(3)."""
+    n, nh, hd = q.shape
+    g = nh // c.nkv
+    k, v = c.values(0, base + n), c.values(1, base + n)
+    hide = np.arange(base + n) > np.arange(base, base + n)[:, None]
+    out, ds = np.zeros(q.shape), np.zeros((n, nh))
+    for h in range(nh):
+        s = q[:, h].astype(np.float64) @ k[:, h // g].T * scale
+        unit = abs(scale) * np.abs(q[:, h]).max(axis=1) / (127 * 2 ** 16) * np.linalg.norm(k[:, h // g], axis=1).max()
+        ds[:, h] = np.sqrt(unit ** 2 / 12 + 2 / 3 * (2.0 ** -24 * np.abs(s).max(axis=1)) ** 2)
+        s[hide] = -np.inf
+        p = np.exp(s - s.max(axis=1, keepdims=True))
+        out[:, h] = p @ v[:, h // g] / p.sum(axis=1, keepdims=True)
+    return out, ds
+
+
+@pytest.mark.parametrize("nh,nkv,hd,block,base,n", [(64, 64, 64, 32, 255, 1), (32, 32, 128, 16, 255, 1), (32, 16, 256, 64, 511, 1),
+                                                    (64, 16, 64, 32, 200, 56), (32, 8, 256, 64, 0, 1024), (48, 8, 128, 16, 0, 1024)])
+@pytest.mark.parametrize("apart", [2.0 ** -8, 2.0 ** -30, 2.0 ** -60])
+@pytest.mark.parametrize("size", [0.0, 0.01, 1.0])
+def test_scales_of_any_mantissa_far_apart(gpu, nh, nkv, hd, block, base, n, apart, size):
+    """Every second block's values are `apart` times the others', with two scales of a kv head and no power of two
+    among them: the small ones count in the sum below alone, and a rounding that all their weights have in common
+    does not drop out. In units of u = 2^-24 and as root mean squares, with m keys: a weight 1.4 (exp 2 at most, its
+    argument and the two halves), m / 16 additions of a third's root each, the sum below 1 (exp), the small blocks'
+    arguments there, up to log2(apart) = 60, half a step of which is 32 ln 2 = 22, over half the keys and weighed by
+    a half, the last steps 0.7. A score's error counts in both sums. Three times their root sum of squares."""
+    rng = np.random.default_rng(nh + n)
+    m = base + n
+    c = K.Cache(nkv, hd, block, m)
+    c.codes[...] = rng.integers(-127, 128, c.codes.shape)
+    c.scales[:, :, 0] = 1 / 60
+    c.scales[:, :, 1] = rng.uniform(0.01, 0.02, nkv)
+    c.scales[1::2, :, 1] = rng.uniform(1, 2, nkv) * 0.01 * apart
+    q = (rng.standard_normal((n, nh, hd)) * size).astype(np.float32)
+    want, ds = plain(q, c, base, 1 / math.sqrt(hd))
+    got = attend(gpu, c, q, base, 1 / math.sqrt(hd), "decode" if n == 1 else "prefill").astype(np.float64)
+    keys = np.arange(base + 1, m + 1)
+    u = 2.0 ** -24
+    rest = 1.4 ** 2 + keys / 48 + 1 + 0.25 * (22 / math.sqrt(3)) ** 2 / np.maximum(keys / 2, 1) + 0.7 ** 2
+    tol = 3 * np.sqrt(u ** 2 * rest[:, None] + (2 * ds) ** 2)
+    err = np.linalg.norm(got - want, axis=2) / np.linalg.norm(want, axis=2) / tol
+    seen = keys > 2 * block          # both kinds
+    assert (err[seen] <= 1).all(), f"worst error {err[seen].max():.2f} of its tolerance, which is {tol[-1].mean() / u:.1f} u"
