@@ -296,13 +296,13 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
 //    of both tiles, the order of the value records' dwords, so V^T P^T runs on
 //    v_mfma_f32_16x16x32_f16 with the codes as f16 (exact) and p in two halves;
 //  - the values' scale s_V = g 2^e goes into the weights: w = 2^(score + e - m)
-//    g 2^13 with a running maximum m of score + e, kept as an integer. So w <
-//    2^13 whatever the scales are, while the sum of the softmax's own weights, w
-//    / s_V, at most 2^92 a key (e >= -79), stays in f32's range. e - m and the
-//    rescaling by 2^(m - m') are exact, and no rounding is common to a block's
-//    keys; those of the exponents, half a step of score + e - m each, are small
-//    where a weight is large. 2^13 keeps w's lower half above f16's subnormals
-//    down to 2^-25 of the largest.
+//    g 2^13 with m an integer near the maximum of score + e, renewed where a
+//    weight would pass 2^15.5. So w is in f16's range whatever the scales are,
+//    while the sum of the softmax's own weights, w / s_V, at most 2^95 a key (e >=
+//    -79), stays in f32's. e - m and the rescaling by 2^(m - m') are exact, and no
+//    rounding is common to a block's keys; those of the exponents, half a step of
+//    score + e - m each, are small where a weight is large. 2^13 keeps w's lower
+//    half above f16's subnormals down to 2^-25 of the largest.
 // No barrier or LDS in the key loop; the waves' maxima, sums and outputs join
 // at the end. Bound by the cache's bytes: 262000 keys of 4 x 256 (537 MB) 85 us,
 // 6.3 TB/s, where a plain read reaches 6.6; 32771 of 8 x 128 (67 MB) 14.0, with
@@ -321,6 +321,7 @@ __device__ __forceinline__ void part_of(uint32_t n, uint32_t sp, kv8_div splits,
 }
 
 #define KV8_P2 13
+#define KV8_OVER 2.5f       // how far an exponent may pass the maximum kept before that is renewed: weights below 2^15.5
 // A block's scale of values as its keys' weights take it.
 struct v_scale { float e, g, rs; };         // exponent, 2^KV8_P2 mantissa, 2^KV8_P2 / 2^e
 __device__ __forceinline__ v_scale v_scale_of(float s) {
@@ -446,19 +447,18 @@ __device__ __forceinline__ v_scale v_scale_usual(uint32_t s) {
 }
 
 // p g as f16 and what is left of it, four of a row: elements at .. at + 3 of the
-// operands. The first half is the product of p's and g's (the mixed fma that
-// would round p g itself takes twice a conversion's or a packed product's
-// cycles), the second what p g exceeds it by, to 2^-22 of p g. UNI: g is the same
-// in every lane, in a scalar register. The compiler does not see the block's
-// instructions: a half is written another instruction after its neighbour, and p,
-// whose exp the next instruction could not take, has been read by then.
+// operands, together to 2^-22 of p g. (A mixed fma for the first half would take
+// two products' and the conversion's cycles, 8.3 against 2.4 and 4.4.) UNI: g is
+// the same in every lane, in a scalar register. The compiler does not see the
+// block's instructions: a half is written another instruction after its
+// neighbour, and p, whose exp the next instruction could not take, has been read
+// by then.
 template <bool UNI>
 __device__ __forceinline__ void split4(const float (&p)[4], float g, f16x8 &hi, f16x8 &lo, int at) {
-    const f16x2 gg = __builtin_convertvector((f32x2){g, g}, f16x2);
     f16x2 h[2];
     uint32_t l[2];
 #pragma unroll
-    for (int i = 0; i < 2; i++) h[i] = __builtin_convertvector((f32x2){p[2 * i], p[2 * i + 1]}, f16x2) * gg;
+    for (int i = 0; i < 2; i++) h[i] = __builtin_convertvector((f32x2){p[2 * i] * g, p[2 * i + 1] * g}, f16x2);
 #define REST(G)                                                                                                                      \
     asm("v_fma_mixlo_f16 %0, %2, %6, -%7 op_sel_hi:[0,0,1]\n\t"                                                                      \
         "v_fma_mixlo_f16 %1, %4, %6, -%8 op_sel_hi:[0,0,1]\n\t"                                                                      \
@@ -501,41 +501,60 @@ __device__ __forceinline__ float rows_max(float m, float v) {
     return max3(m, __uint_as_float(q[0]), __uint_as_float(q[1]));
 }
 
-// One group of UN tiles' scores to weights, online: updates the row's running
-// maximum and sum, gives the weights' f16 halves in operand order and what the
-// output so far is to be multiplied by. x: the integer scores; f: what they are
+// One group of UN tiles' scores to weights, online: updates the row's maximum and
+// sum, gives the weights' f16 halves in operand order and what the output so far
+// is to be multiplied by. x: the integer scores; f: what they are
 // to be multiplied by (scale, q's unit, the keys' scale), v: the values' scale,
 // per tile. Key `key` + 16 u + 4 lg + e is visible up to pos (groups are aligned,
 // so that the sum stays in 32 bits at the last position, too).
 // The usual group has all its keys visible, f >= 0 and the values' scales at
-// least 2^-80. GEN takes any: masked keys apart (a row with no key yet has the
+// least 2^-80, and looks only whether some exponent passes the maximum kept. GEN
+// takes any: masked keys apart (a row with no key yet has the
 // maximum -inf), whose block's scale, NaN perhaps, is not theirs to see.
 template <int UN, bool GEN>
 __device__ __forceinline__ float softmax_step(const float (&x)[UN][4], const float (&f)[UN], const v_scale (&v)[UN], uint32_t key, uint32_t pos,
                                               float &mrun, float &lsum, f16x8 (&ph)[UN / 2], f16x8 (&pl)[UN / 2]) {
     const uint32_t k0 = key + ((threadIdx.x & 63) >> 4 << 2);
-    float tm = -INFINITY;
+    float t[UN][4], al = 1.0f, over;
+    auto exponents = [&]() {
 #pragma unroll
-    for (int u = 0; u < UN; u++) {
-        if (GEN) {
+        for (int u = 0; u < UN; u++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) tm = fmaxf(tm, k0 + 16 * u + e <= pos ? fmaf(x[u][e], f[u], v[u].e) : -INFINITY);
-        } else {
-            const float t = fmaf(max2(max3(x[u][0], x[u][1], x[u][2]), x[u][3]), f[u], v[u].e);
-            tm = u ? max2(tm, t) : t;
+            for (int e = 0; e < 4; e++) t[u][e] = fmaf(x[u][e], f[u], v[u].e - mrun);
+    };
+    if (!GEN) {
+        exponents();
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+            const float m = max3(t[u][0], t[u][1], t[u][2]);
+            over = u ? max3(over, m, t[u][3]) : max2(m, t[u][3]);
         }
     }
-    const float mnew = ceilf(rows_max(mrun, tm));
-    const float al = GEN && mrun == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrun - mnew);
-    mrun = mnew;
-    float l = lsum * al;
+    if (GEN || __builtin_amdgcn_ballot_w64(!(over <= KV8_OVER))) {
+        float tm = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+            if (GEN) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) tm = fmaxf(tm, k0 + 16 * u + e <= pos ? fmaf(x[u][e], f[u], v[u].e) : -INFINITY);
+            } else {
+                tm = max2(tm, fmaf(max2(max3(x[u][0], x[u][1], x[u][2]), x[u][3]), f[u], v[u].e));
+            }
+        }
+        const float mnew = ceilf(rows_max(mrun, tm));
+        al = mrun == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrun - mnew);
+        mrun = mnew;
+        lsum *= al;
+        exponents();
+    }
+    float l = lsum;
 #pragma unroll
     for (int u = 0; u < UN; u++) {
-        const float c = v[u].e - mnew, g = GEN && k0 + 16 * u > pos ? 0.0f : v[u].g;
+        const float g = GEN && k0 + 16 * u > pos ? 0.0f : v[u].g;
         float p[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            p[e] = __builtin_amdgcn_exp2f(fmaf(x[u][e], f[u], c));
+            p[e] = __builtin_amdgcn_exp2f(t[u][e]);
             if (GEN && k0 + 16 * u + e > pos) p[e] = 0.0f;
         }
         l = fmaf((p[0] + p[1]) + (p[2] + p[3]), v[u].rs, l);

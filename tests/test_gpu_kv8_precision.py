@@ -58,3 +58,56 @@ def test_scales_of_any_mantissa_far_apart(gpu, nh, nkv, hd, block, base, n, apar
     err = np.linalg.norm(got - want, axis=2) / np.linalg.norm(want, axis=2) / tol
     seen = keys > 2 * block          # both kinds
     assert (err[seen] <= 1).all(), f"worst error {err[seen].max():.2f} of its tolerance, which is {tol[-1].mean() / u:.1f} u"
+
+
+FORMS = [(8, 2, 128, 32, 99, 1), (24, 4, 256, 64, 2999, 1), (12, 12, 64, 16, 200, 20), (32, 8, 256, 64, 0, 1024), (12, 12, 64, 32, 0, 2500)]
+
+
+@pytest.mark.parametrize("nh,nkv,hd,block,base,n", FORMS)
+def test_one_key_has_all_the_weight(gpu, nh, nkv, hd, block, base, n):
+    """Rows whose best key is exp(40) ahead are its values, with a weight's two halves between (2^-22, 4 u), the
+    sum of their products 2 and the division 1.5: to 8 u of every element."""
+    rng = np.random.default_rng(n)
+    m = base + n
+    c = K.Cache(nkv, hd, block, m)
+    c.codes[...] = rng.integers(-127, 128, c.codes.shape)
+    c.scales[...] = rng.uniform(0.01, 0.02, c.scales.shape)
+    q = (rng.standard_normal((n, nh, hd)) * 1e3).astype(np.float32)
+    got = attend(gpu, c, q, base, 1 / math.sqrt(hd), "decode" if n == 1 else "prefill")
+    k, v = c.values(0, m), c.values(1, m)
+    hide = np.arange(m) > np.arange(base, m)[:, None]
+    checked = 0
+    for h in range(nh):
+        s = q[:, h].astype(np.float64) @ k[:, h * nkv // nh].T / math.sqrt(hd)
+        s[hide] = -np.inf
+        best = s.argmax(axis=1)
+        top = s[np.arange(n), best]
+        s[np.arange(n), best] = -np.inf
+        clear = top - s.max(axis=1) > 41
+        want = v[best, h * nkv // nh]
+        assert (np.abs(got[:, h] - want)[clear] <= 8 * 2.0 ** -24 * np.abs(want)[clear] + 1e-12).all()
+        checked += clear.sum()
+    assert checked >= n * nh / 2
+
+
+@pytest.mark.parametrize("nh,nkv,hd,block,base,n", FORMS)
+@pytest.mark.parametrize("rise", [0.1, 0.6, 1.5, 2.6, 30.0, -0.7])
+def test_scores_that_rise_with_the_keys(gpu, nh, nkv, hd, block, base, n, rise):
+    """A block of 16 keys is `rise` ahead of the one before it, in the exponents of two: maxima that pass the one kept
+    a little, by little steps, by large ones, and never. Tolerance as above, without the small blocks."""
+    rng = np.random.default_rng(n)
+    m = base + n
+    c = K.Cache(nkv, hd, 16, m)
+    c.codes[...] = rng.integers(-127, 128, c.codes.shape)
+    c.codes[:, :, 0] = rng.integers(50, 100, c.codes[:, :, 0].shape)
+    q = rng.uniform(0.5, 1.5, (n, nh, hd)).astype(np.float32)
+    scale = 1 / math.sqrt(hd)
+    c.scales[:, :, 0] = np.arange(1, len(c.scales) + 1)[:, None] * (abs(rise) * math.log(2) / (75 * hd * scale))
+    c.scales[:, :, 1] = rng.uniform(0.01, 0.02, (len(c.scales), nkv))
+    q *= np.float32(math.copysign(1, rise))
+    want, ds = plain(q, c, base, scale)
+    got = attend(gpu, c, q, base, scale, "decode" if n == 1 else "prefill").astype(np.float64)
+    keys, u = np.arange(base + 1, m + 1), 2.0 ** -24
+    tol = 3 * np.sqrt(u ** 2 * (1.4 ** 2 + keys / 48 + 1 + 0.7 ** 2)[:, None] + (2 * ds) ** 2)
+    err = np.linalg.norm(got - want, axis=2) / np.linalg.norm(want, axis=2) / tol
+    assert (err <= 1).all(), f"worst error {err.max():.2f} of its tolerance"
