@@ -435,11 +435,26 @@ __device__ __forceinline__ f16x8 codes_f16(uint32_t a, uint32_t b) {
     return r;
 }
 
+// Exponents up to 2^20 are exact enough next to each other. Past that a maximum m
+// may be rounded by more than the scale's exponent, e, so far rows have their
+// weights times 2^-8 (2^-KV8_OFF), in which the usual scales' e fits.
+#define KV8_FAR 0x1p20f
+#define KV8_OFF 8.0f
+__device__ __forceinline__ float far_off(float m) { return fabsf(m) > KV8_FAR && m != -INFINITY ? KV8_OFF : 0.0f; }
+// The largest scale of keys with which no row of a wave can be far.
+__device__ __forceinline__ float ks_most(float qf, uint32_t hd) {
+    float m = qf;
+    m = fmaxf(m, __uint_as_float(dppu<0xB1>(__float_as_uint(m))));
+    m = fmaxf(m, __uint_as_float(dppu<0x4E>(__float_as_uint(m))));
+    m = fmaxf(m, __uint_as_float(dppu<0x141>(__float_as_uint(m))));
+    m = fmaxf(m, __uint_as_float(dppu<0x128>(__float_as_uint(m))));
+    return fminf(KV8_FAR / (KV8_QMAX * 127.0f) / (float)hd * __builtin_amdgcn_rcpf(m), 0x1.fffffep127f);
+}
 // Whether a record's scales, by their bits, are those of the usual case: keys'
-// zero or positive, values' at least 2^-80, both finite; and the values' of that
-// case, in scalar registers.
-__device__ __forceinline__ bool scales_usual(uint32_t ks, uint32_t vs) {
-    return ks <= 0x7F7FFFFFu && vs - 0x17800000u <= 0x7F7FFFFFu - 0x17800000u;
+// zero or positive and no larger than that, values' finite and at least 2^-80;
+// and the values' of that case, in scalar registers.
+__device__ __forceinline__ bool scales_usual(uint32_t ks, uint32_t vs, uint32_t most) {
+    return ks <= most && vs - 0x17800000u <= 0x7F7FFFFFu - 0x17800000u;
 }
 __device__ __forceinline__ v_scale v_scale_usual(uint32_t s) {
     const uint32_t e = s >> 23;
@@ -507,15 +522,23 @@ __device__ __forceinline__ float rows_max(float m, float v) {
 // to be multiplied by (scale, q's unit, the keys' scale), v: the values' scale,
 // per tile. Key `key` + 16 u + 4 lg + e is visible up to pos (groups are aligned,
 // so that the sum stays in 32 bits at the last position, too).
-// The usual group has all its keys visible, f >= 0 and the values' scales at
-// least 2^-80, and looks only whether some exponent passes the maximum kept. GEN
-// takes any: masked keys apart (a row with no key yet has the
-// maximum -inf), whose block's scale, NaN perhaps, is not theirs to see.
+// The usual group has all its keys visible, f >= 0, exponents within KV8_FAR and
+// the values' scales at least 2^-80, and looks only whether some exponent passes
+// the maximum kept. GEN takes any: masked keys apart (a row with no key yet has
+// the maximum -inf), whose block's scale, NaN perhaps, is not theirs to see; and
+// scores of any size. Next to a far maximum they are rounded before they are
+// compared, all in the same way: an unrounded product can lie whole powers of two
+// above or below its own rounding. far: some row is, and was taken by GEN.
 template <int UN, bool GEN>
 __device__ __forceinline__ float softmax_step(const float (&x)[UN][4], const float (&f)[UN], const v_scale (&v)[UN], uint32_t key, uint32_t pos,
-                                              float &mrun, float &lsum, f16x8 (&ph)[UN / 2], f16x8 (&pl)[UN / 2]) {
+                                              float &mrun, float &lsum, bool &far, f16x8 (&ph)[UN / 2], f16x8 (&pl)[UN / 2]) {
     const uint32_t k0 = key + ((threadIdx.x & 63) >> 4 << 2);
     float t[UN][4], al = 1.0f, over;
+    auto score = [&](int u, int e) {
+        float s = x[u][e] * f[u];
+        asm("" : "+v"(s));          // rounded here
+        return s;
+    };
     auto exponents = [&]() {
 #pragma unroll
         for (int u = 0; u < UN; u++)
@@ -536,16 +559,30 @@ __device__ __forceinline__ float softmax_step(const float (&x)[UN][4], const flo
         for (int u = 0; u < UN; u++) {
             if (GEN) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) tm = fmaxf(tm, k0 + 16 * u + e <= pos ? fmaf(x[u][e], f[u], v[u].e) : -INFINITY);
+                for (int e = 0; e < 4; e++) {
+                    const float m = score(u, e) + v[u].e;
+                    tm = fmaxf(tm, k0 + 16 * u + e <= pos ? m : -INFINITY);
+                }
             } else {
                 tm = max2(tm, fmaf(max2(max3(x[u][0], x[u][1], x[u][2]), x[u][3]), f[u], v[u].e));
             }
         }
         const float mnew = ceilf(rows_max(mrun, tm));
-        al = mrun == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mrun - mnew);
+        const float off = GEN ? far_off(mnew) : 0.0f, was = GEN ? far_off(mrun) : 0.0f;
+        al = mrun == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mrun - mnew) + (was - off));
         mrun = mnew;
         lsum *= al;
         exponents();
+        if (GEN && __builtin_amdgcn_ballot_w64(off != 0.0f)) {
+            far = true;
+#pragma unroll
+            for (int u = 0; u < UN; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float r = (score(u, e) - mrun) + (v[u].e - off);
+                    if (off != 0.0f) t[u][e] = r > KV8_OVER ? KV8_OVER : r;
+                }
+        }
     }
     float l = lsum;
 #pragma unroll
@@ -615,6 +652,7 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
     const q_start start = q_starts();
     v4i qd[3][NC];
     float qf = 0.0f;
+    uint32_t kmost = 0;
     if (any) {
         float xq[NC][16];
         q_load<NC>(a.q + tok * a.q_tok + (size_t)head * a.q_stride, al, lg, xq);
@@ -624,11 +662,13 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
         load_v(step);
         __builtin_amdgcn_sched_barrier(0);
         qf = q_row<NC>(xq, a.scale * 1.44269504088896340736f, qd);
+        kmost = __builtin_amdgcn_readfirstlane(__float_as_uint(ks_most(qf, HD)));
     }
     f32x4 o[NT];
 #pragma unroll
     for (int n = 0; n < NT; n++) o[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
     float mrun = -INFINITY, lsum = 0.0f;
+    bool far = false;
     // The last step stands apart: with its missing loads in the loop, waiting for
     // a step's keys is waiting for its values as well.
     auto work = [&](bool more) {
@@ -656,12 +696,12 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
         }
         const float f[2] = {qf * __uint_as_float(kb[0]), qf * __uint_as_float(kb[1])};
         float al2;
-        if (step * 32 + 31 <= first && scales_usual(kb[0], vb[0]) && scales_usual(kb[1], vb[1])) {
+        if (step * 32 + 31 <= first && !far && scales_usual(kb[0], vb[0], kmost) && scales_usual(kb[1], vb[1], kmost)) {
             const v_scale v[2] = {v_scale_usual(vb[0]), v_scale_usual(vb[1])};
-            al2 = softmax_step<2, false>(sc, f, v, 0, 0, mrun, lsum, ph, pl);
+            al2 = softmax_step<2, false>(sc, f, v, 0, 0, mrun, lsum, far, ph, pl);
         } else {
             const v_scale v[2] = {v_scale_of(vs[0]), v_scale_of(vs[1])};
-            al2 = softmax_step<2, true>(sc, f, v, step * 32, rpos, mrun, lsum, ph, pl);
+            al2 = softmax_step<2, true>(sc, f, v, step * 32, rpos, mrun, lsum, far, ph, pl);
         }
         if (step != s0 + wave && __builtin_amdgcn_ballot_w64(al2 != 1.0f)) {       // the first step has nothing to rescale
 #pragma unroll
@@ -681,6 +721,12 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
     if (any) work(false);
     // join the waves: each leaves its maximum, sum and output (-inf and zeros
     // without a step), one barrier. All of a row's are asked for at once.
+    if (far) {
+        const float k = __builtin_amdgcn_exp2f(far_off(mrun));
+        lsum *= k;
+#pragma unroll
+        for (int n = 0; n < NT; n++) o[n] *= k;
+    }
     lsum += swap16f(lsum);
     lsum += swap32f(lsum);
     if (li < R) {
@@ -861,8 +907,11 @@ __global__ void __launch_bounds__(KV8_NW * 64, HD == 64 ? 4 : 2) k_kv8_tile(sgk_
     if (n) load_k(0);
     v4i qd[3][NC];
     const float qf = q_row<NC>(xq, a.scale * 1.44269504088896340736f, qd);
+    // the usual scales' bounds, keys' or values' as in sn
+    const float least = lane & 4 ? 0x1p-80f : 0.0f, most = lane & 4 ? 0x1.fffffep127f : ks_most(qf, HD);
     const q_start start = q_starts();
     float mrun = -INFINITY, lsum = 0.0f, resc = 1.0f;
+    bool far = false;
     f32x4 o[NT];
 #pragma unroll
     for (int d = 0; d < NT; d++) o[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -899,20 +948,29 @@ __global__ void __launch_bounds__(KV8_NW * 64, HD == 64 ? 4 : 2) k_kv8_tile(sgk_
             if (k < NV) fetch(k + RING - 1);
             __builtin_amdgcn_sched_barrier(0);
         }
-        v4i s[3];
+        // A record's scores are joined behind the next one's first products, in this
+        // order (left to the compiler, joins that wait for their products come
+        // between: 24 heads of 256 on 4, 2048 tokens at 14336 1007 us against 1040 to
+        // 1130, 32 of 128 on 8 807 against 900); at head_dim 64, with one product a
+        // sum, as they come (12 heads 368 against 388).
+        constexpr bool LATE = NC > 1;
+        v4i s[2][3];
+        auto join = [&](int u) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) sc[u][e] = q_join(s[u & 1][0][e], s[u & 1][1][e], s[u & 1][2][e]);
+        };
 #pragma unroll
         for (int k = 0; k < NK; k++) {
             const int u = k / NC, c = k % NC;
-            if (c == 0) { s[0] = start.lo; s[1] = (v4i){0, 0, 0, 0}; s[2] = start.hi; }
+            if (c == 0) { s[u & 1][0] = start.lo; s[u & 1][1] = (v4i){0, 0, 0, 0}; s[u & 1][2] = start.hi; }
 #pragma unroll
             for (int d = 0; d < 3; d++)
-                s[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, fr[(NV + k) % RING]), qd[d][c], s[d], 0, 0, 0);
+                s[u & 1][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, fr[(NV + k) % RING]), qd[d][c], s[u & 1][d], 0, 0, 0);
             fetch(NV + k + RING - 1);
-            if (c == NC - 1) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) sc[u][e] = q_join(s[0][e], s[1][e], s[2][e]);
-            }
+            if (LATE ? u && c == 1 : c == NC - 1) join(LATE ? u - 1 : u);
+            if (LATE) __builtin_amdgcn_sched_barrier(0);
         }
+        if (LATE) join(3);
     };
     auto weights = [&](uint32_t i) {
         auto from = [](float v, int j) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), j)); };
@@ -921,11 +979,10 @@ __global__ void __launch_bounds__(KV8_NW * 64, HD == 64 ? 4 : 2) k_kv8_tile(sgk_
         const v_scale s = v_scale_of(sn);
         const v_scale v[4] = {{from(s.e, 4), from(s.g, 4), from(s.rs, 4)}, {from(s.e, 5), from(s.g, 5), from(s.rs, 5)},
                               {from(s.e, 6), from(s.g, 6), from(s.rs, 6)}, {from(s.e, 7), from(s.g, 7), from(s.rs, 7)}};
-        const float least = lane & 4 ? 0x1p-80f : 0.0f;
-        if (key + 63 <= wfirst && !__builtin_amdgcn_ballot_w64(!(sn >= least)))
-            resc = softmax_step<4, false>(sc, f, v, 0, 0, mrun, lsum, ph, pl);
+        if (key + 63 <= wfirst && !far && !__builtin_amdgcn_ballot_w64(__builtin_amdgcn_fmed3f(sn, least, most) != sn))
+            resc = softmax_step<4, false>(sc, f, v, 0, 0, mrun, lsum, far, ph, pl);
         else
-            resc = softmax_step<4, true>(sc, f, v, key, rpos, mrun, lsum, ph, pl);
+            resc = softmax_step<4, true>(sc, f, v, key, rpos, mrun, lsum, far, ph, pl);
     };
 
     ph[0] = ph[1] = pl[0] = pl[1] = (f16x8){};
@@ -971,6 +1028,12 @@ __global__ void __launch_bounds__(KV8_NW * 64, HD == 64 ? 4 : 2) k_kv8_tile(sgk_
             products(i);
             lds_barrier();
         }
+    }
+    if (far) {
+        const float k = __builtin_amdgcn_exp2f(far_off(mrun));
+        lsum *= k;
+#pragma unroll
+        for (int n = 0; n < NT; n++) o[n] *= k;
     }
     lsum += swap16f(lsum);
     lsum += swap32f(lsum);

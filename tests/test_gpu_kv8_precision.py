@@ -111,3 +111,63 @@ def test_scores_that_rise_with_the_keys(gpu, nh, nkv, hd, block, base, n, rise):
     tol = 3 * np.sqrt(u ** 2 * (1.4 ** 2 + keys / 48 + 1 + 0.7 ** 2)[:, None] + (2 * ds) ** 2)
     err = np.linalg.norm(got - want, axis=2) / np.linalg.norm(want, axis=2) / tol
     assert (err <= 1).all(), f"worst error {err.max():.2f} of its tolerance"
+
+
+@pytest.mark.parametrize("nh,nkv,hd,block,base,n", FORMS)
+@pytest.mark.parametrize("size", [1e5, 1e6, 1e7, 1e8, 1e15, 1e30])
+def test_scores_far_from_zero(gpu, nh, nkv, hd, block, base, n, size):
+    """Scores past 2^20, and past 2^24, where their steps are larger than one: every second head's q times `size`.
+    Such a row is all its best key's (rows whose next one is within the scores' rounding are left out; 8 u as above),
+    and the rows beside it, in the same waves, are what they are by themselves."""
+    rng = np.random.default_rng(n)
+    m = base + n
+    c = K.Cache(nkv, hd, block, m)
+    c.codes[...] = rng.integers(-127, 128, c.codes.shape)
+    c.scales[...] = rng.uniform(0.01, 0.02, c.scales.shape)
+    q = rng.standard_normal((n, nh, hd)).astype(np.float32)
+    small, scale, u = q.copy(), 1 / math.sqrt(hd), 2.0 ** -24
+    q[:, ::2] *= np.float32(size)
+    entry = "decode" if n == 1 else "prefill"
+    got = attend(gpu, c, q, base, scale, entry)
+    assert np.isfinite(got).all()
+    want, ds = plain(small, c, base, scale)
+    keys = np.arange(base + 1, m + 1)
+    tol = 3 * np.sqrt(u ** 2 * (1.4 ** 2 + keys / 48 + 1 + 0.7 ** 2)[:, None] + (2 * ds) ** 2)
+    err = np.linalg.norm(got - want, axis=2) / np.linalg.norm(want, axis=2) / tol
+    assert (err[:, 1::2] <= 1).all()
+    k, v = c.values(0, m), c.values(1, m)
+    hide = np.arange(m) >= keys[:, None]
+    checked = 0
+    for h in range(0, nh, 2):
+        s = q[:, h].astype(np.float64) @ k[:, h * nkv // nh].T * scale
+        s[hide] = -np.inf
+        best = s.argmax(axis=1)
+        top = s[np.arange(n), best]
+        s[np.arange(n), best] = -np.inf
+        # a score's rounding: a unit of q's in every dim, and 16 of its own size
+        off = scale * 2 * u * np.abs(q[:, h]).max(axis=1) * np.abs(k[:, h * nkv // nh]).sum(axis=1).max() + 16 * u * np.abs(top)
+        clear = top - s.max(axis=1) > 2 * off + 41
+        one = v[best, h * nkv // nh]
+        assert (np.abs(got[:, h] - one)[clear] <= 8 * u * np.abs(one)[clear] + 1e-12).all()
+        checked += clear.sum()
+    assert checked >= n * nh / 4
+
+
+@pytest.mark.parametrize("nh,nkv,hd,block,base,n", FORMS)
+@pytest.mark.parametrize("far", [-3e7, -1e10, 3e7, 1e10])
+def test_all_scores_far_from_zero(gpu, nh, nkv, hd, block, base, n, far):
+    """Every key alike, its score `far` from zero on either side: the mean of the values."""
+    rng = np.random.default_rng(n)
+    m = base + n
+    c = K.Cache(nkv, hd, block, m)
+    c.codes[...] = rng.integers(-127, 128, c.codes.shape)
+    c.codes[:, :, 0] = 100
+    c.scales[:, :, 0] = 0.01
+    c.scales[:, :, 1] = rng.uniform(0.01, 0.02, c.scales.shape[:2])
+    q = np.full((n, nh, hd), far / math.sqrt(hd), np.float32)
+    got = attend(gpu, c, q, base, 1 / math.sqrt(hd), "decode" if n == 1 else "prefill")
+    want, _ = plain(q * 0, c, base, 1.0)
+    keys, u = np.arange(base + 1, m + 1), 2.0 ** -24
+    tol = 3 * u * np.sqrt(1.4 ** 2 + keys / 48 + 1 + 0.7 ** 2)
+    assert np.isfinite(got).all()
+    assert (np.linalg.norm(got - want, axis=2) / np.linalg.norm(want, axis=2) <= tol[:, None]).all()
