@@ -380,6 +380,13 @@ sg_err sg_gpu_run_kv8_store(sg_gpu *g, void *k, void *v, void *codes, void *scal
 sg_err sg_gpu_run_kv8_load(sg_gpu *g, void *codes, void *scales, void *k, void *v, const uint32_t params[8]);
 sg_err sg_gpu_run_attn_decode_kv8(sg_gpu *g, void *q, void *codes, void *scales, void *out, const uint32_t params[8]);
 sg_err sg_gpu_run_attn_prefill_kv8(sg_gpu *g, void *q, void *codes, void *scales, void *out, const uint32_t params[8]);
+/* How a call of either runs on this GPU (decode: base = seq - 1, n = 1): the parts
+ * that its keys are split into (where more than one, the handle's scratch holds n *
+ * n_heads * parts * (hd + 2) floats); *waves, unless NULL, is the waves of a
+ * workgroup that streams the keys, 4 or 8, or 0 where rows go in tiles of 128.
+ * 0 for a call that would be refused. */
+uint32_t sg_gpu_attn_kv8_parts(const sg_gpu *g, uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t base, uint32_t n,
+                               uint32_t *waves);
 
 /* Rotary positions with three axes (time, height, width; text has the three
  * alike): x, out [n][heads] slices at row stride p[7] (0 = heads * stride) and

@@ -121,6 +121,7 @@ _SIGS = {
     "sg_gpu_run_kv8_load": (SgErr, [C.c_void_p] * 5 + [C.POINTER(C.c_uint32)]),
     "sg_gpu_run_attn_decode_kv8": (SgErr, [C.c_void_p] * 5 + [C.POINTER(C.c_uint32)]),
     "sg_gpu_run_attn_prefill_kv8": (SgErr, [C.c_void_p] * 5 + [C.POINTER(C.c_uint32)]),
+    "sg_gpu_attn_kv8_parts": (C.c_uint32, [C.c_void_p] + [C.c_uint32] * 5 + [C.POINTER(C.c_uint32)]),
     "sg_gpu_run_rope_axes": (SgErr, [C.c_void_p] * 4 + [C.POINTER(C.c_uint32)]),
     "sg_gpu_run_token_counts": (SgErr, [C.c_void_p] * 3 + [C.POINTER(C.c_uint32)]),
     "sg_gpu_run_logits": (SgErr, [C.c_void_p] * 7 + [C.POINTER(C.c_uint32)]),
@@ -333,6 +334,11 @@ class Gpu:
     def attn_prefill_kv8(self, q, codes, scales, out, p):
         check(lib().sg_gpu_run_attn_prefill_kv8(self.handle, q.handle, codes.handle, scales.handle, out.handle,
                                                 params(p)))
+
+    def attn_kv8_parts(self, n_heads, n_kv, hd, base, n):
+        """(parts, waves): how attention over the 8-bit cache runs such a call."""
+        w = C.c_uint32()
+        return lib().sg_gpu_attn_kv8_parts(self.handle, n_heads, n_kv, hd, base, n, C.byref(w)), w.value
 
     def rope_axes(self, x, pos, out, p):
         check(lib().sg_gpu_run_rope_axes(self.handle, x.handle, pos.handle, out.handle, params(p)))

@@ -1029,6 +1029,14 @@ static sg_err attn_kv8_oneshot(sg_gpu *g, const char *who, void *q, void *codes,
     return back_to(g, was, e);
 }
 
+uint32_t sg_gpu_attn_kv8_parts(const sg_gpu *g, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t base, uint32_t n, uint32_t *waves) {
+    if (waves) *waves = 0;
+    if (!g || !n || !sgk_kv8_shape_ok(nkv, hd, 16) || nkv > 65535 || !nh || nh % nkv || nh / nkv > SGK_KV8_MAX_GROUP ||
+        (uint64_t)base + n > UINT32_MAX - 128u || (uint64_t)n * (nh / nkv) > 1u << 30) return 0;
+    const sgk_kv8_attn a = {.n_heads = nh, .n_kv = nkv, .hd = hd, .block = 16, .base = base, .ntok = n};
+    return sgk_kv8_attn_parts(&a, waves);
+}
+
 sg_err sg_gpu_run_attn_decode_kv8(sg_gpu *g, void *q, void *codes, void *scales, void *out, const uint32_t p[8]) {
     if (!p) return (sg_err){"gpu: attn_decode_kv8 got a NULL argument"};
     const uint32_t seq = p[3];

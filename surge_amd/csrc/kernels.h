@@ -398,6 +398,8 @@ typedef struct {
 #define SGK_KV8_MAX_GROUP 16u       /* query heads per kv head */
 /* scratch: sgk_kv8_attn_scratch(a) bytes, 16-byte aligned (NULL if that is 0). */
 uint64_t sgk_kv8_attn_scratch(const sgk_kv8_attn *a);
+/* The parts of the keys; waves: of a workgroup that streams them, 0 where rows go in tiles. */
+uint32_t sgk_kv8_attn_parts(const sgk_kv8_attn *a, uint32_t *waves);
 hipError_t sgk_kv8_attention(const sgk_kv8_attn *a, void *scratch, hipStream_t s, hipEvent_t done);
 
 /* Rotary positions with three axes (token.hip): pair i turns by pos[axis(i)] *

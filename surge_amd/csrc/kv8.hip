@@ -1192,6 +1192,11 @@ static kv8_plan kv8_plan_of(const sgk_kv8_attn *a) {
     return p;
 }
 
+extern "C" uint32_t sgk_kv8_attn_parts(const sgk_kv8_attn *a, uint32_t *waves) {
+    const kv8_plan p = kv8_plan_of(a);
+    if (waves) *waves = p.waves;
+    return p.splits;
+}
 extern "C" uint64_t sgk_kv8_attn_scratch(const sgk_kv8_attn *a) {
     const kv8_plan p = kv8_plan_of(a);
     return p.splits > 1 ? (uint64_t)a->ntok * a->n_heads * p.splits * (a->hd + 2) * 4 : 0;

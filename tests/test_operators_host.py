@@ -234,3 +234,16 @@ def test_params_takes_what_can_be_iterated(make):
 
 def test_params_of_floats():
     assert list(S.params(x for x in (1.0, np.float32(2.5), np.int32(-2)))) == [1, 2, 0xFFFFFFFE, 0, 0, 0, 0, 0]
+
+
+def test_attention_parts():
+    """The query of how attention over the 8-bit cache runs: on the host alone, 0 for what a call would refuse."""
+    def parts(*a):
+        w = C.c_uint32(9)
+        return S.lib().sg_gpu_attn_kv8_parts(G, *a, C.byref(w)), w.value
+    assert parts(24, 4, 256, 17003, 1) == (64, 4) and parts(24, 4, 256, 383, 1) == (1, 8) and parts(24, 4, 256, 14336, 2048)[1] == 0
+    assert S.lib().sg_gpu_attn_kv8_parts(G, 24, 4, 256, 17003, 1, None) == 64
+    assert S.lib().sg_gpu_attn_kv8_parts(None, 24, 4, 256, 17003, 1, None) == 0
+    for bad in ((24, 4, 256, 17003, 0), (24, 5, 256, 0, 1), (0, 4, 256, 0, 1), (24, 0, 256, 0, 1), (17, 1, 64, 0, 1), (24, 4, 96, 0, 1),
+                (65536, 65536, 64, 0, 1), (24, 4, 256, 0xFFFFFFFF, 1), (16, 1, 64, 0, (1 << 26) + 1)):
+        assert parts(*bad) == (0, 0)
