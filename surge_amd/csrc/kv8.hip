@@ -305,8 +305,8 @@ extern "C" hipError_t sgk_kv8_load(const int8_t *codes, const float *scales, flo
 //    half above f16's subnormals down to 2^-25 of the largest.
 // No barrier or LDS in the key loop; the waves' maxima, sums and outputs join
 // at the end. Bound by the cache's bytes: 262000 keys of 4 x 256 (537 MB) 85 us,
-// 6.3 TB/s, where a plain read reaches 6.6; 32771 of 8 x 128 (67 MB) 14.0, with
-// the waves' start and end in it; 700 of 2 x 256 5.9, one step's chain: 2 us to
+// 6.3 TB/s, where a plain read reaches 6.6; 32771 of 8 x 128 (67 MB) 14.1, with
+// the waves' start and end in it; 700 of 2 x 256 6.0, one step's chain: 2 us to
 // the loads' arrival, then 0.4 in the softmax, 0.7 in either product, 0.9 to join.
 // ---------------------------------------------------------------------------
 struct kv8_part {
@@ -770,19 +770,20 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
 // a lane, no bank conflict), the value codes turned into f16 on the way. The
 // arithmetic is the wave form's.
 // A tile's work for a wave is 112 matrix products of 16 cycles (head_dim 256)
-// and about 265 vector instructions. Waves that run both in step leave the
+// and about 240 vector instructions. Waves that run both in step leave the
 // matrix unit idle through the softmax: 46% busy. So the two waves of a SIMD (w
 // and w + 4) alternate: one is in its products (the last tile's P V, this one's
 // K Q^T) while the other is in its softmax, with a barrier a tile. Beside a
 // wave that keeps the matrix unit busy another issues two vector instructions
-// per product (measured), so 224 products and 530 of those take at least 4200
-// cycles; a tile takes 4800, of which 3584 are the products'.
+// per product (measured), so 224 products and 480 of those take at least 3800
+// cycles, of which 3584 are the products'; over a launch it is busy 63%.
 // Both tiles are double-buffered; a wave stores its part of the next one and
 // requests that of the one after before its softmax.
-// 24 heads of 256 on 4, 2048 tokens at 14336: 1010-1060 us, 750 TFLOP/s of the
+// 24 heads of 256 on 4, 2048 tokens at 14336: 980-1050 us, 770 TFLOP/s of the
 // formula's, and as the matrix unit counts them (weights in two halves, three
-// digits at twice the rate) 1310, where a plain f16 product of 16384^3 reaches
-// 1346: the clock falls to 1.7 GHz under the load.
+// digits at twice the rate) 1340, where a plain f16 product of 16384^3 reaches
+// 1346: the clock falls to 1.7 GHz under the load. At head_dim 128 and 64 the
+// vector instructions bound it: 216 and 204 for 56 and 28 products.
 // Grid: (row block, kv head, key split), the longest rows first.
 // ---------------------------------------------------------------------------
 #define KV8_NW 8
@@ -1147,10 +1148,12 @@ __global__ void __launch_bounds__(TPB) k_kv8_comb(kv8_part p, float *out, uint32
 //  - of eight below head_dim 256 where a CU has more than 64 steps, which its
 //    vector units and not the cache's bytes bound then (32 of 128 on 8, 40 tokens
 //    at 8000 33.3 / 31.4, 20 at 32000 49.0 / 44.3, 262000 keys 96.0 / 95.3).
-// Else row blocks in tiles, one workgroup per CU at a time, their keys split
-// where that shortens the launch: rounds x (a part's tiles + KV8_TAIL for its
-// start and end) tiles of KV8_TILE_US, against the partials' way to memory and
-// back. KV8_SMALL, in waves' steps of 32 keys x head_dim, is where the two meet
+// Else row blocks in tiles, one workgroup per CU at a time (head_dim 64 has room
+// for two), their keys split where that shortens the launch: rounds x (a part's
+// tiles + KV8_TAIL for its start and end) tiles of KV8_TILE_US, against the
+// partials' way to memory and back. A tile's time is measured at head_dim 256 and
+// taken as proportional; at 128 and 64 it is 1.6-1.7 and 1.4 us, so that the rule
+// splits less there than it could. KV8_SMALL, in waves' steps of 32 keys x head_dim, is where the two meet
 // (wave / tile): 24 heads of 256 on 4, 8040 keys, 240 rows (3.9M) 39.4 / 45.2,
 // 1300 keys, 1800 rows (4.7M) 38.1 / 48.2, 8077 keys, 462 rows (7.5M) 53.8 /
 // 55.2, 32020 keys, 120 rows (8.2M) 55.7 / 54.0; 32 of 128 on 8, 8040 keys, 160
