@@ -518,9 +518,8 @@ __device__ __forceinline__ float rows_max(float m, float v) {
 
 // One group of UN tiles' scores to weights, online: updates the row's maximum and
 // sum, gives the weights' f16 halves in operand order and what the output so far
-// is to be multiplied by. x: the integer scores; f: what they are
-// to be multiplied by (scale, q's unit, the keys' scale), v: the values' scale,
-// per tile. Key `key` + 16 u + 4 lg + e is visible up to pos (groups are aligned,
+// is to be multiplied by. x: the integer scores; f: what they are to be multiplied
+// by (scale, q's unit, the keys' scale), v: the values' scale, per tile. Key `key` + 16 u + 4 lg + e is visible up to pos (groups are aligned,
 // so that the sum stays in 32 bits at the last position, too).
 // The usual group has all its keys visible, f >= 0, exponents within KV8_FAR and
 // the values' scales at least 2^-80, and looks only whether some exponent passes
@@ -793,7 +792,8 @@ __global__ void __launch_bounds__(NW * 64, 2) k_kv8_wave(sgk_kv8_attn a, kv8_par
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 // head_dim 64 stays within the 128 registers that let a second workgroup in (12 of
-// 64, 4096 tokens at 8192: 356 us, with one 439).
+// 64, 4096 tokens at 8192: 356 us, with one 439); a row's place, two registers,
+// lies in memory through the loops.
 template <int HD>
 __global__ void __launch_bounds__(KV8_NW * 64, HD == 64 ? 4 : 2) k_kv8_tile(sgk_kv8_attn a, kv8_part part, int al) {
     constexpr int NC = HD / 64, NT = HD / 16, NTH = KV8_NW * 64;
