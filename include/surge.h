@@ -324,8 +324,9 @@ sg_err sg_gpu_run_rmsnorm_gated_chunk(sg_gpu *g, void *y, void *z, void *out, vo
 
 /* ---------------------------------------------------------------------
  * Additions with no reference counterpart: an 8-bit K/V cache with the
- * attention that reads it, rotary positions with several axes, and the choice
- * of a token from processed logits. Manner as above: synchronous on the
+ * attention that reads it, rotary positions with several axes, the choice
+ * of a token from processed logits, a paged f16 cache of several sequences
+ * with its attention and eviction, and sampling. Manner as above: synchronous on the
  * library's stream (work that another stream has queued on a wrapped device
  * buffer must have finished), one caller per sg_gpu at a time, f32 unless
  * stated, buffers 4-byte aligned (codes 16-byte), shapes and sizes checked on
@@ -422,6 +423,76 @@ sg_err sg_gpu_run_token_counts(sg_gpu *g, void *ids, void *counts, const uint32_
  * p: [0]=vocab [1]=rows [2]=repetition bits [3]=frequency bits [4]=presence bits. */
 sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void *mask, void *out, void *token,
                          const uint32_t params[8]);
+
+/* Several sequences over a paged f16 K/V cache: continuations of one prompt, or
+ * conversations. kp, vp f16 pools [pages][page][n_kv][hd], 16-byte aligned; as many
+ * pages as the smaller buffer holds whole. table int32 [n_seq][width]: slot j of
+ * sequence s lies in page table[s][j / page] at row j % page. page = 16, 32, 64,
+ * 128 or 256, hd = 64, 128 or 256, n_kv and n_seq <= 65535, width * page <= 2^30. A
+ * cache [seq][n_kv][hd] of sg_gpu_run_attn_decode_f16 is such a pool, its table 0, 1,
+ * 2, ... A page number outside the pool is never followed: rows for its slots are
+ * dropped, attention passes them over. Entries of the table past a sequence's length
+ * do not count. Beside the pools a caller may keep two arrays [n_seq][n_kv][width *
+ * page], per slot: weight f32, what attention gave the row so far, and pos int32, the
+ * position of the row's token. Sequences may share pages that none of them writes.
+ *
+ * sg_gpu_run_page_store: rows f32 [n_seq][n] from k and v (row stride p[6] floats, 0
+ *   = n_kv hd; [n_kv][hd] in a row), n in [1, 2^27], rounded to f16 (nearest, ties
+ *   to even; inf past f16's range). span int32 [n_seq][3]: first slot, rows, position
+ *   of the first row. Row i < min(rows, n) goes to slot first + i and, where weight
+ *   and pos are given (either may be NULL), weight becomes 0 and pos position + i. A
+ *   negative first slot, or no rows, leaves a sequence out; slots from width * page on
+ *   are dropped. Two rows for one place of the pool: unspecified which of them stays.
+ *   p: [0]=n_kv [1]=hd [2]=page [3]=n_seq [4]=width [5]=n [6]=row stride.
+ * sg_gpu_run_attn_paged: attention of one token a sequence: q [n_seq][n_heads]
+ *   [q_stride], out [n_seq][n_heads][hd] over the slots [0, lens[s]) (lens int32
+ *   [n_seq], taken as 0 below 0 and as width * page above it); zeros where there is
+ *   none. n_heads a multiple of n_kv, at most 16 times it. Where weight_out is given,
+ *   weight_out[s][h][j] = weight[s][h][j] + the softmax weights that the query heads of
+ *   kv head h gave slot j, for j < lens[s] (weight NULL: + 0); the slots behind stay.
+ *   weight_out may be weight (as with the rotary axes' x and out). q, K and products
+ *   keep f32's precision. Elements that are not finite: of q or of a row of K, they make
+ *   the head's outputs and weights NaN, or give the row no weight where its score is
+ *   -inf; of V, they make their dim's outputs not finite. Reruns give the same bits.
+ *   p: [0]=n_heads [1]=n_kv [2]=hd [3]=page [4]=n_seq [5]=width [6]=q_stride
+ *   [7]=scale bits.
+ * sg_gpu_run_page_evict: of each sequence with lens[s] > keep, each kv head keeps
+ *   `keep` of its rows in slots [0, keep): first the recent ones (pos > largest pos of
+ *   the head's slots - recent), then those of the largest weight (NaN below every
+ *   number); alike, the lower slot. Kept rows below slot keep stay where they are; the
+ *   n-th kept row from slot keep on moves to the n-th freed slot, with its K, V,
+ *   weight and pos. weight_out and pos_out get the slots below min(keep, lens[s]), the
+ *   rest stays; they may be weight and pos (as above). Each sequence's length is
+ *   min(keep, lens[s]) then; the caller's lens stays as it is. A row is not moved out
+ *   of or into a page outside the pool (its weight and pos are). Pages that are written
+ *   must belong to one sequence. keep >= 1, recent <= keep.
+ *   p: [0]=n_kv [1]=hd [2]=page [3]=n_seq [4]=width [5]=keep [6]=recent. */
+sg_err sg_gpu_run_page_store(sg_gpu *g, void *k, void *v, void *kp, void *vp, void *table, void *span, void *weight, void *pos,
+                             const uint32_t params[8]);
+sg_err sg_gpu_run_attn_paged(sg_gpu *g, void *q, void *kp, void *vp, void *table, void *lens, void *weight, void *weight_out, void *out,
+                             const uint32_t params[8]);
+sg_err sg_gpu_run_page_evict(sg_gpu *g, void *kp, void *vp, void *table, void *lens, void *weight, void *pos, void *weight_out,
+                             void *pos_out, const uint32_t params[8]);
+
+/* Tokens from logits by given random numbers. settings [rows][4]: temperature f32,
+ * top_k u32, top_p f32, min_p f32. u f32 [rows], from [0, 1). Per row, with w =
+ * exp((x - largest x) / temperature) for the ids whose x is above -inf (NaN and -inf
+ * are never chosen; if the largest is +inf, those alone, alike):
+ *   temperature not above 0: the largest (as top_k 1);
+ *   top_k: the top_k ids of the largest x stay (0, or more than there are: all);
+ *   top_p < 1: of those, in falling order of x, an id stays if the w before it add up
+ *     to less than top_p times the w of all that top_k left; the first always does;
+ *   min_p > 0: of those, the ids with w >= min_p stay, and the largest;
+ *   ids of the same x: the lower id comes first.
+ * token u32 [rows]: the lowest id for which the w of the ids that stayed, up to and
+ * with it, add up to more than u times all of theirs; 0xFFFFFFFF if the row has none.
+ * u outside [0, 1) is taken as the nearest inside, NaN as 0. probs, if not NULL,
+ * f32 [rows][vocab]: w / sum of those that stayed, 0 for the others; it may be logits
+ * (as with the rotary axes). w and sums are held in 64 bits, sums as integers in units
+ * of less than the sum's 2^-60: no order of additions changes a result. vocab < 2^31,
+ * rows <= 65535.
+ * p: [0]=vocab [1]=rows. */
+sg_err sg_gpu_run_sample(sg_gpu *g, void *logits, void *settings, void *u, void *token, void *probs, const uint32_t params[8]);
 
 /* Decode (surge.h:1260-1274). */
 sg_err sg_gpu_load_model(sg_gpu *g, const sg_model *m);

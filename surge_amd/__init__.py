@@ -125,6 +125,10 @@ _SIGS = {
     "sg_gpu_run_rope_axes": (SgErr, [C.c_void_p] * 4 + [C.POINTER(C.c_uint32)]),
     "sg_gpu_run_token_counts": (SgErr, [C.c_void_p] * 3 + [C.POINTER(C.c_uint32)]),
     "sg_gpu_run_logits": (SgErr, [C.c_void_p] * 7 + [C.POINTER(C.c_uint32)]),
+    "sg_gpu_run_page_store": (SgErr, [C.c_void_p] * 9 + [C.POINTER(C.c_uint32)]),
+    "sg_gpu_run_attn_paged": (SgErr, [C.c_void_p] * 9 + [C.POINTER(C.c_uint32)]),
+    "sg_gpu_run_page_evict": (SgErr, [C.c_void_p] * 9 + [C.POINTER(C.c_uint32)]),
+    "sg_gpu_run_sample": (SgErr, [C.c_void_p] * 6 + [C.POINTER(C.c_uint32)]),
     "sg_gpu_splitk_online_dispatches": (C.c_uint64, [C.c_void_p]),
     "sg_gpu_splitk_online_selected": (C.c_bool, [C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32,
                                                  C.c_uint32]),
@@ -352,6 +356,25 @@ class Gpu:
         """counts, bias and mask may be None."""
         h = [b.handle if b is not None else None for b in (logits, counts, bias, mask, out, token)]
         check(lib().sg_gpu_run_logits(self.handle, *h, params(p)))
+
+    def page_store(self, k, v, kp, vp, table, span, weight, pos, p):
+        """weight and pos may be None."""
+        h = [b.handle if b is not None else None for b in (k, v, kp, vp, table, span, weight, pos)]
+        check(lib().sg_gpu_run_page_store(self.handle, *h, params(p)))
+
+    def attn_paged(self, q, kp, vp, table, lens, weight, weight_out, out, p):
+        """weight may be None (zeros), and with it weight_out (no weights)."""
+        h = [b.handle if b is not None else None for b in (q, kp, vp, table, lens, weight, weight_out, out)]
+        check(lib().sg_gpu_run_attn_paged(self.handle, *h, params(p)))
+
+    def page_evict(self, kp, vp, table, lens, weight, pos, weight_out, pos_out, p):
+        h = [b.handle for b in (kp, vp, table, lens, weight, pos, weight_out, pos_out)]
+        check(lib().sg_gpu_run_page_evict(self.handle, *h, params(p)))
+
+    def sample(self, logits, settings, u, token, probs, p):
+        """probs may be None."""
+        check(lib().sg_gpu_run_sample(self.handle, logits.handle, settings.handle, u.handle, token.handle,
+                                      probs.handle if probs is not None else None, params(p)))
 
     def dispatch_counts(self):
         """(per_head, gqa, online) partial dispatches encoded since sg_gpu_state_new."""

@@ -1131,6 +1131,169 @@ sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void
 }
 
 /* ---------------------------------------------------------------------
+ * Several sequences over a paged f16 cache, sampling (surge.h). No reference
+ * counterpart. On the handle's device, as above.
+ * --------------------------------------------------------------------- */
+
+/* The shape, the two pools (the smaller one's whole pages count) and the table. */
+static sg_err pages_check(const char *who, void *kp, void *vp, void *table, uint32_t n_kv, uint32_t hd, uint32_t page, uint32_t n_seq,
+                          uint32_t width, sgk_pages *c) {
+    if (!sgk_pages_shape_ok(n_kv, hd, page))
+        return errf("gpu: %s: n_kv in [1, 65535], head_dim 64, 128 or 256, page 16, 32, 64, 128 or 256", who);
+    if (!n_seq || n_seq > 65535) return errf("gpu: %s: n_seq must be in [1, 65535]", who);
+    if (!width || (uint64_t)width * page > 1u << 30) return errf("gpu: %s: a sequence has 1 to 2^30 slots (width * page)", who);
+    const uint64_t each = (uint64_t)page * n_kv * hd * 2;
+    sg_err e;
+    if (sg_failed(e = need(kp, each, "kp")) || sg_failed(e = need(vp, each, "vp")) ||
+        sg_failed(e = need(table, (uint64_t)n_seq * width * 4, "table"))) return e;
+    if (!aligned(kp, 16) || !aligned(vp, 16) || !aligned(table, 4)) return errf("gpu: %s: pools must be 16-byte, table 4-byte aligned", who);
+    if (overlap(kp, vp) || overlap(kp, table) || overlap(vp, table)) return errf("gpu: %s: pools and table must not overlap", who);
+    uint64_t n = size_of(kp) < size_of(vp) ? size_of(kp) : size_of(vp);
+    n /= each;
+    int log = 4;
+    while (1u << log < page) log++;
+    *c = (sgk_pages){DEV(kp), DEV(vp), DEV(table), n > INT32_MAX ? INT32_MAX : (uint32_t)n, (uint32_t)log, n_kv, hd, n_seq, width};
+    return SG_OK;
+}
+/* A per-slot buffer [n_seq][n_kv][width * page], 4 bytes each. */
+static sg_err slots_check(const char *who, void *buf, const char *what, const sgk_pages *c, void *const *others, int n) {
+    sg_err e = need(buf, (uint64_t)c->n_seq * c->n_kv * c->width * 4 << c->log, what);
+    if (sg_failed(e)) return e;
+    if (!aligned(buf, 4)) return errf("gpu: %s: %s must be 4-byte aligned", who, what);
+    for (int i = 0; i < n; i++)
+        if (overlap(buf, others[i])) return errf("gpu: %s: %s overlaps another buffer", who, what);
+    return SG_OK;
+}
+/* Uploads for an output of which a call writes some slots: what counts before
+ * the call is in the input where the two are one memory, else its own. */
+static sg_err push_pair(void *in, void *out) {
+    sg_err e = SG_OK;
+    if (in && sg_failed(e = sg_gpu_buf_upload(in))) return e;
+    if (!in || DEV(in) != DEV(out)) return sg_gpu_buf_upload(out);
+    return in == out ? e : push_out(out, size_of(in));
+}
+
+sg_err sg_gpu_run_page_store(sg_gpu *g, void *k, void *v, void *kp, void *vp, void *table, void *span, void *weight, void *pos,
+                             const uint32_t p[8]) {
+    if (!g || !k || !v || !kp || !vp || !table || !span || !p) return (sg_err){"gpu: page_store got a NULL argument"};
+    const uint32_t n = p[5];
+    sgk_page_store_args a = {.k = DEV(k), .v = DEV(v), .span = DEV(span), .weight = DEV(weight), .pos = DEV(pos), .n = n};
+    sg_err e = pages_check("page_store", kp, vp, table, p[0], p[1], p[2], p[3], p[4], &a.c);
+    if (sg_failed(e)) return e;
+    if (!n || n > 1u << 27) return (sg_err){"gpu: page_store: n must be in [1, 2^27]"};
+    const uint64_t w = (uint64_t)p[0] * p[1];
+    a.stride = p[6] ? p[6] : w;
+    if (a.stride < w) return (sg_err){"gpu: page_store: row stride below n_kv * head_dim"};
+    const uint64_t rows = (uint64_t)p[3] * n;
+    if (rows > (1ull << 60) / a.stride) return (sg_err){"gpu: page_store: strides are too large"};      /* the sizes below stay in 64 bits */
+    const uint64_t bytes = ((rows - 1) * a.stride + w) * 4;
+    if (sg_failed(e = need(k, bytes, "k")) || sg_failed(e = need(v, bytes, "v")) ||
+        sg_failed(e = need(span, (uint64_t)p[3] * 12, "span"))) return e;
+    if (!aligned(k, 4) || !aligned(v, 4) || !aligned(span, 4)) return (sg_err){"gpu: page_store: rows and span must be 4-byte aligned"};
+    void *bufs[8] = {k, v, table, span, kp, vp, weight, pos};
+    if (overlap(kp, k) || overlap(kp, v) || overlap(kp, span) || overlap(vp, k) || overlap(vp, v) || overlap(vp, span))
+        return (sg_err){"gpu: page_store: the cache must not overlap the rows"};
+    if ((weight && sg_failed(e = slots_check("page_store", weight, "weight", &a.c, bufs, 6))) ||
+        (pos && sg_failed(e = slots_check("page_store", pos, "pos", &a.c, bufs, 7)))) return e;
+    int was;
+    if (sg_failed(e = on_device(g, &was))) return e;
+    if (!sg_failed(e = push(bufs, 8))) e = finish_done(g, sgk_page_store(&a, g->stream, g->done), bufs + 4, 4);
+    return back_to(g, was, e);
+}
+
+sg_err sg_gpu_run_attn_paged(sg_gpu *g, void *q, void *kp, void *vp, void *table, void *lens, void *weight, void *weight_out, void *out,
+                             const uint32_t p[8]) {
+    if (!g || !q || !kp || !vp || !table || !lens || !out || !p) return (sg_err){"gpu: attn_paged got a NULL argument"};
+    if (weight && !weight_out) return (sg_err){"gpu: attn_paged: weight without weight_out"};
+    const uint32_t nh = p[0], nkv = p[1], hd = p[2], n = p[4];
+    sgk_attn_paged_args a = {.q = DEV(q), .lens = DEV(lens), .weight = DEV(weight), .weight_out = DEV(weight_out), .out = DEV(out),
+                             .q_stride = p[6], .n_heads = nh, .scale = fbits(p[7])};
+    sg_err e = pages_check("attn_paged", kp, vp, table, nkv, hd, p[3], n, p[5], &a.c);
+    if (sg_failed(e)) return e;
+    if (!nh || nh % nkv || nh / nkv > SGK_PAGES_MAX_GROUP)
+        return errf("gpu: attn_paged: n_heads must be a multiple of n_kv_heads, at most %u times it", SGK_PAGES_MAX_GROUP);
+    if (p[6] < hd) return (sg_err){"gpu: attn_paged: q_stride < head_dim"};
+    const uint64_t rows = (uint64_t)n * nh;
+    if (sg_failed(e = need(q, ((rows - 1) * p[6] + hd) * 4, "q")) || sg_failed(e = need(out, rows * hd * 4, "out")) ||
+        sg_failed(e = need(lens, (uint64_t)n * 4, "lens"))) return e;
+    if (!aligned(q, 4) || !aligned(out, 4) || !aligned(lens, 4)) return (sg_err){"gpu: attn_paged: q, lens and out must be 4-byte aligned"};
+    void *ins[7] = {q, kp, vp, table, lens, out, weight}, *outs[3] = {out, weight_out, NULL};
+    for (int i = 0; i < 5; i++)
+        if (overlap(out, ins[i])) return (sg_err){"gpu: attn_paged: out overlaps an input"};
+    if ((weight_out && sg_failed(e = slots_check("attn_paged", weight_out, "weight_out", &a.c, ins, 6))) ||
+        (weight && sg_failed(e = slots_check("attn_paged", weight, "weight", &a.c, ins + 5, 1)))) return e;
+    if (weight && overlap(weight, weight_out)) {
+        if (DEV(weight) != DEV(weight_out)) return (sg_err){"gpu: attn_paged: weight_out overlaps weight"};
+        outs[2] = alias_of(weight_out, weight);
+    }
+    int was;
+    if (sg_failed(e = on_device(g, &was))) return e;
+    if (!sg_failed(e = push(ins, 5)) && !sg_failed(e = push_out(out, rows * hd * 4)) &&
+        (!weight_out || !sg_failed(e = push_pair(weight, weight_out)))) {
+        void *t = NULL;
+        if (!sg_failed(e = scratch(g, sgk_attn_paged_scratch(&a), &t))) e = finish_done(g, sgk_attn_paged(&a, t, g->stream, g->done), outs, 3);
+    }
+    return back_to(g, was, e);
+}
+
+sg_err sg_gpu_run_page_evict(sg_gpu *g, void *kp, void *vp, void *table, void *lens, void *weight, void *pos, void *weight_out,
+                             void *pos_out, const uint32_t p[8]) {
+    if (!g || !kp || !vp || !table || !lens || !weight || !pos || !weight_out || !pos_out || !p)
+        return (sg_err){"gpu: page_evict got a NULL argument"};
+    sgk_page_evict_args a = {.lens = DEV(lens), .weight = DEV(weight), .pos = DEV(pos), .weight_out = DEV(weight_out),
+                             .pos_out = DEV(pos_out), .keep = p[5], .recent = p[6]};
+    sg_err e = pages_check("page_evict", kp, vp, table, p[0], p[1], p[2], p[3], p[4], &a.c);
+    if (sg_failed(e)) return e;
+    if (!a.keep || a.recent > a.keep) return (sg_err){"gpu: page_evict: keep must be at least 1, recent at most keep"};
+    if (sg_failed(e = need(lens, (uint64_t)p[3] * 4, "lens"))) return e;
+    if (!aligned(lens, 4)) return (sg_err){"gpu: page_evict: lens must be 4-byte aligned"};
+    if (overlap(kp, lens) || overlap(vp, lens)) return (sg_err){"gpu: page_evict: lens overlaps a pool"};
+    void *ins[6] = {kp, vp, table, lens, weight, pos};
+    if (sg_failed(e = slots_check("page_evict", weight, "weight", &a.c, ins, 2)) ||
+        sg_failed(e = slots_check("page_evict", pos, "pos", &a.c, ins, 2)) ||
+        sg_failed(e = slots_check("page_evict", weight_out, "weight_out", &a.c, ins, 4)) ||
+        sg_failed(e = slots_check("page_evict", pos_out, "pos_out", &a.c, ins, 4))) return e;
+    if (overlap(weight_out, pos) || overlap(weight_out, pos_out) || overlap(pos_out, weight) ||
+        (overlap(weight_out, weight) && DEV(weight_out) != DEV(weight)) || (overlap(pos_out, pos) && DEV(pos_out) != DEV(pos)))
+        return (sg_err){"gpu: page_evict: an output overlaps another buffer"};
+    int was;
+    if (sg_failed(e = on_device(g, &was))) return e;
+    if (a.keep > (uint64_t)a.c.width << a.c.log) a.keep = a.c.width << a.c.log;       /* no more slots than that */
+    void *outs[6] = {kp, vp, weight_out, pos_out, alias_of(weight_out, weight), alias_of(pos_out, pos)}, *t = NULL;
+    if (!sg_failed(e = push(ins, 4)) && !sg_failed(e = push_pair(weight, weight_out)) && !sg_failed(e = push_pair(pos, pos_out)) &&
+        !sg_failed(e = scratch(g, sgk_page_evict_scratch(&a), &t)))
+        e = finish_done(g, sgk_page_evict(&a, t, g->stream, g->done), outs, 6);
+    return back_to(g, was, e);
+}
+
+sg_err sg_gpu_run_sample(sg_gpu *g, void *logits, void *settings, void *u, void *token, void *probs, const uint32_t p[8]) {
+    if (!g || !logits || !settings || !u || !token || !p) return (sg_err){"gpu: sample got a NULL argument"};
+    const uint32_t vocab = p[0], rows = p[1];
+    if (!vocab || vocab > INT32_MAX || !rows || rows > 65535)
+        return (sg_err){"gpu: sample: bad shape (vocab in [1, 2^31), rows in [1, 65535])"};
+    const uint64_t lb = (uint64_t)vocab * rows * 4;
+    sg_err e;
+    if (sg_failed(e = need(logits, lb, "logits")) || sg_failed(e = need(settings, (uint64_t)rows * 16, "settings")) ||
+        sg_failed(e = need(u, (uint64_t)rows * 4, "u")) || sg_failed(e = need(token, (uint64_t)rows * 4, "token")) ||
+        (probs && sg_failed(e = need(probs, lb, "probs")))) return e;
+    void *bufs[5] = {logits, settings, u, token, probs}, *outs[3] = {token, probs, NULL};
+    for (int i = 0; i < 5; i++)
+        if (bufs[i] && !aligned(bufs[i], 4)) return (sg_err){"gpu: sample: buffers must be 4-byte aligned"};
+    for (int i = 0; i < 4; i++)
+        if ((i < 3 && overlap(token, bufs[i])) || (probs && overlap(probs, bufs[i]) && !(i == 0 && DEV(probs) == DEV(logits))))
+            return (sg_err){"gpu: sample: an output overlaps another buffer"};
+    if (probs) outs[2] = alias_of(probs, logits);
+    int was;
+    if (sg_failed(e = on_device(g, &was))) return e;
+    if (!sg_failed(e = push(bufs, 3)) && !sg_failed(e = push_out(token, (uint64_t)rows * 4)) &&
+        (!probs || probs == logits || !sg_failed(e = push_out(probs, outs[2] ? size_of(logits) : lb)))) {
+        const sgk_sample_args a = {DEV(logits), DEV(settings), DEV(u), DEV(token), DEV(probs), vocab, rows};
+        e = finish_done(g, sgk_sample(&a, g->stream, g->done), outs, 3);
+    }
+    return back_to(g, was, e);
+}
+
+/* ---------------------------------------------------------------------
  * prefill per-op hooks (surge.h:787-800, 1133-1142): the chunk kernels the
  * prefill path runs, one synchronous call each, with the reference's
  * argument layouts and params.

@@ -432,6 +432,64 @@ typedef struct {
 uint64_t sgk_logits_part_bytes(uint32_t vocab, uint32_t rows);
 hipError_t sgk_logits(const sgk_logits_args *a, void *part, hipStream_t s, hipEvent_t done);
 
+/* Several sequences over a paged f16 K/V cache (pages.hip): pools [pages][page]
+ * [n_kv][hd], table [n_seq][width]; see surge.h. */
+typedef struct {
+    uint16_t *k, *v;
+    const int32_t *table;
+    uint32_t pages, log, n_kv, hd, n_seq, width;        /* a page is 2^log slots */
+} sgk_pages;
+SGK_HD static inline int sgk_pages_shape_ok(uint32_t n_kv, uint32_t hd, uint32_t page) {
+    return n_kv && n_kv <= 65535 && (hd == 64 || hd == 128 || hd == 256) && page >= 16 && page <= 256 && !(page & (page - 1));
+}
+typedef struct {
+    sgk_pages c;
+    const float *k, *v;         /* [n_seq][n] rows at stride */
+    const int32_t *span;        /* [n_seq][3]: first slot, rows, position of the first */
+    float *weight;              /* or NULL */
+    int32_t *pos;               /* or NULL */
+    uint64_t stride;
+    uint32_t n;
+} sgk_page_store_args;
+hipError_t sgk_page_store(const sgk_page_store_args *a, hipStream_t s, hipEvent_t done);
+#define SGK_PAGES_MAX_GROUP 16u     /* query heads per kv head */
+typedef struct {
+    sgk_pages c;
+    const float *q;
+    const int32_t *lens;
+    const float *weight;        /* or NULL: zeros */
+    float *weight_out;          /* or NULL */
+    float *out;
+    uint64_t q_stride;
+    uint32_t n_heads;
+    float scale;
+} sgk_attn_paged_args;
+/* scratch: sgk_attn_paged_scratch(a) bytes, 16-byte aligned. */
+uint64_t sgk_attn_paged_scratch(const sgk_attn_paged_args *a);
+hipError_t sgk_attn_paged(const sgk_attn_paged_args *a, void *scratch, hipStream_t s, hipEvent_t done);
+typedef struct {
+    sgk_pages c;
+    const int32_t *lens;
+    const float *weight;
+    const int32_t *pos;
+    float *weight_out;
+    int32_t *pos_out;
+    uint32_t keep, recent;
+} sgk_page_evict_args;
+uint64_t sgk_page_evict_scratch(const sgk_page_evict_args *a);
+hipError_t sgk_page_evict(const sgk_page_evict_args *a, void *scratch, hipStream_t s, hipEvent_t done);
+
+/* Tokens from logits and given random numbers (sample.hip). */
+typedef struct {
+    const float *x;
+    const uint32_t *settings;   /* [rows][4]: temperature, top_k, top_p, min_p */
+    const float *u;
+    uint32_t *token;
+    float *probs;               /* or NULL */
+    uint32_t vocab, rows;
+} sgk_sample_args;
+hipError_t sgk_sample(const sgk_sample_args *a, hipStream_t s, hipEvent_t done);
+
 /* The device-resident workspace of the no-allocation entry points: a
  * file-scope device array of SGK_SCRATCH_BYTES in kernels.hip. Call
  * sgk_scratch_init(dev) once per device with that device current; then
