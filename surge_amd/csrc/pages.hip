@@ -10,15 +10,24 @@
 #include "devutil.h"
 #include "kernels.h"
 
+// What no kernel writes while it reads it, at addresses that a wave's lanes share: by scalar loads, which are
+// not counted with the rows'.
+typedef __attribute__((address_space(4))) int32_t scalar_i32;
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
+// An address that a wave's lanes share, as the scalar base of its loads.
+__device__ __forceinline__ const char *uniform(const char *p) {
+    const uint64_t a = (uint64_t)(uintptr_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+    return (const char *)(const __attribute__((address_space(1))) char *)(uintptr_t)((uint64_t)hi << 32 | lo);
+}
 // The row of the pool that slot j of sequence s lies in, or -1.
 __device__ __forceinline__ int64_t page_row(const sgk_pages &c, uint32_t s, uint32_t j) {
     const uint32_t p = (uint32_t)c.table[(uint64_t)s * c.width + (j >> c.log)];
     return p < c.pages ? (int64_t)(((uint64_t)p << c.log) + (j & ((1u << c.log) - 1))) : -1;
 }
 __device__ __forceinline__ uint32_t page_len(const sgk_pages &c, const int32_t *lens, uint32_t s) {
-    return min((uint32_t)max(lens[s], 0), c.width << c.log);
+    return min((uint32_t)max(((const scalar_i32 *)(uintptr_t)lens)[s], 0), c.width << c.log);
 }
 
 // ---------------------------------------------------------------------------
@@ -64,80 +73,326 @@ extern "C" hipError_t sgk_page_store(const sgk_page_store_args *a, hipStream_t s
 }
 
 // ---------------------------------------------------------------------------
-// Attention. A workgroup takes AP_SLOTS slots of one sequence and kv head: the
-// scores of a slot by a thread, the weighted values of a dim by a thread. Each
-// part leaves its maximum, its sum and its weighted values, and the scores where
-// the weights are wanted; the join brings the parts together.
+// Attention. Parts of the sequences, a workgroup each per kv head; in a part the
+// waves take steps of 32 slots in turn, K and V straight from the pages into the
+// matrix instructions' operands, with a running maximum and sum per wave. Their
+// results are added in LDS, those of a sequence's parts by a second launch.
+//
+// Scores^T = K q^T, 16 slots x 16 heads a product: lane (r, g) = (l % 16, l / 16)
+// loads slot r, dims 32 j + 8 g ..+7, and gets the scores of head r at slots
+// 4 g ..+3. Two such tiles make the 32 slots of out^T = V^T p^T, whose k index
+// 8 g + e stands for slot 4 g + e of the first tile (e < 4) or the second: a lane
+// has its own scores as operand. Of V it loads those eight rows, 8 dims each
+// (dims 8 r ..+7 of 128; 4 at head_dim 64), and dim 8 r + j of them is row r of
+// the j-th product, one byte permutation per two values.
+//
+// q is split into three f16 that add up to its f32 (relative to its head's
+// largest element), p into two (2^-22), so that products are exact or nearly so
+// and sums are f32.
+//
+// Parts: T steps in all and room for `most` parts a head give parts of
+// ceil(T / most) steps, at least AP_MIN, the same on every workgroup; a sequence
+// of n steps has ceil(n / per) of them, so there are at most most + n_seq.
 // ---------------------------------------------------------------------------
-#define AP_SLOTS 256u
-struct ap_part { float *m, *l, *acc, *score; uint32_t parts; };     // [seq][head][part], acc x hd; score [seq][head][cap]
+#define AP_STEP 32u
+#define AP_MIN 4u
+#define AP_WAVES 4
+#define AP_P2 14            // p is held times 2^14, so that f16's subnormals start at 2^-28
 
-__global__ void __launch_bounds__(TPB) k_attn_paged(sgk_attn_paged_args a, ap_part w) {
-    __shared__ float qs[16][256], ps[16][AP_SLOTS], red[16][2];
-    const uint32_t t = threadIdx.x, part = blockIdx.x, h = blockIdx.y, s = blockIdx.z, hd = a.c.hd, g = a.n_heads / a.c.n_kv;
-    const uint32_t len = page_len(a.c, a.lens, s), j = part * AP_SLOTS + t;
-    const uint64_t cap = (uint64_t)a.c.width << a.c.log, wide = (uint64_t)a.c.n_kv * hd;
-    if (part * AP_SLOTS >= len) return;
-    for (uint32_t i = t; i < g * hd; i += TPB) qs[i / hd][i % hd] = a.q[((uint64_t)s * a.n_heads + h * g + i / hd) * a.q_stride + i % hd];
-    __shared__ int64_t rowat[AP_SLOTS];
-    const int64_t row = j < len ? page_row(a.c, s, j) : -1;
-    rowat[t] = row;
+struct ap_part {
+    float *m, *l, *acc;     // [part][head], acc x hd
+    float *score;           // [seq][head][cap], or NULL
+    float *ml;              // [seq][head][2]: maximum and sum, for the weights
+    uint32_t *plan;         // [n_seq + 1] first parts, then [parts] sequences; NULL up to 64 sequences
+    uint32_t most, parts;
+};
+
+__device__ __forceinline__ uint32_t ap_steps(const sgk_attn_paged_args &a, uint32_t s) { return (page_len(a.c, a.lens, s) + AP_STEP - 1) / AP_STEP; }
+__device__ __forceinline__ uint32_t ap_per(uint64_t total, uint32_t most) { return max(AP_MIN, (uint32_t)((total + most - 1) / most)); }
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {        // inclusive
+    const uint32_t l = threadIdx.x & 63;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint32_t y = __shfl_up(v, d);
+        if (l >= d) v += y;
+    }
+    return v;
+}
+struct ap_where { uint32_t s, first, n, per; };      // sequence (n_seq: none), its first part and their number
+// Of part x (by_part) or of sequence x.
+__device__ __forceinline__ ap_where ap_find(const sgk_attn_paged_args &a, const ap_part &w, uint32_t x, bool by_part) {
+    const uint32_t ns = a.c.n_seq;
+    if (w.plan) {
+        const uint32_t all = w.plan[ns], s = !by_part ? x : x < all ? w.plan[ns + 2 + x] : ns;
+        if (s >= ns) return (ap_where){ns, 0, 0, 0};
+        return (ap_where){s, w.plan[s], w.plan[s + 1] - w.plan[s], w.plan[ns + 1]};
+    }
+    const uint32_t l = threadIdx.x & 63, st = l < ns ? ap_steps(a, l) : 0;
+    const uint32_t per = ap_per((uint32_t)__builtin_amdgcn_readlane((int)wave_scan(st), 63), w.most);     // 64 x 2^25 steps at most
+    const uint32_t n = (st + per - 1) / per, to = wave_scan(n);
+    const uint32_t s = by_part ? (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(to <= x)) : x;
+    if (s >= ns) return (ap_where){ns, 0, 0, 0};
+    const uint32_t e = (uint32_t)__builtin_amdgcn_readlane((int)to, (int)s), c = (uint32_t)__builtin_amdgcn_readlane((int)n, (int)s);
+    return (ap_where){s, e - c, c, per};
+}
+// The plan of more than 64 sequences: [n_seq] all parts, [n_seq + 1] steps a part.
+__global__ void __launch_bounds__(1024) k_attn_paged_plan(sgk_attn_paged_args a, ap_part w) {
+    __shared__ uint64_t tot[16];
+    __shared__ uint32_t sub[16];
+    const uint32_t t = threadIdx.x, ns = a.c.n_seq;
+    uint64_t sum = 0;
+    for (uint32_t s = t; s < ns; s += 1024) sum += ap_steps(a, s);
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+    if ((t & 63) == 0) tot[t >> 6] = sum;
     __syncthreads();
-    float sc[16];
-    for (uint32_t c = 0; c < 16; c++) sc[c] = 0.0f;
-    if (row >= 0) {
-        const _Float16 *k = (const _Float16 *)a.c.k + (uint64_t)row * wide + h * hd;
-        for (uint32_t d = 0; d < hd; d++) {
-            const float x = (float)k[d];
-            for (uint32_t c = 0; c < 16; c++) if (c < g) sc[c] = fmaf(x, qs[c][d], sc[c]);
+    sum = 0;
+    for (int i = 0; i < 16; i++) sum += tot[i];
+    const uint32_t per = ap_per(sum, w.most);
+    uint32_t at = 0;
+    for (uint32_t s0 = 0; s0 < ns; s0 += 1024) {
+        const uint32_t s = s0 + t, n = s < ns ? (ap_steps(a, s) + per - 1) / per : 0, to = wave_scan(n);
+        __syncthreads();
+        if ((t & 63) == 63) sub[t >> 6] = to;
+        __syncthreads();
+        uint32_t first = at + to - n;
+        for (uint32_t i = 0; i < 16; i++) {
+            if (i < t >> 6) first += sub[i];
+            at += sub[i];
+        }
+        if (s < ns) {
+            w.plan[s] = first;
+            for (uint32_t i = 0; i < n; i++) w.plan[ns + 2 + first + i] = s;
         }
     }
-    for (uint32_t c = 0; c < 16; c++)
-        if (c < g) {
-            const float x = row >= 0 ? sc[c] * a.scale : -INFINITY;
-            ps[c][t] = x;
-            if (w.score && j < len) w.score[((uint64_t)s * a.n_heads + h * g + c) * cap + j] = x;
+    if (t == 0) { w.plan[ns] = at; w.plan[ns + 1] = per; }
+}
+
+__device__ __forceinline__ f16x2 pair_of(uint32_t b, uint32_t a, bool high) {      // the low or the high halves of two dwords
+    union { uint32_t u; f16x2 h; } r;
+    r.u = __builtin_amdgcn_perm(b, a, high ? 0x07060302u : 0x05040100u);
+    return r.h;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(AP_WAVES * 64, 2) k_attn_paged(sgk_attn_paged_args a, ap_part w, int al) {
+    constexpr int NJ = HD / 32, NT = HD / 16, VD = HD == 64 ? 4 : 8, NC = HD / (16 * VD);      // VD dims a lane and chunk of V
+    typedef uint32_t vrow __attribute__((ext_vector_type(VD / 2)));
+    extern __shared__ __align__(16) char lds[];
+    f16x8 (*qs)[NJ][64] = (f16x8 (*)[NJ][64])lds;
+    const uint32_t t = threadIdx.x, l = t & 63, r = l & 15, g = l >> 4, wv = __builtin_amdgcn_readfirstlane(t >> 6);
+    const uint32_t h = blockIdx.y, grp = a.n_heads / a.c.n_kv;
+    const ap_where me = ap_find(a, w, blockIdx.x, true);
+    if (me.s >= a.c.n_seq) return;
+    const uint32_t s = me.s, len = page_len(a.c, a.lens, s), all = (len + AP_STEP - 1) / AP_STEP;
+    const uint32_t st0 = (blockIdx.x - me.first) * me.per, st1 = min(st0 + me.per, all);
+    const uint64_t wide = (uint64_t)a.c.n_kv * HD, cap = (uint64_t)a.c.width << a.c.log;
+    const scalar_i32 *table = (const scalar_i32 *)(uintptr_t)(a.c.table + (uint64_t)s * a.c.width);
+
+    // q of head r, dims 32 j + 8 g ..+7, as three f16: wave w has the j that are w mod the waves
+    float f1;
+    {
+        constexpr int NQ = (NJ + AP_WAVES - 1) / AP_WAVES;
+        float x[NQ][8], am = 0.0f;
+        const float *q = a.q + ((uint64_t)s * a.n_heads + h * grp + min(r, grp - 1)) * a.q_stride + 8 * g;
+        if (al) {
+#pragma unroll
+            for (int i = 0; i < NQ; i++)
+#pragma unroll
+                for (int z = 0; z < 2; z++) {
+                    const f32x4 y = *(const f32x4 *)(q + 32 * ((wv + AP_WAVES * i) % NJ) + 4 * z);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[i][4 * z + e] = y[e];
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NQ; i++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[i][e] = q[32 * ((wv + AP_WAVES * i) % NJ) + e];
         }
-    __syncthreads();
-    if (t < g) {
-        float m = -INFINITY, l = 0.0f;
-        for (uint32_t i = 0; i < AP_SLOTS; i++) m = ps[t][i] > m || ps[t][i] != ps[t][i] ? ps[t][i] : m;
-        for (uint32_t i = 0; i < AP_SLOTS; i++) {
-            const float p = rowat[i] >= 0 ? expf(ps[t][i] - m) : 0.0f;
-            ps[t][i] = p;
-            l += p;
+#pragma unroll
+        for (int i = 0; i < NQ; i++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) am = fmaxf(am, fabsf(x[i][e]));
+        am = fmaxf(am, swap16f(am));
+        am = fmaxf(am, swap32f(am));
+        float *red = (float *)lds;
+        if (g == 0) red[wv * 16 + r] = am;
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < AP_WAVES; v++) am = fmaxf(am, red[v * 16 + r]);
+        __syncthreads();
+        const int ex = am > 0.0f && am < INFINITY ? __builtin_amdgcn_frexp_expf(am) : 0;
+        f1 = __builtin_amdgcn_ldexpf(a.scale, ex - 15);
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            const uint32_t j = wv + AP_WAVES * i;
+            if (j >= NJ) break;
+            f16x8 p[3];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                float y = __builtin_amdgcn_ldexpf(x[i][e], 15 - ex);
+#pragma unroll
+                for (int z = 0; z < 3; z++) {
+                    p[z][e] = (_Float16)y;
+                    y -= (float)p[z][e];
+                }
+            }
+#pragma unroll
+            for (int z = 0; z < 3; z++) qs[z][j][l] = p[z];
         }
-        const uint64_t at = ((uint64_t)s * a.n_heads + h * g + t) * w.parts + part;
-        w.m[at] = m;
-        w.l[at] = l;
     }
     __syncthreads();
-    if (t < hd) {
-        float o[16];
-        for (uint32_t c = 0; c < 16; c++) o[c] = 0.0f;
-        for (uint32_t i = 0; i < AP_SLOTS; i++) {
-            if (rowat[i] < 0) continue;
-            const float v = (float)((const _Float16 *)a.c.v)[(uint64_t)rowat[i] * wide + h * hd + t];
-            for (uint32_t c = 0; c < 16; c++) if (c < g) o[c] = fmaf(ps[c][i], v, o[c]);
+
+    float m = -INFINITY, sum = 0.0f;
+    f32x4 o[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++) o[i] = (f32x4){0, 0, 0, 0};
+    // a half step's rows: whether they are there, and where in the pools (uniform); slots behind the last: its page
+    struct half_at { bool ok; uint64_t off; };
+    auto at = [&](uint32_t j) -> half_at {
+        const uint32_t p = (uint32_t)table[min(j, len - 1) >> a.c.log];
+        const bool ok = p < a.c.pages;
+        return (half_at){ok && j < len, ((((uint64_t)(ok ? p : 0) << a.c.log) + (j & ((1u << a.c.log) - 1))) * wide + h * HD) * 2};
+    };
+    f16x8 kf[2][NJ];
+    const uint32_t koff = (r * (uint32_t)wide + 8 * g) * 2;
+    uint32_t voff[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) voff[e] = ((4 * g + e) * (uint32_t)wide + VD * r) * 2;
+    auto load_k = [&](const half_at (&p)[2]) {
+#pragma unroll
+        for (int z = 0; z < 2; z++)
+#pragma unroll
+            for (int j = 0; j < NJ; j++) kf[z][j] = *(const f16x8 *)(uniform((const char *)a.c.k + p[z].off) + koff + 64 * j);
+    };
+    half_at now[2] = {at((st0 + wv) * AP_STEP), at((st0 + wv) * AP_STEP + 16)};
+    if (st0 + wv < st1) load_k(now);
+    for (uint32_t st = st0 + wv; st < st1; st += AP_WAVES) {
+        const uint32_t j0 = st * AP_STEP;
+        vrow vf[NC][8];
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+#pragma unroll
+            for (int c = 0; c < NC; c++) vf[c][e] = *(const vrow *)(uniform((const char *)a.c.v + now[e / 4].off) + voff[e % 4] + 32 * VD * c);
+        const half_at next[2] = {at(j0 + AP_WAVES * AP_STEP), at(j0 + AP_WAVES * AP_STEP + 16)};
+        asm volatile("" ::: "memory");      // q's parts are read again every step, not kept in registers
+        float x[8];
+        f32x4 d[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+        for (int y = 2; y >= 0; y--)
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                const f16x8 qf = qs[y][j][l];
+#pragma unroll
+                for (int z = 0; z < 2; z++) d[z] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[z][j], qf, d[z], 0, 0, 0);
+            }
+#pragma unroll
+        for (int z = 0; z < 2; z++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[4 * z + e] = now[z].ok && j0 + 16 * z + 4 * g + e < len ? d[z][e] * f1 : -INFINITY;
+        __builtin_amdgcn_sched_barrier(0);
+        if (st + AP_WAVES < st1) load_k(next);
+        __builtin_amdgcn_sched_barrier(0);
+        if (w.score && r < grp) {
+            float *sc = w.score + ((uint64_t)s * a.n_heads + h * grp + r) * cap + j0 + 4 * g;
+#pragma unroll
+            for (int z = 0; z < 2; z++)
+                if (j0 + 16 * z < cap) *(f32x4 *)(sc + 16 * z) = (f32x4){x[4 * z], x[4 * z + 1], x[4 * z + 2], x[4 * z + 3]};
         }
-        for (uint32_t c = 0; c < 16; c++)
-            if (c < g) w.acc[(((uint64_t)s * a.n_heads + h * g + c) * w.parts + part) * hd + t] = o[c];
+        float tm = x[0];
+#pragma unroll
+        for (int e = 1; e < 8; e++) tm = fmaxf(tm, x[e]);
+        tm = fmaxf(tm, swap16f(tm));
+        tm = fmaxf(tm, swap32f(tm));
+        if (__builtin_amdgcn_ballot_w64(tm > m)) {
+            const float mn = fmaxf(m, tm), f = m > -INFINITY ? exp2f((m - mn) * 1.44269504f) : 0.0f;
+            sum *= f;
+#pragma unroll
+            for (int i = 0; i < NT; i++) o[i] *= f;
+            m = mn;
+        }
+        const float mm = m > -INFINITY ? m : 0.0f;
+        f16x8 ph, pl;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float p = exp2f((x[e] - mm) * 1.44269504f) * (float)(1 << AP_P2);
+            sum += p;
+            ph[e] = (_Float16)p;
+            pl[e] = (_Float16)(p - (float)ph[e]);
+        }
+        if (!now[0].ok || !now[1].ok || j0 + AP_STEP > len) {       // rows that are not there may hold anything
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+                    if (!now[e / 4].ok || j0 + 16 * (e / 4) + 4 * g + e % 4 >= len) vf[c][e] = (vrow)0;
+        }
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int j = 0; j < VD; j++) {
+                union { f16x2 p[4]; f16x8 v; } u;
+#pragma unroll
+                for (int e = 0; e < 4; e++) u.p[e] = pair_of(vf[c][2 * e + 1][j / 2], vf[c][2 * e][j / 2], j & 1);
+                f32x4 &d = o[c * VD + j];
+                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(u.v, pl, d, 0, 0, 0);
+                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(u.v, ph, d, 0, 0, 0);
+            }
+        now[0] = next[0];
+        now[1] = next[1];
+    }
+    sum += swap16f(sum);
+    sum += swap32f(sum);
+
+    // the waves' results, added: o[c VD + j][i] of lane (r, g) is head r, dim 16 VD c + VD (4 g + i) + j
+    __syncthreads();
+    float *wm = (float *)lds, *wl = wm + AP_WAVES * 16, *wo = wl + AP_WAVES * 16;       // [wave][16], [wave][16], [wave][grp][HD]
+    if (g == 0) { wm[wv * 16 + r] = m; wl[wv * 16 + r] = sum; }
+    if (r < grp) {
+        float *d = wo + ((uint64_t)wv * grp + r) * HD + 4 * g * VD;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < VD; j += 4)
+                    *(f32x4 *)(d + 16 * VD * c + VD * i + j) = (f32x4){o[c * VD + j][i], o[c * VD + j + 1][i], o[c * VD + j + 2][i], o[c * VD + j + 3][i]};
+    }
+    __syncthreads();
+    for (uint32_t i = t; i < grp * HD; i += AP_WAVES * 64) {
+        const uint32_t c = i / HD;
+        float mx = -INFINITY, lx = 0.0f, ox = 0.0f;
+#pragma unroll
+        for (int v = 0; v < AP_WAVES; v++) mx = fmaxf(mx, wm[v * 16 + c]);
+#pragma unroll
+        for (int v = 0; v < AP_WAVES; v++) {
+            const float mv = wm[v * 16 + c], f = mv > -INFINITY ? exp2f((mv - mx) * 1.44269504f) : 0.0f;
+            lx = fmaf(f, wl[v * 16 + c], lx);
+            ox = fmaf(f, wo[(v * grp) * HD + i], ox);
+        }
+        const uint64_t at = ((uint64_t)blockIdx.x * a.c.n_kv + h) * grp + c;
+        w.acc[at * HD + i % HD] = ox;
+        if (i % HD == 0) { w.m[at] = mx; w.l[at] = lx; }
     }
 }
-// A workgroup per sequence and query head: the parts' sum.
+
+// A workgroup per query head and sequence: the parts, added.
 __global__ void __launch_bounds__(TPB) k_attn_paged_join(sgk_attn_paged_args a, ap_part w) {
     const uint32_t t = threadIdx.x, c = blockIdx.x, s = blockIdx.y, hd = a.c.hd;
-    const uint32_t len = page_len(a.c, a.lens, s), n = (len + AP_SLOTS - 1) / AP_SLOTS;
-    const uint64_t at = ((uint64_t)s * a.n_heads + c) * w.parts;
+    const ap_where me = ap_find(a, w, s, false);
     float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (uint32_t i = 0; i < n; i++) m = w.m[at + i] > m || w.m[at + i] != w.m[at + i] ? w.m[at + i] : m;
-    for (uint32_t i = 0; i < n; i++) {
-        const float f = w.m[at + i] == -INFINITY ? 0.0f : expf(w.m[at + i] - m);
-        l = fmaf(f, w.l[at + i], l);
-        if (t < hd && f != 0.0f) o = fmaf(f, w.acc[(at + i) * hd + t], o);
+    for (uint32_t i = 0; i < me.n; i++) m = fmaxf(m, w.m[(uint64_t)(me.first + i) * a.n_heads + c]);
+    for (uint32_t i = 0; i < me.n; i++) {
+        const uint64_t at = (uint64_t)(me.first + i) * a.n_heads + c;
+        const float mi = w.m[at], f = mi > -INFINITY ? exp2f((mi - m) * 1.44269504f) : 0.0f;
+        l = fmaf(f, w.l[at], l);
+        if (t < hd) o = fmaf(f, w.acc[at * hd + t], o);
     }
-    if (t < hd) a.out[((uint64_t)s * a.n_heads + c) * hd + t] = m == -INFINITY ? 0.0f : o / l;
-    if (w.score && t == 0) { w.m[at] = m; w.l[at] = l; }
+    if (t < hd) a.out[((uint64_t)s * a.n_heads + c) * hd + t] = l == 0.0f ? 0.0f : o / l;
+    if (w.score && t == 0) {
+        w.ml[2 * ((uint64_t)s * a.n_heads + c)] = m;
+        w.ml[2 * ((uint64_t)s * a.n_heads + c) + 1] = l * (1.0f / (1 << AP_P2));
+    }
 }
 __global__ void __launch_bounds__(TPB) k_attn_paged_weights(sgk_attn_paged_args a, ap_part w) {
     const uint32_t h = blockIdx.y, s = blockIdx.z, g = a.n_heads / a.c.n_kv, len = page_len(a.c, a.lens, s);
@@ -148,17 +403,32 @@ __global__ void __launch_bounds__(TPB) k_attn_paged_weights(sgk_attn_paged_args 
         if (page_row(a.c, s, j) >= 0)
             for (uint32_t c = h * g; c < h * g + g; c++) {
                 const uint64_t r = (uint64_t)s * a.n_heads + c;
-                sum += expf(w.score[r * cap + j] - w.m[r * w.parts]) / w.l[r * w.parts];
+                sum += exp2f((w.score[r * cap + j] - w.ml[2 * r]) * 1.44269504f) / w.ml[2 * r + 1];
             }
         a.weight_out[at] = (a.weight ? a.weight[at] : 0.0f) + sum;
     }
 }
-static ap_part ap_plan(const sgk_attn_paged_args *a, void *scratch, uint64_t *bytes) {
+static ap_part ap_plan(const sgk_attn_paged_args *a, char *at, uint64_t *bytes) {
     const uint64_t rows = (uint64_t)a->c.n_seq * a->n_heads, cap = (uint64_t)a->c.width << a->c.log;
-    const uint64_t parts = (cap + AP_SLOTS - 1) / AP_SLOTS;
-    float *f = (float *)scratch;
-    *bytes = 4 * (rows * parts * (2 + a->c.hd) + (a->weight_out ? rows * cap : 0));
-    return (ap_part){f, f + rows * parts, f + 2 * rows * parts, a->weight_out ? f + rows * parts * (2 + a->c.hd) : NULL, (uint32_t)parts};
+    const uint64_t steps = (cap + AP_STEP - 1) / AP_STEP * a->c.n_seq;      // at most
+    uint64_t most = (2 * sgk_device_cus() + a->c.n_kv - 1) / a->c.n_kv;
+    if (most > (steps + AP_MIN - 1) / AP_MIN) most = (steps + AP_MIN - 1) / AP_MIN;
+    ap_part w = {};
+    w.most = (uint32_t)most;
+    w.parts = w.most + a->c.n_seq;
+    const uint64_t heads = (uint64_t)w.parts * a->n_heads;
+    uint64_t n = 0;
+    auto take = [&](uint64_t words) { const uint64_t o = n; n += (words + 3) / 4 * 4; return at + 4 * o; };
+    w.acc = (float *)take(heads * a->c.hd);
+    w.m = (float *)take(heads);
+    w.l = (float *)take(heads);
+    if (a->weight_out) {
+        w.score = (float *)take(rows * cap);
+        w.ml = (float *)take(2 * rows);
+    }
+    if (a->c.n_seq > 64) w.plan = (uint32_t *)take((uint64_t)a->c.n_seq + 2 + w.parts);
+    *bytes = 4 * n;
+    return w;
 }
 extern "C" uint64_t sgk_attn_paged_scratch(const sgk_attn_paged_args *a) {
     uint64_t bytes;
@@ -167,10 +437,23 @@ extern "C" uint64_t sgk_attn_paged_scratch(const sgk_attn_paged_args *a) {
 }
 extern "C" hipError_t sgk_attn_paged(const sgk_attn_paged_args *a, void *scratch, hipStream_t s, hipEvent_t done) {
     uint64_t bytes;
-    const ap_part w = ap_plan(a, scratch, &bytes);
-    launch(k_attn_paged, dim3(w.parts, a->c.n_kv, a->c.n_seq), TPB, s, (hipEvent_t)NULL, *a, w);
+    const ap_part w = ap_plan(a, (char *)scratch, &bytes);
+    const uint32_t hd = a->c.hd, grp = a->n_heads / a->c.n_kv;
+    const int al = !((uintptr_t)a->q & 15) && a->q_stride % 4 == 0;
+    const uint32_t ql = 3 * (hd / 32) * 1024, ol = AP_WAVES * (128 + grp * hd * 4), lds = ql > ol ? ql : ol;
+    if (w.plan) launch(k_attn_paged_plan, dim3(1), 1024, s, (hipEvent_t)NULL, *a, w);
+    const dim3 grid(w.parts, a->c.n_kv);
+    void (*const k)(sgk_attn_paged_args, ap_part, int) = hd == 64 ? k_attn_paged<64> : hd == 128 ? k_attn_paged<128> : k_attn_paged<256>;
+    if (lds > 65536) {      // 16 heads of 256
+        const hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(k, grid, dim3(AP_WAVES * 64), lds, s, *a, w, al);
     launch(k_attn_paged_join, dim3(a->n_heads, a->c.n_seq), TPB, s, a->weight_out ? (hipEvent_t)NULL : done, *a, w);
-    if (a->weight_out) launch(k_attn_paged_weights, dim3(w.parts < 256 ? w.parts : 256, a->c.n_kv, a->c.n_seq), TPB, s, done, *a, w);
+    if (a->weight_out) {
+        const uint64_t need = (((uint64_t)a->c.width << a->c.log) + TPB - 1) / TPB;
+        launch(k_attn_paged_weights, dim3((uint32_t)(need < 256 ? need : 256), a->c.n_kv, a->c.n_seq), TPB, s, done, *a, w);
+    }
     return hipGetLastError();
 }
 
