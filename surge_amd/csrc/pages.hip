@@ -90,33 +90,34 @@ extern "C" hipError_t sgk_page_store(const sgk_page_store_args *a, hipStream_t s
 // largest element), p into two (2^-22), so that products are exact or nearly so
 // and sums are f32.
 //
-// Parts: T steps in all and room for `most` parts a head give parts of
-// ceil(T / most) steps, at least AP_MIN, the same on every workgroup; a sequence
-// of n steps has ceil(n / per) of them, so there are at most most + n_seq.
+// Parts: T steps in all and `most` parts a kv head wanted give parts of `per` =
+// ceil(T / most) steps, a multiple of the waves, the same on every workgroup; a
+// sequence of n steps has ceil(n / per) of them, so there are at most most + n_seq.
 // ---------------------------------------------------------------------------
 #define AP_STEP 32u
-#define AP_MIN 4u
-#define AP_WAVES 4
+#define AP_WAVES 4u
+#define AP_MOST 1024u      // parts of a sequence, at most
 #define AP_P2 14            // p is held times 2^14, so that f16's subnormals start at 2^-28
 
 struct ap_part {
     float *m, *l, *acc;     // [part][head], acc x hd
     float *score;           // [seq][head][cap], or NULL
-    float *ml;              // [seq][head][2]: maximum and sum, for the weights
     uint32_t *plan;         // [n_seq + 1] first parts, then [parts] sequences; NULL up to 64 sequences
     uint32_t most, parts;
 };
 
 __device__ __forceinline__ uint32_t ap_steps(const sgk_attn_paged_args &a, uint32_t s) { return (page_len(a.c, a.lens, s) + AP_STEP - 1) / AP_STEP; }
-__device__ __forceinline__ uint32_t ap_per(uint64_t total, uint32_t most) { return max(AP_MIN, (uint32_t)((total + most - 1) / most)); }
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {        // inclusive
-    const uint32_t l = threadIdx.x & 63;
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const uint32_t y = __shfl_up(v, d);
-        if (l >= d) v += y;
-    }
-    return v;
+__device__ __forceinline__ uint32_t ap_per(uint64_t total, uint32_t most) { return (max((uint32_t)((total + most - 1) / most), 1u) + AP_WAVES - 1) / AP_WAVES * AP_WAVES; }
+// Inclusive prefix sum over the wave: within the rows of 16, then the rows' ends carried on.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_0(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true); }
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v += dpp_or_0<0x111, 0xF>(v);       // row_shr 1, 2, 4, 8
+    v += dpp_or_0<0x112, 0xF>(v);
+    v += dpp_or_0<0x114, 0xF>(v);
+    v += dpp_or_0<0x118, 0xF>(v);
+    v += dpp_or_0<0x142, 0xA>(v);       // row_bcast 15 into rows 1 and 3
+    return v + dpp_or_0<0x143, 0xC>(v); // row_bcast 31 into rows 2 and 3
 }
 struct ap_where { uint32_t s, first, n, per; };      // sequence (n_seq: none), its first part and their number
 // Of part x (by_part) or of sequence x.
@@ -126,6 +127,10 @@ __device__ __forceinline__ ap_where ap_find(const sgk_attn_paged_args &a, const 
         const uint32_t all = w.plan[ns], s = !by_part ? x : x < all ? w.plan[ns + 2 + x] : ns;
         if (s >= ns) return (ap_where){ns, 0, 0, 0};
         return (ap_where){s, w.plan[s], w.plan[s + 1] - w.plan[s], w.plan[ns + 1]};
+    }
+    if (ns == 1) {
+        const uint32_t st = ap_steps(a, 0), per = ap_per(st, w.most), n = (st + per - 1) / per;
+        return (ap_where){by_part && x >= n ? 1u : 0u, 0, n, per};
     }
     const uint32_t l = threadIdx.x & 63, st = l < ns ? ap_steps(a, l) : 0;
     const uint32_t per = ap_per((uint32_t)__builtin_amdgcn_readlane((int)wave_scan(st), 63), w.most);     // 64 x 2^25 steps at most
@@ -180,73 +185,36 @@ __global__ void __launch_bounds__(AP_WAVES * 64, 2) k_attn_paged(sgk_attn_paged_
     extern __shared__ __align__(16) char lds[];
     f16x8 (*qs)[NJ][64] = (f16x8 (*)[NJ][64])lds;
     const uint32_t t = threadIdx.x, l = t & 63, r = l & 15, g = l >> 4, wv = __builtin_amdgcn_readfirstlane(t >> 6);
-    const uint32_t h = blockIdx.y, grp = a.n_heads / a.c.n_kv;
-    const ap_where me = ap_find(a, w, blockIdx.x, true);
+    const uint32_t h = blockIdx.x, part = blockIdx.y, grp = a.n_heads / a.c.n_kv;
+    const ap_where me = ap_find(a, w, part, true);
     if (me.s >= a.c.n_seq) return;
     const uint32_t s = me.s, len = page_len(a.c, a.lens, s), all = (len + AP_STEP - 1) / AP_STEP;
-    const uint32_t st0 = (blockIdx.x - me.first) * me.per, st1 = min(st0 + me.per, all);
+    // the sequence's steps, evenly over its parts (a multiple of the waves)
+    const uint32_t each = ((all + me.n - 1) / me.n + AP_WAVES - 1) / AP_WAVES * AP_WAVES;
+    const uint32_t st0 = min((part - me.first) * each, all), st1 = min(st0 + each, all);
     const uint64_t wide = (uint64_t)a.c.n_kv * HD, cap = (uint64_t)a.c.width << a.c.log;
     const scalar_i32 *table = (const scalar_i32 *)(uintptr_t)(a.c.table + (uint64_t)s * a.c.width);
 
-    // q of head r, dims 32 j + 8 g ..+7, as three f16: wave w has the j that are w mod the waves
-    float f1;
+    // q of head r, dims 32 j + 8 g ..+7: all of it for its largest element, the j that are the wave's mod the waves as three f16
+    float qx[NJ][8];
     {
-        constexpr int NQ = (NJ + AP_WAVES - 1) / AP_WAVES;
-        float x[NQ][8], am = 0.0f;
         const float *q = a.q + ((uint64_t)s * a.n_heads + h * grp + min(r, grp - 1)) * a.q_stride + 8 * g;
         if (al) {
 #pragma unroll
-            for (int i = 0; i < NQ; i++)
+            for (int j = 0; j < NJ; j++)
 #pragma unroll
                 for (int z = 0; z < 2; z++) {
-                    const f32x4 y = *(const f32x4 *)(q + 32 * ((wv + AP_WAVES * i) % NJ) + 4 * z);
+                    const f32x4 y = *(const f32x4 *)(q + 32 * j + 4 * z);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[i][4 * z + e] = y[e];
+                    for (int e = 0; e < 4; e++) qx[j][4 * z + e] = y[e];
                 }
         } else {
 #pragma unroll
-            for (int i = 0; i < NQ; i++)
+            for (int j = 0; j < NJ; j++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[i][e] = q[32 * ((wv + AP_WAVES * i) % NJ) + e];
-        }
-#pragma unroll
-        for (int i = 0; i < NQ; i++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) am = fmaxf(am, fabsf(x[i][e]));
-        am = fmaxf(am, swap16f(am));
-        am = fmaxf(am, swap32f(am));
-        float *red = (float *)lds;
-        if (g == 0) red[wv * 16 + r] = am;
-        __syncthreads();
-#pragma unroll
-        for (int v = 0; v < AP_WAVES; v++) am = fmaxf(am, red[v * 16 + r]);
-        __syncthreads();
-        const int ex = am > 0.0f && am < INFINITY ? __builtin_amdgcn_frexp_expf(am) : 0;
-        f1 = __builtin_amdgcn_ldexpf(a.scale, ex - 15);
-#pragma unroll
-        for (int i = 0; i < NQ; i++) {
-            const uint32_t j = wv + AP_WAVES * i;
-            if (j >= NJ) break;
-            f16x8 p[3];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                float y = __builtin_amdgcn_ldexpf(x[i][e], 15 - ex);
-#pragma unroll
-                for (int z = 0; z < 3; z++) {
-                    p[z][e] = (_Float16)y;
-                    y -= (float)p[z][e];
-                }
-            }
-#pragma unroll
-            for (int z = 0; z < 3; z++) qs[z][j][l] = p[z];
+                for (int e = 0; e < 8; e++) qx[j][e] = q[32 * j + e];
         }
     }
-    __syncthreads();
-
-    float m = -INFINITY, sum = 0.0f;
-    f32x4 o[NT];
-#pragma unroll
-    for (int i = 0; i < NT; i++) o[i] = (f32x4){0, 0, 0, 0};
     // a half step's rows: whether they are there, and where in the pools (uniform); slots behind the last: its page
     struct half_at { bool ok; uint64_t off; };
     auto at = [&](uint32_t j) -> half_at {
@@ -263,17 +231,55 @@ __global__ void __launch_bounds__(AP_WAVES * 64, 2) k_attn_paged(sgk_attn_paged_
 #pragma unroll
         for (int z = 0; z < 2; z++)
 #pragma unroll
-            for (int j = 0; j < NJ; j++) kf[z][j] = *(const f16x8 *)(uniform((const char *)a.c.k + p[z].off) + koff + 64 * j);
+            for (int j = 0; j < NJ; j++) kf[z][j] = __builtin_nontemporal_load((const f16x8 *)(uniform((const char *)a.c.k + p[z].off) + koff + 64 * j));
     };
-    half_at now[2] = {at((st0 + wv) * AP_STEP), at((st0 + wv) * AP_STEP + 16)};
-    if (st0 + wv < st1) load_k(now);
-    for (uint32_t st = st0 + wv; st < st1; st += AP_WAVES) {
-        const uint32_t j0 = st * AP_STEP;
-        vrow vf[NC][8];
+    vrow vf[NC][8];
+    auto load_v = [&](const half_at (&p)[2]) {
 #pragma unroll
         for (int e = 0; e < 8; e++)
 #pragma unroll
-            for (int c = 0; c < NC; c++) vf[c][e] = *(const vrow *)(uniform((const char *)a.c.v + now[e / 4].off) + voff[e % 4] + 32 * VD * c);
+            for (int c = 0; c < NC; c++)
+                vf[c][e] = __builtin_nontemporal_load((const vrow *)(uniform((const char *)a.c.v + p[e / 4].off) + voff[e % 4] + 32 * VD * c));
+    };
+    half_at now[2] = {at((st0 + wv) * AP_STEP), at((st0 + wv) * AP_STEP + 16)};
+    if (st0 + wv < st1) { load_k(now); load_v(now); }
+    __builtin_amdgcn_sched_barrier(0);
+    float f1;
+    {
+        float am = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) am = fmaxf(am, fabsf(qx[j][e]));
+        am = fmaxf(am, swap16f(am));
+        am = fmaxf(am, swap32f(am));
+        const int ex = am > 0.0f && am < INFINITY ? __builtin_amdgcn_frexp_expf(am) : 0;
+        f1 = __builtin_amdgcn_ldexpf(a.scale, ex - 15);
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            if (j % AP_WAVES != wv) continue;
+            f16x8 p[3];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                float y = __builtin_amdgcn_ldexpf(qx[j][e], 15 - ex);
+#pragma unroll
+                for (int z = 0; z < 3; z++) {
+                    p[z][e] = (_Float16)y;
+                    y -= (float)p[z][e];
+                }
+            }
+#pragma unroll
+            for (int z = 0; z < 3; z++) qs[z][j][l] = p[z];
+        }
+    }
+    __syncthreads();
+
+    float m = -INFINITY, sum = 0.0f;
+    f32x4 o[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++) o[i] = (f32x4){0, 0, 0, 0};
+    for (uint32_t st = st0 + wv; st < st1; st += AP_WAVES) {
+        const uint32_t j0 = st * AP_STEP;
         const half_at next[2] = {at(j0 + AP_WAVES * AP_STEP), at(j0 + AP_WAVES * AP_STEP + 16)};
         asm volatile("" ::: "memory");      // q's parts are read again every step, not kept in registers
         float x[8];
@@ -338,6 +344,8 @@ __global__ void __launch_bounds__(AP_WAVES * 64, 2) k_attn_paged(sgk_attn_paged_
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(u.v, pl, d, 0, 0, 0);
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(u.v, ph, d, 0, 0, 0);
             }
+        __builtin_amdgcn_sched_barrier(0);
+        if (st + AP_WAVES < st1) load_v(next);
         now[0] = next[0];
         now[1] = next[1];
     }
@@ -346,10 +354,10 @@ __global__ void __launch_bounds__(AP_WAVES * 64, 2) k_attn_paged(sgk_attn_paged_
 
     // the waves' results, added: o[c VD + j][i] of lane (r, g) is head r, dim 16 VD c + VD (4 g + i) + j
     __syncthreads();
-    float *wm = (float *)lds, *wl = wm + AP_WAVES * 16, *wo = wl + AP_WAVES * 16;       // [wave][16], [wave][16], [wave][grp][HD]
+    float *wm = (float *)lds, *wl = wm + AP_WAVES * 16, *wo = wl + AP_WAVES * 16;       // [wave][16] twice, [wave][grp][HD + 4]
     if (g == 0) { wm[wv * 16 + r] = m; wl[wv * 16 + r] = sum; }
     if (r < grp) {
-        float *d = wo + ((uint64_t)wv * grp + r) * HD + 4 * g * VD;
+        float *d = wo + (wv * grp + r) * (HD + 4) + 4 * g * VD;
 #pragma unroll
         for (int c = 0; c < NC; c++)
 #pragma unroll
@@ -359,60 +367,95 @@ __global__ void __launch_bounds__(AP_WAVES * 64, 2) k_attn_paged(sgk_attn_paged_
                     *(f32x4 *)(d + 16 * VD * c + VD * i + j) = (f32x4){o[c * VD + j][i], o[c * VD + j + 1][i], o[c * VD + j + 2][i], o[c * VD + j + 3][i]};
     }
     __syncthreads();
-    for (uint32_t i = t; i < grp * HD; i += AP_WAVES * 64) {
-        const uint32_t c = i / HD;
-        float mx = -INFINITY, lx = 0.0f, ox = 0.0f;
+    for (uint32_t i = t; i < grp * (HD / 4); i += AP_WAVES * 64) {
+        const uint32_t c = i / (HD / 4), d = i % (HD / 4) * 4;
+        float mx = -INFINITY, lx = 0.0f;
+        f32x4 ox = {0, 0, 0, 0};
 #pragma unroll
-        for (int v = 0; v < AP_WAVES; v++) mx = fmaxf(mx, wm[v * 16 + c]);
+        for (uint32_t v = 0; v < AP_WAVES; v++) mx = fmaxf(mx, wm[v * 16 + c]);
 #pragma unroll
-        for (int v = 0; v < AP_WAVES; v++) {
+        for (uint32_t v = 0; v < AP_WAVES; v++) {
             const float mv = wm[v * 16 + c], f = mv > -INFINITY ? exp2f((mv - mx) * 1.44269504f) : 0.0f;
             lx = fmaf(f, wl[v * 16 + c], lx);
-            ox = fmaf(f, wo[(v * grp) * HD + i], ox);
+            ox += f * *(const f32x4 *)(wo + (v * grp + c) * (HD + 4) + d);
         }
-        const uint64_t at = ((uint64_t)blockIdx.x * a.c.n_kv + h) * grp + c;
-        w.acc[at * HD + i % HD] = ox;
-        if (i % HD == 0) { w.m[at] = mx; w.l[at] = lx; }
+        const uint64_t at = (uint64_t)part * a.n_heads + h * grp + c;
+        *(f32x4 *)(w.acc + at * HD + d) = ox;
+        if (d == 0) { w.m[at] = mx; w.l[at] = lx; }
     }
 }
 
-// A workgroup per query head and sequence: the parts, added.
-__global__ void __launch_bounds__(TPB) k_attn_paged_join(sgk_attn_paged_args a, ap_part w) {
-    const uint32_t t = threadIdx.x, c = blockIdx.x, s = blockIdx.y, hd = a.c.hd;
-    const ap_where me = ap_find(a, w, s, false);
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (uint32_t i = 0; i < me.n; i++) m = fmaxf(m, w.m[(uint64_t)(me.first + i) * a.n_heads + c]);
-    for (uint32_t i = 0; i < me.n; i++) {
-        const uint64_t at = (uint64_t)(me.first + i) * a.n_heads + c;
-        const float mi = w.m[at], f = mi > -INFINITY ? exp2f((mi - m) * 1.44269504f) : 0.0f;
-        l = fmaf(f, w.l[at], l);
-        if (t < hd) o = fmaf(f, w.acc[at * hd + t], o);
+// The largest of n parts' maxima of a head, and the sum of the parts' sums under it: a wave, all lanes get them. f: the
+// parts' factors, or NULL.
+__device__ __forceinline__ f32x2 ap_maxsum(const ap_part &w, uint64_t at, uint32_t n, uint32_t stride, float *f) {
+    const uint32_t l = threadIdx.x & 63;
+    float m = -INFINITY, sum = 0.0f;
+    for (uint32_t i = l; i < n; i += 64) m = fmaxf(m, w.m[at + (uint64_t)i * stride]);
+    m = wave_fmax(m);
+    for (uint32_t i = l; i < n; i += 64) {
+        const float mi = w.m[at + (uint64_t)i * stride], fi = mi > -INFINITY ? exp2f((mi - m) * 1.44269504f) : 0.0f;
+        sum = fmaf(fi, w.l[at + (uint64_t)i * stride], sum);
+        if (f) f[i] = fi;
     }
-    if (t < hd) a.out[((uint64_t)s * a.n_heads + c) * hd + t] = l == 0.0f ? 0.0f : o / l;
-    if (w.score && t == 0) {
-        w.ml[2 * ((uint64_t)s * a.n_heads + c)] = m;
-        w.ml[2 * ((uint64_t)s * a.n_heads + c) + 1] = l * (1.0f / (1 << AP_P2));
-    }
+    return (f32x2){m, wave_fsum(sum)};
 }
-__global__ void __launch_bounds__(TPB) k_attn_paged_weights(sgk_attn_paged_args a, ap_part w) {
-    const uint32_t h = blockIdx.y, s = blockIdx.z, g = a.n_heads / a.c.n_kv, len = page_len(a.c, a.lens, s);
-    const uint64_t cap = (uint64_t)a.c.width << a.c.log;
-    for (uint32_t j = blockIdx.x * TPB + threadIdx.x; j < len; j += gridDim.x * TPB) {
-        const uint64_t at = ((uint64_t)s * a.c.n_kv + h) * cap + j;
+// A workgroup per 64 dims of a query head and sequence adds the parts, four dims a lane, the parts by 16 lane groups in turn.
+// Where the weights are wanted, the workgroups behind take a sequence's slots, one kv head each.
+__global__ void __launch_bounds__(TPB) k_attn_paged_join(sgk_attn_paged_args a, ap_part w) {
+    __shared__ float f[AP_MOST];
+    __shared__ f32x4 red[TPB];
+    __shared__ f32x2 ml[16];
+    const uint32_t t = threadIdx.x, s = blockIdx.y, hd = a.c.hd, g = a.n_heads / a.c.n_kv;
+    const ap_where me = ap_find(a, w, s, false);
+    const uint32_t adders = a.n_heads * (hd / 64);
+    if (blockIdx.x < adders) {
+        const uint32_t head = blockIdx.x / (hd / 64), d = blockIdx.x % (hd / 64) * 64 + t % 16 * 4;
+        const uint64_t at = (uint64_t)me.first * a.n_heads + head;
+        if (t < 64) {
+            const f32x2 r = ap_maxsum(w, at, me.n, a.n_heads, f);
+            if (t == 0) ml[0] = r;
+        }
+        __syncthreads();
+        f32x4 o = {0, 0, 0, 0};
+        const float *acc = w.acc + at * hd + d;
+#pragma unroll 8
+        for (uint32_t i = t / 16; i < me.n; i += TPB / 16) o += f[i] * *(const f32x4 *)(acc + (uint64_t)i * a.n_heads * hd);
+        red[t] = o;
+        __syncthreads();
+        if (t >= 16) return;
+#pragma unroll
+        for (uint32_t i = 1; i < TPB / 16; i++) o += red[t + i * 16];
+        const float l = ml[0][1];
+#pragma unroll
+        for (int e = 0; e < 4; e++) a.out[((uint64_t)s * a.n_heads + head) * hd + d + e] = l == 0.0f ? 0.0f : o[e] / l;
+        return;
+    }
+    const uint32_t x = blockIdx.x - adders, h = x % a.c.n_kv, nb = (gridDim.x - adders) / a.c.n_kv, len = page_len(a.c, a.lens, s);
+    const uint64_t cap = (uint64_t)a.c.width << a.c.log, at = ((uint64_t)s * a.c.n_kv + h) * cap;
+    if ((x / a.c.n_kv) * TPB >= len) return;
+    for (uint32_t c = t >> 6; c < g; c += TPB / 64) {
+        const f32x2 r = ap_maxsum(w, (uint64_t)me.first * a.n_heads + h * g + c, me.n, a.n_heads, NULL);
+        if ((t & 63) == 0) ml[c] = (f32x2){r[0], (float)(1 << AP_P2) / r[1]};
+    }
+    __syncthreads();
+    for (uint32_t j = (x / a.c.n_kv) * TPB + t; j < len; j += nb * TPB) {
         float sum = 0.0f;
-        if (page_row(a.c, s, j) >= 0)
-            for (uint32_t c = h * g; c < h * g + g; c++) {
-                const uint64_t r = (uint64_t)s * a.n_heads + c;
-                sum += exp2f((w.score[r * cap + j] - w.ml[2 * r]) * 1.44269504f) / w.ml[2 * r + 1];
-            }
-        a.weight_out[at] = (a.weight ? a.weight[at] : 0.0f) + sum;
+        const float *sc = w.score + ((uint64_t)s * a.n_heads + h * g) * cap + j;
+        // a slot that is not there has -inf for a score, and so no weight
+        for (uint32_t c = 0; c < g; c++)
+            if (sc[c * cap] != -INFINITY) sum = fmaf(exp2f((sc[c * cap] - ml[c][0]) * 1.44269504f), ml[c][1], sum);
+        a.weight_out[at + j] = (a.weight ? a.weight[at + j] : 0.0f) + sum;
     }
 }
 static ap_part ap_plan(const sgk_attn_paged_args *a, char *at, uint64_t *bytes) {
     const uint64_t rows = (uint64_t)a->c.n_seq * a->n_heads, cap = (uint64_t)a->c.width << a->c.log;
     const uint64_t steps = (cap + AP_STEP - 1) / AP_STEP * a->c.n_seq;      // at most
-    uint64_t most = (2 * sgk_device_cus() + a->c.n_kv - 1) / a->c.n_kv;
-    if (most > (steps + AP_MIN - 1) / AP_MIN) most = (steps + AP_MIN - 1) / AP_MIN;
+    // as many parts as workgroups are resident together; a sequence's last part is counted too, unless there are that many
+    const uint64_t there = (uint64_t)(a->c.hd == 256 ? 2 : a->c.hd == 128 ? 3 : 4) * sgk_device_cus() / a->c.n_kv;
+    uint64_t most = there > 2 * a->c.n_seq ? there - a->c.n_seq : there;
+    if (most > AP_MOST) most = AP_MOST;
+    if (most > (steps + AP_WAVES - 1) / AP_WAVES) most = (steps + AP_WAVES - 1) / AP_WAVES;
+    if (!most) most = 1;
     ap_part w = {};
     w.most = (uint32_t)most;
     w.parts = w.most + a->c.n_seq;
@@ -422,10 +465,7 @@ static ap_part ap_plan(const sgk_attn_paged_args *a, char *at, uint64_t *bytes) 
     w.acc = (float *)take(heads * a->c.hd);
     w.m = (float *)take(heads);
     w.l = (float *)take(heads);
-    if (a->weight_out) {
-        w.score = (float *)take(rows * cap);
-        w.ml = (float *)take(2 * rows);
-    }
+    if (a->weight_out) w.score = (float *)take(rows * cap);
     if (a->c.n_seq > 64) w.plan = (uint32_t *)take((uint64_t)a->c.n_seq + 2 + w.parts);
     *bytes = 4 * n;
     return w;
@@ -440,20 +480,21 @@ extern "C" hipError_t sgk_attn_paged(const sgk_attn_paged_args *a, void *scratch
     const ap_part w = ap_plan(a, (char *)scratch, &bytes);
     const uint32_t hd = a->c.hd, grp = a->n_heads / a->c.n_kv;
     const int al = !((uintptr_t)a->q & 15) && a->q_stride % 4 == 0;
-    const uint32_t ql = 3 * (hd / 32) * 1024, ol = AP_WAVES * (128 + grp * hd * 4), lds = ql > ol ? ql : ol;
+    const uint32_t ql = 3 * (hd / 32) * 1024, ol = AP_WAVES * (128 + grp * (hd + 4) * 4), lds = ql > ol ? ql : ol;
     if (w.plan) launch(k_attn_paged_plan, dim3(1), 1024, s, (hipEvent_t)NULL, *a, w);
-    const dim3 grid(w.parts, a->c.n_kv);
+    const dim3 grid(a->c.n_kv, w.parts);
     void (*const k)(sgk_attn_paged_args, ap_part, int) = hd == 64 ? k_attn_paged<64> : hd == 128 ? k_attn_paged<128> : k_attn_paged<256>;
     if (lds > 65536) {      // 16 heads of 256
         const hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
     hipLaunchKernelGGL(k, grid, dim3(AP_WAVES * 64), lds, s, *a, w, al);
-    launch(k_attn_paged_join, dim3(a->n_heads, a->c.n_seq), TPB, s, a->weight_out ? (hipEvent_t)NULL : done, *a, w);
+    uint32_t more = 0;      // workgroups a kv head for the weights
     if (a->weight_out) {
         const uint64_t need = (((uint64_t)a->c.width << a->c.log) + TPB - 1) / TPB;
-        launch(k_attn_paged_weights, dim3((uint32_t)(need < 256 ? need : 256), a->c.n_kv, a->c.n_seq), TPB, s, done, *a, w);
+        more = (uint32_t)(need < 64 ? need : 64);
     }
+    launch(k_attn_paged_join, dim3(a->n_heads * (hd / 64) + more * a->c.n_kv, a->c.n_seq), TPB, s, done, *a, w);
     return hipGetLastError();
 }
 
