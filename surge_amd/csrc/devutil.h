@@ -77,10 +77,15 @@ __device__ __forceinline__ void st4(float *p, f32x4 v, bool al) {
 // A launch, and with `done` the event of its own completion: waiting for that
 // takes 8.8 us from an empty kernel's launch on, where waiting for the stream,
 // which queues a packet behind the kernel, takes 10.9.
+// launch_lds: with `lds` bytes of dynamic LDS.
+template <typename K, typename... A>
+static inline void launch_lds(K kernel, dim3 grid, uint32_t threads, uint32_t lds, hipStream_t s, hipEvent_t done, A... args) {
+    if (done) hipExtLaunchKernelGGL(kernel, grid, dim3(threads), lds, s, (hipEvent_t) nullptr, done, 0, args...);
+    else hipLaunchKernelGGL(kernel, grid, dim3(threads), lds, s, args...);
+}
 template <typename K, typename... A>
 static inline void launch(K kernel, dim3 grid, uint32_t threads, hipStream_t s, hipEvent_t done, A... args) {
-    if (done) hipExtLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, (hipEvent_t) nullptr, done, 0, args...);
-    else hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, args...);
+    launch_lds(kernel, grid, threads, 0, s, done, args...);
 }
 
 #endif

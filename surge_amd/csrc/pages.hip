@@ -488,7 +488,7 @@ extern "C" hipError_t sgk_attn_paged(const sgk_attn_paged_args *a, void *scratch
         const hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(k, grid, dim3(AP_WAVES * 64), lds, s, *a, w, al);
+    launch_lds(k, grid, AP_WAVES * 64, lds, s, (hipEvent_t)NULL, *a, w, al);
     uint32_t more = 0;      // workgroups a kv head for the weights
     if (a->weight_out) {
         const uint64_t need = (((uint64_t)a->c.width << a->c.log) + TPB - 1) / TPB;
@@ -500,17 +500,20 @@ extern "C" hipError_t sgk_attn_paged(const sgk_attn_paged_args *a, void *scratch
 
 // ---------------------------------------------------------------------------
 // Eviction. The order of a (sequence, kv head)'s slots: recent ones first, then
-// by weight, then the lower slot; the first `keep` stay. A workgroup has the
-// slots' keys in registers and finds the keep-th by its bits, counting the keys
-// from a border on with ballots (a histogram in LDS waits on its own additions:
-// weights share their exponents; 32768 slots 147 us); it stops at a border with
-// just `keep` keys above it. Slots below keep that go are freed places, kept ones
-// from keep on are moved rows: as many, both in rising order, so one prefix sum
-// over both marks numbers them. No row that is read is written, so the moves need
-// no order.
+// by weight, then the lower slot; the first `keep` stay. A workgroup holds the
+// slots' keys in LDS (EV_HELD of them; past that it reads weight and pos again
+// each time) and finds the keep-th by three histograms, of 11, 11 and 10 bits
+// (weights share few exponents: with 8 bits, and lanes with the same bin not added
+// first, the additions wait for each other). Slots below keep that go are freed
+// places, kept ones from keep on are moved rows: as many, both in rising order, so
+// one prefix sum over both marks numbers them. No row that is read is written, so
+// the moves need no order. Loops are not unrolled far: code that runs once comes
+// from memory (keys in registers, 64 a thread: 150 KB of it, slower than LDS).
 // ---------------------------------------------------------------------------
 #define EV_FEW 64u          // rows that the selecting workgroup moves itself
-struct ev_list { uint32_t *hole, *mover, *n; };      // [row][most] twice, [row]: rows to move
+#define EV_HELD 32896u      // keys in LDS: 128 a page past 32768, so that a prompt's new slots fit too
+#define EV_BINS 2048u
+struct ev_list { uint32_t *hole, *mover, *n; };      // [row][most] twice, [row]: rows to move; NULL: the few are moved at once
 __host__ __device__ static inline uint32_t ev_most(uint32_t keep, uint32_t cap) { return keep < cap - keep ? keep : cap - keep; }
 
 // Rising with the order: 0xFFFFFFFF recent, 0 NaN.
@@ -522,14 +525,7 @@ __device__ __forceinline__ uint32_t ev_key(float w, int32_t pos, int64_t after) 
 __device__ __forceinline__ uint32_t lanes_below(uint64_t b) {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
 }
-// The sum over the rows of 16 lanes, in every lane.
-__device__ __forceinline__ uint32_t row_sum(uint32_t v) {
-    v += dppu<0xB1>(v);
-    v += dppu<0x4E>(v);
-    v += dppu<0x141>(v);
-    return v + dppu<0x128>(v);
-}
-// Rows `from` to `to` of the lists: K and V by 16 bytes a thread, weight and pos with the first.
+// Row `from` to `to`: K and V by 16 bytes a thread, weight and pos with the first.
 __device__ __forceinline__ void ev_move(const sgk_page_evict_args &a, uint32_t s, uint32_t h, uint32_t from, uint32_t to, uint32_t u, uint32_t units) {
     const uint64_t cap = (uint64_t)a.c.width << a.c.log, row = ((uint64_t)s * a.c.n_kv + h) * cap, wide = (uint64_t)a.c.n_kv * units;
     const int64_t x = page_row(a.c, s, from), y = page_row(a.c, s, to);
@@ -543,134 +539,190 @@ __device__ __forceinline__ void ev_move(const sgk_page_evict_args &a, uint32_t s
     ((u16x8 *)a.c.k)[yi] = kv;
     ((u16x8 *)a.c.v)[yi] = vv;
 }
+// Over the workgroup: the exclusive prefix sum of v, and the total. tmp: [2][16], halves taken in turn.
+template <int T>
+__device__ __forceinline__ uint32_t ev_scan(uint32_t v, uint32_t *total, uint32_t (*tmp)[16], int &at) {
+    const uint32_t to = wave_scan(v), wv = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 63) tmp[at][wv] = to;
+    __syncthreads();
+    uint32_t before = to - v, all = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < T / 64; i++) {
+        const uint32_t x = tmp[at][i];
+        if (i < wv) before += x;
+        all += x;
+    }
+    at ^= 1;
+    *total = all;
+    return before;
+}
 
-// Up to T * U slots; BITS of the border a step.
-template <int T, int U, int BITS>
+template <int T, bool HELD>
 __global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list w) {
-    constexpr int W = T / 64, C = (1 << BITS) - 1;
-    __shared__ uint32_t cnt[2][C][16], marks[U * W], all;
+    constexpr uint32_t W = T / 64, PER = EV_BINS / T;
+    extern __shared__ uint32_t held[];
+    __shared__ uint32_t bins[EV_BINS], tmp[2][16], marks[T], pick[3];
     __shared__ int32_t lasts[W];
     __shared__ uint32_t few[2][EV_FEW];
     const uint32_t t = threadIdx.x, l = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), h = blockIdx.x, s = blockIdx.y;
-    const uint32_t len = page_len(a.c, a.lens, s), cap = a.c.width << a.c.log, keep = min(a.keep, len), row = s * a.c.n_kv + h;
-    const float *wt = a.weight + (uint64_t)row * cap;
-    const int32_t *ps = a.pos + (uint64_t)row * cap;
-    float *wo = a.weight_out + (uint64_t)row * cap;
-    int32_t *po = a.pos_out + (uint64_t)row * cap;
+    const uint32_t len = page_len(a.c, a.lens, s), cap = a.c.width << a.c.log, keep = min(a.keep, len);
+    const uint64_t row = (uint64_t)s * a.c.n_kv + h;
+    const float *wt = a.weight + row * cap;
+    const int32_t *ps = a.pos + row * cap;
+    float *wo = a.weight_out + row * cap;
+    int32_t *po = a.pos_out + row * cap;
     if (t == 0 && w.n) w.n[row] = 0;
-    if (len <= a.keep) {
+    const bool stays = len <= a.keep;
+    if (stays || w.n) {         // all of the first `keep`; where a second launch moves rows, they come over these
         if (wo != wt) for (uint32_t j = t; j < keep; j += T) wo[j] = wt[j];
         if (po != ps) for (uint32_t j = t; j < keep; j += T) po[j] = ps[j];
-        return;
     }
-    // every loop over a thread's slots ends with the slots, by eights
-#define EV_EACH(i, BODY) _Pragma("unroll") for (int i##8 = 0; i##8 < U / 8; i##8++) { \
-        if (i##8 * 8u * T >= len) break; \
-        _Pragma("unroll") for (int i = 8 * i##8; i < 8 * i##8 + 8; i++) { BODY } }
-    constexpr bool HOLD = U <= 16;      // positions stay in registers until the last one is known; else they are read again
-    uint32_t key[U];
-    int32_t pv[HOLD ? U : 1], last = INT32_MIN;
-    float wr[HOLD ? U : 1];
-    EV_EACH(i, const int32_t x = ps[min(i * T + t, len - 1)]; last = max(last, x); if constexpr (HOLD) { pv[i] = x; wr[i] = wt[min(i * T + t, len - 1)]; })
+    if (stays) return;
+    for (uint32_t i = t; i < EV_BINS; i += T) bins[i] = 0;
+    int32_t last = INT32_MIN;
+#pragma unroll 8
+    for (uint32_t j = t; j < len; j += T) {
+        const int32_t p = ps[j];
+        last = max(last, p);
+        if (HELD) held[j] = (uint32_t)p;
+    }
     last = (int32_t)(wave_umax((uint32_t)last ^ 0x80000000u) ^ 0x80000000u);
     if (l == 0) lasts[wv] = last;
-    if (t < 2 * C * 16) (&cnt[0][0][0])[t] = 0;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < W; i++) last = max(last, lasts[i]);
+    for (uint32_t i = 0; i < W; i++) last = max(last, lasts[i]);
     const int64_t after = (int64_t)last - a.recent;
-    EV_EACH(i, const uint32_t j = i * T + t; int32_t x; float y;
-            if constexpr (HOLD) { x = pv[i]; y = wr[i]; } else { x = ps[min(j, len - 1)]; y = wt[min(j, len - 1)]; }
-            key[i] = j < len ? ev_key(y, x, after) : 0;)
-    // the largest border with `keep` keys from it on at least; behind the last slot a key of 0 is not counted
-    // above the lowest border but 0, which needs no count
-    uint32_t border = 0, from_border = len;
-    int at = 0;
-    for (int shift = 32 - BITS; shift >= 0 && from_border != keep; shift -= BITS, at ^= 1) {
-        uint32_t n[C];
-#pragma unroll
-        for (int c = 0; c < C; c++) n[c] = 0;
-        EV_EACH(i, _Pragma("unroll") for (int c = 0; c < C; c++)
-                n[c] += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(key[i] >= (border | (uint32_t)(c + 1) << shift)));)
-        if (l == 0)
-#pragma unroll
-            for (int c = 0; c < C; c++) cnt[at][c][wv] = n[c];
-        __syncthreads();        // the counts of a step are written two barriers after they were read
-        uint32_t step = 0;
-#pragma unroll
-        for (int c = 0; c < C; c++) {
-            const uint32_t m = (uint32_t)__builtin_amdgcn_readfirstlane((int)row_sum(cnt[at][c][l & 15]));
-            if (m >= keep) { step = (uint32_t)(c + 1) << shift; from_border = m; }
-        }
-        border |= step;
-    }
-    // of the border's keys, all stay, or where there are more than room the first `ties`
-    uint32_t ties = UINT32_MAX;
-    if (from_border != keep) {
-        uint32_t n = 0;
-        EV_EACH(i, const uint32_t m = (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(i * T + t < len && key[i] == border)); n += m;
-                if (l == 0) marks[i * W + wv] = m;)
-        if (l == 0) cnt[at][0][wv] = n;
+    if (HELD) {
+#pragma unroll 8
+        for (uint32_t j = t; j < len; j += T) held[j] = ev_key(wt[j], (int32_t)held[j], after);     // a thread's own
         __syncthreads();
-        n = (uint32_t)__builtin_amdgcn_readfirstlane((int)row_sum(cnt[at][0][l & 15]));
-        at ^= 1;
-        ties = keep - (from_border - n);
     }
-    // a prefix sum over the marks of the slots' 64s, which their waves counted
-    const uint32_t spans = min(U, (len + 8 * T - 1) / (8 * T) * 8) * W;
-    auto scan = [&]() {
-        uint32_t v[(U * W + T - 1) / T], sum = 0;
+    auto key_of = [&](uint32_t j) { return HELD ? held[j] : ev_key(wt[j], ps[j], after); };
+    const uint32_t spans = (len + 63) / 64;
+    // the keep-th key: `left` of the `here` keys with the border's upper bits stay
+    uint32_t border = 0, left = keep, here = len;
+    int at = 0;
+    for (int pass = 0; pass < 3 && left != here; pass++) {
+        const uint32_t shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, mask = pass == 2 ? 1023u : 2047u, up = pass == 0 ? 31 : pass == 1 ? 21 : 10;
+        if (pass) {
+            for (uint32_t i = t; i < EV_BINS; i += T) bins[i] = 0;
+            __syncthreads();
+        }
+        for (uint32_t i0 = wv * 4; i0 < spans; i0 += W * 4) {
+            uint32_t key[4];
 #pragma unroll
-        for (int i = 0; i < (U * W + T - 1) / T; i++) {
-            const uint32_t j = t * ((U * W + T - 1) / T) + i;
-            v[i] = j < spans ? marks[j] : 0;
+            for (uint32_t i = 0; i < 4; i++) key[i] = key_of(min((i0 + i) * 64 + l, len - 1));
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const uint32_t d = key[i] >> shift & mask;
+                const bool in = (i0 + i) * 64 + l < len && (!pass || (key[i] ^ border) >> up == 0);
+                const uint64_t m = __builtin_amdgcn_ballot_w64(in);
+                if (!m) continue;
+                // the first lane's bin is often most lanes': they add once
+                const uint32_t f = (uint32_t)__builtin_amdgcn_readlane((int)d, (int)__builtin_ctzll(m));
+                const uint64_t same = __builtin_amdgcn_ballot_w64(in && d == f);
+                if (l == 0) atomicAdd(&bins[f], (uint32_t)__popcll(same));
+                if (in && d != f) atomicAdd(&bins[d], 1u);
+            }
+        }
+        __syncthreads();
+        // from the top: the bin in which `left` keys are reached
+        uint32_t v[PER], sum = 0, unused;
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            v[i] = bins[EV_BINS - 1 - (t * PER + i)];
             sum += v[i];
         }
-        const uint32_t to = wave_scan(sum);
-        if (l == 63) cnt[at][0][wv] = to;
-        __syncthreads();
-        uint32_t before = to - sum, total = 0;
+        uint32_t above = ev_scan<T>(sum, &unused, tmp, at);
 #pragma unroll
-        for (int i = 0; i < W; i++) {
-            const uint32_t x = cnt[at][0][i];
-            if (i < (int)wv) before += x;
-            total += x;
-        }
-#pragma unroll
-        for (int i = 0; i < (U * W + T - 1) / T; i++) {
-            const uint32_t j = t * ((U * W + T - 1) / T) + i;
-            if (j < spans) marks[j] = before;
-            before += v[i];
-        }
-        if (t == 0) all = total;
-        at ^= 1;
-        __syncthreads();
-    };
-    if (ties != UINT32_MAX) scan();
-    uint64_t kept = 0, mark = 0;        // a bit a slot of the thread
-    EV_EACH(i, bool k = i * T + t < len && key[i] >= border;
-            if (ties != UINT32_MAX) {
-                const uint64_t b = __builtin_amdgcn_ballot_w64(i * T + t < len && key[i] == border);
-                if (key[i] == border) k = k && marks[i * W + wv] + lanes_below(b) < ties;
+        for (uint32_t i = 0; i < PER; i++) {
+            if (above < left && above + v[i] >= left) {
+                pick[0] = EV_BINS - 1 - (t * PER + i);
+                pick[1] = above;
+                pick[2] = v[i];
             }
-            kept |= (uint64_t)k << i;
-            if (i * T + t < len) mark |= (uint64_t)((i * T + t < keep) != k) << i;)
-    __syncthreads();
-    EV_EACH(i, const uint64_t m = __builtin_amdgcn_ballot_w64(mark >> i & 1); if (l == 0) marks[i * W + wv] = (uint32_t)__popcll(m);)
-    __syncthreads();
-    scan();
-    const uint32_t moves = all / 2, most = ev_most(a.keep, cap);
-    EV_EACH(i, const uint32_t j = i * T + t;
-            const uint32_t r = marks[i * W + wv] + lanes_below(__builtin_amdgcn_ballot_w64(mark >> i & 1));
-            if (mark >> i & 1) {
-                const uint32_t x = j < keep ? r : r - moves;
-                if (w.n) (j < keep ? w.hole : w.mover)[(uint64_t)row * most + x] = j;
-                else few[j < keep ? 0 : 1][x] = j;
-            } else if (j < keep) {
+            above += v[i];
+        }
+        __syncthreads();
+        border |= pick[0] << shift;
+        left -= pick[1];
+        here = pick[2];
+    }
+    // Keys above the border stay and all of its own, or its own up to slot `tie`. A pass that was not needed left
+    // lower bits 0.
+    uint32_t tie = UINT32_MAX;
+    if (left != here) {
+        uint32_t seen = 0;
+        for (uint32_t i0 = 0; i0 < spans; i0 += T) {
+            for (uint32_t i = i0 + wv; i < min(i0 + T, spans); i += W) {
+                const uint32_t j = i * 64 + l;
+                const uint64_t m = __builtin_amdgcn_ballot_w64(j < len && key_of(min(j, len - 1)) == border);
+                if (l == 0) marks[i - i0] = (uint32_t)__popcll(m);
+            }
+            __syncthreads();
+            const uint32_t v = i0 + t < spans ? marks[t] : 0;
+            uint32_t all;
+            const uint32_t before = seen + ev_scan<T>(v, &all, tmp, at);
+            if (before < left && before + v >= left) { pick[0] = i0 + t; pick[1] = before; }
+            seen += all;
+            __syncthreads();
+            if (seen >= left) break;
+        }
+        const uint32_t j = pick[0] * 64 + l;
+        const bool mine = j < len && key_of(min(j, len - 1)) == border;
+        const uint64_t m = __builtin_amdgcn_ballot_w64(mine);
+        tie = pick[0] * 64 + (uint32_t)__builtin_ctzll(__builtin_amdgcn_ballot_w64(mine && pick[1] + lanes_below(m) + 1 == left));
+    }
+    auto marked = [&](uint32_t j) {
+        const uint32_t key = key_of(min(j, len - 1));
+        return j < len && (j < keep) != (key > border || (key == border && j <= tie));
+    };
+    // the marks of each 64 slots, and all of them
+    uint32_t moves = 0;
+    for (uint32_t i0 = 0; i0 < spans; i0 += T) {
+        __syncthreads();
+        for (uint32_t i = i0 + wv; i < min(i0 + T, spans); i += W) {
+            const uint64_t m = __builtin_amdgcn_ballot_w64(marked(i * 64 + l));
+            if (l == 0) marks[i - i0] = (uint32_t)__popcll(m);
+        }
+        __syncthreads();
+        uint32_t all;
+        const uint32_t before = ev_scan<T>(i0 + t < spans ? marks[t] : 0, &all, tmp, at);
+        if (spans <= T) {
+            __syncthreads();
+            marks[t] = before;
+        }
+        moves += all;
+    }
+    moves /= 2;
+    uint32_t *const holes = w.n ? w.hole + row * ev_most(a.keep, cap) : few[0], *const movers = w.n ? w.mover + row * ev_most(a.keep, cap) : few[1];
+    uint32_t seen = 0;
+    for (uint32_t i0 = 0; i0 < spans; i0 += T) {
+        __syncthreads();
+        if (spans > T) {        // again, a part of them at a time
+            for (uint32_t i = i0 + wv; i < min(i0 + T, spans); i += W) {
+                const uint64_t m = __builtin_amdgcn_ballot_w64(marked(i * 64 + l));
+                if (l == 0) marks[i - i0] = (uint32_t)__popcll(m);
+            }
+            __syncthreads();
+            uint32_t all;
+            const uint32_t before = seen + ev_scan<T>(i0 + t < spans ? marks[t] : 0, &all, tmp, at);
+            __syncthreads();
+            marks[t] = before;
+            seen += all;
+            __syncthreads();
+        }
+        for (uint32_t i = i0 + wv; i < min(i0 + T, spans); i += W) {
+            const uint32_t j = i * 64 + l;
+            const bool m = marked(j);
+            const uint32_t r = marks[i - i0] + lanes_below(__builtin_amdgcn_ballot_w64(m));
+            if (m) *(j < keep ? holes + r : movers + (r - moves)) = j;
+            else if (!w.n && j < keep) {
                 if (wo != wt) wo[j] = wt[j];
                 if (po != ps) po[j] = ps[j];
-            })
-#undef EV_EACH
+            }
+        }
+    }
     if (w.n) {
         if (t == 0) w.n[row] = moves;
         return;
@@ -679,78 +731,6 @@ __global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list
     const uint32_t units = a.c.hd / 8;
     for (uint32_t i = t; i < moves * units; i += T) ev_move(a, s, h, few[1][i / units], few[0][i / units], i % units, units);
 }
-
-// Any number of slots: the keys by their digits, 8 bits a pass over the slots, which are read again each time.
-#define EV_THREADS 1024
-// exclusive prefix sum over the workgroup, and the total
-__device__ __forceinline__ uint32_t ev_scan(uint32_t v, uint32_t *total, uint32_t *tmp) {
-    const uint32_t t = threadIdx.x, x = wave_scan(v);
-    __syncthreads();
-    if ((t & 63) == 63) tmp[t >> 6] = x;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (uint32_t i = 0; i < EV_THREADS / 64; i++) {
-        if (i < t >> 6) before += tmp[i];
-        all += tmp[i];
-    }
-    *total = all;
-    return before + x - v;
-}
-__global__ void __launch_bounds__(EV_THREADS) k_page_evict_long(sgk_page_evict_args a, ev_list w) {
-    __shared__ uint32_t hist[256], tmp[EV_THREADS / 64], pick[2];
-    __shared__ int32_t lastp[EV_THREADS / 64];
-    const uint32_t t = threadIdx.x, h = blockIdx.x, s = blockIdx.y, len = page_len(a.c, a.lens, s);
-    const uint64_t cap = (uint64_t)a.c.width << a.c.log, row = (uint64_t)s * a.c.n_kv + h;
-    const float *wt = a.weight + row * cap;
-    const int32_t *ps = a.pos + row * cap;
-    const uint32_t keep = min(a.keep, len), most = ev_most(a.keep, (uint32_t)cap);
-    if (a.weight_out != a.weight) for (uint32_t j = t; j < keep; j += EV_THREADS) a.weight_out[row * cap + j] = wt[j];
-    if (a.pos_out != a.pos) for (uint32_t j = t; j < keep; j += EV_THREADS) a.pos_out[row * cap + j] = ps[j];
-    if (t == 0) w.n[row] = 0;
-    if (len <= a.keep) return;
-    int32_t last = INT32_MIN;
-    for (uint32_t j = t; j < len; j += EV_THREADS) last = max(last, ps[j]);
-    last = (int32_t)(wave_umax((uint32_t)last ^ 0x80000000u) ^ 0x80000000u);
-    if ((t & 63) == 0) lastp[t >> 6] = last;
-    __syncthreads();
-    for (uint32_t i = 0; i < EV_THREADS / 64; i++) last = max(last, lastp[i]);
-    const int64_t after = (int64_t)last - a.recent;
-    uint32_t prefix = 0, left = keep;           // of slots with the prefix, `left` stay
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (t < 256) hist[t] = 0;
-        __syncthreads();
-        for (uint32_t j = t; j < len; j += EV_THREADS) {
-            const uint32_t key = ev_key(wt[j], ps[j], after);
-            if (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[key >> shift & 255], 1u);
-        }
-        __syncthreads();
-        if (t == 0) {
-            uint32_t b = 255;
-            while (hist[b] < left) left -= hist[b--];
-            pick[0] = prefix | b << shift;
-            pick[1] = left;
-        }
-        __syncthreads();
-        prefix = pick[0];
-        left = pick[1];
-    }
-    // prefix is the keep-th key; `left` of its slots stay, the lowest
-    uint32_t ties = 0, holes = 0, movers = 0;
-    for (uint32_t j0 = 0; j0 < len; j0 += EV_THREADS) {
-        const uint32_t j = j0 + t, key = j < len ? ev_key(wt[j], ps[j], after) : 0;
-        uint32_t n;
-        const uint32_t tie = j < len && key == prefix, rank = ties + ev_scan(tie, &n, tmp);
-        ties += n;
-        const bool kept = j < len && (key > prefix || (tie && rank < left));
-        const uint32_t hole = j < keep && !kept, hr = holes + ev_scan(hole, &n, tmp);
-        holes += n;
-        const uint32_t mover = j >= keep && kept, mr = movers + ev_scan(mover, &n, tmp);
-        movers += n;
-        if (hole) w.hole[row * most + hr] = j;
-        if (mover) w.mover[row * most + mr] = j;
-    }
-    if (t == 0) w.n[row] = holes;
-}
 __global__ void __launch_bounds__(TPB) k_page_evict_move(sgk_page_evict_args a, ev_list w) {
     const uint32_t h = blockIdx.y, s = blockIdx.z, units = a.c.hd / 8, most = ev_most(a.keep, a.c.width << a.c.log);
     const uint64_t row = (uint64_t)s * a.c.n_kv + h, n = (uint64_t)w.n[row] * units;
@@ -758,24 +738,26 @@ __global__ void __launch_bounds__(TPB) k_page_evict_move(sgk_page_evict_args a, 
         ev_move(a, s, h, w.mover[row * most + i / units], w.hole[row * most + i / units], (uint32_t)(i % units), units);
 }
 extern "C" uint64_t sgk_page_evict_scratch(const sgk_page_evict_args *a) {
-    const uint32_t cap = a->c.width << a->c.log, most = ev_most(a->keep, cap);
-    return cap <= 65536 && most <= EV_FEW ? 0 : 4 * (uint64_t)a->c.n_seq * a->c.n_kv * (2 * (uint64_t)most + 1);
+    const uint32_t most = ev_most(a->keep, a->c.width << a->c.log);
+    return most <= EV_FEW ? 0 : 4 * (uint64_t)a->c.n_seq * a->c.n_kv * (2 * (uint64_t)most + 1);
 }
 extern "C" hipError_t sgk_page_evict(const sgk_page_evict_args *a, void *scratch, hipStream_t s, hipEvent_t done) {
     const uint32_t cap = a->c.width << a->c.log, most = ev_most(a->keep, cap);
     const uint64_t rows = (uint64_t)a->c.n_seq * a->c.n_kv, each = rows * most;
-    const bool few = cap <= 65536 && most <= EV_FEW;
+    const bool few = most <= EV_FEW;
     uint32_t *u = (uint32_t *)scratch;
     const ev_list w = {few ? NULL : u, few ? NULL : u + each, few ? NULL : u + 2 * each};
-    const dim3 grid(a->c.n_kv, a->c.n_seq);
-    const hipEvent_t ev = few ? done : (hipEvent_t)NULL;
-    if (cap <= 4096) launch(k_page_evict<256, 16, 2>, grid, 256, s, ev, *a, w);
-    else if (cap <= 16384) launch(k_page_evict<1024, 16, 1>, grid, 1024, s, ev, *a, w);
-    else if (cap <= 65536) launch(k_page_evict<1024, 64, 1>, grid, 1024, s, ev, *a, w);
-    else launch(k_page_evict_long, grid, EV_THREADS, s, ev, *a, w);
+    const bool small = cap <= 4096, held = cap <= EV_HELD;
+    void (*const k)(sgk_page_evict_args, ev_list) = small ? k_page_evict<256, true> : held ? k_page_evict<1024, true> : k_page_evict<1024, false>;
+    const uint32_t lds = held ? cap * 4 : 0;
+    if (lds > 49152) {
+        const hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    launch_lds(k, dim3(a->c.n_kv, a->c.n_seq), small ? 256 : 1024, lds, s, few ? done : (hipEvent_t)NULL, *a, w);
     if (!few) {
         const uint64_t b = ((uint64_t)most * (a->c.hd / 8) + TPB - 1) / TPB;
-        launch(k_page_evict_move, dim3((uint32_t)(b < 1 ? 1 : b < 256 ? b : 256), a->c.n_kv, a->c.n_seq), TPB, s, done, *a, w);
+        launch(k_page_evict_move, dim3((uint32_t)(b < 256 ? b : 256), a->c.n_kv, a->c.n_seq), TPB, s, done, *a, w);
     }
     return hipGetLastError();
 }
