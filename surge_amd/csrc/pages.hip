@@ -513,14 +513,15 @@ extern "C" hipError_t sgk_attn_paged(const sgk_attn_paged_args *a, void *scratch
 #define EV_FEW 64u          // rows that the selecting workgroup moves itself
 #define EV_HELD 32896u      // keys in LDS: 128 a page past 32768, so that a prompt's new slots fit too
 #define EV_BINS 2048u
+#define EV_OUT 16u          // rows too many that go one by one
 struct ev_list { uint32_t *hole, *mover, *n; };      // [row][most] twice, [row]: rows to move; NULL: the few are moved at once
 __host__ __device__ static inline uint32_t ev_most(uint32_t keep, uint32_t cap) { return keep < cap - keep ? keep : cap - keep; }
 
-// Rising with the order: 0xFFFFFFFF recent, 0 NaN.
-__device__ __forceinline__ uint32_t ev_key(float w, int32_t pos, int64_t after) {
+// Rising with the order: 0xFFFFFFFF recent, 0 NaN. last: the largest position, so that last - pos does not wrap.
+__device__ __forceinline__ uint32_t ev_key(float w, int32_t pos, int32_t last, uint32_t recent) {
     const uint32_t b = __float_as_uint(w + 0.0f);       // -0 as 0
-    const uint32_t key = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return (int64_t)pos > after ? 0xFFFFFFFFu : w != w ? 0u : key;
+    const uint32_t key = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+    return (uint32_t)last - (uint32_t)pos < recent ? 0xFFFFFFFFu : w != w ? 0u : key;
 }
 __device__ __forceinline__ uint32_t lanes_below(uint64_t b) {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
@@ -563,7 +564,9 @@ __global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list
     extern __shared__ uint32_t held[];
     __shared__ uint32_t bins[EV_BINS], tmp[2][16], marks[T], pick[3];
     __shared__ int32_t lasts[W];
-    __shared__ uint32_t few[2][EV_FEW];
+    __shared__ uint32_t few[2][EV_FEW], gone[EV_OUT];
+    __shared__ uint64_t out[2][W];
+    uint64_t dropped = 0;       // a bit a slot of the thread
     const uint32_t t = threadIdx.x, l = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), h = blockIdx.x, s = blockIdx.y;
     const uint32_t len = page_len(a.c, a.lens, s), cap = a.c.width << a.c.log, keep = min(a.keep, len);
     const uint64_t row = (uint64_t)s * a.c.n_kv + h;
@@ -572,12 +575,10 @@ __global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list
     float *wo = a.weight_out + row * cap;
     int32_t *po = a.pos_out + row * cap;
     if (t == 0 && w.n) w.n[row] = 0;
-    const bool stays = len <= a.keep;
-    if (stays || w.n) {         // all of the first `keep`; where a second launch moves rows, they come over these
-        if (wo != wt) for (uint32_t j = t; j < keep; j += T) wo[j] = wt[j];
-        if (po != ps) for (uint32_t j = t; j < keep; j += T) po[j] = ps[j];
-    }
-    if (stays) return;
+    // all of the first `keep`; moved rows come over them, behind a barrier or a launch
+    if (wo != wt) for (uint32_t j = t; j < keep; j += T) wo[j] = wt[j];
+    if (po != ps) for (uint32_t j = t; j < keep; j += T) po[j] = ps[j];
+    if (len <= a.keep) return;
     for (uint32_t i = t; i < EV_BINS; i += T) bins[i] = 0;
     int32_t last = INT32_MIN;
 #pragma unroll 8
@@ -591,13 +592,58 @@ __global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list
     __syncthreads();
 #pragma unroll
     for (uint32_t i = 0; i < W; i++) last = max(last, lasts[i]);
-    const int64_t after = (int64_t)last - a.recent;
     if (HELD) {
 #pragma unroll 8
-        for (uint32_t j = t; j < len; j += T) held[j] = ev_key(wt[j], (int32_t)held[j], after);     // a thread's own
+        for (uint32_t j = t; j < len; j += T) held[j] = ev_key(wt[j], (int32_t)held[j], last, a.recent);     // a thread's own
         __syncthreads();
     }
-    auto key_of = [&](uint32_t j) { return HELD ? held[j] : ev_key(wt[j], ps[j], after); };
+    auto key_of = [&](uint32_t j) { return HELD ? held[j] : ev_key(wt[j], ps[j], last, a.recent); };
+    uint32_t moves = 0;
+    uint32_t *const holes = w.n ? w.hole + row * ev_most(a.keep, cap) : few[0], *const movers = w.n ? w.mover + row * ev_most(a.keep, cap) : few[1];
+    if (HELD && len - keep <= EV_OUT) {
+        // few rows too many, as in a cache that is held at `keep`: the lowest one (of alike keys the highest slot) out at a
+        // time. A thread has the lowest of its slots in hand and looks again only when that one went.
+        auto lowest = [&]() {
+            uint64_t m = ~0ull;
+            for (uint32_t j = t; j < len; j += T) m = min(m, (uint64_t)held[j] << 32 | (uint32_t)~j);
+            return m;
+        };
+        uint64_t mine = lowest();
+        for (uint32_t i = 0; i < len - keep; i++) {
+            uint64_t m = mine;
+            for (int d = 1; d < 64; d <<= 1) m = min(m, (uint64_t)__shfl_xor(m, d));
+            if (l == 0) out[i & 1][wv] = m;
+            __syncthreads();
+#pragma unroll
+            for (uint32_t v = 0; v < W; v++) m = min(m, out[i & 1][v]);
+            const uint32_t j = ~(uint32_t)m;
+            if (t == 0) gone[i] = j;
+            if (j % T == t) {               // its own slot, in no other thread's hands
+                dropped |= 1ull << j / T;
+                mine = ~0ull;
+                for (uint32_t x = t; x < len; x += T)
+                    if (!(dropped >> x / T & 1)) mine = min(mine, (uint64_t)held[x] << 32 | (uint32_t)~x);
+            }
+        }
+        __syncthreads();
+        // their places below keep in rising order, and the slots from keep on that stay
+        if (t < 64) {
+            const uint32_t n = len - keep, g = t < n ? gone[t] : UINT32_MAX, x = keep + t;
+            uint32_t below = 0;
+            bool stays = t < n;
+            for (uint32_t i = 0; i < n; i++) {
+                const uint32_t o = gone[i];
+                below += o < g;
+                stays = stays && o != x;
+            }
+            if (g < keep) holes[below] = g;
+            const uint64_t m = __builtin_amdgcn_ballot_w64(stays);
+            if (stays) movers[lanes_below(m)] = x;
+            if (t == 0) pick[0] = (uint32_t)__popcll(m);
+        }
+        __syncthreads();
+        moves = pick[0];
+    } else {
     const uint32_t spans = (len + 63) / 64;
     // the keep-th key: `left` of the `here` keys with the border's upper bits stay
     uint32_t border = 0, left = keep, here = len;
@@ -678,7 +724,6 @@ __global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list
         return j < len && (j < keep) != (key > border || (key == border && j <= tie));
     };
     // the marks of each 64 slots, and all of them
-    uint32_t moves = 0;
     for (uint32_t i0 = 0; i0 < spans; i0 += T) {
         __syncthreads();
         for (uint32_t i = i0 + wv; i < min(i0 + T, spans); i += W) {
@@ -695,7 +740,6 @@ __global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list
         moves += all;
     }
     moves /= 2;
-    uint32_t *const holes = w.n ? w.hole + row * ev_most(a.keep, cap) : few[0], *const movers = w.n ? w.mover + row * ev_most(a.keep, cap) : few[1];
     uint32_t seen = 0;
     for (uint32_t i0 = 0; i0 < spans; i0 += T) {
         __syncthreads();
@@ -717,11 +761,8 @@ __global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list
             const bool m = marked(j);
             const uint32_t r = marks[i - i0] + lanes_below(__builtin_amdgcn_ballot_w64(m));
             if (m) *(j < keep ? holes + r : movers + (r - moves)) = j;
-            else if (!w.n && j < keep) {
-                if (wo != wt) wo[j] = wt[j];
-                if (po != ps) po[j] = ps[j];
-            }
         }
+    }
     }
     if (w.n) {
         if (t == 0) w.n[row] = moves;
