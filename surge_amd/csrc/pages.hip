@@ -512,8 +512,9 @@ extern "C" hipError_t sgk_attn_paged(const sgk_attn_paged_args *a, void *scratch
 // ---------------------------------------------------------------------------
 #define EV_FEW 64u          // rows that the selecting workgroup moves itself
 #define EV_HELD 32896u      // keys in LDS: 128 a page past 32768, so that a prompt's new slots fit too
+#define EV_THREADS 1024
 #define EV_BINS 2048u
-#define EV_OUT 16u          // rows too many that go one by one
+#define EV_OUT 8u          // rows too many that go one by one
 struct ev_list { uint32_t *hole, *mover, *n; };      // [row][most] twice, [row]: rows to move; NULL: the few are moved at once
 __host__ __device__ static inline uint32_t ev_most(uint32_t keep, uint32_t cap) { return keep < cap - keep ? keep : cap - keep; }
 
@@ -525,6 +526,15 @@ __device__ __forceinline__ uint32_t ev_key(float w, int32_t pos, int32_t last, u
 }
 __device__ __forceinline__ uint32_t lanes_below(uint64_t b) {
     return __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+}
+// The lowest of 16 lanes' values, in all of them.
+template <uint32_t (*F)(uint32_t)>
+__device__ __forceinline__ uint64_t both(uint64_t v) { return (uint64_t)F((uint32_t)(v >> 32)) << 32 | F((uint32_t)v); }
+__device__ __forceinline__ uint64_t row_min(uint64_t v) {
+    v = min(v, both<dppu<0xB1>>(v));
+    v = min(v, both<dppu<0x4E>>(v));
+    v = min(v, both<dppu<0x141>>(v));
+    return min(v, both<dppu<0x128>>(v));
 }
 // Row `from` to `to`: K and V by 16 bytes a thread, weight and pos with the first.
 __device__ __forceinline__ void ev_move(const sgk_page_evict_args &a, uint32_t s, uint32_t h, uint32_t from, uint32_t to, uint32_t u, uint32_t units) {
@@ -541,14 +551,13 @@ __device__ __forceinline__ void ev_move(const sgk_page_evict_args &a, uint32_t s
     ((u16x8 *)a.c.v)[yi] = vv;
 }
 // Over the workgroup: the exclusive prefix sum of v, and the total. tmp: [2][16], halves taken in turn.
-template <int T>
 __device__ __forceinline__ uint32_t ev_scan(uint32_t v, uint32_t *total, uint32_t (*tmp)[16], int &at) {
     const uint32_t to = wave_scan(v), wv = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 63) tmp[at][wv] = to;
     __syncthreads();
     uint32_t before = to - v, all = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < T / 64; i++) {
+    for (uint32_t i = 0; i < EV_THREADS / 64; i++) {
         const uint32_t x = tmp[at][i];
         if (i < wv) before += x;
         all += x;
@@ -558,14 +567,14 @@ __device__ __forceinline__ uint32_t ev_scan(uint32_t v, uint32_t *total, uint32_
     return before;
 }
 
-template <int T, bool HELD>
-__global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list w) {
-    constexpr uint32_t W = T / 64, PER = EV_BINS / T;
+template <bool HELD>
+__global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a, ev_list w) {
+    constexpr uint32_t T = EV_THREADS, W = T / 64, PER = EV_BINS / T;
     extern __shared__ uint32_t held[];
     __shared__ uint32_t bins[EV_BINS], tmp[2][16], marks[T], pick[3];
     __shared__ int32_t lasts[W];
     __shared__ uint32_t few[2][EV_FEW], gone[EV_OUT];
-    __shared__ uint64_t out[2][W];
+    __shared__ uint64_t out[2][16];
     uint64_t dropped = 0;       // a bit a slot of the thread
     const uint32_t t = threadIdx.x, l = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), h = blockIdx.x, s = blockIdx.y;
     const uint32_t len = page_len(a.c, a.lens, s), cap = a.c.width << a.c.log, keep = min(a.keep, len);
@@ -610,13 +619,12 @@ __global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list
         };
         uint64_t mine = lowest();
         for (uint32_t i = 0; i < len - keep; i++) {
-            uint64_t m = mine;
-            for (int d = 1; d < 64; d <<= 1) m = min(m, (uint64_t)__shfl_xor(m, d));
+            uint64_t m = row_min(mine);
+            m = min(m, both<swap16>(m));
+            m = min(m, both<swap32>(m));
             if (l == 0) out[i & 1][wv] = m;
             __syncthreads();
-#pragma unroll
-            for (uint32_t v = 0; v < W; v++) m = min(m, out[i & 1][v]);
-            const uint32_t j = ~(uint32_t)m;
+            const uint32_t j = ~(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)row_min(out[i & 1][l & 15]));
             if (t == 0) gone[i] = j;
             if (j % T == t) {               // its own slot, in no other thread's hands
                 dropped |= 1ull << j / T;
@@ -679,7 +687,7 @@ __global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list
             v[i] = bins[EV_BINS - 1 - (t * PER + i)];
             sum += v[i];
         }
-        uint32_t above = ev_scan<T>(sum, &unused, tmp, at);
+        uint32_t above = ev_scan(sum, &unused, tmp, at);
 #pragma unroll
         for (uint32_t i = 0; i < PER; i++) {
             if (above < left && above + v[i] >= left) {
@@ -708,7 +716,7 @@ __global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list
             __syncthreads();
             const uint32_t v = i0 + t < spans ? marks[t] : 0;
             uint32_t all;
-            const uint32_t before = seen + ev_scan<T>(v, &all, tmp, at);
+            const uint32_t before = seen + ev_scan(v, &all, tmp, at);
             if (before < left && before + v >= left) { pick[0] = i0 + t; pick[1] = before; }
             seen += all;
             __syncthreads();
@@ -732,7 +740,7 @@ __global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list
         }
         __syncthreads();
         uint32_t all;
-        const uint32_t before = ev_scan<T>(i0 + t < spans ? marks[t] : 0, &all, tmp, at);
+        const uint32_t before = ev_scan(i0 + t < spans ? marks[t] : 0, &all, tmp, at);
         if (spans <= T) {
             __syncthreads();
             marks[t] = before;
@@ -750,7 +758,7 @@ __global__ void __launch_bounds__(T) k_page_evict(sgk_page_evict_args a, ev_list
             }
             __syncthreads();
             uint32_t all;
-            const uint32_t before = seen + ev_scan<T>(i0 + t < spans ? marks[t] : 0, &all, tmp, at);
+            const uint32_t before = seen + ev_scan(i0 + t < spans ? marks[t] : 0, &all, tmp, at);
             __syncthreads();
             marks[t] = before;
             seen += all;
@@ -788,14 +796,14 @@ extern "C" hipError_t sgk_page_evict(const sgk_page_evict_args *a, void *scratch
     const bool few = most <= EV_FEW;
     uint32_t *u = (uint32_t *)scratch;
     const ev_list w = {few ? NULL : u, few ? NULL : u + each, few ? NULL : u + 2 * each};
-    const bool small = cap <= 4096, held = cap <= EV_HELD;
-    void (*const k)(sgk_page_evict_args, ev_list) = small ? k_page_evict<256, true> : held ? k_page_evict<1024, true> : k_page_evict<1024, false>;
+    const bool held = cap <= EV_HELD;
+    void (*const k)(sgk_page_evict_args, ev_list) = held ? k_page_evict<true> : k_page_evict<false>;
     const uint32_t lds = held ? cap * 4 : 0;
     if (lds > 49152) {
         const hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    launch_lds(k, dim3(a->c.n_kv, a->c.n_seq), small ? 256 : 1024, lds, s, few ? done : (hipEvent_t)NULL, *a, w);
+    launch_lds(k, dim3(a->c.n_kv, a->c.n_seq), EV_THREADS, lds, s, few ? done : (hipEvent_t)NULL, *a, w);
     if (!few) {
         const uint64_t b = ((uint64_t)most * (a->c.hd / 8) + TPB - 1) / TPB;
         launch(k_page_evict_move, dim3((uint32_t)(b < 256 ? b : 256), a->c.n_kv, a->c.n_seq), TPB, s, done, *a, w);
