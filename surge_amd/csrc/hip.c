@@ -1288,7 +1288,8 @@ sg_err sg_gpu_run_sample(sg_gpu *g, void *logits, void *settings, void *u, void 
     if (!sg_failed(e = push(bufs, 3)) && !sg_failed(e = push_out(token, (uint64_t)rows * 4)) &&
         (!probs || probs == logits || !sg_failed(e = push_out(probs, outs[2] ? size_of(logits) : lb)))) {
         const sgk_sample_args a = {DEV(logits), DEV(settings), DEV(u), DEV(token), DEV(probs), vocab, rows};
-        e = finish_done(g, sgk_sample(&a, g->stream, g->done), outs, 3);
+        void *t = NULL;
+        if (!sg_failed(e = scratch(g, sgk_sample_scratch(&a), &t))) e = finish_done(g, sgk_sample(&a, t, g->stream, g->done), outs, 3);
     }
     return back_to(g, was, e);
 }

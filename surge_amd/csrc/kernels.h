@@ -488,7 +488,9 @@ typedef struct {
     float *probs;               /* or NULL */
     uint32_t vocab, rows;
 } sgk_sample_args;
-hipError_t sgk_sample(const sgk_sample_args *a, hipStream_t s, hipEvent_t done);
+/* scratch: sgk_sample_scratch(a) bytes, 16-byte aligned. */
+uint64_t sgk_sample_scratch(const sgk_sample_args *a);
+hipError_t sgk_sample(const sgk_sample_args *a, void *scratch, hipStream_t s, hipEvent_t done);
 
 /* The device-resident workspace of the no-allocation entry points: a
  * file-scope device array of SGK_SCRATCH_BYTES in kernels.hip. Call

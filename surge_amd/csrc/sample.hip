@@ -8,17 +8,81 @@
 // An id's weight is exp((x - max) / temperature), in 64 bits. Sums of weights
 // are integers in units of the row's whole sum / 2^61 or so: whatever order the
 // additions come in, the sums, the kept ids and the token are the same.
-// A workgroup per row; the borders of top-k and top-p by the digits of the
-// logits' keys, 8 bits a pass over the row.
+//
+// A row is SM_IDS ids a workgroup, four a thread, over the chip, in four launches
+// that each need what all of the last one found. A row's settings are known on the
+// device alone, so each launch does for a row what its kind needs:
+//   few    top_k of SM_FEW at most (greedy: 1). The top_k-th largest of the waves'
+//          maxima (1) is a bound that at least top_k ids reach, and hardly more:
+//          those are listed (2), ranked by comparing all with all, and the token
+//          is found among them (3).
+//   all    no top_k, no top_p: the parts' sums (2), then the part in which the
+//          token lies finds it (3).
+//   border a histogram of the logits' distance from the largest, counts and sums
+//          (2), gives the bins in which top_k and top_p end; their ids are listed,
+//          the sums of the ids above them taken (3), and the list ranked for the
+//          exact borders (4).
+// A list that does not fit (thousands of ids alike at a border) leaves the row to
+// one workgroup, which goes over it digit by digit (4).
 // ---------------------------------------------------------------------------
-#define SM_THREADS 1024
+#define SM_THREADS 512
+#define SM_WAVES (SM_THREADS / 64)
+#define SM_IDS (4 * SM_THREADS)
+#define SM_PARTS 512u       // of a row, at most: its parts take several rounds of SM_IDS past that
+#define SM_FEW 128u
+#define SM_LIST 2048u
+#define SM_BINS 2048u
 #define SM_NONE 0xFFFFFFFFu
+
+// What the first launch found of a row: the largest and the lowest key, the ids that may be chosen, the weights' sum.
+struct sm_all { uint32_t best, low, ok; float top; double sum; };
+// Where top_k and top_p end: the bin of top_k's last id (SM_BINS: no top_k), ids and units before that bin; the bins in
+// which top_p may end (SM_BINS: no top_p) and the units before them; the first bin that is listed; all units.
+struct sm_border { uint32_t kbin, kabove, plo, phi, first; uint64_t ksum, psum, whole; };
+
+// A row's place in the scratch memory.
+struct sm_row {
+    uint32_t *wave, *low, *ok;          // [parts][SM_WAVES] largest keys, [parts] lowest, [parts] ids that may be chosen
+    double *sum;                        // [parts] of weights relative to the part's largest
+    uint64_t *kept, *list, *binsum;     // [parts] units that stay, [SM_LIST] key and ~id, [SM_BINS]
+    uint32_t *bincnt, *listed, *out;    // [SM_BINS], [1], [1 + 2 SM_FEW] few: number, ids, probabilities
+    struct sm_all *all;                 // what 1 found, by 2
+    struct sm_border *border;           // what 3 found
+};
+struct sm_plan { uint32_t parts, rounds; uint64_t row_bytes; char *at; };
+
+__device__ __forceinline__ sm_row sm_at(const sm_plan &p, uint32_t r) {
+    char *c = p.at + r * p.row_bytes;
+    sm_row w;
+    auto take = [&](uint64_t bytes) { char *x = c; c += (bytes + 15) / 16 * 16; return x; };
+    w.sum = (double *)take(8 * p.parts);
+    w.kept = (uint64_t *)take(8 * p.parts);
+    w.list = (uint64_t *)take(8 * SM_LIST);
+    w.binsum = (uint64_t *)take(8 * SM_BINS);
+    w.bincnt = (uint32_t *)take(4 * SM_BINS);
+    w.wave = (uint32_t *)take(4 * p.parts * SM_WAVES);
+    w.low = (uint32_t *)take(4 * p.parts);
+    w.ok = (uint32_t *)take(4 * p.parts);
+    w.listed = (uint32_t *)take(4);
+    w.out = (uint32_t *)take(4 * (1 + 2 * SM_FEW));
+    w.all = (sm_all *)take(sizeof(sm_all));
+    w.border = (sm_border *)take(sizeof(sm_border));
+    return w;
+}
+static uint64_t sm_row_bytes(uint64_t parts) {
+    uint64_t n = 0;
+    auto take = [&](uint64_t bytes) { n += (bytes + 15) / 16 * 16; };
+    take(8 * parts); take(8 * parts); take(8 * SM_LIST); take(8 * SM_BINS); take(4 * SM_BINS);
+    take(4 * parts * SM_WAVES); take(4 * parts); take(4 * parts); take(4); take(4 * (1 + 2 * SM_FEW)); take(sizeof(sm_all)); take(sizeof(sm_border));
+    return n;
+}
 
 // Rising with x; 0 for what is never chosen (NaN, -inf).
 __device__ __forceinline__ uint32_t sm_key(float x) {
     const uint32_t b = __float_as_uint(x + 0.0f);       // -0 as 0
     return x > -INFINITY ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0;
 }
+__device__ __forceinline__ float sm_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 __device__ __forceinline__ double sm_weight(float x, float top, double inv) {
     return x == top ? 1.0 : x > -INFINITY ? exp(((double)x - (double)top) * inv) : 0.0;
 }
@@ -30,7 +94,8 @@ __device__ __forceinline__ T sm_sum(T v, T *tmp) {
     if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
     __syncthreads();
     T r = 0;
-    for (int i = 0; i < SM_THREADS / 64; i++) r += tmp[i];
+#pragma unroll
+    for (int i = 0; i < SM_WAVES; i++) r += tmp[i];
     return r;
 }
 template <typename T>
@@ -45,7 +110,8 @@ __device__ __forceinline__ T sm_scan(T v, T *total, T *tmp) {      // exclusive
     if ((t & 63) == 63) tmp[t >> 6] = x;
     __syncthreads();
     T before = 0, all = 0;
-    for (uint32_t i = 0; i < SM_THREADS / 64; i++) {
+#pragma unroll
+    for (uint32_t i = 0; i < SM_WAVES; i++) {
         if (i < t >> 6) before += tmp[i];
         all += tmp[i];
     }
@@ -53,18 +119,503 @@ __device__ __forceinline__ T sm_scan(T v, T *total, T *tmp) {      // exclusive
     return before + x - v;
 }
 
-__global__ void __launch_bounds__(SM_THREADS) k_sample(sgk_sample_args a) {
-    __shared__ uint64_t hist[256], tmp[SM_THREADS / 64], pick[2];
-    __shared__ uint32_t tmp32[SM_THREADS / 64], token;
-    const uint32_t t = threadIdx.x, r = blockIdx.x, v = a.vocab;
-    const float *x = a.x + (uint64_t)r * v;
+struct sm_set { float temp, top_p, min_p, u; uint32_t top_k; double inv; bool few; };
+__device__ __forceinline__ sm_set sm_settings(const sgk_sample_args &a, const sm_plan &p, uint32_t r) {
     const uint32_t *set = a.settings + 4ull * r;
-    float temp = __uint_as_float(set[0]), top_p = __uint_as_float(set[2]);
-    uint32_t top_k = set[1];
-    const float min_p = __uint_as_float(set[3]);
-    float u = a.u[r];
-    u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
-    if (!(temp > 0.0f)) { temp = 1.0f; top_k = 1; }
+    sm_set s = {__uint_as_float(set[0]), __uint_as_float(set[2]), __uint_as_float(set[3]), a.u[r], set[1]};
+    s.u = s.u > 0.0f ? fminf(s.u, 0x1.fffffep-1f) : 0.0f;
+    if (!(s.temp > 0.0f)) { s.temp = 1.0f; s.top_k = 1; }
+    if (!(s.top_p < 1.0f)) s.top_p = 1.0f;
+    if (!(s.min_p > 0.0f)) s.min_p = 0.0f;
+    s.inv = 1.0 / (double)s.temp;
+    s.few = s.top_k && s.top_k <= SM_FEW && s.top_k <= p.parts * SM_WAVES;
+    return s;
+}
+// Four ids of round m of a part: their first, and their logits (NaN behind the last).
+__device__ __forceinline__ uint32_t sm_load(const sgk_sample_args &a, const sm_plan &p, uint32_t r, uint32_t part, uint32_t m, int al, float (&x)[4]) {
+    const uint64_t i = ((uint64_t)part * p.rounds + m) * SM_IDS + 4 * threadIdx.x;
+    const float *q = a.x + (uint64_t)r * a.vocab + i;
+    if (al && i < a.vocab) {
+        const f32x4 v = *(const f32x4 *)q;
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = v[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = i + e < a.vocab ? q[e] : NAN;
+    }
+    return (uint32_t)i;
+}
+__device__ __forceinline__ sm_all sm_read(const sm_row &w, const sm_plan &p, const sm_set &s, uint64_t *tmp) {
+    const uint32_t t = threadIdx.x;
+    uint32_t mine = 0, ok = 0, low = 0xFFFFFFFFu;
+    double sum = 0.0;
+    if (t < p.parts) {
+#pragma unroll
+        for (uint32_t i = 0; i < SM_WAVES; i++) mine = max(mine, w.wave[t * SM_WAVES + i]);
+        ok = w.ok[t];
+        low = w.low[t];
+        if (!s.few) sum = w.sum[t];
+    }
+    uint32_t *red = (uint32_t *)tmp;
+    const uint32_t b = wave_umax(mine), lw = ~wave_umax(~low);
+    __syncthreads();
+    if ((t & 63) == 0) { red[t >> 6] = b; red[SM_WAVES + (t >> 6)] = lw; }
+    __syncthreads();
+    sm_all r = {};
+    r.low = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = 0; i < SM_WAVES; i++) { r.best = max(r.best, red[i]); r.low = min(r.low, red[SM_WAVES + i]); }
+    r.ok = sm_sum(ok, (uint32_t *)tmp);
+    r.top = sm_value(r.best);
+    if (!s.few) {
+        if (mine && mine != r.best) sum *= sm_weight(sm_value(mine), r.top, s.inv);
+        r.sum = sm_sum(mine ? sum : 0.0, (double *)tmp);
+    }
+    return r;
+}
+__device__ __forceinline__ double sm_unit(double sum) { return ldexp(1.0, 61 - ilogb(sum)); }
+
+// ---- 1: the parts' maxima and sums
+__global__ void __launch_bounds__(SM_THREADS) k_sample_parts(sgk_sample_args a, sm_plan p, int al) {
+    __shared__ uint64_t tmp[SM_WAVES];
+    __shared__ uint32_t red[2 * SM_WAVES];
+    const uint32_t t = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
+    const sm_row w = sm_at(p, r);
+    const sm_set s = sm_settings(a, p, r);
+    uint32_t best = 0, low = 0xFFFFFFFFu, ok = 0;
+    float x[4];
+    for (uint32_t m = 0; m < p.rounds; m++) {
+        sm_load(a, p, r, part, m, al, x);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint32_t key = sm_key(x[e]);
+            best = max(best, key);
+            low = min(low, key - 1);
+            ok += key != 0;
+        }
+    }
+    for (uint32_t i = part * SM_THREADS + t; i < SM_BINS && !s.few; i += p.parts * SM_THREADS) { w.bincnt[i] = 0; w.binsum[i] = 0; }
+    if (part == 0 && t == 0) { *w.listed = 0; w.out[0] = 0; }
+    best = wave_umax(best);
+    low = ~wave_umax(~low);
+    if ((t & 63) == 0) { w.wave[part * SM_WAVES + (t >> 6)] = best; red[t >> 6] = best; red[SM_WAVES + (t >> 6)] = low; }
+    ok = sm_sum(ok, (uint32_t *)tmp);
+#pragma unroll
+    for (int i = 0; i < SM_WAVES; i++) { best = max(best, red[i]); low = min(low, red[SM_WAVES + i]); }
+    if (t == 0) { w.ok[part] = ok; w.low[part] = ok ? low + 1 : 0xFFFFFFFFu; }
+    if (s.few) return;
+    double sum = 0.0;
+    const float top = sm_value(best);
+    for (uint32_t m = 0; m < p.rounds && best; m++) {
+        if (p.rounds > 1) sm_load(a, p, r, part, m, al, x);
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum += sm_weight(x[e], top, s.inv);
+    }
+    sum = sm_sum(sum, (double *)tmp);
+    if (t == 0) w.sum[part] = sum;
+}
+
+// The bins of the third kind: by distance from the largest logit, a range in which top_p ends whatever the logits are
+// (weights below exp(-40) of the largest do not add up to 2^-24 of it), or all of it if that is less.
+__device__ __forceinline__ float sm_bin_scale(const sm_set &s, const sm_all &all) {
+    const float span = fminf(fmaxf(40.0f * s.temp, 24.0f), all.top - sm_value(all.low));
+    return span > 0.0f && span < INFINITY ? (float)(SM_BINS - 2) / span : 0.0f;
+}
+__device__ __forceinline__ uint32_t sm_bin(float x, float top, float scale) {
+    return x == top ? 0 : (uint32_t)fminf((top - x) * scale, (float)(SM_BINS - 1));
+}
+// Appends the ids of a thread that `in` marks to the row's list.
+__device__ __forceinline__ void sm_append(const sm_row &w, const float (&x)[4], uint32_t i, uint32_t in) {
+    uint32_t n = __popc(in), to = n;
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint32_t y = __shfl_up(to, d);
+        if ((threadIdx.x & 63) >= d) to += y;
+    }
+    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)to, 63);
+    if (!all) return;
+    uint32_t base = 0;
+    if ((threadIdx.x & 63) == 0) base = atomicAdd(w.listed, all);
+    base = (uint32_t)__builtin_amdgcn_readfirstlane((int)base) + to - n;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (in >> e & 1) {
+            if (base < SM_LIST) w.list[base] = (uint64_t)sm_key(x[e]) << 32 | (uint32_t)~(i + e);
+            base++;
+        }
+}
+
+// ---- 2: the few listed, the parts' sums, or the histogram
+__global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, sm_plan p, int al) {
+    __shared__ uint64_t tmp[2 * SM_WAVES], sums[SM_BINS];
+    __shared__ uint32_t cnts[SM_BINS];
+    const uint32_t t = threadIdx.x, l = t & 63, part = blockIdx.x, r = blockIdx.y;
+    const sm_row w = sm_at(p, r);
+    const sm_set s = sm_settings(a, p, r);
+    float x[4];
+    uint32_t i = sm_load(a, p, r, part, 0, al, x);
+    const sm_all all = sm_read(w, p, s, tmp);
+    if (part == 0 && t == 0) *w.all = all;
+    if (!all.ok) return;
+    if (s.few) {
+        // a bound that at least top_k ids reach: the top_k-th of the waves' maxima, its upper bits (every wave by itself)
+        const uint32_t n = p.parts * SM_WAVES;
+        uint32_t bound = 0;
+        if (n <= 64 * 16) {
+            uint32_t c[16], least = 0xFFFFFFFFu;
+#pragma unroll
+            for (uint32_t j = 0; j < 16; j++) {
+                c[j] = j * 64 + l < n ? w.wave[j * 64 + l] : 0;
+                if (j * 64 + l < n) least = min(least, c[j]);
+            }
+            least = ~wave_umax(~least);
+            const uint32_t differ = all.best ^ least, high = differ ? 31 - __builtin_clz(differ) : 0;
+            bound = least & ~((2u << high) - 1);
+            for (int b = (int)high; b >= 0 && b > (int)high - 16; b--) {
+                uint32_t k = 0;
+#pragma unroll
+                for (uint32_t j = 0; j < 16; j++) {
+                    if (j % 4 == 0 && j * 64 >= n) break;
+                    k += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(c[j] >= (bound | 1u << b)));
+                }
+                if (k >= s.top_k) bound |= 1u << b;
+            }
+        } else {
+            for (int b = 31; b >= 12; b--) {
+                uint32_t k = 0;
+                for (uint32_t j = l; j < (n + 63) / 64 * 64; j += 64) k += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(j < n && w.wave[j] >= (bound | 1u << b)));
+                if (k >= s.top_k) bound |= 1u << b;
+            }
+        }
+        bound = max(bound, 1u);
+        for (uint32_t m = 0; m < p.rounds; m++) {
+            if (m) i = sm_load(a, p, r, part, m, al, x);
+            uint32_t in = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) in |= (uint32_t)(sm_key(x[e]) >= bound) << e;
+            sm_append(w, x, i, in);
+        }
+        return;
+    }
+    const double up = sm_unit(all.sum);
+    if ((!s.top_k || s.top_k >= all.ok) && s.top_p == 1.0f) {
+        uint64_t q = 0;
+        for (uint32_t m = 0; m < p.rounds; m++) {
+            if (m) sm_load(a, p, r, part, m, al, x);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const double y = sm_weight(x[e], all.top, s.inv);
+                if (y >= (double)s.min_p || x[e] == all.top) q += sm_units(y, up);
+            }
+        }
+        q = sm_sum(q, tmp);
+        if (t == 0) w.kept[part] = q;
+        return;
+    }
+    for (uint32_t j = t; j < SM_BINS; j += SM_THREADS) { cnts[j] = 0; sums[j] = 0; }
+    __syncthreads();
+    const float scale = sm_bin_scale(s, all);
+    for (uint32_t m = 0; m < p.rounds; m++) {
+        if (m) sm_load(a, p, r, part, m, al, x);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (x[e] > -INFINITY) {
+                const uint32_t b = sm_bin(x[e], all.top, scale);
+                atomicAdd(&cnts[b], 1u);
+                atomicAdd((unsigned long long *)&sums[b], (unsigned long long)sm_units(sm_weight(x[e], all.top, s.inv), up));
+            }
+    }
+    __syncthreads();
+    for (uint32_t j = t; j < SM_BINS; j += SM_THREADS)
+        if (cnts[j]) {
+            atomicAdd(w.bincnt + j, cnts[j]);
+            atomicAdd((unsigned long long *)w.binsum + j, (unsigned long long)sums[j]);
+        }
+}
+
+
+// ---- a list of ids in LDS: order (key, then ~id: the larger comes first), units, bin with SM_LOW if the weight is below min_p
+#define SM_LOW 0x80000000u
+struct sm_list { uint64_t order[SM_LIST], unit[SM_LIST]; uint32_t bin[SM_LIST], n; uint64_t border, ksum; };
+
+template <uint32_t (*F)(uint32_t)>
+__device__ __forceinline__ uint64_t sm_both(uint64_t v) { return (uint64_t)F((uint32_t)(v >> 32)) << 32 | F((uint32_t)v); }
+__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
+    v += sm_both<dppu<0xB1>>(v);
+    v += sm_both<dppu<0x4E>>(v);
+    v += sm_both<dppu<0x141>>(v);
+    v += sm_both<dppu<0x128>>(v);
+    v += sm_both<swap16>(v);
+    return v + sm_both<swap32>(v);
+}
+// Below, a wave over the list's entries j that in(j) takes.
+// The largest value V (32 bits) for which `before` and the units of the entries with val(j) >= V add up to `want`, the
+// lowest entry's if none does, but never above the highest's.
+template <typename In, typename Val>
+__device__ __forceinline__ uint32_t sm_top(const sm_list &s, uint64_t before, uint64_t want, In in, Val val) {
+    const uint32_t l = threadIdx.x & 63;
+    uint32_t lo = 0xFFFFFFFFu, hi = 0;
+    for (uint32_t j = l; j < s.n; j += 64)
+        if (in(j)) { lo = min(lo, val(j)); hi = max(hi, val(j)); }
+    lo = ~wave_umax(~lo);
+    hi = wave_umax(hi);
+    if (lo >= hi) return hi;
+    uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi), at = lo & ~(2 * bit - 1);
+    for (; bit; bit >>= 1) {
+        uint64_t sum = 0;
+        for (uint32_t j = l; j < s.n; j += 64)
+            if (in(j) && val(j) >= (at | bit)) sum += s.unit[j];
+        sum = wave_sum64(sum);
+        if (sum && before + sum >= want) at |= bit;
+    }
+    return max(at, lo);
+}
+// The order of the room-th entry.
+template <typename In>
+__device__ __forceinline__ uint64_t sm_nth(const sm_list &s, uint32_t room, In in) {
+    const uint32_t l = threadIdx.x & 63;
+    uint64_t at = 0;
+    for (int half = 0; half < 2; half++) {      // the key, then ~id among that key's
+        auto val = [&](uint32_t j) { return half ? (uint32_t)s.order[j] : (uint32_t)(s.order[j] >> 32); };
+        auto here = [&](uint32_t j) { return in(j) && (!half || s.order[j] >> 32 == at >> 32); };
+        uint32_t lo = 0xFFFFFFFFu, hi = 0;
+        for (uint32_t j = l; j < s.n; j += 64)
+            if (here(j)) { lo = min(lo, val(j)); hi = max(hi, val(j)); }
+        lo = ~wave_umax(~lo);
+        hi = wave_umax(hi);
+        uint32_t v = lo, from = UINT32_MAX;     // from: entries from v on
+        if (lo < hi) {
+            uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi);
+            v &= ~(2 * bit - 1);
+            for (; bit && from != room; bit >>= 1) {
+                uint32_t m = 0;
+                for (uint32_t j0 = 0; j0 < s.n; j0 += 64) m += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(j0 + l < s.n && here(j0 + l) && val(j0 + l) >= (v | bit)));
+                if (m >= room) { v |= bit; from = m; }
+            }
+        }
+        if (half) return at | v;
+        if (from == room) return (uint64_t)v << 32;
+        at = (uint64_t)v << 32;
+        for (uint32_t j0 = 0; j0 < s.n; j0 += 64) room -= (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(j0 + l < s.n && in(j0 + l) && (uint32_t)(s.order[j0 + l] >> 32) > v));
+    }
+    return at;
+}
+template <typename In>
+__device__ __forceinline__ uint32_t sm_count(const sm_list &s, In in) {
+    uint32_t m = 0;
+    for (uint32_t j0 = 0; j0 < s.n; j0 += 64) m += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(j0 + (threadIdx.x & 63) < s.n && in(j0 + (threadIdx.x & 63))));
+    return m;
+}
+template <typename In>
+__device__ __forceinline__ uint64_t sm_units_of(const sm_list &s, In in) {
+    uint64_t sum = 0;
+    for (uint32_t j = threadIdx.x & 63; j < s.n; j += 64)
+        if (in(j)) sum += s.unit[j];
+    return wave_sum64(sum);
+}
+// The list from memory, and the lowest order that stays under top_k and top_p; all threads. False: it does not fit.
+__device__ __forceinline__ bool sm_resolve(sm_list &s, const sm_row &w, const sm_set &set, const sm_all &all, const sm_border &b, double up, float scale) {
+    const uint32_t t = threadIdx.x;
+    const uint32_t n = *w.listed;
+    if (n > SM_LIST) return false;
+    for (uint32_t j = t; j < n; j += SM_THREADS) {
+        const uint64_t o = w.list[j];
+        const float x = sm_value((uint32_t)(o >> 32));
+        const double y = sm_weight(x, all.top, set.inv);
+        s.order[j] = o;
+        s.unit[j] = sm_units(y, up);
+        s.bin[j] = (set.few ? 0 : sm_bin(x, all.top, scale)) | (y >= (double)set.min_p || x == all.top ? 0 : SM_LOW);
+    }
+    if (t == 0) s.n = n;
+    __syncthreads();
+    if (t < 64) {
+        uint64_t border = 0, whole = b.whole;
+        if (b.kbin < SM_BINS) {
+            auto in = [&](uint32_t j) { return (s.bin[j] & ~SM_LOW) == b.kbin; };
+            if (sm_count(s, in) > set.top_k - b.kabove) border = sm_nth(s, set.top_k - b.kabove, in);
+            whole = b.ksum + sm_units_of(s, [&](uint32_t j) { return in(j) && s.order[j] >= border; });
+        }
+        if (b.plo < SM_BINS) {
+            const double want = (double)set.top_p * (double)whole;
+            const uint64_t units = want > 0.0 ? (uint64_t)ceil(want) : 0;
+            auto in = [&](uint32_t j) { const uint32_t x = s.bin[j] & ~SM_LOW; return x >= b.plo && x <= b.phi && s.order[j] >= border; };
+            const uint32_t key = sm_top(s, b.psum, units, in, [&](uint32_t j) { return (uint32_t)(s.order[j] >> 32); });
+            // of that key's ids, as many as it takes
+            auto same = [&](uint32_t j) { return in(j) && s.order[j] >> 32 == key; };
+            const uint64_t ahead = b.psum + sm_units_of(s, [&](uint32_t j) { return in(j) && s.order[j] >> 32 > key; });
+            const uint32_t ties = sm_count(s, same);
+            const uint64_t unit = sm_units(sm_weight(sm_value(key), all.top, set.inv), up);
+            const uint64_t room = units > ahead ? unit ? (units - ahead + unit - 1) / unit : ties : 1;
+            border = max(border, room < ties ? sm_nth(s, (uint32_t)room, same) : (uint64_t)key << 32);
+        }
+        if (t == 0) s.border = border;
+    }
+    __syncthreads();
+    return true;
+}
+
+// The token of a row's part in which the units pass `want` (counted from the part's start), and the part's probabilities.
+template <typename Stays>
+__device__ __forceinline__ void sm_pick(const sgk_sample_args &a, const sm_plan &p, uint32_t r, uint32_t part, int al, const sm_set &s, float top, double up,
+                                        double whole, bool here, uint64_t want, uint64_t *tmp, uint32_t *least, Stays stays) {
+    if (!here && !a.probs) return;
+    uint64_t before = 0;
+    if (threadIdx.x == 0) *least = SM_NONE;
+    for (uint32_t m = 0; m < p.rounds; m++) {
+        float x[4], out[4];
+        const uint32_t i = sm_load(a, p, r, part, m, al, x);
+        uint64_t q[4], mine = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const double y = sm_weight(x[e], top, s.inv);
+            const bool k = x[e] > -INFINITY && (y >= (double)s.min_p || x[e] == top) && stays(x[e], i + e);
+            q[e] = k ? sm_units(y, up) : 0;
+            out[e] = q[e] ? (float)(y * up / whole) : 0.0f;
+            mine += q[e];
+        }
+        if (here) {
+            uint64_t all, at = before + sm_scan(mine, &all, tmp);
+            before += all;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                at += q[e];
+                if (q[e] && at > want) { atomicMin(least, i + e); break; }
+            }
+        }
+        if (a.probs && i < a.vocab) {
+            float *d = a.probs + (uint64_t)r * a.vocab + i;
+            if (al) *(f32x4 *)d = (f32x4){out[0], out[1], out[2], out[3]};
+            else
+                for (int e = 0; e < 4; e++) if (i + e < a.vocab) d[e] = out[e];
+        }
+    }
+    if (!here) return;
+    __syncthreads();
+    if (threadIdx.x == 0) a.token[r] = *least;
+}
+
+// ---- 3
+__global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a, sm_plan p, int al) {
+    __shared__ uint64_t tmp[SM_WAVES];
+    __shared__ uint32_t least, tmp32[SM_WAVES];
+    __shared__ sm_border found;
+    __shared__ sm_list list;
+    const uint32_t t = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
+    const sm_row w = sm_at(p, r);
+    const sm_set s = sm_settings(a, p, r);
+    if (s.few && part) return;
+    const sm_all all = *w.all;
+    if (!all.ok) return;
+    if (s.few) {
+        const double up = 0x1p54;           // 2^7 ids at most
+        const sm_border b = {0, 0, s.top_p < 1.0f ? 0 : SM_BINS, 0, 0, 0, 0, 0};
+        if (!sm_resolve(list, w, s, all, b, up, 0.0f)) return;
+        auto in = [&](uint32_t j) { return list.order[j] >= list.border && !(list.bin[j] & SM_LOW); };
+        if (t >= 64) return;
+        const uint64_t whole = sm_units_of(list, in), want = (uint64_t)((double)s.u * (double)whole) + 1;
+        const uint32_t id = ~sm_top(list, 0, want, in, [&](uint32_t j) { return (uint32_t)list.order[j]; });
+        if (t == 0) a.token[r] = id;
+        if (!a.probs) return;
+        uint32_t n = 0;
+        for (uint32_t j0 = 0; j0 < list.n; j0 += 64) {
+            const uint32_t j = j0 + t;
+            const bool k = j < list.n && in(j);
+            const uint64_t m = __builtin_amdgcn_ballot_w64(k);
+            const uint32_t at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+            if (k && at < SM_FEW) {
+                w.out[1 + 2 * at] = ~(uint32_t)list.order[j];
+                w.out[2 + 2 * at] = __float_as_uint((float)(sm_weight(sm_value((uint32_t)(list.order[j] >> 32)), all.top, s.inv) * up / (double)whole));
+            }
+            n += (uint32_t)__popcll(m);
+        }
+        if (t == 0) w.out[0] = min(n, SM_FEW);
+        return;
+    }
+    const double up = sm_unit(all.sum);
+    const bool k_on = s.top_k && s.top_k < all.ok, p_on = s.top_p < 1.0f;
+    if (!k_on && !p_on) {
+        uint64_t whole;
+        const uint64_t mine = t < p.parts ? w.kept[t] : 0, before = sm_scan(mine, &whole, tmp), want = (uint64_t)((double)s.u * (double)whole);
+        if (t == part) { found.ksum = before; found.psum = mine; }
+        __syncthreads();
+        const bool here = want >= found.ksum && want < found.ksum + found.psum;
+        sm_pick(a, p, r, part, al, s, all.top, up, (double)whole, here, want - found.ksum, tmp, &least, [](float, uint32_t) { return true; });
+        return;
+    }
+    // the bins in which top_k and top_p end
+    constexpr uint32_t PER = SM_BINS / SM_THREADS;
+    const float scale = sm_bin_scale(s, all);
+    uint32_t cnt[PER], c = 0, nall;
+    uint64_t sum[PER], u = 0, whole;
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) {
+        cnt[i] = w.bincnt[t * PER + i];
+        sum[i] = w.binsum[t * PER + i];
+        c += cnt[i];
+        u += sum[i];
+    }
+    c = sm_scan(c, &nall, tmp32);
+    u = sm_scan(u, &whole, tmp);
+    if (t == 0) found = (sm_border){SM_BINS, 0, SM_BINS, SM_BINS, 0, 0, 0, whole};
+    __syncthreads();
+    uint64_t klo = whole, khi = whole;
+    if (k_on) {
+        uint32_t cc = c;
+        uint64_t uu = u;
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            if (cc < s.top_k && cc + cnt[i] >= s.top_k) { found.kbin = t * PER + i; found.kabove = cc; found.ksum = uu; found.psum = uu + sum[i]; }
+            cc += cnt[i];
+            uu += sum[i];
+        }
+        __syncthreads();
+        klo = found.ksum;
+        khi = found.psum;
+        __syncthreads();
+    }
+    if (p_on) {
+        const double dlo = ceil((double)s.top_p * (double)klo), dhi = ceil((double)s.top_p * (double)khi);
+        const uint64_t wlo = dlo > 1.0 ? (uint64_t)dlo : 1, whi = dhi > 1.0 ? (uint64_t)dhi : 1;
+        uint64_t uu = u;
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            if (uu < wlo && uu + sum[i] >= wlo) { found.plo = t * PER + i; found.psum = uu; }
+            if (uu < whi && uu + sum[i] >= whi) found.phi = t * PER + i;
+            uu += sum[i];
+        }
+        __syncthreads();
+    }
+    sm_border b = found;
+    if (p_on && b.kbin < SM_BINS) b.phi = min(b.phi, b.kbin);
+    b.first = p_on ? b.plo : b.kbin;
+    if (part == 0 && t == 0) *w.border = b;
+    uint64_t q = 0;
+    for (uint32_t m = 0; m < p.rounds; m++) {
+        float x[4];
+        const uint32_t i = sm_load(a, p, r, part, m, al, x);
+        uint32_t in = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (!(x[e] > -INFINITY)) continue;
+            const uint32_t y = sm_bin(x[e], all.top, scale);
+            if (y < b.first) {
+                const double z = sm_weight(x[e], all.top, s.inv);
+                if (z >= (double)s.min_p || x[e] == all.top) q += sm_units(z, up);
+            } else if (y == b.kbin || (p_on && y <= b.phi)) {
+                in |= 1u << e;
+            }
+        }
+        sm_append(w, x, i, in);
+    }
+    q = sm_sum(q, tmp);
+    if (t == 0) w.kept[part] = q;
+}
+
+// A row whose list does not fit: one workgroup, the borders of top_k and top_p by the digits of the keys, 8 bits a pass over the row.
+__device__ __noinline__ void sm_slow(const sgk_sample_args &a, uint32_t r, const sm_set &set, sm_list *room) {
+    uint64_t *const hist = room->order, *const tmp = hist + 256, *const pick = tmp + SM_WAVES;
+    uint32_t *const tmp32 = room->bin, &token = room->n;
+    const uint32_t t = threadIdx.x, v = a.vocab, top_k = set.top_k;
+    const float *x = a.x + (uint64_t)r * v, top_p = set.top_p, min_p = set.min_p, u = set.u;
     uint32_t best = 0, ok = 0;
     for (uint32_t i = t; i < v; i += SM_THREADS) {
         const uint32_t key = sm_key(x[i]);
@@ -74,17 +625,12 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample(sgk_sample_args a) {
     for (int d = 1; d < 64; d <<= 1) best = max(best, (uint32_t)__shfl_xor(best, d));
     if ((t & 63) == 0) tmp32[t >> 6] = best;
     __syncthreads();
-    for (int i = 0; i < SM_THREADS / 64; i++) best = max(best, tmp32[i]);
+    for (int i = 0; i < (int)SM_WAVES; i++) best = max(best, tmp32[i]);
     __syncthreads();
     ok = sm_sum(ok, tmp32);
     float *probs = a.probs ? a.probs + (uint64_t)r * v : NULL;
-    if (!ok) {
-        if (t == 0) a.token[r] = SM_NONE;
-        if (probs) for (uint32_t i = t; i < v; i += SM_THREADS) probs[i] = 0.0f;
-        return;
-    }
     const float top = __uint_as_float(best & 0x80000000u ? best ^ 0x80000000u : ~best);
-    const double inv = 1.0 / (double)temp;
+    const double inv = set.inv;
     // top-k: the last key that stays, and how many of its ids
     uint32_t border = 0, ties = SM_NONE;
     if (top_k && top_k < ok) {
@@ -191,7 +737,95 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample(sgk_sample_args a) {
     __syncthreads();
     if (t == 0) a.token[r] = token;
 }
-extern "C" hipError_t sgk_sample(const sgk_sample_args *a, hipStream_t s, hipEvent_t done) {
-    launch(k_sample, dim3(a->rows), SM_THREADS, s, done, *a);
+// ---- 4
+__global__ void __launch_bounds__(SM_THREADS) k_sample_last(sgk_sample_args a, sm_plan p, int al) {
+    __shared__ uint64_t tmp[SM_WAVES];
+    __shared__ uint32_t least;
+    __shared__ sm_list list;
+    const uint32_t t = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
+    const sm_row w = sm_at(p, r);
+    const sm_set s = sm_settings(a, p, r);
+    const sm_all all = *w.all;
+    const bool zero = !all.ok || s.few;
+    if (!all.ok && part == 0 && t == 0) a.token[r] = SM_NONE;
+    const bool k_on = s.top_k && s.top_k < all.ok, p_on = s.top_p < 1.0f;
+    if (all.ok && (s.few || k_on || p_on) && *w.listed > SM_LIST) {
+        if (part == 0) sm_slow(a, r, s, &list);
+        return;
+    }
+    if (zero) {
+        if (!a.probs) return;
+        for (uint32_t m = 0; m < p.rounds; m++) {
+            const uint64_t i0 = ((uint64_t)part * p.rounds + m) * SM_IDS;
+            for (uint32_t e = t; e < SM_IDS && i0 + e < a.vocab; e += SM_THREADS) a.probs[(uint64_t)r * a.vocab + i0 + e] = 0.0f;
+        }
+        __syncthreads();
+        if (all.ok && t < w.out[0]) {
+            const uint32_t id = w.out[1 + 2 * t];
+            if (id / (SM_IDS * p.rounds) == part) a.probs[(uint64_t)r * a.vocab + id] = __uint_as_float(w.out[2 + 2 * t]);
+        }
+        return;
+    }
+    if (!k_on && !p_on) return;
+    const double up = sm_unit(all.sum);
+    const sm_border b = *w.border;
+    const float scale = sm_bin_scale(s, all);
+    sm_resolve(list, w, s, all, b, up, scale);
+    // the units that stay: above the listed bins by parts, and the list's
+    const uint32_t i0 = part * p.rounds * SM_IDS, i1 = i0 + p.rounds * SM_IDS;
+    uint64_t whole = 0, before = 0, mine = 0;
+    if (t < p.parts) {
+        const uint64_t q = w.kept[t];
+        whole = q;
+        if (t < part) before = q;
+        if (t == part) mine = q;
+    }
+    for (uint32_t j = t; j < list.n; j += SM_THREADS)
+        if (list.order[j] >= list.border && !(list.bin[j] & SM_LOW)) {
+            const uint32_t id = ~(uint32_t)list.order[j];
+            whole += list.unit[j];
+            if (id < i0) before += list.unit[j];
+            else if (id < i1) mine += list.unit[j];
+        }
+    whole = sm_sum(whole, tmp);
+    before = sm_sum(before, tmp);
+    mine = sm_sum(mine, tmp);
+    const uint64_t want = (uint64_t)((double)s.u * (double)whole), border = list.border;
+    sm_pick(a, p, r, part, al, s, all.top, up, (double)whole, want >= before && want < before + mine, want - before, tmp, &least,
+            [&](float x, uint32_t i) {
+                const uint32_t y = sm_bin(x, all.top, scale);
+                return y < b.first || ((y == b.kbin || (p_on && y <= b.phi)) && ((uint64_t)sm_key(x) << 32 | (uint32_t)~i) >= border);
+            });
+}
+
+static sm_plan sm_plan_of(uint32_t vocab, void *at) {
+    sm_plan p;
+    const uint64_t chunks = ((uint64_t)vocab + SM_IDS - 1) / SM_IDS;
+    p.rounds = (uint32_t)((chunks + SM_PARTS - 1) / SM_PARTS);
+    p.parts = (uint32_t)((chunks + p.rounds - 1) / p.rounds);
+    p.row_bytes = sm_row_bytes(p.parts);
+    p.at = (char *)at;
+    return p;
+}
+// Rows go by SM_ROWS at a time, so that the scratch memory has an end.
+#define SM_ROWS 1024u
+extern "C" uint64_t sgk_sample_scratch(const sgk_sample_args *a) { return sm_plan_of(a->vocab, NULL).row_bytes * min(a->rows, SM_ROWS); }
+extern "C" hipError_t sgk_sample(const sgk_sample_args *a, void *scratch, hipStream_t s, hipEvent_t done) {
+    const sm_plan p = sm_plan_of(a->vocab, scratch);
+    const int al = !(((uintptr_t)a->x | (uintptr_t)a->probs) & 15) && a->vocab % 4 == 0;
+    for (uint32_t r = 0; r < a->rows; r += SM_ROWS) {
+        sgk_sample_args b = *a;
+        b.x += (uint64_t)r * a->vocab;
+        b.settings += 4ull * r;
+        b.u += r;
+        b.token += r;
+        if (b.probs) b.probs += (uint64_t)r * a->vocab;
+        b.rows = min(a->rows - r, SM_ROWS);
+        const dim3 grid(p.parts, b.rows);
+        launch(k_sample_parts, grid, SM_THREADS, s, (hipEvent_t)NULL, b, p, al);
+        launch(k_sample_count, grid, SM_THREADS, s, (hipEvent_t)NULL, b, p, al);
+        launch(k_sample_border, grid, SM_THREADS, s, (hipEvent_t)NULL, b, p, al);
+        launch(k_sample_last, grid, SM_THREADS, s, r + SM_ROWS < a->rows ? (hipEvent_t)NULL : done, b, p, al);
+    }
     return hipGetLastError();
 }
