@@ -63,6 +63,53 @@ __device__ __forceinline__ float wave_fsum(float v) {
     return v + swap32f(v);
 }
 
+// 64-bit values of partner lanes, and their sum and lowest over the wave or a row of 16.
+template <uint32_t (*F)(uint32_t)>
+__device__ __forceinline__ uint64_t both(uint64_t v) { return (uint64_t)F((uint32_t)(v >> 32)) << 32 | F((uint32_t)v); }
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
+    v += both<dppu<0xB1>>(v);
+    v += both<dppu<0x4E>>(v);
+    v += both<dppu<0x141>>(v);
+    v += both<dppu<0x128>>(v);
+    v += both<swap16>(v);
+    return v + both<swap32>(v);
+}
+__device__ __forceinline__ uint64_t row_min(uint64_t v) {
+    v = min(v, both<dppu<0xB1>>(v));
+    v = min(v, both<dppu<0x4E>>(v));
+    v = min(v, both<dppu<0x141>>(v));
+    return min(v, both<dppu<0x128>>(v));
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+    v += dppu<0xB1>(v);
+    v += dppu<0x4E>(v);
+    v += dppu<0x141>(v);
+    v += dppu<0x128>(v);
+    v += swap16(v);
+    return v + swap32(v);
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#define WS_STEP(F) v += __longlong_as_double((long long)both<F>((uint64_t)__double_as_longlong(v)))
+    WS_STEP(dppu<0xB1>); WS_STEP(dppu<0x4E>); WS_STEP(dppu<0x141>); WS_STEP(dppu<0x128>); WS_STEP(swap16); WS_STEP(swap32);
+#undef WS_STEP
+    return v;
+}
+// Inclusive prefix sums over the wave: within the rows of 16, then the rows' ends carried on.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_0(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true); }
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+#define WS_STEP(CTRL, ROWS) if constexpr (sizeof(T) == 8) v += both<dpp_or_0<CTRL, ROWS>>(v); else v += dpp_or_0<CTRL, ROWS>(v)
+    WS_STEP(0x111, 0xF); WS_STEP(0x112, 0xF); WS_STEP(0x114, 0xF); WS_STEP(0x118, 0xF);     // row_shr 1, 2, 4, 8
+    WS_STEP(0x142, 0xA);        // row_bcast 15 into rows 1 and 3
+    WS_STEP(0x143, 0xC);        // row_bcast 31 into rows 2 and 3
+#undef WS_STEP
+    return v;
+}
+__device__ __forceinline__ uint32_t lanes_below(uint64_t b) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
+}
+
 // Four consecutive floats: one 16-byte access where al (the address is
 // 16-byte aligned, uniform over the launch), else four.
 __device__ __forceinline__ f32x4 ld4(const float *p, bool al) {

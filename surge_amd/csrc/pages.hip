@@ -108,17 +108,6 @@ struct ap_part {
 
 __device__ __forceinline__ uint32_t ap_steps(const sgk_attn_paged_args &a, uint32_t s) { return (page_len(a.c, a.lens, s) + AP_STEP - 1) / AP_STEP; }
 __device__ __forceinline__ uint32_t ap_per(uint64_t total, uint32_t most) { return (max((uint32_t)((total + most - 1) / most), 1u) + AP_WAVES - 1) / AP_WAVES * AP_WAVES; }
-// Inclusive prefix sum over the wave: within the rows of 16, then the rows' ends carried on.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_or_0(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, true); }
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-    v += dpp_or_0<0x111, 0xF>(v);       // row_shr 1, 2, 4, 8
-    v += dpp_or_0<0x112, 0xF>(v);
-    v += dpp_or_0<0x114, 0xF>(v);
-    v += dpp_or_0<0x118, 0xF>(v);
-    v += dpp_or_0<0x142, 0xA>(v);       // row_bcast 15 into rows 1 and 3
-    return v + dpp_or_0<0x143, 0xC>(v); // row_bcast 31 into rows 2 and 3
-}
 struct ap_where { uint32_t s, first, n, per; };      // sequence (n_seq: none), its first part and their number
 // Of part x (by_part) or of sequence x.
 __device__ __forceinline__ ap_where ap_find(const sgk_attn_paged_args &a, const ap_part &w, uint32_t x, bool by_part) {
@@ -523,18 +512,6 @@ __device__ __forceinline__ uint32_t ev_key(float w, int32_t pos, int32_t last, u
     const uint32_t b = __float_as_uint(w + 0.0f);       // -0 as 0
     const uint32_t key = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
     return (uint32_t)last - (uint32_t)pos < recent ? 0xFFFFFFFFu : w != w ? 0u : key;
-}
-__device__ __forceinline__ uint32_t lanes_below(uint64_t b) {
-    return __builtin_amdgcn_mbcnt_hi((uint32_t)(b >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)b, 0));
-}
-// The lowest of 16 lanes' values, in all of them.
-template <uint32_t (*F)(uint32_t)>
-__device__ __forceinline__ uint64_t both(uint64_t v) { return (uint64_t)F((uint32_t)(v >> 32)) << 32 | F((uint32_t)v); }
-__device__ __forceinline__ uint64_t row_min(uint64_t v) {
-    v = min(v, both<dppu<0xB1>>(v));
-    v = min(v, both<dppu<0x4E>>(v));
-    v = min(v, both<dppu<0x141>>(v));
-    return min(v, both<dppu<0x128>>(v));
 }
 // Row `from` to `to`: K and V by 16 bytes a thread, weight and pos with the first.
 __device__ __forceinline__ void ev_move(const sgk_page_evict_args &a, uint32_t s, uint32_t h, uint32_t from, uint32_t to, uint32_t u, uint32_t units) {

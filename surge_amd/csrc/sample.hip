@@ -87,36 +87,33 @@ __device__ __forceinline__ double sm_weight(float x, float top, double inv) {
     return x == top ? 1.0 : x > -INFINITY ? exp(((double)x - (double)top) * inv) : 0.0;
 }
 __device__ __forceinline__ uint64_t sm_units(double w, double up) { return w > 0.0 ? max((uint64_t)1, (uint64_t)rint(w * up)) : 0; }
+// Over the workgroup, with 64 bits a wave in tmp.
 template <typename T>
-__device__ __forceinline__ T sm_sum(T v, T *tmp) {
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+__device__ __forceinline__ T sm_sum(T v, void *tmp) {
+    T *const x = (T *)tmp, w = wave_sum(v);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) tmp[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) x[threadIdx.x >> 6] = w;
     __syncthreads();
     T r = 0;
 #pragma unroll
-    for (int i = 0; i < SM_WAVES; i++) r += tmp[i];
+    for (int i = 0; i < SM_WAVES; i++) r += x[i];
     return r;
 }
 template <typename T>
-__device__ __forceinline__ T sm_scan(T v, T *total, T *tmp) {      // exclusive
-    const uint32_t t = threadIdx.x;
-    T x = v;
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const T y = __shfl_up(x, d);
-        if ((t & 63) >= d) x += y;
-    }
+__device__ __forceinline__ T sm_scan(T v, T *total, void *tmp) {      // exclusive
+    T *const x = (T *)tmp;
+    const T to = wave_scan(v);
     __syncthreads();
-    if ((t & 63) == 63) tmp[t >> 6] = x;
+    if ((threadIdx.x & 63) == 63) x[threadIdx.x >> 6] = to;
     __syncthreads();
     T before = 0, all = 0;
 #pragma unroll
     for (uint32_t i = 0; i < SM_WAVES; i++) {
-        if (i < t >> 6) before += tmp[i];
-        all += tmp[i];
+        if (i < threadIdx.x >> 6) before += x[i];
+        all += x[i];
     }
     *total = all;
-    return before + x - v;
+    return before + to - v;
 }
 
 struct sm_set { float temp, top_p, min_p, u; uint32_t top_k; double inv; bool few; };
@@ -146,7 +143,7 @@ __device__ __forceinline__ uint32_t sm_load(const sgk_sample_args &a, const sm_p
     return (uint32_t)i;
 }
 __device__ __forceinline__ sm_all sm_read(const sm_row &w, const sm_plan &p, const sm_set &s, uint64_t *tmp) {
-    const uint32_t t = threadIdx.x;
+    const uint32_t t = threadIdx.x, wv = t >> 6;
     uint32_t mine = 0, ok = 0, low = 0xFFFFFFFFu;
     double sum = 0.0;
     if (t < p.parts) {
@@ -154,23 +151,19 @@ __device__ __forceinline__ sm_all sm_read(const sm_row &w, const sm_plan &p, con
         for (uint32_t i = 0; i < SM_WAVES; i++) mine = max(mine, w.wave[t * SM_WAVES + i]);
         ok = w.ok[t];
         low = w.low[t];
-        if (!s.few) sum = w.sum[t];
+        sum = w.sum[t];
     }
-    uint32_t *red = (uint32_t *)tmp;
-    const uint32_t b = wave_umax(mine), lw = ~wave_umax(~low);
-    __syncthreads();
-    if ((t & 63) == 0) { red[t >> 6] = b; red[SM_WAVES + (t >> 6)] = lw; }
+    uint32_t *const red = (uint32_t *)tmp;      // [3][SM_WAVES], and doubles behind
+    const uint32_t b = wave_umax(mine), lw = ~wave_umax(~low), n = wave_sum(ok);
+    if ((t & 63) == 0) { red[wv] = b; red[SM_WAVES + wv] = lw; red[2 * SM_WAVES + wv] = n; }
     __syncthreads();
     sm_all r = {};
     r.low = 0xFFFFFFFFu;
 #pragma unroll
-    for (int i = 0; i < SM_WAVES; i++) { r.best = max(r.best, red[i]); r.low = min(r.low, red[SM_WAVES + i]); }
-    r.ok = sm_sum(ok, (uint32_t *)tmp);
+    for (int i = 0; i < SM_WAVES; i++) { r.best = max(r.best, red[i]); r.low = min(r.low, red[SM_WAVES + i]); r.ok += red[2 * SM_WAVES + i]; }
     r.top = sm_value(r.best);
-    if (!s.few) {
-        if (mine && mine != r.best) sum *= sm_weight(sm_value(mine), r.top, s.inv);
-        r.sum = sm_sum(mine ? sum : 0.0, (double *)tmp);
-    }
+    if (mine && mine != r.best) sum *= sm_weight(sm_value(mine), r.top, s.inv);
+    r.sum = sm_sum(mine ? sum : 0.0, tmp + 2 * SM_WAVES);
     return r;
 }
 __device__ __forceinline__ double sm_unit(double sum) { return ldexp(1.0, 61 - ilogb(sum)); }
@@ -199,7 +192,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_parts(sgk_sample_args a, 
     best = wave_umax(best);
     low = ~wave_umax(~low);
     if ((t & 63) == 0) { w.wave[part * SM_WAVES + (t >> 6)] = best; red[t >> 6] = best; red[SM_WAVES + (t >> 6)] = low; }
-    ok = sm_sum(ok, (uint32_t *)tmp);
+    ok = sm_sum(ok, tmp);
 #pragma unroll
     for (int i = 0; i < SM_WAVES; i++) { best = max(best, red[i]); low = min(low, red[SM_WAVES + i]); }
     if (t == 0) { w.ok[part] = ok; w.low[part] = ok ? low + 1 : 0xFFFFFFFFu; }
@@ -211,7 +204,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_parts(sgk_sample_args a, 
 #pragma unroll
         for (int e = 0; e < 4; e++) sum += sm_weight(x[e], top, s.inv);
     }
-    sum = sm_sum(sum, (double *)tmp);
+    sum = sm_sum(sum, tmp);
     if (t == 0) w.sum[part] = sum;
 }
 
@@ -226,16 +219,11 @@ __device__ __forceinline__ uint32_t sm_bin(float x, float top, float scale) {
 }
 // Appends the ids of a thread that `in` marks to the row's list.
 __device__ __forceinline__ void sm_append(const sm_row &w, const float (&x)[4], uint32_t i, uint32_t in) {
-    uint32_t n = __popc(in), to = n;
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const uint32_t y = __shfl_up(to, d);
-        if ((threadIdx.x & 63) >= d) to += y;
-    }
-    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)to, 63);
-    if (!all) return;
+    if (!__builtin_amdgcn_ballot_w64(in != 0)) return;
+    const uint32_t n = __popc(in), to = wave_scan(n);
     uint32_t base = 0;
-    if ((threadIdx.x & 63) == 0) base = atomicAdd(w.listed, all);
-    base = (uint32_t)__builtin_amdgcn_readfirstlane((int)base) + to - n;
+    if ((threadIdx.x & 63) == 63) base = atomicAdd(w.listed, to);
+    base = (uint32_t)__builtin_amdgcn_readlane((int)base, 63) + to - n;
 #pragma unroll
     for (int e = 0; e < 4; e++)
         if (in >> e & 1) {
@@ -246,31 +234,31 @@ __device__ __forceinline__ void sm_append(const sm_row &w, const float (&x)[4], 
 
 // ---- 2: the few listed, the parts' sums, or the histogram
 __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, sm_plan p, int al) {
-    __shared__ uint64_t tmp[2 * SM_WAVES], sums[SM_BINS];
+    __shared__ uint64_t tmp[3 * SM_WAVES], sums[SM_BINS];
     __shared__ uint32_t cnts[SM_BINS];
     const uint32_t t = threadIdx.x, l = t & 63, part = blockIdx.x, r = blockIdx.y;
     const sm_row w = sm_at(p, r);
     const sm_set s = sm_settings(a, p, r);
     float x[4];
     uint32_t i = sm_load(a, p, r, part, 0, al, x);
-    const sm_all all = sm_read(w, p, s, tmp);
-    if (part == 0 && t == 0) *w.all = all;
-    if (!all.ok) return;
     if (s.few) {
         // a bound that at least top_k ids reach: the top_k-th of the waves' maxima, its upper bits (every wave by itself)
         const uint32_t n = p.parts * SM_WAVES;
-        uint32_t bound = 0;
+        uint32_t bound = 0, best = 0, least = 0xFFFFFFFFu;
         if (n <= 64 * 16) {
-            uint32_t c[16], least = 0xFFFFFFFFu;
+            uint32_t c[16];
+#pragma unroll
+            for (uint32_t j = 0; j < 16; j++) c[j] = j * 64 + l < n ? w.wave[j * 64 + l] : 0;
 #pragma unroll
             for (uint32_t j = 0; j < 16; j++) {
-                c[j] = j * 64 + l < n ? w.wave[j * 64 + l] : 0;
+                best = max(best, c[j]);
                 if (j * 64 + l < n) least = min(least, c[j]);
             }
+            best = wave_umax(best);
             least = ~wave_umax(~least);
-            const uint32_t differ = all.best ^ least, high = differ ? 31 - __builtin_clz(differ) : 0;
+            const uint32_t differ = best ^ least, high = differ ? 31 - __builtin_clz(differ) : 0;
             bound = least & ~((2u << high) - 1);
-            for (int b = (int)high; b >= 0 && b > (int)high - 16; b--) {
+            for (int b = (int)high; b >= 0 && b > (int)high - 14; b--) {
                 uint32_t k = 0;
 #pragma unroll
                 for (uint32_t j = 0; j < 16; j++) {
@@ -278,14 +266,18 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
                     k += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(c[j] >= (bound | 1u << b)));
                 }
                 if (k >= s.top_k) bound |= 1u << b;
+                if (k == s.top_k) break;
             }
         } else {
+            for (uint32_t j = l; j < n; j += 64) best = max(best, w.wave[j]);
+            best = wave_umax(best);
             for (int b = 31; b >= 12; b--) {
                 uint32_t k = 0;
                 for (uint32_t j = l; j < (n + 63) / 64 * 64; j += 64) k += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(j < n && w.wave[j] >= (bound | 1u << b)));
                 if (k >= s.top_k) bound |= 1u << b;
             }
         }
+        if (part == 0 && t == 0) *w.all = (sm_all){best, 0, best != 0, sm_value(best), 0.0};
         bound = max(bound, 1u);
         for (uint32_t m = 0; m < p.rounds; m++) {
             if (m) i = sm_load(a, p, r, part, m, al, x);
@@ -296,6 +288,9 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
         }
         return;
     }
+    const sm_all all = sm_read(w, p, s, tmp);
+    if (part == 0 && t == 0) *w.all = all;
+    if (!all.ok) return;
     const double up = sm_unit(all.sum);
     if ((!s.top_k || s.top_k >= all.ok) && s.top_p == 1.0f) {
         uint64_t q = 0;
@@ -314,105 +309,156 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
     for (uint32_t j = t; j < SM_BINS; j += SM_THREADS) { cnts[j] = 0; sums[j] = 0; }
     __syncthreads();
     const float scale = sm_bin_scale(s, all);
+    const bool k_on = s.top_k && s.top_k < all.ok, p_on = s.top_p < 1.0f;       // counts for top_k, sums for top_p
     for (uint32_t m = 0; m < p.rounds; m++) {
         if (m) sm_load(a, p, r, part, m, al, x);
 #pragma unroll
         for (int e = 0; e < 4; e++)
             if (x[e] > -INFINITY) {
                 const uint32_t b = sm_bin(x[e], all.top, scale);
-                atomicAdd(&cnts[b], 1u);
-                atomicAdd((unsigned long long *)&sums[b], (unsigned long long)sm_units(sm_weight(x[e], all.top, s.inv), up));
+                if (k_on) atomicAdd(&cnts[b], 1u);
+                if (p_on) atomicAdd((unsigned long long *)&sums[b], (unsigned long long)sm_units(sm_weight(x[e], all.top, s.inv), up));
             }
     }
     __syncthreads();
-    for (uint32_t j = t; j < SM_BINS; j += SM_THREADS)
-        if (cnts[j]) {
-            atomicAdd(w.bincnt + j, cnts[j]);
-            atomicAdd((unsigned long long *)w.binsum + j, (unsigned long long)sums[j]);
-        }
+    for (uint32_t j = t; j < SM_BINS; j += SM_THREADS) {
+        if (cnts[j]) atomicAdd(w.bincnt + j, cnts[j]);
+        if (sums[j]) atomicAdd((unsigned long long *)w.binsum + j, (unsigned long long)sums[j]);
+    }
 }
-
 
 // ---- a list of ids in LDS: order (key, then ~id: the larger comes first), units, bin with SM_LOW if the weight is below min_p
 #define SM_LOW 0x80000000u
-struct sm_list { uint64_t order[SM_LIST], unit[SM_LIST]; uint32_t bin[SM_LIST], n; uint64_t border, ksum; };
+struct sm_list { uint64_t order[SM_LIST], unit[SM_LIST]; uint32_t bin[SM_LIST], n; uint64_t border; };
 
-template <uint32_t (*F)(uint32_t)>
-__device__ __forceinline__ uint64_t sm_both(uint64_t v) { return (uint64_t)F((uint32_t)(v >> 32)) << 32 | F((uint32_t)v); }
-__device__ __forceinline__ uint64_t wave_sum64(uint64_t v) {
-    v += sm_both<dppu<0xB1>>(v);
-    v += sm_both<dppu<0x4E>>(v);
-    v += sm_both<dppu<0x141>>(v);
-    v += sm_both<dppu<0x128>>(v);
-    v += sm_both<swap16>(v);
-    return v + sm_both<swap32>(v);
-}
-// Below, a wave over the list's entries j that in(j) takes.
-// The largest value V (32 bits) for which `before` and the units of the entries with val(j) >= V add up to `want`, the
-// lowest entry's if none does, but never above the highest's.
-template <typename In, typename Val>
-__device__ __forceinline__ uint32_t sm_top(const sm_list &s, uint64_t before, uint64_t want, In in, Val val) {
-    const uint32_t l = threadIdx.x & 63;
-    uint32_t lo = 0xFFFFFFFFu, hi = 0;
-    for (uint32_t j = l; j < s.n; j += 64)
-        if (in(j)) { lo = min(lo, val(j)); hi = max(hi, val(j)); }
-    lo = ~wave_umax(~lo);
-    hi = wave_umax(hi);
-    if (lo >= hi) return hi;
-    uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi), at = lo & ~(2 * bit - 1);
-    for (; bit; bit >>= 1) {
-        uint64_t sum = 0;
-        for (uint32_t j = l; j < s.n; j += 64)
-            if (in(j) && val(j) >= (at | bit)) sum += s.unit[j];
-        sum = wave_sum64(sum);
-        if (sum && before + sum >= want) at |= bit;
+// A wave over the list: entry i of a lane is place 64 i + lane. Up to 64 U of them are in registers, more are read again.
+template <int U>
+struct sm_wave {
+    const sm_list &s;
+    const uint32_t n, l, each;
+    uint32_t key[U ? U : 1], low[U ? U : 1], bin[U ? U : 1];
+    uint64_t unit[U ? U : 1];
+    __device__ __forceinline__ sm_wave(const sm_list &list) : s(list), n(list.n), l(threadIdx.x & 63), each((list.n + 63) / 64) {
+        if constexpr (U > 0)
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                const uint32_t j = min(64 * i + l, n - 1);
+                key[i] = (uint32_t)(s.order[j] >> 32);
+                low[i] = (uint32_t)s.order[j];
+                bin[i] = 64 * i + l < n ? s.bin[j] : 0xFFFFFFFFu;
+                unit[i] = s.unit[j];
+            }
     }
-    return max(at, lo);
-}
-// The order of the room-th entry.
-template <typename In>
-__device__ __forceinline__ uint64_t sm_nth(const sm_list &s, uint32_t room, In in) {
-    const uint32_t l = threadIdx.x & 63;
-    uint64_t at = 0;
-    for (int half = 0; half < 2; half++) {      // the key, then ~id among that key's
-        auto val = [&](uint32_t j) { return half ? (uint32_t)s.order[j] : (uint32_t)(s.order[j] >> 32); };
-        auto here = [&](uint32_t j) { return in(j) && (!half || s.order[j] >> 32 == at >> 32); };
-        uint32_t lo = 0xFFFFFFFFu, hi = 0;
-        for (uint32_t j = l; j < s.n; j += 64)
-            if (here(j)) { lo = min(lo, val(j)); hi = max(hi, val(j)); }
-        lo = ~wave_umax(~lo);
-        hi = wave_umax(hi);
-        uint32_t v = lo, from = UINT32_MAX;     // from: entries from v on
-        if (lo < hi) {
-            uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi);
-            v &= ~(2 * bit - 1);
-            for (; bit && from != room; bit >>= 1) {
-                uint32_t m = 0;
-                for (uint32_t j0 = 0; j0 < s.n; j0 += 64) m += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(j0 + l < s.n && here(j0 + l) && val(j0 + l) >= (v | bit)));
-                if (m >= room) { v |= bit; from = m; }
+    // f(i, key, ~id, bin, unit) for the lane's entries; what is behind the list has bin 0xFFFFFFFF
+    template <typename F>
+    __device__ __forceinline__ void all(F f) const {
+        if constexpr (U > 0) {
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                if ((uint32_t)i >= each) break;
+                f(key[i], low[i], bin[i], unit[i]);
+            }
+        } else {
+            for (uint32_t i = 0; i < each; i++) {
+                const uint32_t j = min(64 * i + l, n - 1);
+                f((uint32_t)(s.order[j] >> 32), (uint32_t)s.order[j], 64 * i + l < n ? s.bin[j] : 0xFFFFFFFFu, s.unit[j]);
             }
         }
-        if (half) return at | v;
-        if (from == room) return (uint64_t)v << 32;
-        at = (uint64_t)v << 32;
-        for (uint32_t j0 = 0; j0 < s.n; j0 += 64) room -= (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(j0 + l < s.n && in(j0 + l) && (uint32_t)(s.order[j0 + l] >> 32) > v));
     }
-    return at;
+    template <typename In>
+    __device__ __forceinline__ uint32_t count(In in) const {
+        uint32_t m = 0;
+        all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t) { m += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(b != 0xFFFFFFFFu && in(k, d, b))); });
+        return m;
+    }
+    template <typename In>
+    __device__ __forceinline__ uint64_t units(In in) const {
+        uint64_t m = 0;
+        all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t u) { if (b != 0xFFFFFFFFu && in(k, d, b)) m += u; });
+        return wave_sum(m);
+    }
+    // The lowest and the highest key, or ~id, of the entries that in() takes.
+    template <bool LOW, typename In>
+    __device__ __forceinline__ void ends(In in, uint32_t &lo, uint32_t &hi) const {
+        lo = 0xFFFFFFFFu;
+        hi = 0;
+        all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t) {
+            if (b != 0xFFFFFFFFu && in(k, d, b)) { lo = min(lo, LOW ? d : k); hi = max(hi, LOW ? d : k); }
+        });
+        lo = ~wave_umax(~lo);
+        hi = wave_umax(hi);
+    }
+    // The largest key (or ~id) from which on the units of the entries that in() takes, and `before`, add up to `want`; the
+    // lowest entry's if none does, but never above the highest's.
+    template <bool LOW, typename In>
+    __device__ __forceinline__ uint32_t top(uint64_t before, uint64_t want, In in) const {
+        uint32_t lo, hi;
+        ends<LOW>(in, lo, hi);
+        if (lo >= hi) return hi;
+        uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi), at = lo & ~(2 * bit - 1);
+        for (; bit; bit >>= 1) {
+            const uint64_t sum = units([&](uint32_t k, uint32_t d, uint32_t b) { return in(k, d, b) && (LOW ? d : k) >= (at | bit); });
+            if (sum && before + sum >= want) at |= bit;
+        }
+        return max(at, lo);
+    }
+    // The room-th key (or ~id) of those that in() takes, and how many are above it.
+    template <bool LOW, typename In>
+    __device__ __forceinline__ uint32_t nth(uint32_t room, In in, uint32_t &above) const {
+        uint32_t lo, hi, from = UINT32_MAX;
+        ends<LOW>(in, lo, hi);
+        uint32_t at = lo;
+        if (lo < hi) {
+            uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi);
+            at &= ~(2 * bit - 1);
+            for (; bit && from != room; bit >>= 1) {
+                const uint32_t m = count([&](uint32_t k, uint32_t d, uint32_t b) { return in(k, d, b) && (LOW ? d : k) >= (at | bit); });
+                if (m >= room) { at |= bit; from = m; }
+            }
+        }
+        above = from == room ? 0 : count([&](uint32_t k, uint32_t d, uint32_t b) { return in(k, d, b) && (LOW ? d : k) > at; });
+        if (from == room) above = room;         // all from `at` on stay: nothing to be chosen among its own
+        return at;
+    }
+    // The order from which on `room` entries stay.
+    template <typename In>
+    __device__ __forceinline__ uint64_t first(uint32_t room, In in) const {
+        uint32_t above, unused;
+        const uint32_t key0 = nth<false>(room, in, above);
+        if (above >= room) return (uint64_t)key0 << 32;
+        auto same = [&](uint32_t k, uint32_t d, uint32_t b) { return k == key0 && in(k, d, b); };
+        return (uint64_t)key0 << 32 | nth<true>(room - above, same, unused);
+    }
+};
+// The lowest order that stays under top_k and top_p.
+template <int U>
+__device__ __forceinline__ uint64_t sm_end(const sm_list &list, const sm_set &set, const sm_all &all, const sm_border &b, double up) {
+    const sm_wave<U> v(list);
+    uint64_t border = 0, whole = b.whole;
+    if (b.kbin < SM_BINS) {
+        auto in = [&](uint32_t, uint32_t, uint32_t bin) { return (bin & ~SM_LOW) == b.kbin; };
+        if (v.count(in) > set.top_k - b.kabove) border = v.first(set.top_k - b.kabove, in);
+        if (b.plo < SM_BINS)
+            whole = b.ksum + v.units([&](uint32_t k, uint32_t d, uint32_t bin) { return in(k, d, bin) && ((uint64_t)k << 32 | d) >= border; });
+    }
+    if (b.plo < SM_BINS) {
+        const double want = (double)set.top_p * (double)whole;
+        const uint64_t units = want > 0.0 ? (uint64_t)ceil(want) : 0;
+        auto in = [&](uint32_t k, uint32_t d, uint32_t bin) { const uint32_t x = bin & ~SM_LOW; return x >= b.plo && x <= b.phi && ((uint64_t)k << 32 | d) >= border; };
+        const uint32_t key = v.template top<false>(b.psum, units, in);
+        // of that key's ids, as many as it takes
+        auto same = [&](uint32_t k, uint32_t d, uint32_t bin) { return k == key && in(k, d, bin); };
+        const uint64_t ahead = b.psum + v.units([&](uint32_t k, uint32_t d, uint32_t bin) { return k > key && in(k, d, bin); });
+        const uint32_t ties = v.count(same);
+        const uint64_t unit = sm_units(sm_weight(sm_value(key), all.top, set.inv), up);
+        const uint64_t room = units > ahead ? unit ? (units - ahead + unit - 1) / unit : ties : 1;
+        uint32_t unused;
+        const uint64_t low = room < ties ? v.template nth<true>((uint32_t)room, same, unused) : 0;
+        border = max(border, (uint64_t)key << 32 | low);
+    }
+    return border;
 }
-template <typename In>
-__device__ __forceinline__ uint32_t sm_count(const sm_list &s, In in) {
-    uint32_t m = 0;
-    for (uint32_t j0 = 0; j0 < s.n; j0 += 64) m += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(j0 + (threadIdx.x & 63) < s.n && in(j0 + (threadIdx.x & 63))));
-    return m;
-}
-template <typename In>
-__device__ __forceinline__ uint64_t sm_units_of(const sm_list &s, In in) {
-    uint64_t sum = 0;
-    for (uint32_t j = threadIdx.x & 63; j < s.n; j += 64)
-        if (in(j)) sum += s.unit[j];
-    return wave_sum64(sum);
-}
-// The list from memory, and the lowest order that stays under top_k and top_p; all threads. False: it does not fit.
+// The list from memory, and its border; all threads. False: it does not fit.
 __device__ __forceinline__ bool sm_resolve(sm_list &s, const sm_row &w, const sm_set &set, const sm_all &all, const sm_border &b, double up, float scale) {
     const uint32_t t = threadIdx.x;
     const uint32_t n = *w.listed;
@@ -428,29 +474,19 @@ __device__ __forceinline__ bool sm_resolve(sm_list &s, const sm_row &w, const sm
     if (t == 0) s.n = n;
     __syncthreads();
     if (t < 64) {
-        uint64_t border = 0, whole = b.whole;
-        if (b.kbin < SM_BINS) {
-            auto in = [&](uint32_t j) { return (s.bin[j] & ~SM_LOW) == b.kbin; };
-            if (sm_count(s, in) > set.top_k - b.kabove) border = sm_nth(s, set.top_k - b.kabove, in);
-            whole = b.ksum + sm_units_of(s, [&](uint32_t j) { return in(j) && s.order[j] >= border; });
-        }
-        if (b.plo < SM_BINS) {
-            const double want = (double)set.top_p * (double)whole;
-            const uint64_t units = want > 0.0 ? (uint64_t)ceil(want) : 0;
-            auto in = [&](uint32_t j) { const uint32_t x = s.bin[j] & ~SM_LOW; return x >= b.plo && x <= b.phi && s.order[j] >= border; };
-            const uint32_t key = sm_top(s, b.psum, units, in, [&](uint32_t j) { return (uint32_t)(s.order[j] >> 32); });
-            // of that key's ids, as many as it takes
-            auto same = [&](uint32_t j) { return in(j) && s.order[j] >> 32 == key; };
-            const uint64_t ahead = b.psum + sm_units_of(s, [&](uint32_t j) { return in(j) && s.order[j] >> 32 > key; });
-            const uint32_t ties = sm_count(s, same);
-            const uint64_t unit = sm_units(sm_weight(sm_value(key), all.top, set.inv), up);
-            const uint64_t room = units > ahead ? unit ? (units - ahead + unit - 1) / unit : ties : 1;
-            border = max(border, room < ties ? sm_nth(s, (uint32_t)room, same) : (uint64_t)key << 32);
-        }
+        const uint64_t border = n <= 64 ? sm_end<1>(s, set, all, b, up) : n <= 512 ? sm_end<8>(s, set, all, b, up) : sm_end<0>(s, set, all, b, up);
         if (t == 0) s.border = border;
     }
     __syncthreads();
     return true;
+}
+// The token among the list's ids that stay, by a wave, and their units.
+template <int U>
+__device__ __forceinline__ uint32_t sm_choose(const sm_list &list, float u, uint64_t &whole) {
+    const sm_wave<U> v(list);
+    auto in = [&](uint32_t k, uint32_t d, uint32_t bin) { return ((uint64_t)k << 32 | d) >= list.border && !(bin & SM_LOW); };
+    whole = v.units(in);
+    return ~v.template top<true>(0, (uint64_t)((double)u * (double)whole) + 1, in);
 }
 
 // The token of a row's part in which the units pass `want` (counted from the part's start), and the part's probabilities.
@@ -509,10 +545,10 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a,
         const double up = 0x1p54;           // 2^7 ids at most
         const sm_border b = {0, 0, s.top_p < 1.0f ? 0 : SM_BINS, 0, 0, 0, 0, 0};
         if (!sm_resolve(list, w, s, all, b, up, 0.0f)) return;
-        auto in = [&](uint32_t j) { return list.order[j] >= list.border && !(list.bin[j] & SM_LOW); };
         if (t >= 64) return;
-        const uint64_t whole = sm_units_of(list, in), want = (uint64_t)((double)s.u * (double)whole) + 1;
-        const uint32_t id = ~sm_top(list, 0, want, in, [&](uint32_t j) { return (uint32_t)list.order[j]; });
+        auto in = [&](uint32_t j) { return list.order[j] >= list.border && !(list.bin[j] & SM_LOW); };
+        uint64_t whole;
+        const uint32_t id = list.n <= 64 ? sm_choose<1>(list, s.u, whole) : list.n <= 512 ? sm_choose<8>(list, s.u, whole) : sm_choose<0>(list, s.u, whole);
         if (t == 0) a.token[r] = id;
         if (!a.probs) return;
         uint32_t n = 0;
@@ -520,7 +556,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a,
             const uint32_t j = j0 + t;
             const bool k = j < list.n && in(j);
             const uint64_t m = __builtin_amdgcn_ballot_w64(k);
-            const uint32_t at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+            const uint32_t at = n + lanes_below(m);
             if (k && at < SM_FEW) {
                 w.out[1 + 2 * at] = ~(uint32_t)list.order[j];
                 w.out[2 + 2 * at] = __float_as_uint((float)(sm_weight(sm_value((uint32_t)(list.order[j] >> 32)), all.top, s.inv) * up / (double)whole));
@@ -611,7 +647,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a,
 }
 
 // A row whose list does not fit: one workgroup, the borders of top_k and top_p by the digits of the keys, 8 bits a pass over the row.
-__device__ __noinline__ void sm_slow(const sgk_sample_args &a, uint32_t r, const sm_set &set, sm_list *room) {
+__device__ __forceinline__ void sm_slow(const sgk_sample_args &a, uint32_t r, const sm_set &set, sm_list *room) {
     uint64_t *const hist = room->order, *const tmp = hist + 256, *const pick = tmp + SM_WAVES;
     uint32_t *const tmp32 = room->bin, &token = room->n;
     const uint32_t t = threadIdx.x, v = a.vocab, top_k = set.top_k;
@@ -659,7 +695,7 @@ __device__ __noinline__ void sm_slow(const sgk_sample_args &a, uint32_t r, const
     // the sum of what top-k left: first in floating point, for the unit, then in units
     double part = 0.0;
     for (uint32_t i = t; i < v; i += SM_THREADS) if (sm_key(x[i]) > border) part += sm_weight(x[i], top, inv);
-    double sum = sm_sum(part, (double *)tmp);
+    double sum = sm_sum(part, tmp);
     const float bx = __uint_as_float(border & 0x80000000u ? border ^ 0x80000000u : ~border);
     if (border) sum += ties * sm_weight(bx, top, inv);
     const double up = ldexp(1.0, 61 - ilogb(sum));
