@@ -18,6 +18,12 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
+// What no kernel writes while it reads it, at addresses that a wave's lanes share: by scalar loads, which are not
+// counted with the vector ones.
+typedef __attribute__((address_space(4))) int32_t scalar_i32;
+typedef __attribute__((address_space(4))) uint32_t scalar_u32;
+typedef __attribute__((address_space(4))) float scalar_f32;
+
 // Partner lanes: quad_perm [1,0,3,2] and [2,3,0,1], row_half_mirror (i <-> 7-i
 // in each 8 lanes), row_ror:8, and the gfx950 swaps across rows and half-waves.
 template <int CTRL>

@@ -10,9 +10,6 @@
 #include "devutil.h"
 #include "kernels.h"
 
-// What no kernel writes while it reads it, at addresses that a wave's lanes share: by scalar loads, which are
-// not counted with the rows'.
-typedef __attribute__((address_space(4))) int32_t scalar_i32;
 typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 
 // An address that a wave's lanes share, as the scalar base of its loads.

@@ -30,7 +30,11 @@
 #define SM_IDS (4 * SM_THREADS)
 #define SM_PARTS 512u       // of a row, at most: its parts take several rounds of SM_IDS past that
 #define SM_FEW 128u
+#ifndef SM_WGS
+#define SM_WGS 1024u
+#endif
 #define SM_LIST 2048u
+#define SM_RANKED 128u      // entries that are compared all with all
 #define SM_BINS 2048u
 #define SM_NONE 0xFFFFFFFFu
 
@@ -118,8 +122,8 @@ __device__ __forceinline__ T sm_scan(T v, T *total, void *tmp) {      // exclusi
 
 struct sm_set { float temp, top_p, min_p, u; uint32_t top_k; double inv; bool few; };
 __device__ __forceinline__ sm_set sm_settings(const sgk_sample_args &a, const sm_plan &p, uint32_t r) {
-    const uint32_t *set = a.settings + 4ull * r;
-    sm_set s = {__uint_as_float(set[0]), __uint_as_float(set[2]), __uint_as_float(set[3]), a.u[r], set[1]};
+    const scalar_u32 *set = (const scalar_u32 *)(uintptr_t)(a.settings + 4ull * r);
+    sm_set s = {__uint_as_float(set[0]), __uint_as_float(set[2]), __uint_as_float(set[3]), ((const scalar_f32 *)(uintptr_t)a.u)[r], set[1]};
     s.u = s.u > 0.0f ? fminf(s.u, 0x1.fffffep-1f) : 0.0f;
     if (!(s.temp > 0.0f)) { s.temp = 1.0f; s.top_k = 1; }
     if (!(s.top_p < 1.0f)) s.top_p = 1.0f;
@@ -252,21 +256,26 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
 #pragma unroll
             for (uint32_t j = 0; j < 16; j++) {
                 best = max(best, c[j]);
-                if (j * 64 + l < n) least = min(least, c[j]);
+                if (c[j]) least = min(least, c[j]);
             }
             best = wave_umax(best);
             least = ~wave_umax(~least);
             const uint32_t differ = best ^ least, high = differ ? 31 - __builtin_clz(differ) : 0;
-            bound = least & ~((2u << high) - 1);
-            for (int b = (int)high; b >= 0 && b > (int)high - 14; b--) {
-                uint32_t k = 0;
+            uint32_t have = 0;
 #pragma unroll
-                for (uint32_t j = 0; j < 16; j++) {
-                    if (j % 4 == 0 && j * 64 >= n) break;
-                    k += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(c[j] >= (bound | 1u << b)));
+            for (uint32_t j = 0; j < 16; j++) have += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(c[j] != 0));
+            // 11 bits of it at least, and more until few more waves reach it than have to
+            if (have >= s.top_k) {
+                bound = least & ~((2u << high) - 1);
+                for (int b = (int)high; b >= 0 && (b > (int)high - 11 || have > s.top_k + s.top_k / 8); b--) {
+                    uint32_t k = 0;
+#pragma unroll
+                    for (uint32_t j = 0; j < 16; j++) {
+                        if (j % 4 == 0 && j * 64 >= n) break;
+                        k += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(c[j] >= (bound | 1u << b)));
+                    }
+                    if (k >= s.top_k) { bound |= 1u << b; have = k; }
                 }
-                if (k >= s.top_k) bound |= 1u << b;
-                if (k == s.top_k) break;
             }
         } else {
             for (uint32_t j = l; j < n; j += 64) best = max(best, w.wave[j]);
@@ -329,57 +338,62 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
 
 // ---- a list of ids in LDS: order (key, then ~id: the larger comes first), units, bin with SM_LOW if the weight is below min_p
 #define SM_LOW 0x80000000u
-struct sm_list { uint64_t order[SM_LIST], unit[SM_LIST]; uint32_t bin[SM_LIST], n; uint64_t border; };
+struct sm_list { uint64_t order[SM_LIST], unit[SM_LIST]; uint32_t bin[SM_LIST], n; uint64_t border, tmp[2][SM_WAVES]; };
 
-// A wave over the list: entry i of a lane is place 64 i + lane. Up to 64 U of them are in registers, more are read again.
-template <int U>
-struct sm_wave {
-    const sm_list &s;
-    const uint32_t n, l, each;
-    uint32_t key[U ? U : 1], low[U ? U : 1], bin[U ? U : 1];
-    uint64_t unit[U ? U : 1];
-    __device__ __forceinline__ sm_wave(const sm_list &list) : s(list), n(list.n), l(threadIdx.x & 63), each((list.n + 63) / 64) {
-        if constexpr (U > 0)
+// Who goes over the list: a wave alone while its entries fit into 8 registers a lane (SM_ALONE), past that the workgroup,
+// whose steps each take a barrier (300 entries: 6 us less alone). Entry i of a thread is place i THREADS + its own.
+#define SM_ALONE 512u
+template <int THREADS, int U>
+struct sm_over {
+    const uint32_t t, each;
+    uint64_t (*const tmp)[SM_WAVES];        // a step's results go through half `at`, so that one barrier a step is enough
+    int at;
+    uint32_t key[U], low[U], bin[U];        // bin: 0xFFFFFFFF behind the list
+    uint64_t unit[U];
+    __device__ __forceinline__ sm_over(sm_list &s) : t(threadIdx.x), each((s.n + THREADS - 1) / THREADS), tmp(s.tmp), at(0) {
 #pragma unroll
-            for (int i = 0; i < U; i++) {
-                const uint32_t j = min(64 * i + l, n - 1);
-                key[i] = (uint32_t)(s.order[j] >> 32);
-                low[i] = (uint32_t)s.order[j];
-                bin[i] = 64 * i + l < n ? s.bin[j] : 0xFFFFFFFFu;
-                unit[i] = s.unit[j];
-            }
+        for (int i = 0; i < U; i++) {
+            const uint32_t j = i * THREADS + t;
+            const bool here = j < s.n;
+            key[i] = here ? (uint32_t)(s.order[j] >> 32) : 0;
+            low[i] = here ? (uint32_t)s.order[j] : 0;
+            bin[i] = here ? s.bin[j] : 0xFFFFFFFFu;
+            unit[i] = here ? s.unit[j] : 0;
+        }
+        if (THREADS > 64) __syncthreads();
     }
-    // f(i, key, ~id, bin, unit) for the lane's entries; what is behind the list has bin 0xFFFFFFFF
     template <typename F>
     __device__ __forceinline__ void all(F f) const {
-        if constexpr (U > 0) {
 #pragma unroll
-            for (int i = 0; i < U; i++) {
-                if ((uint32_t)i >= each) break;
-                f(key[i], low[i], bin[i], unit[i]);
-            }
-        } else {
-            for (uint32_t i = 0; i < each; i++) {
-                const uint32_t j = min(64 * i + l, n - 1);
-                f((uint32_t)(s.order[j] >> 32), (uint32_t)s.order[j], 64 * i + l < n ? s.bin[j] : 0xFFFFFFFFu, s.unit[j]);
-            }
-        }
+        for (int i = 0; i < U; i++)
+            if ((uint32_t)i < each) f(key[i], low[i], bin[i], unit[i]);
+    }
+    // v of the waves, added
+    __device__ __forceinline__ uint64_t add(uint64_t v) {
+        if (THREADS == 64) return v;
+        if ((t & 63) == 0) tmp[at][t >> 6] = v;
+        __syncthreads();
+        uint64_t r = 0;
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; i++) r += tmp[at][i];
+        at ^= 1;
+        return r;
     }
     template <typename In>
-    __device__ __forceinline__ uint32_t count(In in) const {
+    __device__ __forceinline__ uint32_t count(In in) {
         uint32_t m = 0;
         all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t) { m += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(b != 0xFFFFFFFFu && in(k, d, b))); });
-        return m;
+        return (uint32_t)add(m);
     }
     template <typename In>
-    __device__ __forceinline__ uint64_t units(In in) const {
+    __device__ __forceinline__ uint64_t units(In in) {
         uint64_t m = 0;
         all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t u) { if (b != 0xFFFFFFFFu && in(k, d, b)) m += u; });
-        return wave_sum(m);
+        return add(wave_sum(m));
     }
     // The lowest and the highest key, or ~id, of the entries that in() takes.
     template <bool LOW, typename In>
-    __device__ __forceinline__ void ends(In in, uint32_t &lo, uint32_t &hi) const {
+    __device__ __forceinline__ void ends(In in, uint32_t &lo, uint32_t &hi) {
         lo = 0xFFFFFFFFu;
         hi = 0;
         all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t) {
@@ -387,42 +401,49 @@ struct sm_wave {
         });
         lo = ~wave_umax(~lo);
         hi = wave_umax(hi);
+        if (THREADS == 64) return;
+        if ((t & 63) == 0) tmp[at][t >> 6] = (uint64_t)~lo << 32 | hi;
+        __syncthreads();
+        uint32_t a = 0;
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; i++) { a = max(a, (uint32_t)(tmp[at][i] >> 32)); hi = max(hi, (uint32_t)tmp[at][i]); }
+        at ^= 1;
+        lo = ~a;
     }
     // The largest key (or ~id) from which on the units of the entries that in() takes, and `before`, add up to `want`; the
     // lowest entry's if none does, but never above the highest's.
     template <bool LOW, typename In>
-    __device__ __forceinline__ uint32_t top(uint64_t before, uint64_t want, In in) const {
+    __device__ __forceinline__ uint32_t top(uint64_t before, uint64_t want, In in) {
         uint32_t lo, hi;
         ends<LOW>(in, lo, hi);
         if (lo >= hi) return hi;
-        uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi), at = lo & ~(2 * bit - 1);
+        uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi), from = lo & ~(2 * bit - 1);
         for (; bit; bit >>= 1) {
-            const uint64_t sum = units([&](uint32_t k, uint32_t d, uint32_t b) { return in(k, d, b) && (LOW ? d : k) >= (at | bit); });
-            if (sum && before + sum >= want) at |= bit;
+            const uint64_t sum = units([&](uint32_t k, uint32_t d, uint32_t b) { return in(k, d, b) && (LOW ? d : k) >= (from | bit); });
+            if (sum && before + sum >= want) from |= bit;
         }
-        return max(at, lo);
+        return max(from, lo);
     }
-    // The room-th key (or ~id) of those that in() takes, and how many are above it.
+    // The room-th key (or ~id) of those that in() takes, and how many are above it (room: all its own stay).
     template <bool LOW, typename In>
-    __device__ __forceinline__ uint32_t nth(uint32_t room, In in, uint32_t &above) const {
-        uint32_t lo, hi, from = UINT32_MAX;
+    __device__ __forceinline__ uint32_t nth(uint32_t room, In in, uint32_t &above) {
+        uint32_t lo, hi, have = UINT32_MAX;
         ends<LOW>(in, lo, hi);
-        uint32_t at = lo;
+        uint32_t from = lo;
         if (lo < hi) {
             uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi);
-            at &= ~(2 * bit - 1);
-            for (; bit && from != room; bit >>= 1) {
-                const uint32_t m = count([&](uint32_t k, uint32_t d, uint32_t b) { return in(k, d, b) && (LOW ? d : k) >= (at | bit); });
-                if (m >= room) { at |= bit; from = m; }
+            from &= ~(2 * bit - 1);
+            for (; bit && have != room; bit >>= 1) {
+                const uint32_t m = count([&](uint32_t k, uint32_t d, uint32_t b) { return in(k, d, b) && (LOW ? d : k) >= (from | bit); });
+                if (m >= room) { from |= bit; have = m; }
             }
         }
-        above = from == room ? 0 : count([&](uint32_t k, uint32_t d, uint32_t b) { return in(k, d, b) && (LOW ? d : k) > at; });
-        if (from == room) above = room;         // all from `at` on stay: nothing to be chosen among its own
-        return at;
+        above = have == room ? room : count([&](uint32_t k, uint32_t d, uint32_t b) { return in(k, d, b) && (LOW ? d : k) > from; });
+        return from;
     }
     // The order from which on `room` entries stay.
     template <typename In>
-    __device__ __forceinline__ uint64_t first(uint32_t room, In in) const {
+    __device__ __forceinline__ uint64_t first(uint32_t room, In in) {
         uint32_t above, unused;
         const uint32_t key0 = nth<false>(room, in, above);
         if (above >= room) return (uint64_t)key0 << 32;
@@ -430,10 +451,12 @@ struct sm_wave {
         return (uint64_t)key0 << 32 | nth<true>(room - above, same, unused);
     }
 };
+typedef sm_over<64, SM_ALONE / 64> sm_alone;
+typedef sm_over<SM_THREADS, SM_LIST / SM_THREADS> sm_together;
 // The lowest order that stays under top_k and top_p.
-template <int U>
-__device__ __forceinline__ uint64_t sm_end(const sm_list &list, const sm_set &set, const sm_all &all, const sm_border &b, double up) {
-    const sm_wave<U> v(list);
+template <typename Over>
+__device__ __forceinline__ uint64_t sm_end(sm_list &list, const sm_set &set, const sm_all &all, const sm_border &b, double up) {
+    Over v(list);
     uint64_t border = 0, whole = b.whole;
     if (b.kbin < SM_BINS) {
         auto in = [&](uint32_t, uint32_t, uint32_t bin) { return (bin & ~SM_LOW) == b.kbin; };
@@ -448,12 +471,15 @@ __device__ __forceinline__ uint64_t sm_end(const sm_list &list, const sm_set &se
         const uint32_t key = v.template top<false>(b.psum, units, in);
         // of that key's ids, as many as it takes
         auto same = [&](uint32_t k, uint32_t d, uint32_t bin) { return k == key && in(k, d, bin); };
-        const uint64_t ahead = b.psum + v.units([&](uint32_t k, uint32_t d, uint32_t bin) { return k > key && in(k, d, bin); });
         const uint32_t ties = v.count(same);
-        const uint64_t unit = sm_units(sm_weight(sm_value(key), all.top, set.inv), up);
-        const uint64_t room = units > ahead ? unit ? (units - ahead + unit - 1) / unit : ties : 1;
-        uint32_t unused;
-        const uint64_t low = room < ties ? v.template nth<true>((uint32_t)room, same, unused) : 0;
+        uint64_t low = 0;
+        if (ties > 1) {
+            const uint64_t ahead = b.psum + v.units([&](uint32_t k, uint32_t d, uint32_t bin) { return k > key && in(k, d, bin); });
+            const uint64_t unit = sm_units(sm_weight(sm_value(key), all.top, set.inv), up);
+            const uint64_t room = units > ahead ? unit ? (units - ahead + unit - 1) / unit : ties : 1;
+            uint32_t unused;
+            if (room < ties) low = v.template nth<true>((uint32_t)room, same, unused);
+        }
         border = max(border, (uint64_t)key << 32 | low);
     }
     return border;
@@ -473,20 +499,25 @@ __device__ __forceinline__ bool sm_resolve(sm_list &s, const sm_row &w, const sm
     }
     if (t == 0) s.n = n;
     __syncthreads();
-    if (t < 64) {
-        const uint64_t border = n <= 64 ? sm_end<1>(s, set, all, b, up) : n <= 512 ? sm_end<8>(s, set, all, b, up) : sm_end<0>(s, set, all, b, up);
+    if (n > SM_ALONE) {
+        const uint64_t border = sm_end<sm_together>(s, set, all, b, up);
+        if (t == 0) s.border = border;
+    } else if (t < 64) {
+        const uint64_t border = sm_end<sm_alone>(s, set, all, b, up);
         if (t == 0) s.border = border;
     }
     __syncthreads();
     return true;
 }
-// The token among the list's ids that stay, by a wave, and their units.
-template <int U>
-__device__ __forceinline__ uint32_t sm_choose(const sm_list &list, float u, uint64_t &whole) {
-    const sm_wave<U> v(list);
-    auto in = [&](uint32_t k, uint32_t d, uint32_t bin) { return ((uint64_t)k << 32 | d) >= list.border && !(bin & SM_LOW); };
-    whole = v.units(in);
-    return ~v.template top<true>(0, (uint64_t)((double)u * (double)whole) + 1, in);
+
+// The token among the list's ids that stay, and their units.
+template <typename Over>
+__device__ __forceinline__ uint32_t sm_choose(sm_list &list, float u, uint64_t &whole) {
+    Over v(list);
+    const uint64_t border = list.border;
+    auto stays = [&](uint32_t k, uint32_t d, uint32_t bin) { return ((uint64_t)k << 32 | d) >= border && !(bin & SM_LOW); };
+    whole = v.units(stays);
+    return ~v.template top<true>(0, (uint64_t)((double)u * (double)whole) + 1, stays);
 }
 
 // The token of a row's part in which the units pass `want` (counted from the part's start), and the part's probabilities.
@@ -535,6 +566,8 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a,
     __shared__ uint32_t least, tmp32[SM_WAVES];
     __shared__ sm_border found;
     __shared__ sm_list list;
+    __shared__ uint32_t ranks[4][SM_RANKED];
+    __shared__ uint64_t aheads[4][SM_RANKED];
     const uint32_t t = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
     const sm_row w = sm_at(p, r);
     const sm_set s = sm_settings(a, p, r);
@@ -543,14 +576,92 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a,
     if (!all.ok) return;
     if (s.few) {
         const double up = 0x1p54;           // 2^7 ids at most
+        const uint32_t listed = *w.listed;
+        if (listed <= SM_RANKED) {
+            // each entry against all: four groups of waves take a quarter of the others each, for 64 or 128 entries
+            const uint32_t l = t & 63, half = t >> 6 & 1, j = 64 * half + l, from = (t >> 7) * (SM_RANKED / 4);
+            if (t < SM_RANKED) {
+                const uint64_t o = t < listed ? w.list[t] : 0;
+                const double y = t < listed ? sm_weight(sm_value((uint32_t)(o >> 32)), all.top, s.inv) : 0.0;
+                list.order[t] = o;
+                list.unit[t] = sm_units(y, up);
+                list.bin[t] = t < listed && (y >= (double)s.min_p || sm_value((uint32_t)(o >> 32)) == all.top) ? 0 : SM_LOW;
+            }
+            __syncthreads();
+            uint32_t rank = 0;
+            uint64_t ahead = 0;
+            if (64 * half < listed) {
+                const uint64_t o = list.order[j];
+                for (uint32_t i = from; i < min(from + SM_RANKED / 4, listed); i++)
+                    if (list.order[i] > o) { rank++; ahead += list.unit[i]; }
+            }
+            ranks[t >> 7][j] = rank;
+            aheads[t >> 7][j] = ahead;
+            __syncthreads();
+            if (t >= 64) return;
+            // lane l has entries l and 64 + l
+            uint64_t unit[2], before[2], kept = 0;
+            uint32_t id[2];
+            bool stays[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint32_t x = 64 * i + l, k = ranks[0][x] + ranks[1][x] + ranks[2][x] + ranks[3][x];
+                before[i] = aheads[0][x] + aheads[1][x] + aheads[2][x] + aheads[3][x];
+                unit[i] = list.unit[x];
+                id[i] = ~(uint32_t)list.order[x];
+                stays[i] = x < listed && k < s.top_k;
+                kept += stays[i] ? unit[i] : 0;
+            }
+            if (s.top_p < 1.0f) {
+                const double want = ceil((double)s.top_p * (double)wave_sum(kept));
+                const uint64_t units = want > 1.0 ? (uint64_t)want : 1;
+                stays[0] = stays[0] && before[0] < units;
+                stays[1] = stays[1] && before[1] < units;
+            }
+            kept = 0;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                stays[i] = stays[i] && !(list.bin[64 * i + l] & SM_LOW);
+                kept += stays[i] ? unit[i] : 0;
+            }
+            const uint64_t whole = wave_sum(kept), want = (uint64_t)((double)s.u * (double)whole);
+            // the units of the ids up to an entry's own, over those that stay
+            uint64_t upto[2] = {0, 0};
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                uint64_t left = __builtin_amdgcn_ballot_w64(stays[i]);
+                if (a.probs && stays[i]) {
+                    const uint32_t at = m + lanes_below(left);
+                    w.out[1 + 2 * at] = id[i];
+                    w.out[2 + 2 * at] = __float_as_uint((float)(sm_weight(sm_value((uint32_t)(list.order[64 * i + l] >> 32)), all.top, s.inv) * up / (double)whole));
+                }
+                m += (uint32_t)__popcll(left);
+                for (; left; left &= left - 1) {
+                    const int x = __builtin_ctzll(left);
+                    const uint32_t d = (uint32_t)__builtin_amdgcn_readlane((int)id[i], x);
+                    const uint64_t y = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(unit[i] >> 32), x) << 32 |
+                                       (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)unit[i], x);
+                    if (d <= id[0]) upto[0] += y;
+                    if (d <= id[1]) upto[1] += y;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if (stays[i] && unit[i] && upto[i] > want && upto[i] - unit[i] <= want) a.token[r] = id[i];
+            if (t == 0) w.out[0] = m;
+            return;
+        }
         const sm_border b = {0, 0, s.top_p < 1.0f ? 0 : SM_BINS, 0, 0, 0, 0, 0};
         if (!sm_resolve(list, w, s, all, b, up, 0.0f)) return;
-        if (t >= 64) return;
-        auto in = [&](uint32_t j) { return list.order[j] >= list.border && !(list.bin[j] & SM_LOW); };
+        const uint64_t border = list.border;
         uint64_t whole;
-        const uint32_t id = list.n <= 64 ? sm_choose<1>(list, s.u, whole) : list.n <= 512 ? sm_choose<8>(list, s.u, whole) : sm_choose<0>(list, s.u, whole);
+        uint32_t id;
+        if (list.n > SM_ALONE) id = sm_choose<sm_together>(list, s.u, whole);
+        else if (t < 64) id = sm_choose<sm_alone>(list, s.u, whole);
         if (t == 0) a.token[r] = id;
-        if (!a.probs) return;
+        if (!a.probs || t >= 64) return;
+        auto in = [&](uint32_t j) { return list.order[j] >= border && !(list.bin[j] & SM_LOW); };
         uint32_t n = 0;
         for (uint32_t j0 = 0; j0 < list.n; j0 += 64) {
             const uint32_t j = j0 + t;
@@ -775,7 +886,7 @@ __device__ __forceinline__ void sm_slow(const sgk_sample_args &a, uint32_t r, co
 }
 // ---- 4
 __global__ void __launch_bounds__(SM_THREADS) k_sample_last(sgk_sample_args a, sm_plan p, int al) {
-    __shared__ uint64_t tmp[SM_WAVES];
+    __shared__ uint64_t tmp[SM_WAVES], sums[3][SM_WAVES];
     __shared__ uint32_t least;
     __shared__ sm_list list;
     const uint32_t t = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
@@ -823,9 +934,14 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_last(sgk_sample_args a, s
             if (id < i0) before += list.unit[j];
             else if (id < i1) mine += list.unit[j];
         }
-    whole = sm_sum(whole, tmp);
-    before = sm_sum(before, tmp);
-    mine = sm_sum(mine, tmp);
+    whole = wave_sum(whole);
+    before = wave_sum(before);
+    mine = wave_sum(mine);
+    if ((t & 63) == 0) { sums[0][t >> 6] = whole; sums[1][t >> 6] = before; sums[2][t >> 6] = mine; }
+    __syncthreads();
+    whole = before = mine = 0;
+#pragma unroll
+    for (int i = 0; i < SM_WAVES; i++) { whole += sums[0][i]; before += sums[1][i]; mine += sums[2][i]; }
     const uint64_t want = (uint64_t)((double)s.u * (double)whole), border = list.border;
     sm_pick(a, p, r, part, al, s, all.top, up, (double)whole, want >= before && want < before + mine, want - before, tmp, &least,
             [&](float x, uint32_t i) {
@@ -834,10 +950,11 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_last(sgk_sample_args a, s
             });
 }
 
-static sm_plan sm_plan_of(uint32_t vocab, void *at) {
+// Parts of a row: one round each until the rows have SM_WGS of them together.
+static sm_plan sm_plan_of(uint32_t vocab, uint32_t rows, void *at) {
     sm_plan p;
-    const uint64_t chunks = ((uint64_t)vocab + SM_IDS - 1) / SM_IDS;
-    p.rounds = (uint32_t)((chunks + SM_PARTS - 1) / SM_PARTS);
+    const uint64_t chunks = ((uint64_t)vocab + SM_IDS - 1) / SM_IDS, most = min(SM_PARTS, max(SM_WGS / rows, 8u));
+    p.rounds = (uint32_t)((chunks + most - 1) / most);
     p.parts = (uint32_t)((chunks + p.rounds - 1) / p.rounds);
     p.row_bytes = sm_row_bytes(p.parts);
     p.at = (char *)at;
@@ -845,9 +962,9 @@ static sm_plan sm_plan_of(uint32_t vocab, void *at) {
 }
 // Rows go by SM_ROWS at a time, so that the scratch memory has an end.
 #define SM_ROWS 1024u
-extern "C" uint64_t sgk_sample_scratch(const sgk_sample_args *a) { return sm_plan_of(a->vocab, NULL).row_bytes * min(a->rows, SM_ROWS); }
+extern "C" uint64_t sgk_sample_scratch(const sgk_sample_args *a) { return sm_plan_of(a->vocab, min(a->rows, SM_ROWS), NULL).row_bytes * min(a->rows, SM_ROWS); }
 extern "C" hipError_t sgk_sample(const sgk_sample_args *a, void *scratch, hipStream_t s, hipEvent_t done) {
-    const sm_plan p = sm_plan_of(a->vocab, scratch);
+    const sm_plan p = sm_plan_of(a->vocab, min(a->rows, SM_ROWS), scratch);
     const int al = !(((uintptr_t)a->x | (uintptr_t)a->probs) & 15) && a->vocab % 4 == 0;
     for (uint32_t r = 0; r < a->rows; r += SM_ROWS) {
         sgk_sample_args b = *a;
