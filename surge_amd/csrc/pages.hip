@@ -371,66 +371,103 @@ __global__ void __launch_bounds__(AP_WAVES * 64, 2) k_attn_paged(sgk_attn_paged_
     }
 }
 
-// The largest of n parts' maxima of a head, and the sum of the parts' sums under it: a wave, all lanes get them. f: the
-// parts' factors, or NULL.
-__device__ __forceinline__ f32x2 ap_maxsum(const ap_part &w, uint64_t at, uint32_t n, uint32_t stride, float *f) {
+// A head's parts, one a lane (of the first 64; the others are read when they are needed).
+struct ap_lane { float m, l; };
+__device__ __forceinline__ ap_lane ap_read(const ap_part &w, uint64_t at, uint32_t i, uint32_t n, uint32_t stride) {
+    if (i >= n) return (ap_lane){-INFINITY, 0.0f};
+    return (ap_lane){w.m[at + (uint64_t)i * stride], w.l[at + (uint64_t)i * stride]};
+}
+__device__ __forceinline__ float ap_factor(float mi, float m) { return mi > -INFINITY ? exp2f((mi - m) * 1.44269504f) : 0.0f; }
+// The largest of the parts' maxima, and the sum of their sums under it: a wave, all lanes get them. f: the parts'
+// factors, or NULL.
+__device__ __forceinline__ f32x2 ap_maxsum(const ap_part &w, ap_lane x, uint64_t at, uint32_t n, uint32_t stride, float *f) {
     const uint32_t l = threadIdx.x & 63;
-    float m = -INFINITY, sum = 0.0f;
-    for (uint32_t i = l; i < n; i += 64) m = fmaxf(m, w.m[at + (uint64_t)i * stride]);
+    float m = x.m;
+    for (uint32_t i = l + 64; i < n; i += 64) m = fmaxf(m, ap_read(w, at, i, n, stride).m);
     m = wave_fmax(m);
+    float sum = 0.0f;
     for (uint32_t i = l; i < n; i += 64) {
-        const float mi = w.m[at + (uint64_t)i * stride], fi = mi > -INFINITY ? exp2f((mi - m) * 1.44269504f) : 0.0f;
-        sum = fmaf(fi, w.l[at + (uint64_t)i * stride], sum);
+        if (i != l) x = ap_read(w, at, i, n, stride);
+        const float fi = ap_factor(x.m, m);
+        sum = fmaf(fi, x.l, sum);
         if (f) f[i] = fi;
     }
     return (f32x2){m, wave_fsum(sum)};
 }
 // A workgroup per 64 dims of a query head and sequence adds the parts, four dims a lane, the parts by 16 lane groups in turn.
-// Where the weights are wanted, the workgroups behind take a sequence's slots, one kv head each.
+// Where the weights are wanted, the workgroups behind take a sequence's slots, one kv head each. Whatever can be asked
+// for is, before the first of it is waited for: the launch is three trips to memory long.
 __global__ void __launch_bounds__(TPB) k_attn_paged_join(sgk_attn_paged_args a, ap_part w) {
     __shared__ float f[AP_MOST];
     __shared__ f32x4 red[TPB];
     __shared__ f32x2 ml[16];
-    const uint32_t t = threadIdx.x, s = blockIdx.y, hd = a.c.hd, g = a.n_heads / a.c.n_kv;
+    const uint32_t t = threadIdx.x, s = blockIdx.y, hd = a.c.hd, g = a.n_heads / a.c.n_kv, adders = a.n_heads * (hd / 64);
     const ap_where me = ap_find(a, w, s, false);
-    const uint32_t adders = a.n_heads * (hd / 64);
     if (blockIdx.x < adders) {
         const uint32_t head = blockIdx.x / (hd / 64), d = blockIdx.x % (hd / 64) * 64 + t % 16 * 4;
         const uint64_t at = (uint64_t)me.first * a.n_heads + head;
+        ap_lane x = {};
+        if (t < 64) x = ap_read(w, at, t, me.n, a.n_heads);
+        const float *acc = w.acc + at * hd + d;
+        constexpr uint32_t A = 4, G = TPB / 16;
+        f32x4 o = {0, 0, 0, 0}, y[A];
+#pragma unroll
+        for (uint32_t i = 0; i < A; i++) y[i] = t / 16 + i * G < me.n ? *(const f32x4 *)(acc + (uint64_t)(t / 16 + i * G) * a.n_heads * hd) : (f32x4){0, 0, 0, 0};
         if (t < 64) {
-            const f32x2 r = ap_maxsum(w, at, me.n, a.n_heads, f);
+            const f32x2 r = ap_maxsum(w, x, at, me.n, a.n_heads, f);
             if (t == 0) ml[0] = r;
         }
         __syncthreads();
-        f32x4 o = {0, 0, 0, 0};
-        const float *acc = w.acc + at * hd + d;
-#pragma unroll 8
-        for (uint32_t i = t / 16; i < me.n; i += TPB / 16) o += f[i] * *(const f32x4 *)(acc + (uint64_t)i * a.n_heads * hd);
+#pragma unroll
+        for (uint32_t i = 0; i < A; i++)
+            if (t / 16 + i * G < me.n) o += f[t / 16 + i * G] * y[i];
+#pragma unroll 4
+        for (uint32_t i = t / 16 + A * G; i < me.n; i += G) o += f[i] * *(const f32x4 *)(acc + (uint64_t)i * a.n_heads * hd);
         red[t] = o;
         __syncthreads();
         if (t >= 16) return;
 #pragma unroll
-        for (uint32_t i = 1; i < TPB / 16; i++) o += red[t + i * 16];
+        for (uint32_t i = 1; i < G; i++) o += red[t + i * 16];
         const float l = ml[0][1];
 #pragma unroll
         for (int e = 0; e < 4; e++) a.out[((uint64_t)s * a.n_heads + head) * hd + d + e] = l == 0.0f ? 0.0f : o[e] / l;
         return;
     }
     const uint32_t x = blockIdx.x - adders, h = x % a.c.n_kv, nb = (gridDim.x - adders) / a.c.n_kv, len = page_len(a.c, a.lens, s);
-    const uint64_t cap = (uint64_t)a.c.width << a.c.log, at = ((uint64_t)s * a.c.n_kv + h) * cap;
-    if ((x / a.c.n_kv) * TPB >= len) return;
-    for (uint32_t c = t >> 6; c < g; c += TPB / 64) {
-        const f32x2 r = ap_maxsum(w, (uint64_t)me.first * a.n_heads + h * g + c, me.n, a.n_heads, NULL);
+    const uint64_t cap = (uint64_t)a.c.width << a.c.log, at = ((uint64_t)s * a.c.n_kv + h) * cap, head0 = (uint64_t)me.first * a.n_heads + h * g;
+    uint32_t j = (x / a.c.n_kv) * TPB + t;
+    if (j - t >= len) return;
+    ap_lane y[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; i++)
+        if (t / 64 + 4 * i < g) y[i] = ap_read(w, head0 + t / 64 + 4 * i, t & 63, me.n, a.n_heads);
+    const float *sc = w.score + ((uint64_t)s * a.n_heads + h * g) * cap;
+    float z[16], before = 0.0f;
+    auto fetch = [&]() {
+        if (j >= len) return;
+#pragma unroll
+        for (uint32_t c = 0; c < 16; c++)
+            if (c < g) z[c] = sc[c * cap + j];
+        before = a.weight ? a.weight[at + j] : 0.0f;
+    };
+    fetch();
+#pragma unroll
+    for (uint32_t i = 0; i < 4; i++) {
+        const uint32_t c = t / 64 + 4 * i;
+        if (c >= g) break;
+        const f32x2 r = ap_maxsum(w, y[i], head0 + c, me.n, a.n_heads, NULL);
         if ((t & 63) == 0) ml[c] = (f32x2){r[0], (float)(1 << AP_P2) / r[1]};
     }
     __syncthreads();
-    for (uint32_t j = (x / a.c.n_kv) * TPB + t; j < len; j += nb * TPB) {
+    while (j < len) {
         float sum = 0.0f;
-        const float *sc = w.score + ((uint64_t)s * a.n_heads + h * g) * cap + j;
         // a slot that is not there has -inf for a score, and so no weight
-        for (uint32_t c = 0; c < g; c++)
-            if (sc[c * cap] != -INFINITY) sum = fmaf(exp2f((sc[c * cap] - ml[c][0]) * 1.44269504f), ml[c][1], sum);
-        a.weight_out[at + j] = (a.weight ? a.weight[at + j] : 0.0f) + sum;
+#pragma unroll
+        for (uint32_t c = 0; c < 16; c++)
+            if (c < g && z[c] != -INFINITY) sum = fmaf(exp2f((z[c] - ml[c][0]) * 1.44269504f), ml[c][1], sum);
+        a.weight_out[at + j] = before + sum;
+        j += nb * TPB;
+        fetch();
     }
 }
 static ap_part ap_plan(const sgk_attn_paged_args *a, char *at, uint64_t *bytes) {
