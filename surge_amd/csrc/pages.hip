@@ -512,10 +512,11 @@ extern "C" hipError_t sgk_attn_paged(const sgk_attn_paged_args *a, void *scratch
         if (e != hipSuccess) return e;
     }
     launch_lds(k, grid, AP_WAVES * 64, lds, s, (hipEvent_t)NULL, *a, w, al);
-    uint32_t more = 0;      // workgroups a kv head for the weights
+    uint32_t more = 0;      // workgroups a kv head for the weights: about 1024 in all, or 16 (16 x 4 heads: 16 9.8 us, 64 11.7; 8 heads: 16 10.8, 64 6.4)
     if (a->weight_out) {
         const uint64_t need = (((uint64_t)a->c.width << a->c.log) + TPB - 1) / TPB;
-        more = (uint32_t)(need < 64 ? need : 64);
+        const uint32_t most = max(16u, 1024u / (a->c.n_seq * a->c.n_kv));
+        more = (uint32_t)(need < most ? need : most);
     }
     launch(k_attn_paged_join, dim3(a->n_heads * (hd / 64) + more * a->c.n_kv, a->c.n_seq), TPB, s, done, *a, w);
     return hipGetLastError();
@@ -537,6 +538,7 @@ extern "C" hipError_t sgk_attn_paged(const sgk_attn_paged_args *a, void *scratch
 #define EV_HELD 32896u      // keys in LDS: 128 a page past 32768, so that a prompt's new slots fit too
 #define EV_THREADS 1024
 #define EV_BINS 2048u
+#define EV_LIST 2048u       // keys of the first histogram's bin that are listed
 #define EV_OUT 8u          // rows too many that go one by one
 struct ev_list { uint32_t *hole, *mover, *n; };      // [row][most] twice, [row]: rows to move; NULL: the few are moved at once
 __host__ __device__ static inline uint32_t ev_most(uint32_t keep, uint32_t cap) { return keep < cap - keep ? keep : cap - keep; }
@@ -582,7 +584,7 @@ template <bool HELD>
 __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a, ev_list w) {
     constexpr uint32_t T = EV_THREADS, W = T / 64, PER = EV_BINS / T;
     extern __shared__ uint32_t held[];
-    __shared__ uint32_t bins[EV_BINS], tmp[2][16], marks[T], pick[3];
+    __shared__ uint32_t bins[EV_BINS], tmp[2][16], marks[T], pick[4], list[EV_LIST];
     __shared__ int32_t lasts[W];
     __shared__ uint32_t few[2][EV_FEW], gone[EV_OUT];
     __shared__ uint64_t out[2][16];
@@ -601,7 +603,7 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a
     if (len <= a.keep) return;
     for (uint32_t i = t; i < EV_BINS; i += T) bins[i] = 0;
     int32_t last = INT32_MIN;
-#pragma unroll 8
+#pragma unroll 16
     for (uint32_t j = t; j < len; j += T) {
         const int32_t p = ps[j];
         last = max(last, p);
@@ -613,7 +615,7 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a
 #pragma unroll
     for (uint32_t i = 0; i < W; i++) last = max(last, lasts[i]);
     if (HELD) {
-#pragma unroll 8
+#pragma unroll 16
         for (uint32_t j = t; j < len; j += T) held[j] = ev_key(wt[j], (int32_t)held[j], last, a.recent);     // a thread's own
         __syncthreads();
     }
@@ -665,7 +667,7 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a
     } else {
     const uint32_t spans = (len + 63) / 64;
     // the keep-th key: `left` of the `here` keys with the border's upper bits stay
-    uint32_t border = 0, left = keep, here = len;
+    uint32_t border = 0, left = keep, here = len, listed = UINT32_MAX;
     int at = 0;
     for (int pass = 0; pass < 3 && left != here; pass++) {
         const uint32_t shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, mask = pass == 2 ? 1023u : 2047u, up = pass == 0 ? 31 : pass == 1 ? 21 : 10;
@@ -673,21 +675,17 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a
             for (uint32_t i = t; i < EV_BINS; i += T) bins[i] = 0;
             __syncthreads();
         }
-        for (uint32_t i0 = wv * 4; i0 < spans; i0 += W * 4) {
-            uint32_t key[4];
-#pragma unroll
-            for (uint32_t i = 0; i < 4; i++) key[i] = key_of(min((i0 + i) * 64 + l, len - 1));
-#pragma unroll
-            for (uint32_t i = 0; i < 4; i++) {
-                const uint32_t d = key[i] >> shift & mask;
-                const bool in = (i0 + i) * 64 + l < len && (!pass || (key[i] ^ border) >> up == 0);
-                const uint64_t m = __builtin_amdgcn_ballot_w64(in);
-                if (!m) continue;
-                // the first lane's bin is often most lanes': they add once
-                const uint32_t f = (uint32_t)__builtin_amdgcn_readlane((int)d, (int)__builtin_ctzll(m));
-                const uint64_t same = __builtin_amdgcn_ballot_w64(in && d == f);
-                if (l == 0) atomicAdd(&bins[f], (uint32_t)__popcll(same));
-                if (in && d != f) atomicAdd(&bins[d], 1u);
+        if (pass == 0) {
+#pragma unroll 8
+            for (uint32_t j = t; j < len; j += T) atomicAdd(&bins[key_of(j) >> 21], 1u);
+        } else if (listed <= EV_LIST) {
+            for (uint32_t i = t; i < listed; i += T)
+                if ((list[i] ^ border) >> up == 0) atomicAdd(&bins[list[i] >> shift & mask], 1u);
+        } else {
+#pragma unroll 8
+            for (uint32_t j = t; j < len; j += T) {
+                const uint32_t key = key_of(j);
+                if ((key ^ border) >> up == 0) atomicAdd(&bins[key >> shift & mask], 1u);
             }
         }
         __syncthreads();
@@ -712,6 +710,16 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a
         border |= pick[0] << shift;
         left -= pick[1];
         here = pick[2];
+        if (pass == 0 && left != here && here <= EV_LIST) {         // the other passes over that bin's keys alone
+            listed = here;
+            if (t == 0) pick[3] = 0;
+            __syncthreads();
+#pragma unroll 8
+            for (uint32_t j = t; j < len; j += T) {
+                const uint32_t key = key_of(j);
+                if (key >> 21 == border >> 21) list[atomicAdd(&pick[3], 1u)] = key;
+            }
+        }
     }
     // Keys above the border stay and all of its own, or its own up to slot `tie`. A pass that was not needed left
     // lower bits 0.
@@ -738,20 +746,36 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a
         const uint64_t m = __builtin_amdgcn_ballot_w64(mine);
         tie = pick[0] * 64 + (uint32_t)__builtin_ctzll(__builtin_amdgcn_ballot_w64(mine && pick[1] + lanes_below(m) + 1 == left));
     }
-    auto marked = [&](uint32_t j) {
-        const uint32_t key = key_of(min(j, len - 1));
-        return j < len && (j < keep) != (key > border || (key == border && j <= tie));
+    // of four 64s of slots from i0 on, which of a lane's are freed (below keep) or moved (from keep on)
+    auto marked = [&](uint32_t i0, bool (&m)[4]) {
+        uint32_t key[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) key[i] = key_of(min((i0 + i) * 64 + l, len - 1));
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            const uint32_t j = (i0 + i) * 64 + l;
+            const bool stays = tie == UINT32_MAX ? key[i] >= border : key[i] > border || (key[i] == border && j <= tie);
+            m[i] = j < len && (j < keep) != stays;
+        }
     };
     // the marks of each 64 slots, and all of them
-    for (uint32_t i0 = 0; i0 < spans; i0 += T) {
-        __syncthreads();
-        for (uint32_t i = i0 + wv; i < min(i0 + T, spans); i += W) {
-            const uint64_t m = __builtin_amdgcn_ballot_w64(marked(i * 64 + l));
-            if (l == 0) marks[i - i0] = (uint32_t)__popcll(m);
+    auto count = [&](uint32_t s0) {
+        for (uint32_t i0 = s0 + 4 * wv; i0 < min(s0 + T, spans); i0 += 4 * W) {
+            bool m[4];
+            marked(i0, m);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const uint64_t b = __builtin_amdgcn_ballot_w64(m[i]);
+                if (l == 0) marks[i0 + i - s0] = (uint32_t)__popcll(b);
+            }
         }
         __syncthreads();
+    };
+    for (uint32_t s0 = 0; s0 < spans; s0 += T) {
+        __syncthreads();
+        count(s0);
         uint32_t all;
-        const uint32_t before = ev_scan(i0 + t < spans ? marks[t] : 0, &all, tmp, at);
+        const uint32_t before = ev_scan(s0 + t < spans ? marks[t] : 0, &all, tmp, at);
         if (spans <= T) {
             __syncthreads();
             marks[t] = before;
@@ -760,26 +784,25 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a
     }
     moves /= 2;
     uint32_t seen = 0;
-    for (uint32_t i0 = 0; i0 < spans; i0 += T) {
+    for (uint32_t s0 = 0; s0 < spans; s0 += T) {
         __syncthreads();
         if (spans > T) {        // again, a part of them at a time
-            for (uint32_t i = i0 + wv; i < min(i0 + T, spans); i += W) {
-                const uint64_t m = __builtin_amdgcn_ballot_w64(marked(i * 64 + l));
-                if (l == 0) marks[i - i0] = (uint32_t)__popcll(m);
-            }
-            __syncthreads();
+            count(s0);
             uint32_t all;
-            const uint32_t before = seen + ev_scan(i0 + t < spans ? marks[t] : 0, &all, tmp, at);
+            const uint32_t before = seen + ev_scan(s0 + t < spans ? marks[t] : 0, &all, tmp, at);
             __syncthreads();
             marks[t] = before;
             seen += all;
             __syncthreads();
         }
-        for (uint32_t i = i0 + wv; i < min(i0 + T, spans); i += W) {
-            const uint32_t j = i * 64 + l;
-            const bool m = marked(j);
-            const uint32_t r = marks[i - i0] + lanes_below(__builtin_amdgcn_ballot_w64(m));
-            if (m) *(j < keep ? holes + r : movers + (r - moves)) = j;
+        for (uint32_t i0 = s0 + 4 * wv; i0 < min(s0 + T, spans); i0 += 4 * W) {
+            bool m[4];
+            marked(i0, m);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                const uint32_t j = (i0 + i) * 64 + l, r = marks[i0 + i - s0] + lanes_below(__builtin_amdgcn_ballot_w64(m[i]));
+                if (m[i]) *(j < keep ? holes + r : movers + (r - moves)) = j;
+            }
         }
     }
     }
