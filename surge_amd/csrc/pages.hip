@@ -597,28 +597,45 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a
     float *wo = a.weight_out + row * cap;
     int32_t *po = a.pos_out + row * cap;
     if (t == 0 && w.n) w.n[row] = 0;
-    // all of the first `keep`; moved rows come over them, behind a barrier or a launch
-    if (wo != wt) for (uint32_t j = t; j < keep; j += T) wo[j] = wt[j];
-    if (po != ps) for (uint32_t j = t; j < keep; j += T) po[j] = ps[j];
-    if (len <= a.keep) return;
+    // all of the first `keep` to the outputs; moved rows come over them, behind a barrier or a launch
+    const bool cw = wo != wt, cp = po != ps;
+    if (len <= a.keep) {
+        if (cw) for (uint32_t j = t; j < keep; j += T) wo[j] = wt[j];
+        if (cp) for (uint32_t j = t; j < keep; j += T) po[j] = ps[j];
+        return;
+    }
     for (uint32_t i = t; i < EV_BINS; i += T) bins[i] = 0;
+    // eight of a thread's slots under way, the last one in place of those behind it
     int32_t last = INT32_MIN;
-#pragma unroll 16
-    for (uint32_t j = t; j < len; j += T) {
-        const int32_t p = ps[j];
-        last = max(last, p);
-        if (HELD) held[j] = (uint32_t)p;
+    for (uint32_t j0 = t; j0 - t < len; j0 += 8 * T) {
+        int32_t p[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) p[i] = ps[min(j0 + i * T, len - 1)];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t j = j0 + i * T;
+            last = max(last, p[i]);
+            if (HELD && j < len) held[j] = (uint32_t)p[i];
+            if (cp && j < keep) po[j] = p[i];
+        }
     }
     last = (int32_t)(wave_umax((uint32_t)last ^ 0x80000000u) ^ 0x80000000u);
     if (l == 0) lasts[wv] = last;
     __syncthreads();
 #pragma unroll
     for (uint32_t i = 0; i < W; i++) last = max(last, lasts[i]);
-    if (HELD) {
-#pragma unroll 16
-        for (uint32_t j = t; j < len; j += T) held[j] = ev_key(wt[j], (int32_t)held[j], last, a.recent);     // a thread's own
-        __syncthreads();
+    for (uint32_t j0 = t; j0 - t < len && (HELD || (cw && j0 - t < keep)); j0 += 8 * T) {
+        float y[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) y[i] = wt[min(j0 + i * T, len - 1)];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t j = j0 + i * T;
+            if (HELD && j < len) held[j] = ev_key(y[i], (int32_t)held[j], last, a.recent);      // a thread's own
+            if (cw && j < keep) wo[j] = y[i];
+        }
     }
+    __syncthreads();
     auto key_of = [&](uint32_t j) { return HELD ? held[j] : ev_key(wt[j], ps[j], last, a.recent); };
     uint32_t moves = 0;
     uint32_t *const holes = w.n ? w.hole + row * ev_most(a.keep, cap) : few[0], *const movers = w.n ? w.mover + row * ev_most(a.keep, cap) : few[1];
@@ -676,8 +693,14 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a
             __syncthreads();
         }
         if (pass == 0) {
-#pragma unroll 8
-            for (uint32_t j = t; j < len; j += T) atomicAdd(&bins[key_of(j) >> 21], 1u);
+            for (uint32_t j0 = t; j0 - t < len; j0 += 8 * T) {
+                uint32_t key[8];
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++) key[i] = key_of(min(j0 + i * T, len - 1));
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++)
+                    if (j0 + i * T < len) atomicAdd(&bins[key[i] >> 21], 1u);
+            }
         } else if (listed <= EV_LIST) {
             for (uint32_t i = t; i < listed; i += T)
                 if ((list[i] ^ border) >> up == 0) atomicAdd(&bins[list[i] >> shift & mask], 1u);
@@ -714,10 +737,13 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a
             listed = here;
             if (t == 0) pick[3] = 0;
             __syncthreads();
-#pragma unroll 8
-            for (uint32_t j = t; j < len; j += T) {
-                const uint32_t key = key_of(j);
-                if (key >> 21 == border >> 21) list[atomicAdd(&pick[3], 1u)] = key;
+            for (uint32_t j0 = t; j0 - t < len; j0 += 8 * T) {
+                uint32_t key[8];
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++) key[i] = key_of(min(j0 + i * T, len - 1));
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++)
+                    if (key[i] >> 21 == border >> 21 && j0 + i * T < len) list[atomicAdd(&pick[3], 1u)] = key[i];
             }
         }
     }
@@ -758,9 +784,13 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a
             m[i] = j < len && (j < keep) != stays;
         }
     };
-    // the marks of each 64 slots, and all of them
+    // The marks of each 64 slots, T of those at a time, and their prefix sums. A lane's marks are the bits of `mine`.
+    uint64_t mine = 0;
+    static_assert(T / W <= 64, "a bit for each 64 slots of a wave");
     auto count = [&](uint32_t s0) {
-        for (uint32_t i0 = s0 + 4 * wv; i0 < min(s0 + T, spans); i0 += 4 * W) {
+        mine = 0;
+        uint32_t at = 0;
+        for (uint32_t i0 = s0 + 4 * wv; i0 < min(s0 + T, spans); i0 += 4 * W, at += 4) {
             bool m[4];
             marked(i0, m);
 #pragma unroll
@@ -768,40 +798,47 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a
                 const uint64_t b = __builtin_amdgcn_ballot_w64(m[i]);
                 if (l == 0) marks[i0 + i - s0] = (uint32_t)__popcll(b);
             }
+            mine |= (uint64_t)(m[0] | m[1] << 1 | m[2] << 2 | m[3] << 3) << at;
         }
         __syncthreads();
     };
-    for (uint32_t s0 = 0; s0 < spans; s0 += T) {
-        __syncthreads();
-        count(s0);
-        uint32_t all;
-        const uint32_t before = ev_scan(s0 + t < spans ? marks[t] : 0, &all, tmp, at);
-        if (spans <= T) {
-            __syncthreads();
-            marks[t] = before;
-        }
-        moves += all;
-    }
-    moves /= 2;
     uint32_t seen = 0;
-    for (uint32_t s0 = 0; s0 < spans; s0 += T) {
+    auto number = [&](uint32_t s0) {
+        uint32_t all;
+        const uint32_t before = seen + ev_scan(s0 + t < spans ? marks[t] : 0, &all, tmp, at);
         __syncthreads();
-        if (spans > T) {        // again, a part of them at a time
+        marks[t] = before;
+        seen += all;
+        __syncthreads();
+    };
+    if (spans <= T) {
+        __syncthreads();
+        count(0);
+        number(0);
+        moves = seen / 2;
+    } else {                    // all marks' number comes first
+        for (uint32_t s0 = 0; s0 < spans; s0 += T) {
+            __syncthreads();
             count(s0);
-            uint32_t all;
-            const uint32_t before = seen + ev_scan(s0 + t < spans ? marks[t] : 0, &all, tmp, at);
-            __syncthreads();
-            marks[t] = before;
-            seen += all;
-            __syncthreads();
+            number(s0);
         }
-        for (uint32_t i0 = s0 + 4 * wv; i0 < min(s0 + T, spans); i0 += 4 * W) {
-            bool m[4];
-            marked(i0, m);
+        moves = seen / 2;
+        seen = 0;
+    }
+    for (uint32_t s0 = 0; s0 < spans; s0 += T) {
+        if (spans > T) {
+            __syncthreads();
+            count(s0);
+            number(s0);
+        }
+        uint32_t at = 0;
+        for (uint32_t i0 = s0 + 4 * wv; i0 < min(s0 + T, spans); i0 += 4 * W, at += 4) {
+            const uint32_t four = (uint32_t)(mine >> at) & 15;
+            if (!__builtin_amdgcn_ballot_w64(four != 0)) continue;
 #pragma unroll
             for (uint32_t i = 0; i < 4; i++) {
-                const uint32_t j = (i0 + i) * 64 + l, r = marks[i0 + i - s0] + lanes_below(__builtin_amdgcn_ballot_w64(m[i]));
-                if (m[i]) *(j < keep ? holes + r : movers + (r - moves)) = j;
+                const uint32_t j = (i0 + i) * 64 + l, r = marks[i0 + i - s0] + lanes_below(__builtin_amdgcn_ballot_w64(four >> i & 1));
+                if (four >> i & 1) *(j < keep ? holes + r : movers + (r - moves)) = j;
             }
         }
     }
