@@ -428,7 +428,7 @@ sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void
  * conversations. kp, vp f16 pools [pages][page][n_kv][hd], 16-byte aligned; as many
  * pages as the smaller buffer holds whole. table int32 [n_seq][width]: slot j of
  * sequence s lies in page table[s][j / page] at row j % page. page = 16, 32, 64,
- * 128 or 256, hd = 64, 128 or 256, n_kv and n_seq <= 65535, width * page <= 2^30. A
+ * 128 or 256, hd = 64, 128 or 256, n_kv <= 65535, n_seq <= 32768, width * page <= 2^30. A
  * cache [seq][n_kv][hd] of sg_gpu_run_attn_decode_f16 is such a pool, its table 0, 1,
  * 2, ... A page number outside the pool is never followed: rows for its slots are
  * dropped, attention passes them over. Entries of the table past a sequence's length

@@ -1140,7 +1140,7 @@ static sg_err pages_check(const char *who, void *kp, void *vp, void *table, uint
                           uint32_t width, sgk_pages *c) {
     if (!sgk_pages_shape_ok(n_kv, hd, page))
         return errf("gpu: %s: n_kv in [1, 65535], head_dim 64, 128 or 256, page 16, 32, 64, 128 or 256", who);
-    if (!n_seq || n_seq > 65535) return errf("gpu: %s: n_seq must be in [1, 65535]", who);
+    if (!n_seq || n_seq > 32768) return errf("gpu: %s: n_seq must be in [1, 32768]", who);
     if (!width || (uint64_t)width * page > 1u << 30) return errf("gpu: %s: a sequence has 1 to 2^30 slots (width * page)", who);
     const uint64_t each = (uint64_t)page * n_kv * hd * 2;
     sg_err e;

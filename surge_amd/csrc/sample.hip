@@ -30,9 +30,7 @@
 #define SM_IDS (4 * SM_THREADS)
 #define SM_PARTS 512u       // of a row, at most: its parts take several rounds of SM_IDS past that
 #define SM_FEW 128u
-#ifndef SM_WGS
-#define SM_WGS 1024u
-#endif
+#define SM_WGS 1024u        // workgroups that a launch has about
 #define SM_LIST 2048u
 #define SM_RANKED 128u      // entries that are compared all with all
 #define SM_BINS 2048u
@@ -88,7 +86,7 @@ __device__ __forceinline__ uint32_t sm_key(float x) {
 }
 __device__ __forceinline__ float sm_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 __device__ __forceinline__ double sm_weight(float x, float top, double inv) {
-    return x == top ? 1.0 : x > -INFINITY ? exp(((double)x - (double)top) * inv) : 0.0;
+    return x == top ? 1.0 : x > -INFINITY && top < INFINITY ? exp(((double)x - (double)top) * inv) : 0.0;
 }
 __device__ __forceinline__ uint64_t sm_units(double w, double up) { return w > 0.0 ? max((uint64_t)1, (uint64_t)rint(w * up)) : 0; }
 // Over the workgroup, with 64 bits a wave in tmp.

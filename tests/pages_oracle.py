@@ -105,7 +105,7 @@ def sample(x, temperature, top_k, top_p, min_p, u):
         ids = ids[:top_k]
     top = x[ids[0]]
     with np.errstate(invalid="ignore", over="ignore"):
-        w = np.where(x[ids] == top, 1.0, np.exp((x[ids] - top) / temperature))
+        w = np.where(x[ids] == top, 1.0, np.exp((x[ids] - top) / temperature) if top < np.inf else 0.0)
     w = w.astype(np.longdouble)
     margin = 1.0
     if top_p < 1:

@@ -44,10 +44,10 @@ def changed(name, change):
 
 @pytest.mark.parametrize("name,change,match", [
     (STORE, {0: 0}, "n_kv"), (STORE, {0: 65536}, "n_kv"), (STORE, {1: 96}, "head_dim"), (STORE, {2: 8}, "page 16"), (STORE, {2: 48}, "page 16"),
-    (STORE, {2: 512}, "page 16"), (STORE, {3: 0}, "n_seq"), (STORE, {3: 65536}, "n_seq"), (STORE, {4: 0}, "slots"), (STORE, {4: 1 << 27}, "slots"),
+    (STORE, {2: 512}, "page 16"), (STORE, {3: 0}, "n_seq"), (STORE, {3: 32769}, "n_seq"), (STORE, {4: 0}, "slots"), (STORE, {4: 1 << 27}, "slots"),
     (STORE, {4: 0xFFFFFFFF}, "slots"), (STORE, {3: 4}, "table holds"), (STORE, {4: 5}, "table holds"), (STORE, {2: 256, 1: 128}, "kp holds"),
     (STORE, {5: 0}, "n must"), (STORE, {5: (1 << 27) + 1}, "n must"), (STORE, {5: 6}, "k holds"), (STORE, {6: 127}, "stride"),
-    (STORE, {6: 129}, "k holds"), (STORE, {3: 65535, 4: 1, 5: 1 << 27, 6: 0xFFFFFFFF}, "table holds"),
+    (STORE, {6: 129}, "k holds"), (STORE, {3: 32768, 4: 1, 5: 1 << 27, 6: 0xFFFFFFFF}, "table holds"),
     (ATTN, {0: 0}, "n_heads"), (ATTN, {0: 5}, "n_heads"), (ATTN, {0: 34}, "n_heads"), (ATTN, {1: 0}, "n_kv"), (ATTN, {2: 32}, "head_dim"),
     (ATTN, {3: 17}, "page 16"), (ATTN, {4: 0}, "n_seq"), (ATTN, {5: 0}, "slots"), (ATTN, {5: 5}, "table holds"), (ATTN, {6: 63}, "q_stride"),
     (ATTN, {6: 65}, "q holds"), (ATTN, {6: 0xFFFFFFFF}, "q holds"), (ATTN, {0: 8}, "q holds"),
