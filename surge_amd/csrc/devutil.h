@@ -94,6 +94,7 @@ __device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
     v += swap16(v);
     return v + swap32(v);
 }
+__device__ __forceinline__ float wave_sum(float v) { return wave_fsum(v); }
 __device__ __forceinline__ double wave_sum(double v) {
 #define WS_STEP(F) v += __longlong_as_double((long long)both<F>((uint64_t)__double_as_longlong(v)))
     WS_STEP(dppu<0xB1>); WS_STEP(dppu<0x4E>); WS_STEP(dppu<0x141>); WS_STEP(dppu<0x128>); WS_STEP(swap16); WS_STEP(swap32);

@@ -36,8 +36,8 @@
 #define SM_BINS 2048u
 #define SM_NONE 0xFFFFFFFFu
 
-// What the first launch found of a row: the largest and the lowest key, the ids that may be chosen, the weights' sum.
-struct sm_all { uint32_t best, low, ok; float top; double sum; };
+// What the first launch found of a row: the largest and the lowest key, the ids that may be chosen, the weights' sum roughly.
+struct sm_all { uint32_t best, low, ok; float top, sum; };
 // Where top_k and top_p end: the bin of top_k's last id (SM_BINS: no top_k), ids and units before that bin; the bins in
 // which top_p may end (SM_BINS: no top_p) and the units before them; the first bin that is listed; all units.
 struct sm_border { uint32_t kbin, kabove, plo, phi, first; uint64_t ksum, psum, whole; };
@@ -45,7 +45,7 @@ struct sm_border { uint32_t kbin, kabove, plo, phi, first; uint64_t ksum, psum, 
 // A row's place in the scratch memory.
 struct sm_row {
     uint32_t *wave, *low, *ok;          // [parts][SM_WAVES] largest keys, [parts] lowest, [parts] ids that may be chosen
-    double *sum;                        // [parts] of weights relative to the part's largest
+    float *sum;                         // [parts] of weights relative to the part's largest, roughly: for the units' size
     uint64_t *kept, *list, *binsum;     // [parts] units that stay, [SM_LIST] key and ~id, [SM_BINS]
     uint32_t *bincnt, *listed, *out;    // [SM_BINS], [1], [1 + 2 SM_FEW] few: number, ids, probabilities
     struct sm_all *all;                 // what 1 found, by 2
@@ -57,7 +57,7 @@ __device__ __forceinline__ sm_row sm_at(const sm_plan &p, uint32_t r) {
     char *c = p.at + r * p.row_bytes;
     sm_row w;
     auto take = [&](uint64_t bytes) { char *x = c; c += (bytes + 15) / 16 * 16; return x; };
-    w.sum = (double *)take(8 * p.parts);
+    w.sum = (float *)take(4 * p.parts);
     w.kept = (uint64_t *)take(8 * p.parts);
     w.list = (uint64_t *)take(8 * SM_LIST);
     w.binsum = (uint64_t *)take(8 * SM_BINS);
@@ -74,7 +74,7 @@ __device__ __forceinline__ sm_row sm_at(const sm_plan &p, uint32_t r) {
 static uint64_t sm_row_bytes(uint64_t parts) {
     uint64_t n = 0;
     auto take = [&](uint64_t bytes) { n += (bytes + 15) / 16 * 16; };
-    take(8 * parts); take(8 * parts); take(8 * SM_LIST); take(8 * SM_BINS); take(4 * SM_BINS);
+    take(4 * parts); take(8 * parts); take(8 * SM_LIST); take(8 * SM_BINS); take(4 * SM_BINS);
     take(4 * parts * SM_WAVES); take(4 * parts); take(4 * parts); take(4); take(4 * (1 + 2 * SM_FEW)); take(sizeof(sm_all)); take(sizeof(sm_border));
     return n;
 }
@@ -85,8 +85,23 @@ __device__ __forceinline__ uint32_t sm_key(float x) {
     return x > -INFINITY ? (b & 0x80000000u ? ~b : b | 0x80000000u) : 0;
 }
 __device__ __forceinline__ float sm_value(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+// exp(z), z <= 0: 2^k e^r, |r| <= ln 2 / 2, by the series to r^12 (the next term is below 2^-52 of it). ln 2 in two parts, the
+// first with 21 bits free below it, so that k times it is exact.
+__device__ __forceinline__ double sm_exp(double z) {
+    z = fmax(z, -1100.0);                       // 0 in 64 bits; NaN too
+    const double k = rint(z * 1.4426950408889634);
+    const double r = fma(-k, 0x1.a39ef35793c76p-33, fma(-k, 0x1.62e42feep-1, z));
+    double p = 1.0 / 479001600;
+    const double c[12] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320, 1.0 / 362880, 1.0 / 3628800, 1.0 / 39916800};
+#pragma unroll
+    for (int i = 11; i >= 0; i--) p = fma(p, r, c[i]);
+    return __builtin_amdgcn_ldexp(p, (int)k);
+}
 __device__ __forceinline__ double sm_weight(float x, float top, double inv) {
-    return x == top ? 1.0 : x > -INFINITY && top < INFINITY ? exp(((double)x - (double)top) * inv) : 0.0;
+    return x == top ? 1.0 : x > -INFINITY && top < INFINITY ? sm_exp(((double)x - (double)top) * inv) : 0.0;
+}
+__device__ __forceinline__ float sm_rough(float x, float top, double inv) {
+    return x == top ? 1.0f : x > -INFINITY && top < INFINITY ? exp2f((float)(((double)x - (double)top) * inv) * 1.44269504f) : 0.0f;
 }
 __device__ __forceinline__ uint64_t sm_units(double w, double up) { return w > 0.0 ? max((uint64_t)1, (uint64_t)rint(w * up)) : 0; }
 // Over the workgroup, with 64 bits a wave in tmp.
@@ -147,7 +162,7 @@ __device__ __forceinline__ uint32_t sm_load(const sgk_sample_args &a, const sm_p
 __device__ __forceinline__ sm_all sm_read(const sm_row &w, const sm_plan &p, const sm_set &s, uint64_t *tmp) {
     const uint32_t t = threadIdx.x, wv = t >> 6;
     uint32_t mine = 0, ok = 0, low = 0xFFFFFFFFu;
-    double sum = 0.0;
+    float sum = 0.0f;
     if (t < p.parts) {
 #pragma unroll
         for (uint32_t i = 0; i < SM_WAVES; i++) mine = max(mine, w.wave[t * SM_WAVES + i]);
@@ -164,11 +179,10 @@ __device__ __forceinline__ sm_all sm_read(const sm_row &w, const sm_plan &p, con
 #pragma unroll
     for (int i = 0; i < SM_WAVES; i++) { r.best = max(r.best, red[i]); r.low = min(r.low, red[SM_WAVES + i]); r.ok += red[2 * SM_WAVES + i]; }
     r.top = sm_value(r.best);
-    if (mine && mine != r.best) sum *= sm_weight(sm_value(mine), r.top, s.inv);
-    r.sum = sm_sum(mine ? sum : 0.0, tmp + 2 * SM_WAVES);
+    r.sum = fmaxf(sm_sum(mine ? sum * sm_rough(sm_value(mine), r.top, s.inv) : 0.0f, tmp + 2 * SM_WAVES), 1.0f);
     return r;
 }
-__device__ __forceinline__ double sm_unit(double sum) { return ldexp(1.0, 61 - ilogb(sum)); }
+__device__ __forceinline__ double sm_unit(float sum) { return ldexp(1.0, 60 - ilogbf(sum)); }
 
 // ---- 1: the parts' maxima and sums
 __global__ void __launch_bounds__(SM_THREADS) k_sample_parts(sgk_sample_args a, sm_plan p, int al) {
@@ -199,12 +213,12 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_parts(sgk_sample_args a, 
     for (int i = 0; i < SM_WAVES; i++) { best = max(best, red[i]); low = min(low, red[SM_WAVES + i]); }
     if (t == 0) { w.ok[part] = ok; w.low[part] = ok ? low + 1 : 0xFFFFFFFFu; }
     if (s.few) return;
-    double sum = 0.0;
+    float sum = 0.0f;
     const float top = sm_value(best);
     for (uint32_t m = 0; m < p.rounds && best; m++) {
         if (p.rounds > 1) sm_load(a, p, r, part, m, al, x);
 #pragma unroll
-        for (int e = 0; e < 4; e++) sum += sm_weight(x[e], top, s.inv);
+        for (int e = 0; e < 4; e++) sum += sm_rough(x[e], top, s.inv);
     }
     sum = sm_sum(sum, tmp);
     if (t == 0) w.sum[part] = sum;
@@ -284,7 +298,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
                 if (k >= s.top_k) bound |= 1u << b;
             }
         }
-        if (part == 0 && t == 0) *w.all = (sm_all){best, 0, best != 0, sm_value(best), 0.0};
+        if (part == 0 && t == 0) *w.all = (sm_all){best, 0, best != 0, sm_value(best), 1.0f};
         bound = max(bound, 1u);
         for (uint32_t m = 0; m < p.rounds; m++) {
             if (m) i = sm_load(a, p, r, part, m, al, x);
