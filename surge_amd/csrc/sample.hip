@@ -391,25 +391,32 @@ struct sm_over {
         at ^= 1;
         return r;
     }
+    // From here on only the entries of which in(key, ~id, bin) is true: the others are no key's equal and weigh nothing.
+    template <typename In>
+    __device__ __forceinline__ void keep(In in) {
+#pragma unroll
+        for (int i = 0; i < U; i++)
+            if (bin[i] == 0xFFFFFFFFu || !in(key[i], low[i], bin[i])) { key[i] = low[i] = 0; bin[i] = 0xFFFFFFFFu; unit[i] = 0; }
+    }
     template <typename In>
     __device__ __forceinline__ uint32_t count(In in) {
         uint32_t m = 0;
-        all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t) { m += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(b != 0xFFFFFFFFu && in(k, d, b))); });
+        all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t) { m += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(in(k, d, b))); });
         return (uint32_t)add(m);
     }
     template <typename In>
     __device__ __forceinline__ uint64_t units(In in) {
         uint64_t m = 0;
-        all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t u) { if (b != 0xFFFFFFFFu && in(k, d, b)) m += u; });
+        all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t u) { if (in(k, d, b)) m += u; });
         return add(wave_sum(m));
     }
-    // The lowest and the highest key, or ~id, of the entries that in() takes.
-    template <bool LOW, typename In>
-    __device__ __forceinline__ void ends(In in, uint32_t &lo, uint32_t &hi) {
+    // The lowest and the highest key, or ~id.
+    template <bool LOW>
+    __device__ __forceinline__ void ends(uint32_t &lo, uint32_t &hi) {
         lo = 0xFFFFFFFFu;
         hi = 0;
         all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t) {
-            if (b != 0xFFFFFFFFu && in(k, d, b)) { lo = min(lo, LOW ? d : k); hi = max(hi, LOW ? d : k); }
+            if (b != 0xFFFFFFFFu) { lo = min(lo, LOW ? d : k); hi = max(hi, LOW ? d : k); }
         });
         lo = ~wave_umax(~lo);
         hi = wave_umax(hi);
@@ -422,45 +429,44 @@ struct sm_over {
         at ^= 1;
         lo = ~a;
     }
-    // The largest key (or ~id) from which on the units of the entries that in() takes, and `before`, add up to `want`; the
-    // lowest entry's if none does, but never above the highest's.
-    template <bool LOW, typename In>
-    __device__ __forceinline__ uint32_t top(uint64_t before, uint64_t want, In in) {
+    // The largest key (or ~id) from which on the entries' units, and `before`, add up to `want`; the lowest entry's if none
+    // does, but never above the highest's.
+    template <bool LOW>
+    __device__ __forceinline__ uint32_t top(uint64_t before, uint64_t want) {
         uint32_t lo, hi;
-        ends<LOW>(in, lo, hi);
+        ends<LOW>(lo, hi);
         if (lo >= hi) return hi;
         uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi), from = lo & ~(2 * bit - 1);
         for (; bit; bit >>= 1) {
-            const uint64_t sum = units([&](uint32_t k, uint32_t d, uint32_t b) { return in(k, d, b) && (LOW ? d : k) >= (from | bit); });
+            const uint64_t sum = units([&](uint32_t k, uint32_t d, uint32_t) { return (LOW ? d : k) >= (from | bit); });
             if (sum && before + sum >= want) from |= bit;
         }
         return max(from, lo);
     }
-    // The room-th key (or ~id) of those that in() takes, and how many are above it (room: all its own stay).
-    template <bool LOW, typename In>
-    __device__ __forceinline__ uint32_t nth(uint32_t room, In in, uint32_t &above) {
+    // The room-th key (or ~id), and how many are above it (room: all its own stay).
+    template <bool LOW>
+    __device__ __forceinline__ uint32_t nth(uint32_t room, uint32_t &above) {
         uint32_t lo, hi, have = UINT32_MAX;
-        ends<LOW>(in, lo, hi);
+        ends<LOW>(lo, hi);
         uint32_t from = lo;
         if (lo < hi) {
             uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi);
             from &= ~(2 * bit - 1);
             for (; bit && have != room; bit >>= 1) {
-                const uint32_t m = count([&](uint32_t k, uint32_t d, uint32_t b) { return in(k, d, b) && (LOW ? d : k) >= (from | bit); });
+                const uint32_t m = count([&](uint32_t k, uint32_t d, uint32_t) { return (LOW ? d : k) >= (from | bit); });
                 if (m >= room) { from |= bit; have = m; }
             }
         }
-        above = have == room ? room : count([&](uint32_t k, uint32_t d, uint32_t b) { return in(k, d, b) && (LOW ? d : k) > from; });
+        above = have == room ? room : count([&](uint32_t k, uint32_t d, uint32_t) { return (LOW ? d : k) > from; });
         return from;
     }
-    // The order from which on `room` entries stay.
-    template <typename In>
-    __device__ __forceinline__ uint64_t first(uint32_t room, In in) {
+    // The order from which on `room` entries stay; of the entries it leaves that key's own, if it had to choose among them.
+    __device__ __forceinline__ uint64_t first(uint32_t room) {
         uint32_t above, unused;
-        const uint32_t key0 = nth<false>(room, in, above);
+        const uint32_t key0 = nth<false>(room, above);
         if (above >= room) return (uint64_t)key0 << 32;
-        auto same = [&](uint32_t k, uint32_t d, uint32_t b) { return k == key0 && in(k, d, b); };
-        return (uint64_t)key0 << 32 | nth<true>(room - above, same, unused);
+        keep([&](uint32_t k, uint32_t, uint32_t) { return k == key0; });
+        return (uint64_t)key0 << 32 | nth<true>(room - above, unused);
     }
 };
 typedef sm_over<64, SM_ALONE / 64> sm_alone;
@@ -468,29 +474,33 @@ typedef sm_over<SM_THREADS, SM_LIST / SM_THREADS> sm_together;
 // The lowest order that stays under top_k and top_p.
 template <typename Over>
 __device__ __forceinline__ uint64_t sm_end(sm_list &list, const sm_set &set, const sm_all &all, const sm_border &b, double up) {
-    Over v(list);
     uint64_t border = 0, whole = b.whole;
     if (b.kbin < SM_BINS) {
         auto in = [&](uint32_t, uint32_t, uint32_t bin) { return (bin & ~SM_LOW) == b.kbin; };
-        if (v.count(in) > set.top_k - b.kabove) border = v.first(set.top_k - b.kabove, in);
-        if (b.plo < SM_BINS)
-            whole = b.ksum + v.units([&](uint32_t k, uint32_t d, uint32_t bin) { return in(k, d, bin) && ((uint64_t)k << 32 | d) >= border; });
+        Over v(list);
+        v.keep(in);
+        if (v.count([](uint32_t, uint32_t, uint32_t bin) { return bin != 0xFFFFFFFFu; }) > set.top_k - b.kabove) border = v.first(set.top_k - b.kabove);
     }
     if (b.plo < SM_BINS) {
+        Over v(list);
+        if (b.kbin < SM_BINS)
+            whole = b.ksum + v.units([&](uint32_t k, uint32_t d, uint32_t bin) { return (bin & ~SM_LOW) == b.kbin && ((uint64_t)k << 32 | d) >= border; });
         const double want = (double)set.top_p * (double)whole;
         const uint64_t units = want > 0.0 ? (uint64_t)ceil(want) : 0;
-        auto in = [&](uint32_t k, uint32_t d, uint32_t bin) { const uint32_t x = bin & ~SM_LOW; return x >= b.plo && x <= b.phi && ((uint64_t)k << 32 | d) >= border; };
-        const uint32_t key = v.template top<false>(b.psum, units, in);
+        v.keep([&](uint32_t k, uint32_t d, uint32_t bin) { const uint32_t x = bin & ~SM_LOW; return x >= b.plo && x <= b.phi && ((uint64_t)k << 32 | d) >= border; });
+        const uint32_t key = v.template top<false>(b.psum, units);
         // of that key's ids, as many as it takes
-        auto same = [&](uint32_t k, uint32_t d, uint32_t bin) { return k == key && in(k, d, bin); };
-        const uint32_t ties = v.count(same);
+        const uint32_t ties = v.count([&](uint32_t k, uint32_t, uint32_t) { return k == key; });
         uint64_t low = 0;
         if (ties > 1) {
-            const uint64_t ahead = b.psum + v.units([&](uint32_t k, uint32_t d, uint32_t bin) { return k > key && in(k, d, bin); });
+            const uint64_t ahead = b.psum + v.units([&](uint32_t k, uint32_t, uint32_t) { return k > key; });
             const uint64_t unit = sm_units(sm_weight(sm_value(key), all.top, set.inv), up);
             const uint64_t room = units > ahead ? unit ? (units - ahead + unit - 1) / unit : ties : 1;
-            uint32_t unused;
-            if (room < ties) low = v.template nth<true>((uint32_t)room, same, unused);
+            if (room < ties) {
+                uint32_t unused;
+                v.keep([&](uint32_t k, uint32_t, uint32_t) { return k == key; });
+                low = v.template nth<true>((uint32_t)room, unused);
+            }
         }
         border = max(border, (uint64_t)key << 32 | low);
     }
@@ -527,9 +537,9 @@ template <typename Over>
 __device__ __forceinline__ uint32_t sm_choose(sm_list &list, float u, uint64_t &whole) {
     Over v(list);
     const uint64_t border = list.border;
-    auto stays = [&](uint32_t k, uint32_t d, uint32_t bin) { return ((uint64_t)k << 32 | d) >= border && !(bin & SM_LOW); };
-    whole = v.units(stays);
-    return ~v.template top<true>(0, (uint64_t)((double)u * (double)whole) + 1, stays);
+    v.keep([&](uint32_t k, uint32_t d, uint32_t bin) { return ((uint64_t)k << 32 | d) >= border && !(bin & SM_LOW); });
+    whole = v.units([](uint32_t, uint32_t, uint32_t) { return true; });
+    return ~v.template top<true>(0, (uint64_t)((double)u * (double)whole) + 1);
 }
 
 // The token of a row's part in which the units pass `want` (counted from the part's start), and the part's probabilities.
