@@ -1214,6 +1214,7 @@ sg_err sg_gpu_run_attn_paged(sg_gpu *g, void *q, void *kp, void *vp, void *table
         return errf("gpu: attn_paged: n_heads must be a multiple of n_kv_heads, at most %u times it", SGK_PAGES_MAX_GROUP);
     if (p[6] < hd) return (sg_err){"gpu: attn_paged: q_stride < head_dim"};
     const uint64_t rows = (uint64_t)n * nh;
+    if (rows > (1ull << 60) / p[6]) return (sg_err){"gpu: attn_paged: q_stride is too large"};      /* the sizes below stay in 64 bits */
     if (sg_failed(e = need(q, ((rows - 1) * p[6] + hd) * 4, "q")) || sg_failed(e = need(out, rows * hd * 4, "out")) ||
         sg_failed(e = need(lens, (uint64_t)n * 4, "lens"))) return e;
     if (!aligned(q, 4) || !aligned(out, 4) || !aligned(lens, 4)) return (sg_err){"gpu: attn_paged: q, lens and out must be 4-byte aligned"};

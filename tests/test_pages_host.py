@@ -107,6 +107,12 @@ def test_overlapping_buffers_are_refused():
     both(SAMPLE, 0, 4, 16)
 
 
+def test_sizes_past_64_bits_are_refused():
+    """32768 sequences of 65535 x 16 heads at the largest stride: 2^67 bytes, which would wrap to a size that fits."""
+    h = [far(1 << 39), far(1 << 28), far(1 << 28), far(1 << 18), far(1 << 18), None, None, far(1 << 39)]
+    refused(ATTN, h, [65535 * 16, 65535, 64, 16, 32768, 1, 0xFFFFFFFF, F(0.125)], "too large")
+
+
 def test_plain_sampling_follows_its_rules():
     """A worked example: weights 4, 2, 2, 1, 1 of ten."""
     x = np.log(np.array([2.0, 1.0, 4.0, 2.0, 1.0]))
