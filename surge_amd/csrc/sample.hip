@@ -47,7 +47,7 @@ struct sm_row {
     uint32_t *wave, *low, *ok;          // [parts][SM_WAVES] largest keys, [parts] lowest, [parts] ids that may be chosen
     float *sum;                         // [parts] of weights relative to the part's largest, roughly: for the units' size
     uint64_t *kept, *list, *binsum;     // [parts] units that stay, [SM_LIST] key and ~id, [SM_BINS]
-    uint32_t *bincnt, *listed, *out;    // [SM_BINS], [1], [1 + 2 SM_FEW] few: number, ids, probabilities
+    uint32_t *bincnt, *listed, *arrived, *out;      // [SM_BINS], [1], [1], [1 + 2 SM_FEW] few: number, ids, probabilities
     struct sm_all *all;                 // what 1 found, by 2
     struct sm_border *border;           // what 3 found
 };
@@ -65,7 +65,8 @@ __device__ __forceinline__ sm_row sm_at(const sm_plan &p, uint32_t r) {
     w.wave = (uint32_t *)take(4 * p.parts * SM_WAVES);
     w.low = (uint32_t *)take(4 * p.parts);
     w.ok = (uint32_t *)take(4 * p.parts);
-    w.listed = (uint32_t *)take(4);
+    w.listed = (uint32_t *)take(8);
+    w.arrived = w.listed + 1;
     w.out = (uint32_t *)take(4 * (1 + 2 * SM_FEW));
     w.all = (sm_all *)take(sizeof(sm_all));
     w.border = (sm_border *)take(sizeof(sm_border));
@@ -75,7 +76,7 @@ static uint64_t sm_row_bytes(uint64_t parts) {
     uint64_t n = 0;
     auto take = [&](uint64_t bytes) { n += (bytes + 15) / 16 * 16; };
     take(4 * parts); take(8 * parts); take(8 * SM_LIST); take(8 * SM_BINS); take(4 * SM_BINS);
-    take(4 * parts * SM_WAVES); take(4 * parts); take(4 * parts); take(4); take(4 * (1 + 2 * SM_FEW)); take(sizeof(sm_all)); take(sizeof(sm_border));
+    take(4 * parts * SM_WAVES); take(4 * parts); take(4 * parts); take(8); take(4 * (1 + 2 * SM_FEW)); take(sizeof(sm_all)); take(sizeof(sm_border));
     return n;
 }
 
@@ -204,7 +205,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_parts(sgk_sample_args a, 
         }
     }
     for (uint32_t i = part * SM_THREADS + t; i < SM_BINS && !s.few; i += p.parts * SM_THREADS) { w.bincnt[i] = 0; w.binsum[i] = 0; }
-    if (part == 0 && t == 0) { *w.listed = 0; w.out[0] = 0; }
+    if (part == 0 && t == 0) { *w.listed = *w.arrived = 0; w.out[0] = 0; }
     best = wave_umax(best);
     low = ~wave_umax(~low);
     if ((t & 63) == 0) { w.wave[part * SM_WAVES + (t >> 6)] = best; red[t >> 6] = best; red[SM_WAVES + (t >> 6)] = low; }
@@ -243,7 +244,7 @@ __device__ __forceinline__ void sm_append(const sm_row &w, const float (&x)[4], 
 #pragma unroll
     for (int e = 0; e < 4; e++)
         if (in >> e & 1) {
-            if (base < SM_LIST) w.list[base] = (uint64_t)sm_key(x[e]) << 32 | (uint32_t)~(i + e);
+            if (base < SM_LIST) __hip_atomic_store(w.list + base, (uint64_t)sm_key(x[e]) << 32 | (uint32_t)~(i + e), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             base++;
         }
 }
@@ -509,10 +510,10 @@ __device__ __forceinline__ uint64_t sm_end(sm_list &list, const sm_set &set, con
 // The list from memory, and its border; all threads. False: it does not fit.
 __device__ __forceinline__ bool sm_resolve(sm_list &s, const sm_row &w, const sm_set &set, const sm_all &all, const sm_border &b, double up, float scale) {
     const uint32_t t = threadIdx.x;
-    const uint32_t n = *w.listed;
+    const uint32_t n = __hip_atomic_load(w.listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (n > SM_LIST) return false;
     for (uint32_t j = t; j < n; j += SM_THREADS) {
-        const uint64_t o = w.list[j];
+        const uint64_t o = __hip_atomic_load(w.list + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const float x = sm_value((uint32_t)(o >> 32));
         const double y = sm_weight(x, all.top, set.inv);
         s.order[j] = o;
@@ -580,203 +581,6 @@ __device__ __forceinline__ void sm_pick(const sgk_sample_args &a, const sm_plan 
     if (!here) return;
     __syncthreads();
     if (threadIdx.x == 0) a.token[r] = *least;
-}
-
-// ---- 3
-__global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a, sm_plan p, int al) {
-    __shared__ uint64_t tmp[SM_WAVES];
-    __shared__ uint32_t least, tmp32[SM_WAVES];
-    __shared__ sm_border found;
-    __shared__ sm_list list;
-    __shared__ uint32_t ranks[4][SM_RANKED];
-    __shared__ uint64_t aheads[4][SM_RANKED];
-    const uint32_t t = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
-    const sm_row w = sm_at(p, r);
-    const sm_set s = sm_settings(a, p, r);
-    if (s.few && part) return;
-    const sm_all all = *w.all;
-    if (!all.ok) return;
-    if (s.few) {
-        const double up = 0x1p54;           // 2^7 ids at most
-        const uint32_t listed = *w.listed;
-        if (listed <= SM_RANKED) {
-            // each entry against all: four groups of waves take a quarter of the others each, for 64 or 128 entries
-            const uint32_t l = t & 63, half = t >> 6 & 1, j = 64 * half + l, from = (t >> 7) * (SM_RANKED / 4);
-            if (t < SM_RANKED) {
-                const uint64_t o = t < listed ? w.list[t] : 0;
-                const double y = t < listed ? sm_weight(sm_value((uint32_t)(o >> 32)), all.top, s.inv) : 0.0;
-                list.order[t] = o;
-                list.unit[t] = sm_units(y, up);
-                list.bin[t] = t < listed && (y >= (double)s.min_p || sm_value((uint32_t)(o >> 32)) == all.top) ? 0 : SM_LOW;
-            }
-            __syncthreads();
-            uint32_t rank = 0;
-            uint64_t ahead = 0;
-            if (64 * half < listed) {
-                const uint64_t o = list.order[j];
-                for (uint32_t i = from; i < min(from + SM_RANKED / 4, listed); i++)
-                    if (list.order[i] > o) { rank++; ahead += list.unit[i]; }
-            }
-            ranks[t >> 7][j] = rank;
-            aheads[t >> 7][j] = ahead;
-            __syncthreads();
-            if (t >= 64) return;
-            // lane l has entries l and 64 + l
-            uint64_t unit[2], before[2], kept = 0;
-            uint32_t id[2];
-            bool stays[2];
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const uint32_t x = 64 * i + l, k = ranks[0][x] + ranks[1][x] + ranks[2][x] + ranks[3][x];
-                before[i] = aheads[0][x] + aheads[1][x] + aheads[2][x] + aheads[3][x];
-                unit[i] = list.unit[x];
-                id[i] = ~(uint32_t)list.order[x];
-                stays[i] = x < listed && k < s.top_k;
-                kept += stays[i] ? unit[i] : 0;
-            }
-            if (s.top_p < 1.0f) {
-                const double want = ceil((double)s.top_p * (double)wave_sum(kept));
-                const uint64_t units = want > 1.0 ? (uint64_t)want : 1;
-                stays[0] = stays[0] && before[0] < units;
-                stays[1] = stays[1] && before[1] < units;
-            }
-            kept = 0;
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                stays[i] = stays[i] && !(list.bin[64 * i + l] & SM_LOW);
-                kept += stays[i] ? unit[i] : 0;
-            }
-            const uint64_t whole = wave_sum(kept), want = (uint64_t)((double)s.u * (double)whole);
-            // the units of the ids up to an entry's own, over those that stay
-            uint64_t upto[2] = {0, 0};
-            uint32_t m = 0;
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                uint64_t left = __builtin_amdgcn_ballot_w64(stays[i]);
-                if (a.probs && stays[i]) {
-                    const uint32_t at = m + lanes_below(left);
-                    w.out[1 + 2 * at] = id[i];
-                    w.out[2 + 2 * at] = __float_as_uint((float)(sm_weight(sm_value((uint32_t)(list.order[64 * i + l] >> 32)), all.top, s.inv) * up / (double)whole));
-                }
-                m += (uint32_t)__popcll(left);
-                for (; left; left &= left - 1) {
-                    const int x = __builtin_ctzll(left);
-                    const uint32_t d = (uint32_t)__builtin_amdgcn_readlane((int)id[i], x);
-                    const uint64_t y = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(unit[i] >> 32), x) << 32 |
-                                       (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)unit[i], x);
-                    if (d <= id[0]) upto[0] += y;
-                    if (d <= id[1]) upto[1] += y;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-                if (stays[i] && unit[i] && upto[i] > want && upto[i] - unit[i] <= want) a.token[r] = id[i];
-            if (t == 0) w.out[0] = m;
-            return;
-        }
-        const sm_border b = {0, 0, s.top_p < 1.0f ? 0 : SM_BINS, 0, 0, 0, 0, 0};
-        if (!sm_resolve(list, w, s, all, b, up, 0.0f)) return;
-        const uint64_t border = list.border;
-        uint64_t whole;
-        uint32_t id;
-        if (list.n > SM_ALONE) id = sm_choose<sm_together>(list, s.u, whole);
-        else if (t < 64) id = sm_choose<sm_alone>(list, s.u, whole);
-        if (t == 0) a.token[r] = id;
-        if (!a.probs || t >= 64) return;
-        auto in = [&](uint32_t j) { return list.order[j] >= border && !(list.bin[j] & SM_LOW); };
-        uint32_t n = 0;
-        for (uint32_t j0 = 0; j0 < list.n; j0 += 64) {
-            const uint32_t j = j0 + t;
-            const bool k = j < list.n && in(j);
-            const uint64_t m = __builtin_amdgcn_ballot_w64(k);
-            const uint32_t at = n + lanes_below(m);
-            if (k && at < SM_FEW) {
-                w.out[1 + 2 * at] = ~(uint32_t)list.order[j];
-                w.out[2 + 2 * at] = __float_as_uint((float)(sm_weight(sm_value((uint32_t)(list.order[j] >> 32)), all.top, s.inv) * up / (double)whole));
-            }
-            n += (uint32_t)__popcll(m);
-        }
-        if (t == 0) w.out[0] = min(n, SM_FEW);
-        return;
-    }
-    const double up = sm_unit(all.sum);
-    const bool k_on = s.top_k && s.top_k < all.ok, p_on = s.top_p < 1.0f;
-    if (!k_on && !p_on) {
-        uint64_t whole;
-        const uint64_t mine = t < p.parts ? w.kept[t] : 0, before = sm_scan(mine, &whole, tmp), want = (uint64_t)((double)s.u * (double)whole);
-        if (t == part) { found.ksum = before; found.psum = mine; }
-        __syncthreads();
-        const bool here = want >= found.ksum && want < found.ksum + found.psum;
-        sm_pick(a, p, r, part, al, s, all.top, up, (double)whole, here, want - found.ksum, tmp, &least, [](float, uint32_t) { return true; });
-        return;
-    }
-    // the bins in which top_k and top_p end
-    constexpr uint32_t PER = SM_BINS / SM_THREADS;
-    const float scale = sm_bin_scale(s, all);
-    uint32_t cnt[PER], c = 0, nall;
-    uint64_t sum[PER], u = 0, whole;
-#pragma unroll
-    for (uint32_t i = 0; i < PER; i++) {
-        cnt[i] = w.bincnt[t * PER + i];
-        sum[i] = w.binsum[t * PER + i];
-        c += cnt[i];
-        u += sum[i];
-    }
-    c = sm_scan(c, &nall, tmp32);
-    u = sm_scan(u, &whole, tmp);
-    if (t == 0) found = (sm_border){SM_BINS, 0, SM_BINS, SM_BINS, 0, 0, 0, whole};
-    __syncthreads();
-    uint64_t klo = whole, khi = whole;
-    if (k_on) {
-        uint32_t cc = c;
-        uint64_t uu = u;
-#pragma unroll
-        for (uint32_t i = 0; i < PER; i++) {
-            if (cc < s.top_k && cc + cnt[i] >= s.top_k) { found.kbin = t * PER + i; found.kabove = cc; found.ksum = uu; found.psum = uu + sum[i]; }
-            cc += cnt[i];
-            uu += sum[i];
-        }
-        __syncthreads();
-        klo = found.ksum;
-        khi = found.psum;
-        __syncthreads();
-    }
-    if (p_on) {
-        const double dlo = ceil((double)s.top_p * (double)klo), dhi = ceil((double)s.top_p * (double)khi);
-        const uint64_t wlo = dlo > 1.0 ? (uint64_t)dlo : 1, whi = dhi > 1.0 ? (uint64_t)dhi : 1;
-        uint64_t uu = u;
-#pragma unroll
-        for (uint32_t i = 0; i < PER; i++) {
-            if (uu < wlo && uu + sum[i] >= wlo) { found.plo = t * PER + i; found.psum = uu; }
-            if (uu < whi && uu + sum[i] >= whi) found.phi = t * PER + i;
-            uu += sum[i];
-        }
-        __syncthreads();
-    }
-    sm_border b = found;
-    if (p_on && b.kbin < SM_BINS) b.phi = min(b.phi, b.kbin);
-    b.first = p_on ? b.plo : b.kbin;
-    if (part == 0 && t == 0) *w.border = b;
-    uint64_t q = 0;
-    for (uint32_t m = 0; m < p.rounds; m++) {
-        float x[4];
-        const uint32_t i = sm_load(a, p, r, part, m, al, x);
-        uint32_t in = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (!(x[e] > -INFINITY)) continue;
-            const uint32_t y = sm_bin(x[e], all.top, scale);
-            if (y < b.first) {
-                const double z = sm_weight(x[e], all.top, s.inv);
-                if (z >= (double)s.min_p || x[e] == all.top) q += sm_units(z, up);
-            } else if (y == b.kbin || (p_on && y <= b.phi)) {
-                in |= 1u << e;
-            }
-        }
-        sm_append(w, x, i, in);
-    }
-    q = sm_sum(q, tmp);
-    if (t == 0) w.kept[part] = q;
 }
 
 // A row whose list does not fit: one workgroup, the borders of top_k and top_p by the digits of the keys, 8 bits a pass over the row.
@@ -906,6 +710,241 @@ __device__ __forceinline__ void sm_slow(const sgk_sample_args &a, uint32_t r, co
     __syncthreads();
     if (t == 0) a.token[r] = token;
 }
+// ---- 3. LAST: the row's last workgroup goes on to the token, and no fourth launch follows; what it takes from the others
+// has been written through to memory.
+template <bool LAST>
+__global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a, sm_plan p, int al) {
+    __shared__ uint64_t tmp[SM_WAVES];
+    __shared__ uint32_t least, tmp32[SM_WAVES];
+    __shared__ sm_border found;
+    __shared__ sm_list list;
+    __shared__ struct { uint32_t rank[4][SM_RANKED]; uint64_t ahead[4][SM_RANKED]; } ranked;
+    auto &ranks = ranked.rank;
+    auto &aheads = ranked.ahead;
+    const uint32_t t = threadIdx.x, part = blockIdx.x, r = blockIdx.y;
+    const sm_row w = sm_at(p, r);
+    const sm_set s = sm_settings(a, p, r);
+    if (s.few && part) return;
+    const sm_all all = *w.all;
+    if (!all.ok) {
+        if (LAST && part == 0 && t == 0) a.token[r] = SM_NONE;
+        return;
+    }
+    if (s.few) {
+        const double up = 0x1p54;           // 2^7 ids at most
+        const uint32_t listed = *w.listed;
+        if (listed <= SM_RANKED) {
+            // each entry against all: four groups of waves take a quarter of the others each, for 64 or 128 entries
+            const uint32_t l = t & 63, half = t >> 6 & 1, j = 64 * half + l, from = (t >> 7) * (SM_RANKED / 4);
+            if (t < SM_RANKED) {
+                const uint64_t o = t < listed ? w.list[t] : 0;
+                const double y = t < listed ? sm_weight(sm_value((uint32_t)(o >> 32)), all.top, s.inv) : 0.0;
+                list.order[t] = o;
+                list.unit[t] = sm_units(y, up);
+                list.bin[t] = t < listed && (y >= (double)s.min_p || sm_value((uint32_t)(o >> 32)) == all.top) ? 0 : SM_LOW;
+            }
+            __syncthreads();
+            uint32_t rank = 0;
+            uint64_t ahead = 0;
+            if (64 * half < listed) {
+                const uint64_t o = list.order[j];
+                for (uint32_t i = from; i < min(from + SM_RANKED / 4, listed); i++)
+                    if (list.order[i] > o) { rank++; ahead += list.unit[i]; }
+            }
+            ranks[t >> 7][j] = rank;
+            aheads[t >> 7][j] = ahead;
+            __syncthreads();
+            if (t >= 64) return;
+            // lane l has entries l and 64 + l
+            uint64_t unit[2], before[2], kept = 0;
+            uint32_t id[2];
+            bool stays[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint32_t x = 64 * i + l, k = ranks[0][x] + ranks[1][x] + ranks[2][x] + ranks[3][x];
+                before[i] = aheads[0][x] + aheads[1][x] + aheads[2][x] + aheads[3][x];
+                unit[i] = list.unit[x];
+                id[i] = ~(uint32_t)list.order[x];
+                stays[i] = x < listed && k < s.top_k;
+                kept += stays[i] ? unit[i] : 0;
+            }
+            if (s.top_p < 1.0f) {
+                const double want = ceil((double)s.top_p * (double)wave_sum(kept));
+                const uint64_t units = want > 1.0 ? (uint64_t)want : 1;
+                stays[0] = stays[0] && before[0] < units;
+                stays[1] = stays[1] && before[1] < units;
+            }
+            kept = 0;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                stays[i] = stays[i] && !(list.bin[64 * i + l] & SM_LOW);
+                kept += stays[i] ? unit[i] : 0;
+            }
+            const uint64_t whole = wave_sum(kept), want = (uint64_t)((double)s.u * (double)whole);
+            // the units of the ids up to an entry's own, over those that stay
+            uint64_t upto[2] = {0, 0};
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                uint64_t left = __builtin_amdgcn_ballot_w64(stays[i]);
+                if (a.probs && stays[i]) {
+                    const uint32_t at = m + lanes_below(left);
+                    w.out[1 + 2 * at] = id[i];
+                    w.out[2 + 2 * at] = __float_as_uint((float)(sm_weight(sm_value((uint32_t)(list.order[64 * i + l] >> 32)), all.top, s.inv) * up / (double)whole));
+                }
+                m += (uint32_t)__popcll(left);
+                for (; left; left &= left - 1) {
+                    const int x = __builtin_ctzll(left);
+                    const uint32_t d = (uint32_t)__builtin_amdgcn_readlane((int)id[i], x);
+                    const uint64_t y = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(unit[i] >> 32), x) << 32 |
+                                       (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)unit[i], x);
+                    if (d <= id[0]) upto[0] += y;
+                    if (d <= id[1]) upto[1] += y;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if (stays[i] && unit[i] && upto[i] > want && upto[i] - unit[i] <= want) a.token[r] = id[i];
+            if (t == 0) w.out[0] = m;
+            return;
+        }
+        const sm_border b = {0, 0, s.top_p < 1.0f ? 0 : SM_BINS, 0, 0, 0, 0, 0};
+        if (!sm_resolve(list, w, s, all, b, up, 0.0f)) {
+            if (LAST) sm_slow(a, r, s, &list);
+            return;
+        }
+        const uint64_t border = list.border;
+        uint64_t whole;
+        uint32_t id;
+        if (list.n > SM_ALONE) id = sm_choose<sm_together>(list, s.u, whole);
+        else if (t < 64) id = sm_choose<sm_alone>(list, s.u, whole);
+        if (t == 0) a.token[r] = id;
+        if (!a.probs || t >= 64) return;
+        auto in = [&](uint32_t j) { return list.order[j] >= border && !(list.bin[j] & SM_LOW); };
+        uint32_t n = 0;
+        for (uint32_t j0 = 0; j0 < list.n; j0 += 64) {
+            const uint32_t j = j0 + t;
+            const bool k = j < list.n && in(j);
+            const uint64_t m = __builtin_amdgcn_ballot_w64(k);
+            const uint32_t at = n + lanes_below(m);
+            if (k && at < SM_FEW) {
+                w.out[1 + 2 * at] = ~(uint32_t)list.order[j];
+                w.out[2 + 2 * at] = __float_as_uint((float)(sm_weight(sm_value((uint32_t)(list.order[j] >> 32)), all.top, s.inv) * up / (double)whole));
+            }
+            n += (uint32_t)__popcll(m);
+        }
+        if (t == 0) w.out[0] = min(n, SM_FEW);
+        return;
+    }
+    const double up = sm_unit(all.sum);
+    const bool k_on = s.top_k && s.top_k < all.ok, p_on = s.top_p < 1.0f;
+    if (!k_on && !p_on) {
+        uint64_t whole;
+        const uint64_t mine = t < p.parts ? w.kept[t] : 0, before = sm_scan(mine, &whole, tmp), want = (uint64_t)((double)s.u * (double)whole);
+        if (t == part) { found.ksum = before; found.psum = mine; }
+        __syncthreads();
+        const bool here = want >= found.ksum && want < found.ksum + found.psum;
+        sm_pick(a, p, r, part, al, s, all.top, up, (double)whole, here, want - found.ksum, tmp, &least, [](float, uint32_t) { return true; });
+        return;
+    }
+    // the bins in which top_k and top_p end
+    constexpr uint32_t PER = SM_BINS / SM_THREADS;
+    const float scale = sm_bin_scale(s, all);
+    uint32_t cnt[PER], c = 0, nall;
+    uint64_t sum[PER], u = 0, whole;
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) {
+        cnt[i] = w.bincnt[t * PER + i];
+        sum[i] = w.binsum[t * PER + i];
+        c += cnt[i];
+        u += sum[i];
+    }
+    c = sm_scan(c, &nall, tmp32);
+    u = sm_scan(u, &whole, tmp);
+    if (t == 0) found = (sm_border){SM_BINS, 0, SM_BINS, SM_BINS, 0, 0, 0, whole};
+    __syncthreads();
+    uint64_t klo = whole, khi = whole;
+    if (k_on) {
+        uint32_t cc = c;
+        uint64_t uu = u;
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            if (cc < s.top_k && cc + cnt[i] >= s.top_k) { found.kbin = t * PER + i; found.kabove = cc; found.ksum = uu; found.psum = uu + sum[i]; }
+            cc += cnt[i];
+            uu += sum[i];
+        }
+        __syncthreads();
+        klo = found.ksum;
+        khi = found.psum;
+        __syncthreads();
+    }
+    if (p_on) {
+        const double dlo = ceil((double)s.top_p * (double)klo), dhi = ceil((double)s.top_p * (double)khi);
+        const uint64_t wlo = dlo > 1.0 ? (uint64_t)dlo : 1, whi = dhi > 1.0 ? (uint64_t)dhi : 1;
+        uint64_t uu = u;
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            if (uu < wlo && uu + sum[i] >= wlo) { found.plo = t * PER + i; found.psum = uu; }
+            if (uu < whi && uu + sum[i] >= whi) found.phi = t * PER + i;
+            uu += sum[i];
+        }
+        __syncthreads();
+    }
+    sm_border b = found;
+    if (p_on && b.kbin < SM_BINS) b.phi = min(b.phi, b.kbin);
+    b.first = p_on ? b.plo : b.kbin;
+    if (part == 0 && t == 0) *w.border = b;
+    uint64_t q = 0;
+    for (uint32_t m = 0; m < p.rounds; m++) {
+        float x[4];
+        const uint32_t i = sm_load(a, p, r, part, m, al, x);
+        uint32_t in = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (!(x[e] > -INFINITY)) continue;
+            const uint32_t y = sm_bin(x[e], all.top, scale);
+            if (y < b.first) {
+                const double z = sm_weight(x[e], all.top, s.inv);
+                if (z >= (double)s.min_p || x[e] == all.top) q += sm_units(z, up);
+            } else if (y == b.kbin || (p_on && y <= b.phi)) {
+                in |= 1u << e;
+            }
+        }
+        sm_append(w, x, i, in);
+    }
+    q = sm_sum(q, tmp);
+    if (t == 0) __hip_atomic_store(w.kept + part, q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (!LAST) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // what this wave wrote has arrived
+    __syncthreads();
+    if (t == 0) least = __hip_atomic_fetch_add(w.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (least != p.parts - 1) return;
+    __syncthreads();
+    if (!sm_resolve(list, w, s, all, b, up, scale)) {
+        sm_slow(a, r, s, &list);
+        return;
+    }
+    // the parts' units that stay: above the listed bins, and the list's
+    uint64_t *const units = &aheads[0][0];
+    static_assert(4 * SM_RANKED >= SM_PARTS, "room for the parts");
+    if (t < p.parts) units[t] = __hip_atomic_load(w.kept + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    for (uint32_t j = t; j < list.n; j += SM_THREADS)
+        if (list.order[j] >= list.border && !(list.bin[j] & SM_LOW))
+            atomicAdd((unsigned long long *)units + ~(uint32_t)list.order[j] / (SM_IDS * p.rounds), (unsigned long long)list.unit[j]);
+    __syncthreads();
+    uint64_t total;
+    const uint64_t mine = t < p.parts ? units[t] : 0, before = sm_scan(mine, &total, tmp), want = (uint64_t)((double)s.u * (double)total);
+    if (want >= before && want < before + mine) { found.kabove = t; found.ksum = before; }
+    __syncthreads();
+    const uint64_t border = list.border;
+    sm_pick(a, p, r, found.kabove, al, s, all.top, up, (double)total, true, want - found.ksum, tmp, &least, [&](float x, uint32_t i) {
+        const uint32_t y = sm_bin(x, all.top, scale);
+        return y < b.first || ((y == b.kbin || (p_on && y <= b.phi)) && ((uint64_t)sm_key(x) << 32 | (uint32_t)~i) >= border);
+    });
+}
+
 // ---- 4
 __global__ void __launch_bounds__(SM_THREADS) k_sample_last(sgk_sample_args a, sm_plan p, int al) {
     __shared__ uint64_t tmp[SM_WAVES], sums[3][SM_WAVES];
@@ -999,8 +1038,13 @@ extern "C" hipError_t sgk_sample(const sgk_sample_args *a, void *scratch, hipStr
         const dim3 grid(p.parts, b.rows);
         launch(k_sample_parts, grid, SM_THREADS, s, (hipEvent_t)NULL, b, p, al);
         launch(k_sample_count, grid, SM_THREADS, s, (hipEvent_t)NULL, b, p, al);
-        launch(k_sample_border, grid, SM_THREADS, s, (hipEvent_t)NULL, b, p, al);
-        launch(k_sample_last, grid, SM_THREADS, s, r + SM_ROWS < a->rows ? (hipEvent_t)NULL : done, b, p, al);
+        const hipEvent_t ev = r + SM_ROWS < a->rows ? (hipEvent_t)NULL : done;
+        if (!b.probs) {
+            launch(k_sample_border<true>, grid, SM_THREADS, s, ev, b, p, al);
+            continue;
+        }
+        launch(k_sample_border<false>, grid, SM_THREADS, s, (hipEvent_t)NULL, b, p, al);
+        launch(k_sample_last, grid, SM_THREADS, s, ev, b, p, al);
     }
     return hipGetLastError();
 }
