@@ -351,159 +351,143 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
 
 // ---- a list of ids in LDS: order (key, then ~id: the larger comes first), units, bin with SM_LOW if the weight is below min_p
 #define SM_LOW 0x80000000u
-struct sm_list { uint64_t order[SM_LIST], unit[SM_LIST]; uint32_t bin[SM_LIST], n; uint64_t border, tmp[2][SM_WAVES]; };
+struct sm_list { uint64_t order[SM_LIST], unit[SM_LIST]; uint32_t bin[SM_LIST], n; uint64_t border, tmp[2][SM_WAVES], sums[6][64]; };
 
-// Who goes over the list: a wave alone while its entries fit into 8 registers a lane (SM_ALONE), past that the workgroup,
-// whose steps each take a barrier (300 entries: 6 us less alone). Entry i of a thread is place i THREADS + its own.
-#define SM_ALONE 512u
-template <int THREADS, int U>
+// The workgroup over the list: entry i of a thread is place i SM_THREADS + t. All threads get every result.
+struct sm_found { uint32_t value; uint64_t above, own; };       // units (or entries) above the value, and its own
 struct sm_over {
+    static constexpr int U = SM_LIST / SM_THREADS;
+    sm_list &s;
     const uint32_t t, each;
-    uint64_t (*const tmp)[SM_WAVES];        // a step's results go through half `at`, so that one barrier a step is enough
-    int at;
+    int at;                                 // a step's results go through half `at` of tmp, so that one barrier a step is enough
     uint32_t key[U], low[U], bin[U];        // bin: 0xFFFFFFFF behind the list
     uint64_t unit[U];
-    __device__ __forceinline__ sm_over(sm_list &s) : t(threadIdx.x), each((s.n + THREADS - 1) / THREADS), tmp(s.tmp), at(0) {
+    __device__ __forceinline__ sm_over(sm_list &list) : s(list), t(threadIdx.x), each((list.n + SM_THREADS - 1) / SM_THREADS), at(0) {
 #pragma unroll
         for (int i = 0; i < U; i++) {
-            const uint32_t j = i * THREADS + t;
+            const uint32_t j = i * SM_THREADS + t;
             const bool here = j < s.n;
             key[i] = here ? (uint32_t)(s.order[j] >> 32) : 0;
             low[i] = here ? (uint32_t)s.order[j] : 0;
             bin[i] = here ? s.bin[j] : 0xFFFFFFFFu;
             unit[i] = here ? s.unit[j] : 0;
         }
-        if (THREADS > 64) __syncthreads();
-    }
-    template <typename F>
-    __device__ __forceinline__ void all(F f) const {
-#pragma unroll
-        for (int i = 0; i < U; i++)
-            if ((uint32_t)i < each) f(key[i], low[i], bin[i], unit[i]);
-    }
-    // v of the waves, added
-    __device__ __forceinline__ uint64_t add(uint64_t v) {
-        if (THREADS == 64) return v;
-        if ((t & 63) == 0) tmp[at][t >> 6] = v;
         __syncthreads();
-        uint64_t r = 0;
-#pragma unroll
-        for (int i = 0; i < THREADS / 64; i++) r += tmp[at][i];
-        at ^= 1;
-        return r;
     }
-    // From here on only the entries of which in(key, ~id, bin) is true: the others are no key's equal and weigh nothing.
+    // From here on only the entries of which in(key, ~id, bin, units) is true.
     template <typename In>
     __device__ __forceinline__ void keep(In in) {
 #pragma unroll
         for (int i = 0; i < U; i++)
-            if (bin[i] == 0xFFFFFFFFu || !in(key[i], low[i], bin[i])) { key[i] = low[i] = 0; bin[i] = 0xFFFFFFFFu; unit[i] = 0; }
+            if (bin[i] == 0xFFFFFFFFu || !in(key[i], low[i], bin[i], unit[i])) { key[i] = low[i] = 0; bin[i] = 0xFFFFFFFFu; unit[i] = 0; }
     }
-    template <typename In>
-    __device__ __forceinline__ uint32_t count(In in) {
+    __device__ __forceinline__ uint64_t add(uint64_t v) {       // v: the wave's
+        if ((t & 63) == 0) s.tmp[at][t >> 6] = v;
+        __syncthreads();
+        uint64_t r = 0;
+#pragma unroll
+        for (int i = 0; i < SM_WAVES; i++) r += s.tmp[at][i];
+        at ^= 1;
+        return r;
+    }
+    __device__ __forceinline__ uint32_t count() {
         uint32_t m = 0;
-        all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t) { m += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(in(k, d, b))); });
+#pragma unroll
+        for (int i = 0; i < U; i++) m += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(bin[i] != 0xFFFFFFFFu));
         return (uint32_t)add(m);
     }
     template <typename In>
     __device__ __forceinline__ uint64_t units(In in) {
         uint64_t m = 0;
-        all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t u) { if (in(k, d, b)) m += u; });
+#pragma unroll
+        for (int i = 0; i < U; i++)
+            if (in(key[i], low[i], bin[i])) m += unit[i];
         return add(wave_sum(m));
     }
-    // The lowest and the highest key, or ~id.
-    template <bool LOW>
-    __device__ __forceinline__ void ends(uint32_t &lo, uint32_t &hi) {
-        lo = 0xFFFFFFFFu;
-        hi = 0;
-        all([&](uint32_t k, uint32_t d, uint32_t b, uint64_t) {
-            if (b != 0xFFFFFFFFu) { lo = min(lo, LOW ? d : k); hi = max(hi, LOW ? d : k); }
-        });
+    // The largest key (or ~id) from which on the entries' units (or the entries), and `before`, come to `want`; the lowest if
+    // none does. Six bits a step, from the highest in which they differ: the values' sums in LDS, which every wave adds up.
+    // want > before; entries of no units do not count where units do.
+    template <bool LOW, bool UNITS>
+    __device__ __forceinline__ sm_found reach(uint64_t before, uint64_t want) {
+        uint32_t lo = 0xFFFFFFFFu, hi = 0;
+#pragma unroll
+        for (int i = 0; i < U; i++)
+            if (bin[i] != 0xFFFFFFFFu) { lo = min(lo, LOW ? low[i] : key[i]); hi = max(hi, LOW ? low[i] : key[i]); }
         lo = ~wave_umax(~lo);
         hi = wave_umax(hi);
-        if (THREADS == 64) return;
-        if ((t & 63) == 0) tmp[at][t >> 6] = (uint64_t)~lo << 32 | hi;
+        if ((t & 63) == 0) s.tmp[at][t >> 6] = (uint64_t)~lo << 32 | hi;
+        if (t < 6 * 64) s.sums[t / 64][t % 64] = 0;
         __syncthreads();
-        uint32_t a = 0;
+        uint32_t low_ = 0;
 #pragma unroll
-        for (int i = 0; i < THREADS / 64; i++) { a = max(a, (uint32_t)(tmp[at][i] >> 32)); hi = max(hi, (uint32_t)tmp[at][i]); }
+        for (int i = 0; i < SM_WAVES; i++) { low_ = max(low_, (uint32_t)(s.tmp[at][i] >> 32)); hi = max(hi, (uint32_t)s.tmp[at][i]); }
         at ^= 1;
-        lo = ~a;
-    }
-    // The largest key (or ~id) from which on the entries' units, and `before`, add up to `want`; the lowest entry's if none
-    // does, but never above the highest's.
-    template <bool LOW>
-    __device__ __forceinline__ uint32_t top(uint64_t before, uint64_t want) {
-        uint32_t lo, hi;
-        ends<LOW>(lo, hi);
-        if (lo >= hi) return hi;
-        uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi), from = lo & ~(2 * bit - 1);
-        for (; bit; bit >>= 1) {
-            const uint64_t sum = units([&](uint32_t k, uint32_t d, uint32_t) { return (LOW ? d : k) >= (from | bit); });
-            if (sum && before + sum >= want) from |= bit;
-        }
-        return max(from, lo);
-    }
-    // The room-th key (or ~id), and how many are above it (room: all its own stay).
-    template <bool LOW>
-    __device__ __forceinline__ uint32_t nth(uint32_t room, uint32_t &above) {
-        uint32_t lo, hi, have = UINT32_MAX;
-        ends<LOW>(lo, hi);
-        uint32_t from = lo;
-        if (lo < hi) {
-            uint32_t bit = 0x80000000u >> __builtin_clz(lo ^ hi);
-            from &= ~(2 * bit - 1);
-            for (; bit && have != room; bit >>= 1) {
-                const uint32_t m = count([&](uint32_t k, uint32_t d, uint32_t) { return (LOW ? d : k) >= (from | bit); });
-                if (m >= room) { from |= bit; have = m; }
+        lo = ~low_;
+        int top = lo < hi ? 32 - __builtin_clz(lo ^ hi) : 0;       // bits that are not known yet
+        uint64_t above = 0, own = 0;
+        uint32_t value = top < 32 ? hi >> top << top : 0;
+        for (int level = 0;; level++) {
+            const int shift = max(top - 6, 0);
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                const uint32_t v = LOW ? low[i] : key[i];
+                if (bin[i] != 0xFFFFFFFFu && (top == 32 || (v ^ value) >> top == 0))
+                    atomicAdd((unsigned long long *)&s.sums[level][(v ^ value) >> shift], (unsigned long long)(UNITS ? unit[i] : 1));
             }
+            __syncthreads();
+            // from the highest on: the first at which `want` is reached, or the last that has any
+            const uint32_t l = t & 63;
+            const uint64_t mine = s.sums[level][63 - l], to = wave_scan(mine);
+            const uint64_t has = __builtin_amdgcn_ballot_w64(mine != 0), hit = __builtin_amdgcn_ballot_w64(mine != 0 && before + above + to >= want);
+            const int x = hit ? __builtin_ctzll(hit) : has ? 63 - __builtin_clzll(has) : 63;
+            const uint64_t sum = to - mine;
+            above += (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(sum >> 32), x) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)sum, x);
+            own = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(mine >> 32), x) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, x);
+            value |= (uint32_t)(63 - x) << shift;
+            top = shift;
+            if (!top) break;
         }
-        above = have == room ? room : count([&](uint32_t k, uint32_t d, uint32_t) { return (LOW ? d : k) > from; });
-        return from;
+        __syncthreads();        // the sums are cleared again by the next call
+        return (sm_found){value, above, own};
     }
-    // The order from which on `room` entries stay; of the entries it leaves that key's own, if it had to choose among them.
+    // The order from which on `room` entries stay.
     __device__ __forceinline__ uint64_t first(uint32_t room) {
-        uint32_t above, unused;
-        const uint32_t key0 = nth<false>(room, above);
-        if (above >= room) return (uint64_t)key0 << 32;
-        keep([&](uint32_t k, uint32_t, uint32_t) { return k == key0; });
-        return (uint64_t)key0 << 32 | nth<true>(room - above, unused);
+        const sm_found k = reach<false, false>(0, room);
+        if (k.above + k.own <= room) return (uint64_t)k.value << 32;
+        keep([&](uint32_t x, uint32_t, uint32_t, uint64_t) { return x == k.value; });
+        return (uint64_t)k.value << 32 | reach<true, false>(k.above, room).value;
     }
 };
-typedef sm_over<64, SM_ALONE / 64> sm_alone;
-typedef sm_over<SM_THREADS, SM_LIST / SM_THREADS> sm_together;
 // The lowest order that stays under top_k and top_p.
-template <typename Over>
 __device__ __forceinline__ uint64_t sm_end(sm_list &list, const sm_set &set, const sm_all &all, const sm_border &b, double up) {
     uint64_t border = 0, whole = b.whole;
     if (b.kbin < SM_BINS) {
-        auto in = [&](uint32_t, uint32_t, uint32_t bin) { return (bin & ~SM_LOW) == b.kbin; };
-        Over v(list);
-        v.keep(in);
-        if (v.count([](uint32_t, uint32_t, uint32_t bin) { return bin != 0xFFFFFFFFu; }) > set.top_k - b.kabove) border = v.first(set.top_k - b.kabove);
+        sm_over v(list);
+        v.keep([&](uint32_t, uint32_t, uint32_t bin, uint64_t) { return (bin & ~SM_LOW) == b.kbin; });
+        if (v.count() > set.top_k - b.kabove) border = v.first(set.top_k - b.kabove);
+        __syncthreads();
     }
     if (b.plo < SM_BINS) {
-        Over v(list);
+        sm_over v(list);
         if (b.kbin < SM_BINS)
             whole = b.ksum + v.units([&](uint32_t k, uint32_t d, uint32_t bin) { return (bin & ~SM_LOW) == b.kbin && ((uint64_t)k << 32 | d) >= border; });
-        const double want = (double)set.top_p * (double)whole;
-        const uint64_t units = want > 0.0 ? (uint64_t)ceil(want) : 0;
-        v.keep([&](uint32_t k, uint32_t d, uint32_t bin) { const uint32_t x = bin & ~SM_LOW; return x >= b.plo && x <= b.phi && ((uint64_t)k << 32 | d) >= border; });
-        const uint32_t key = v.template top<false>(b.psum, units);
+        const double limit = ceil((double)set.top_p * (double)whole);
+        const uint64_t want = max(limit > 0.0 ? (uint64_t)limit : 0, b.psum + 1);
+        // ids of no units never stay: those of all others come first, and add up to more than is wanted
+        v.keep([&](uint32_t k, uint32_t d, uint32_t bin, uint64_t u) {
+            const uint32_t x = bin & ~SM_LOW;
+            return u && x >= b.plo && x <= b.phi && ((uint64_t)k << 32 | d) >= border;
+        });
+        const sm_found k = v.reach<false, true>(b.psum, want);
         // of that key's ids, as many as it takes
-        const uint32_t ties = v.count([&](uint32_t k, uint32_t, uint32_t) { return k == key; });
+        const uint64_t unit = max((uint64_t)1, sm_units(sm_weight(sm_value(k.value), all.top, set.inv), up));
+        const uint64_t ties = k.own / unit, ahead = b.psum + k.above, room = want > ahead ? (want - ahead + unit - 1) / unit : 1;
         uint64_t low = 0;
-        if (ties > 1) {
-            const uint64_t ahead = b.psum + v.units([&](uint32_t k, uint32_t, uint32_t) { return k > key; });
-            const uint64_t unit = sm_units(sm_weight(sm_value(key), all.top, set.inv), up);
-            const uint64_t room = units > ahead ? unit ? (units - ahead + unit - 1) / unit : ties : 1;
-            if (room < ties) {
-                uint32_t unused;
-                v.keep([&](uint32_t k, uint32_t, uint32_t) { return k == key; });
-                low = v.template nth<true>((uint32_t)room, unused);
-            }
+        if (room < ties) {
+            v.keep([&](uint32_t x, uint32_t, uint32_t, uint64_t) { return x == k.value; });
+            low = v.reach<true, false>(0, room).value;
         }
-        border = max(border, (uint64_t)key << 32 | low);
+        border = max(border, (uint64_t)k.value << 32 | low);
     }
     return border;
 }
@@ -522,25 +506,19 @@ __device__ __forceinline__ bool sm_resolve(sm_list &s, const sm_row &w, const sm
     }
     if (t == 0) s.n = n;
     __syncthreads();
-    if (n > SM_ALONE) {
-        const uint64_t border = sm_end<sm_together>(s, set, all, b, up);
-        if (t == 0) s.border = border;
-    } else if (t < 64) {
-        const uint64_t border = sm_end<sm_alone>(s, set, all, b, up);
-        if (t == 0) s.border = border;
-    }
+    const uint64_t border = sm_end(s, set, all, b, up);
+    if (t == 0) s.border = border;
     __syncthreads();
     return true;
 }
 
 // The token among the list's ids that stay, and their units.
-template <typename Over>
 __device__ __forceinline__ uint32_t sm_choose(sm_list &list, float u, uint64_t &whole) {
-    Over v(list);
+    sm_over v(list);
     const uint64_t border = list.border;
-    v.keep([&](uint32_t k, uint32_t d, uint32_t bin) { return ((uint64_t)k << 32 | d) >= border && !(bin & SM_LOW); });
+    v.keep([&](uint32_t k, uint32_t d, uint32_t bin, uint64_t units) { return units && ((uint64_t)k << 32 | d) >= border && !(bin & SM_LOW); });
     whole = v.units([](uint32_t, uint32_t, uint32_t) { return true; });
-    return ~v.template top<true>(0, (uint64_t)((double)u * (double)whole) + 1);
+    return ~v.reach<true, true>(0, (uint64_t)((double)u * (double)whole) + 1).value;
 }
 
 // The token of a row's part in which the units pass `want` (counted from the part's start), and the part's probabilities.
@@ -815,9 +793,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a,
         }
         const uint64_t border = list.border;
         uint64_t whole;
-        uint32_t id;
-        if (list.n > SM_ALONE) id = sm_choose<sm_together>(list, s.u, whole);
-        else if (t < 64) id = sm_choose<sm_alone>(list, s.u, whole);
+        const uint32_t id = sm_choose(list, s.u, whole);
         if (t == 0) a.token[r] = id;
         if (!a.probs || t >= 64) return;
         auto in = [&](uint32_t j) { return list.order[j] >= border && !(list.bin[j] & SM_LOW); };
