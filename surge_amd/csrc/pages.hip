@@ -473,9 +473,12 @@ __global__ void __launch_bounds__(TPB) k_attn_paged_join(sgk_attn_paged_args a, 
 static ap_part ap_plan(const sgk_attn_paged_args *a, char *at, uint64_t *bytes) {
     const uint64_t rows = (uint64_t)a->c.n_seq * a->n_heads, cap = (uint64_t)a->c.width << a->c.log;
     const uint64_t steps = (cap + AP_STEP - 1) / AP_STEP * a->c.n_seq;      // at most
-    // as many parts as workgroups are resident together; a sequence's last part is counted too, unless there are that many
-    const uint64_t there = (uint64_t)(a->c.hd == 256 ? 2 : a->c.hd == 128 ? 3 : 4) * sgk_device_cus() / a->c.n_kv;
-    uint64_t most = there > 2 * a->c.n_seq ? there - a->c.n_seq : there;
+    // Workgroups that are there together: two a CU, which even out sequences of unlike lengths, or one where a single sequence
+    // is cut evenly anyway and 64 KB a CU are still asked for at once (head_dim 128; 64 has two). More of them are slower:
+    // 262000 slots of 256 178 us with one, 182 with two, 196 with four; 200000 of one head of 128 40, 44, 48.5 (three);
+    // 8 sequences of 128 56.7 with two, 59.9 with three. A sequence's last part is short, so that n_seq - 1 more may come up.
+    const uint64_t there = (uint64_t)(a->c.n_seq == 1 && a->c.hd >= 128 ? 1 : 2) * sgk_device_cus() / a->c.n_kv;
+    uint64_t most = there >= 2 * a->c.n_seq ? there - (a->c.n_seq - 1) : there;
     if (most > AP_MOST) most = AP_MOST;
     if (most > (steps + AP_WAVES - 1) / AP_WAVES) most = (steps + AP_WAVES - 1) / AP_WAVES;
     if (!most) most = 1;
