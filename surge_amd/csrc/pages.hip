@@ -546,6 +546,8 @@ extern "C" hipError_t sgk_attn_paged(const sgk_attn_paged_args *a, void *scratch
 #define EV_THREADS 1024
 #define EV_BINS 2048u
 #define EV_LIST 2048u       // keys of the first histogram's bin that are listed
+#define EV_PART 4096u       // slots of a workgroup where a row has several
+#define EV_WIDE 24576u      // slots of a row from which on it has several
 #define EV_OUT 8u          // rows too many that go one by one
 struct ev_list { uint32_t *hole, *mover, *n; };      // [row][most] twice, [row]: rows to move; NULL: the few are moved at once
 __host__ __device__ static inline uint32_t ev_most(uint32_t keep, uint32_t cap) { return keep < cap - keep ? keep : cap - keep; }
@@ -858,33 +860,294 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict(sgk_page_evict_args a
     const uint32_t units = a.c.hd / 8;
     for (uint32_t i = t; i < moves * units; i += T) ev_move(a, s, h, few[1][i / units], few[0][i / units], i % units, units);
 }
+// The same over several workgroups a row, EV_PART slots each, in three launches: the histograms of the parts (1); the border
+// bin, the parts' marks that it decides, its keys listed in the order of their slots (2); the border and the marks (3). What a
+// part's marks are numbered from follows from the counts of the parts before it and the list, so that no launch waits within.
+struct ev_wide {
+    uint32_t *hist, *count, *found;     // [row][parts][EV_BINS], [row][parts][2]: freed and moved, [row][4]: last, bin, left, here
+    uint64_t *list;                     // [row][cap]: key, slot
+    uint32_t parts;
+};
+struct ev_part {
+    uint32_t len, keep, j0, used;       // used: parts with slots
+    uint64_t row, cap;
+    bool whole;                         // all slots stay
+};
+__device__ __forceinline__ ev_part ev_part_of(const sgk_page_evict_args &a) {
+    ev_part p;
+    p.len = page_len(a.c, a.lens, blockIdx.z);
+    p.cap = (uint64_t)a.c.width << a.c.log;
+    p.whole = p.len <= a.keep;
+    p.keep = min(a.keep, p.len);
+    p.j0 = blockIdx.x * EV_PART;
+    p.used = (p.len + EV_PART - 1) / EV_PART;
+    p.row = (uint64_t)blockIdx.z * a.c.n_kv + blockIdx.y;
+    return p;
+}
+constexpr uint32_t EV_OWN = EV_PART / EV_THREADS;
+__device__ __forceinline__ void ev_own(const sgk_page_evict_args &a, const ev_part &p, int32_t last, uint32_t (&key)[EV_OWN]) {
+    float y[EV_OWN];
+    int32_t x[EV_OWN];
+#pragma unroll
+    for (uint32_t i = 0; i < EV_OWN; i++) {
+        const uint32_t j = min(p.j0 + i * EV_THREADS + threadIdx.x, p.len - 1);
+        y[i] = a.weight[p.row * p.cap + j];
+        x[i] = a.pos[p.row * p.cap + j];
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < EV_OWN; i++) key[i] = ev_key(y[i], x[i], last, a.recent);
+}
+// The numbers, in the order of the slots, of a part's marked slots.
+__device__ __forceinline__ void ev_number(const bool (&m)[EV_OWN], uint32_t (&at)[EV_OWN], uint32_t *sub) {
+    static_assert(EV_OWN * (EV_THREADS / 64) == 64, "a lane each");
+    const uint32_t t = threadIdx.x, l = t & 63, wv = t >> 6;
+    uint64_t b[EV_OWN];
+#pragma unroll
+    for (uint32_t i = 0; i < EV_OWN; i++) {
+        b[i] = __builtin_amdgcn_ballot_w64(m[i]);
+        if (l == 0) sub[i * (EV_THREADS / 64) + wv] = (uint32_t)__popcll(b[i]);
+    }
+    __syncthreads();
+    const uint32_t v = sub[l], before = wave_scan(v) - v;
+#pragma unroll
+    for (uint32_t i = 0; i < EV_OWN; i++)
+        at[i] = (uint32_t)__builtin_amdgcn_readlane((int)before, i * (EV_THREADS / 64) + __builtin_amdgcn_readfirstlane((int)wv)) + lanes_below(b[i]);
+}
+// Over the workgroup, two sums.
+__device__ __forceinline__ void ev_sums(uint32_t &x, uint32_t &y, uint32_t (*tmp)[16]) {
+    x = wave_sum(x);
+    y = wave_sum(y);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) { tmp[0][threadIdx.x >> 6] = x; tmp[1][threadIdx.x >> 6] = y; }
+    __syncthreads();
+    x = y = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < EV_THREADS / 64; i++) { x += tmp[0][i]; y += tmp[1][i]; }
+    __syncthreads();
+}
+// The bin in which `left` keys from the top are reached, for all threads: bin, keys above it, its own. v: thread t's two bins,
+// EV_BINS - 1 - 2 t and the one below.
+__device__ __forceinline__ void ev_find(uint32_t left, uint32_t v0, uint32_t v1, uint32_t *pick, uint32_t (*tmp)[16], int &at) {
+    static_assert(EV_BINS == 2 * EV_THREADS, "two bins a thread");
+    uint32_t unused;
+    const uint32_t b = EV_BINS - 1 - 2 * threadIdx.x, above = ev_scan(v0 + v1, &unused, tmp, at);
+    if (above < left && above + v0 >= left) { pick[0] = b; pick[1] = above; pick[2] = v0; }
+    else if (above + v0 < left && above + v0 + v1 >= left) { pick[0] = b - 1; pick[1] = above + v0; pick[2] = v1; }
+    __syncthreads();
+}
+__global__ void __launch_bounds__(EV_THREADS) k_page_evict_hist(sgk_page_evict_args a, ev_list w, ev_wide v) {
+    constexpr uint32_t T = EV_THREADS, W = T / 64;
+    __shared__ uint32_t bins[EV_BINS];
+    __shared__ int32_t lasts[W];
+    const uint32_t t = threadIdx.x;
+    const ev_part p = ev_part_of(a);
+    const float *wt = a.weight + p.row * p.cap;
+    const int32_t *ps = a.pos + p.row * p.cap;
+    float *wo = a.weight_out + p.row * p.cap;
+    int32_t *po = a.pos_out + p.row * p.cap;
+    if (blockIdx.x == 0 && t == 0) w.n[p.row] = 0;
+    // all of the first `keep` to the outputs; moved rows come over them in a later launch
+#pragma unroll
+    for (uint32_t i = 0; i < EV_OWN; i++) {
+        const uint32_t j = p.j0 + i * T + t;
+        if (j < p.keep && wo != wt) wo[j] = wt[j];
+        if (j < p.keep && po != ps) po[j] = ps[j];
+    }
+    if (p.whole || p.j0 >= p.len) return;
+    for (uint32_t i = t; i < EV_BINS; i += T) bins[i] = 0;
+    int32_t last = INT32_MIN;
+    for (uint32_t j0 = t; j0 - t < p.len; j0 += 16 * T) {
+        int32_t x[16];
+#pragma unroll
+        for (uint32_t i = 0; i < 16; i++) x[i] = ps[min(j0 + i * T, p.len - 1)];
+#pragma unroll
+        for (uint32_t i = 0; i < 16; i++) last = max(last, x[i]);
+    }
+    last = (int32_t)(wave_umax((uint32_t)last ^ 0x80000000u) ^ 0x80000000u);
+    if ((t & 63) == 0) lasts[t >> 6] = last;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < W; i++) last = max(last, lasts[i]);
+    uint32_t key[EV_OWN];
+    ev_own(a, p, last, key);
+#pragma unroll
+    for (uint32_t i = 0; i < EV_OWN; i++)
+        if (p.j0 + i * T + t < p.len) atomicAdd(&bins[key[i] >> 21], 1u);
+    __syncthreads();
+    uint32_t *to = v.hist + (p.row * v.parts + blockIdx.x) * EV_BINS;
+    for (uint32_t i = t; i < EV_BINS; i += T) to[i] = bins[i];
+    if (blockIdx.x == 0 && t == 0) v.found[4 * p.row] = (uint32_t)last;
+}
+__global__ void __launch_bounds__(EV_THREADS) k_page_evict_list(sgk_page_evict_args a, ev_wide v) {
+    constexpr uint32_t T = EV_THREADS;
+    __shared__ uint32_t tmp[2][16], pick[3], sub[64];
+    const uint32_t t = threadIdx.x;
+    const ev_part p = ev_part_of(a);
+    if (p.whole || p.j0 >= p.len) return;
+    const int32_t last = (int32_t)v.found[4 * p.row];
+    uint32_t key[EV_OWN];
+    ev_own(a, p, last, key);
+    const uint32_t *hist = v.hist + p.row * v.parts * EV_BINS;
+    int at = 0;
+    uint64_t two = 0;       // a pair of bins: their sums stay below 2^32
+#pragma unroll 8
+    for (uint32_t q = 0; q < p.used; q++) two += *(const uint64_t *)(hist + q * EV_BINS + EV_BINS - 2 - 2 * t);
+    ev_find(p.keep, (uint32_t)(two >> 32), (uint32_t)two, pick, tmp, at);
+    const uint32_t bin = pick[0], left = p.keep - pick[1], here = pick[2];
+    if (blockIdx.x == 0 && t == 0) { v.found[4 * p.row + 1] = bin; v.found[4 * p.row + 2] = left; v.found[4 * p.row + 3] = here; }
+    uint32_t freed = 0, moved = 0;
+    bool in[EV_OWN];
+#pragma unroll
+    for (uint32_t i = 0; i < EV_OWN; i++) {
+        const uint32_t j = p.j0 + i * T + t, x = key[i] >> 21;
+        in[i] = left != here && j < p.len && x == bin;
+        freed += j < p.keep && x < bin;
+        moved += j >= p.keep && j < p.len && x > bin;
+    }
+    ev_sums(freed, moved, tmp);
+    if (t == 0) { v.count[2 * (p.row * v.parts + blockIdx.x)] = freed; v.count[2 * (p.row * v.parts + blockIdx.x) + 1] = moved; }
+    if (left == here) return;
+    uint32_t base = 0, to[EV_OWN];
+    for (uint32_t q = t & 63; q < blockIdx.x; q += 64) base += hist[q * EV_BINS + bin];
+    base = wave_sum(base);
+    ev_number(in, to, sub);
+#pragma unroll
+    for (uint32_t i = 0; i < EV_OWN; i++)
+        if (in[i]) v.list[p.row * p.cap + base + to[i]] = (uint64_t)key[i] << 32 | (p.j0 + i * T + t);
+}
+__global__ void __launch_bounds__(EV_THREADS) k_page_evict_mark(sgk_page_evict_args a, ev_list w, ev_wide v) {
+    constexpr uint32_t T = EV_THREADS;
+    __shared__ uint32_t bins[EV_BINS], tmp[2][16], pick[3], sub[64];
+    const uint32_t t = threadIdx.x;
+    const ev_part p = ev_part_of(a);
+    if (p.whole || p.j0 >= p.len) return;
+    const uint32_t *found = v.found + 4 * p.row;
+    const uint32_t listed = found[3];
+    uint32_t border = found[1] << 21, left = found[2], here = listed, tie = UINT32_MAX;
+    const uint64_t *list = v.list + p.row * p.cap;
+    const bool all = left == here;      // the whole border bin stays: there is no list
+    uint32_t key[EV_OWN];
+    ev_own(a, p, (int32_t)found[0], key);
+    int at = 0;
+    for (int pass = 1; pass < 3 && left != here; pass++) {
+        const uint32_t shift = pass == 1 ? 10 : 0, mask = pass == 1 ? 2047u : 1023u, up = pass == 1 ? 21 : 10;
+        for (uint32_t i = t; i < EV_BINS; i += T) bins[i] = 0;
+        __syncthreads();
+#pragma unroll 4
+        for (uint32_t i = t; i < listed; i += T) {
+            const uint32_t k = (uint32_t)(list[i] >> 32);
+            if ((k ^ border) >> up == 0) atomicAdd(&bins[k >> shift & mask], 1u);
+        }
+        __syncthreads();
+        ev_find(left, bins[EV_BINS - 1 - 2 * t], bins[EV_BINS - 2 - 2 * t], pick, tmp, at);
+        border |= pick[0] << shift;
+        left -= pick[1];
+        here = pick[2];
+        __syncthreads();
+    }
+    if (left != here) {     // alike ones: up to the left-th slot
+        uint32_t seen = 0;
+        for (uint32_t i0 = 0; i0 < listed && seen < left; i0 += T) {
+            const uint64_t e = i0 + t < listed ? list[i0 + t] : 0;
+            const uint32_t is = i0 + t < listed && (uint32_t)(e >> 32) == border;
+            uint32_t n;
+            const uint32_t before = seen + ev_scan(is, &n, tmp, at);
+            if (is && before + 1 == left) pick[0] = (uint32_t)e;
+            seen += n;
+        }
+        __syncthreads();
+        tie = pick[0];
+    }
+    auto stays = [&](uint32_t k, uint32_t j) { return tie == UINT32_MAX ? k >= border : k > border || (k == border && j <= tie); };
+    // marks in front of the part's, and all freed ones
+    uint32_t front = 0, moves = 0;
+    for (uint32_t q = t; q < p.used; q += T) {
+        const uint32_t *n = v.count + 2 * (p.row * v.parts + q);
+        moves += n[0];
+        if (q < blockIdx.x) front += n[0] + n[1];
+    }
+    for (uint32_t i = t; i < listed && !all; i += T) {
+        const uint32_t j = (uint32_t)list[i];
+        const bool s = stays((uint32_t)(list[i] >> 32), j), m = (j < p.keep) != s;
+        moves += j < p.keep && !s;
+        front += m && j < p.j0;
+    }
+    ev_sums(front, moves, tmp);
+    bool m[EV_OWN];
+    uint32_t to[EV_OWN];
+#pragma unroll
+    for (uint32_t i = 0; i < EV_OWN; i++) {
+        const uint32_t j = p.j0 + i * T + t;
+        m[i] = j < p.len && (j < p.keep) != stays(key[i], j);
+    }
+    ev_number(m, to, sub);
+    const uint64_t most = ev_most(a.keep, (uint32_t)p.cap);
+#pragma unroll
+    for (uint32_t i = 0; i < EV_OWN; i++) {
+        const uint32_t j = p.j0 + i * T + t, r = front + to[i];
+        if (m[i]) *(j < p.keep ? w.hole + p.row * most + r : w.mover + p.row * most + (r - moves)) = j;
+    }
+    if (blockIdx.x == 0 && t == 0) w.n[p.row] = moves;
+}
 __global__ void __launch_bounds__(TPB) k_page_evict_move(sgk_page_evict_args a, ev_list w) {
     const uint32_t h = blockIdx.y, s = blockIdx.z, units = a.c.hd / 8, most = ev_most(a.keep, a.c.width << a.c.log);
     const uint64_t row = (uint64_t)s * a.c.n_kv + h, n = (uint64_t)w.n[row] * units;
     for (uint64_t i = (uint64_t)blockIdx.x * TPB + threadIdx.x; i < n; i += (uint64_t)gridDim.x * TPB)
         ev_move(a, s, h, w.mover[row * most + i / units], w.hole[row * most + i / units], (uint32_t)(i % units), units);
 }
+// The parts of a row that are selected by as many workgroups; 0: one workgroup.
+static uint32_t ev_parts(const sgk_page_evict_args *a) {
+    const uint32_t cap = a->c.width << a->c.log, parts = (cap + EV_PART - 1) / EV_PART;
+    if (ev_most(a->keep, cap) <= EV_FEW || cap < EV_WIDE) return 0;
+    return (uint64_t)parts * a->c.n_seq * a->c.n_kv <= 3ull * sgk_device_cus() / 2 ? parts : 0;
+}
+static uint64_t ev_plan(const sgk_page_evict_args *a, char *at, ev_list *w, ev_wide *v) {
+    const uint64_t rows = (uint64_t)a->c.n_seq * a->c.n_kv, cap = (uint64_t)a->c.width << a->c.log, most = ev_most(a->keep, (uint32_t)cap);
+    uint64_t n = 0;
+    auto take = [&](uint64_t words) { char *o = at + 4 * n; n += (words + 3) / 4 * 4; return o; };
+    *w = (ev_list){};
+    *v = (ev_wide){};
+    if (most <= EV_FEW) return 0;
+    w->hole = (uint32_t *)take(rows * most);
+    w->mover = (uint32_t *)take(rows * most);
+    w->n = (uint32_t *)take(rows);
+    v->parts = ev_parts(a);
+    if (!v->parts) return 4 * n;
+    v->list = (uint64_t *)take(2 * rows * cap);
+    v->hist = (uint32_t *)take(rows * v->parts * EV_BINS);
+    v->count = (uint32_t *)take(2 * rows * v->parts);
+    v->found = (uint32_t *)take(4 * rows);
+    return 4 * n;
+}
 extern "C" uint64_t sgk_page_evict_scratch(const sgk_page_evict_args *a) {
-    const uint32_t most = ev_most(a->keep, a->c.width << a->c.log);
-    return most <= EV_FEW ? 0 : 4 * (uint64_t)a->c.n_seq * a->c.n_kv * (2 * (uint64_t)most + 1);
+    ev_list w;
+    ev_wide v;
+    return ev_plan(a, NULL, &w, &v);
 }
 extern "C" hipError_t sgk_page_evict(const sgk_page_evict_args *a, void *scratch, hipStream_t s, hipEvent_t done) {
-    const uint32_t cap = a->c.width << a->c.log, most = ev_most(a->keep, cap);
-    const uint64_t rows = (uint64_t)a->c.n_seq * a->c.n_kv, each = rows * most;
-    const bool few = most <= EV_FEW;
-    uint32_t *u = (uint32_t *)scratch;
-    const ev_list w = {few ? NULL : u, few ? NULL : u + each, few ? NULL : u + 2 * each};
-    const bool held = cap <= EV_HELD;
-    void (*const k)(sgk_page_evict_args, ev_list) = held ? k_page_evict<true> : k_page_evict<false>;
-    const uint32_t lds = held ? cap * 4 : 0;
-    if (lds > 49152) {
-        const hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess) return e;
+    const uint32_t cap = a->c.width << a->c.log, most = ev_most(a->keep, cap), rows = a->c.n_seq * a->c.n_kv;
+    ev_list w;
+    ev_wide v;
+    ev_plan(a, (char *)scratch, &w, &v);
+    const bool few = !w.n;
+    if (v.parts) {
+        const dim3 grid(v.parts, a->c.n_kv, a->c.n_seq);
+        launch(k_page_evict_hist, grid, EV_THREADS, s, (hipEvent_t)NULL, *a, w, v);
+        launch(k_page_evict_list, grid, EV_THREADS, s, (hipEvent_t)NULL, *a, v);
+        launch(k_page_evict_mark, grid, EV_THREADS, s, (hipEvent_t)NULL, *a, w, v);
+    } else {
+        const bool held = cap <= EV_HELD;
+        void (*const k)(sgk_page_evict_args, ev_list) = held ? k_page_evict<true> : k_page_evict<false>;
+        const uint32_t lds = held ? cap * 4 : 0;
+        if (lds > 49152) {
+            const hipError_t e = hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e != hipSuccess) return e;
+        }
+        launch_lds(k, dim3(a->c.n_kv, a->c.n_seq), EV_THREADS, lds, s, few ? done : (hipEvent_t)NULL, *a, w);
     }
-    launch_lds(k, dim3(a->c.n_kv, a->c.n_seq), EV_THREADS, lds, s, few ? done : (hipEvent_t)NULL, *a, w);
-    if (!few) {
-        const uint64_t b = ((uint64_t)most * (a->c.hd / 8) + TPB - 1) / TPB;
-        launch(k_page_evict_move, dim3((uint32_t)(b < 256 ? b : 256), a->c.n_kv, a->c.n_seq), TPB, s, done, *a, w);
+    if (!few) {     // a trip a thread, but about 8192 workgroups in all
+        const uint64_t b = ((uint64_t)most * (a->c.hd / 8) + TPB - 1) / TPB, all = max(8u, 8192u / rows);
+        launch(k_page_evict_move, dim3((uint32_t)(b < all ? b : all), a->c.n_kv, a->c.n_seq), TPB, s, done, *a, w);
     }
     return hipGetLastError();
 }
