@@ -1002,7 +1002,7 @@ __global__ void __launch_bounds__(EV_THREADS) k_page_evict_list(sgk_page_evict_a
         const uint32_t j = p.j0 + i * T + t, x = key[i] >> 21;
         in[i] = left != here && j < p.len && x == bin;
         freed += j < p.keep && x < bin;
-        moved += j >= p.keep && j < p.len && x > bin;
+        moved += j >= p.keep && j < p.len && x + (left == here) > bin;     // all of the bin stay, or the list tells
     }
     ev_sums(freed, moved, tmp);
     if (t == 0) { v.count[2 * (p.row * v.parts + blockIdx.x)] = freed; v.count[2 * (p.row * v.parts + blockIdx.x) + 1] = moved; }
