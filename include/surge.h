@@ -489,8 +489,8 @@ sg_err sg_gpu_run_page_evict(sg_gpu *g, void *kp, void *vp, void *table, void *l
  * u outside [0, 1) is taken as the nearest inside, NaN as 0. probs, if not NULL,
  * f32 [rows][vocab]: w / sum of those that stayed, 0 for the others; it may be logits
  * (as with the rotary axes). w and sums are held in 64 bits, sums as integers in units
- * of less than the sum's 2^-60: no order of additions changes a result. vocab < 2^31,
- * rows <= 65535.
+ * of the sum's 2^-54 at most (an id that stays has one at least): no order of additions
+ * changes a result. vocab < 2^31, rows <= 65535.
  * p: [0]=vocab [1]=rows. */
 sg_err sg_gpu_run_sample(sg_gpu *g, void *logits, void *settings, void *u, void *token, void *probs, const uint32_t params[8]);
 

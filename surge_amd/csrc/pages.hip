@@ -28,7 +28,11 @@ __device__ __forceinline__ uint32_t page_len(const sgk_pages &c, const int32_t *
 }
 
 // ---------------------------------------------------------------------------
-// Store: 8 dims of K and of V per thread, rounded to f16 (nearest even).
+// Store: 8 dims of K and of V per thread, rounded to f16 (nearest even). Bound by
+// memory (8190 rows of 4 x 256, 100 MB read and written: 20.4 us, 4.9 TB/s, as a
+// copy) or, a few rows, by one trip to the spans, the table and the rows (3.1 us).
+// Asking for the data before the span and the page are known changes neither
+// (3.0; 21.2).
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ f16x8 half8(const float *p, bool al) {
     const f32x4 a = ld4(p, al), b = ld4(p + 4, al);
@@ -89,7 +93,18 @@ extern "C" hipError_t sgk_page_store(const sgk_page_store_args *a, hipStream_t s
 //
 // Parts: T steps in all and `most` parts a kv head wanted give parts of `per` =
 // ceil(T / most) steps, a multiple of the waves, the same on every workgroup; a
-// sequence of n steps has ceil(n / per) of them, so there are at most most + n_seq.
+// sequence of n steps has ceil(n / per) of them, so there are at most most + n_seq,
+// and its steps are spread over them evenly (64 sequences of 1800 to 2300 slots: 78
+// us, 94 with a short last part).
+//
+// Bound by reading K and V once: a step's products are a tenth of its time on the
+// matrix units. A wave has its next step's K and V under way all the time, 8 to 32 KB,
+// and 32 slots a step are what its registers hold at head_dim 256 (242 of 256). What
+// is read once goes past the caches' order of use (non-temporal: 262000 slots of 4 x
+// 256 178 us against 185). 174 us for those 1073 MB, 6.2 TB/s (a plain read of as much
+// 181), 77 for 64 sequences' 401 MB, 50.9 for 16 of 91 to 16411 slots, 231 MB. About 9
+// us of each are the chain that a short call consists of (4 sequences of 57 to 700
+// slots, 9.2): lengths, table, rows, two products, the waves' sums.
 // ---------------------------------------------------------------------------
 #define AP_STEP 32u
 #define AP_WAVES 4u
@@ -533,22 +548,31 @@ extern "C" hipError_t sgk_attn_paged(const sgk_attn_paged_args *a, void *scratch
 // Eviction. The order of a (sequence, kv head)'s slots: recent ones first, then
 // by weight, then the lower slot; the first `keep` stay. A workgroup holds the
 // slots' keys in LDS (EV_HELD of them; past that it reads weight and pos again
-// each time) and finds the keep-th by three histograms, of 11, 11 and 10 bits
-// (weights share few exponents: with 8 bits, and lanes with the same bin not added
-// first, the additions wait for each other). Slots below keep that go are freed
-// places, kept ones from keep on are moved rows: as many, both in rising order, so
-// one prefix sum over both marks numbers them. No row that is read is written, so
-// the moves need no order. Loops are not unrolled far: code that runs once comes
-// from memory (keys in registers, 64 a thread: 150 KB of it, slower than LDS).
+// each time) and finds the keep-th by histograms of 11, 11 and 10 bits (weights
+// share few exponents: with 8 bits the additions wait for each other), the last
+// two over the keys of the first one's bin alone where those can be listed. Slots
+// below keep that go are freed places, kept ones from keep on are moved rows: as
+// many, both in rising order, so one prefix sum over both marks numbers them. No
+// row that is read is written, so the moves need no order.
+//
+// A few rows too many (a cache that is held at keep) go one by one, the lowest of
+// the workgroup's lowest. Long rows, where they are few, have several workgroups
+// (below). Bound by the chain of passes of a CU over its keys, each some trips to
+// LDS long, then by the moves: 64 rows of 2049 slots to 2048 5.9 us, 8 of 32768 to
+// 4096 8.8 + 6.8 + 6.9 us in three launches (31.3 by one workgroup a row), and 15.2
+// for the moves (59 MB, behind two dependent trips). 256 threads
+// a row are slower even at 4000 slots (23 us, 14). Loops are not unrolled far: code
+// that runs once comes from memory (keys in registers, 64 a thread: 150 KB of it,
+// 45 us).
 // ---------------------------------------------------------------------------
-#define EV_FEW 64u          // rows that the selecting workgroup moves itself
+#define EV_FEW 64u          // rows that the selecting workgroup moves itself (32 of 2080: 12.0 us; with a launch for them 12.2 + 4.1)
 #define EV_HELD 32896u      // keys in LDS: 128 a page past 32768, so that a prompt's new slots fit too
 #define EV_THREADS 1024
 #define EV_BINS 2048u
-#define EV_LIST 2048u       // keys of the first histogram's bin that are listed
+#define EV_LIST 2048u       // keys of the first histogram's bin that are listed (as many as fit beside EV_HELD)
 #define EV_PART 4096u       // slots of a workgroup where a row has several
-#define EV_WIDE 24576u      // slots of a row from which on it has several
-#define EV_OUT 8u          // rows too many that go one by one
+#define EV_WIDE 24576u      // slots of a row from which on it has several (16000: 19.4 us and two more launches, 18.6 by one; 24000: 21.1, 24.1)
+#define EV_OUT 8u           // rows too many that go one by one (2048 stay: 2 6.6 us, 11.3 by the border; 8 11.0, 11.6; 16 16.7, 11.8)
 struct ev_list { uint32_t *hole, *mover, *n; };      // [row][most] twice, [row]: rows to move; NULL: the few are moved at once
 __host__ __device__ static inline uint32_t ev_most(uint32_t keep, uint32_t cap) { return keep < cap - keep ? keep : cap - keep; }
 

@@ -6,12 +6,15 @@
 
 // ---------------------------------------------------------------------------
 // An id's weight is exp((x - max) / temperature), in 64 bits. Sums of weights
-// are integers in units of the row's whole sum / 2^61 or so: whatever order the
-// additions come in, the sums, the kept ids and the token are the same.
+// are integers in units of the row's whole sum / 2^60 or so (the largest weight /
+// 2^54 where at most 128 ids stay): whatever order the additions come in, the sums,
+// the kept ids and the token are the same.
 //
-// A row is SM_IDS ids a workgroup, four a thread, over the chip, in four launches
-// that each need what all of the last one found. A row's settings are known on the
-// device alone, so each launch does for a row what its kind needs:
+// A row is SM_IDS ids a workgroup, four a thread, over the chip, in three launches
+// that each need what all of the last one found, and a fourth where the
+// probabilities are wanted (without them the row's last workgroup of the third
+// goes on). A row's settings are known on the device alone, so each launch does
+// for a row what its kind needs:
 //   few    top_k of SM_FEW at most (greedy: 1). The top_k-th largest of the waves'
 //          maxima (1) is a bound that at least top_k ids reach, and hardly more:
 //          those are listed (2), ranked by comparing all with all, and the token
@@ -20,17 +23,25 @@
 //          token lies finds it (3).
 //   border a histogram of the logits' distance from the largest, counts and sums
 //          (2), gives the bins in which top_k and top_p end; their ids are listed,
-//          the sums of the ids above them taken (3), and the list ranked for the
-//          exact borders (4).
+//          the sums of the ids above them taken (3), and the list searched for the
+//          exact borders (3 or 4).
 // A list that does not fit (thousands of ids alike at a border) leaves the row to
-// one workgroup, which goes over it digit by digit (4).
+// one workgroup, which goes over it digit by digit.
+//
+// The logits are read once from memory and then from the last cache; what bounds
+// a call is the chain of launches, each a few trips to memory long. One row of
+// 151936 ids, top_k 20 and top_p 0.8: 3.0 + 6.4 + 5.8 us, the call 25.6, of which
+// 8.8 are any call's. 16 rows of all kinds 6.0 + 11.4 + 20.0 (46.4); 4 rows with
+// top_p and probabilities 4.4 + 9.0 + 8.1 + 13.4 (43). Ranking a few row's list in
+// the second launch's last workgroup: 12.4 + 2.0 us against 6.4 + 5.9, so it is
+// left to the third.
 // ---------------------------------------------------------------------------
 #define SM_THREADS 512
 #define SM_WAVES (SM_THREADS / 64)
 #define SM_IDS (4 * SM_THREADS)
 #define SM_PARTS 512u       // of a row, at most: its parts take several rounds of SM_IDS past that
-#define SM_FEW 128u
-#define SM_WGS 1024u        // workgroups that a launch has about
+#define SM_FEW 128u         // one row, the third launch: top_k 20 5.7 us, 15.6 as the third kind; 127 10.5, 15.6
+#define SM_WGS 1024u        // workgroups that a launch has about (16 rows of 151936, the launches together: 512 40.2 us, 1024 38.6, 2048 41.8)
 #define SM_LIST 2048u
 #define SM_RANKED 128u      // entries that are compared all with all
 #define SM_BINS 2048u
