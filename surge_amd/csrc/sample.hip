@@ -44,6 +44,7 @@
 #define SM_WGS 1024u        // workgroups that a launch has about (16 rows of 151936, the launches together: 512 40.2 us, 1024 38.6, 2048 41.8)
 #define SM_LIST 2048u
 #define SM_RANKED 128u      // entries that are compared all with all
+#define SM_NEAR 256u        // entries of a list that is searched by comparing all with all
 #define SM_BINS 2048u
 #define SM_NONE 0xFFFFFFFFu
 
@@ -362,151 +363,187 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
 
 // ---- a list of ids in LDS: order (key, then ~id: the larger comes first), units, bin with SM_LOW if the weight is below min_p
 #define SM_LOW 0x80000000u
-struct sm_list { uint64_t order[SM_LIST], unit[SM_LIST]; uint32_t bin[SM_LIST], n; uint64_t border, tmp[2][SM_WAVES], sums[6][64]; };
+struct sm_list { uint64_t order[SM_LIST], unit[SM_LIST]; uint32_t bin[SM_LIST], n; uint64_t tmp[2][SM_WAVES], sums[6][64], ahead[SM_THREADS]; uint32_t cnt[SM_WAVES], rank[SM_THREADS]; };
 
-// The workgroup over the list: entry i of a thread is place i SM_THREADS + t. All threads get every result.
-struct sm_found { uint32_t value; uint64_t above, own; };       // units (or entries) above the value, and its own
-struct sm_over {
-    static constexpr int U = SM_LIST / SM_THREADS;
-    sm_list &s;
-    const uint32_t t, each;
-    int at;                                 // a step's results go through half `at` of tmp, so that one barrier a step is enough
-    uint32_t key[U], low[U], bin[U];        // bin: 0xFFFFFFFF behind the list
-    uint64_t unit[U];
-    __device__ __forceinline__ sm_over(sm_list &list) : s(list), t(threadIdx.x), each((list.n + SM_THREADS - 1) / SM_THREADS), at(0) {
+// The search of a list, by the workgroup: what stays under top_k and top_p (the lowest order that does), and, where `token`,
+// the units of what stays and the token among it. It takes up to six jobs, one loop over one piece of code, since code that runs
+// once comes from memory: 0 top_k's last key; 1, of alike keys, its last id; 2 the units that top_k left; 3 top_p's last key; 4 its
+// last id; 5 the token. A job puts its entries aside, and finds the largest key (or ~id) from which on their units (or their number)
+// and `before` come to `want`, the lowest if none does: six bits a step, from the highest in which they differ, the next six bits'
+// sums in LDS, which every wave adds up. want > before; entries of no units do not count where units do.
+__device__ __forceinline__ uint64_t wave_least(uint64_t v) {
+    v = row_min(v);
+    v = min(v, both<swap16>(v));
+    return min(v, both<swap32>(v));
+}
+struct sm_result { uint64_t border, whole; uint32_t id; };
+__device__ __forceinline__ uint64_t sm_lane(uint64_t v, int x) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), x) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, x);
+}
+__device__ __forceinline__ sm_result sm_search(sm_list &s, const sm_set &set, const sm_all &all, const sm_border &b, double up, bool token) {
+    const uint32_t t = threadIdx.x, l = t & 63, wv = t >> 6, n = s.n;
+    const bool k_on = b.kbin < SM_BINS, p_on = b.plo < SM_BINS;
+    sm_result r = {0, b.whole, SM_NONE};
+    uint32_t value = 0;
+    uint64_t before = 0, want = 0;
+    const bool near = n <= SM_NEAR;
+    if (near) {
+        // a short list: each entry against all, by two or four threads: how many are above it, and their units in top_p's bins
+        uint64_t *const inside = &s.sums[0][0];
+        static_assert(sizeof(s.sums) / 8 >= SM_NEAR && SM_NEAR == SM_THREADS / 2, "the units' place");
+        const uint32_t each = n <= SM_THREADS / 4 ? SM_THREADS / 4 : SM_THREADS / 2, share = SM_THREADS / each, j = t & (each - 1);
+        const uint32_t part = ((n + share - 1) / share + 7) / 8 * 8, from = t / each * part;
+        const bool first = t < each && j < n;
+        const uint32_t y = first ? s.bin[t] & ~SM_LOW : 0;
+        const uint64_t u = first ? s.unit[t] : 0;
+        if (t < SM_NEAR) inside[t] = y >= b.plo && y <= b.phi ? u : 0;
+        if (t >= n && t < SM_NEAR) s.order[t] = 0;
+        const uint64_t earlier = __builtin_amdgcn_ballot_w64(first && y != b.kbin);        // in bins before top_k's
+        if (l == 0) s.cnt[wv] = (uint32_t)__popcll(earlier);
+        __syncthreads();
+        const uint64_t o = j < n ? s.order[j] : ~0ull;
+        uint32_t rank = 0;
+        uint64_t ahead = 0;
+        for (uint32_t i = from; i < from + part; i += 8) {
+            uint64_t x[8], z[8];
 #pragma unroll
-        for (int i = 0; i < U; i++) {
-            const uint32_t j = i * SM_THREADS + t;
-            const bool here = j < s.n;
-            key[i] = here ? (uint32_t)(s.order[j] >> 32) : 0;
-            low[i] = here ? (uint32_t)s.order[j] : 0;
-            bin[i] = here ? s.bin[j] : 0xFFFFFFFFu;
-            unit[i] = here ? s.unit[j] : 0;
+            for (uint32_t e = 0; e < 8; e++) { x[e] = s.order[i + e]; z[e] = inside[i + e]; }
+#pragma unroll
+            for (uint32_t e = 0; e < 8; e++) { rank += x[e] > o; ahead += x[e] > o ? z[e] : 0; }
         }
+        s.rank[t] = rank;
+        s.ahead[t] = ahead;
+        __syncthreads();
+        for (uint32_t i = 1; i < share; i++) {
+            rank += s.rank[(t + i * each) & (SM_THREADS - 1)];
+            ahead += s.ahead[(t + i * each) & (SM_THREADS - 1)];
+        }
+        uint32_t before_k = b.kabove;
+#pragma unroll
+        for (int i = 0; i < SM_WAVES; i++) before_k -= s.cnt[i];
+        const bool ks = first && (y != b.kbin || before_k + rank < set.top_k);      // listed bins are not past top_k's
+        if (k_on && p_on) {
+            const uint64_t sum = wave_sum(ks && y == b.kbin ? u : 0);
+            if (l == 0) s.tmp[0][wv] = sum;
+            __syncthreads();
+            r.whole = b.ksum;
+#pragma unroll
+            for (int i = 0; i < SM_WAVES; i++) r.whole += s.tmp[0][i];
+        }
+        bool stays = ks;
+        if (p_on) {
+            const double limit = ceil((double)set.top_p * (double)r.whole);
+            want = max(limit > 0.0 ? (uint64_t)limit : 0, b.psum + 1);
+            stays = ks && u && y >= b.plo && y <= b.phi && b.psum + ahead < want;
+        }
+        uint64_t lowest = wave_least(stays ? o : ~0ull);
+        if (l == 0) s.tmp[1][wv] = lowest;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < SM_WAVES; i++) lowest = min(lowest, s.tmp[1][i]);
+        r.border = lowest;
         __syncthreads();
     }
-    // From here on only the entries of which in(key, ~id, bin, units) is true.
-    template <typename In>
-    __device__ __forceinline__ void keep(In in) {
-#pragma unroll
-        for (int i = 0; i < U; i++)
-            if (bin[i] == 0xFFFFFFFFu || !in(key[i], low[i], bin[i], unit[i])) { key[i] = low[i] = 0; bin[i] = 0xFFFFFFFFu; unit[i] = 0; }
-    }
-    __device__ __forceinline__ uint64_t add(uint64_t v) {       // v: the wave's
-        if ((t & 63) == 0) s.tmp[at][t >> 6] = v;
-        __syncthreads();
-        uint64_t r = 0;
-#pragma unroll
-        for (int i = 0; i < SM_WAVES; i++) r += s.tmp[at][i];
-        at ^= 1;
-        return r;
-    }
-    __device__ __forceinline__ uint32_t count() {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < U; i++) m += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(bin[i] != 0xFFFFFFFFu));
-        return (uint32_t)add(m);
-    }
-    template <typename In>
-    __device__ __forceinline__ uint64_t units(In in) {
-        uint64_t m = 0;
-#pragma unroll
-        for (int i = 0; i < U; i++)
-            if (in(key[i], low[i], bin[i])) m += unit[i];
-        return add(wave_sum(m));
-    }
-    // The largest key (or ~id) from which on the entries' units (or the entries), and `before`, come to `want`; the lowest if
-    // none does. Six bits a step, from the highest in which they differ: the values' sums in LDS, which every wave adds up.
-    // want > before; entries of no units do not count where units do.
-    template <bool LOW, bool UNITS>
-    __device__ __forceinline__ sm_found reach(uint64_t before, uint64_t want) {
-        uint32_t lo = 0xFFFFFFFFu, hi = 0;
-#pragma unroll
-        for (int i = 0; i < U; i++)
-            if (bin[i] != 0xFFFFFFFFu) { lo = min(lo, LOW ? low[i] : key[i]); hi = max(hi, LOW ? low[i] : key[i]); }
+    for (int job = near ? 5 : k_on ? 0 : 3; job < (token ? 6 : 5); job++) {
+        if (job >= 2 && job < 5 && !p_on) continue;
+        const bool low = job == 1 || job >= 4, units = job >= 3;
+        uint32_t mask = 0, cnt = 0, lo = 0xFFFFFFFFu, hi = 0;
+        uint64_t sum = 0;
+#pragma unroll 1
+        for (uint32_t j = t, bit = 1; j < n; j += SM_THREADS, bit <<= 1) {
+            const uint64_t o = s.order[j], u = s.unit[j];
+            const uint32_t x = s.bin[j], y = x & ~SM_LOW, k = (uint32_t)(o >> 32), v = low ? (uint32_t)o : k;
+            bool in = job < 3 ? y == b.kbin : u && (job < 5 ? y >= b.plo && y <= b.phi : !(x & SM_LOW));
+            in = in && (job < 2 || o >= r.border) && ((job != 1 && job != 4) || k == value);
+            if (!in) continue;
+            mask |= bit;
+            cnt++;
+            sum += u;
+            lo = min(lo, v);
+            hi = max(hi, v);
+        }
+        sum = wave_sum(sum);
+        cnt = wave_sum(cnt);
         lo = ~wave_umax(~lo);
         hi = wave_umax(hi);
-        if ((t & 63) == 0) s.tmp[at][t >> 6] = (uint64_t)~lo << 32 | hi;
+        if (l == 0) { s.tmp[0][wv] = sum; s.tmp[1][wv] = (uint64_t)lo << 32 | hi; s.cnt[wv] = cnt; }
         if (t < 6 * 64) s.sums[t / 64][t % 64] = 0;
         __syncthreads();
-        uint32_t low_ = 0;
-#pragma unroll
-        for (int i = 0; i < SM_WAVES; i++) { low_ = max(low_, (uint32_t)(s.tmp[at][i] >> 32)); hi = max(hi, (uint32_t)s.tmp[at][i]); }
-        at ^= 1;
-        lo = ~low_;
-        int top = lo < hi ? 32 - __builtin_clz(lo ^ hi) : 0;       // bits that are not known yet
-        uint64_t above = 0, own = 0;
-        uint32_t value = top < 32 ? hi >> top << top : 0;
-        for (int level = 0;; level++) {
-            const int shift = max(top - 6, 0);
-#pragma unroll
-            for (int i = 0; i < U; i++) {
-                const uint32_t v = LOW ? low[i] : key[i];
-                if (bin[i] != 0xFFFFFFFFu && (top == 32 || (v ^ value) >> top == 0))
-                    atomicAdd((unsigned long long *)&s.sums[level][(v ^ value) >> shift], (unsigned long long)(UNITS ? unit[i] : 1));
+        // a wave's lanes 0 to 7 (and 8 to 15, ...) have the waves'
+        const uint64_t lh = s.tmp[1][l % SM_WAVES];
+        lo = ~wave_umax(~(uint32_t)(lh >> 32));
+        hi = wave_umax((uint32_t)lh);
+        cnt = wave_sum(l < SM_WAVES ? s.cnt[l] : 0);
+        sum = wave_sum(l < SM_WAVES ? s.tmp[0][l] : 0);
+        bool skip = false;
+        if (job == 0) {
+            before = 0;
+            want = set.top_k - b.kabove;
+            skip = cnt <= want;
+            if (skip) job = 1;
+        } else if (job == 2) {
+            r.whole = b.ksum + sum;
+            skip = true;
+        } else if (job == 3) {
+            const double limit = ceil((double)set.top_p * (double)r.whole);
+            before = b.psum;
+            want = max(limit > 0.0 ? (uint64_t)limit : 0, before + 1);
+        } else if (job == 5) {
+            r.whole = sum;
+            before = 0;
+            want = (uint64_t)((double)set.u * (double)sum) + 1;
+        }
+        if (!skip) {
+            int top = lo < hi ? 32 - __builtin_clz(lo ^ hi) : 0;       // bits that are not known yet
+            uint64_t above = 0, own = 0;
+            uint32_t found = top < 32 ? hi >> top << top : 0;
+            for (int level = 0;; level++) {
+                const int shift = max(top - 6, 0);
+#pragma unroll 1
+                for (uint32_t j = t, m = mask; m; j += SM_THREADS, m >>= 1) {
+                    const uint64_t o = s.order[j];
+                    const uint32_t v = (low ? (uint32_t)o : (uint32_t)(o >> 32)) ^ found;
+                    if ((m & 1) && (top == 32 || v >> top == 0))
+                        atomicAdd((unsigned long long *)&s.sums[level][v >> shift], (unsigned long long)(units ? s.unit[j] : 1));
+                }
+                __syncthreads();
+                // from the highest on: the first at which `want` is reached, or the last that has any
+                const uint64_t mine = s.sums[level][63 - l], to = wave_scan(mine);
+                const uint64_t has = __builtin_amdgcn_ballot_w64(mine != 0), hit = __builtin_amdgcn_ballot_w64(mine != 0 && before + above + to >= want);
+                const int x = hit ? __builtin_ctzll(hit) : has ? 63 - __builtin_clzll(has) : 63;
+                above += sm_lane(to - mine, x);
+                own = sm_lane(mine, x);
+                found |= (uint32_t)(63 - x) << shift;
+                top = shift;
+                if (!top) break;
             }
-            __syncthreads();
-            // from the highest on: the first at which `want` is reached, or the last that has any
-            const uint32_t l = t & 63;
-            const uint64_t mine = s.sums[level][63 - l], to = wave_scan(mine);
-            const uint64_t has = __builtin_amdgcn_ballot_w64(mine != 0), hit = __builtin_amdgcn_ballot_w64(mine != 0 && before + above + to >= want);
-            const int x = hit ? __builtin_ctzll(hit) : has ? 63 - __builtin_clzll(has) : 63;
-            const uint64_t sum = to - mine;
-            above += (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(sum >> 32), x) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)sum, x);
-            own = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(mine >> 32), x) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)mine, x);
-            value |= (uint32_t)(63 - x) << shift;
-            top = shift;
-            if (!top) break;
+            if (job == 0) {
+                value = found;
+                r.border = (uint64_t)found << 32;
+                if (above + own <= want) job = 1;       // all of that key
+                before = above;
+            } else if (job == 3) {
+                // of that key's ids, as many as it takes: of alike weights, so one or all are known without job 4
+                value = found;
+                r.border = max(r.border, (uint64_t)found << 32);
+                before += above;
+                if (before + own <= want || own == sm_units(sm_weight(sm_value(found), all.top, set.inv), up)) job = 4;
+            } else if (job == 5) {
+                r.id = ~found;
+            } else {
+                r.border = max(r.border, (uint64_t)value << 32 | found);
+            }
         }
-        __syncthreads();        // the sums are cleared again by the next call
-        return (sm_found){value, above, own};
+        __syncthreads();        // the sums are cleared again
     }
-    // The order from which on `room` entries stay.
-    __device__ __forceinline__ uint64_t first(uint32_t room) {
-        const sm_found k = reach<false, false>(0, room);
-        if (k.above + k.own <= room) return (uint64_t)k.value << 32;
-        keep([&](uint32_t x, uint32_t, uint32_t, uint64_t) { return x == k.value; });
-        return (uint64_t)k.value << 32 | reach<true, false>(k.above, room).value;
-    }
-};
-// The lowest order that stays under top_k and top_p.
-__device__ __forceinline__ uint64_t sm_end(sm_list &list, const sm_set &set, const sm_all &all, const sm_border &b, double up) {
-    uint64_t border = 0, whole = b.whole;
-    if (b.kbin < SM_BINS) {
-        sm_over v(list);
-        v.keep([&](uint32_t, uint32_t, uint32_t bin, uint64_t) { return (bin & ~SM_LOW) == b.kbin; });
-        if (v.count() > set.top_k - b.kabove) border = v.first(set.top_k - b.kabove);
-        __syncthreads();
-    }
-    if (b.plo < SM_BINS) {
-        sm_over v(list);
-        if (b.kbin < SM_BINS)
-            whole = b.ksum + v.units([&](uint32_t k, uint32_t d, uint32_t bin) { return (bin & ~SM_LOW) == b.kbin && ((uint64_t)k << 32 | d) >= border; });
-        const double limit = ceil((double)set.top_p * (double)whole);
-        const uint64_t want = max(limit > 0.0 ? (uint64_t)limit : 0, b.psum + 1);
-        // ids of no units never stay: those of all others come first, and add up to more than is wanted
-        v.keep([&](uint32_t k, uint32_t d, uint32_t bin, uint64_t u) {
-            const uint32_t x = bin & ~SM_LOW;
-            return u && x >= b.plo && x <= b.phi && ((uint64_t)k << 32 | d) >= border;
-        });
-        const sm_found k = v.reach<false, true>(b.psum, want);
-        // of that key's ids, as many as it takes
-        const uint64_t unit = max((uint64_t)1, sm_units(sm_weight(sm_value(k.value), all.top, set.inv), up));
-        const uint64_t ties = k.own / unit, ahead = b.psum + k.above, room = want > ahead ? (want - ahead + unit - 1) / unit : 1;
-        uint64_t low = 0;
-        if (room < ties) {
-            v.keep([&](uint32_t x, uint32_t, uint32_t, uint64_t) { return x == k.value; });
-            low = v.reach<true, false>(0, room).value;
-        }
-        border = max(border, (uint64_t)k.value << 32 | low);
-    }
-    return border;
+    return r;
 }
-// The list from memory, and its border; all threads. False: it does not fit.
-__device__ __forceinline__ bool sm_resolve(sm_list &s, const sm_row &w, const sm_set &set, const sm_all &all, const sm_border &b, double up, float scale) {
+// The list from memory; all threads. False: it does not fit.
+__device__ __forceinline__ bool sm_fetch(sm_list &s, const sm_row &w, const sm_set &set, const sm_all &all, double up, float scale) {
     const uint32_t t = threadIdx.x;
     const uint32_t n = __hip_atomic_load(w.listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (n > SM_LIST) return false;
+#pragma unroll 1
     for (uint32_t j = t; j < n; j += SM_THREADS) {
         const uint64_t o = __hip_atomic_load(w.list + j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const float x = sm_value((uint32_t)(o >> 32));
@@ -517,19 +554,7 @@ __device__ __forceinline__ bool sm_resolve(sm_list &s, const sm_row &w, const sm
     }
     if (t == 0) s.n = n;
     __syncthreads();
-    const uint64_t border = sm_end(s, set, all, b, up);
-    if (t == 0) s.border = border;
-    __syncthreads();
     return true;
-}
-
-// The token among the list's ids that stay, and their units.
-__device__ __forceinline__ uint32_t sm_choose(sm_list &list, float u, uint64_t &whole) {
-    sm_over v(list);
-    const uint64_t border = list.border;
-    v.keep([&](uint32_t k, uint32_t d, uint32_t bin, uint64_t units) { return units && ((uint64_t)k << 32 | d) >= border && !(bin & SM_LOW); });
-    whole = v.units([](uint32_t, uint32_t, uint32_t) { return true; });
-    return ~v.reach<true, true>(0, (uint64_t)((double)u * (double)whole) + 1).value;
 }
 
 // The token of a row's part in which the units pass `want` (counted from the part's start), and the part's probabilities.
@@ -539,9 +564,14 @@ __device__ __forceinline__ void sm_pick(const sgk_sample_args &a, const sm_plan 
     if (!here && !a.probs) return;
     uint64_t before = 0;
     if (threadIdx.x == 0) *least = SM_NONE;
+    float next[4];
+    uint32_t ni = sm_load(a, p, r, part, 0, al, next);
     for (uint32_t m = 0; m < p.rounds; m++) {
         float x[4], out[4];
-        const uint32_t i = sm_load(a, p, r, part, m, al, x);
+        const uint32_t i = ni;
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = next[e];
+        if (m + 1 < p.rounds) ni = sm_load(a, p, r, part, m + 1, al, next);
         uint64_t q[4], mine = 0;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -719,8 +749,14 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a,
         if (LAST && part == 0 && t == 0) a.token[r] = SM_NONE;
         return;
     }
+    const bool k_on = s.top_k && s.top_k < all.ok, p_on = s.top_p < 1.0f, listed_kind = s.few || k_on || p_on;
+    const double up = s.few ? 0x1p54 : sm_unit(all.sum);        // few: 2^7 ids at most
+    const float scale = s.few ? 0.0f : sm_bin_scale(s, all);
+    sm_border b;
+    bool here = true;
+    uint32_t mine_part = part;
+    uint64_t want = 0, total = 0;
     if (s.few) {
-        const double up = 0x1p54;           // 2^7 ids at most
         const uint32_t listed = *w.listed;
         if (listed <= SM_RANKED) {
             // each entry against all: four groups of waves take a quarter of the others each, for 64 or 128 entries
@@ -797,17 +833,101 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a,
             if (t == 0) w.out[0] = m;
             return;
         }
-        const sm_border b = {0, 0, s.top_p < 1.0f ? 0 : SM_BINS, 0, 0, 0, 0, 0};
-        if (!sm_resolve(list, w, s, all, b, up, 0.0f)) {
+        b = (sm_border){0, 0, s.top_p < 1.0f ? 0 : SM_BINS, 0, 0, 0, 0, 0};
+    } else if (!k_on && !p_on) {
+        const uint64_t mine = t < p.parts ? w.kept[t] : 0, before = sm_scan(mine, &total, tmp);
+        want = (uint64_t)((double)s.u * (double)total);
+        if (t == part) { found.ksum = before; found.psum = mine; }
+        __syncthreads();
+        here = want >= found.ksum && want < found.ksum + found.psum;
+        want -= found.ksum;
+    } else {
+        // the bins in which top_k and top_p end
+        constexpr uint32_t PER = SM_BINS / SM_THREADS;
+        uint32_t cnt[PER], c = 0, nall;
+        uint64_t sum[PER], u = 0, whole;
+#pragma unroll
+        for (uint32_t i = 0; i < PER; i++) {
+            cnt[i] = w.bincnt[t * PER + i];
+            sum[i] = w.binsum[t * PER + i];
+            c += cnt[i];
+            u += sum[i];
+        }
+        c = sm_scan(c, &nall, tmp32);
+        u = sm_scan(u, &whole, tmp);
+        if (t == 0) found = (sm_border){SM_BINS, 0, SM_BINS, SM_BINS, 0, 0, 0, whole};
+        __syncthreads();
+        uint64_t klo = whole, khi = whole;
+        if (k_on) {
+            uint32_t cc = c;
+            uint64_t uu = u;
+#pragma unroll
+            for (uint32_t i = 0; i < PER; i++) {
+                if (cc < s.top_k && cc + cnt[i] >= s.top_k) { found.kbin = t * PER + i; found.kabove = cc; found.ksum = uu; found.psum = uu + sum[i]; }
+                cc += cnt[i];
+                uu += sum[i];
+            }
+            __syncthreads();
+            klo = found.ksum;
+            khi = found.psum;
+            __syncthreads();
+        }
+        if (p_on) {
+            const double dlo = ceil((double)s.top_p * (double)klo), dhi = ceil((double)s.top_p * (double)khi);
+            const uint64_t wlo = dlo > 1.0 ? (uint64_t)dlo : 1, whi = dhi > 1.0 ? (uint64_t)dhi : 1;
+            uint64_t uu = u;
+#pragma unroll
+            for (uint32_t i = 0; i < PER; i++) {
+                if (uu < wlo && uu + sum[i] >= wlo) { found.plo = t * PER + i; found.psum = uu; }
+                if (uu < whi && uu + sum[i] >= whi) found.phi = t * PER + i;
+                uu += sum[i];
+            }
+            __syncthreads();
+        }
+        b = found;
+        if (p_on && b.kbin < SM_BINS) b.phi = min(b.phi, b.kbin);
+        b.first = p_on ? b.plo : b.kbin;
+        if (part == 0 && t == 0) *w.border = b;
+        uint64_t q = 0;
+        for (uint32_t m = 0; m < p.rounds; m++) {
+            float x[4];
+            const uint32_t i = sm_load(a, p, r, part, m, al, x);
+            uint32_t in = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (!(x[e] > -INFINITY)) continue;
+                const uint32_t y = sm_bin(x[e], all.top, scale);
+                if (y < b.first) {
+                    const double z = sm_weight(x[e], all.top, s.inv);
+                    if (z >= (double)s.min_p || x[e] == all.top) q += sm_units(z, up);
+                } else if (y == b.kbin || (p_on && y <= b.phi)) {
+                    in |= 1u << e;
+                }
+            }
+            sm_append(w, x, i, in);
+        }
+        q = sm_sum(q, tmp);
+        if (t == 0) __hip_atomic_store(w.kept + part, q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (!LAST) return;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // what this wave wrote has arrived
+        __syncthreads();
+        if (t == 0) least = __hip_atomic_fetch_add(w.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (least != p.parts - 1) return;
+        __syncthreads();
+    }
+    sm_result f = {};
+    if (listed_kind) {
+        if (!sm_fetch(list, w, s, all, up, scale)) {
             if (LAST) sm_slow(a, r, s, &list);
             return;
         }
-        const uint64_t border = list.border;
-        uint64_t whole;
-        const uint32_t id = sm_choose(list, s.u, whole);
-        if (t == 0) a.token[r] = id;
+        f = sm_search(list, s, all, b, up, s.few);
+    }
+    auto in = [&](uint32_t j) { return list.order[j] >= f.border && !(list.bin[j] & SM_LOW); };
+    if (s.few) {
+        if (t == 0) a.token[r] = f.id;
         if (!a.probs || t >= 64) return;
-        auto in = [&](uint32_t j) { return list.order[j] >= border && !(list.bin[j] & SM_LOW); };
         uint32_t n = 0;
         for (uint32_t j0 = 0; j0 < list.n; j0 += 64) {
             const uint32_t j = j0 + t;
@@ -816,119 +936,33 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a,
             const uint32_t at = n + lanes_below(m);
             if (k && at < SM_FEW) {
                 w.out[1 + 2 * at] = ~(uint32_t)list.order[j];
-                w.out[2 + 2 * at] = __float_as_uint((float)(sm_weight(sm_value((uint32_t)(list.order[j] >> 32)), all.top, s.inv) * up / (double)whole));
+                w.out[2 + 2 * at] = __float_as_uint((float)(sm_weight(sm_value((uint32_t)(list.order[j] >> 32)), all.top, s.inv) * up / (double)f.whole));
             }
             n += (uint32_t)__popcll(m);
         }
         if (t == 0) w.out[0] = min(n, SM_FEW);
         return;
     }
-    const double up = sm_unit(all.sum);
-    const bool k_on = s.top_k && s.top_k < all.ok, p_on = s.top_p < 1.0f;
-    if (!k_on && !p_on) {
-        uint64_t whole;
-        const uint64_t mine = t < p.parts ? w.kept[t] : 0, before = sm_scan(mine, &whole, tmp), want = (uint64_t)((double)s.u * (double)whole);
-        if (t == part) { found.ksum = before; found.psum = mine; }
+    if (listed_kind) {      // the parts' units that stay: above the listed bins, and the list's
+        uint64_t *const units = &aheads[0][0];
+        static_assert(4 * SM_RANKED >= SM_PARTS, "room for the parts");
+        if (t < p.parts) units[t] = __hip_atomic_load(w.kept + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         __syncthreads();
-        const bool here = want >= found.ksum && want < found.ksum + found.psum;
-        sm_pick(a, p, r, part, al, s, all.top, up, (double)whole, here, want - found.ksum, tmp, &least, [](float, uint32_t) { return true; });
-        return;
-    }
-    // the bins in which top_k and top_p end
-    constexpr uint32_t PER = SM_BINS / SM_THREADS;
-    const float scale = sm_bin_scale(s, all);
-    uint32_t cnt[PER], c = 0, nall;
-    uint64_t sum[PER], u = 0, whole;
-#pragma unroll
-    for (uint32_t i = 0; i < PER; i++) {
-        cnt[i] = w.bincnt[t * PER + i];
-        sum[i] = w.binsum[t * PER + i];
-        c += cnt[i];
-        u += sum[i];
-    }
-    c = sm_scan(c, &nall, tmp32);
-    u = sm_scan(u, &whole, tmp);
-    if (t == 0) found = (sm_border){SM_BINS, 0, SM_BINS, SM_BINS, 0, 0, 0, whole};
-    __syncthreads();
-    uint64_t klo = whole, khi = whole;
-    if (k_on) {
-        uint32_t cc = c;
-        uint64_t uu = u;
-#pragma unroll
-        for (uint32_t i = 0; i < PER; i++) {
-            if (cc < s.top_k && cc + cnt[i] >= s.top_k) { found.kbin = t * PER + i; found.kabove = cc; found.ksum = uu; found.psum = uu + sum[i]; }
-            cc += cnt[i];
-            uu += sum[i];
-        }
+#pragma unroll 1
+        for (uint32_t j = t; j < list.n; j += SM_THREADS)
+            if (in(j)) atomicAdd((unsigned long long *)units + ~(uint32_t)list.order[j] / (SM_IDS * p.rounds), (unsigned long long)list.unit[j]);
         __syncthreads();
-        klo = found.ksum;
-        khi = found.psum;
+        const uint64_t mine = t < p.parts ? units[t] : 0, before = sm_scan(mine, &total, tmp);
+        want = (uint64_t)((double)s.u * (double)total);
+        if (want >= before && want < before + mine) { found.kabove = t; found.ksum = before; }
         __syncthreads();
+        mine_part = found.kabove;
+        want -= found.ksum;
     }
-    if (p_on) {
-        const double dlo = ceil((double)s.top_p * (double)klo), dhi = ceil((double)s.top_p * (double)khi);
-        const uint64_t wlo = dlo > 1.0 ? (uint64_t)dlo : 1, whi = dhi > 1.0 ? (uint64_t)dhi : 1;
-        uint64_t uu = u;
-#pragma unroll
-        for (uint32_t i = 0; i < PER; i++) {
-            if (uu < wlo && uu + sum[i] >= wlo) { found.plo = t * PER + i; found.psum = uu; }
-            if (uu < whi && uu + sum[i] >= whi) found.phi = t * PER + i;
-            uu += sum[i];
-        }
-        __syncthreads();
-    }
-    sm_border b = found;
-    if (p_on && b.kbin < SM_BINS) b.phi = min(b.phi, b.kbin);
-    b.first = p_on ? b.plo : b.kbin;
-    if (part == 0 && t == 0) *w.border = b;
-    uint64_t q = 0;
-    for (uint32_t m = 0; m < p.rounds; m++) {
-        float x[4];
-        const uint32_t i = sm_load(a, p, r, part, m, al, x);
-        uint32_t in = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (!(x[e] > -INFINITY)) continue;
-            const uint32_t y = sm_bin(x[e], all.top, scale);
-            if (y < b.first) {
-                const double z = sm_weight(x[e], all.top, s.inv);
-                if (z >= (double)s.min_p || x[e] == all.top) q += sm_units(z, up);
-            } else if (y == b.kbin || (p_on && y <= b.phi)) {
-                in |= 1u << e;
-            }
-        }
-        sm_append(w, x, i, in);
-    }
-    q = sm_sum(q, tmp);
-    if (t == 0) __hip_atomic_store(w.kept + part, q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (!LAST) return;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // what this wave wrote has arrived
-    __syncthreads();
-    if (t == 0) least = __hip_atomic_fetch_add(w.arrived, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (least != p.parts - 1) return;
-    __syncthreads();
-    if (!sm_resolve(list, w, s, all, b, up, scale)) {
-        sm_slow(a, r, s, &list);
-        return;
-    }
-    // the parts' units that stay: above the listed bins, and the list's
-    uint64_t *const units = &aheads[0][0];
-    static_assert(4 * SM_RANKED >= SM_PARTS, "room for the parts");
-    if (t < p.parts) units[t] = __hip_atomic_load(w.kept + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    for (uint32_t j = t; j < list.n; j += SM_THREADS)
-        if (list.order[j] >= list.border && !(list.bin[j] & SM_LOW))
-            atomicAdd((unsigned long long *)units + ~(uint32_t)list.order[j] / (SM_IDS * p.rounds), (unsigned long long)list.unit[j]);
-    __syncthreads();
-    uint64_t total;
-    const uint64_t mine = t < p.parts ? units[t] : 0, before = sm_scan(mine, &total, tmp), want = (uint64_t)((double)s.u * (double)total);
-    if (want >= before && want < before + mine) { found.kabove = t; found.ksum = before; }
-    __syncthreads();
-    const uint64_t border = list.border;
-    sm_pick(a, p, r, found.kabove, al, s, all.top, up, (double)total, true, want - found.ksum, tmp, &least, [&](float x, uint32_t i) {
+    sm_pick(a, p, r, mine_part, al, s, all.top, up, (double)total, here, want, tmp, &least, [&](float x, uint32_t i) {
+        if (!listed_kind) return true;
         const uint32_t y = sm_bin(x, all.top, scale);
-        return y < b.first || ((y == b.kbin || (p_on && y <= b.phi)) && ((uint64_t)sm_key(x) << 32 | (uint32_t)~i) >= border);
+        return y < b.first || ((y == b.kbin || (p_on && y <= b.phi)) && ((uint64_t)sm_key(x) << 32 | (uint32_t)~i) >= f.border);
     });
 }
 
@@ -965,7 +999,8 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_last(sgk_sample_args a, s
     const double up = sm_unit(all.sum);
     const sm_border b = *w.border;
     const float scale = sm_bin_scale(s, all);
-    sm_resolve(list, w, s, all, b, up, scale);
+    sm_fetch(list, w, s, all, up, scale);
+    const sm_result f = sm_search(list, s, all, b, up, false);
     // the units that stay: above the listed bins by parts, and the list's
     const uint32_t i0 = part * p.rounds * SM_IDS, i1 = i0 + p.rounds * SM_IDS;
     uint64_t whole = 0, before = 0, mine = 0;
@@ -976,7 +1011,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_last(sgk_sample_args a, s
         if (t == part) mine = q;
     }
     for (uint32_t j = t; j < list.n; j += SM_THREADS)
-        if (list.order[j] >= list.border && !(list.bin[j] & SM_LOW)) {
+        if (list.order[j] >= f.border && !(list.bin[j] & SM_LOW)) {
             const uint32_t id = ~(uint32_t)list.order[j];
             whole += list.unit[j];
             if (id < i0) before += list.unit[j];
@@ -990,7 +1025,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_last(sgk_sample_args a, s
     whole = before = mine = 0;
 #pragma unroll
     for (int i = 0; i < SM_WAVES; i++) { whole += sums[0][i]; before += sums[1][i]; mine += sums[2][i]; }
-    const uint64_t want = (uint64_t)((double)s.u * (double)whole), border = list.border;
+    const uint64_t want = (uint64_t)((double)s.u * (double)whole), border = f.border;
     sm_pick(a, p, r, part, al, s, all.top, up, (double)whole, want >= before && want < before + mine, want - before, tmp, &least,
             [&](float x, uint32_t i) {
                 const uint32_t y = sm_bin(x, all.top, scale);
