@@ -87,3 +87,23 @@ def test_infinite_temperature_and_logits(gpu):
     sets = [(np.inf, 0, 1.0, 0.0), (np.inf, 3, 1.0, 0.0), (np.inf, 0, 0.333, 0.0), (1.0, 0, 0.5, 0.0), (1.0, 0, 1.0, 0.5), (np.inf, 2000, 0.9999, 0.1)]
     check(gpu, np.repeat(x[None], len(sets), 0), sets, np.full(len(sets), 0.377))
     check(gpu, np.repeat(y[None], len(sets), 0), sets, np.full(len(sets), 0.377))
+
+
+@pytest.mark.parametrize("n", [1, 2, 7, 8, 9, 31, 33, 127, 128, 129, 131, 254, 255, 256, 257, 300])
+@pytest.mark.parametrize("width", [1e-3, 0.05, 0.3])
+@pytest.mark.parametrize("alike", [False, True])
+def test_lists_of_every_short_length(gpu, n, width, alike):
+    """Both borders anywhere in a crowd over one bin or several, a quarter of its ids alike or none: the lists that are compared
+    all with all, and the first ones past them."""
+    rng = np.random.default_rng(n)
+    x = crowd(rng, 3000, n, width)
+    if alike:
+        at = np.flatnonzero(x > 3.9)[::4]
+        x[at] = np.float32(4 + width / 2)
+    w = np.sort(np.exp(x.astype(np.float64) - x.max()))[::-1].cumsum()
+    sets = []
+    for a in (0.1, 0.5, 0.93):
+        k, p = 6 + max(1, int(a * n)), (w[5] + (a + 0.013) * (w[5 + n] - w[5])) / w[-1]
+        sets += [(1.0, k, 1.0, 0.0), (1.0, 0, p, 0.0), (1.0, k, p, 0.0), (1.0, 6 + n, p, 0.0), (1.0, max(k, 140), 0.9 * p, 0.0), (1.0, k, 0.9999, 0.04)]
+    check(gpu, np.repeat(x[None], len(sets), 0), sets, rng.random(len(sets)))
+    check(gpu, np.repeat(x[None], len(sets), 0), sets, rng.random(len(sets)), probs=False)
