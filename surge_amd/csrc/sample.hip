@@ -24,15 +24,15 @@
 //   border a histogram of the logits' distance from the largest, counts and sums
 //          (2), gives the bins in which top_k and top_p end; their ids are listed,
 //          the sums of the ids above them taken (3), and the list searched for the
-//          exact borders (3 or 4).
+//          exact borders (3 or 4): all with all, or past SM_NEAR entries by digits.
 // A list that does not fit (thousands of ids alike at a border) leaves the row to
 // one workgroup, which goes over it digit by digit.
 //
 // The logits are read once from memory and then from the last cache; what bounds
 // a call is the chain of launches, each a few trips to memory long. One row of
 // 151936 ids, top_k 20 and top_p 0.8: 3.0 + 6.4 + 5.8 us, the call 25.6, of which
-// 8.8 are any call's. 16 rows of all kinds 6.0 + 11.4 + 20.0 (46.4); 4 rows with
-// top_p and probabilities 4.4 + 9.0 + 8.1 + 13.4 (43). Ranking a few row's list in
+// 8.8 are any call's. 16 rows of all kinds 6.1 + 11.8 + 17.3 (45 to 48); 4 rows with
+// top_p and probabilities 4.4 + 8.8 + 7.9 + 12.7 (42). Ranking a few row's list in
 // the second launch's last workgroup: 12.4 + 2.0 us against 6.4 + 5.9, so it is
 // left to the third.
 // ---------------------------------------------------------------------------
@@ -44,7 +44,7 @@
 #define SM_WGS 1024u        // workgroups that a launch has about (16 rows of 151936, the launches together: 512 40.2 us, 1024 38.6, 2048 41.8)
 #define SM_LIST 2048u
 #define SM_RANKED 128u      // entries that are compared all with all
-#define SM_NEAR 256u        // entries of a list that is searched by comparing all with all
+#define SM_NEAR 256u        // entries of a list that is searched by comparing all with all (about 100 of them: 2 us, by digits 5)
 #define SM_BINS 2048u
 #define SM_NONE 0xFFFFFFFFu
 
