@@ -482,7 +482,8 @@ sg_err sg_gpu_run_page_evict(sg_gpu *g, void *kp, void *vp, void *table, void *l
  *   top_k: the top_k ids of the largest x stay (0, or more than there are: all);
  *   top_p < 1: of those, in falling order of x, an id stays if the w before it add up
  *     to less than top_p times the w of all that top_k left; the first always does;
- *   min_p > 0: of those, the ids with w >= min_p stay, and the largest;
+ *   min_p > 0: of those, the ids with w >= min_p stay, and the largest (above 1 it
+ *     alone, the lowest id of those alike);
  *   ids of the same x: the lower id comes first.
  * token u32 [rows]: the lowest id for which the w of the ids that stayed, up to and
  * with it, add up to more than u times all of theirs; 0xFFFFFFFF if the row has none.

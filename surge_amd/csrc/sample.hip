@@ -154,6 +154,7 @@ __device__ __forceinline__ sm_set sm_settings(const sgk_sample_args &a, const sm
     if (!(s.temp > 0.0f)) { s.temp = 1.0f; s.top_k = 1; }
     if (!(s.top_p < 1.0f)) s.top_p = 1.0f;
     if (!(s.min_p > 0.0f)) s.min_p = 0.0f;
+    if (s.min_p > 1.0f) s.top_k = 1;        // no weight is: the largest alone stays, of alike ones the lowest id
     s.inv = 1.0 / (double)s.temp;
     s.few = s.top_k && s.top_k <= SM_FEW && s.top_k <= p.parts * SM_WAVES;
     return s;
