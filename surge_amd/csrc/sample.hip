@@ -15,10 +15,10 @@
 // probabilities are wanted (without them the row's last workgroup of the third
 // goes on). A row's settings are known on the device alone, so each launch does
 // for a row what its kind needs:
-//   few    top_k of SM_FEW at most (greedy: 1). The top_k-th largest of the waves'
-//          maxima (1) is a bound that at least top_k ids reach, and hardly more:
-//          those are listed (2), ranked by comparing all with all, and the token
-//          is found among them (3).
+//   few    top_k of SM_FEW at most (greedy: 1), in a row of SM_MAXIMA waves at most.
+//          The top_k-th largest of the waves' maxima (1) is a bound that at least
+//          top_k ids reach, and hardly more: those are listed (2), ranked by
+//          comparing all with all, and the token is found among them (3).
 //   all    no top_k, no top_p: the parts' sums (2), then the part in which the
 //          token lies finds it (3).
 //   border a histogram of the logits' distance from the largest, counts and sums
@@ -41,6 +41,7 @@
 #define SM_IDS (4 * SM_THREADS)
 #define SM_PARTS 512u       // of a row, at most: its parts take several rounds of SM_IDS past that
 #define SM_FEW 128u         // one row, the third launch: top_k 20 5.7 us, 15.6 as the third kind; 127 10.5, 15.6
+#define SM_MAXIMA 1024u     // waves of a row of few, 16 a lane (a call with top_k 20: 262144 ids 25.2 us, 262145 as the third kind 35.5, with loops over the maxima 69; a million 47.7, 197)
 #define SM_WGS 1024u        // workgroups that a launch has about (16 rows of 151936, the launches together: 512 40.2 us, 1024 38.6, 2048 41.8)
 #define SM_LIST 2048u
 #define SM_RANKED 128u      // entries that are compared all with all
@@ -156,7 +157,7 @@ __device__ __forceinline__ sm_set sm_settings(const sgk_sample_args &a, const sm
     if (!(s.min_p > 0.0f)) s.min_p = 0.0f;
     if (s.min_p > 1.0f) s.top_k = 1;        // no weight is: the largest alone stays, of alike ones the lowest id
     s.inv = 1.0 / (double)s.temp;
-    s.few = s.top_k && s.top_k <= SM_FEW && s.top_k <= p.parts * SM_WAVES;
+    s.few = s.top_k && s.top_k <= SM_FEW && s.top_k <= p.parts * SM_WAVES && p.parts * SM_WAVES <= SM_MAXIMA;
     return s;
 }
 // Four ids of round m of a part: their first, and their logits (NaN behind the last).
@@ -275,41 +276,32 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
         // a bound that at least top_k ids reach: the top_k-th of the waves' maxima, its upper bits (every wave by itself)
         const uint32_t n = p.parts * SM_WAVES;
         uint32_t bound = 0, best = 0, least = 0xFFFFFFFFu;
-        if (n <= 64 * 16) {
-            uint32_t c[16];
+        constexpr uint32_t C = SM_MAXIMA / 64;
+        uint32_t c[C];
 #pragma unroll
-            for (uint32_t j = 0; j < 16; j++) c[j] = j * 64 + l < n ? w.wave[j * 64 + l] : 0;
+        for (uint32_t j = 0; j < C; j++) c[j] = j * 64 + l < n ? w.wave[j * 64 + l] : 0;
 #pragma unroll
-            for (uint32_t j = 0; j < 16; j++) {
-                best = max(best, c[j]);
-                if (c[j]) least = min(least, c[j]);
-            }
-            best = wave_umax(best);
-            least = ~wave_umax(~least);
-            const uint32_t differ = best ^ least, high = differ ? 31 - __builtin_clz(differ) : 0;
-            uint32_t have = 0;
+        for (uint32_t j = 0; j < C; j++) {
+            best = max(best, c[j]);
+            if (c[j]) least = min(least, c[j]);
+        }
+        best = wave_umax(best);
+        least = ~wave_umax(~least);
+        const uint32_t differ = best ^ least, high = differ ? 31 - __builtin_clz(differ) : 0;
+        uint32_t have = 0;
 #pragma unroll
-            for (uint32_t j = 0; j < 16; j++) have += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(c[j] != 0));
-            // 11 bits of it at least, and more until few more waves reach it than have to
-            if (have >= s.top_k) {
-                bound = least & ~((2u << high) - 1);
-                for (int b = (int)high; b >= 0 && (b > (int)high - 11 || have > s.top_k + s.top_k / 8); b--) {
-                    uint32_t k = 0;
-#pragma unroll
-                    for (uint32_t j = 0; j < 16; j++) {
-                        if (j % 4 == 0 && j * 64 >= n) break;
-                        k += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(c[j] >= (bound | 1u << b)));
-                    }
-                    if (k >= s.top_k) { bound |= 1u << b; have = k; }
-                }
-            }
-        } else {
-            for (uint32_t j = l; j < n; j += 64) best = max(best, w.wave[j]);
-            best = wave_umax(best);
-            for (int b = 31; b >= 12; b--) {
+        for (uint32_t j = 0; j < C; j++) have += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(c[j] != 0));
+        // 11 bits of it at least, and more until few more waves reach it than have to
+        if (have >= s.top_k) {
+            bound = least & ~((2u << high) - 1);
+            for (int b = (int)high; b >= 0 && (b > (int)high - 11 || have > s.top_k + s.top_k / 8); b--) {
                 uint32_t k = 0;
-                for (uint32_t j = l; j < (n + 63) / 64 * 64; j += 64) k += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(j < n && w.wave[j] >= (bound | 1u << b)));
-                if (k >= s.top_k) bound |= 1u << b;
+#pragma unroll
+                for (uint32_t j = 0; j < C; j++) {
+                    if (j % 4 == 0 && j * 64 >= n) break;
+                    k += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(c[j] >= (bound | 1u << b)));
+                }
+                if (k >= s.top_k) { bound |= 1u << b; have = k; }
             }
         }
         if (part == 0 && t == 0) *w.all = (sm_all){best, 0, best != 0, sm_value(best), 1.0f};
