@@ -18,15 +18,18 @@
 //   few    top_k of SM_FEW at most (greedy: 1), in a row of SM_MAXIMA waves at most.
 //          The top_k-th largest of the waves' maxima (1) is a bound that at least
 //          top_k ids reach, and hardly more: those are listed (2), ranked by
-//          comparing all with all, and the token is found among them (3).
+//          comparing all with all, and the token is found among them (3). Where
+//          fewer waves than top_k have any id (a mask, a short vocabulary), all ids
+//          are listed, or past SM_LIST those that one workgroup (3) finds by a histogram.
 //   all    no top_k, no top_p: the parts' sums (2), then the part in which the
 //          token lies finds it (3).
 //   border a histogram of the logits' distance from the largest, counts and sums
 //          (2), gives the bins in which top_k and top_p end; their ids are listed,
 //          the sums of the ids above them taken (3), and the list searched for the
 //          exact borders (3 or 4): all with all, or past SM_NEAR entries by digits.
-// A list that does not fit (thousands of ids alike at a border) leaves the row to
-// one workgroup, which goes over it digit by digit.
+// A list that does not fit (thousands of ids alike at a border, or above a few row's
+// bound where the largest lie together in a few waves) leaves the row to one
+// workgroup, which goes over it digit by digit.
 //
 // The logits are read once from memory and then from the last cache; what bounds
 // a call is the chain of launches, each a few trips to memory long. One row of
@@ -160,9 +163,8 @@ __device__ __forceinline__ sm_set sm_settings(const sgk_sample_args &a, const sm
     s.few = s.top_k && s.top_k <= SM_FEW && s.top_k <= p.parts * SM_WAVES && p.parts * SM_WAVES <= SM_MAXIMA;
     return s;
 }
-// Four ids of round m of a part: their first, and their logits (NaN behind the last).
-__device__ __forceinline__ uint32_t sm_load(const sgk_sample_args &a, const sm_plan &p, uint32_t r, uint32_t part, uint32_t m, int al, float (&x)[4]) {
-    const uint64_t i = ((uint64_t)part * p.rounds + m) * SM_IDS + 4 * threadIdx.x;
+// The logits of ids i to i + 3 (NaN behind the last).
+__device__ __forceinline__ void sm_four(const sgk_sample_args &a, uint32_t r, uint64_t i, int al, float (&x)[4]) {
     const float *q = a.x + (uint64_t)r * a.vocab + i;
     if (al && i < a.vocab) {
         const f32x4 v = *(const f32x4 *)q;
@@ -172,6 +174,11 @@ __device__ __forceinline__ uint32_t sm_load(const sgk_sample_args &a, const sm_p
 #pragma unroll
         for (int e = 0; e < 4; e++) x[e] = i + e < a.vocab ? q[e] : NAN;
     }
+}
+// Four ids of round m of a part: their first, and their logits.
+__device__ __forceinline__ uint32_t sm_load(const sgk_sample_args &a, const sm_plan &p, uint32_t r, uint32_t part, uint32_t m, int al, float (&x)[4]) {
+    const uint64_t i = ((uint64_t)part * p.rounds + m) * SM_IDS + 4 * threadIdx.x;
+    sm_four(a, r, i, al, x);
     return (uint32_t)i;
 }
 __device__ __forceinline__ sm_all sm_read(const sm_row &w, const sm_plan &p, const sm_set &s, uint64_t *tmp) {
@@ -272,10 +279,12 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
     const sm_set s = sm_settings(a, p, r);
     float x[4];
     uint32_t i = sm_load(a, p, r, part, 0, al, x);
+    uint32_t bound = 0, best = 0;
+    bool unbound = false;
     if (s.few) {
         // a bound that at least top_k ids reach: the top_k-th of the waves' maxima, its upper bits (every wave by itself)
         const uint32_t n = p.parts * SM_WAVES;
-        uint32_t bound = 0, best = 0, least = 0xFFFFFFFFu;
+        uint32_t least = 0xFFFFFFFFu;
         constexpr uint32_t C = SM_MAXIMA / 64;
         uint32_t c[C];
 #pragma unroll
@@ -288,9 +297,10 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
         best = wave_umax(best);
         least = ~wave_umax(~least);
         const uint32_t differ = best ^ least, high = differ ? 31 - __builtin_clz(differ) : 0;
-        uint32_t have = 0;
+        uint32_t waves = 0;     // that have any id
 #pragma unroll
-        for (uint32_t j = 0; j < C; j++) have += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(c[j] != 0));
+        for (uint32_t j = 0; j < C; j++) waves += (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(c[j] != 0));
+        uint32_t have = waves;
         // 11 bits of it at least, and more until few more waves reach it than have to
         if (have >= s.top_k) {
             bound = least & ~((2u << high) - 1);
@@ -304,6 +314,13 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
                 if (k >= s.top_k) { bound |= 1u << b; have = k; }
             }
         }
+        // too few waves for a bound, or just as many of which the last has few ids and so may have set a low one; and room for
+        // more ids in them than can be listed
+        unbound = waves < s.top_k + (p.rounds == 1 && a.vocab % 256 - 1 < 63) && waves * p.rounds > SM_LIST / 256;
+    }
+    sm_all all = {};
+    if (!s.few || unbound) all = sm_read(w, p, s, tmp);
+    if (s.few && (!unbound || all.ok <= SM_LIST)) {
         if (part == 0 && t == 0) *w.all = (sm_all){best, 0, best != 0, sm_value(best), 1.0f};
         bound = max(bound, 1u);
         for (uint32_t m = 0; m < p.rounds; m++) {
@@ -315,9 +332,8 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
         }
         return;
     }
-    const sm_all all = sm_read(w, p, s, tmp);
     if (part == 0 && t == 0) *w.all = all;
-    if (!all.ok) return;
+    if (s.few || !all.ok) return;
     const double up = sm_unit(all.sum);
     if ((!s.top_k || s.top_k >= all.ok) && s.top_p == 1.0f) {
         uint64_t q = 0;
@@ -722,6 +738,68 @@ __device__ __forceinline__ void sm_slow(const sgk_sample_args &a, uint32_t r, co
     __syncthreads();
     if (t == 0) a.token[r] = token;
 }
+// A few row whose waves give no bound and whose ids (all.ok) are too many: the ids of the waves that have any, down to the bin in
+// which top_k ends, are listed. By one workgroup; `room` is used.
+__device__ __forceinline__ void sm_narrow(const sgk_sample_args &a, const sm_plan &p, uint32_t r, const sm_row &w, int al, const sm_set &s, const sm_all &all,
+                                          sm_list *room) {
+    constexpr uint32_t PER = SM_BINS / SM_THREADS, A = 4;       // A of a wave's blocks of 256 ids under way
+    static_assert(SM_BINS + SM_FEW + 1 <= 2 * SM_LIST, "room for the counts and the waves");
+    uint32_t *const cnts = (uint32_t *)room->order, *const some = cnts + SM_BINS, *const last = some + SM_FEW;
+    const uint32_t t = threadIdx.x, l = t & 63, waves = p.parts * SM_WAVES;
+    const float scale = sm_bin_scale(s, all);
+    for (uint32_t j = t; j < SM_BINS; j += SM_THREADS) cnts[j] = 0;
+    uint32_t n = 0;         // waves that have any: top_k at most
+    for (uint32_t j = l; j - l < waves; j += 64) {
+        const bool has = j < waves && w.wave[j];
+        const uint64_t any = __builtin_amdgcn_ballot_w64(has);
+        if (has && t < 64 && n + lanes_below(any) < SM_FEW) some[n + lanes_below(any)] = j;
+        n += (uint32_t)__popcll(any);
+    }
+    __syncthreads();
+    const uint32_t blocks = min(n, SM_FEW) * p.rounds;
+    auto each = [&](auto f) {
+        for (uint32_t q0 = __builtin_amdgcn_readfirstlane(t >> 6); q0 < blocks; q0 += A * SM_WAVES) {
+            float x[A][4];
+            uint64_t i[A];
+#pragma unroll
+            for (uint32_t b = 0; b < A; b++) {
+                const uint32_t q = q0 + b * SM_WAVES, v = q < blocks ? some[q / p.rounds] : 0;
+                i[b] = q < blocks ? ((uint64_t)(v / SM_WAVES) * p.rounds + q % p.rounds) * SM_IDS + 4 * (v % SM_WAVES * 64 + l) : a.vocab;
+                sm_four(a, r, i[b], al, x[b]);
+            }
+#pragma unroll
+            for (uint32_t b = 0; b < A; b++) f(x[b], (uint32_t)i[b]);
+        }
+    };
+    each([&](const float (&x)[4], uint32_t) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (x[e] > -INFINITY) atomicAdd(&cnts[sm_bin(x[e], all.top, scale)], 1u);
+    });
+    __syncthreads();
+    uint32_t cnt[PER], c = 0, unused;
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) {
+        cnt[i] = cnts[t * PER + i];
+        c += cnt[i];
+    }
+    c = sm_scan(c, &unused, room->tmp);
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) {
+        if (c < s.top_k && c + cnt[i] >= s.top_k) *last = t * PER + i;
+        c += cnt[i];
+    }
+    __syncthreads();
+    const uint32_t bin = *last;
+    each([&](const float (&x)[4], uint32_t i) {
+        uint32_t in = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) in |= (uint32_t)(x[e] > -INFINITY && sm_bin(x[e], all.top, scale) <= bin) << e;
+        sm_append(w, x, i, in);
+    });
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");        // what this wave wrote has arrived
+    __syncthreads();
+}
 // ---- 3. LAST: the row's last workgroup goes on to the token, and no fourth launch follows; what it takes from the others
 // has been written through to memory.
 template <bool LAST>
@@ -750,12 +828,14 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a,
     uint32_t mine_part = part;
     uint64_t want = 0, total = 0;
     if (s.few) {
-        const uint32_t listed = *w.listed;
+        // (32000 ids, top_k 126 of 125 waves: a call 44 us, 318 with all ids listed; 4096 in a row of a mask, top_k 18 of 17: 29, 950)
+        if (__builtin_expect(all.ok > 1, 0)) sm_narrow(a, p, r, w, al, s, all, &list);
+        const uint32_t listed = __hip_atomic_load(w.listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (listed <= SM_RANKED) {
             // each entry against all: four groups of waves take a quarter of the others each, for 64 or 128 entries
             const uint32_t l = t & 63, half = t >> 6 & 1, j = 64 * half + l, from = (t >> 7) * (SM_RANKED / 4);
             if (t < SM_RANKED) {
-                const uint64_t o = t < listed ? w.list[t] : 0;
+                const uint64_t o = t < listed ? __hip_atomic_load(w.list + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
                 const double y = t < listed ? sm_weight(sm_value((uint32_t)(o >> 32)), all.top, s.inv) : 0.0;
                 list.order[t] = o;
                 list.unit[t] = sm_units(y, up);
