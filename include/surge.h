@@ -450,8 +450,9 @@ sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void
  *   none. n_heads a multiple of n_kv, at most 16 times it. Where weight_out is given,
  *   weight_out[s][h][j] = weight[s][h][j] + the softmax weights that the query heads of
  *   kv head h gave slot j, for j < lens[s] (weight NULL: + 0); the slots behind stay.
- *   weight_out may be weight (as with the rotary axes' x and out). q, K and products
- *   keep f32's precision. Elements that are not finite: of q or of a row of K, they make
+ *   weight_out may be weight (as with the rotary axes' x and out). An element of q
+ *   counts to 2^-39 of its head's largest (all its bits do down to 2^-15 of that); K
+ *   and products with it are exact, sums f32. Elements that are not finite: of q or of a row of K, they make
  *   the head's outputs and weights NaN, or give the row no weight where its score is
  *   -inf; of V, they make their dim's outputs not finite. Reruns give the same bits.
  *   p: [0]=n_heads [1]=n_kv [2]=hd [3]=page [4]=n_seq [5]=width [6]=q_stride

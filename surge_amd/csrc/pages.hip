@@ -87,9 +87,10 @@ extern "C" hipError_t sgk_page_store(const sgk_page_store_args *a, hipStream_t s
 // (dims 8 r ..+7 of 128; 4 at head_dim 64), and dim 8 r + j of them is row r of
 // the j-th product, one byte permutation per two values.
 //
-// q is split into three f16 that add up to its f32 (relative to its head's
-// largest element), p into two (2^-22), so that products are exact or nearly so
-// and sums are f32.
+// q is split into three f16, scaled so that its head's largest element is 2^14 to
+// 2^15: what is left of an element is below 2^-25 then (half of f16's smallest), 2^-39
+// of the largest, and nothing of elements from 2^-15 of it on. p is split into two
+// (2^-22). So products are exact or nearly so, and sums are f32.
 //
 // Parts: T steps in all and `most` parts a kv head wanted give parts of `per` =
 // ceil(T / most) steps, a multiple of the waves, the same on every workgroup; a
