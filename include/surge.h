@@ -429,8 +429,8 @@ sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void
  * pages as the smaller buffer holds whole. table int32 [n_seq][width]: slot j of
  * sequence s lies in page table[s][j / page] at row j % page. page = 16, 32, 64,
  * 128 or 256, hd = 64, 128 or 256, n_kv <= 65535, n_seq <= 32768, width * page <= 2^30. A
- * cache [seq][n_kv][hd] of sg_gpu_run_attn_decode_f16 is such a pool, its table 0, 1,
- * 2, ... A page number outside the pool is never followed: rows for its slots are
+ * cache [seq][n_kv][hd] of sg_gpu_run_attn_decode_f16 is such a pool (as far as whole
+ * pages go), its table 0, 1, 2, ... A page number outside the pool is never followed: rows for its slots are
  * dropped, attention passes them over. Entries of the table past a sequence's length
  * do not count. Beside the pools a caller may keep two arrays [n_seq][n_kv][width *
  * page], per slot: weight f32, what attention gave the row so far, and pos int32, the
@@ -452,9 +452,12 @@ sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void
  *   kv head h gave slot j, for j < lens[s] (weight NULL: + 0); the slots behind stay.
  *   weight_out may be weight (as with the rotary axes' x and out). An element of q
  *   counts to 2^-39 of its head's largest (all its bits do down to 2^-15 of that); K
- *   and products with it are exact, sums f32. Elements that are not finite: of q or of a row of K, they make
- *   the head's outputs and weights NaN, or give the row no weight where its score is
- *   -inf; of V, they make their dim's outputs not finite. Reruns give the same bits.
+ *   and products with it are exact, sums f32. With weight_out the handle holds n_seq
+ *   n_heads width page floats of workspace from then on, whatever the lengths are: a
+ *   table no wider than its sequences may grow saves that. Elements that are not
+ *   finite: of q or of a row of K, they make the head's outputs and weights NaN, or
+ *   give the row no weight where its score is -inf; of V, they make their dim's outputs
+ *   not finite. Reruns give the same bits.
  *   p: [0]=n_heads [1]=n_kv [2]=hd [3]=page [4]=n_seq [5]=width [6]=q_stride
  *   [7]=scale bits.
  * sg_gpu_run_page_evict: of each sequence with lens[s] > keep, each kv head keeps
