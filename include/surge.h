@@ -430,11 +430,12 @@ sg_err sg_gpu_run_logits(sg_gpu *g, void *logits, void *counts, void *bias, void
  * sequence s lies in page table[s][j / page] at row j % page. page = 16, 32, 64,
  * 128 or 256, hd = 64, 128 or 256, n_kv <= 65535, n_seq <= 32768, width * page <= 2^30. A
  * cache [seq][n_kv][hd] of sg_gpu_run_attn_decode_f16 is such a pool (as far as whole
- * pages go), its table 0, 1, 2, ... A page number outside the pool is never followed: rows for its slots are
- * dropped, attention passes them over. Entries of the table past a sequence's length
- * do not count. Beside the pools a caller may keep two arrays [n_seq][n_kv][width *
- * page], per slot: weight f32, what attention gave the row so far, and pos int32, the
- * position of the row's token. Sequences may share pages that none of them writes.
+ * pages go), its table 0, 1, 2, ... A page number outside the pool is never followed:
+ * rows for its slots are dropped, attention passes them over. Entries of the table past
+ * a sequence's length do not count. Beside the pools a caller may keep two arrays
+ * [n_seq][n_kv][width * page], per slot: weight f32, what attention gave the row so
+ * far, and pos int32, the position of the row's token. Sequences may share pages that
+ * none of them writes.
  *
  * sg_gpu_run_page_store: rows f32 [n_seq][n] from k and v (row stride p[6] floats, 0
  *   = n_kv hd; [n_kv][hd] in a row), n in [1, 2^27], rounded to f16 (nearest, ties

@@ -102,8 +102,9 @@ extern "C" hipError_t sgk_page_store(const sgk_page_store_args *a, hipStream_t s
 // matrix units. A wave has its next step's K and V under way all the time, 8 to 32 KB,
 // and 32 slots a step are what its registers hold at head_dim 256 (242 of 256). What
 // is read once goes past the caches' order of use (non-temporal: 262000 slots of 4 x
-// 256 178 us against 185). 174 us for those 1073 MB, 6.2 TB/s (a plain read of as much
-// 181), 77 for 64 sequences' 401 MB, 50.9 for 16 of 91 to 16411 slots, 231 MB. About 9
+// 256 178 us against 185, then with two workgroups a CU). 175 us for those 1073 MB, 6.1
+// TB/s (a plain read of as much 181), 78 for 64 sequences' 401 MB, 51 for 16 of 91 to
+// 16411 slots, 231 MB. Past 64 sequences the plan is a launch of its own (3.9 us). About 9
 // us of each are the chain that a short call consists of (4 sequences of 57 to 700
 // slots, 9.2): lengths, table, rows, two products, the waves' sums.
 // ---------------------------------------------------------------------------
@@ -491,8 +492,8 @@ static ap_part ap_plan(const sgk_attn_paged_args *a, char *at, uint64_t *bytes) 
     const uint64_t rows = (uint64_t)a->c.n_seq * a->n_heads, cap = (uint64_t)a->c.width << a->c.log;
     const uint64_t steps = (cap + AP_STEP - 1) / AP_STEP * a->c.n_seq;      // at most
     // Workgroups that are there together: two a CU, which even out sequences of unlike lengths, or one where a single sequence
-    // is cut evenly anyway and 64 KB a CU are still asked for at once (head_dim 128; 64 has two). More of them are slower:
-    // 262000 slots of 256 178 us with one, 182 with two, 196 with four; 200000 of one head of 128 40, 44, 48.5 (three);
+    // is cut evenly anyway and 64 KB a CU are still asked for at once (head_dim 128; 64 has two). More of them are slower, us
+    // a call: 262000 slots of 256 186 with one, 190 with two, 196 with four; 200000 of one head of 128 40, 44, 48.5 (three);
     // 8 sequences of 128 56.7 with two, 59.9 with three. A sequence's last part is short, so that n_seq - 1 more may come up.
     const uint64_t there = (uint64_t)(a->c.n_seq == 1 && a->c.hd >= 128 ? 1 : 2) * sgk_device_cus() / a->c.n_kv;
     uint64_t most = there >= 2 * a->c.n_seq ? there - (a->c.n_seq - 1) : there;
@@ -508,7 +509,7 @@ static ap_part ap_plan(const sgk_attn_paged_args *a, char *at, uint64_t *bytes) 
     w.acc = (float *)take(heads * a->c.hd);
     w.m = (float *)take(heads);
     w.l = (float *)take(heads);
-    if (a->weight_out) w.score = (float *)take(rows * cap);
+    if (a->weight_out) w.score = (float *)take(rows * cap);     // by the table: the lengths are on the device
     if (a->c.n_seq > 64) w.plan = (uint32_t *)take((uint64_t)a->c.n_seq + 2 + w.parts);
     *bytes = 4 * n;
     return w;
@@ -560,14 +561,22 @@ extern "C" hipError_t sgk_attn_paged(const sgk_attn_paged_args *a, void *scratch
 // the workgroup's lowest. Long rows, where they are few, have several workgroups
 // (below). Bound by the chain of passes of a CU over its keys, each some trips to
 // LDS long, then by the moves: 64 rows of 2049 slots to 2048 5.9 us, 8 of 32768 to
-// 4096 8.8 + 6.8 + 6.9 us in three launches (31.3 by one workgroup a row), and 15.2
-// for the moves (59 MB, behind two dependent trips). 256 threads
-// a row are slower even at 4000 slots (23 us, 14). Loops are not unrolled far: code
-// that runs once comes from memory (keys in registers, 64 a thread: 150 KB of it,
-// 45 us).
+// 4096 7.6 + 6.3 + 6.6 us in three launches (31.3 by one workgroup a row), and 16.2
+// for the moves (59 MB, behind two dependent trips).
+//
+// The form follows the table, whose slots the host knows, not the lengths: one row out
+// of a wider table pays for the launches that the table could need. 16 x 2049 to 2048,
+// us a call: 14.7 in 2080 slots, 18.3 in 2128, 19.9 in 4096 to 32768, 23.5 in 65536;
+// 2 x 4097 to 4096 14.7 in 4128, 26.4 in 32832. And more than EV_HELD slots that are
+// held tight stay with one workgroup a row, which reads the keys again on every pass:
+// 2 x 65537 to 65536 66 in as many slots, 32 in 131072.
+//
+// 256 threads a row are slower even at 4000 slots (23 us, 14). Loops are not unrolled
+// far: code that runs once comes from memory (keys in registers, 64 a thread: 150 KB of
+// it, 45 us).
 // ---------------------------------------------------------------------------
-#define EV_FEW 64u          // rows that the selecting workgroup moves itself (32 of 2080: 12.0 us; with a launch for them 12.2 + 4.1)
-#define EV_HELD 32896u      // keys in LDS: 128 a page past 32768, so that a prompt's new slots fit too
+#define EV_FEW 64u          // rows that the selecting workgroup moves itself (16 x 2080 slots to 2048: a call 19.1 us; with a launch for them 22.7)
+#define EV_HELD 32896u      // keys in LDS: 32768 and a page of up to 128 more (one of 256 is past it)
 #define EV_THREADS 1024
 #define EV_BINS 2048u
 #define EV_LIST 2048u       // keys of the first histogram's bin that are listed (as many as fit beside EV_HELD)

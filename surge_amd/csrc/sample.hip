@@ -20,22 +20,25 @@
 //          top_k ids reach, and hardly more: those are listed (2), ranked by
 //          comparing all with all, and the token is found among them (3). Where
 //          fewer waves than top_k have any id (a mask, a short vocabulary), all ids
-//          are listed, or past SM_LIST those that one workgroup (3) finds by a histogram.
+//          are listed, or past SM_LIST those that one workgroup finds by a histogram
+//          (3).
 //   all    no top_k, no top_p: the parts' sums (2), then the part in which the
 //          token lies finds it (3).
 //   border a histogram of the logits' distance from the largest, counts and sums
 //          (2), gives the bins in which top_k and top_p end; their ids are listed,
 //          the sums of the ids above them taken (3), and the list searched for the
 //          exact borders (3 or 4): all with all, or past SM_NEAR entries by digits.
-// A list that does not fit (thousands of ids alike at a border, or above a few row's
-// bound where the largest lie together in a few waves) leaves the row to one
-// workgroup, which goes over it digit by digit.
+// A list that does not fit leaves the row to one workgroup, which goes over it digit by
+// digit: thousands of ids in a bin at a border (alike ones, as 16-bit logits about 10 or
+// 20 are, or a border 40 temperatures down), or above a few row's bound where the
+// largest lie together in a few waves. One row of 151936 takes 1.0 to 1.5 ms then (bf16
+// logits of mean 20 and deviation 2, top_p 0.95: 1.4; the same in f32 39 us).
 //
 // The logits are read once from memory and then from the last cache; what bounds
 // a call is the chain of launches, each a few trips to memory long. One row of
-// 151936 ids, top_k 20 and top_p 0.8: 3.0 + 6.4 + 5.8 us, the call 25.6, of which
-// 8.8 are any call's. 16 rows of all kinds 6.1 + 11.8 + 17.3 (45 to 48); 4 rows with
-// top_p and probabilities 4.4 + 8.8 + 7.9 + 12.7 (42). Ranking a few row's list in
+// 151936 ids, top_k 20 and top_p 0.8: 3.0 + 6.8 + 5.9 us, the call 24.9, of which
+// 8.8 are any call's. 16 rows of all kinds 6.2 + 11.4 + 17.6 (42); 4 rows with
+// top_p and probabilities 4.4 + 8.5 + 7.4 + 13.1 (41). Ranking a few row's list in
 // the second launch's last workgroup: 12.4 + 2.0 us against 6.4 + 5.9, so it is
 // left to the third.
 // ---------------------------------------------------------------------------
@@ -43,9 +46,11 @@
 #define SM_WAVES (SM_THREADS / 64)
 #define SM_IDS (4 * SM_THREADS)
 #define SM_PARTS 512u       // of a row, at most: its parts take several rounds of SM_IDS past that
-#define SM_FEW 128u         // one row, the third launch: top_k 20 5.7 us, 15.6 as the third kind; 127 10.5, 15.6
-#define SM_MAXIMA 1024u     // waves of a row of few, 16 a lane (a call with top_k 20: 262144 ids 25.2 us, 262145 as the third kind 35.5, with loops over the maxima 69; a million 47.7, 197)
-#define SM_WGS 1024u        // workgroups that a launch has about (16 rows of 151936, the launches together: 512 40.2 us, 1024 38.6, 2048 41.8)
+#define SM_FEW 128u         // a call, one row of 151936: top_k 20 25.4 us, 33.0 as the third kind; 127 29.7, 33.1 (16 rows, 20: 31.6, 52.7)
+// Waves of a row of few, 16 a lane. A call with top_k 20: 262144 ids 25.2 us, 262145 as the third kind 35.5, as few by loops over the
+// maxima 69; a million 47.7, 197.
+#define SM_MAXIMA 1024u
+#define SM_WGS 1024u        // workgroups that a launch has about (16 rows of 151936, a call with settings of all kinds: 512 42.7 us, 1024 41.4, 2048 46.4)
 #define SM_LIST 2048u
 #define SM_RANKED 128u      // entries that are compared all with all
 #define SM_NEAR 256u        // entries of a list that is searched by comparing all with all (about 100 of them: 2 us, by digits 5)
@@ -53,6 +58,7 @@
 #define SM_NONE 0xFFFFFFFFu
 
 // What the first launch found of a row: the largest and the lowest key, the ids that may be chosen, the weights' sum roughly.
+// Of a few row that has been listed: ok is whether it has any id. One whose ok is more has yet to be.
 struct sm_all { uint32_t best, low, ok; float top, sum; };
 // Where top_k and top_p end: the bin of top_k's last id (SM_BINS: no top_k), ids and units before that bin; the bins in
 // which top_p may end (SM_BINS: no top_p) and the units before them; the first bin that is listed; all units.
@@ -279,12 +285,10 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
     const sm_set s = sm_settings(a, p, r);
     float x[4];
     uint32_t i = sm_load(a, p, r, part, 0, al, x);
-    uint32_t bound = 0, best = 0;
-    bool unbound = false;
     if (s.few) {
         // a bound that at least top_k ids reach: the top_k-th of the waves' maxima, its upper bits (every wave by itself)
         const uint32_t n = p.parts * SM_WAVES;
-        uint32_t least = 0xFFFFFFFFu;
+        uint32_t bound = 0, best = 0, least = 0xFFFFFFFFu;
         constexpr uint32_t C = SM_MAXIMA / 64;
         uint32_t c[C];
 #pragma unroll
@@ -316,11 +320,13 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
         }
         // too few waves for a bound, or just as many of which the last has few ids and so may have set a low one; and room for
         // more ids in them than can be listed
-        unbound = waves < s.top_k + (p.rounds == 1 && a.vocab % 256 - 1 < 63) && waves * p.rounds > SM_LIST / 256;
-    }
-    sm_all all = {};
-    if (!s.few || unbound) all = sm_read(w, p, s, tmp);
-    if (s.few && (!unbound || all.ok <= SM_LIST)) {
+        if (__builtin_expect(waves < s.top_k + (p.rounds == 1 && a.vocab % 256 - 1 < 63) && waves * p.rounds > SM_LIST / 256, 0)) {
+            const sm_all all = sm_read(w, p, s, tmp);
+            if (all.ok > SM_LIST) {
+                if (part == 0 && t == 0) *w.all = all;
+                return;
+            }
+        }
         if (part == 0 && t == 0) *w.all = (sm_all){best, 0, best != 0, sm_value(best), 1.0f};
         bound = max(bound, 1u);
         for (uint32_t m = 0; m < p.rounds; m++) {
@@ -332,8 +338,9 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_count(sgk_sample_args a, 
         }
         return;
     }
+    const sm_all all = sm_read(w, p, s, tmp);
     if (part == 0 && t == 0) *w.all = all;
-    if (s.few || !all.ok) return;
+    if (!all.ok) return;
     const double up = sm_unit(all.sum);
     if ((!s.top_k || s.top_k >= all.ok) && s.top_p == 1.0f) {
         uint64_t q = 0;
@@ -816,6 +823,7 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a,
     const sm_set s = sm_settings(a, p, r);
     if (s.few && part) return;
     const sm_all all = *w.all;
+    const uint32_t few_listed = s.few ? *w.listed : 0;      // with all, before anything waits for that
     if (!all.ok) {
         if (LAST && part == 0 && t == 0) a.token[r] = SM_NONE;
         return;
@@ -828,14 +836,17 @@ __global__ void __launch_bounds__(SM_THREADS) k_sample_border(sgk_sample_args a,
     uint32_t mine_part = part;
     uint64_t want = 0, total = 0;
     if (s.few) {
-        // (32000 ids, top_k 126 of 125 waves: a call 44 us, 318 with all ids listed; 4096 in a row of a mask, top_k 18 of 17: 29, 950)
-        if (__builtin_expect(all.ok > 1, 0)) sm_narrow(a, p, r, w, al, s, all, &list);
-        const uint32_t listed = __hip_atomic_load(w.listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // not listed yet (32000 ids, top_k 126 of 125 waves: a call 44 us, 318 with all ids listed; 4096 in a row of a mask, top_k 18 of 17: 29, 950)
+        uint32_t listed = few_listed;
+        if (__builtin_expect(all.ok > 1, 0)) {
+            sm_narrow(a, p, r, w, al, s, all, &list);
+            listed = __hip_atomic_load(w.listed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
         if (listed <= SM_RANKED) {
             // each entry against all: four groups of waves take a quarter of the others each, for 64 or 128 entries
             const uint32_t l = t & 63, half = t >> 6 & 1, j = 64 * half + l, from = (t >> 7) * (SM_RANKED / 4);
             if (t < SM_RANKED) {
-                const uint64_t o = t < listed ? __hip_atomic_load(w.list + t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+                const uint64_t o = t < listed ? w.list[t] : 0;
                 const double y = t < listed ? sm_weight(sm_value((uint32_t)(o >> 32)), all.top, s.inv) : 0.0;
                 list.order[t] = o;
                 list.unit[t] = sm_units(y, up);

@@ -4,6 +4,7 @@ import time
 import numpy as np
 import pytest
 
+import pages_oracle as P
 from test_gpu_kv8 import Bufs
 from test_gpu_operator_aliases import Alias
 from test_gpu_sample import check, rows_of, sample, settings
@@ -81,3 +82,23 @@ def test_rows_of_both_kinds_together(gpu):
         check(gpu, x, [s] * 6, rng.random(6))
         tok, _ = sample(gpu, x, [s] * 6, [0.4] * 6, probs=False)
         assert tok[2] == 0xFFFFFFFF
+
+
+@pytest.mark.parametrize("rows,vocab,left", [(140, 60000, 20000), (140, 60003, 3000), (1100, 9000, 4000)])
+def test_many_rows_over_few_waves(gpu, rows, vocab, left):
+    """Parts of several rounds, and more rows than go at once; a mask that leaves `left` ids in a row, another place in each row."""
+    rng = np.random.default_rng(vocab)
+    x = (2 * rng.standard_normal((rows, vocab))).astype(np.float32)
+    for r in range(rows):
+        first = int(rng.integers(0, vocab - left))
+        x[r, :first] = x[r, first + left:] = -np.inf
+    sets = [(0.9, (20, 37, 40, 64)[r % 4], (0.9, 1.0)[r % 3 == 0], 0.0) for r in range(rows)]
+    u = rng.random(rows).astype(np.float32)
+    tok, pr = sample(gpu, x, sets, u)
+    again, _ = sample(gpu, x, sets, u, probs=False)
+    assert np.array_equal(tok, again)
+    for r in np.unique(np.concatenate([np.arange(8), rng.integers(0, rows, 12), [min(1023, rows - 1), min(1024, rows - 1), rows - 1]])):
+        want, probs, margin = P.sample(x[r], *sets[r], u[r])
+        assert margin > 1e-11 and int(tok[r]) == want
+        assert (np.abs(pr[r] - probs) <= probs * (2.0 ** -24 + 1e-9) + 2.0 ** -149).all()
+        assert np.array_equal(pr[r] > 0, probs.astype(np.float32) > 0)
