@@ -561,7 +561,7 @@ extern "C" hipError_t sgk_attn_paged(const sgk_attn_paged_args *a, void *scratch
 // the workgroup's lowest. Long rows, where they are few, have several workgroups
 // (below). Bound by the chain of passes of a CU over its keys, each some trips to
 // LDS long, then by the moves: 64 rows of 2049 slots to 2048 5.9 us, 8 of 32768 to
-// 4096 7.6 + 6.3 + 6.6 us in three launches (31.3 by one workgroup a row), and 16.2
+// 4096 8 + 6.4 + 6.6 us in three launches (31.3 by one workgroup a row), and 15 to 16
 // for the moves (59 MB, behind two dependent trips).
 //
 // The form follows the table, whose slots the host knows, not the lengths: one row out

@@ -36,9 +36,9 @@
 //
 // The logits are read once from memory and then from the last cache; what bounds
 // a call is the chain of launches, each a few trips to memory long. One row of
-// 151936 ids, top_k 20 and top_p 0.8: 3.0 + 6.8 + 5.9 us, the call 24.9, of which
-// 8.8 are any call's. 16 rows of all kinds 6.2 + 11.4 + 17.6 (42); 4 rows with
-// top_p and probabilities 4.4 + 8.5 + 7.4 + 13.1 (41). Ranking a few row's list in
+// 151936 ids, top_k 20 and top_p 0.8: 3.0 + 6.7 + 5.8 us, the call 26, of which
+// 8.8 are any call's. 16 rows of all kinds 6.2 + 11.9 + 17.2 (42 to 49); 4 rows with
+// top_p and probabilities 4.4 + 8.4 + 6.9 + 13.1 (42). Ranking a few row's list in
 // the second launch's last workgroup: 12.4 + 2.0 us against 6.4 + 5.9, so it is
 // left to the third.
 // ---------------------------------------------------------------------------
